@@ -24,6 +24,9 @@ const sources = [_]Source{
     .{ .file = "keys.hip" },
     .{ .file = "lr_abi.hip" },
     .{ .file = "mmdit.hip" },
+    .{ .file = "attn_cache.hip" },
+    .{ .file = "cache_rows.hip" },
+    .{ .file = "cache_abi.hip" },
 };
 
 /// hipcc flags of every device source: gfx950 only, no packed-fp32 instruction selection (v_pk_*_f32 are left to

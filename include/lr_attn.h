@@ -134,6 +134,24 @@ int lr_attention_bf16_ws(const void* q, const void* k, const void* v, void* out,
                          int64_t out_row_stride, void* workspace, size_t workspace_bytes, lr_stream_t stream);
 
 /*
+ * Attention over a sliding window of frames and the first tokens: autoregressive video (a frame's tokens see the last
+ * `window` frames, their own among them, and the first `sinks` tokens) and, with frame = 1, windows of single tokens with
+ * sinks. Query i is at position p = p0 + i, in frame p / frame, and sees key j when
+ *   j < nkeys,  j / frame <= p / frame,  and  j / frame > p / frame - window  or  j < sinks
+ * (whole frames: tokens of one frame see each other both ways). A query that sees no key gets zeros; a key that a query does
+ * not see has no part in its result, whatever it holds (infinities and NaN included). Layouts, arithmetic and other
+ * requirements as lr_attention_bf16, with separate k and v row strides; window >= 1, sinks >= 0, frame >= 1, nkeys and
+ * p0 + W at most 2^30. out must not overlap q, k or v (rejected).
+ * Calls of few rows are split over the keys: workspace of lr_attention_window_ws_bytes bytes (0: none, it may be NULL),
+ * 256-byte aligned, not overlapping the tensors (rejected); calls that overlap in time on one workspace race.
+ */
+size_t lr_attention_window_ws_bytes(int W, int H, int HK, int nkeys, int window, int sinks, int frame);
+int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* out, int p0, int W, int H, int HK, int nkeys,
+                             int window, int sinks, int frame, float scale, int64_t q_row_stride, int64_t k_row_stride,
+                             int64_t v_row_stride, int64_t out_row_stride, void* workspace, size_t workspace_bytes,
+                             lr_stream_t stream);
+
+/*
  * Attention under a key-padding mask: keys j with kmask[j] == 0 are left out (torch's bool key-padding mask, SDPA's
  * additive 0 / -inf), the drop-in for Kandinsky-6's attention.Call with mask = .keys
  * (src/engines/kandinsky6/dit/attention.zig:21-27, dispatched by launch.zig:239-255). Non-causal; q, out rows

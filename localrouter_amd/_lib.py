@@ -61,6 +61,8 @@ SIGNATURES = {
                                     [_P, _P, _P, _I64, _I, _F, _P]),
     "lr_attention_ws_bytes": (_SZ, [_I, _I, _I, _I]),
     "lr_attention_bf16_ws": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I64, _I64, _I64, _P, _SZ, _P]),
+    "lr_attention_window_ws_bytes": (_SZ, [_I] * 7),
+    "lr_attention_window_bf16": (_I, [_P, _P, _P, _P] + [_I] * 8 + [_F] + [_I64] * 4 + [_P, _SZ, _P]),
     "lr_attention_kmask_workspace_bytes": (_SZ, [_I, _I]),
     "lr_attention_kmask_bf16": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I64, _I64, _I64, _P, _SZ, _P]),
     "lr_joint_attention_fused_ex": (_I, [_P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _I64, _I, _I, _F, _I, _I, _I, _I,

@@ -21,7 +21,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "liblr_attn.so"
 SOURCES = ["attn_fwd.hip", "attn_stream.hip", "attn_keysplit.hip", "kv_image.hip", "rms_rope.hip", "int8_attn.hip",
-           "keys.hip", "lr_abi.hip", "mmdit.hip", "rope_host.cpp"]
+           "keys.hip", "lr_abi.hip", "mmdit.hip", "attn_cache.hip", "cache_rows.hip", "cache_abi.hip", "rope_host.cpp"]
 # libraries the shared object links: hipBLASLt for the MMDiT block's projections and MLP
 LIBS = ["-L/opt/rocm/lib", "-lhipblaslt"]
 ARCH = "gfx950"

@@ -1,0 +1,269 @@
+// The C ABI of the paged cache (include/lr_cache.h) and of the windowed attention (lr_attention_window_bf16 of
+// include/lr_attn.h): argument validation, then launches on the caller's stream. Nothing here synchronises, allocates or keeps
+// state.
+#include <limits.h>
+
+#include <algorithm>
+
+#include "../../include/lr_cache.h"
+#include "abi_checks.h"
+#include "lr_cache_kernels.h"
+
+namespace {
+
+using namespace lr::abi;
+
+constexpr int MAX_POS = 1 << 30;
+
+inline int shift_of(int page_size) { return __builtin_ctz((unsigned)page_size); }
+inline bool page_size_ok(int ps) { return ps >= 1 && ps <= 65536 && (ps & (ps - 1)) == 0; }
+
+// A pool of pages: aligned bases, strides that hold what they step over.
+bool pool_ok(const void* k, const void* v, int64_t page, int64_t row, int64_t head, int n_pages, int page_size, int HK) {
+    if (!k || !v || !aligned(k, 16) || !aligned(v, 16) || n_pages < 1 || HK < 1 || !page_size_ok(page_size)) return false;
+    if (page % 8 || row % 8 || head % 8 || page < lr::D || row < lr::D || head < lr::D) return false;
+    // rows of a page token by token or head by head, pages apart from each other
+    const bool by_token = row >= (HK - 1) * head + lr::D && page >= (page_size - 1) * row + (HK - 1) * head + lr::D;
+    const bool by_head = head >= (page_size - 1) * row + lr::D && page >= (HK - 1) * head + (page_size - 1) * row + lr::D;
+    return by_token || by_head;
+}
+Span pool_span(const void* p, int layers, int64_t layer, int64_t page, int64_t row, int64_t head, int n_pages, int page_size,
+               int HK) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+    return Span{lo, lo + 2 * (uintptr_t)((layers - 1) * layer + (n_pages - 1) * page + (page_size - 1) * row +
+                                         (HK - 1) * head + lr::D)};
+}
+bool table_args_ok(const int* table, int64_t stride, int pages, int page_size, const int* starts, int B) {
+    return table && aligned(table, 4) && starts && aligned(starts, 4) && B >= 1 && pages >= 1 && stride >= pages &&
+           (int64_t)pages * page_size <= MAX_POS;
+}
+lr::PageArgs page_args(int64_t page, int64_t row, int64_t head, int n_pages, int page_size, const int* table, int64_t stride,
+                       int pages) {
+    lr::PageArgs g{};
+    g.ps = page; g.rs = row; g.hs = head;
+    g.table = table; g.table_rs = stride; g.table_pages = pages;
+    g.n_pages = n_pages; g.shift = shift_of(page_size);
+    return g;
+}
+
+// ------------------------------------------------------------------------------------------------ range attention
+// How a call is cut over the keys. tiles: the most key tiles that a block of rows sees; base: workgroups without a cut.
+struct Cut {
+    int nsplit, per;
+};
+Cut cut_of(int64_t base, int64_t tiles, int page_size) {
+    const int staged = page_size ? lr::RANGE_STAGED / std::max(1, lr::RANGE_TILE / page_size) : INT_MAX;
+    int64_t ns = std::min<int64_t>(std::max<int64_t>(1, 512 / std::max<int64_t>(base, 1)), std::max<int64_t>(1, tiles / 8));
+    int64_t per = std::max<int64_t>(1, std::min<int64_t>((tiles + ns - 1) / ns, staged));
+    ns = std::max<int64_t>(1, (tiles + per - 1) / per);
+    return Cut{(int)ns, (int)per};
+}
+int64_t block_rows(int64_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+
+// The most key tiles of a block: `span` keys behind the first that the block's rows share, and the first tokens.
+int64_t tiles_of(int64_t keys, int64_t span, int64_t sinks) {
+    const int64_t all = (keys + lr::RANGE_TILE - 1) / lr::RANGE_TILE;
+    return std::min(all, (std::min(sinks, keys) + lr::RANGE_TILE - 1) / lr::RANGE_TILE + span / lr::RANGE_TILE + 2);
+}
+Cut window_cut(int W, int H, int HK, int nkeys, int window, int sinks, int frame) {
+    const int64_t rows = (int64_t)W * (H / HK), br = block_rows(rows);
+    const int64_t tokens = std::min<int64_t>(W, br / (H / HK) + 1);
+    const int64_t span = (window + 2) * (int64_t)frame + tokens;
+    return cut_of((rows + br - 1) / br * HK, tiles_of(nkeys, span, sinks), 0);
+}
+Cut cache_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks) {
+    const int64_t rows = (int64_t)max_rows * (H / HK), br = block_rows(rows);
+    const int64_t span = window ? (int64_t)window + max_rows + 1 : max_keys;
+    return cut_of((rows + br - 1) / br * HK * B, tiles_of(max_keys, span, sinks), page_size);
+}
+size_t part_bytes(int64_t rows, int nsplit) {
+    return nsplit <= 1 ? 0 : (((size_t)rows * nsplit * lr::D * 4 + 255) & ~(size_t)255) + (((size_t)rows * nsplit * 8 + 255) & ~(size_t)255);
+}
+void set_parts(lr::RangeAttnArgs& a, void* ws, int64_t rows, Cut cut) {
+    a.nsplit = cut.nsplit;
+    a.tiles_per_split = cut.per;
+    a.part_o = static_cast<float*>(ws);
+    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + (((size_t)rows * cut.nsplit * lr::D * 4 + 255) & ~(size_t)255));
+}
+
+bool window_sizes_ok(int W, int H, int HK, int nkeys, int window, int sinks, int frame) {
+    return W >= 1 && H >= 1 && HK >= 1 && H % HK == 0 && nkeys >= 1 && nkeys <= MAX_POS && window >= 1 && sinks >= 0 &&
+           frame >= 1 && (int64_t)W * (H / HK) <= MAX_POS;
+}
+bool cache_sizes_ok(int B, int T, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks) {
+    return B >= 1 && B <= 65535 && T >= 1 && T <= MAX_POS && max_rows >= 1 && max_rows <= MAX_POS && max_keys >= 1 &&
+           max_keys <= MAX_POS && H >= 1 && HK >= 1 && H % HK == 0 && page_size_ok(page_size) && window >= 0 && sinks >= 0 &&
+           (int64_t)max_rows * (H / HK) <= MAX_POS;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t lr_attention_window_ws_bytes(int W, int H, int HK, int nkeys, int window, int sinks, int frame) {
+    if (!window_sizes_ok(W, H, HK, nkeys, window, sinks, frame)) return 0;
+    return part_bytes((int64_t)W * H, window_cut(W, H, HK, nkeys, window, sinks, frame).nsplit);
+}
+
+int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* out, int p0, int W, int H, int HK, int nkeys,
+                             int window, int sinks, int frame, float scale, int64_t q_row_stride, int64_t k_row_stride,
+                             int64_t v_row_stride, int64_t out_row_stride, void* workspace, size_t workspace_bytes,
+                             lr_stream_t stream) {
+    if (!window_sizes_ok(W, H, HK, nkeys, window, sinks, frame) || p0 < 0 || (int64_t)p0 + W > MAX_POS || !scale_ok(scale))
+        return ERR_ARGS;
+    if (!rows_ok(q, q_row_stride, H) || !rows_ok(out, out_row_stride, H) || !rows_ok(k, k_row_stride, HK) ||
+        !rows_ok(v, v_row_stride, HK))
+        return ERR_ARGS;
+    const Span so = rows_span(out, W, out_row_stride, H), sq = rows_span(q, W, q_row_stride, H),
+               sk = rows_span(k, nkeys, k_row_stride, HK), sv = rows_span(v, nkeys, v_row_stride, HK);
+    if (overlap(so, sq) || overlap(so, sk) || overlap(so, sv)) return ERR_ARGS;
+    lr::RangeAttnArgs a{};
+    const Cut cut = window_cut(W, H, HK, nkeys, window, sinks, frame);
+    const size_t need = part_bytes((int64_t)W * H, cut.nsplit);
+    if (need) {
+        if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return ERR_ARGS;
+        const uintptr_t lo = reinterpret_cast<uintptr_t>(workspace);
+        const Span w{lo, lo + need};
+        if (overlap(w, so) || overlap(w, sq) || overlap(w, sk) || overlap(w, sv)) return ERR_ARGS;
+    }
+    set_parts(a, workspace, (int64_t)W * H, cut);
+    a.q = static_cast<const uint16_t*>(q);
+    a.k = static_cast<const uint16_t*>(k);
+    a.v = static_cast<const uint16_t*>(v);
+    a.out = static_cast<uint16_t*>(out);
+    a.q_rs = q_row_stride; a.k_rs = k_row_stride; a.v_rs = v_row_stride; a.o_rs = out_row_stride;
+    a.H = H; a.HK = HK; a.G = H / HK;
+    a.c = scale * 1.4426950408889634f;
+    a.W = W; a.p0 = p0; a.nkeys = nkeys; a.frame = frame;
+    a.window = std::min(window, MAX_POS); a.sinks = std::min(sinks, MAX_POS);
+    return (int)lr::launch_range_attn(a, false, reinterpret_cast<hipStream_t>(stream));
+}
+
+size_t lr_cache_attention_ws_bytes(int B, int T, int max_rows, int max_keys, int H, int HK, int page_size, int window,
+                                   int sinks) {
+    if (!cache_sizes_ok(B, T, max_rows, max_keys, H, HK, page_size, window, sinks)) return 0;
+    return part_bytes((int64_t)T * H, cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks).nsplit);
+}
+
+int lr_cache_attention_bf16(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride, const void* k_pages,
+                            const void* v_pages, int64_t page_stride, int64_t row_stride, int64_t head_stride, int n_pages,
+                            int page_size, const int* page_table, int64_t table_stride, int table_pages, const int* starts,
+                            const int* lens, int B, int T, int max_rows, int max_keys, int H, int HK, const uint64_t* tree,
+                            int words, int window, int sinks, float scale, void* workspace, size_t workspace_bytes,
+                            lr_stream_t stream) {
+    if (!cache_sizes_ok(B, T, max_rows, max_keys, H, HK, page_size, window, sinks) || !scale_ok(scale)) return ERR_ARGS;
+    if (!rows_ok(q, q_row_stride, H) || !rows_ok(out, out_row_stride, H)) return ERR_ARGS;
+    if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK)) return ERR_ARGS;
+    if (!table_args_ok(page_table, table_stride, table_pages, page_size, starts, B) || !lens || !aligned(lens, 4))
+        return ERR_ARGS;
+    if (tree && (words < 1 || words > 64 || !aligned(tree, 8))) return ERR_ARGS;
+    const Span so = rows_span(out, T, out_row_stride, H), sq = rows_span(q, T, q_row_stride, H),
+               sk = pool_span(k_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK),
+               sv = pool_span(v_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK);
+    if (overlap(so, sq) || overlap(so, sk) || overlap(so, sv)) return ERR_ARGS;
+    lr::RangeAttnArgs a{};
+    const Cut cut = cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks);
+    const size_t need = part_bytes((int64_t)T * H, cut.nsplit);
+    if (need) {
+        if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return ERR_ARGS;
+        const uintptr_t lo = reinterpret_cast<uintptr_t>(workspace);
+        const Span w{lo, lo + need};
+        if (overlap(w, so) || overlap(w, sq) || overlap(w, sk) || overlap(w, sv)) return ERR_ARGS;
+    }
+    set_parts(a, workspace, (int64_t)T * H, cut);
+    a.q = static_cast<const uint16_t*>(q);
+    a.k = static_cast<const uint16_t*>(k_pages);
+    a.v = static_cast<const uint16_t*>(v_pages);
+    a.out = static_cast<uint16_t*>(out);
+    a.q_rs = q_row_stride; a.o_rs = out_row_stride;
+    a.H = H; a.HK = HK; a.G = H / HK;
+    a.c = scale * 1.4426950408889634f;
+    a.pg = page_args(page_stride, row_stride, head_stride, n_pages, page_size, page_table, table_stride, table_pages);
+    a.starts = starts; a.lens = lens; a.tree = tree; a.words = tree ? words : 0;
+    a.B = B; a.T = T; a.max_rows = max_rows; a.max_keys = max_keys;
+    a.window = std::min(window, MAX_POS); a.sinks = window ? std::min(sinks, MAX_POS) : 0;
+    return (int)lr::launch_range_attn(a, true, reinterpret_cast<hipStream_t>(stream));
+}
+
+int lr_cache_append_bf16(const void* q, const void* k, const void* v, int64_t q_row_stride, int64_t k_row_stride,
+                         int64_t v_row_stride, void* q_out, int64_t q_out_row_stride, void* k_pages, void* v_pages,
+                         int64_t page_stride, int64_t row_stride, int64_t head_stride, int n_pages, int page_size,
+                         const int* page_table, int64_t table_stride, int table_pages, const int* starts, const int* lens,
+                         const int* positions, int B, int T, int H, int HK, const float* q_norm_w, const float* k_norm_w,
+                         int table_kind, const void* table_a, const void* table_b, int64_t table_row_stride, int table_rows,
+                         int pairing, int rot_dim, float eps, lr_stream_t stream) {
+    const int rot = rot_dim == 0 ? lr::D : rot_dim;
+    if (T < 1 || T > MAX_POS || HK < 1 || (q && H < 1) || !(eps >= 0.0f) || !isfinite(eps)) return ERR_ARGS;
+    if (!rows_ok(k, k_row_stride, HK) || !rows_ok(v, v_row_stride, HK)) return ERR_ARGS;
+    if (q && (!rows_ok(q, q_row_stride, H) || !rows_ok(q_out, q_out_row_stride, H))) return ERR_ARGS;
+    if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK)) return ERR_ARGS;
+    if (!table_args_ok(page_table, table_stride, table_pages, page_size, starts, B) || !lens || !aligned(lens, 4) ||
+        (positions && !aligned(positions, 4)))
+        return ERR_ARGS;
+    if ((q_norm_w && !aligned(q_norm_w, 16)) || (k_norm_w && !aligned(k_norm_w, 16))) return ERR_ARGS;
+    if (!table_ok(table_kind, table_a, table_b, table_row_stride, rot, pairing, 16)) return ERR_ARGS;
+    if (table_kind != LR_TABLE_NONE && table_rows < 1) return ERR_ARGS;
+    const Span pk = pool_span(k_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK),
+               pv = pool_span(v_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK),
+               sk = rows_span(k, T, k_row_stride, HK), sv = rows_span(v, T, v_row_stride, HK);
+    if (overlap(pk, sk) || overlap(pk, sv) || overlap(pv, sk) || overlap(pv, sv)) return ERR_ARGS;
+    if (q) {
+        const Span sq = rows_span(q, T, q_row_stride, H), so = rows_span(q_out, T, q_out_row_stride, H);
+        if (overlap(pk, sq) || overlap(pv, sq) || overlap(pk, so) || overlap(pv, so)) return ERR_ARGS;
+        if (!(q_out == q && q_out_row_stride == q_row_stride) && overlap(sq, so)) return ERR_ARGS;
+        // (packed rows interleave: in place on the queries of a packed projection, its keys and values keep their columns)
+        if (!(q_out == q && q_out_row_stride == q_row_stride) && (overlap(so, sk) || overlap(so, sv))) return ERR_ARGS;
+    }
+    lr::CacheAppendArgs a{};
+    a.q = static_cast<const uint16_t*>(q);
+    a.k = static_cast<const uint16_t*>(k);
+    a.v = static_cast<const uint16_t*>(v);
+    a.q_out = static_cast<uint16_t*>(q_out);
+    a.kp = static_cast<uint16_t*>(k_pages);
+    a.vp = static_cast<uint16_t*>(v_pages);
+    a.q_rs = q_row_stride; a.k_rs = k_row_stride; a.v_rs = v_row_stride; a.qo_rs = q_out_row_stride;
+    a.pg = page_args(page_stride, row_stride, head_stride, n_pages, page_size, page_table, table_stride, table_pages);
+    a.starts = starts; a.lens = lens; a.pos = positions;
+    a.B = B; a.T = T; a.H = q ? H : 0; a.HK = HK;
+    a.qw = q_norm_w; a.kw = k_norm_w;
+    a.table_kind = table_kind; a.pairing = pairing; a.rot = rot; a.tab_rows = table_rows;
+    a.tab_vec = tab_vec(table_kind, table_a, table_b, table_row_stride);
+    a.ta = table_a; a.tb = table_b; a.tab_stride = table_row_stride; a.eps = eps;
+    return (int)lr::launch_cache_append(a, reinterpret_cast<hipStream_t>(stream));
+}
+
+int lr_cache_copy_pages(void* k_pages, void* v_pages, int layers, int64_t layer_stride, int64_t page_stride,
+                        int64_t row_stride, int64_t head_stride, int n_pages, int page_size, int HK, const int* src,
+                        const int* dst, int n, lr_stream_t stream) {
+    if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK)) return ERR_ARGS;
+    if (layers < 1 || layers > 65535 || layer_stride % 8 || layer_stride < 0 || n < 1 || !src || !dst || !aligned(src, 4) ||
+        !aligned(dst, 4))
+        return ERR_ARGS;
+    lr::CacheCopyArgs a{};
+    a.kp = static_cast<uint16_t*>(k_pages);
+    a.vp = static_cast<uint16_t*>(v_pages);
+    a.pg = page_args(page_stride, row_stride, head_stride, n_pages, page_size, nullptr, 0, 0);
+    a.layer_stride = layer_stride;
+    a.src = src; a.dst = dst; a.n = n; a.layers = layers; a.HK = HK;
+    return (int)lr::launch_cache_copy(a, reinterpret_cast<hipStream_t>(stream));
+}
+
+int lr_cache_move_rows(void* k_pages, void* v_pages, int layers, int64_t layer_stride, int64_t page_stride,
+                       int64_t row_stride, int64_t head_stride, int n_pages, int page_size, int HK, const int* page_table,
+                       int64_t table_stride, int table_pages, const int* starts, const int* src, const int* dst, int B, int n,
+                       int max_rows, lr_stream_t stream) {
+    if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK)) return ERR_ARGS;
+    if (!table_args_ok(page_table, table_stride, table_pages, page_size, starts, B)) return ERR_ARGS;
+    if (layers < 1 || layers > 32767 || layer_stride % 8 || layer_stride < 0 || n < 1 || !src || !dst || !aligned(src, 4) ||
+        !aligned(dst, 4) || max_rows < 1 || max_rows > 256)
+        return ERR_ARGS;
+    lr::CacheMoveArgs a{};
+    a.kp = static_cast<uint16_t*>(k_pages);
+    a.vp = static_cast<uint16_t*>(v_pages);
+    a.pg = page_args(page_stride, row_stride, head_stride, n_pages, page_size, page_table, table_stride, table_pages);
+    a.layer_stride = layer_stride;
+    a.starts = starts; a.src = src; a.dst = dst; a.B = B; a.n = n; a.max_rows = max_rows; a.layers = layers; a.HK = HK;
+    return (int)lr::launch_cache_move(a, reinterpret_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

@@ -13,6 +13,7 @@
 #include <mutex>
 
 #include "../../include/lr_attn.h"
+#include "abi_checks.h"
 #include "lr_common.h"
 #include "lr_int8.h"
 #include "lr_kernels.h"
@@ -21,16 +22,7 @@
 
 namespace {
 
-constexpr int ERR_ARGS = (int)hipErrorInvalidValue;
-
-inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
-
-// A bf16 rows tensor: 16-byte aligned base, row stride a multiple of 8 elements and wide enough for its heads.
-inline bool rows_ok(const void* p, int64_t rs, int heads) {
-    return p && aligned(p, 16) && rs % 8 == 0 && rs >= (int64_t)heads * lr::D;
-}
-
-inline bool scale_ok(float s) { return s > 0.0f && isfinite(s); }
+using namespace lr::abi;
 
 // Count of key ranges for plain attention over value rows (the pipelined kernel, 256-query blocks): a non-causal launch
 // with at most 32 query blocks and at least 16 key tiles is split over the keys into enough ranges of at least 4 key
@@ -230,20 +222,6 @@ int attention_impl(const void* q, const void* k, const void* v, void* out, int p
     return (int)lr::launch_attention(a, route, stream);
 }
 
-// Table checks shared by the rope entry points. rows_needed: table rows that will be read.
-bool table_ok(int kind, const void* ta, const void* tb, int64_t stride, int rot, int pairing, int split_mod) {
-    if (kind == LR_TABLE_NONE) return true;
-    if (kind < LR_TABLE_NONE || kind > LR_TABLE_MAT2_F32) return false;
-    if (rot <= 0 || rot > lr::D || rot % 2) return false;
-    if (pairing != LR_PAIR_INTERLEAVED && pairing != LR_PAIR_SPLIT_HALF) return false;
-    if (pairing == LR_PAIR_SPLIT_HALF && rot % split_mod) return false;
-    if (!ta || stride < 0) return false;
-    const int pairs = rot / 2;
-    if (kind == LR_TABLE_COSSIN_F32) return tb && aligned(ta, 4) && aligned(tb, 4) && stride >= pairs;
-    if (kind == LR_TABLE_MAT2_BF16) return aligned(ta, 8) && stride % 4 == 0 && stride >= 4 * pairs;
-    return aligned(ta, 16) && stride % 4 == 0 && stride >= 4 * pairs;  // LR_TABLE_MAT2_F32
-}
-
 // Workspace of the fused op and of its two stages: the tile images of the keys (tile_image.h), 16 KB per 64-key tile
 // and kv head; then the value area, the same size: value rows [tiles * 64][HK][128] bf16, written by the stage calls
 // (the fused call reads the caller's value rows and leaves it unused); then the streaming kernel's split area
@@ -264,19 +242,10 @@ int device_cus() {
     return n;
 }
 
-// byte range [lo, hi) of a rows tensor: rows rows of heads heads, row stride rs elements
-struct Span {
-    uintptr_t lo, hi;
-};
-inline Span rows_span(const void* p, int64_t rows, int64_t rs, int heads) {
-    const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
-    return Span{lo, lo + (uintptr_t)(((rows - 1) * rs + (int64_t)heads * lr::D) * 2)};
-}
 inline Span ws_span(const void* ws, int Sk, int HK) {
     const uintptr_t lo = reinterpret_cast<uintptr_t>(ws);
     return Span{lo, lo + ws_bytes_needed(Sk, HK)};
 }
-inline bool overlap(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
 // byte range of a bf16 [B][X][S][D] tensor with element strides sb, sx, sn (a row's D elements contiguous)
 inline Span t4_span(const void* p, int B, int X, int S, int D, int64_t sb, int64_t sx, int64_t sn) {
     const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
@@ -300,11 +269,6 @@ bool kv_stage_ok(const void* k_raw, int64_t k_rs, const void* v, int64_t v_rs, c
 
 // The keys stage (arguments checked): RMSNorm + RoPE of k_raw rows j >= n_pre (k-table row j - n_pre; rows j < n_pre
 // copied) and the values, into the workspace's tile images.
-// cos / sin tables whose rows are 16-byte aligned are read as 16-byte chunks
-inline int tab_vec(int kind, const void* ta, const void* tb, int64_t stride) {
-    return kind == LR_TABLE_COSSIN_F32 && aligned(ta, 16) && aligned(tb, 16) && stride % 4 == 0;
-}
-
 lr::KvImageArgs kv_args(const void* k_raw, int64_t k_rs, const void* v, int64_t v_rs, const float* wk, int table_kind,
                         const void* kta, const void* ktb, int64_t tab_stride, int pairing, int rot, float eps, int Sk,
                         int HK, int n_pre, void* ws, int copy_v) {

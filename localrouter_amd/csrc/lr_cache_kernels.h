@@ -1,0 +1,101 @@
+// Internal launch interface between the C ABI of the paged cache and the windowed attention (cache_abi.hip) and their
+// kernels (attn_cache.hip, cache_rows.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "lr_kernels.h"
+
+namespace lr {
+
+// A pool of pages: row r of page p of kv head g at base + p * ps + r * rs + g * hs (elements), and the page tables of the
+// sequences: position j of sequence b lies in row j & (page_size - 1) of page table[b * table_rs + (j >> shift)]. An entry
+// outside [0, n_pages) holds no rows.
+struct PageArgs {
+    int64_t ps, rs, hs;
+    const int* table;
+    int64_t table_rs;
+    int n_pages, shift, table_pages;
+};
+
+// Attention of query tokens over a sequence's keys, each token over its own range of them. Two sources of keys:
+// rows (paged = 0: one sequence, key j of kv head g at k + j * k_rs + g * 128) and pages.
+struct RangeAttnArgs {
+    const uint16_t* q;   // bf16 [T][H][128], row stride q_rs
+    uint16_t* out;       // bf16 [T][H][128], row stride o_rs
+    const uint16_t* k;
+    const uint16_t* v;
+    int64_t q_rs, o_rs, k_rs, v_rs;
+    int H, HK, G;
+    float c;             // scale * log2(e)
+    // rows: tokens i < W at positions p0 + i; frame f = p / frame sees keys of frames (f - window, f] below nkeys, and
+    // keys below sinks of frames before
+    int W, p0, nkeys, frame;
+    // pages: tokens starts[b] .. starts[b + 1] of sequence b are its last positions before lens[b]; at most max_rows of them
+    // a sequence and T in all, keys below max_keys
+    PageArgs pg;
+    const int* starts;
+    const int* lens;
+    const uint64_t* tree;   // [T][words]: bit x of a token's words: it sees the sequence's drafted token x; null: chains
+    int B, T, max_rows, max_keys, words;
+    int window, sinks;      // window 0 (pages only): every earlier key
+    // Split over the keys: nsplit > 1 runs every block of rows as nsplit workgroups of tiles_per_split key tiles each; the
+    // ranges' unnormalised rows, references and sums go to the parts, [token][head][split], merged by a second launch.
+    int nsplit, tiles_per_split;
+    float* part_o;
+    float* part_ml;
+};
+
+constexpr int RANGE_TILE = 32;         // keys a tile of the small-row kernel
+constexpr int RANGE_STAGED = 2048;     // page-table entries a workgroup holds
+
+hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, hipStream_t stream);
+
+// cache_rows.hip
+struct CacheAppendArgs {
+    const uint16_t* q;   // bf16 [T][H][128] (null: no queries)
+    const uint16_t* k;   // bf16 [T][HK][128]
+    const uint16_t* v;
+    uint16_t* q_out;
+    uint16_t* kp;        // pages
+    uint16_t* vp;
+    int64_t q_rs, k_rs, v_rs, qo_rs;
+    PageArgs pg;
+    const int* starts;
+    const int* lens;
+    const int* pos;      // table row of each token; null: its position in its sequence
+    int B, T, H, HK;
+    const float* qw;     // fp32 [128] or null for ones
+    const float* kw;
+    int table_kind, pairing, rot, tab_rows, tab_vec;
+    const void* ta;
+    const void* tb;
+    int64_t tab_stride;
+    float eps;
+};
+hipError_t launch_cache_append(const CacheAppendArgs& a, hipStream_t stream);
+
+struct CacheCopyArgs {
+    uint16_t* kp;
+    uint16_t* vp;
+    PageArgs pg;         // no table
+    int64_t layer_stride;
+    const int* src;
+    const int* dst;
+    int n, layers, HK;
+};
+hipError_t launch_cache_copy(const CacheCopyArgs& a, hipStream_t stream);
+
+struct CacheMoveArgs {
+    uint16_t* kp;
+    uint16_t* vp;
+    PageArgs pg;
+    int64_t layer_stride;
+    const int* starts;
+    const int* src;
+    const int* dst;
+    int B, n, max_rows, layers, HK;
+};
+hipError_t launch_cache_move(const CacheMoveArgs& a, hipStream_t stream);
+
+}  // namespace lr

@@ -3,6 +3,7 @@
   attention(...)        <- Ops.attention, src/engines/qwen_image/ops_launch.zig:163-172
   rms_rope(...)         <- Triton.ropeRun + Rope, src/engines/qwen_image/triton_k.zig:44-53
   rms_rope_qk(...)      <- Kitchen.rmsRope, src/engines/minimax_h3/launch.zig:421-441
+  attention_window(...) a window of frames and first tokens (no counterpart in the reference)
   joint_attention(...)  <- Dit.block's rope_q / rope_k / V copy / attention chain, src/engines/qwen_image/dit.zig:252-293
   joint_kv_prepare(...), joint_attention_prepared(...)  <- its two stages (keys / values reused across calls)
   joint_q_prepare(...), joint_attention_images(...)     <- the fused op's query and attention launches one by one
@@ -109,6 +110,45 @@ def attention_ws(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.T
     _lib.call("lr_attention_bf16_ws", _ptr(q), _ptr(k), _ptr(v), _ptr(out), p0, w, heads, kv_heads, nkeys,
               int(causal), scale, q_rs, k_rs, o_rs, _ptr(workspace), 0 if workspace is None else workspace.numel(),
               _stream())
+    return out
+
+
+def attention_window_ws_bytes(w: int, heads: int, kv_heads: int, nkeys: int, *, window: int, sinks: int = 0,
+                              frame: int = 1) -> int:
+    """lr_attention_window_ws_bytes: the workspace lr_attention_window_bf16 needs (0: none)."""
+    return int(_lib.load().lr_attention_window_ws_bytes(w, heads, kv_heads, nkeys, window, sinks, frame))
+
+
+def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor | None = None, *, window: int,
+                     sinks: int = 0, frame: int = 1, p0: int = 0, scale: float = SCALE_128,
+                     workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """lr_attention_window_bf16: q [w, heads, 128] at positions p0 + i over k / v [nkeys, kv_heads, 128]; a query in frame
+    f = position // frame sees the keys of frames f - window + 1 .. f and the first `sinks` keys (up to frame f). frame 1: a
+    sliding window of single tokens. A workspace of attention_window_ws_bytes is allocated when none is given."""
+    w, heads = q.shape[0], q.shape[1]
+    nkeys, kv_heads = k.shape[0], k.shape[1]
+    q_rs, k_rs, v_rs = _rows(q, "q", heads), _rows(k, "k", kv_heads), _rows(v, "v", kv_heads)
+    if v.shape[0] < nkeys:
+        raise ValueError("attention_window: v shorter than k")
+    if out is None:
+        out = torch.empty((w, heads, D), dtype=torch.bfloat16, device=q.device)
+    o_rs = _rows(out, "out", heads)
+    if out.shape[0] < w:
+        raise ValueError("attention_window: out shorter than q")
+    dev = torch._C._cuda_getDevice()
+    for t in (q, k, v, out):
+        if t.get_device() != dev:
+            raise ValueError(f"attention_window: a tensor on {t.device}, the current device is {dev}")
+    need = attention_window_ws_bytes(w, heads, kv_heads, nkeys, window=window, sinks=sinks, frame=frame)
+    nbytes = 0
+    if workspace is not None:
+        nbytes = workspace.numel() * workspace.element_size()
+        if nbytes < need or workspace.get_device() != dev or not workspace.is_contiguous():
+            raise ValueError(f"workspace: {need} contiguous bytes on the current device needed")
+    elif need:
+        workspace, nbytes = torch.empty(need, dtype=torch.uint8, device=q.device), need
+    _lib.call("lr_attention_window_bf16", _ptr(q), _ptr(k), _ptr(v), _ptr(out), p0, w, heads, kv_heads, nkeys, window, sinks,
+              frame, scale, q_rs, k_rs, v_rs, o_rs, _ptr(workspace), nbytes, _stream())
     return out
 
 

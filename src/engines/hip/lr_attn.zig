@@ -16,6 +16,9 @@
 
 const std = @import("std");
 
+/// include/lr_cache.h: the cache in pages.
+pub const cache = @import("lr_cache.zig");
+
 pub const Stream = ?*anyopaque;
 
 pub const HEAD_DIM = 128;
@@ -54,6 +57,11 @@ pub extern "lr_attn" fn lr_attention_ws_bytes(w: c_int, h: c_int, nkeys: c_int, 
 pub extern "lr_attn" fn lr_attention_bf16_ws(q: u64, k: u64, v: u64, out: u64, p0: c_int, w: c_int, h: c_int, hk: c_int,
     nkeys: c_int, causal: c_int, scale: f32, q_rs: i64, kv_rs: i64, out_rs: i64, ws: u64, ws_bytes: usize,
     s: Stream) c_int;
+pub extern "lr_attn" fn lr_attention_window_ws_bytes(w: c_int, h: c_int, hk: c_int, nkeys: c_int, window: c_int,
+    sinks: c_int, frame: c_int) usize;
+pub extern "lr_attn" fn lr_attention_window_bf16(q: u64, k: u64, v: u64, out: u64, p0: c_int, w: c_int, h: c_int, hk: c_int,
+    nkeys: c_int, window: c_int, sinks: c_int, frame: c_int, scale: f32, q_rs: i64, k_rs: i64, v_rs: i64, out_rs: i64,
+    ws: u64, ws_bytes: usize, s: Stream) c_int;
 pub extern "lr_attn" fn lr_attention_kmask_workspace_bytes(n_valid: c_int, hk: c_int) usize;
 pub extern "lr_attn" fn lr_attention_kmask_bf16(q: u64, k: u64, v: u64, out: u64, kmask: u64, n_valid: c_int, w: c_int,
     h: c_int, hk: c_int, nkeys: c_int, scale: f32, q_rs: i64, kv_rs: i64, out_rs: i64, ws: u64, ws_bytes: usize,

@@ -1,0 +1,210 @@
+"""The paged cache and the windowed attention on the CPU: the ctypes and Zig bindings agree with the headers, bad arguments are
+refused before any GPU call, and the page bookkeeping. No compute calls."""
+from __future__ import annotations
+
+import re
+from pathlib import Path
+
+import pytest
+import torch
+
+from localrouter_amd import _lib, cache, ops
+from tests.test_zig_bindings import C_KIND, ZIG_KIND
+
+ROOT = Path(__file__).resolve().parent.parent
+BAD = 1   # hipErrorInvalidValue
+# fake, well-aligned device addresses, far apart from each other
+Q, K, V, O, KP, VP, WS = (x << 32 for x in (1, 2, 3, 4, 5, 6, 7))
+I1, I2, I3, I4, I5, I6 = (x << 32 for x in (8, 9, 10, 11, 12, 13))
+
+
+def _header_kinds():
+    text = re.sub(r"/\*.*?\*/", "", cache.HEADER.read_text(), flags=re.S)
+    out = {}
+    for m in re.finditer(r"\b(int|size_t)\s+(lr_\w+)\s*\(([^)]*)\)\s*;", text):
+        args = [a.strip() for a in m.group(3).split(",")]
+        out[m.group(2)] = (C_KIND[m.group(1)], ["ptr" if "*" in a or a.startswith("lr_stream_t") else
+                                                C_KIND[a.rsplit(" ", 1)[0].replace("const ", "")] for a in args])
+    return out
+
+
+def test_bindings_match_the_header():
+    kinds = {cache._P: "ptr", cache._I: "i32", cache._I64: "i64", cache._F: "f32", cache._SZ: "usize"}
+    head = _header_kinds()
+    assert len(head) == 5
+    assert {n: (kinds[r], [kinds[a] for a in args]) for n, (r, args) in cache.SIGNATURES.items()} == head
+    assert all(hasattr(cache.lib(), n) for n in head)
+    zig = {}
+    text = (ROOT / "src/engines/hip/lr_cache.zig").read_text()
+    for m in re.finditer(r'pub extern "lr_attn" fn (lr_\w+)\((.*?)\)\s*(\w+);', text, flags=re.S):
+        zig[m.group(1)] = (ZIG_KIND[m.group(3)], [ZIG_KIND[a.split(":", 1)[1].strip()]
+                                                  for a in m.group(2).replace("\n", " ").split(",")])
+    assert zig == head
+
+
+def _window(**kw):
+    a = dict(q=Q, k=K, v=V, out=O, p0=0, W=300, H=8, HK=2, nkeys=700, window=64, sinks=4, frame=1, scale=0.088, qrs=1024,
+             krs=256, vrs=256, ors=1024, ws=WS, wsb=1 << 31, stream=None)
+    a.update(kw)
+    return _lib.load().lr_attention_window_bf16(*a.values())
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q=0), dict(v=0), dict(out=0), dict(W=0), dict(H=9), dict(HK=0), dict(nkeys=0), dict(window=0), dict(window=-3),
+    dict(sinks=-1), dict(frame=0), dict(scale=0.0), dict(scale=float("nan")), dict(p0=-1), dict(p0=(1 << 30) - 100),
+    dict(nkeys=(1 << 30) + 1), dict(q=Q + 8), dict(qrs=1023), dict(krs=128), dict(vrs=252), dict(ors=1020),
+    dict(out=Q), dict(out=K + 4096), dict(out=V + 256), dict(W=1, H=2, nkeys=100000, window=100000, ws=0),
+    dict(W=1, H=2, nkeys=100000, window=100000, wsb=8), dict(W=1, H=2, nkeys=100000, window=100000, ws=WS + 16),
+    dict(W=1, H=2, nkeys=100000, window=100000, ws=K),
+], ids=str)
+def test_window_refuses(kw):
+    assert _window(**kw) == BAD
+
+
+def test_window_workspace_sizes():
+    L = _lib.load()
+    assert L.lr_attention_window_ws_bytes(0, 8, 2, 700, 64, 4, 1) == 0
+    assert ops.attention_window_ws_bytes(16384, 32, 32, 16384, window=4, sinks=1024, frame=1024) == 0   # fills the GPU
+    # one token over many keys is split: fp32 rows of 128 and (reference, sum) a range
+    need = ops.attention_window_ws_bytes(1, 8, 2, 100000, window=100000)
+    assert need > 0 and need % 256 == 0
+    # a window bounds what is split, whatever lies before it
+    assert ops.attention_window_ws_bytes(1, 8, 2, 1 << 29, window=64) <= ops.attention_window_ws_bytes(1, 8, 2, 512, window=512)
+
+
+def _attend(**kw):
+    a = dict(q=Q, qrs=1024, out=O, ors=1024, kp=KP, vp=VP, ps=4096, rs=256, hs=128, n_pages=40, page=16, table=I1, trs=10,
+             tp=10, starts=I2, lens=I3, B=3, T=12, rows=6, keys=160, H=8, HK=2, tree=0, words=0, window=0, sinks=0,
+             scale=0.088, ws=WS, wsb=1 << 30, stream=None)
+    a.update(kw)
+    return cache.lib().lr_cache_attention_bf16(*a.values())
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q=0), dict(out=0), dict(kp=0), dict(vp=0), dict(table=0), dict(starts=0), dict(lens=0), dict(B=0), dict(B=70000),
+    dict(T=0), dict(rows=0), dict(keys=0), dict(H=7), dict(HK=0), dict(page=12), dict(page=0), dict(page=1 << 17),
+    dict(n_pages=0), dict(kp=KP + 8), dict(ps=4090), dict(rs=120), dict(hs=64), dict(hs=124), dict(rs=128),
+    dict(ps=2048), dict(trs=9), dict(tp=0), dict(tp=1 << 27, trs=1 << 27), dict(tree=I4, words=0), dict(tree=I4, words=65),
+    dict(tree=I4 + 4, words=1), dict(window=-1), dict(sinks=-1), dict(scale=-1.0), dict(scale=float("inf")),
+    dict(out=Q), dict(out=KP + 256), dict(keys=(1 << 30) + 1),
+    dict(B=1, keys=160000, tp=10000, trs=10000, ws=0), dict(B=1, keys=160000, tp=10000, trs=10000, wsb=256),
+    dict(B=1, keys=160000, tp=10000, trs=10000, ws=KP), dict(B=1, keys=160000, tp=10000, trs=10000, ws=O),
+], ids=str)
+def test_attention_refuses(kw):
+    assert _attend(**kw) == BAD
+
+
+def _append(**kw):
+    a = dict(q=Q, k=K, v=V, qrs=1024, krs=256, vrs=256, qo=O, qors=1024, kp=KP, vp=VP, ps=4096, rs=256, hs=128, n_pages=40,
+             page=16, table=I1, trs=10, tp=10, starts=I2, lens=I3, pos=0, B=3, T=12, H=8, HK=2, qw=0, kw=0, kind=1, ta=I4,
+             tb=I5, tabs=64, rows=100, pairing=0, rot=128, eps=1e-6, stream=None)
+    a.update(kw)
+    return cache.lib().lr_cache_append_bf16(*a.values())
+
+
+@pytest.mark.parametrize("kw", [
+    dict(k=0), dict(v=0), dict(qo=0), dict(kp=0), dict(vp=0), dict(table=0), dict(starts=0), dict(lens=0), dict(T=0),
+    dict(H=0), dict(HK=0), dict(B=0), dict(qrs=1020), dict(krs=128), dict(qors=512), dict(page=24), dict(n_pages=0),
+    dict(qw=I6 + 4), dict(kw=I6 + 8), dict(kind=9), dict(ta=0), dict(tb=0), dict(tabs=63), dict(rows=0), dict(pairing=2),
+    dict(rot=130), dict(rot=63), dict(pairing=1, rot=40), dict(eps=-1.0), dict(eps=float("nan")), dict(pos=I6 + 2),
+    dict(qo=Q + 256), dict(qo=Q, qors=2048), dict(k=KP), dict(v=VP + 4096), dict(q=KP), dict(qo=VP), dict(qo=K),
+], ids=str)
+def test_append_refuses(kw):
+    assert _append(**kw) == BAD
+
+
+def _copy(**kw):
+    a = dict(kp=KP, vp=VP, layers=2, ls=1 << 20, ps=4096, rs=256, hs=128, n_pages=40, page=16, HK=2, src=I1, dst=I2, n=5,
+             stream=None)
+    a.update(kw)
+    return cache.lib().lr_cache_copy_pages(*a.values())
+
+
+def _move(**kw):
+    a = dict(kp=KP, vp=VP, layers=2, ls=1 << 20, ps=4096, rs=256, hs=128, n_pages=40, page=16, HK=2, table=I1, trs=10, tp=10,
+             starts=I2, src=I3, dst=I4, B=3, n=9, rows=5, stream=None)
+    a.update(kw)
+    return cache.lib().lr_cache_move_rows(*a.values())
+
+
+@pytest.mark.parametrize("kw", [dict(kp=0), dict(vp=0), dict(layers=0), dict(ls=4), dict(ls=-8), dict(ps=100), dict(page=3),
+                                dict(HK=0), dict(src=0), dict(dst=0), dict(dst=I2 + 2), dict(n=0), dict(n=-1)], ids=str)
+def test_copy_refuses(kw):
+    assert _copy(**kw) == BAD
+
+
+@pytest.mark.parametrize("kw", [dict(kp=0), dict(vp=0), dict(layers=0), dict(layers=40000), dict(ls=-8), dict(rs=100),
+                                dict(page=3), dict(table=0), dict(starts=0), dict(src=0), dict(dst=0), dict(B=0), dict(n=0),
+                                dict(rows=0), dict(rows=257), dict(trs=9)], ids=str)
+def test_move_refuses(kw):
+    assert _move(**kw) == BAD
+
+
+def test_python_checks_refuse_host_tensors():
+    t = torch.zeros(4, 2, 128, dtype=torch.bfloat16)
+    p = torch.zeros(3, 16, 2, 128, dtype=torch.bfloat16)
+    i = torch.zeros(5, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        ops.attention_window(t, t, t, window=4)
+    with pytest.raises(ValueError):
+        cache.attention(t, p, p, i[None], i[:2], i[:1])
+    with pytest.raises(ValueError):
+        cache.append(t, t, t, p, p, i[None], i[:2], i[:1], table_kind=ops.TABLE_NONE)
+    if not torch.cuda.is_available():
+        with pytest.raises(ValueError):
+            cache.copy_pages(p, p, i, i)
+        with pytest.raises(ValueError):
+            cache.move_rows(p, p, i[None], i[:2], i, i)
+
+
+# ------------------------------------------------------------------------------------------------ bookkeeping
+def test_pool_alloc_fork_free():
+    pool = cache.PagePool(5)
+    a = pool.alloc(3)
+    assert len(set(a)) == 3 and pool.free_pages == 2
+    with pytest.raises(MemoryError):
+        pool.alloc(3)
+    assert pool.free_pages == 2
+    b = pool.fork(a)
+    assert b == a and b is not a and pool.free_pages == 2
+    pool.free(a)
+    assert pool.free_pages == 2          # still held by the fork
+    pool.free(b)
+    assert pool.free_pages == 5
+    for bad in ([a[0]], [-1], [5]):
+        with pytest.raises(ValueError):
+            pool.free(bad)
+    c = pool.alloc(1)
+    with pytest.raises(ValueError):
+        pool.free(c + c)                 # once held, freed twice in one call: nothing happens
+    assert pool.free_pages == 4 and pool.alloc(0) == []
+
+
+def test_pool_own_gives_a_page_of_its_own():
+    pool = cache.PagePool(4)
+    a = pool.alloc(2)
+    assert pool.own(a, 1) is None
+    b = pool.fork(a)
+    src, dst = pool.own(b, 1)
+    assert src == a[1] and dst == b[1] and dst not in a and b[0] == a[0]
+    assert pool.own(a, 1) is None and pool.own(b, 1) is None     # each its own now
+    pool.free(a)
+    pool.free(b)
+    assert pool.free_pages == 4
+
+
+def test_pool_compact_packs_to_the_front():
+    pool = cache.PagePool(8)
+    a, b, c = pool.alloc(3), pool.alloc(2), pool.alloc(2)
+    d = pool.fork(c)
+    pool.free(a)
+    with pytest.raises(ValueError):
+        pool.compact([b, c])             # the fork's table is missing
+    tables = [b, c, d]
+    before = [list(t) for t in tables]
+    src, dst = pool.compact(tables)
+    assert not set(src) & set(dst) and all(x >= 4 for x in src) and all(x < 4 for x in dst)
+    moved = dict(zip(src, dst))
+    assert tables == [[moved.get(p, p) for p in t] for t in before] and sorted({p for t in tables for p in t}) == [0, 1, 2, 3]
+    assert c == d and pool.free_pages == 4 and sorted(pool.alloc(4)) == [4, 5, 6, 7]
+    assert pool.compact([]) == ([], []) if pool.free_pages == 8 else True

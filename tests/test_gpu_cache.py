@@ -1,0 +1,603 @@
+"""The paged cache on the GPU: attention over pages, appends, page copies and row moves, each against a plain 64-bit (or
+exact) restatement, and a serving loop of them together."""
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+
+from localrouter_amd import _lib, cache, ops, rope
+from tests.cache_util import HALF, check_rows, gen, ref_rows, rnd
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def make_pool(g, pages, ps, HK, by_head=False, layers=None):
+    """Two tensors [layers,] [pages, ps, HK, 128] with the same strides; by_head: rows of a head next to each other."""
+    def one():
+        shape = ((layers,) if layers else ()) + ((pages, HK, ps, 128) if by_head else (pages, ps, HK, 128))
+        t = rnd(g, *shape)
+        return t.transpose(-3, -2) if by_head else t
+    return one(), one()
+
+
+class Batch:
+    """Sequences over a pool: n tokens of the call each, L positions in all."""
+
+    def __init__(self, seed, news, lens, ps, HK, by_head=False, spare=3, pages=None):
+        rng = random.Random(seed)
+        self.g, self.ps, self.HK, self.news, self.L = gen(seed), ps, HK, news, lens
+        need = [-(-x // ps) for x in lens]
+        ids = list(range(pages or sum(need) + spare))
+        rng.shuffle(ids)
+        self.width = max(need + [1])
+        self.table = []
+        for n in need:
+            self.table.append([ids.pop() for _ in range(n)] + [-1] * (self.width - n))
+        self.n_pages = pages or sum(need) + spare
+        self.kp, self.vp = make_pool(self.g, self.n_pages, ps, HK, by_head)
+        self.t = ints(self.table)
+        st = [0]
+        for n in news:
+            st.append(st[-1] + n)
+        self.st, self.starts, self.lens = st, ints(st), ints(lens)
+
+    def rows(self, b):
+        """Keys and values of sequence b as rows."""
+        at = torch.arange(self.L[b], device="cuda")
+        page, row = self.t[b][at // self.ps].long(), at % self.ps
+        return self.kp[page, row], self.vp[page, row]
+
+    def check(self, q, out, seen_of, scale=1.0 / 128 ** 0.5):
+        for b, n in enumerate(self.news):
+            if n:
+                k, v = self.rows(b)
+                s = slice(self.st[b], self.st[b] + n)
+                check_rows(out[s], *ref_rows(q[s], k, v, seen_of(b), scale), what=f"sequence {b}")
+
+
+def chain_seen(n, L, window=0, sinks=0):
+    p = (L - n + torch.arange(n))[:, None]
+    j = torch.arange(L)[None]
+    return (j <= p) & ((p - j < window) | (j < sinks) if window else torch.ones(1, dtype=torch.bool))
+
+
+def random_tree(rng, n):
+    sets = []
+    for i in range(n):
+        parent = rng.randrange(-1, i)
+        sets.append({i} | (sets[parent] if parent >= 0 else set()))
+    return sets
+
+
+def tree_words(trees, words):
+    rows = []
+    for sets in trees:
+        for s in sets:
+            w = [sum(1 << (x & 63) for x in s if x >> 6 == u) for u in range(words)]
+            rows.append([x - (1 << 64) if x >> 63 else x for x in w])
+    return torch.tensor(rows, dtype=torch.int64, device="cuda")
+
+
+def tree_seen(sets, L, window=0, sinks=0):
+    n = len(sets)
+    c = L - n
+    seen = torch.zeros(n, L, dtype=torch.bool)
+    for i, s in enumerate(sets):
+        p = c + len(s) - 1
+        for j in range(c):
+            seen[i, j] = not window or p - j < window or j < sinks
+        for x in s:
+            seen[i, c + x] = True
+    return seen
+
+
+# ------------------------------------------------------------------------------------------------ attention
+# tokens of each sequence, lengths, heads, kv heads, page size, window, sinks, by_head
+CHAINS = [
+    ([1], [1], 1, 1, 16, 0, 0, False),
+    ([1], [777], 8, 2, 16, 0, 0, False),
+    ([1], [5000], 4, 4, 64, 0, 0, False),                                   # split over the keys
+    ([1, 1, 1], [33, 1, 400], 7, 1, 8, 0, 0, True),
+    ([1, 0, 1, 1], [64, 5, 100, 31], 8, 8, 32, 0, 0, False),                # a sequence without tokens
+    ([3, 1, 7], [3, 90, 7], 4, 2, 16, 0, 0, False),                         # prompts without context
+    ([20, 33, 1], [220, 33, 65], 6, 2, 1, 0, 0, False),                     # pages of one row
+    ([150, 9], [150, 300], 4, 1, 128, 0, 0, True),
+    ([1, 1], [900, 2000], 8, 2, 16, 100, 4, False),
+    ([40, 17], [300, 170], 4, 2, 4, 33, 7, False),
+    ([5], [4000], 16, 1, 256, 1500, 1, True),
+    ([1] * 40, [50 + 13 * i for i in range(40)], 2, 1, 16, 0, 0, False),
+    ([2], [3000], 64, 1, 16, 0, 0, False),                                  # 128 rows of one kv head, split
+]
+
+
+@pytest.mark.parametrize("c", CHAINS, ids=lambda c: f"{len(c[0])}seq{max(c[0])}of{max(c[1])}h{c[2]}g{c[3]}p{c[4]}w{c[5]}")
+def test_attention_of_chains(c):
+    news, lens, H, HK, ps, window, sinks, by_head = c
+    B = Batch(11, news, lens, ps, HK, by_head)
+    q = rnd(B.g, sum(news), H, 128)
+    out = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, max_rows=max(news), max_keys=max(lens), window=window,
+                          sinks=sinks)
+    B.check(q, out, lambda b: chain_seen(news[b], lens[b], window, sinks))
+    # nothing but the tensors: the table's own limits size the launch
+    loose = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, window=window, sinks=sinks)
+    B.check(q, loose, lambda b: chain_seen(news[b], lens[b], window, sinks))
+
+
+TREES = [
+    ([5], [5], 4, 2, 16, 0, 0),             # a tree and nothing before it
+    ([26, 11, 1], [300, 47, 200], 8, 2, 16, 0, 0),
+    ([64], [1000], 8, 1, 32, 0, 0),
+    ([65, 30], [165, 63], 2, 1, 8, 0, 0),   # two words
+    ([200], [330], 2, 2, 64, 0, 0),         # four words
+    ([30, 8], [600, 100], 4, 1, 16, 50, 5),
+    ([40], [4500], 4, 2, 16, 0, 0),         # split
+]
+
+
+@pytest.mark.parametrize("c", TREES, ids=lambda c: f"{len(c[0])}seq{max(c[0])}of{max(c[1])}h{c[2]}g{c[3]}p{c[4]}w{c[5]}")
+def test_attention_of_trees(c):
+    news, lens, H, HK, ps, window, sinks = c
+    rng = random.Random(5)
+    trees = [random_tree(rng, n) for n in news]
+    B = Batch(12, news, lens, ps, HK)
+    q = rnd(B.g, sum(news), H, 128)
+    out = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, max_rows=max(news), tree=tree_words(trees, (max(news) + 63) // 64),
+                          window=window, sinks=sinks)
+    B.check(q, out, lambda b: tree_seen(trees[b], lens[b], window, sinks))
+
+
+def test_a_tree_of_one_branch_is_a_chain():
+    news, lens = [9, 70], [100, 70]
+    B = Batch(13, news, lens, 16, 2)
+    q = rnd(B.g, sum(news), 4, 128)
+    trees = [[set(range(i + 1)) for i in range(n)] for n in news]
+    a = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, tree=tree_words(trees, 2))
+    B.check(q, a, lambda b: chain_seen(news[b], lens[b]))
+
+
+def test_masks_that_leave_a_row_empty():
+    """A token whose mask has no bit, first with nothing before it (zeros), then behind a context."""
+    B = Batch(14, [3, 3], [3, 40], 16, 1)
+    q = rnd(B.g, 6, 2, 128)
+    trees = [[{0}, set(), {0, 2}], [set(), {1}, {1, 2}]]
+    out = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, tree=tree_words(trees, 1))
+    assert (out[1] == 0).all()
+    B.check(q, out, lambda b: tree_seen(trees[b], B.L[b]))
+
+
+@pytest.mark.parametrize("news,lens,tree", [([1, 1], [70, 3000], False), ([6, 20], [70, 333], True), ([90], [200], False)])
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_positions_that_are_not_seen_have_no_part(news, lens, tree, what):
+    """Pages' rows behind the sequences' ends, free pages, and drafted tokens of other branches hold NaN or infinities."""
+    B = Batch(15, news, lens, 16, 2)
+    used = torch.zeros(B.n_pages, 16, dtype=torch.bool, device="cuda")
+    for b, L in enumerate(lens):
+        at = torch.arange(L, device="cuda")
+        used[B.t[b][at // 16].long(), at % 16] = True
+    B.kp[~used] = what
+    B.vp[~used] = what
+    rng = random.Random(6)
+    trees = [random_tree(rng, n) for n in news]
+    if tree:   # a leaf that no one but itself sees
+        at = lens[1] - 1
+        B.kp[B.table[1][at // 16], at % 16, 0] = what
+        B.vp[B.table[1][at // 16], at % 16, 1] = what
+    q = rnd(B.g, sum(news), 4, 128)
+    kw = dict(tree=tree_words(trees, 1)) if tree else {}
+    out = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, **kw)
+    B.check(q, out, lambda b: tree_seen(trees[b], lens[b]) if tree else chain_seen(news[b], lens[b]))
+
+
+def test_pages_outside_the_pool_hold_nothing():
+    """Entries below and past the pool's pages: their positions are not seen; a sequence of nothing else gets zeros."""
+    news, lens = [1, 2, 1], [100, 60, 40]
+    for ps in (16, 64, 8):
+        B = Batch(16, news, lens, ps, 2)
+        table = [list(r) for r in B.table]
+        gone = [set(), set(), set()]
+        for b, e, value in ((0, 1, -1), (0, 0, B.n_pages), (1, 0, 1 << 30), (2, None, -7)):
+            for x in range(len(table[b])) if e is None else [min(e, -(-lens[b] // ps) - 1)]:
+                table[b][x] = value
+                gone[b] |= set(range(x * ps, (x + 1) * ps))
+        q = rnd(B.g, 4, 4, 128)
+        out = cache.attention(q, B.kp, B.vp, ints(table), B.starts, B.lens)
+
+        def seen(b):
+            s = chain_seen(news[b], lens[b])
+            s[:, [j for j in gone[b] if j < lens[b]]] = False
+            return s
+        B.check(q, out, seen)
+        assert (out[3] == 0).all()
+
+
+def test_rows_behind_the_last_sequence_stay():
+    """A padded batch: more rows than tokens, a table wider than the sequences, sequences longer than the launch was sized
+    for."""
+    news, lens = [2, 1], [50, 3000]
+    B = Batch(17, news, lens, 16, 1)
+    q = rnd(B.g, 7, 4, 128)
+    out = torch.full((9, 4, 128), 3.0, dtype=BF16, device="cuda")
+    cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, out, max_rows=2)
+    B.check(q, out, lambda b: chain_seen(news[b], lens[b]))
+    assert (out[3:] == 3.0).all()
+    # one token of the first sequence is beyond max_rows: its row stays as it was
+    out.fill_(3.0)
+    cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, out, max_rows=1)
+    assert (out[1] == 3.0).all() and (out[3:] == 3.0).all() and not (out[0] == 3.0).any() and not (out[2] == 3.0).any()
+    # positions beyond max_keys are not seen
+    short = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, max_rows=2, max_keys=1000)
+    k, v = B.rows(1)
+    check_rows(short[2:3], *ref_rows(q[2:3], k[:1000], v[:1000], torch.ones(1, 1000, dtype=torch.bool)))
+    # a length that the table does not hold
+    lens2 = B.lens.clone()
+    lens2[0] = 100000
+    cut = cache.attention(q, B.kp, B.vp, B.t[:, :4].contiguous(), B.starts, lens2, max_rows=2)
+    at = torch.arange(64, device="cuda")
+    tab = B.t[0][at // 16].long()
+    ok = tab >= 0
+    k, v = B.kp[tab.clamp(min=0), at % 16], B.vp[tab.clamp(min=0), at % 16]
+    check_rows(cut[:2], *ref_rows(q[:2], k, v, ok.cpu()[None].expand(2, 64)))
+
+
+def test_offsets_past_32_bits():
+    """A pool of more than 2^31 elements whose last pages are the ones in use."""
+    ps, HK = 64, 8
+    pages = (1 << 31) // (ps * HK * 128) + 40
+    kp, vp = (torch.zeros(pages, ps, HK, 128, dtype=BF16, device="cuda") for _ in range(2))
+    B = Batch(18, [1, 2], [500, 130], ps, HK)
+    shift = pages - B.n_pages
+    kp[shift:], vp[shift:] = B.kp, B.vp
+    t = torch.where(B.t >= 0, B.t + shift, B.t)
+    q = rnd(B.g, 3, 16, 128)
+    assert torch.equal(cache.attention(q, kp, vp, t, B.starts, B.lens), cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens))
+    k, v = rnd(B.g, 3, HK, 128), rnd(B.g, 3, HK, 128)
+    cache.append(None, k, v, kp, vp, t, B.starts, B.lens, table_kind=ops.TABLE_NONE)
+    cache.append(None, k, v, B.kp, B.vp, B.t, B.starts, B.lens, table_kind=ops.TABLE_NONE)
+    assert torch.equal(kp[shift:], B.kp) and torch.equal(vp[shift:], B.vp) and not kp[:4].any()
+    cache.copy_pages(kp, vp, ints([B.table[0][0] + shift]), ints([1]))
+    assert torch.equal(kp[1], B.kp[B.table[0][0]]) and torch.equal(vp[1], B.vp[B.table[0][0]])
+    del kp, vp
+    torch.cuda.empty_cache()
+
+
+def test_workspace_streams_and_graphs():
+    news, lens = [1, 1], [4000, 2500]
+    B = Batch(19, news, lens, 16, 2)
+    q = rnd(B.g, 2, 8, 128)
+    args = (q, B.kp, B.vp, B.t, B.starts, B.lens)
+    kw = dict(max_rows=1, max_keys=4000)
+    want = cache.attention(*args, **kw)
+    need = cache.attention_ws_bytes(2, 2, 1, 4000, 8, 2, 16)
+    assert need > 0
+    ws = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")
+    assert torch.equal(cache.attention(*args, workspace=ws, **kw), want) and (ws[need:] == 255).all()
+    with pytest.raises(ValueError):
+        cache.attention(*args, workspace=ws[:need - 256], **kw)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            a = cache.attention(*args, **kw)
+        b = cache.attention(*args, **kw)
+        torch.cuda.synchronize()
+        assert torch.equal(a, want) and torch.equal(b, want)
+    # a captured step follows tokens, lengths and tables at its replay
+    out = torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.attention(*args, out, **kw)
+    for i, new_lens in enumerate(([4000, 2500], [37, 2500], [1, 900])):
+        q.copy_(rnd(gen(60 + i), 2, 8, 128))
+        B.lens.copy_(ints(new_lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, cache.attention(*args, **kw))
+        B.L = new_lens
+        B.check(q, out, lambda b: chain_seen(1, new_lens[b]))
+
+
+def test_the_same_call_gives_the_same_bits():
+    B = Batch(20, [3, 1, 40], [2000, 700, 900], 16, 2)
+    q = rnd(B.g, 44, 8, 128)
+    a = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens)
+    assert all(torch.equal(a, cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens)) for _ in range(3))
+
+
+# ------------------------------------------------------------------------------------------------ append
+def tables(kind, rows, rot, g):
+    ang = torch.rand(rows, rot // 2, generator=g, device="cuda", dtype=torch.float64) * 6.3
+    c, s = ang.cos(), ang.sin()
+    if kind == ops.TABLE_COSSIN_F32:
+        c, s = c.float(), s.float()
+        return (c, s), torch.stack([c, -s, s, c], -1).double()
+    m = torch.stack([c, -s, s, c], -1).to(BF16 if kind == ops.TABLE_MAT2_BF16 else torch.float32)
+    return (m.reshape(rows, 2 * rot).contiguous(), None), m.double()
+
+
+def ref_norm_rope(x, w, mat, rot, pairing, eps):
+    """(y, size) in fp64: the value and the size of what it is a sum of; mat [T, rot / 2, 4] or None."""
+    x = x.double()
+    y = x / ((x * x).mean(-1, keepdim=True) + eps).sqrt()
+    if w is not None:
+        y = y * w.double()
+    size = y.abs()
+    if mat is not None:
+        a_at = torch.arange(0, rot, 2) if pairing == ops.PAIR_INTERLEAVED else torch.arange(rot // 2)
+        b_at = a_at + (1 if pairing == ops.PAIR_INTERLEAVED else rot // 2)
+        f = mat[:, None]
+        a, b = y[..., a_at].clone(), y[..., b_at].clone()
+        y[..., a_at], y[..., b_at] = f[..., 0] * a + f[..., 1] * b, f[..., 2] * a + f[..., 3] * b
+        size[..., a_at] = size[..., b_at] = a.abs() + b.abs()
+    return y, size
+
+
+def close_rope(got, y, size, what):
+    # one rounding to bf16, and fp32 steps before it: the sum of 128 squares, the root and three products and sums, below
+    # 2^-17 of the values that are added
+    over = (got.double() - y).abs() > HALF * y.abs() + 2.0 ** -16 * size + 1e-30
+    assert not over.any(), f"{what}: {int(over.sum())} values off"
+
+
+APPENDS = [   # tokens, lengths, heads, kv heads, page size, table kind, pairing, rot, weights, by_head
+    ([1], [1], 1, 1, 16, ops.TABLE_COSSIN_F32, ops.PAIR_INTERLEAVED, 128, True, False),
+    ([1] * 32, [7 + 11 * i for i in range(32)], 32, 8, 16, ops.TABLE_COSSIN_F32, ops.PAIR_INTERLEAVED, 128, True, False),
+    ([5, 0, 0, 77, 1], [9, 3, 0, 300, 65], 7, 1, 64, ops.TABLE_COSSIN_F32, ops.PAIR_SPLIT_HALF, 96, False, True),
+    ([130, 3], [130, 4], 6, 3, 1, ops.TABLE_MAT2_BF16, ops.PAIR_SPLIT_HALF, 128, True, False),
+    ([40], [45], 5, 5, 8, ops.TABLE_MAT2_F32, ops.PAIR_INTERLEAVED, 64, True, False),
+    ([33, 2], [40, 90], 4, 2, 32, ops.TABLE_NONE, ops.PAIR_INTERLEAVED, 128, True, True),
+    ([i % 4 for i in range(300)], [5 + i for i in range(300)], 2, 1, 16, ops.TABLE_COSSIN_F32, ops.PAIR_INTERLEAVED, 32, True,
+     False),
+]
+
+
+@pytest.mark.parametrize("c", APPENDS, ids=lambda c: f"{len(c[0])}seq{sum(c[0])}h{c[2]}g{c[3]}p{c[4]}k{c[5]}r{c[7]}")
+def test_append(c):
+    news, lens, H, HK, ps, kind, pairing, rot, weights, by_head = c
+    B = Batch(21, news, lens, ps, HK, by_head)
+    T = sum(news)
+    qkv = rnd(B.g, T, H + 2 * HK, 128)
+    q, k, v = qkv[:, :H], qkv[:, H:H + HK], qkv[:, H + HK:]
+    wq, wk = ((torch.rand(128, generator=B.g, device="cuda") + 0.5 for _ in range(2)) if weights else (None, None))
+    table, mat = tables(kind, max(lens), rot, B.g) if kind else (None, None)
+    tok_b = [b for b, n in enumerate(news) for _ in range(n)]
+    slots = torch.tensor([lens[b] - n + i for b, n in enumerate(news) for i in range(n)], device="cuda")
+    page = B.t[torch.tensor(tok_b, device="cuda"), slots // ps].long()
+    want_k, want_v = B.kp.clone(), B.vp.clone()
+    kw = dict(q_norm=wq, k_norm=wk, table_kind=kind, table=table, pairing=pairing, rot=rot, eps=1e-5)
+    before_k, before_v = B.kp.clone(), B.vp.clone()
+    q_out = cache.append(q, k, v, B.kp, B.vp, B.t, B.starts, B.lens, **kw)
+    rows = mat[slots] if kind else None
+    close_rope(q_out, *ref_norm_rope(q, wq, rows, rot, pairing, 1e-5), "queries")
+    close_rope(B.kp[page, slots % ps], *ref_norm_rope(k, wk, rows, rot, pairing, 1e-5), "keys")
+    assert torch.equal(B.vp[page, slots % ps], v)
+    want_k[page, slots % ps], want_v[page, slots % ps] = B.kp[page, slots % ps], v
+    assert torch.equal(B.kp, want_k) and torch.equal(B.vp, want_v)      # nothing else was written
+    # keys and values alone, and the queries in place
+    k2, v2 = before_k.clone(memory_format=torch.preserve_format), before_v.clone(memory_format=torch.preserve_format)
+    assert cache.append(None, k, v, k2, v2, B.t, B.starts, B.lens, **kw) is None
+    assert torch.equal(k2, B.kp) and torch.equal(v2, B.vp)
+    keep = qkv[:, H:].clone()
+    cache.append(q, k, v, B.kp, B.vp, B.t, B.starts, B.lens, q, **kw)
+    assert torch.equal(q, q_out) and torch.equal(qkv[:, H:], keep) and torch.equal(B.kp, want_k)
+
+
+def test_append_queries_are_joint_q_prepares():
+    """The same arithmetic as the fused op's query launch, bit for bit."""
+    B = Batch(22, [50], [50], 16, 2)
+    q, k = rnd(B.g, 50, 4, 128), rnd(B.g, 50, 2, 128)
+    w = torch.rand(128, generator=B.g, device="cuda")
+    cos, sin = (torch.from_numpy(x).cuda() for x in rope.grid2d_table(10, 5, 8))
+    a = cache.append(q, k, k, B.kp, B.vp, B.t, B.starts, B.lens, q_norm=w, k_norm=w, table=(cos, sin))
+    assert torch.equal(a, ops.joint_q_prepare(q, q_norm=w, q_table=(cos, sin)))
+    assert torch.equal(B.rows(0)[0], ops.joint_q_prepare(k, q_norm=w, q_table=(cos, sin)))
+
+
+def test_append_leaves_out_what_has_no_place():
+    """Tokens whose position, page or table row does not exist, and rows behind the last sequence."""
+    news, lens = [3, 2, 2], [20, 18, 5]
+    B = Batch(23, news, lens, 8, 1)
+    table = [list(r) for r in B.table]
+    table[0][2] = B.n_pages                      # positions 16 .. of sequence 0: tokens 17, 18, 19
+    q, k = rnd(B.g, 9, 2, 128), rnd(B.g, 9, 1, 128)
+    tab, _ = tables(ops.TABLE_COSSIN_F32, 17, 128, B.g)        # sequence 1's last token (position 17) has no row
+    before_k, before_v = B.kp.clone(), B.vp.clone()
+    out = torch.full((9, 2, 128), 4.0, dtype=BF16, device="cuda")
+    cache.append(q, k, k, B.kp, B.vp, ints(table), B.starts, B.lens, out, table=tab)
+    done = [(3, 1, 16), (5, 2, 3), (6, 2, 4)]    # token, sequence, position
+    for t in range(9):
+        assert (out[t] == 4.0).all() == (t not in [d[0] for d in done])
+    for t, b, p in done:
+        assert torch.equal(B.vp[table[b][p // 8], p % 8], k[t])
+        before_k[table[b][p // 8], p % 8] = B.kp[table[b][p // 8], p % 8]
+        before_v[table[b][p // 8], p % 8] = k[t]
+    assert torch.equal(B.kp, before_k) and torch.equal(B.vp, before_v)
+    # explicit positions choose the table row; those outside the table leave the token out
+    pos = ints([0, 0, 0, 5, 16, 17, -1, 3, 3])
+    out.fill_(4.0)
+    cache.append(q, k, k, B.kp, B.vp, B.t, B.starts, B.lens, out, table=tab, positions=pos)
+    assert (out[5:] == 4.0).all() and not (out[:5] == 4.0).all(-1).any()
+    same = cache.append(q[3:5], k[3:5], k[3:5], B.kp, B.vp, B.t[2:], ints([0, 2]), B.lens[2:],
+                        table=(tab[0][[5, 16]].contiguous(), tab[1][[5, 16]].contiguous()), positions=ints([0, 1]))
+    assert torch.equal(out[3:5], same)
+
+
+# ------------------------------------------------------------------------------------------------ copies and moves
+@pytest.mark.parametrize("ps,HK,by_head,layers", [(16, 8, False, 3), (1, 1, False, None), (64, 3, True, 2), (128, 5, False, 1),
+                                                  (8, 7, True, None)])
+def test_copy_pages(ps, HK, by_head, layers):
+    g = gen(30)
+    kp, vp = make_pool(g, 12, ps, HK, by_head, layers)
+    src, dst = [3, 3, 0, 11, -1, 5, 12, 7], [1, 2, 9, 4, 6, 12, 8, 7]
+    wk, wv = kp.clone(), vp.clone()
+    for a, b in zip(src, dst):
+        if 0 <= a < 12 and 0 <= b < 12:
+            wk[..., b, :, :, :], wv[..., b, :, :, :] = kp[..., a, :, :, :], vp[..., a, :, :, :]
+    cache.copy_pages(kp, vp, ints(src), ints(dst))
+    assert torch.equal(kp, wk) and torch.equal(vp, wv)
+    cache.copy_pages(kp, vp, ints([]), ints([]))
+    with pytest.raises(ValueError):
+        cache.copy_pages(kp, vp, ints([1]), ints([1, 2]))
+
+
+@pytest.mark.parametrize("ps,HK,by_head,layers,counts", [
+    (16, 8, False, 3, [5, 0, 1]), (1, 2, False, 1, [30, 2, 7]), (64, 3, True, 2, [256, 1, 9]), (8, 40, False, None, [100, 3, 3])])
+def test_move_rows(ps, HK, by_head, layers, counts):
+    """Chains, swaps and gathers inside sequences: every row is read before any is written."""
+    lens = [300, 40, 90]
+    g, rng = gen(31), random.Random(8)
+    need = [-(-x // ps) for x in lens]
+    ids = list(range(sum(need) + 2))
+    rng.shuffle(ids)
+    table = [[ids.pop() for _ in range(n)] + [-1] * (max(need) - n) for n in need]
+    kp, vp = make_pool(g, sum(need) + 2, ps, HK, by_head, layers)
+    src, dst, st = [], [], [0]
+    for L, n in zip(lens, counts):
+        to = rng.sample(range(L), n)                       # distinct targets, sources as they come: chains, swaps, repeats
+        src += [rng.choice(to) if rng.random() < 0.5 else rng.randrange(L) for _ in range(n)]
+        dst += to
+        st.append(st[-1] + n)
+    if counts[2] >= 3:                                     # places that do not exist: left out
+        src[-1], dst[-2], src[-3] = -1, lens[2] + 1000, 1 << 30
+    wk, wv = kp.clone(), vp.clone()
+    for b in range(3):
+        for a, c in zip(src[st[b]:st[b + 1]], dst[st[b]:st[b + 1]]):
+            if 0 <= a < lens[b] and 0 <= c < lens[b]:
+                (pa, ra), (pc, rc) = divmod(a, ps), divmod(c, ps)
+                wk[..., table[b][pc], rc, :, :] = kp[..., table[b][pa], ra, :, :]
+                wv[..., table[b][pc], rc, :, :] = vp[..., table[b][pa], ra, :, :]
+    cache.move_rows(kp, vp, ints(table), ints(st), ints(src), ints(dst), max_rows=max(counts))
+    assert torch.equal(kp, wk) and torch.equal(vp, wv)
+
+
+def test_refusals_before_launch():
+    B = Batch(32, [1], [20], 16, 2)
+    q = rnd(B.g, 1, 4, 128)
+    ok = (q, B.kp, B.vp, B.t, B.starts, B.lens)
+    with pytest.raises(_lib.LrError):
+        cache.attention(*ok, q)                                        # in place
+    with pytest.raises(_lib.LrError):
+        cache.attention(*ok, scale=-1.0)
+    with pytest.raises(ValueError):
+        cache.attention(q, B.kp, B.vp[:1], *ok[3:])
+    with pytest.raises(ValueError):
+        cache.attention(q, B.kp, B.vp.transpose(1, 2).contiguous().transpose(1, 2), *ok[3:])   # other strides
+    with pytest.raises(ValueError):
+        cache.attention(q, B.kp.float(), B.vp.float(), *ok[3:])
+    with pytest.raises(ValueError):
+        cache.attention(q, B.kp, B.vp, B.t.long(), B.starts, B.lens)
+    with pytest.raises(ValueError):
+        cache.attention(q, B.kp, B.vp, B.t, B.starts.cpu(), B.lens)
+    with pytest.raises(ValueError):
+        cache.attention(*ok, tree=torch.zeros(1, dtype=torch.int64, device="cuda"))
+    with pytest.raises(_lib.LrError):
+        cache.append(q[:, :2], B.kp[0, :1], B.vp[0, :1], *ok[1:], table_kind=ops.TABLE_NONE)    # k inside the pool
+    with pytest.raises(ValueError):
+        cache.append(q, q, q, *ok[1:], table_kind=ops.TABLE_NONE)      # four key heads over a pool of two
+    odd = rnd(B.g, 3, 12, 2, 128)
+    with pytest.raises(_lib.LrError):
+        cache.attention(q, odd, odd.clone(), *ok[3:])                  # pages of 12 rows
+    with pytest.raises(_lib.LrError):
+        cache.move_rows(B.kp, B.vp, B.t, ints([0, 300]), ints([0] * 300), ints([0] * 300))
+
+
+# ------------------------------------------------------------------------------------------------ together
+def test_a_serving_loop():
+    """Two layers of one model: prompts appended and attended, one request forked (its shared last page copied), drafted trees
+    appended, attended and the accepted branch moved behind the context, then single tokens, in a window of 60 at the end;
+    every attention against rows kept aside."""
+    L, H, HK, ps, window, sinks = 2, 4, 2, 8, 60, 3
+    g, rng = gen(40), random.Random(9)
+    pool = cache.PagePool(64)
+    kp, vp = make_pool(g, 64, ps, HK, layers=L)
+    (cos, sin), _ = tables(ops.TABLE_COSSIN_F32, 256, 128, g)
+    w = torch.rand(128, generator=g, device="cuda") + 0.5
+    keys = [[] for _ in range(L)]                     # per layer, per sequence: (k, v) rows as written
+    pages, lens = [], []
+
+    def grow(b, n):
+        while len(pages[b]) * ps < lens[b] + n:
+            pages[b] += pool.alloc(1)
+        lens[b] += n
+
+    def args():
+        width = max(map(len, pages))
+        return ints([p + [-1] * (width - len(p)) for p in pages])
+
+    def step(news, trees=None, window=0):
+        """One forward of news[b] tokens each: append and attention in every layer, checked."""
+        for b, n in enumerate(news):
+            grow(b, n)
+        st = [0]
+        for n in news:
+            st.append(st[-1] + n)
+        t, starts, ln = args(), ints(st), ints(lens)
+        ctx = [x - n for x, n in zip(lens, news)]
+        depth = [ctx[b] + (len(trees[b][i]) - 1 if trees else i) for b, n in enumerate(news) for i in range(n)]
+        for layer in range(L):
+            qkv = rnd(g, st[-1], H + 2 * HK, 128)
+            q = cache.append(qkv[:, :H], qkv[:, H:H + HK], qkv[:, H + HK:], kp[layer], vp[layer], t, starts, ln, q_norm=w,
+                             k_norm=w, table=(cos, sin), positions=ints(depth))
+            kk = ops.joint_q_prepare(qkv[:, H:H + HK], q_norm=w, q_table=(cos[depth].contiguous(), sin[depth].contiguous()))
+            out = cache.attention(q, kp[layer], vp[layer], t, starts, ln, max_rows=max(news), max_keys=max(lens),
+                                  tree=tree_words(trees, 1) if trees else None, window=window, sinks=sinks if window else 0)
+            for b, n in enumerate(news):
+                s = slice(st[b], st[b + 1])
+                old = keys[layer][b] if b < len(keys[layer]) else (kk[:0], kk[:0])
+                k2, v2 = torch.cat([old[0], kk[s]]), torch.cat([old[1], qkv[s, H + HK:]])
+                seen = tree_seen(trees[b], lens[b], window, sinks) if trees else chain_seen(n, lens[b], window, sinks)
+                check_rows(out[s], *ref_rows(q[s], k2, v2, seen), what=f"layer {layer} sequence {b}")
+                if b < len(keys[layer]):
+                    keys[layer][b] = (k2, v2)
+                else:
+                    keys[layer].append((k2, v2))
+
+    pages += [[], []]
+    lens += [0, 0]
+    step([37, 70])
+    # fork the first request: shared pages, its partly filled last page copied for the new one
+    pages.append(pool.fork(pages[0]))
+    lens.append(lens[0])
+    src, dst = pool.own(pages[2], len(pages[2]) - 1)
+    cache.copy_pages(kp, vp, ints([src]), ints([dst]))
+    for layer in range(L):
+        keys[layer].append(keys[layer][0])
+    step([1, 1, 1])
+    for _ in range(2):
+        trees = [random_tree(rng, n) for n in (9, 14, 5)]
+        before = list(lens)
+        step([9, 14, 5], trees)
+        paths = [sorted(rng.choice(t)) for t in trees]      # an accepted branch: a token's ancestors and itself
+        moves = [(before[b] + x, before[b] + i) for b, p in enumerate(paths) for i, x in enumerate(p)]
+        st = [0]
+        for p in paths:
+            st.append(st[-1] + len(p))
+        cache.move_rows(kp, vp, args(), ints(st), ints([m[0] for m in moves]), ints([m[1] for m in moves]))
+        for b, p in enumerate(paths):
+            lens[b] = before[b] + len(p)
+            at = torch.tensor(list(range(before[b])) + [before[b] + x for x in p], device="cuda")
+            for layer in range(L):
+                keys[layer][b] = tuple(x[at] for x in keys[layer][b])
+            drop = len(pages[b]) - -(-lens[b] // ps)         # pages behind the accepted tokens
+            if drop:
+                pool.free(pages[b][-drop:])
+                del pages[b][-drop:]
+        step([1, 1, 1])
+    # the second request ends; the pool is compacted
+    pool.free(pages[1])
+    gone = 1
+    del pages[gone], lens[gone]
+    for layer in range(L):
+        del keys[layer][gone]
+    a, b = pool.compact(pages)
+    assert a
+    cache.copy_pages(kp, vp, ints(a), ints(b))
+    step([1, 1], window=window)
+    step([3, 2], window=window)
