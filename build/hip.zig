@@ -25,6 +25,7 @@ const sources = [_]Source{
     .{ .file = "lr_abi.hip" },
     .{ .file = "mmdit.hip" },
     .{ .file = "attn_cache.hip" },
+    .{ .file = "attn_cache_wide.hip", .extra = &.{ "-mllvm", "-pragma-unroll-threshold=1000000" } },
     .{ .file = "cache_rows.hip" },
     .{ .file = "cache_abi.hip" },
 };

@@ -22,68 +22,7 @@ namespace {
 
 #include "attn_common.inc"
 
-// What a token of a sequence sees.
-struct Sees {
-    int lo, hi;   // keys lo <= j < hi, and j < min(sinks, lo)
-};
-
-// One sequence of a call as a workgroup needs it.
-struct Seq {
-    int t0, n;        // first token, tokens
-    int p0;           // position of the first token (the first drafted key under a tree)
-    int end;          // keys that exist
-};
-
-template <bool PAGED>
-__device__ __forceinline__ Seq seq_of(const RangeAttnArgs& a, int b) {
-    Seq s;
-    if constexpr (PAGED) {
-        const int s0 = a.starts[b], s1 = a.starts[b + 1], len = a.lens[b];
-        s.t0 = max(0, s0);
-        s.n = min(min(s1, a.T) - s.t0, a.max_rows);
-        // a first token that the call does not have, or more keys than an int's tokens: nothing is done for it
-        if (s0 < 0 || len < 0) s.n = 0;
-        s.p0 = len - (s1 - s0);
-        const int64_t cap = (int64_t)a.pg.table_pages << a.pg.shift;
-        s.end = (int)min((int64_t)min(len, a.max_keys), cap);
-    } else {
-        s.t0 = 0;
-        s.n = a.W;
-        s.p0 = a.p0;
-        s.end = a.nkeys;
-    }
-    return s;
-}
-
-template <bool PAGED>
-__device__ __forceinline__ Sees sees_of(const RangeAttnArgs& a, const Seq& s, int i) {
-    Sees r;
-    if constexpr (PAGED) {
-        int p = s.p0 + i;
-        r.hi = min(s.end, p + 1);
-        if (a.tree) {
-            int bits = 0;
-            for (int w = 0; w < a.words; ++w) bits += __popcll(a.tree[(int64_t)(s.t0 + i) * a.words + w]);
-            p = s.p0 + bits - 1;
-            r.hi = s.end;
-        }
-        r.lo = a.window ? max(0, p - a.window + 1) : 0;
-    } else {
-        const int f = (s.p0 + i) / a.frame;
-        r.hi = (int)min((int64_t)s.end, ((int64_t)f + 1) * a.frame);
-        r.lo = (int)max((int64_t)0, ((int64_t)f - a.window + 1) * a.frame);
-    }
-    r.hi = max(r.hi, 0);
-    r.lo = min(r.lo, r.hi);
-    return r;
-}
-
-__device__ __forceinline__ int wave_max_i(int x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x = max(x, __shfl_xor(x, d, 64));
-    return x;
-}
-__device__ __forceinline__ int wave_min_i(int x) { return -wave_max_i(-x); }
+#include "range_attn.inc"
 
 template <int RB, int KG, int NS, bool PAGED>
 __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(RangeAttnArgs a) {
@@ -110,19 +49,9 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     const int64_t rows = (int64_t)max(sq.n, 0) * a.G;
     if (row0 >= rows) return;
     const int i_first = row0 / a.G, i_last = (int)min((int64_t)sq.n - 1, ((int64_t)row0 + 32 * RB - 1) / a.G);
-    int lo_min, hi_max;
-    if (PAGED && a.tree) {
-        lo_min = a.window ? max(0, min(sq.p0 - a.window, sq.end)) : 0;
-        hi_max = max(sq.end, 0);
-    } else {
-        lo_min = sees_of<PAGED>(a, sq, i_first).lo;
-        hi_max = sees_of<PAGED>(a, sq, i_last).hi;
-    }
-    const int st = (min(a.sinks, lo_min) + BT - 1) / BT;            // tiles of first tokens
-    const int lt = max(st, lo_min / BT), ht = (hi_max + BT - 1) / BT;
-    const int total = st + max(0, ht - lt);
-    const int x0 = split * a.tiles_per_split, x1 = min(total, x0 + a.tiles_per_split);
-    auto key0_of = [&](int x) { return BT * (x < st ? x : lt + x - st); };
+    TileList<BT, PAGED> tl;
+    tl.init(a, sq, i_first, i_last, split);
+    const int x0 = tl.x0, x1 = tl.x1;
 
     // ---- this lane's row
     const int wr0 = row0 + 32 * rb, r = wr0 + n;
@@ -135,33 +64,7 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
 
     const int64_t k_rs = PAGED ? a.pg.rs : a.k_rs, v_rs = PAGED ? a.pg.rs : a.v_rs;
     const int64_t hoff = (int64_t)hk * (PAGED ? a.pg.hs : D);
-    const int shift = PAGED ? a.pg.shift : 0;
-    const int per_tile = PAGED ? max(1, BT >> shift) : 1;
-    bool bad = false;
-    if constexpr (PAGED) {
-        const int cnt = max(0, x1 - x0) * per_tile;
-        for (int e = tid; e < cnt; e += NW * 64) {
-            const int j = key0_of(x0 + e / per_tile) + (e % per_tile << shift);
-            int page = -1;
-            if (j < sq.end) {
-                page = a.pg.table[(int64_t)b * a.pg.table_rs + (j >> shift)];
-                if (page < 0 || page >= a.pg.n_pages) page = -1;
-                bad |= page < 0;
-            }
-            staged[e] = page;
-        }
-        bad = __syncthreads_or(bad);
-    }
-    // row `row` of tile x: its key clamped to the last that exists, and its offset in elements from the head's first
-    auto entry = [&](int x, int row) { return PAGED ? staged[(x - x0) * per_tile + (per_tile > 1 ? row >> shift : 0)] : 0; };
-    auto offset = [&](int x, int row, int64_t rs) -> int64_t {
-        const int key0 = key0_of(x);
-        const int j = min(key0 + row, sq.end - 1);
-        if constexpr (PAGED)
-            return (int64_t)max(entry(x, j - key0), 0) * a.pg.ps + (int64_t)(j & ((1 << shift) - 1)) * rs;
-        else
-            return (int64_t)j * rs;
-    };
+    const bool bad = tl.template stage<NW * 64>(a, b, staged);
 
     // ---- direct loads of a tile: instruction u fills rows 4u .. 4u + 3, swizzled as attn_fwd.hip's
     const int lrow = lane >> 4, lchunk = lane & 15;
@@ -170,9 +73,9 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
             const int inst = rb + RB * u, row = 4 * inst + lrow;
-            const int64_t o = offset(x, row, k_rs);
+            const int64_t o = tl.offset(a, x, row, k_rs);
             dma16(a.k + hoff + o + 8 * (lchunk ^ (row & 15)), kr_lds + 2 * (slot * TILE + 512 * inst));
-            const int64_t ov = PAGED ? o : offset(x, row, v_rs);
+            const int64_t ov = PAGED ? o : tl.offset(a, x, row, v_rs);
             dma16(a.v + hoff + ov + 8 * (lchunk ^ (lrow << 2)), vr_lds + 2 * (slot * TILE + 512 * inst));
         }
     };
@@ -205,20 +108,6 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
         vtr[db] = (8 * (g >> 1) + (sl >> 2)) * D + 8 * chunk + 4 * (sl & 1);
     }
 
-    // whether this lane's row sees key j = key0 + row of tile x
-    auto sees = [&](int x, int key0, int row) {
-        const int j = key0 + row;
-        bool ok = j < me.hi && (j >= me.lo || j < a.sinks);
-        if constexpr (PAGED) {
-            if (a.tree && j >= sq.p0) {
-                const int d = j - sq.p0;
-                ok = j < sq.end && (d >> 6) < a.words && (a.tree[(int64_t)(sq.t0 + i) * a.words + (d >> 6)] >> (d & 63) & 1);
-            }
-            if (bad && ok) ok = entry(x, row) >= 0;
-        }
-        return ok;
-    };
-
     f32x16 o[4];
 #pragma unroll
     for (int db = 0; db < 4; ++db) o[db] = f32x16{};
@@ -238,7 +127,7 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
             if (t + NS - 1 < mine) load_tile(tile_of(t + NS - 1), (t + NS - 1) % NS);
         }
         if (have && any) {
-            const int x = tile_of(t), key0 = key0_of(x);
+            const int x = tile_of(t), key0 = tl.key0(x);
             const uint16_t* kt = reinterpret_cast<const uint16_t*>(ring) + kg * NS * TILE * 2 + (t % NS) * TILE;
             const uint16_t* vt = kt + NS * TILE;
             f32x16 s{};
@@ -249,11 +138,10 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
             }
             const bool whole = key0 + BT <= hi_all && (key0 >= lo_all || key0 + BT <= a.sinks) && !bad;
             if (!whole) {
+                const uint32_t m = seen_bits<BT, PAGED>(a, sq, tl, bad, i, me, x, 0) >> (8 * hf);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int row = 16 * (e >> 3) + 8 * hf + (e & 7);
-                    if (!sees(x, key0, row)) s[e] = -INFINITY;
-                }
+                for (int e = 0; e < 16; ++e)
+                    if (!(m >> (16 * (e >> 3) + (e & 7)) & 1)) s[e] = -INFINITY;
             }
             float mx = s[0];
 #pragma unroll
@@ -356,7 +244,7 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     const bool broken = live && !(fabsf(chk) < INFINITY);
     if (live) {
         if (a.nsplit > 1) {
-            const int64_t slot = ((int64_t)(sq.t0 + i) * a.H + head) * a.nsplit + split;
+            const int64_t slot = part_slot(a, sq, i, head, split);
             float* po = a.part_o + slot * D + 4 * hf;
             if (m_used > -INFINITY) {
 #pragma unroll
@@ -385,78 +273,13 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
         }
     }
 
-    // ---- rows with an infinity or NaN: zero times it may have come from a key that the row does not see (0 * NaN in the
-    // products). Those rows again, key by key over the seen ones only: lane = key for the scores, lane = two dims for the sum.
+    // rows with an infinity or NaN again, over the seen keys only
     uint64_t again = __builtin_amdgcn_ballot_w64(broken);
     again = (again | again >> 32) & 0xffffffffu;
     while (again) {
         const int src = __builtin_ctzll(again);
         again &= again - 1;
-        const int ri = __shfl(i, src, 64), rhead = __shfl(head, src, 64);
-        const uint16_t* qrow = a.q + (int64_t)(sq.t0 + ri) * a.q_rs + rhead * D;
-        float m = -INFINITY, ls = 0.0f, o0 = 0.0f, o1 = 0.0f;
-        const Sees rs_ = sees_of<PAGED>(a, sq, ri);
-        for (int x = x0; x < x1; ++x) {
-            const int key0 = key0_of(x), j = key0 + n;
-            bool ok = j < rs_.hi && (j >= rs_.lo || j < a.sinks);
-            if constexpr (PAGED) {
-                if (a.tree && j >= sq.p0) {
-                    const int d = j - sq.p0;
-                    ok = j < sq.end && (d >> 6) < a.words &&
-                         (a.tree[(int64_t)(sq.t0 + ri) * a.words + (d >> 6)] >> (d & 63) & 1);
-                }
-                if (ok) ok = entry(x, n) >= 0;
-            }
-            ok = ok && hf == 0;
-            float s = -INFINITY;
-            if (ok) {
-                const uint16_t* kr = a.k + hoff + offset(x, n, k_rs);
-                s = 0.0f;
-                for (int d = 0; d < D; d += 8) {
-                    const u32x4 kw = *reinterpret_cast<const u32x4*>(kr + d), qw = *reinterpret_cast<const u32x4*>(qrow + d);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s = fmaf(lo_bf16(kw[e]), lo_bf16(qw[e]), s);
-                        s = fmaf(hi_bf16(kw[e]), hi_bf16(qw[e]), s);
-                    }
-                }
-                s *= c;
-            }
-            float mx = s;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
-            const float mn = fmaxf(m, mx), ref = mn > -INFINITY ? mn : 0.0f;
-            const float alpha = m > -INFINITY ? __builtin_amdgcn_exp2f(m - ref) : 1.0f;
-            m = mn;
-            const float p = ok ? __builtin_amdgcn_exp2f(s - ref) : 0.0f;
-            ls = ls * alpha + p;   // (per lane: summed at the end)
-            o0 *= alpha;
-            o1 *= alpha;
-            uint64_t seen = __builtin_amdgcn_ballot_w64(ok);
-            while (seen) {
-                const int kk = __builtin_ctzll(seen);
-                seen &= seen - 1;
-                const float pk = __shfl(p, kk, 64);
-                const uint32_t vw = *reinterpret_cast<const uint32_t*>(a.v + hoff + offset(x, kk, v_rs) + 2 * lane);
-                o0 = fmaf(pk, lo_bf16(vw), o0);
-                o1 = fmaf(pk, hi_bf16(vw), o1);
-            }
-        }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) ls += __shfl_xor(ls, d, 64);
-        if (a.nsplit > 1) {
-            const int64_t slot = ((int64_t)(sq.t0 + ri) * a.H + rhead) * a.nsplit + split;
-            *reinterpret_cast<float2*>(a.part_o + slot * D + 2 * lane) = float2{o0, o1};
-            if (lane == 0) {
-                // (a range whose sum is NaN counts whatever its reference)
-                a.part_ml[2 * slot] = m > -INFINITY || ls == 0.0f ? m : 0.0f;
-                a.part_ml[2 * slot + 1] = ls;
-            }
-        } else {
-            const float inv = ls != 0.0f ? 1.0f / ls : 0.0f;
-            *reinterpret_cast<uint32_t*>(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D + 2 * lane) =
-                pack_bf16x2(o0 * inv, o1 * inv);
-        }
+        redo_row<BT, PAGED>(a, sq, tl, hk, split, __shfl(i, src, 64), __shfl(head, src, 64));
     }
 }
 
@@ -505,10 +328,11 @@ hipError_t launch_blocks(const RangeAttnArgs& a, bool paged, hipStream_t stream)
 
 }  // namespace
 
-hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, hipStream_t stream) {
+hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, bool wide, hipStream_t stream) {
     const int64_t rows = (int64_t)(paged ? a.max_rows : a.W) * a.G;
     hipError_t e;
-    if (rows <= 32) e = launch_blocks<1, 4, 2>(a, paged, stream);
+    if (wide) e = launch_range_wide(a, paged, stream);
+    else if (rows <= 32) e = launch_blocks<1, 4, 2>(a, paged, stream);
     else if (rows <= 64) e = launch_blocks<2, 2, 4>(a, paged, stream);
     else e = launch_blocks<4, 2, 4>(a, paged, stream);
     if (e != hipSuccess || a.nsplit <= 1) return e;

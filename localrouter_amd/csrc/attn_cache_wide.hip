@@ -1,0 +1,419 @@
+// The ranged attention (attn_cache.hip) of calls with many rows of a kv head: chunks, frames and large trees, where the matrix
+// products bound it. The same contract; the loop is that of the key-split kernel (attn_keysplit.hip): a half-step of 16 MFMA
+// slots runs the next half-tile's scores, the previous one's products and this one's exponentials. A workgroup is 128 rows
+// (tokens x the query heads of one kv head), four waves of 32 rows over a ring of two key tiles and two value tiles; two
+// workgroups share a CU, one's start, end and waits under the other's products. What differs from there:
+//
+//  * The tiles are a list (the first tokens' tiles, then the rows' own range), and a half-tile that some row of the wave does
+//    not see whole takes a masked step: its 32 keys' visibility as one word a row, built from the row's limits (and its tree
+//    bits), two instructions a score to apply.
+//  * A row's softmax reference is the maximum of the first half-tile in which it sees a key, which a window's list does not
+//    put first for every row: until each row of the wave has one, half-tiles take the masked step, which also sets references.
+//  * Pages hold at least 16 rows, so the 16 rows of a value load are in one page, and the 32 rows of a key load in at most
+//    two: scalar bases from the staged page-table entries.
+//  * A row that overflowed its reference, or met an infinity or NaN, is computed again over the keys that it sees.
+#include "lr_common.h"
+#include "lr_cache_kernels.h"
+#include "tile_image.h"
+
+namespace lr {
+
+namespace {
+
+#include "attn_common.inc"
+
+constexpr int RA = 3;             // fragments read ahead
+constexpr int FR = 4;             // fragment ring entries
+constexpr int QW = 4;             // waves (of 32 rows)
+constexpr int KBM = 32 * QW;      // rows per block
+constexpr int RING_LDS = 4 * IMG_TILE_BYTES;   // two key tiles, two value tiles
+static_assert(2 * (RING_LDS + 4 * RANGE_WIDE_STAGED + 256) <= 160 * 1024, "two workgroups a CU");
+static_assert(KBM == RANGE_WIDE_ROWS && IMG_TILE_KEYS == RANGE_WIDE_TILE, "the host's cut");
+
+#include "attn_tiles.inc"
+#include "range_attn.inc"
+
+// One 1 KB direct load, global -> LDS: lane l's 16 bytes come from gaddr + voff and land at lds + 16 l.
+__device__ __forceinline__ void dma1(uint64_t gaddr, uint32_t voff, uint32_t lds) {
+    LR_ASM_M0_BEGIN
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(gaddr), "s"(lds)
+                 : "memory", "m0");
+    LR_ASM_M0_END
+}
+// The same from a lane's own address + OFF, to lds + 16 l (the instruction offset applies to both addresses).
+template <int OFF>
+__device__ __forceinline__ void dma1_far(uint64_t addr, uint32_t lds) {
+    LR_ASM_M0_BEGIN
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2" ::"v"(addr), "s"(lds - OFF), "n"(OFF)
+                 : "memory", "m0");
+    LR_ASM_M0_END
+}
+
+// The sequence of rank `rank` when the batch is ordered longest first (B <= 64), so that the last workgroups to start are
+// short ones.
+__device__ __forceinline__ int seq_by_length(const RangeAttnArgs& a, int rank) {
+    const int lane = threadIdx.x & 63;
+    const int len = lane < a.B ? a.lens[lane] : INT32_MIN;
+    int before = 0;
+    for (int j = 0; j < a.B; ++j) {
+        const int other = __builtin_amdgcn_readlane(len, j);
+        before += other > len || (other == len && j < lane);
+    }
+    return __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < a.B && before == rank));
+}
+
+template <bool PAGED>
+__global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void range_wide_kernel(RangeAttnArgs a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[RING_LDS];
+    __shared__ int staged[PAGED ? RANGE_WIDE_STAGED : 1];
+    constexpr int BT = IMG_TILE_KEYS;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, hf = lane >> 5;
+
+    // ---- the block. Hardware workgroup b runs on XCD b % 8. Rows: an XCD works on whole heads where they divide evenly (the
+    // blocks of a head share its keys in the XCD's L2), the last blocks of a head first: without a full window they are the
+    // longest. Pages: longest sequences first; the blocks of one sequence and head next to each other on one XCD.
+    const int nblk = (int)(((int64_t)(PAGED ? a.max_rows : a.W) * a.G + KBM - 1) / KBM);
+    int b = 0, hk, blk, split;
+    {
+        const int id = blockIdx.x, xcd = id & 7, per_pair = nblk * a.nsplit;
+        int pair, at;
+        if (PAGED) {
+            pair = id / (8 * per_pair) * 8 + xcd;
+            at = id / 8 % per_pair;
+            if (pair >= a.B * a.HK) return;
+        } else if (a.HK % 8 == 0) {
+            pair = id / 8 / per_pair + xcd * (a.HK / 8);
+            at = id / 8 % per_pair;
+        } else {
+            pair = id % a.HK;
+            at = id / a.HK;
+        }
+        hk = pair % a.HK;
+        if (PAGED) b = a.B > 1 && a.B <= 64 ? seq_by_length(a, pair / a.HK) : pair / a.HK;
+        split = at % a.nsplit;
+        blk = nblk - 1 - at / a.nsplit;
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    const Seq sq = seq_of<PAGED>(a, b);
+    const int row0 = blk * KBM;
+    const int64_t rows = (int64_t)max(sq.n, 0) * a.G;
+    if (row0 >= rows) return;
+    TileList<BT, PAGED> tl;
+    tl.init(a, sq, row0 / a.G, (int)min((int64_t)sq.n - 1, ((int64_t)row0 + KBM - 1) / a.G), split);
+    const bool bad = tl.template stage<256>(a, b, staged);
+    const int x0 = tl.x0, x1 = tl.x1;
+
+    // ---- this lane's row
+    const int r = row0 + 32 * wv + n, rr = min(r, (int)rows - 1);
+    const bool live = r < rows;
+    const int i = rr / a.G, head = hk * a.G + rr - i * a.G;
+    const Sees me = sees_of<PAGED>(a, sq, i);
+    if (x0 >= x1) {   // nothing to see in this part
+        if (live) {
+            if (a.nsplit > 1) {
+                const int64_t slot = part_slot(a, sq, i, head, split);
+                if (hf == 0) a.part_ml[2 * slot] = -INFINITY;
+                else a.part_ml[2 * slot + 1] = 0.0f;
+            } else {
+                uint16_t* dst = a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D + 64 * hf;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) *reinterpret_cast<u32x4*>(dst + 8 * e) = u32x4{0, 0, 0, 0};
+            }
+        }
+        return;
+    }
+    // half-tiles that every row of the wave sees whole need no mask
+    const int hi_all = __builtin_amdgcn_readfirstlane(PAGED && a.tree ? max(0, min(sq.p0, sq.end)) : wave_min_i(me.hi));
+    const int lo_all = __builtin_amdgcn_readfirstlane(wave_max_i(me.lo));
+    const int nsteps = x1 - x0;
+
+    // ---- direct loads: a tile is four 1 KB loads of each wave. Load u of a key tile: fragment 4 wv + u (key
+    // block wv >> 1, k-step 4 (wv & 1) + u), lane 32 hf + n row img_key_perm(n) of the block. Load u of a value tile: rows
+    // 16 wv + 4 u + vt_lane_row(lane) in the row-block layout (attn_tiles.inc). Rows past the last key read that one.
+    const int64_t k_rs = PAGED ? a.pg.rs : a.k_rs, v_rs = PAGED ? a.pg.rs : a.v_rs;
+    const int64_t hoff = (int64_t)hk * (PAGED ? a.pg.hs : D);
+    const uint64_t khead = (uint64_t)(uintptr_t)(a.k + hoff), vhead = (uint64_t)(uintptr_t)(a.v + hoff);
+    const uint32_t krowb = (uint32_t)k_rs * 2u, rowb = (uint32_t)v_rs * 2u;   // (strides at most 2^24: the host checks)
+    const uint32_t lds0 = lds_addr(lds), ring = lds0, vring = ring + 2 * IMG_TILE_BYTES;
+    const uint32_t lane16 = (uint32_t)lane * 16u;
+    const uint32_t kr16 = (uint32_t)img_key_perm(n) & 15u, kcol = (uint32_t)(128 * (wv & 1) + 16 * hf);
+    const bool khalf = (n & 16) != 0;
+    const uint32_t vr16 = (uint32_t)vt_lane_row(lane), vchunk = (uint32_t)(16 * vt_lane_chunk(lane));
+    auto tile_of = [&](int u) __attribute__((always_inline)) { return min(x0 + u, x1 - 1); };
+    // the base of 16-row group g of tile x, and the last row of it that exists
+    auto group = [&](int x, int g, int64_t rs, int& last) __attribute__((always_inline)) {
+        const int k0 = tl.key0(x), j = min(k0 + 16 * g, (tl.end - 1) & ~15);
+        last = min(15, tl.end - 1 - j);
+        if constexpr (PAGED) {
+            const int page = __builtin_amdgcn_readfirstlane(max(tl.entry(x, j - k0), 0));
+            return (uint64_t)(((int64_t)page * a.pg.ps + (int64_t)(j & ((1 << tl.shift) - 1)) * rs) * 2);
+        }
+        return (uint64_t)((int64_t)j * rs * 2);
+    };
+    auto k_src = [&](int x) __attribute__((always_inline)) {
+        int l0, l1;
+        const uint64_t b0 = khead + group(x, 2 * (wv >> 1), k_rs, l0), b1 = khead + group(x, 2 * (wv >> 1) + 1, k_rs, l1);
+        return (khalf ? b1 : b0) + (min(kr16, (uint32_t)(khalf ? l1 : l0)) * krowb + kcol);
+    };
+    int vlast = 15;
+    auto v_src = [&](int x) __attribute__((always_inline)) { return vhead + group(x, wv, v_rs, vlast); };
+    auto load_k1 = [&](uint64_t src, uint32_t dst, int u) __attribute__((always_inline)) {
+        const uint32_t to = dst + (uint32_t)(wv * 4096 + 1024 * u);
+        if (u == 0) dma1_far<0>(src, to);
+        else if (u == 1) dma1_far<32>(src, to);
+        else if (u == 2) dma1_far<64>(src, to);
+        else dma1_far<96>(src, to);
+    };
+    auto load_v1 = [&](uint64_t src, uint32_t dst, int u) __attribute__((always_inline)) {
+        dma1(src, min(vr16 + 4 * u, (uint32_t)vlast) * rowb + vchunk, dst + (uint32_t)(wv * 4096 + 1024 * u));
+    };
+
+    // ---- registers (as the key-split kernel's)
+    bf16x8 qa[8];
+    f32x16 o[4], s[2], negm;
+    u32x4 p[2][2];
+    float ls = 0.0f;
+    bf16x8 fr[FR];
+    const uint32_t vlane = (uint32_t)vt_lane(lane);
+    auto vfrag_off = [](int x) __attribute__((always_inline)) { return 4096 * (x >> 2) + 256 * (x & 3); };
+
+    {
+        const uint16_t* src = a.q + (int64_t)(sq.t0 + i) * a.q_rs + head * D + 8 * hf;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) qa[ks] = *reinterpret_cast<const bf16x8*>(src + 16 * ks);
+        const uint64_t ks = k_src(tile_of(0));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) load_k1(ks, ring, u);
+    }
+
+    // ---- masked half-tiles: what the row does not see out, and a reference for the rows that have none yet
+    float mref = 0.0f;
+    const float c = a.c;
+    bool set = !live;
+    bool unset_any = true;
+    auto special = [&](int x, int half) __attribute__((always_inline)) {
+        const int kb = tl.key0(x) + 32 * half;
+        return unset_any || bad || !(kb + 32 <= hi_all && (kb >= lo_all || kb + 32 <= a.sinks));
+    };
+    auto mask_half = [&](f32x16& sb, int x, int half) __attribute__((always_inline)) {
+        const uint32_t m = seen_bits<BT, PAGED>(a, sq, tl, bad, i, me, x, 32 * half) >> (8 * hf);
+#pragma unroll
+        for (int q = 0; q < 16; ++q)
+            if (!(m >> (16 * (q >> 3) + (q & 7)) & 1)) sb[q] = -INFINITY;
+        if (unset_any) {
+            float mx = sb[0];
+#pragma unroll
+            for (int q = 1; q < 16; ++q) mx = fmaxf(mx, sb[q]);
+            mx = wave_pair_max(mx);
+            // (the scores of a row without a reference are relative to 0)
+            const float dm = !set && mx > -INFINITY ? mx : 0.0f;
+            set = set || mx > -INFINITY;
+            sb -= dm;
+            negm -= dm;
+            mref = fmaf(dm, c, mref);
+            asm volatile(LR_NOP48 : "+v"(negm));
+            // rows that see nothing further on need none
+            const int next = tl.key0(x) + 32 * half + 32;
+            unset_any = __builtin_amdgcn_ballot_w64(!set && me.hi > next) != 0;
+        }
+    };
+
+    float e0 = 0.0f, e1 = 0.0f;
+    auto stage_e = [&](const f32x16& sb, int w) __attribute__((always_inline)) {
+        e0 = __builtin_amdgcn_exp2f(sb[8 * (w >> 2) + 2 * (w & 3)] * c);
+        e1 = __builtin_amdgcn_exp2f(sb[8 * (w >> 2) + 2 * (w & 3) + 1] * c);
+        asm volatile("" ::"v"(e0), "v"(e1));   // computed in this slot, not sunk towards the next use
+    };
+    const bf16x2 ones2 = {(bf16)1.0f, (bf16)1.0f};
+    auto stage_c = [&](u32x4 (&pb)[2], int w) __attribute__((always_inline)) {
+        const uint32_t x = pack_bf16x2(e0, e1);
+        pb[w >> 2][w & 3] = x;
+        ls = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), ones2, ls, false);
+        asm volatile("" ::"v"(x), "v"(ls));
+    };
+    auto half_step = [&](f32x16& so, const u32x4 (&ppv)[2], const f32x16& si, u32x4 (&po)[2], auto pv_tag,
+                         auto&& rd) __attribute__((always_inline)) {
+        constexpr bool HAS_PV = decltype(pv_tag)::value;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int f = 0; f < 16; ++f) {
+            if (f < 8) {
+                if (f == 0) qk_init(so, fr[0], qa[0], negm);
+                else qk_acc(so, fr[f % FR], qa[f]);
+            } else {
+                if constexpr (HAS_PV) pv(o[(f - 8) & 3], fr[f % FR], ppv[(f - 8) >> 2]);
+            }
+            if ((f & 1) == 0) stage_e(si, f >> 1);
+            else stage_c(po, f >> 1);
+            rd(f + RA);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // a step's refills, one load every other slot of its first half: V(u), then K(u + 1) (past the last tile a repeat of it,
+    // never read)
+    auto refill = [&](int f, uint64_t vs, uint32_t vd, uint64_t ks, uint32_t kd) __attribute__((always_inline)) {
+        if (f % 2 == 0) {
+            if (f < 8) load_v1(vs, vd, f / 2);
+            else load_k1(ks, kd, (f - 8) / 2);
+        }
+    };
+
+    // ---- the queries and K(0) resident; S of the first half-tile, and the rows' references
+#pragma unroll
+    for (int db = 0; db < 4; ++db) o[db] = f32x16{};
+    negm = f32x16{};
+    LR_WAIT_VMCNT(0);
+    block_barrier();
+    {
+        const uint64_t vs = v_src(tile_of(0));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) load_v1(vs, vring, u);
+    }
+    {
+        uint32_t kb0 = ring + lane16;
+        asm volatile("" : "+v"(kb0));
+        fence_q8(qa);
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+            const bf16x8 kf = frag_at(kb0 + (uint32_t)(ks * IMG_FRAG_BYTES));
+            if (ks == 0) qk_zero(s[0], kf, qa[0]);
+            else qk_acc(s[0], kf, qa[ks]);
+        }
+        fence_s(s[0]);
+        mask_half(s[0], x0, 0);
+    }
+    // ---- step 0: S of half-tile 1 (K(0), fragments 8-15), P of half-tile 0
+    {
+        const uint64_t ks = k_src(tile_of(1));   // (one tile in all: a repeat of it, never read)
+        uint32_t kb = ring + lane16;
+        asm volatile("" : "+v"(kb));
+        auto rd0 = [&](int f) __attribute__((always_inline)) {
+            if (f < 8) fr[f % FR] = frag_at(kb + (8 + f) * IMG_FRAG_BYTES);
+        };
+#pragma unroll
+        for (int f = 0; f < RA; ++f) rd0(f);
+        half_step(s[1], p[1], s[0], p[0], BoolTag<false>{}, [&](int f) __attribute__((always_inline)) {
+            if ((f - RA) % 2 == 0 && f - RA < 8) load_k1(ks, ring + IMG_TILE_BYTES, (f - RA) / 2);
+            rd0(f);
+        });
+        LR_WAIT_VMCNT(0);
+        block_barrier();
+    }
+    // ---- step u: key tile u (both halves), value tile u - 1. Its refills go to the slots of V(u - 2) and K(u - 1), both
+    // read before the last barrier, and have landed at its end.
+    for (int u = 1; u < nsteps; ++u) {
+        const int x = x0 + u, xp = x - 1;
+        const uint32_t par = (uint32_t)((u & 1) * IMG_TILE_BYTES), par1 = par ^ IMG_TILE_BYTES;
+        const uint64_t vs = v_src(tile_of(u)), ks = k_src(tile_of(u + 1));
+        uint32_t kb = ring + par + lane16, vb = vring + par1 + vlane;
+        asm volatile("" : "+v"(kb), "+v"(vb));
+        auto rd_b = [&](int f) __attribute__((always_inline)) {
+            if (f < 8) fr[f % FR] = frag_at(kb + f * IMG_FRAG_BYTES);
+            else if (f < 16) fr[f % FR] = vfrag_at(vb + vfrag_off(f - 8));
+            else fr[f % FR] = frag_at(kb + (f - 8) * IMG_FRAG_BYTES);
+        };
+        auto rd_a = [&](int f) __attribute__((always_inline)) {
+            if (f < 8) fr[f % FR] = frag_at(kb + (8 + f) * IMG_FRAG_BYTES);
+            else if (f < 16) fr[f % FR] = vfrag_at(vb + vfrag_off(f));
+        };
+#pragma unroll
+        for (int f = 0; f < RA; ++f) rd_b(f);
+        if (special(xp, 1)) mask_half(s[1], xp, 1);
+        half_step(s[0], p[0], s[1], p[1], BoolTag<true>{}, [&](int f) __attribute__((always_inline)) {
+            refill(f - RA, vs, vring + par, ks, ring + par1);
+            rd_b(f);
+        });
+        if (special(x, 0)) mask_half(s[0], x, 0);
+        half_step(s[1], p[1], s[0], p[0], BoolTag<true>{}, rd_a);
+        LR_WAIT_VMCNT(0);
+        block_barrier();
+    }
+    // ---- the last half-tile's P and the last value tile's products
+    {
+        const int u = nsteps - 1, x = x0 + u;
+        if (special(x, 1)) mask_half(s[1], x, 1);
+        uint32_t vb0 = vring + (uint32_t)((u & 1) * IMG_TILE_BYTES) + vlane;
+        asm volatile("" : "+v"(vb0));
+        bf16x8 vf[4];
+#pragma unroll
+        for (int y = 0; y < 3; ++y) vf[y] = vfrag_at(vb0 + vfrag_off(y));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int y = 0; y < 16; ++y) {
+            if (y + 3 < 16) vf[(y + 3) & 3] = vfrag_at(vb0 + vfrag_off(y + 3));
+            pv(o[y & 3], vf[y & 3], (y < 8 ? p[0] : p[1])[(y >> 2) & 1]);
+            if (y < 8) {
+                stage_e(s[1], y);
+                stage_c(p[1], y);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // ---- rows out. (A row that saw a key has a sum of at least 1; a sum past 2^100, or not a number, means that its reference
+    // was overflowed.)
+    const float l = wave_pair_sum(ls);
+    float nan = l <= 0x1p100f ? 0.0f : __builtin_nanf("");   // NaN iff the row is not finite
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) nan = fmaf(0.0f, o[db][e], nan);
+    uint64_t again = __builtin_amdgcn_ballot_w64(nan != 0.0f && live);
+    again = (again | again >> 32) & 0xffffffffu;
+    if (a.nsplit > 1) {
+        if (live) {
+            const int64_t slot = part_slot(a, sq, i, head, split);
+            float* po = a.part_o + slot * D + 4 * hf;
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+#pragma unroll
+                for (int gg = 0; gg < 4; ++gg)
+                    *reinterpret_cast<f32x4*>(po + 32 * db + 8 * gg) =
+                        f32x4{o[db][4 * gg], o[db][4 * gg + 1], o[db][4 * gg + 2], o[db][4 * gg + 3]};
+            if (hf == 0) {
+                a.part_ml[2 * slot] = l > 0.0f ? mref : -INFINITY;
+                a.part_ml[2 * slot + 1] = l;
+            }
+        }
+    } else {
+        // 8 dims a store: the lower lanes take both halves' words of the even 8-dim groups, the upper lanes of the odd ones
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        uint16_t* dst = a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D + 8 * hf;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                uint32_t w[2][2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int at = 4 * (2 * x + e);
+                    w[e][0] = pack_bf16x2(o[db][at] * inv, o[db][at + 1] * inv);
+                    w[e][1] = pack_bf16x2(o[db][at + 2] * inv, o[db][at + 3] * inv);
+                }
+                const auto r0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+                const auto r1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+                if (live) *reinterpret_cast<u32x4*>(dst + 32 * db + 16 * x) = u32x4{r0[0], r1[0], r0[1], r1[1]};
+            }
+    }
+    while (again) {
+        const int q = __builtin_ctzll(again);
+        again &= again - 1;
+        redo_row<BT, PAGED>(a, sq, tl, hk, split, __builtin_amdgcn_readlane(i, q), __builtin_amdgcn_readlane(head, q));
+    }
+}
+
+}  // namespace
+
+hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, hipStream_t stream) {
+    const int64_t nblk = ((int64_t)(paged ? a.max_rows : a.W) * a.G + KBM - 1) / KBM;
+    const int64_t pairs = paged ? ((int64_t)a.B * a.HK + 7) / 8 * 8 : a.HK;
+    const int64_t blocks = nblk * a.nsplit * pairs;
+    if (blocks > 1 << 23) return hipErrorInvalidValue;   // (a grid's work-items are counted in 32 bits)
+    if (paged) hipLaunchKernelGGL(range_wide_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL(range_wide_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace lr

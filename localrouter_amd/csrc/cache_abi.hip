@@ -47,34 +47,35 @@ lr::PageArgs page_args(int64_t page, int64_t row, int64_t head, int n_pages, int
 }
 
 // ------------------------------------------------------------------------------------------------ range attention
-// How a call is cut over the keys. tiles: the most key tiles that a block of rows sees; base: workgroups without a cut.
+// How a call is cut: the kernel (wide: many rows, attn_cache_wide.hip), and over the keys, nsplit parts of `per` key tiles.
 struct Cut {
+    bool wide;
     int nsplit, per;
 };
-Cut cut_of(int64_t base, int64_t tiles, int page_size) {
-    const int staged = page_size ? lr::RANGE_STAGED / std::max(1, lr::RANGE_TILE / page_size) : INT_MAX;
-    int64_t ns = std::min<int64_t>(std::max<int64_t>(1, 512 / std::max<int64_t>(base, 1)), std::max<int64_t>(1, tiles / 8));
-    int64_t per = std::max<int64_t>(1, std::min<int64_t>((tiles + ns - 1) / ns, staged));
-    ns = std::max<int64_t>(1, (tiles + per - 1) / per);
-    return Cut{(int)ns, (int)per};
-}
-int64_t block_rows(int64_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+int64_t block_rows(int64_t rows, bool wide) { return wide ? lr::RANGE_WIDE_ROWS : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
-// The most key tiles of a block: `span` keys behind the first that the block's rows share, and the first tokens.
-int64_t tiles_of(int64_t keys, int64_t span, int64_t sinks) {
-    const int64_t all = (keys + lr::RANGE_TILE - 1) / lr::RANGE_TILE;
-    return std::min(all, (std::min(sinks, keys) + lr::RANGE_TILE - 1) / lr::RANGE_TILE + span / lr::RANGE_TILE + 2);
+// rows of a kv head a sequence; pairs: sequences x kv heads; keys: the most positions of a sequence; span: the most that a
+// block of rows needs of them beside the first `sinks`.
+Cut cut_of(bool wide, int64_t rows, int64_t pairs, int64_t keys, int64_t span, int64_t sinks, int page_size) {
+    const int bt = wide ? lr::RANGE_WIDE_TILE : lr::RANGE_TILE, entries = wide ? lr::RANGE_WIDE_STAGED : lr::RANGE_STAGED;
+    const int64_t tiles = std::min((keys + bt - 1) / bt, (std::min(sinks, keys) + bt - 1) / bt + span / bt + 2);
+    const int64_t br = block_rows(rows, wide), base = (rows + br - 1) / br * pairs;
+    const int64_t staged = page_size ? entries / std::max(1, bt / page_size) : INT_MAX;
+    int64_t ns = std::min(std::max<int64_t>(1, (wide ? 256 : 512) / base), std::max<int64_t>(1, tiles / 8));
+    const int64_t per = std::max<int64_t>(1, std::min((tiles + ns - 1) / ns, staged));
+    ns = std::max<int64_t>(1, (tiles + per - 1) / per);
+    return Cut{wide, (int)ns, (int)per};
 }
-Cut window_cut(int W, int H, int HK, int nkeys, int window, int sinks, int frame) {
-    const int64_t rows = (int64_t)W * (H / HK), br = block_rows(rows);
-    const int64_t tokens = std::min<int64_t>(W, br / (H / HK) + 1);
+Cut window_cut(int W, int H, int HK, int nkeys, int window, int sinks, int frame, bool narrow) {
+    const int64_t rows = (int64_t)W * (H / HK);
+    const int64_t tokens = std::min<int64_t>(W, 128 / (H / HK) + 2);
     const int64_t span = (window + 2) * (int64_t)frame + tokens;
-    return cut_of((rows + br - 1) / br * HK, tiles_of(nkeys, span, sinks), 0);
+    return cut_of(narrow && rows > 64, rows, HK, nkeys, span, sinks, 0);
 }
 Cut cache_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks) {
-    const int64_t rows = (int64_t)max_rows * (H / HK), br = block_rows(rows);
+    const int64_t rows = (int64_t)max_rows * (H / HK);
     const int64_t span = window ? (int64_t)window + max_rows + 1 : max_keys;
-    return cut_of((rows + br - 1) / br * HK * B, tiles_of(max_keys, span, sinks), page_size);
+    return cut_of(rows > 64 && page_size >= lr::RANGE_WIDE_MIN_PAGE, rows, (int64_t)B * HK, max_keys, span, sinks, page_size);
 }
 size_t part_bytes(int64_t rows, int nsplit) {
     return nsplit <= 1 ? 0 : (((size_t)rows * nsplit * lr::D * 4 + 255) & ~(size_t)255) + (((size_t)rows * nsplit * 8 + 255) & ~(size_t)255);
@@ -102,7 +103,7 @@ extern "C" {
 
 size_t lr_attention_window_ws_bytes(int W, int H, int HK, int nkeys, int window, int sinks, int frame) {
     if (!window_sizes_ok(W, H, HK, nkeys, window, sinks, frame)) return 0;
-    return part_bytes((int64_t)W * H, window_cut(W, H, HK, nkeys, window, sinks, frame).nsplit);
+    return part_bytes((int64_t)W * H, window_cut(W, H, HK, nkeys, window, sinks, frame, true).nsplit);
 }
 
 int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* out, int p0, int W, int H, int HK, int nkeys,
@@ -118,7 +119,8 @@ int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* 
                sk = rows_span(k, nkeys, k_row_stride, HK), sv = rows_span(v, nkeys, v_row_stride, HK);
     if (overlap(so, sq) || overlap(so, sk) || overlap(so, sv)) return ERR_ARGS;
     lr::RangeAttnArgs a{};
-    const Cut cut = window_cut(W, H, HK, nkeys, window, sinks, frame);
+    const bool narrow = k_row_stride <= lr::STREAM_MAX_V_RS && v_row_stride <= lr::STREAM_MAX_V_RS;
+    const Cut cut = window_cut(W, H, HK, nkeys, window, sinks, frame, narrow);
     const size_t need = part_bytes((int64_t)W * H, cut.nsplit);
     if (need) {
         if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return ERR_ARGS;
@@ -136,7 +138,7 @@ int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* 
     a.c = scale * 1.4426950408889634f;
     a.W = W; a.p0 = p0; a.nkeys = nkeys; a.frame = frame;
     a.window = std::min(window, MAX_POS); a.sinks = std::min(sinks, MAX_POS);
-    return (int)lr::launch_range_attn(a, false, reinterpret_cast<hipStream_t>(stream));
+    return (int)lr::launch_range_attn(a, false, cut.wide, reinterpret_cast<hipStream_t>(stream));
 }
 
 size_t lr_cache_attention_ws_bytes(int B, int T, int max_rows, int max_keys, int H, int HK, int page_size, int window,
@@ -182,7 +184,7 @@ int lr_cache_attention_bf16(const void* q, int64_t q_row_stride, void* out, int6
     a.starts = starts; a.lens = lens; a.tree = tree; a.words = tree ? words : 0;
     a.B = B; a.T = T; a.max_rows = max_rows; a.max_keys = max_keys;
     a.window = std::min(window, MAX_POS); a.sinks = window ? std::min(sinks, MAX_POS) : 0;
-    return (int)lr::launch_range_attn(a, true, reinterpret_cast<hipStream_t>(stream));
+    return (int)lr::launch_range_attn(a, true, cut.wide, reinterpret_cast<hipStream_t>(stream));
 }
 
 int lr_cache_append_bf16(const void* q, const void* k, const void* v, int64_t q_row_stride, int64_t k_row_stride,

@@ -46,10 +46,17 @@ struct RangeAttnArgs {
     float* part_ml;
 };
 
-constexpr int RANGE_TILE = 32;         // keys a tile of the small-row kernel
-constexpr int RANGE_STAGED = 2048;     // page-table entries a workgroup holds
+constexpr int RANGE_TILE = 32;              // attn_cache.hip: keys a tile,
+constexpr int RANGE_STAGED = 2048;          // page-table entries a workgroup holds
+constexpr int RANGE_WIDE_TILE = 64;         // attn_cache_wide.hip: the same, and
+constexpr int RANGE_WIDE_STAGED = 3840;
+constexpr int RANGE_WIDE_ROWS = 128;        // rows of a kv head a workgroup,
+constexpr int RANGE_WIDE_MIN_PAGE = 16;     // rows a page at least
 
-hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, hipStream_t stream);
+// The attention and, with a.nsplit > 1, the merge of its parts. wide: the kernel of attn_cache_wide.hip (the cut's tiles are
+// then its own; row strides at most STREAM_MAX_V_RS).
+hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, bool wide, hipStream_t stream);
+hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, hipStream_t stream);
 
 // cache_rows.hip
 struct CacheAppendArgs {
