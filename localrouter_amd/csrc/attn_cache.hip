@@ -38,25 +38,22 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     const int rb = wave % RB, kg = wave / RB;
 
     // ---- which rows, which keys
-    int idx = blockIdx.x;
-    const int split = idx % a.nsplit;
-    idx /= a.nsplit;
-    const int hk = idx % a.HK;
+    const int idx = blockIdx.x;
+    const int at = div_small(idx, a.nsplit, a.rcp_split), split = idx - at * a.nsplit;
+    const int blk = div_small(at, a.HK, a.rcp_hk), hk = at - blk * a.HK;
     const int b = blockIdx.y;
-    const int blk = idx / a.HK;
     const Seq sq = seq_of<PAGED>(a, b);
     const int row0 = blk * 32 * RB;
-    const int64_t rows = (int64_t)max(sq.n, 0) * a.G;
+    const int rows = max(sq.n, 0) * a.G;   // (at most 2^30: the host checks)
     if (row0 >= rows) return;
-    const int i_first = row0 / a.G, i_last = (int)min((int64_t)sq.n - 1, ((int64_t)row0 + 32 * RB - 1) / a.G);
     TileList<BT, PAGED> tl;
-    tl.init(a, sq, i_first, i_last, split);
+    tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + 32 * RB) - 1, a.G, a.rcp_g), split);
     const int x0 = tl.x0, x1 = tl.x1;
 
     // ---- this lane's row
     const int wr0 = row0 + 32 * rb, r = wr0 + n;
     const bool live = r < rows;
-    const int i = min(r, (int)rows - 1) / a.G, head = hk * a.G + min(r, (int)rows - 1) % a.G;
+    const int rr = min(r, rows - 1), i = div_small(rr, a.G, a.rcp_g), head = hk * a.G + rr - i * a.G;
     const Sees me = sees_of<PAGED>(a, sq, i);
     // tiles that every row of the wave sees whole need no mask
     const int hi_all = PAGED && a.tree ? max(0, min(sq.p0, sq.end)) : wave_min_i(me.hi);
@@ -328,10 +325,10 @@ hipError_t launch_blocks(const RangeAttnArgs& a, bool paged, hipStream_t stream)
 
 }  // namespace
 
-hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, bool wide, hipStream_t stream) {
+hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int wide, hipStream_t stream) {
     const int64_t rows = (int64_t)(paged ? a.max_rows : a.W) * a.G;
     hipError_t e;
-    if (wide) e = launch_range_wide(a, paged, stream);
+    if (wide) e = launch_range_wide(a, paged, wide, stream);
     else if (rows <= 32) e = launch_blocks<1, 4, 2>(a, paged, stream);
     else if (rows <= 64) e = launch_blocks<2, 2, 4>(a, paged, stream);
     else e = launch_blocks<4, 2, 4>(a, paged, stream);

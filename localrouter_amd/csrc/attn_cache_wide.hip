@@ -24,27 +24,18 @@ namespace {
 
 constexpr int RA = 3;             // fragments read ahead
 constexpr int FR = 4;             // fragment ring entries
-constexpr int QW = 4;             // waves (of 32 rows)
-constexpr int KBM = 32 * QW;      // rows per block
-constexpr int RING_LDS = 4 * IMG_TILE_BYTES;   // two key tiles, two value tiles
-static_assert(2 * (RING_LDS + 4 * RANGE_WIDE_STAGED + 256) <= 160 * 1024, "two workgroups a CU");
-static_assert(KBM == RANGE_WIDE_ROWS && IMG_TILE_KEYS == RANGE_WIDE_TILE, "the host's cut");
+static_assert(IMG_TILE_KEYS == RANGE_WIDE_TILE, "the host's cut");
 
 #include "attn_tiles.inc"
 #include "range_attn.inc"
 
-// One 1 KB direct load, global -> LDS: lane l's 16 bytes come from gaddr + voff and land at lds + 16 l.
-__device__ __forceinline__ void dma1(uint64_t gaddr, uint32_t voff, uint32_t lds) {
-    LR_ASM_M0_BEGIN
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(gaddr), "s"(lds)
-                 : "memory", "m0");
-    LR_ASM_M0_END
-}
-// The same from a lane's own address + OFF, to lds + 16 l (the instruction offset applies to both addresses).
+// One 1 KB direct load, global -> LDS: lane l's 16 bytes come from gaddr + voff + OFF and land at lds + 16 l (the instruction
+// offset applies to both addresses).
 template <int OFF>
-__device__ __forceinline__ void dma1_far(uint64_t addr, uint32_t lds) {
+__device__ __forceinline__ void dma1_at(uint64_t gaddr, uint32_t voff, uint32_t lds) {
     LR_ASM_M0_BEGIN
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2" ::"v"(addr), "s"(lds - OFF), "n"(OFF)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3" ::"v"(voff), "s"(gaddr), "s"(lds - OFF),
+                 "n"(OFF)
                  : "memory", "m0");
     LR_ASM_M0_END
 }
@@ -62,8 +53,12 @@ __device__ __forceinline__ int seq_by_length(const RangeAttnArgs& a, int rank) {
     return __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < a.B && before == rank));
 }
 
-template <bool PAGED>
-__global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void range_wide_kernel(RangeAttnArgs a) {
+template <int QW, bool PAGED>
+__global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu(2, 2))) void range_wide_kernel(RangeAttnArgs a) {
+    constexpr int KBM = 32 * QW;                        // rows per block
+    constexpr int RING_LDS = 4 * IMG_TILE_BYTES;        // two key tiles, two value tiles
+    constexpr int LP = 16 / QW;                         // direct loads of a tile per wave
+    static_assert(8 / QW * (RING_LDS + 4 * RANGE_WIDE_STAGED + 256) <= 160 * 1024, "8 waves a CU");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[RING_LDS];
     __shared__ int staged[PAGED ? RANGE_WIDE_STAGED : 1];
     constexpr int BT = IMG_TILE_KEYS;
@@ -75,48 +70,59 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     // ---- the block. Hardware workgroup b runs on XCD b % 8. Rows: an XCD works on whole heads where they divide evenly (the
     // blocks of a head share its keys in the XCD's L2), the last blocks of a head first: without a full window they are the
     // longest. Pages: longest sequences first; the blocks of one sequence and head next to each other on one XCD.
-    const int nblk = (int)(((int64_t)(PAGED ? a.max_rows : a.W) * a.G + KBM - 1) / KBM);
+    const int nblk = a.nblk;
     int b = 0, hk, blk, split;
     {
-        const int id = blockIdx.x, xcd = id & 7, per_pair = nblk * a.nsplit;
+        const int id = blockIdx.x, xcd = id & 7, per_pair = nblk * a.nsplit, of_xcd = (int)gridDim.x / 8;
+        // Workgroups 32 apart of an XCD share a CU: where all of them are resident at once, the second 32 go in the opposite
+        // order, the shortest beside the longest.
+        int idx = id / 8;
+        if (of_xcd <= 64 && idx >= 32) idx = of_xcd + 31 - idx;
         int pair, at;
         if (PAGED) {
-            pair = id / (8 * per_pair) * 8 + xcd;
-            at = id / 8 % per_pair;
+            pair = div_small(idx, per_pair, a.rcp_pair);
+            at = idx - pair * per_pair;
+            pair = pair * 8 + xcd;
             if (pair >= a.B * a.HK) return;
         } else if (a.HK % 8 == 0) {
-            pair = id / 8 / per_pair + xcd * (a.HK / 8);
-            at = id / 8 % per_pair;
+            pair = div_small(idx, per_pair, a.rcp_pair);
+            at = idx - pair * per_pair;
+            pair += xcd * (a.HK / 8);
         } else {
-            pair = id % a.HK;
-            at = id / a.HK;
+            at = div_small(id, a.HK, a.rcp_hk);
+            pair = id - at * a.HK;
         }
-        hk = pair % a.HK;
-        if (PAGED) b = a.B > 1 && a.B <= 64 ? seq_by_length(a, pair / a.HK) : pair / a.HK;
-        split = at % a.nsplit;
-        blk = nblk - 1 - at / a.nsplit;
+        hk = pair;
+        if (PAGED) {
+            b = div_small(pair, a.HK, a.rcp_hk);
+            hk = pair - b * a.HK;
+            if (a.B > 1 && a.B <= 64) b = seq_by_length(a, b);
+        }
+        blk = div_small(at, a.nsplit, a.rcp_split);
+        split = at - blk * a.nsplit;
+        blk = nblk - 1 - blk;
     }
     b = __builtin_amdgcn_readfirstlane(b);
     const Seq sq = seq_of<PAGED>(a, b);
     const int row0 = blk * KBM;
-    const int64_t rows = (int64_t)max(sq.n, 0) * a.G;
+    const int rows = max(sq.n, 0) * a.G;   // (at most 2^30: the host checks)
     if (row0 >= rows) return;
     TileList<BT, PAGED> tl;
-    tl.init(a, sq, row0 / a.G, (int)min((int64_t)sq.n - 1, ((int64_t)row0 + KBM - 1) / a.G), split);
-    const bool bad = tl.template stage<256>(a, b, staged);
+    tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + KBM) - 1, a.G, a.rcp_g), split);
+    const bool bad = tl.template stage<64 * QW>(a, b, staged);
     const int x0 = tl.x0, x1 = tl.x1;
 
     // ---- this lane's row
-    const int r = row0 + 32 * wv + n, rr = min(r, (int)rows - 1);
+    const int r = row0 + 32 * wv + n, rr = min(r, rows - 1);
     const bool live = r < rows;
-    const int i = rr / a.G, head = hk * a.G + rr - i * a.G;
+    const int i = div_small(rr, a.G, a.rcp_g), head = hk * a.G + rr - i * a.G;
     const Sees me = sees_of<PAGED>(a, sq, i);
     if (x0 >= x1) {   // nothing to see in this part
         if (live) {
             if (a.nsplit > 1) {
-                const int64_t slot = part_slot(a, sq, i, head, split);
-                if (hf == 0) a.part_ml[2 * slot] = -INFINITY;
-                else a.part_ml[2 * slot + 1] = 0.0f;
+                const int64_t at = part_slot(a, sq, i, head, split);
+                if (hf == 0) a.part_ml[2 * at] = -INFINITY;
+                else a.part_ml[2 * at + 1] = 0.0f;
             } else {
                 uint16_t* dst = a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D + 64 * hf;
 #pragma unroll
@@ -125,9 +131,16 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         }
         return;
     }
-    // half-tiles that every row of the wave sees whole need no mask
-    const int hi_all = __builtin_amdgcn_readfirstlane(PAGED && a.tree ? max(0, min(sq.p0, sq.end)) : wave_min_i(me.hi));
-    const int lo_all = __builtin_amdgcn_readfirstlane(wave_max_i(me.lo));
+    // half-tiles (h = 2 x + half) that every row of the wave sees whole need no mask: h < free_s among the first tokens',
+    // free_lo <= h < free_hi of the rows' own range
+    int free_s = 0, free_lo = 0, free_hi = 0;
+    if (!bad) {
+        const int hi_all = __builtin_amdgcn_readfirstlane(PAGED && a.tree ? max(0, min(sq.p0, sq.end)) : wave_min_i(me.hi));
+        const int lo_all = __builtin_amdgcn_readfirstlane(wave_max_i(me.lo)), skip = 2 * (tl.lt - tl.st);
+        free_s = min(2 * tl.st, min(a.sinks, hi_all) / 32);
+        free_lo = max(2 * tl.st, (lo_all + 31) / 32 - skip);
+        free_hi = hi_all / 32 - skip;
+    }
     const int nsteps = x1 - x0;
 
     // ---- direct loads: a tile is four 1 KB loads of each wave. Load u of a key tile: fragment 4 wv + u (key
@@ -136,39 +149,62 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     const int64_t k_rs = PAGED ? a.pg.rs : a.k_rs, v_rs = PAGED ? a.pg.rs : a.v_rs;
     const int64_t hoff = (int64_t)hk * (PAGED ? a.pg.hs : D);
     const uint64_t khead = (uint64_t)(uintptr_t)(a.k + hoff), vhead = (uint64_t)(uintptr_t)(a.v + hoff);
-    const uint32_t krowb = (uint32_t)k_rs * 2u, rowb = (uint32_t)v_rs * 2u;   // (strides at most 2^24: the host checks)
-    const uint32_t lds0 = lds_addr(lds), ring = lds0, vring = ring + 2 * IMG_TILE_BYTES;
+    const uint32_t krowb = (uint32_t)k_rs * 2u, rowb = (uint32_t)v_rs * 2u;   // (below 2^24: the host checks)
+    const uint32_t ring = lds_addr(lds), vring = ring + 2 * IMG_TILE_BYTES;
     const uint32_t lane16 = (uint32_t)lane * 16u;
-    const uint32_t kr16 = (uint32_t)img_key_perm(n) & 15u, kcol = (uint32_t)(128 * (wv & 1) + 16 * hf);
-    const bool khalf = (n & 16) != 0;
-    const uint32_t vr16 = (uint32_t)vt_lane_row(lane), vchunk = (uint32_t)(16 * vt_lane_chunk(lane));
+    const uint32_t krow = (uint32_t)img_key_perm(n), kcol = (uint32_t)(32 * LP * (wv % (QW / 2)) + 16 * hf);
+    const uint32_t vrow = (uint32_t)(vt_lane_row(lane) + 4 * LP * wv % 16), vchunk = (uint32_t)(16 * vt_lane_chunk(lane));
     auto tile_of = [&](int u) __attribute__((always_inline)) { return min(x0 + u, x1 - 1); };
-    // the base of 16-row group g of tile x, and the last row of it that exists
-    auto group = [&](int x, int g, int64_t rs, int& last) __attribute__((always_inline)) {
-        const int k0 = tl.key0(x), j = min(k0 + 16 * g, (tl.end - 1) & ~15);
-        last = min(15, tl.end - 1 - j);
-        if constexpr (PAGED) {
-            const int page = __builtin_amdgcn_readfirstlane(max(tl.entry(x, j - k0), 0));
-            return (uint64_t)(((int64_t)page * a.pg.ps + (int64_t)(j & ((1 << tl.shift) - 1)) * rs) * 2);
-        }
+    // the first of the `run` rows of tile x from its row g on (16: a page's least), clamped to the last run that exists
+    auto first = [&](int x, int g, int run) __attribute__((always_inline)) { return min(tl.key0(x) + g, (tl.end - 1) & -run); };
+    auto page = [&](int x, int g, int run) __attribute__((always_inline)) {
+        return PAGED ? tl.entry(x, first(x, g, run) - tl.key0(x)) : 0;
+    };
+    // its base, given its page, and the last row of it that exists
+    auto base_of = [&](int x, int g, int run, int64_t rs, int entry, int& last) __attribute__((always_inline)) {
+        const int j = first(x, g, run);
+        last = min(run, tl.end - j) - 1;
+        if constexpr (PAGED)
+            return (uint64_t)(((int64_t)__builtin_amdgcn_readfirstlane(max(entry, 0)) * a.pg.ps +
+                               (int64_t)(j & ((1 << tl.shift) - 1)) * rs) * 2);
         return (uint64_t)((int64_t)j * rs * 2);
     };
+    // the page-table entries of the next refills, read a half-step ahead (read where they are used, each kept the wave's
+    // products waiting for LDS)
+    int ev = 0, ek = 0, ek1 = 0;
+    const int vg = 16 * (4 * wv / QW), kg = 32 * (2 * wv / QW);
+    const bool two_pages = PAGED && tl.shift == 4;   // a key load's 32 rows (whose distance fits 32 bits: the host checks)
+    auto v_page = [&](int x) __attribute__((always_inline)) { ev = page(x, vg, 16); };
+    auto k_page = [&](int x) __attribute__((always_inline)) {
+        ek = page(x, kg, two_pages ? 16 : 32);
+        if (two_pages) ek1 = page(x, kg + 16, 16);
+    };
+    uint32_t ko = 0;
     auto k_src = [&](int x) __attribute__((always_inline)) {
-        int l0, l1;
-        const uint64_t b0 = khead + group(x, 2 * (wv >> 1), k_rs, l0), b1 = khead + group(x, 2 * (wv >> 1) + 1, k_rs, l1);
-        return (khalf ? b1 : b0) + (min(kr16, (uint32_t)(khalf ? l1 : l0)) * krowb + kcol);
+        int last;
+        if (two_pages) {
+            int last1;
+            const uint64_t b0 = base_of(x, kg, 16, k_rs, ek, last), b1 = base_of(x, kg + 16, 16, k_rs, ek1, last1);
+            const uint64_t b = b0 < b1 ? b0 : b1;
+            const bool up = (krow & 16) != 0;
+            ko = __umul24(min(krow & 15, (uint32_t)(up ? last1 : last)), krowb) + kcol + (uint32_t)((up ? b1 : b0) - b);
+            return khead + b;
+        }
+        const uint64_t b = base_of(x, kg, 32, k_rs, ek, last);
+        ko = __umul24(min(krow, (uint32_t)last), krowb) + kcol;
+        return khead + b;
     };
     int vlast = 15;
-    auto v_src = [&](int x) __attribute__((always_inline)) { return vhead + group(x, wv, v_rs, vlast); };
+    auto v_src = [&](int x) __attribute__((always_inline)) { return vhead + base_of(x, vg, 16, v_rs, ev, vlast); };
     auto load_k1 = [&](uint64_t src, uint32_t dst, int u) __attribute__((always_inline)) {
-        const uint32_t to = dst + (uint32_t)(wv * 4096 + 1024 * u);
-        if (u == 0) dma1_far<0>(src, to);
-        else if (u == 1) dma1_far<32>(src, to);
-        else if (u == 2) dma1_far<64>(src, to);
-        else dma1_far<96>(src, to);
+        const uint32_t to = dst + (uint32_t)(1024 * (LP * wv + u));
+        if (u == 0) dma1_at<0>(src, ko, to);
+        else if (u == 1) dma1_at<32>(src, ko, to);
+        else if (u == 2) dma1_at<64>(src, ko, to);
+        else dma1_at<96>(src, ko, to);
     };
     auto load_v1 = [&](uint64_t src, uint32_t dst, int u) __attribute__((always_inline)) {
-        dma1(src, min(vr16 + 4 * u, (uint32_t)vlast) * rowb + vchunk, dst + (uint32_t)(wv * 4096 + 1024 * u));
+        dma1_at<0>(src, __umul24(min(vrow + 4 * u, (uint32_t)vlast), rowb) + vchunk, dst + (uint32_t)(1024 * (LP * wv + u)));
     };
 
     // ---- registers (as the key-split kernel's)
@@ -184,9 +220,10 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         const uint16_t* src = a.q + (int64_t)(sq.t0 + i) * a.q_rs + head * D + 8 * hf;
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) qa[ks] = *reinterpret_cast<const bf16x8*>(src + 16 * ks);
+        k_page(tile_of(0));
         const uint64_t ks = k_src(tile_of(0));
 #pragma unroll
-        for (int u = 0; u < 4; ++u) load_k1(ks, ring, u);
+        for (int u = 0; u < LP; ++u) load_k1(ks, ring, u);
     }
 
     // ---- masked half-tiles: what the row does not see out, and a reference for the rows that have none yet
@@ -195,8 +232,8 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     bool set = !live;
     bool unset_any = true;
     auto special = [&](int x, int half) __attribute__((always_inline)) {
-        const int kb = tl.key0(x) + 32 * half;
-        return unset_any || bad || !(kb + 32 <= hi_all && (kb >= lo_all || kb + 32 <= a.sinks));
+        const int h = 2 * x + half;
+        return unset_any || !(h < free_s || (h >= free_lo && h < free_hi));
     };
     auto mask_half = [&](f32x16& sb, int x, int half) __attribute__((always_inline)) {
         const uint32_t m = seen_bits<BT, PAGED>(a, sq, tl, bad, i, me, x, 32 * half) >> (8 * hf);
@@ -252,12 +289,16 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // a step's refills, one load every other slot of its first half: V(u), then K(u + 1) (past the last tile a repeat of it,
-    // never read)
-    auto refill = [&](int f, uint64_t vs, uint32_t vd, uint64_t ks, uint32_t kd) __attribute__((always_inline)) {
-        if (f % 2 == 0) {
-            if (f < 8) load_v1(vs, vd, f / 2);
-            else load_k1(ks, kd, (f - 8) / 2);
+    auto slot = [](int x) __attribute__((always_inline)) { return (uint32_t)(x % 2 * IMG_TILE_BYTES); };
+    // a step's refills, one load every other slot of its first half: V(t) from slot 1 on, then K(t + 1) (past the last tile
+    // repeats of it, never read); their addresses in the slots before, under the products
+    uint64_t src = 0;
+    auto refill = [&](int f, int t) __attribute__((always_inline)) {
+        if (f == 0) src = v_src(tile_of(t));
+        if (f == 2 * LP) src = k_src(tile_of(t + 1));
+        if (f % 2 == 1) {
+            if (f / 2 < LP) load_v1(src, vring + slot(t), f / 2);
+            else if (f / 2 < 2 * LP) load_k1(src, ring + slot(t + 1), f / 2 - LP);
         }
     };
 
@@ -268,9 +309,10 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     LR_WAIT_VMCNT(0);
     block_barrier();
     {
+        v_page(tile_of(0));
         const uint64_t vs = v_src(tile_of(0));
 #pragma unroll
-        for (int u = 0; u < 4; ++u) load_v1(vs, vring, u);
+        for (int u = 0; u < LP; ++u) load_v1(vs, vring, u);
     }
     {
         uint32_t kb0 = ring + lane16;
@@ -287,7 +329,10 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     }
     // ---- step 0: S of half-tile 1 (K(0), fragments 8-15), P of half-tile 0
     {
+        k_page(tile_of(1));
         const uint64_t ks = k_src(tile_of(1));   // (one tile in all: a repeat of it, never read)
+        v_page(tile_of(1));   // (of step 1's refills)
+        k_page(tile_of(2));
         uint32_t kb = ring + lane16;
         asm volatile("" : "+v"(kb));
         auto rd0 = [&](int f) __attribute__((always_inline)) {
@@ -296,7 +341,7 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 #pragma unroll
         for (int f = 0; f < RA; ++f) rd0(f);
         half_step(s[1], p[1], s[0], p[0], BoolTag<false>{}, [&](int f) __attribute__((always_inline)) {
-            if ((f - RA) % 2 == 0 && f - RA < 8) load_k1(ks, ring + IMG_TILE_BYTES, (f - RA) / 2);
+            if ((f - RA) % 2 == 0 && f - RA < 2 * LP) load_k1(ks, ring + slot(1), (f - RA) / 2);
             rd0(f);
         });
         LR_WAIT_VMCNT(0);
@@ -306,9 +351,7 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     // read before the last barrier, and have landed at its end.
     for (int u = 1; u < nsteps; ++u) {
         const int x = x0 + u, xp = x - 1;
-        const uint32_t par = (uint32_t)((u & 1) * IMG_TILE_BYTES), par1 = par ^ IMG_TILE_BYTES;
-        const uint64_t vs = v_src(tile_of(u)), ks = k_src(tile_of(u + 1));
-        uint32_t kb = ring + par + lane16, vb = vring + par1 + vlane;
+        uint32_t kb = ring + slot(u) + lane16, vb = vring + slot(u - 1) + vlane;
         asm volatile("" : "+v"(kb), "+v"(vb));
         auto rd_b = [&](int f) __attribute__((always_inline)) {
             if (f < 8) fr[f % FR] = frag_at(kb + f * IMG_FRAG_BYTES);
@@ -316,6 +359,10 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
             else fr[f % FR] = frag_at(kb + (f - 8) * IMG_FRAG_BYTES);
         };
         auto rd_a = [&](int f) __attribute__((always_inline)) {
+            if (PAGED && f == 8) {
+                v_page(tile_of(u + 1));
+                k_page(tile_of(u + 2));
+            }
             if (f < 8) fr[f % FR] = frag_at(kb + (8 + f) * IMG_FRAG_BYTES);
             else if (f < 16) fr[f % FR] = vfrag_at(vb + vfrag_off(f));
         };
@@ -323,7 +370,7 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         for (int f = 0; f < RA; ++f) rd_b(f);
         if (special(xp, 1)) mask_half(s[1], xp, 1);
         half_step(s[0], p[0], s[1], p[1], BoolTag<true>{}, [&](int f) __attribute__((always_inline)) {
-            refill(f - RA, vs, vring + par, ks, ring + par1);
+            refill(f - RA, u);
             rd_b(f);
         });
         if (special(x, 0)) mask_half(s[0], x, 0);
@@ -335,7 +382,7 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     {
         const int u = nsteps - 1, x = x0 + u;
         if (special(x, 1)) mask_half(s[1], x, 1);
-        uint32_t vb0 = vring + (uint32_t)((u & 1) * IMG_TILE_BYTES) + vlane;
+        uint32_t vb0 = vring + slot(u) + vlane;
         asm volatile("" : "+v"(vb0));
         bf16x8 vf[4];
 #pragma unroll
@@ -364,8 +411,8 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     again = (again | again >> 32) & 0xffffffffu;
     if (a.nsplit > 1) {
         if (live) {
-            const int64_t slot = part_slot(a, sq, i, head, split);
-            float* po = a.part_o + slot * D + 4 * hf;
+            const int64_t at = part_slot(a, sq, i, head, split);
+            float* po = a.part_o + at * D + 4 * hf;
 #pragma unroll
             for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -373,8 +420,8 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
                     *reinterpret_cast<f32x4*>(po + 32 * db + 8 * gg) =
                         f32x4{o[db][4 * gg], o[db][4 * gg + 1], o[db][4 * gg + 2], o[db][4 * gg + 3]};
             if (hf == 0) {
-                a.part_ml[2 * slot] = l > 0.0f ? mref : -INFINITY;
-                a.part_ml[2 * slot + 1] = l;
+                a.part_ml[2 * at] = l > 0.0f ? mref : -INFINITY;
+                a.part_ml[2 * at + 1] = l;
             }
         }
     } else {
@@ -404,16 +451,24 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     }
 }
 
-}  // namespace
-
-hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, hipStream_t stream) {
-    const int64_t nblk = ((int64_t)(paged ? a.max_rows : a.W) * a.G + KBM - 1) / KBM;
+template <int QW>
+hipError_t launch_waves(const RangeAttnArgs& a, bool paged, hipStream_t stream) {
+    RangeAttnArgs w = a;
+    const int64_t nblk = ((int64_t)(paged ? a.max_rows : a.W) * a.G + 32 * QW - 1) / (32 * QW);
     const int64_t pairs = paged ? ((int64_t)a.B * a.HK + 7) / 8 * 8 : a.HK;
     const int64_t blocks = nblk * a.nsplit * pairs;
-    if (blocks > 1 << 23) return hipErrorInvalidValue;   // (a grid's work-items are counted in 32 bits)
-    if (paged) hipLaunchKernelGGL(range_wide_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL(range_wide_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    if (blocks > 1 << 22) return hipErrorInvalidValue;   // (a grid's work-items are counted in 32 bits)
+    w.nblk = (int)nblk;
+    w.rcp_pair = rcp_small(nblk * a.nsplit);
+    if (paged) hipLaunchKernelGGL((range_wide_kernel<QW, true>), dim3((unsigned)blocks), dim3(64 * QW), 0, stream, w);
+    else hipLaunchKernelGGL((range_wide_kernel<QW, false>), dim3((unsigned)blocks), dim3(64 * QW), 0, stream, w);
     return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, int waves, hipStream_t stream) {
+    return waves == 8 ? launch_waves<8>(a, paged, stream) : launch_waves<4>(a, paged, stream);
 }
 
 }  // namespace lr

@@ -47,24 +47,26 @@ lr::PageArgs page_args(int64_t page, int64_t row, int64_t head, int n_pages, int
 }
 
 // ------------------------------------------------------------------------------------------------ range attention
-// How a call is cut: the kernel (wide: many rows, attn_cache_wide.hip), and over the keys, nsplit parts of `per` key tiles.
+// How a call is cut: the kernel (wide: 0, or the waves of the kernel of attn_cache_wide.hip), and over the keys, nsplit parts
+// of `per` key tiles.
 struct Cut {
-    bool wide;
-    int nsplit, per;
+    int wide, nsplit, per;
 };
-int64_t block_rows(int64_t rows, bool wide) { return wide ? lr::RANGE_WIDE_ROWS : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+int64_t block_rows(int64_t rows, int wide) { return wide ? 32 * wide : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 // rows of a kv head a sequence; pairs: sequences x kv heads; keys: the most positions of a sequence; span: the most that a
 // block of rows needs of them beside the first `sinks`.
 Cut cut_of(bool wide, int64_t rows, int64_t pairs, int64_t keys, int64_t span, int64_t sinks, int page_size) {
     const int bt = wide ? lr::RANGE_WIDE_TILE : lr::RANGE_TILE, entries = wide ? lr::RANGE_WIDE_STAGED : lr::RANGE_STAGED;
     const int64_t tiles = std::min((keys + bt - 1) / bt, (std::min(sinks, keys) + bt - 1) / bt + span / bt + 2);
-    const int64_t br = block_rows(rows, wide), base = (rows + br - 1) / br * pairs;
+    const int64_t big = (rows + 255) / 256 * pairs;
+    const int waves = !wide ? 0 : tiles >= 64 && big >= 256 && (big % 256 == 0 || big >= 1024) ? 8 : 4;
+    const int64_t br = block_rows(rows, waves), base = (rows + br - 1) / br * pairs;
     const int64_t staged = page_size ? entries / std::max(1, bt / page_size) : INT_MAX;
     int64_t ns = std::min(std::max<int64_t>(1, (wide ? 256 : 512) / base), std::max<int64_t>(1, tiles / 8));
     const int64_t per = std::max<int64_t>(1, std::min((tiles + ns - 1) / ns, staged));
     ns = std::max<int64_t>(1, (tiles + per - 1) / per);
-    return Cut{wide, (int)ns, (int)per};
+    return Cut{waves, (int)ns, (int)per};
 }
 Cut window_cut(int W, int H, int HK, int nkeys, int window, int sinks, int frame, bool narrow) {
     const int64_t rows = (int64_t)W * (H / HK);
@@ -72,16 +74,19 @@ Cut window_cut(int W, int H, int HK, int nkeys, int window, int sinks, int frame
     const int64_t span = (window + 2) * (int64_t)frame + tokens;
     return cut_of(narrow && rows > 64, rows, HK, nkeys, span, sinks, 0);
 }
-Cut cache_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks) {
+Cut cache_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks, bool narrow) {
     const int64_t rows = (int64_t)max_rows * (H / HK);
     const int64_t span = window ? (int64_t)window + max_rows + 1 : max_keys;
-    return cut_of(rows > 64 && page_size >= lr::RANGE_WIDE_MIN_PAGE, rows, (int64_t)B * HK, max_keys, span, sinks, page_size);
+    return cut_of(narrow && rows > 64 && page_size >= lr::RANGE_WIDE_MIN_PAGE, rows, (int64_t)B * HK, max_keys, span, sinks, page_size);
 }
 size_t part_bytes(int64_t rows, int nsplit) {
     return nsplit <= 1 ? 0 : (((size_t)rows * nsplit * lr::D * 4 + 255) & ~(size_t)255) + (((size_t)rows * nsplit * 8 + 255) & ~(size_t)255);
 }
 void set_parts(lr::RangeAttnArgs& a, void* ws, int64_t rows, Cut cut) {
     a.nsplit = cut.nsplit;
+    a.rcp_split = lr::rcp_small(cut.nsplit);
+    a.rcp_g = lr::rcp_small(a.G);
+    a.rcp_hk = lr::rcp_small(a.HK);
     a.tiles_per_split = cut.per;
     a.part_o = static_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + (((size_t)rows * cut.nsplit * lr::D * 4 + 255) & ~(size_t)255));
@@ -103,7 +108,8 @@ extern "C" {
 
 size_t lr_attention_window_ws_bytes(int W, int H, int HK, int nkeys, int window, int sinks, int frame) {
     if (!window_sizes_ok(W, H, HK, nkeys, window, sinks, frame)) return 0;
-    return part_bytes((int64_t)W * H, window_cut(W, H, HK, nkeys, window, sinks, frame, true).nsplit);
+    return std::max(part_bytes((int64_t)W * H, window_cut(W, H, HK, nkeys, window, sinks, frame, true).nsplit),
+                    part_bytes((int64_t)W * H, window_cut(W, H, HK, nkeys, window, sinks, frame, false).nsplit));
 }
 
 int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* out, int p0, int W, int H, int HK, int nkeys,
@@ -119,7 +125,7 @@ int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* 
                sk = rows_span(k, nkeys, k_row_stride, HK), sv = rows_span(v, nkeys, v_row_stride, HK);
     if (overlap(so, sq) || overlap(so, sk) || overlap(so, sv)) return ERR_ARGS;
     lr::RangeAttnArgs a{};
-    const bool narrow = k_row_stride <= lr::STREAM_MAX_V_RS && v_row_stride <= lr::STREAM_MAX_V_RS;
+    const bool narrow = k_row_stride < lr::RANGE_WIDE_MAX_RS && v_row_stride < lr::RANGE_WIDE_MAX_RS;
     const Cut cut = window_cut(W, H, HK, nkeys, window, sinks, frame, narrow);
     const size_t need = part_bytes((int64_t)W * H, cut.nsplit);
     if (need) {
@@ -128,7 +134,6 @@ int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* 
         const Span w{lo, lo + need};
         if (overlap(w, so) || overlap(w, sq) || overlap(w, sk) || overlap(w, sv)) return ERR_ARGS;
     }
-    set_parts(a, workspace, (int64_t)W * H, cut);
     a.q = static_cast<const uint16_t*>(q);
     a.k = static_cast<const uint16_t*>(k);
     a.v = static_cast<const uint16_t*>(v);
@@ -136,7 +141,9 @@ int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* 
     a.q_rs = q_row_stride; a.k_rs = k_row_stride; a.v_rs = v_row_stride; a.o_rs = out_row_stride;
     a.H = H; a.HK = HK; a.G = H / HK;
     a.c = scale * 1.4426950408889634f;
-    a.W = W; a.p0 = p0; a.nkeys = nkeys; a.frame = frame;
+    set_parts(a, workspace, (int64_t)W * H, cut);
+    a.W = W; a.p0 = p0; a.nkeys = nkeys; a.frame = std::min(frame, MAX_POS);   // (positions are below it either way)
+    a.rcp_frame = lr::rcp_small(a.frame);
     a.window = std::min(window, MAX_POS); a.sinks = std::min(sinks, MAX_POS);
     return (int)lr::launch_range_attn(a, false, cut.wide, reinterpret_cast<hipStream_t>(stream));
 }
@@ -144,7 +151,8 @@ int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* 
 size_t lr_cache_attention_ws_bytes(int B, int T, int max_rows, int max_keys, int H, int HK, int page_size, int window,
                                    int sinks) {
     if (!cache_sizes_ok(B, T, max_rows, max_keys, H, HK, page_size, window, sinks)) return 0;
-    return part_bytes((int64_t)T * H, cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks).nsplit);
+    return std::max(part_bytes((int64_t)T * H, cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks, true).nsplit),
+                    part_bytes((int64_t)T * H, cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks, false).nsplit));
 }
 
 int lr_cache_attention_bf16(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride, const void* k_pages,
@@ -164,7 +172,8 @@ int lr_cache_attention_bf16(const void* q, int64_t q_row_stride, void* out, int6
                sv = pool_span(v_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK);
     if (overlap(so, sq) || overlap(so, sk) || overlap(so, sv)) return ERR_ARGS;
     lr::RangeAttnArgs a{};
-    const Cut cut = cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks);
+    const bool narrow = row_stride < lr::RANGE_WIDE_MAX_RS && (page_size > lr::RANGE_WIDE_MIN_PAGE || sk.hi - sk.lo < (1ull << 32));
+    const Cut cut = cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks, narrow);
     const size_t need = part_bytes((int64_t)T * H, cut.nsplit);
     if (need) {
         if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return ERR_ARGS;
@@ -172,7 +181,6 @@ int lr_cache_attention_bf16(const void* q, int64_t q_row_stride, void* out, int6
         const Span w{lo, lo + need};
         if (overlap(w, so) || overlap(w, sq) || overlap(w, sk) || overlap(w, sv)) return ERR_ARGS;
     }
-    set_parts(a, workspace, (int64_t)T * H, cut);
     a.q = static_cast<const uint16_t*>(q);
     a.k = static_cast<const uint16_t*>(k_pages);
     a.v = static_cast<const uint16_t*>(v_pages);
@@ -181,6 +189,7 @@ int lr_cache_attention_bf16(const void* q, int64_t q_row_stride, void* out, int6
     a.H = H; a.HK = HK; a.G = H / HK;
     a.c = scale * 1.4426950408889634f;
     a.pg = page_args(page_stride, row_stride, head_stride, n_pages, page_size, page_table, table_stride, table_pages);
+    set_parts(a, workspace, (int64_t)T * H, cut);
     a.starts = starts; a.lens = lens; a.tree = tree; a.words = tree ? words : 0;
     a.B = B; a.T = T; a.max_rows = max_rows; a.max_keys = max_keys;
     a.window = std::min(window, MAX_POS); a.sinks = window ? std::min(sinks, MAX_POS) : 0;

@@ -44,19 +44,25 @@ struct RangeAttnArgs {
     int nsplit, tiles_per_split;
     float* part_o;
     float* part_ml;
+    // rcp_small of the divisors; nblk (and rcp_pair, of nblk * nsplit): blocks of rows a sequence and kv head, set by the launch
+    uint32_t rcp_g, rcp_hk, rcp_frame, rcp_split, rcp_pair;
+    int nblk;
 };
+
+// floor(2^32 / d), 2^32 - 1 for d = 1: what the kernels divide by d with.
+inline uint32_t rcp_small(int64_t d) { return d > 1 ? (uint32_t)(((uint64_t)1 << 32) / (uint64_t)d) : 0xffffffffu; }
 
 constexpr int RANGE_TILE = 32;              // attn_cache.hip: keys a tile,
 constexpr int RANGE_STAGED = 2048;          // page-table entries a workgroup holds
 constexpr int RANGE_WIDE_TILE = 64;         // attn_cache_wide.hip: the same, and
-constexpr int RANGE_WIDE_STAGED = 3840;
-constexpr int RANGE_WIDE_ROWS = 128;        // rows of a kv head a workgroup,
-constexpr int RANGE_WIDE_MIN_PAGE = 16;     // rows a page at least
+constexpr int RANGE_WIDE_STAGED = 3840;     // (both of its forms: 4 and 8 waves of 32 rows);
+constexpr int RANGE_WIDE_MIN_PAGE = 16;     // rows a page at least (of 16 rows: in pools of less than 4 GB),
+constexpr int64_t RANGE_WIDE_MAX_RS = 1 << 23;   // and row strides (elements) below this
 
-// The attention and, with a.nsplit > 1, the merge of its parts. wide: the kernel of attn_cache_wide.hip (the cut's tiles are
-// then its own; row strides at most STREAM_MAX_V_RS).
-hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, bool wide, hipStream_t stream);
-hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, hipStream_t stream);
+// The attention and, with a.nsplit > 1, the merge of its parts. wide: 0, or the waves of the kernel of attn_cache_wide.hip (the
+// cut's tiles are then its own).
+hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int wide, hipStream_t stream);
+hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, int waves, hipStream_t stream);
 
 // cache_rows.hip
 struct CacheAppendArgs {

@@ -154,6 +154,31 @@ def test_attention_of_trees(c):
     B.check(q, out, lambda b: tree_seen(trees[b], lens[b], window, sinks))
 
 
+@pytest.mark.parametrize("ps", [16, 64])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attention_of_whole_rounds(ps, tree):
+    """Enough blocks and keys for the workgroups of eight waves: 8 sequences of 64 tokens x 128 heads over 8; the first and last
+    tokens of some checked, with a page that the pool does not have."""
+    news, lens = [64, 40, 64, 1, 64, 64, 50, 64], [4300, 5000, 64, 4100, 4200, 130, 4999, 2500]
+    B = Batch(24, news, lens, ps, 8)
+    rng = random.Random(7)
+    trees = [random_tree(rng, n) for n in news]
+    table = [list(r) for r in B.table]
+    table[6][3] = -5
+    gone = range(3 * ps, 4 * ps)
+    q = rnd(B.g, sum(news), 128, 128)
+    out = cache.attention(q, B.kp, B.vp, ints(table), B.starts, B.lens, max_rows=64, max_keys=5000,
+                          tree=tree_words(trees, 1) if tree else None)
+    for b in (0, 2, 3, 6):
+        at = sorted({0, min(1, news[b] - 1), news[b] - 1})
+        seen = (tree_seen(trees[b], lens[b]) if tree else chain_seen(news[b], lens[b]))[at]
+        if b == 6:
+            seen[:, list(gone)] = False
+        k, v = B.rows(b)
+        rows = [B.st[b] + i for i in at]
+        check_rows(out[rows], *ref_rows(q[rows], k, v, seen), what=f"sequence {b}")
+
+
 def test_a_tree_of_one_branch_is_a_chain():
     news, lens = [9, 70], [100, 70]
     B = Batch(13, news, lens, 16, 2)

@@ -48,6 +48,16 @@ def test_window_matches_64_bits(c):
     check_rows(out, *ref_rows(q, k, v, window_seen(w, n, p0, window, sinks, frame)))
 
 
+@pytest.mark.parametrize("frame,window,sinks", [(1, 4100, 5), (500, 9, 700)])
+def test_window_of_whole_rounds(frame, window, sinks):
+    """Enough blocks and keys for the workgroups of eight waves: 1,024 queries x 64 heads over 8; some queries checked."""
+    g = gen(21)
+    q, k, v = rnd(g, 1024, 64, 128), rnd(g, 5500, 8, 128), rnd(g, 5500, 8, 128)
+    out = ops.attention_window(q, k, v, window=window, sinks=sinks, frame=frame, p0=4400)
+    at = [0, 1, 31, 32, 33, 63, 64, 99, 100, 511, 600, 1022, 1023]
+    check_rows(out[at], *ref_rows(q[at], k, v, window_seen(1024, 5500, 4400, window, sinks, frame)[at]))
+
+
 @pytest.mark.parametrize("scale", [0.02, 1.0])
 def test_window_scale_and_large_scores(scale):
     """Scores far from zero, rising along the keys, so that the reference of every row is raised again and again."""
