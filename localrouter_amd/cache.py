@@ -17,12 +17,13 @@ without the built library every call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 from pathlib import Path
 
 import torch
 
 from . import _lib
-from .ops import D, PAIR_INTERLEAVED, SCALE_128, TABLE_COSSIN_F32, TABLE_NONE, _ptr, _rows, _stream
+from .ops import D, PAIR_INTERLEAVED, SCALE_128, TABLE_COSSIN_F32, TABLE_NONE
 
 HEADER = Path(__file__).resolve().parent.parent / "include" / "lr_cache.h"
 
@@ -39,6 +40,9 @@ SIGNATURES = {
 }
 
 _bound = None
+_BF16, _I32, _I64T, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
+# (looked up once: a small call's ~10 us are mostly its checks)
+_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def lib() -> ctypes.CDLL:
@@ -53,51 +57,57 @@ def lib() -> ctypes.CDLL:
 
 
 def _call(name: str, *args) -> None:
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(_bound or lib(), name)(*args)
     if rc != 0:
         raise _lib.LrError(name, rc)
 
 
-def _here(t: torch.Tensor, name: str) -> None:
-    if not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
-        raise ValueError(f"{name}: expected a tensor on the current device, got {t.device}")
+def _rows(t: torch.Tensor, name: str, dev: int, n: int, heads: int) -> int:
+    """The row stride of bf16 rows [>= n, heads, 128] on device dev."""
+    s, st = t.shape, t.stride()
+    if (t.get_device() != dev or t.dtype is not _BF16 or len(s) != 3 or s[0] < n or s[1] != heads or s[2] != D or st[2] != 1
+            or (st[1] != D and heads > 1)):
+        raise ValueError(f"{name}: expected bf16 [{n}, {heads}, 128] with contiguous heads on the current device, got {t.dtype} "
+                         f"{tuple(s)} / {st} on {t.device}")
+    return st[0] if s[0] > 1 else heads * D
 
 
-def _ints(t: torch.Tensor, name: str, n: int) -> int:
-    _here(t, name)
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < n or (n > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name}: expected contiguous int32 [{n}], got {t.dtype} {tuple(t.shape)}")
+def _ints(t: torch.Tensor, name: str, dev: int, n: int) -> int:
+    if t.get_device() != dev or t.dtype is not _I32 or t.dim() != 1 or t.numel() < n or not t.is_contiguous():
+        raise ValueError(f"{name}: expected contiguous int32 [{n}] on the current device, got {t.dtype} {tuple(t.shape)} on "
+                         f"{t.device}")
     return t.data_ptr()
 
 
-def _pool(k: torch.Tensor, v: torch.Tensor, layers: bool = False):
+def _pool(k: torch.Tensor, v: torch.Tensor, dev: int, layers: bool = False) -> tuple:
     """(k pointer, v pointer, [layers, layer stride,] page, row and head strides, pages, page size, heads)."""
-    for t, name in ((k, "k_pages"), (v, "v_pages")):
-        _here(t, name)
-        if t.dtype != torch.bfloat16 or t.shape[-1] != D or t.stride(-1) != 1:
-            raise ValueError(f"{name}: expected bf16 rows of 128 with unit stride, got {t.dtype} {tuple(t.shape)}")
     s, st = k.shape, k.stride()
-    if v.shape != s or v.stride() != st:
-        raise ValueError("k_pages and v_pages need the same shape and strides")
-    if len(s) == 4:
-        lead = (1, 0) if layers else ()
-    elif len(s) == 5 and layers:
-        lead = (s[0], st[0] if s[0] > 1 else 0)
-    else:
-        raise ValueError(f"k_pages: expected [n_pages, page_size, heads, 128]{' or [layers, ...]' if layers else ''}, got {tuple(s)}")
+    n = len(s)
+    if (k.get_device() != dev or v.get_device() != dev or k.dtype is not _BF16 or v.dtype is not _BF16 or v.shape != s
+            or v.stride() != st or not (n == 4 or (layers and n == 5)) or s[-1] != D or st[-1] != 1 or 0 in s):
+        raise ValueError(f"k_pages, v_pages: expected bf16 [n_pages, page_size, heads, 128]{' or [layers, ...]' if layers else ''} "
+                         f"of the same shape and strides on the current device, got {k.dtype} {tuple(s)} / {st} on {k.device} and "
+                         f"{v.dtype} {tuple(v.shape)} / {v.stride()} on {v.device}")
     P, R, H = s[-4:-1]
+    ps, rs, hs = st[-4:-1]
     # (a dimension of one element has whatever stride its view left: taken as packed)
-    hs = st[-2] if H > 1 else D
-    rs = st[-3] if R > 1 else max(D, (H - 1) * hs + D)
-    ps = st[-4] if P > 1 else max((R - 1) * rs, 0) + (H - 1) * hs + D
-    return (k.data_ptr(), v.data_ptr(), *lead, ps, rs, hs, P, R, H)
+    if H == 1:
+        hs = D
+    if R == 1:
+        rs = max(D, (H - 1) * hs + D)
+    if P == 1:
+        ps = (R - 1) * rs + (H - 1) * hs + D
+    if layers:
+        return (k.data_ptr(), v.data_ptr(), s[0] if n == 5 else 1, st[0] if n == 5 and s[0] > 1 else 0, ps, rs, hs, P, R, H)
+    return k.data_ptr(), v.data_ptr(), ps, rs, hs, P, R, H
 
 
-def _table(t: torch.Tensor, B: int):
-    _here(t, "page_table")
-    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] < B or t.stride(1) != 1 and t.shape[1] > 1:
-        raise ValueError(f"page_table: expected int32 [{B}, pages] with contiguous rows, got {t.dtype} {tuple(t.shape)}")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1], t.shape[1]
+def _table(t: torch.Tensor, dev: int, B: int) -> tuple:
+    s, st = t.shape, t.stride()
+    if t.get_device() != dev or t.dtype is not _I32 or len(s) != 2 or s[0] < B or (st[1] != 1 and s[1] > 1):
+        raise ValueError(f"page_table: expected int32 [{B}, pages] with contiguous rows on the current device, got {t.dtype} "
+                         f"{tuple(s)} on {t.device}")
+    return t.data_ptr(), st[0] if s[0] > 1 else s[1], s[1]
 
 
 def append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -109,57 +119,62 @@ def append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: to
     normalised and rotated into q_out (allocated when None; q itself is allowed), keys the same way into their pages, values
     as they are. table = (table_a, table_b), one row a position; positions int32 [T]: each token's table row (default its
     position in its sequence). q None: keys and values only. Returns q_out."""
-    T, HK = k.shape[0], k.shape[1]
-    B = lens.shape[0]
-    H, q_rs, o_rs = 0, 0, 0
-    k_rs, v_rs = _rows(k, "k", HK), _rows(v, "v", HK)
-    _here(k, "k")
-    _here(v, "v")
-    if v.shape[0] != T:
-        raise ValueError("append: k and v of different lengths")
+    dev = _device()
+    pool = _pool(k_pages, v_pages, dev)
+    HK = pool[7]
+    T, B = k.shape[0], lens.shape[0]
+    k_rs, v_rs = _rows(k, "k", dev, T, HK), _rows(v, "v", dev, T, HK)
+    H = q_rs = o_rs = 0
+    q_ptr = o_ptr = None
     if q is not None:
         H = q.shape[1]
-        q_rs = _rows(q, "q", H)
-        _here(q, "q")
-        if q.shape[0] != T:
-            raise ValueError("append: q and k of different lengths")
+        q_rs = _rows(q, "q", dev, T, H)
         if q_out is None:
-            q_out = torch.empty((T, H, D), dtype=torch.bfloat16, device=q.device)
-        o_rs = _rows(q_out, "q_out", H)
-        _here(q_out, "q_out")
-        if q_out.shape[0] < T:
-            raise ValueError("append: q_out shorter than q")
-    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if t is not None:
-            _here(t, name)
-            if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != D:
-                raise ValueError(f"{name}: expected fp32 [128]")
-    ta = tb = None
+            q_out = torch.empty((T, H, D), dtype=_BF16, device=q.device)
+        o_rs = _rows(q_out, "q_out", dev, T, H)
+        q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
+    if v.shape[0] != T or (q is not None and q.shape[0] != T):
+        raise ValueError("append: q, k and v of different lengths")
+    qw = kw = ta = tb = pos = None
     stride = rows = 0
+    for t in (q_norm, k_norm):
+        if t is not None and (t.get_device() != dev or t.dtype is not _F32 or t.numel() != D or not t.is_contiguous()):
+            raise ValueError("q_norm, k_norm: expected fp32 [128] on the current device")
+    if q_norm is not None:
+        qw = q_norm.data_ptr()
+    if k_norm is not None:
+        kw = k_norm.data_ptr()
     if table_kind != TABLE_NONE:
         if table is None:
             raise ValueError("append: table required")
-        ta, tb = table
-        stride, rows = ta.stride(0), ta.shape[0]
-        want = torch.bfloat16 if table_kind == 2 else torch.float32
-        for t in (ta,) if tb is None else (ta, tb):
-            _here(t, "table")
-            if t.dtype != want or t.stride(0) != stride or t.shape[0] != rows:
-                raise ValueError(f"table: expected {want} tensors of the same rows and row stride")
-    pool = _pool(k_pages, v_pages)
-    if pool[-1] != HK:
-        raise ValueError(f"append: {HK} key heads, the pool has {pool[-1]}")
-    _call("lr_cache_append_bf16", _ptr(q), k.data_ptr(), v.data_ptr(), q_rs, k_rs, v_rs, _ptr(q_out) if q is not None else None,
-          o_rs, *pool[:7], *_table(page_table, B), _ints(starts, "starts", B + 1), _ints(lens, "lens", B),
-          None if positions is None else _ints(positions, "positions", T), B, T, H, HK, _ptr(q_norm), _ptr(k_norm), table_kind,
-          _ptr(ta), _ptr(tb), stride, rows, pairing, rot, eps, _stream())
+        a, b = table
+        want = _BF16 if table_kind == 2 else _F32
+        st, rows = a.stride(), a.shape[0]
+        stride = st[0]
+        if a.get_device() != dev or a.dtype is not want or a.dim() != 2 or st[1] != 1:
+            raise ValueError(f"table: expected {want} rows on the current device")
+        ta = a.data_ptr()
+        if b is not None:
+            if b.get_device() != dev or b.dtype is not want or b.shape != a.shape or b.stride() != st:
+                raise ValueError("table: expected two tensors of the same type, shape and strides")
+            tb = b.data_ptr()
+    if positions is not None:
+        pos = _ints(positions, "positions", dev, T)
+    _call("lr_cache_append_bf16", q_ptr, k.data_ptr(), v.data_ptr(), q_rs, k_rs, v_rs, o_ptr, o_rs, *pool[:7],
+          *_table(page_table, dev, B), _ints(starts, "starts", dev, B + 1), _ints(lens, "lens", dev, B), pos, B, T, H, HK, qw, kw,
+          table_kind, ta, tb, stride, rows, pairing, rot, eps, _raw_stream(dev))
     return q_out
+
+
+@functools.lru_cache(maxsize=1024)
+def _ws_bytes(*sizes: int) -> int:
+    return int(lib().lr_cache_attention_ws_bytes(*sizes))
 
 
 def attention_ws_bytes(B: int, T: int, max_rows: int, max_keys: int, heads: int, kv_heads: int, page_size: int, *,
                        window: int = 0, sinks: int = 0) -> int:
     """lr_cache_attention_ws_bytes: the workspace a call needs (0: none)."""
-    return int(lib().lr_cache_attention_ws_bytes(B, T, max_rows, max_keys, heads, kv_heads, page_size, window, sinks))
+    return _ws_bytes(B, T, max_rows, max_keys, heads, kv_heads, page_size, window, sinks)
 
 
 def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor,
@@ -172,51 +187,52 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     positions (under a tree: those before the call's tokens) only where p - j < n or j < sinks. max_rows: the most tokens of a
     sequence (default T); max_keys: the longest sequence (default what the table holds). A workspace of attention_ws_bytes is
     allocated when none is given."""
+    dev = _device()
     T, H = q.shape[0], q.shape[1]
     B = lens.shape[0]
-    q_rs = _rows(q, "q", H)
-    _here(q, "q")
-    pool = _pool(k_pages, v_pages)
+    q_rs = _rows(q, "q", dev, T, H)
+    pool = _pool(k_pages, v_pages, dev)
     ps, HK = pool[6], pool[7]
     if out is None:
-        out = torch.empty((T, H, D), dtype=torch.bfloat16, device=q.device)
-    o_rs = _rows(out, "out", H)
-    _here(out, "out")
-    if out.shape[0] < T:
-        raise ValueError("attention: out shorter than q")
-    tab = _table(page_table, B)
-    max_rows = T if max_rows is None else min(max_rows, T)
-    max_keys = tab[2] * ps if max_keys is None else min(max_keys, tab[2] * ps)
-    words = 0
+        out = torch.empty((T, H, D), dtype=_BF16, device=q.device)
+    o_rs = _rows(out, "out", dev, T, H)
+    tab = _table(page_table, dev, B)
+    most = tab[2] * ps
+    max_rows = T if max_rows is None or max_rows > T else max_rows
+    max_keys = most if max_keys is None or max_keys > most else max_keys
+    words, tree_ptr = 0, None
     if tree is not None:
-        _here(tree, "tree")
-        if tree.dtype != torch.int64 or tree.dim() != 2 or tree.shape[0] < T or not tree.is_contiguous():
-            raise ValueError(f"tree: expected contiguous int64 [{T}, words], got {tree.dtype} {tuple(tree.shape)}")
-        words = tree.shape[1]
-    need = attention_ws_bytes(B, T, max_rows, max_keys, H, HK, ps, window=window, sinks=sinks)
-    nbytes = 0
+        if (tree.get_device() != dev or tree.dtype is not _I64T or tree.dim() != 2 or tree.shape[0] < T
+                or not tree.is_contiguous()):
+            raise ValueError(f"tree: expected contiguous int64 [{T}, words] on the current device, got {tree.dtype} "
+                             f"{tuple(tree.shape)} on {tree.device}")
+        words, tree_ptr = tree.shape[1], tree.data_ptr()
+    need = _ws_bytes(B, T, max_rows, max_keys, H, HK, ps, window, sinks)
+    ws, nbytes = None, 0
     if workspace is not None:
-        _here(workspace, "workspace")
         nbytes = workspace.numel() * workspace.element_size()
-        if nbytes < need or not workspace.is_contiguous():
-            raise ValueError(f"workspace: {need} contiguous bytes needed")
+        if nbytes < need or workspace.get_device() != dev or not workspace.is_contiguous():
+            raise ValueError(f"workspace: {need} contiguous bytes on the current device needed")
+        ws = workspace.data_ptr()
     elif need:
         workspace, nbytes = torch.empty(need, dtype=torch.uint8, device=q.device), need
-    _call("lr_cache_attention_bf16", q.data_ptr(), q_rs, out.data_ptr(), o_rs, *pool[:7], *tab, _ints(starts, "starts", B + 1),
-          _ints(lens, "lens", B), B, T, max_rows, max_keys, H, HK, _ptr(tree), words, window, sinks, scale, _ptr(workspace),
-          nbytes, _stream())
+        ws = workspace.data_ptr()
+    _call("lr_cache_attention_bf16", q.data_ptr(), q_rs, out.data_ptr(), o_rs, *pool[:7], *tab,
+          _ints(starts, "starts", dev, B + 1), _ints(lens, "lens", dev, B), B, T, max_rows, max_keys, H, HK, tree_ptr, words,
+          window, sinks, scale, ws, nbytes, _raw_stream(dev))
     return out
 
 
 def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
     """lr_cache_copy_pages: page src[i] to page dst[i] (int32 [n] on the device) in every layer of [layers, n_pages, page_size,
     heads, 128] (or one layer's pool). No target may occur twice or be a source."""
+    dev = _device()
     n = src.shape[0]
-    pool = _pool(k_pages, v_pages, layers=True)
+    pool = _pool(k_pages, v_pages, dev, True)
     if dst.shape[0] != n:
         raise ValueError("copy_pages: src and dst of different lengths")
     if n:
-        _call("lr_cache_copy_pages", *pool, _ints(src, "src", n), _ints(dst, "dst", n), n, _stream())
+        _call("lr_cache_copy_pages", *pool, _ints(src, "src", dev, n), _ints(dst, "dst", dev, n), n, _raw_stream(dev))
 
 
 def move_rows(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor,
@@ -224,13 +240,15 @@ def move_rows(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Te
     """lr_cache_move_rows: for the moves starts[b] .. starts[b + 1] of sequence b, its position src[i] to its position dst[i],
     in every layer; a sequence's rows are all read before any is written. max_rows: the most moves of a sequence (at most 256;
     default all of them)."""
+    dev = _device()
     n, B = src.shape[0], starts.shape[0] - 1
-    pool = _pool(k_pages, v_pages, layers=True)
+    pool = _pool(k_pages, v_pages, dev, True)
     if dst.shape[0] != n:
         raise ValueError("move_rows: src and dst of different lengths")
     if n:
-        _call("lr_cache_move_rows", *pool, *_table(page_table, B), _ints(starts, "starts", B + 1), _ints(src, "src", n),
-              _ints(dst, "dst", n), B, n, n if max_rows is None else min(max_rows, n), _stream())
+        _call("lr_cache_move_rows", *pool, *_table(page_table, dev, B), _ints(starts, "starts", dev, B + 1),
+              _ints(src, "src", dev, n), _ints(dst, "dst", dev, n), B, n, n if max_rows is None or max_rows > n else max_rows,
+              _raw_stream(dev))
 
 
 class PagePool:

@@ -47,7 +47,8 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     const int rows = max(sq.n, 0) * a.G;   // (at most 2^30: the host checks)
     if (row0 >= rows) return;
     TileList<BT, PAGED> tl;
-    tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + 32 * RB) - 1, a.G, a.rcp_g), split);
+    tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + 32 * RB) - 1, a.G, a.rcp_g));
+    tl.part(split, a.per);
     const int x0 = tl.x0, x1 = tl.x1;
 
     // ---- this lane's row
@@ -241,7 +242,7 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     const bool broken = live && !(fabsf(chk) < INFINITY);
     if (live) {
         if (a.nsplit > 1) {
-            const int64_t slot = part_slot(a, sq, i, head, split);
+            const int64_t slot = ((int64_t)(sq.t0 + i) * a.H + head) * a.nsplit + split;
             float* po = a.part_o + slot * D + 4 * hf;
             if (m_used > -INFINITY) {
 #pragma unroll
@@ -276,40 +277,21 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     while (again) {
         const int src = __builtin_ctzll(again);
         again &= again - 1;
-        redo_row<BT, PAGED>(a, sq, tl, hk, split, __shfl(i, src, 64), __shfl(head, src, 64));
+        const int ri = __shfl(i, src, 64), rhead = __shfl(head, src, 64);
+        redo_row<BT, PAGED>(a, sq, tl, hk, ri, rhead,
+                            a.nsplit > 1 ? ((int64_t)(sq.t0 + ri) * a.H + rhead) * a.nsplit + split : -1);
     }
 }
 
-// One wave per (token, head): the ranges' parts merged, two dims a lane. A range that saw no key (reference -inf) has left its
-// row unwritten.
+// One wave per (token, head) merges its parts.
 template <bool PAGED>
 __global__ __launch_bounds__(256) void range_merge_kernel(RangeAttnArgs a) {
-    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
+    const int at = blockIdx.x * 4 + (threadIdx.x >> 6);
     const Seq sq = seq_of<PAGED>(a, blockIdx.y);
     if (at >= (int64_t)max(sq.n, 0) * a.H) return;
-    const int head = (int)(at % a.H);
-    const int64_t tok = sq.t0 + at / a.H, r = tok * a.H + head;
-    const float* ml = a.part_ml + r * a.nsplit * 2;
-    const float* po = a.part_o + r * a.nsplit * D + 2 * lane;
-    float M = -INFINITY;
-    for (int s = lane; s < a.nsplit; s += 64) M = fmaxf(M, ml[2 * s]);
-#pragma unroll
-    for (int x = 32; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
-    float L = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    if (M > -INFINITY) {
-        for (int s = 0; s < a.nsplit; ++s) {
-            const float m = ml[2 * s];
-            if (!(m > -INFINITY)) continue;
-            const float w = __builtin_amdgcn_exp2f(m - M);
-            const float2 v = *reinterpret_cast<const float2*>(po + (int64_t)s * D);
-            L = fmaf(w, ml[2 * s + 1], L);
-            o0 = fmaf(w, v.x, o0);
-            o1 = fmaf(w, v.y, o1);
-        }
-    }
-    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-    *reinterpret_cast<uint32_t*>(a.out + tok * a.o_rs + head * D + 2 * lane) = pack_bf16x2(o0 * inv, o1 * inv);
+    const int i = at / a.H, head = at - i * a.H;
+    const int64_t tok = sq.t0 + i;
+    merge_parts(a, (tok * a.H + head) * a.nsplit, a.nsplit, a.out + tok * a.o_rs + head * D);
 }
 
 template <int RB, int KG, int NS>
@@ -326,10 +308,10 @@ hipError_t launch_blocks(const RangeAttnArgs& a, bool paged, hipStream_t stream)
 }  // namespace
 
 hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int wide, hipStream_t stream) {
+    if (wide) return launch_range_wide(a, paged, wide, stream);
     const int64_t rows = (int64_t)(paged ? a.max_rows : a.W) * a.G;
     hipError_t e;
-    if (wide) e = launch_range_wide(a, paged, wide, stream);
-    else if (rows <= 32) e = launch_blocks<1, 4, 2>(a, paged, stream);
+    if (rows <= 32) e = launch_blocks<1, 4, 2>(a, paged, stream);
     else if (rows <= 64) e = launch_blocks<2, 2, 4>(a, paged, stream);
     else e = launch_blocks<4, 2, 4>(a, paged, stream);
     if (e != hipSuccess || a.nsplit <= 1) return e;

@@ -53,6 +53,48 @@ __device__ __forceinline__ int seq_by_length(const RangeAttnArgs& a, int rank) {
     return __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < a.B && before == rank));
 }
 
+// The block of rows of workgroup `id`, its part (0 <= split < nsplit) and its number among the blocks that are cut (-1: whole).
+// Hardware workgroup id runs on XCD id % 8; `idx` is its number there. Rows: an XCD works on whole heads where they divide
+// evenly (the blocks of a head share its keys in the XCD's L2), the last blocks of a head first: without a full window they are
+// the longest; otherwise the heads alternate. Pages: longest sequences first, the blocks of one sequence and head next to each
+// other on one XCD. The first `whole` blocks (of an XCD, or of the launch where the heads do not divide) are not cut.
+template <bool PAGED>
+__device__ __forceinline__ bool block_of(const RangeAttnArgs& a, int id, int& b, int& hk, int& blk, int& split, int& cut) {
+    const bool by_xcd = PAGED || a.HK % 8 == 0;
+    const int xcd = by_xcd ? id & 7 : 0;
+    int idx = by_xcd ? id >> 3 : id;
+    // Workgroups 32 apart of an XCD share a CU: where all of them are resident at once, the second 32 go in the opposite
+    // order, the shortest beside the longest.
+    if (by_xcd && a.nsplit == 1 && a.local <= 64 && idx >= 32) idx = a.local + 31 - idx;
+    split = 0;
+    cut = -1;
+    if (a.nsplit > 1 && idx >= a.whole) {
+        const int at = idx - a.whole, q = div_small(at, a.nsplit, a.rcp_split);
+        split = at - q * a.nsplit;
+        idx = a.whole + q;
+        cut = xcd * (a.local - a.whole) + q;
+    }
+    b = 0;
+    if (by_xcd) {
+        int pair = div_small(idx, a.nblk, a.rcp_nblk);
+        blk = a.nblk - 1 - (idx - pair * a.nblk);
+        if (PAGED) {
+            pair = pair * 8 + xcd;
+            if (pair >= a.B * a.HK) return false;
+            b = div_small(pair, a.HK, a.rcp_hk);
+            hk = pair - b * a.HK;
+            if (a.B > 1 && a.B <= 64) b = seq_by_length(a, b);
+        } else {
+            hk = pair + xcd * (a.HK / 8);
+        }
+    } else {
+        const int at = div_small(idx, a.HK, a.rcp_hk);
+        hk = idx - at * a.HK;
+        blk = a.nblk - 1 - at;
+    }
+    return true;
+}
+
 template <int QW, bool PAGED>
 __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu(2, 2))) void range_wide_kernel(RangeAttnArgs a) {
     constexpr int KBM = 32 * QW;                        // rows per block
@@ -67,48 +109,16 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, hf = lane >> 5;
 
-    // ---- the block. Hardware workgroup b runs on XCD b % 8. Rows: an XCD works on whole heads where they divide evenly (the
-    // blocks of a head share its keys in the XCD's L2), the last blocks of a head first: without a full window they are the
-    // longest. Pages: longest sequences first; the blocks of one sequence and head next to each other on one XCD.
-    const int nblk = a.nblk;
-    int b = 0, hk, blk, split;
-    {
-        const int id = blockIdx.x, xcd = id & 7, per_pair = nblk * a.nsplit, of_xcd = (int)gridDim.x / 8;
-        // Workgroups 32 apart of an XCD share a CU: where all of them are resident at once, the second 32 go in the opposite
-        // order, the shortest beside the longest.
-        int idx = id / 8;
-        if (of_xcd <= 64 && idx >= 32) idx = of_xcd + 31 - idx;
-        int pair, at;
-        if (PAGED) {
-            pair = div_small(idx, per_pair, a.rcp_pair);
-            at = idx - pair * per_pair;
-            pair = pair * 8 + xcd;
-            if (pair >= a.B * a.HK) return;
-        } else if (a.HK % 8 == 0) {
-            pair = div_small(idx, per_pair, a.rcp_pair);
-            at = idx - pair * per_pair;
-            pair += xcd * (a.HK / 8);
-        } else {
-            at = div_small(id, a.HK, a.rcp_hk);
-            pair = id - at * a.HK;
-        }
-        hk = pair;
-        if (PAGED) {
-            b = div_small(pair, a.HK, a.rcp_hk);
-            hk = pair - b * a.HK;
-            if (a.B > 1 && a.B <= 64) b = seq_by_length(a, b);
-        }
-        blk = div_small(at, a.nsplit, a.rcp_split);
-        split = at - blk * a.nsplit;
-        blk = nblk - 1 - blk;
-    }
+    int b, hk, blk, split, cut;
+    if (!block_of<PAGED>(a, blockIdx.x, b, hk, blk, split, cut)) return;
     b = __builtin_amdgcn_readfirstlane(b);
     const Seq sq = seq_of<PAGED>(a, b);
     const int row0 = blk * KBM;
     const int rows = max(sq.n, 0) * a.G;   // (at most 2^30: the host checks)
     if (row0 >= rows) return;
     TileList<BT, PAGED> tl;
-    tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + KBM) - 1, a.G, a.rcp_g), split);
+    tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + KBM) - 1, a.G, a.rcp_g));
+    if (cut >= 0) tl.part(split, a.per ? a.per : div_small(tl.total + a.nsplit - 1, a.nsplit, a.rcp_split));
     const bool bad = tl.template stage<64 * QW>(a, b, staged);
     const int x0 = tl.x0, x1 = tl.x1;
 
@@ -117,10 +127,12 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     const bool live = r < rows;
     const int i = div_small(rr, a.G, a.rcp_g), head = hk * a.G + rr - i * a.G;
     const Sees me = sees_of<PAGED>(a, sq, i);
+    // its slot among the parts
+    auto slot_of = [&](int q) __attribute__((always_inline)) { return ((int64_t)cut * KBM + q) * a.nsplit + split; };
     if (x0 >= x1) {   // nothing to see in this part
         if (live) {
-            if (a.nsplit > 1) {
-                const int64_t at = part_slot(a, sq, i, head, split);
+            if (cut >= 0) {
+                const int64_t at = slot_of(32 * wv + n);
                 if (hf == 0) a.part_ml[2 * at] = -INFINITY;
                 else a.part_ml[2 * at + 1] = 0.0f;
             } else {
@@ -409,9 +421,9 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         for (int e = 0; e < 16; ++e) nan = fmaf(0.0f, o[db][e], nan);
     uint64_t again = __builtin_amdgcn_ballot_w64(nan != 0.0f && live);
     again = (again | again >> 32) & 0xffffffffu;
-    if (a.nsplit > 1) {
+    if (cut >= 0) {
         if (live) {
-            const int64_t at = part_slot(a, sq, i, head, split);
+            const int64_t at = slot_of(32 * wv + n);
             float* po = a.part_o + at * D + 4 * hf;
 #pragma unroll
             for (int db = 0; db < 4; ++db)
@@ -447,28 +459,46 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     while (again) {
         const int q = __builtin_ctzll(again);
         again &= again - 1;
-        redo_row<BT, PAGED>(a, sq, tl, hk, split, __builtin_amdgcn_readlane(i, q), __builtin_amdgcn_readlane(head, q));
+        redo_row<BT, PAGED>(a, sq, tl, hk, __builtin_amdgcn_readlane(i, q), __builtin_amdgcn_readlane(head, q),
+                            cut >= 0 ? slot_of(32 * wv + q) : -1);
     }
 }
 
-template <int QW>
-hipError_t launch_waves(const RangeAttnArgs& a, bool paged, hipStream_t stream) {
-    RangeAttnArgs w = a;
-    const int64_t nblk = ((int64_t)(paged ? a.max_rows : a.W) * a.G + 32 * QW - 1) / (32 * QW);
-    const int64_t pairs = paged ? ((int64_t)a.B * a.HK + 7) / 8 * 8 : a.HK;
-    const int64_t blocks = nblk * a.nsplit * pairs;
-    if (blocks > 1 << 22) return hipErrorInvalidValue;   // (a grid's work-items are counted in 32 bits)
-    w.nblk = (int)nblk;
-    w.rcp_pair = rcp_small(nblk * a.nsplit);
-    if (paged) hipLaunchKernelGGL((range_wide_kernel<QW, true>), dim3((unsigned)blocks), dim3(64 * QW), 0, stream, w);
-    else hipLaunchKernelGGL((range_wide_kernel<QW, false>), dim3((unsigned)blocks), dim3(64 * QW), 0, stream, w);
+// The parts of the blocks that were cut, a wave a row: workgroup (cut block, four rows).
+template <int KBM, bool PAGED>
+__global__ __launch_bounds__(256) void range_wide_merge_kernel(RangeAttnArgs a) {
+    const int c = blockIdx.x / (KBM / 4), q = blockIdx.x % (KBM / 4) * 4 + (threadIdx.x >> 6);
+    const int of = a.local - a.whole;   // cut blocks an XCD
+    const bool by_xcd = PAGED || a.HK % 8 == 0;
+    const int xcd = by_xcd ? c / of : 0, first = a.whole + (c - xcd * of) * a.nsplit;   // the block's first workgroup
+    int b, hk, blk, split, cut;
+    if (!block_of<PAGED>(a, by_xcd ? 8 * first + xcd : first, b, hk, blk, split, cut)) return;
+    b = __builtin_amdgcn_readfirstlane(b);
+    const Seq sq = seq_of<PAGED>(a, b);
+    const int r = blk * KBM + q;
+    if (r >= max(sq.n, 0) * a.G) return;
+    const int i = div_small(r, a.G, a.rcp_g), head = hk * a.G + r - i * a.G;
+    merge_parts(a, ((int64_t)cut * KBM + q) * a.nsplit, a.nsplit, a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D);
+}
+
+template <int QW, bool PAGED>
+hipError_t launch_waves(const RangeAttnArgs& a, hipStream_t stream) {
+    const int xcds = PAGED || a.HK % 8 == 0 ? 8 : 1;
+    const int64_t of = a.nsplit > 1 ? a.local - a.whole : 0;   // cut blocks
+    const int64_t blocks = xcds * (a.local + of * (a.nsplit - 1)), merge = xcds * of * (8 * QW);
+    if (blocks > 1 << 22 || merge > 1 << 23) return hipErrorInvalidValue;   // (a grid's work-items are counted in 32 bits)
+    hipLaunchKernelGGL((range_wide_kernel<QW, PAGED>), dim3((unsigned)blocks), dim3(64 * QW), 0, stream, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || of == 0) return e;
+    hipLaunchKernelGGL((range_wide_merge_kernel<32 * QW, PAGED>), dim3((unsigned)merge), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, int waves, hipStream_t stream) {
-    return waves == 8 ? launch_waves<8>(a, paged, stream) : launch_waves<4>(a, paged, stream);
+    if (waves == 8) return paged ? launch_waves<8, true>(a, stream) : launch_waves<8, false>(a, stream);
+    return paged ? launch_waves<4, true>(a, stream) : launch_waves<4, false>(a, stream);
 }
 
 }  // namespace lr

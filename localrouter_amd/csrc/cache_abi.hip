@@ -47,49 +47,97 @@ lr::PageArgs page_args(int64_t page, int64_t row, int64_t head, int n_pages, int
 }
 
 // ------------------------------------------------------------------------------------------------ range attention
-// How a call is cut: the kernel (wide: 0, or the waves of the kernel of attn_cache_wide.hip), and over the keys, nsplit parts
-// of `per` key tiles.
+// How a call is cut: the kernel (wide: 0, or the waves of the kernel of attn_cache_wide.hip) and its blocks over the keys
+// (RangeAttnArgs: nsplit, per, whole, local, nblk), and the rows of the parts.
 struct Cut {
-    int wide, nsplit, per;
+    int wide, nsplit, per, whole, local, nblk;
+    int64_t part_rows;
 };
-int64_t block_rows(int64_t rows, int wide) { return wide ? 32 * wide : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
-// rows of a kv head a sequence; pairs: sequences x kv heads; keys: the most positions of a sequence; span: the most that a
-// block of rows needs of them beside the first `sinks`.
-Cut cut_of(bool wide, int64_t rows, int64_t pairs, int64_t keys, int64_t span, int64_t sinks, int page_size) {
-    const int bt = wide ? lr::RANGE_WIDE_TILE : lr::RANGE_TILE, entries = wide ? lr::RANGE_WIDE_STAGED : lr::RANGE_STAGED;
-    const int64_t tiles = std::min((keys + bt - 1) / bt, (std::min(sinks, keys) + bt - 1) / bt + span / bt + 2);
-    const int64_t big = (rows + 255) / 256 * pairs;
-    const int waves = !wide ? 0 : tiles >= 64 && big >= 256 && (big % 256 == 0 || big >= 1024) ? 8 : 4;
-    const int64_t br = block_rows(rows, waves), base = (rows + br - 1) / br * pairs;
-    const int64_t staged = page_size ? entries / std::max(1, bt / page_size) : INT_MAX;
-    int64_t ns = std::min(std::max<int64_t>(1, (wide ? 256 : 512) / base), std::max<int64_t>(1, tiles / 8));
+// The most key tiles of bt keys that a block of rows needs: of `span` keys beside the first `sinks`, of `keys` in all.
+int64_t tiles_of(int64_t keys, int64_t span, int64_t sinks, int bt) {
+    return std::min((keys + bt - 1) / bt, (std::min(sinks, keys) + bt - 1) / bt + span / bt + 2);
+}
+
+// attn_cache.hip: every block in parts of `per` tiles. rows of a kv head a sequence; pairs: sequences x kv heads; tokens x heads
+// of the call.
+Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int64_t token_rows, int page_size) {
+    const int64_t br = rows <= 32 ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
+    const int64_t staged = page_size ? lr::RANGE_STAGED / std::max(1, lr::RANGE_TILE / page_size) : INT_MAX;
+    int64_t ns = std::min(std::max<int64_t>(1, 512 / base), std::max<int64_t>(1, tiles / 8));
     const int64_t per = std::max<int64_t>(1, std::min((tiles + ns - 1) / ns, staged));
     ns = std::max<int64_t>(1, (tiles + per - 1) / per);
-    return Cut{waves, (int)ns, (int)per};
+    Cut c{};
+    c.nsplit = (int)ns; c.per = (int)per;
+    c.part_rows = ns > 1 ? token_rows * ns : 0;
+    return c;
 }
+
+// attn_cache_wide.hip. Two workgroups of 4 waves are resident on a CU, 64 on an XCD. Where the last round of them is not full,
+// its blocks may be cut: a block alone on its CU takes ~1.1 us a tile, beside another 1.8, and parts cost a launch (~6 us) and
+// their rows written and read (2,319 tokens x 32 heads over 8, 512 + 72 blocks, windows of 1,024, 2,048 and 8,192: 66.6, 114 and 400
+// us uncut, .
+Cut cut_wide(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool by_xcd) {
+    const int64_t big = (rows + 255) / 256 * pairs;
+    Cut c{};
+    // 8 waves: half the keys and values moved into LDS. Long ranges that fill the rounds of 256 such workgroups (us, 8 / 4
+    // waves: 4,096 tokens x 32 heads, windows of 8,192 and 1,024 tokens 493 / 511 and 100 / 92; 3,000 x 32, 1.5 rounds, 91 / 82).
+    c.wide = tiles >= 64 && big >= 256 && (big % 256 == 0 || big >= 1024) ? 8 : 4;
+    const int br = 32 * c.wide, xcds = by_xcd ? 8 : 1, round = (c.wide == 8 ? 256 : 512) / xcds;
+    c.nblk = (int)((rows + br - 1) / br);
+    c.local = (int)((pairs + xcds - 1) / xcds * c.nblk);
+    c.whole = c.local;
+    c.nsplit = 1;
+    const int64_t staged = page_size ? lr::RANGE_WIDE_STAGED / std::max(1, lr::RANGE_WIDE_TILE / page_size) : INT_MAX;
+    int64_t tail = c.local % round, ns = 1;
+    // (under pages the lengths are the device's: only launches of less than a round are cut, into parts of a fixed length)
+    if (page_size && c.local > round) tail = 0;
+    if (tail) {
+        auto cost = [&](int64_t n) {
+            return (double)((tiles + n - 1) / n) * (2 * tail * n <= round ? 1.1 : 1.8) +
+                   (n > 1 ? 6.0 + 2.0 * (double)(tail * xcds * br * n) * lr::D * 4 / 5e6 : 0.0);
+        };
+        for (int64_t n = 2; n <= std::min<int64_t>(std::min(round / tail, tiles / 2), 64); ++n)
+            if (cost(n) < cost(ns)) ns = n;
+    }
+    if (page_size) {
+        const int64_t per = std::max<int64_t>(1, std::min((tiles + ns - 1) / ns, staged));
+        ns = std::max<int64_t>(1, (tiles + per - 1) / per);
+        c.per = (int)per;
+        tail = c.local;
+    }
+    if (ns > 1) {
+        c.nsplit = (int)ns;
+        c.whole = (int)(c.local - tail);
+        c.part_rows = tail * xcds * br * ns;
+    }
+    return c;
+}
+
 Cut window_cut(int W, int H, int HK, int nkeys, int window, int sinks, int frame, bool narrow) {
-    const int64_t rows = (int64_t)W * (H / HK);
-    const int64_t tokens = std::min<int64_t>(W, 128 / (H / HK) + 2);
+    const int64_t rows = (int64_t)W * (H / HK), tokens = std::min<int64_t>(W, 256 / (H / HK) + 2);
     const int64_t span = (window + 2) * (int64_t)frame + tokens;
-    return cut_of(narrow && rows > 64, rows, HK, nkeys, span, sinks, 0);
+    if (narrow && rows > 64) return cut_wide(rows, HK, tiles_of(nkeys, span, sinks, lr::RANGE_WIDE_TILE), 0, HK % 8 == 0);
+    return cut_small(rows, HK, tiles_of(nkeys, span, sinks, lr::RANGE_TILE), (int64_t)W * H, 0);
 }
-Cut cache_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks, bool narrow) {
-    const int64_t rows = (int64_t)max_rows * (H / HK);
+Cut cache_cut(int B, int T, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks, bool narrow) {
+    const int64_t rows = (int64_t)max_rows * (H / HK), pairs = (int64_t)B * HK;
     const int64_t span = window ? (int64_t)window + max_rows + 1 : max_keys;
-    return cut_of(narrow && rows > 64 && page_size >= lr::RANGE_WIDE_MIN_PAGE, rows, (int64_t)B * HK, max_keys, span, sinks, page_size);
+    if (narrow && rows > 64 && page_size >= lr::RANGE_WIDE_MIN_PAGE)
+        return cut_wide(rows, pairs, tiles_of(max_keys, span, sinks, lr::RANGE_WIDE_TILE), page_size, true);
+    return cut_small(rows, pairs, tiles_of(max_keys, span, sinks, lr::RANGE_TILE), (int64_t)T * H, page_size);
 }
-size_t part_bytes(int64_t rows, int nsplit) {
-    return nsplit <= 1 ? 0 : (((size_t)rows * nsplit * lr::D * 4 + 255) & ~(size_t)255) + (((size_t)rows * nsplit * 8 + 255) & ~(size_t)255);
+size_t part_bytes(const Cut& c) {
+    return (((size_t)c.part_rows * lr::D * 4 + 255) & ~(size_t)255) + (((size_t)c.part_rows * 8 + 255) & ~(size_t)255);
 }
-void set_parts(lr::RangeAttnArgs& a, void* ws, int64_t rows, Cut cut) {
-    a.nsplit = cut.nsplit;
-    a.rcp_split = lr::rcp_small(cut.nsplit);
+void set_cut(lr::RangeAttnArgs& a, void* ws, const Cut& c) {
+    a.nsplit = c.nsplit; a.per = c.per; a.whole = c.whole; a.local = c.local; a.nblk = c.nblk;
+    a.rcp_split = lr::rcp_small(c.nsplit);
+    a.rcp_nblk = lr::rcp_small(c.nblk);
     a.rcp_g = lr::rcp_small(a.G);
     a.rcp_hk = lr::rcp_small(a.HK);
-    a.tiles_per_split = cut.per;
     a.part_o = static_cast<float*>(ws);
-    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + (((size_t)rows * cut.nsplit * lr::D * 4 + 255) & ~(size_t)255));
+    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + (((size_t)c.part_rows * lr::D * 4 + 255) & ~(size_t)255));
 }
 
 bool window_sizes_ok(int W, int H, int HK, int nkeys, int window, int sinks, int frame) {
@@ -108,8 +156,8 @@ extern "C" {
 
 size_t lr_attention_window_ws_bytes(int W, int H, int HK, int nkeys, int window, int sinks, int frame) {
     if (!window_sizes_ok(W, H, HK, nkeys, window, sinks, frame)) return 0;
-    return std::max(part_bytes((int64_t)W * H, window_cut(W, H, HK, nkeys, window, sinks, frame, true).nsplit),
-                    part_bytes((int64_t)W * H, window_cut(W, H, HK, nkeys, window, sinks, frame, false).nsplit));
+    return std::max(part_bytes(window_cut(W, H, HK, nkeys, window, sinks, frame, true)),
+                    part_bytes(window_cut(W, H, HK, nkeys, window, sinks, frame, false)));
 }
 
 int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* out, int p0, int W, int H, int HK, int nkeys,
@@ -127,7 +175,7 @@ int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* 
     lr::RangeAttnArgs a{};
     const bool narrow = k_row_stride < lr::RANGE_WIDE_MAX_RS && v_row_stride < lr::RANGE_WIDE_MAX_RS;
     const Cut cut = window_cut(W, H, HK, nkeys, window, sinks, frame, narrow);
-    const size_t need = part_bytes((int64_t)W * H, cut.nsplit);
+    const size_t need = part_bytes(cut);
     if (need) {
         if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return ERR_ARGS;
         const uintptr_t lo = reinterpret_cast<uintptr_t>(workspace);
@@ -141,7 +189,7 @@ int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* 
     a.q_rs = q_row_stride; a.k_rs = k_row_stride; a.v_rs = v_row_stride; a.o_rs = out_row_stride;
     a.H = H; a.HK = HK; a.G = H / HK;
     a.c = scale * 1.4426950408889634f;
-    set_parts(a, workspace, (int64_t)W * H, cut);
+    set_cut(a, workspace, cut);
     a.W = W; a.p0 = p0; a.nkeys = nkeys; a.frame = std::min(frame, MAX_POS);   // (positions are below it either way)
     a.rcp_frame = lr::rcp_small(a.frame);
     a.window = std::min(window, MAX_POS); a.sinks = std::min(sinks, MAX_POS);
@@ -151,8 +199,8 @@ int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* 
 size_t lr_cache_attention_ws_bytes(int B, int T, int max_rows, int max_keys, int H, int HK, int page_size, int window,
                                    int sinks) {
     if (!cache_sizes_ok(B, T, max_rows, max_keys, H, HK, page_size, window, sinks)) return 0;
-    return std::max(part_bytes((int64_t)T * H, cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks, true).nsplit),
-                    part_bytes((int64_t)T * H, cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks, false).nsplit));
+    return std::max(part_bytes(cache_cut(B, T, max_rows, max_keys, H, HK, page_size, window, sinks, true)),
+                    part_bytes(cache_cut(B, T, max_rows, max_keys, H, HK, page_size, window, sinks, false)));
 }
 
 int lr_cache_attention_bf16(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride, const void* k_pages,
@@ -173,8 +221,8 @@ int lr_cache_attention_bf16(const void* q, int64_t q_row_stride, void* out, int6
     if (overlap(so, sq) || overlap(so, sk) || overlap(so, sv)) return ERR_ARGS;
     lr::RangeAttnArgs a{};
     const bool narrow = row_stride < lr::RANGE_WIDE_MAX_RS && (page_size > lr::RANGE_WIDE_MIN_PAGE || sk.hi - sk.lo < (1ull << 32));
-    const Cut cut = cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks, narrow);
-    const size_t need = part_bytes((int64_t)T * H, cut.nsplit);
+    const Cut cut = cache_cut(B, T, max_rows, max_keys, H, HK, page_size, window, sinks, narrow);
+    const size_t need = part_bytes(cut);
     if (need) {
         if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return ERR_ARGS;
         const uintptr_t lo = reinterpret_cast<uintptr_t>(workspace);
@@ -189,7 +237,7 @@ int lr_cache_attention_bf16(const void* q, int64_t q_row_stride, void* out, int6
     a.H = H; a.HK = HK; a.G = H / HK;
     a.c = scale * 1.4426950408889634f;
     a.pg = page_args(page_stride, row_stride, head_stride, n_pages, page_size, page_table, table_stride, table_pages);
-    set_parts(a, workspace, (int64_t)T * H, cut);
+    set_cut(a, workspace, cut);
     a.starts = starts; a.lens = lens; a.tree = tree; a.words = tree ? words : 0;
     a.B = B; a.T = T; a.max_rows = max_rows; a.max_keys = max_keys;
     a.window = std::min(window, MAX_POS); a.sinks = window ? std::min(sinks, MAX_POS) : 0;

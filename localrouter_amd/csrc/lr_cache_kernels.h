@@ -39,13 +39,16 @@ struct RangeAttnArgs {
     const uint64_t* tree;   // [T][words]: bit x of a token's words: it sees the sequence's drafted token x; null: chains
     int B, T, max_rows, max_keys, words;
     int window, sinks;      // window 0 (pages only): every earlier key
-    // Split over the keys: nsplit > 1 runs every block of rows as nsplit workgroups of tiles_per_split key tiles each; the
-    // ranges' unnormalised rows, references and sums go to the parts, [token][head][split], merged by a second launch.
-    int nsplit, tiles_per_split;
+    // Split over the keys: with nsplit > 1 a block of rows is nsplit workgroups, each a part of its key tiles, whose unnormalised
+    // rows, references and sums go to the parts (fp32 [slot][128] and [slot][2]), merged by a second launch. attn_cache.hip: every
+    // block, `per` tiles a part, slots [token][head][part]. attn_cache_wide.hip: the blocks from number `whole` on, in the order
+    // in which an XCD's workgroups start (`local` blocks an XCD, or in all: see its kernel), `per` tiles a part or, per 0, equal
+    // parts; slots [block][row][part].
+    int nsplit, per, whole, local;
     float* part_o;
     float* part_ml;
-    // rcp_small of the divisors; nblk (and rcp_pair, of nblk * nsplit): blocks of rows a sequence and kv head, set by the launch
-    uint32_t rcp_g, rcp_hk, rcp_frame, rcp_split, rcp_pair;
+    // rcp_small of the divisors; nblk: blocks of rows a sequence and kv head
+    uint32_t rcp_g, rcp_hk, rcp_frame, rcp_split, rcp_nblk;
     int nblk;
 };
 
