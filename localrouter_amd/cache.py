@@ -42,7 +42,7 @@ SIGNATURES = {
 _bound = None
 _BF16, _I32, _I64T, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
 # (looked up once: a small call's ~10 us are mostly its checks)
-_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_current, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def lib() -> ctypes.CDLL:
@@ -54,6 +54,13 @@ def lib() -> ctypes.CDLL:
             fn.restype, fn.argtypes = res, args
         _bound = L
     return _bound
+
+
+def _device(t: torch.Tensor) -> int:
+    """The current device; a host tensor is refused (there may be no device to ask)."""
+    if not t.is_cuda:
+        raise ValueError(f"expected tensors on the GPU, got one on {t.device}")
+    return _current()
 
 
 def _call(name: str, *args) -> None:
@@ -119,7 +126,7 @@ def append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: to
     normalised and rotated into q_out (allocated when None; q itself is allowed), keys the same way into their pages, values
     as they are. table = (table_a, table_b), one row a position; positions int32 [T]: each token's table row (default its
     position in its sequence). q None: keys and values only. Returns q_out."""
-    dev = _device()
+    dev = _device(k_pages)
     pool = _pool(k_pages, v_pages, dev)
     HK = pool[7]
     T, B = k.shape[0], lens.shape[0]
@@ -187,7 +194,7 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     positions (under a tree: those before the call's tokens) only where p - j < n or j < sinks. max_rows: the most tokens of a
     sequence (default T); max_keys: the longest sequence (default what the table holds). A workspace of attention_ws_bytes is
     allocated when none is given."""
-    dev = _device()
+    dev = _device(q)
     T, H = q.shape[0], q.shape[1]
     B = lens.shape[0]
     q_rs = _rows(q, "q", dev, T, H)
@@ -226,7 +233,7 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
 def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
     """lr_cache_copy_pages: page src[i] to page dst[i] (int32 [n] on the device) in every layer of [layers, n_pages, page_size,
     heads, 128] (or one layer's pool). No target may occur twice or be a source."""
-    dev = _device()
+    dev = _device(k_pages)
     n = src.shape[0]
     pool = _pool(k_pages, v_pages, dev, True)
     if dst.shape[0] != n:
@@ -240,7 +247,7 @@ def move_rows(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Te
     """lr_cache_move_rows: for the moves starts[b] .. starts[b + 1] of sequence b, its position src[i] to its position dst[i],
     in every layer; a sequence's rows are all read before any is written. max_rows: the most moves of a sequence (at most 256;
     default all of them)."""
-    dev = _device()
+    dev = _device(k_pages)
     n, B = src.shape[0], starts.shape[0] - 1
     pool = _pool(k_pages, v_pages, dev, True)
     if dst.shape[0] != n:

@@ -24,12 +24,14 @@ namespace {
 
 #include "range_attn.inc"
 
+constexpr uint64_t PART_DONE = 0x7ff4a3c57fb5d96e;
+
 template <int RB, int KG, int NS, bool PAGED>
 __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(RangeAttnArgs a) {
     constexpr int BT = RANGE_TILE, TILE = BT * D, NW = RB * KG;
     constexpr int LOADS = 8 / RB;   // direct loads (4 rows each) per wave per K or V tile
     typedef __attribute__((address_space(3))) i16x4_t lds_i16x4;
-    constexpr int RING = KG * NS * TILE * 2 * 2, MERGE = (KG - 1) * RB * (64 * 64 + 2 * 64) * 4;
+    constexpr int RING = KG * NS * TILE * 2 * 2, MERGE = KG * RB * (64 * 64 + 2 * 64) * 4;
     __shared__ __attribute__((aligned(1024))) char ring[RING > MERGE ? RING : MERGE];
     __shared__ int staged[PAGED ? RANGE_STAGED : 1];
 
@@ -49,6 +51,8 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     TileList<BT, PAGED> tl;
     tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + 32 * RB) - 1, a.G, a.rcp_g));
     tl.part(split, a.per);
+    const int parts = max(1, (tl.total + a.per - 1) / a.per);   // of this block: the sequence may be shorter than the longest
+    if (split >= parts) return;
     const int x0 = tl.x0, x1 = tl.x1;
 
     // ---- this lane's row
@@ -62,26 +66,7 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
 
     const int64_t k_rs = PAGED ? a.pg.rs : a.k_rs, v_rs = PAGED ? a.pg.rs : a.v_rs;
     const int64_t hoff = (int64_t)hk * (PAGED ? a.pg.hs : D);
-    const bool bad = tl.template stage<NW * 64>(a, b, staged);
-
-    // ---- direct loads of a tile: instruction u fills rows 4u .. 4u + 3, swizzled as attn_fwd.hip's
-    const int lrow = lane >> 4, lchunk = lane & 15;
-    const uint32_t kr_lds = lds_addr(ring) + kg * NS * TILE * 4, vr_lds = kr_lds + NS * TILE * 2;
-    auto load_tile = [&](int x, int slot) {
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-            const int inst = rb + RB * u, row = 4 * inst + lrow;
-            const int64_t o = tl.offset(a, x, row, k_rs);
-            dma16(a.k + hoff + o + 8 * (lchunk ^ (row & 15)), kr_lds + 2 * (slot * TILE + 512 * inst));
-            const int64_t ov = PAGED ? o : tl.offset(a, x, row, v_rs);
-            dma16(a.v + hoff + ov + 8 * (lchunk ^ (lrow << 2)), vr_lds + 2 * (slot * TILE + 512 * inst));
-        }
-    };
-
-    const int mine = x1 > x0 + kg ? (x1 - x0 - kg + KG - 1) / KG : 0;   // tiles of this group
-    const int steps = x1 > x0 ? (x1 - x0 + KG - 1) / KG : 0;             // of group 0: every group's barriers
-    auto tile_of = [&](int t) { return x0 + kg + t * KG; };
-
+    // (the queries first: under pages they arrive while the table's entries are waited for)
     bf16x8 qf[8];
     {
         const uint16_t* src = a.q + (int64_t)(sq.t0 + i) * a.q_rs + head * D + 8 * hf;
@@ -92,7 +77,43 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
             qf[ks] = __builtin_bit_cast(bf16x8, w);
         }
     }
-    LR_WAIT_VMCNT(0);
+    const bool bad = tl.template stage<NW * 64>(a, b, staged);
+
+    // ---- direct loads of a tile: instruction u fills rows 4u .. 4u + 3, swizzled as attn_fwd.hip's
+    const int lrow = lane >> 4, lchunk = lane & 15;
+    const uint32_t kr_lds = lds_addr(ring) + kg * NS * TILE * 4, vr_lds = kr_lds + NS * TILE * 2;
+    const bool runs = !PAGED || tl.shift >= 5;   // a whole tile's rows are one run
+    auto load_tile = [&](int x, int slot) {
+        const int key0 = tl.key0(x);
+        const uint16_t *kp = a.k + hoff, *vp = a.v + hoff;
+        if (runs && key0 + BT <= sq.end) {
+            const int64_t row = (PAGED ? key0 & ((1 << tl.shift) - 1) : key0) + 4 * rb + lrow;
+            const int64_t pg = PAGED ? (int64_t)max(tl.entry(x, 0), 0) * a.pg.ps : 0;
+            kp += pg + row * k_rs;
+            vp += pg + row * v_rs + 8 * (lchunk ^ (lrow << 2));
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u) {
+                const int inst = rb + RB * u;
+                dma16(kp + 8 * (lchunk ^ ((4 * inst + lrow) & 15)), kr_lds + 2 * (slot * TILE + 512 * inst));
+                dma16(vp, vr_lds + 2 * (slot * TILE + 512 * inst));
+                kp += 4 * RB * k_rs;
+                vp += 4 * RB * v_rs;
+            }
+            return;
+        }
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int inst = rb + RB * u, row = 4 * inst + lrow;
+            const int64_t o = tl.offset(a, x, row, k_rs), ov = PAGED ? o : tl.offset(a, x, row, v_rs);
+            dma16(kp + o + 8 * (lchunk ^ (row & 15)), kr_lds + 2 * (slot * TILE + 512 * inst));
+            dma16(vp + ov + 8 * (lchunk ^ (lrow << 2)), vr_lds + 2 * (slot * TILE + 512 * inst));
+        }
+    };
+
+    const int mine = x1 > x0 + kg ? (x1 - x0 - kg + KG - 1) / KG : 0;   // tiles of this group
+    const int steps = x1 > x0 ? (x1 - x0 + KG - 1) / KG : 0;             // of group 0: every group's barriers
+    auto tile_of = [&](int t) { return x0 + kg + t * KG; };
+
     constexpr int AHEAD = RB == 1 ? NS : NS - 1;   // tiles in flight before the first step
     for (int t = 0; t < AHEAD && t < mine; ++t) load_tile(tile_of(t), t);
 
@@ -185,113 +206,171 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
         }
     }
 
-    // ---- merge the key groups in group 0
+    // ---- merge the key groups: group u takes the 32-dim blocks u, u + KG, ... of its rows from all of them
+    static_assert(KG > 1 && 4 % KG == 0, "groups");
+    constexpr int OWN = 4 / KG;   // blocks a group
     float l = wave_pair_sum(l_sum);
-    if constexpr (KG > 1) {
+    float own[OWN][16];
+    {
         __syncthreads();
         float* mo = reinterpret_cast<float*>(ring);
-        float* mml = mo + (KG - 1) * RB * 64 * 64;
-        if (kg > 0) {
-            const int at = (kg - 1) * RB + rb;
+        float* mml = mo + KG * RB * 64 * 64;
 #pragma unroll
-            for (int db = 0; db < 4; ++db)
+        for (int db = 0; db < 4; ++db)
+            if (db % KG != kg)
 #pragma unroll
                 for (int q4 = 0; q4 < 4; ++q4)
-                    *reinterpret_cast<f32x4*>(mo + (at * 16 + 4 * db + q4) * 256 + 4 * lane) =
+                    *reinterpret_cast<f32x4*>(mo + ((kg * RB + rb) * 16 + 4 * db + q4) * 256 + 4 * lane) =
                         f32x4{o[db][4 * q4], o[db][4 * q4 + 1], o[db][4 * q4 + 2], o[db][4 * q4 + 3]};
-            mml[at * 128 + lane] = m_used;
-            mml[at * 128 + 64 + lane] = l;
-        }
+        *reinterpret_cast<float2*>(mml + (kg * RB + rb) * 128 + 2 * lane) = float2{m_used, l};
         __syncthreads();
-        if (kg > 0) return;
-        float ms[KG], mm = m_used;
+        float mm = -INFINITY, w[KG];
+        float2 ml[KG];
 #pragma unroll
-        for (int u = 1; u < KG; ++u) {
-            ms[u] = mml[((u - 1) * RB + rb) * 128 + lane];
-            mm = fmaxf(mm, ms[u]);
+        for (int u = 0; u < KG; ++u) {
+            ml[u] = *reinterpret_cast<const float2*>(mml + (u * RB + rb) * 128 + 2 * lane);
+            mm = fmaxf(mm, ml[u].x);
         }
         const float ref = mm > -INFINITY ? mm : 0.0f;
-        const float w0 = __builtin_amdgcn_exp2f(m_used - ref);
-        l *= w0;
+        l = 0.0f;
 #pragma unroll
-        for (int db = 0; db < 4; ++db) o[db] *= w0;
-#pragma unroll
-        for (int u = 1; u < KG; ++u) {
-            const int at = (u - 1) * RB + rb;
-            const float w = __builtin_amdgcn_exp2f(ms[u] - ref);
-            l = fmaf(w, mml[at * 128 + 64 + lane], l);
-#pragma unroll
-            for (int db = 0; db < 4; ++db)
-#pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(mo + (at * 16 + 4 * db + q4) * 256 + 4 * lane);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[db][4 * q4 + e] = fmaf(w, x[e], o[db][4 * q4 + e]);
-                }
+        for (int u = 0; u < KG; ++u) {
+            w[u] = __builtin_amdgcn_exp2f(ml[u].x - ref);
+            l = fmaf(w[u], ml[u].y, l);
         }
         m_used = mm;
+        // (in the groups' order, whichever group it is)
+#pragma unroll
+        for (int x = 0; x < OWN; ++x)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                f32x4 sum{};
+#pragma unroll
+                for (int u = 0; u < KG; ++u) {
+                    f32x4 y;
+                    if (u == kg) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            y[e] = 0.0f;
+#pragma unroll
+                            for (int g2 = 0; g2 < KG; ++g2) y[e] = g2 == kg ? o[g2 + KG * x][4 * q4 + e] : y[e];
+                        }
+                    } else {
+                        y = *reinterpret_cast<const f32x4*>(mo + ((u * RB + rb) * 16 + 4 * (kg + KG * x) + q4) * 256 + 4 * lane);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[e] = fmaf(w[u], y[e], sum[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) own[x][4 * q4 + e] = sum[e];
+            }
     }
-    if (!any) return;
 
-    // ---- rows out: O / l, or this range's part
-    float chk = l;
+    // ---- rows out: O / l, or this part of them
+    constexpr int BR = 32 * RB;
+    const bool whole_block = parts == 1;
+    const int64_t block = ((int64_t)b * a.nblk + blk) * a.HK + hk;
+    // (sc1: coherent at device scope, not kept in this XCD's L2; the last workgroup of the block may run on another)
+    const __amdgpu_buffer_rsrc_t rs_o = __builtin_amdgcn_make_buffer_rsrc(a.part_o + block * a.nsplit * BR * D, 0, a.nsplit * BR * D * 4, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rs_ml = __builtin_amdgcn_make_buffer_rsrc(a.part_ml + block * a.nsplit * BR * 2, 0, a.nsplit * BR * 8, 0x00020000);
+    auto put_part = [&](int q, float m, float ps) {
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(ps)}, rs_ml, (split * BR + q) * 8, 0, 16);
+    };
+    uint64_t bits = 0;
+    // (dims of block x of this group's, quarter q4: 32 (kg + KG x) + 8 q4 + 4 hf .. + 3)
+    if (any) {
+        float chk = l;
 #pragma unroll
-    for (int db = 0; db < 4; ++db)
+        for (int x = 0; x < OWN; ++x)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) chk = fmaf(0.0f, o[db][e], chk);
-    const bool broken = live && !(fabsf(chk) < INFINITY);
-    if (live) {
-        if (a.nsplit > 1) {
-            const int64_t slot = ((int64_t)(sq.t0 + i) * a.H + head) * a.nsplit + split;
-            float* po = a.part_o + slot * D + 4 * hf;
-            if (m_used > -INFINITY) {
-#pragma unroll
-                for (int db = 0; db < 4; ++db)
-#pragma unroll
-                    for (int q4 = 0; q4 < 4; ++q4)
-                        *reinterpret_cast<f32x4*>(po + 32 * db + 8 * q4) =
-                            f32x4{o[db][4 * q4], o[db][4 * q4 + 1], o[db][4 * q4 + 2], o[db][4 * q4 + 3]};
-            }
-            if (hf == 0) {
-                a.part_ml[2 * slot] = m_used;
-                a.part_ml[2 * slot + 1] = l;
-            }
-        } else {
+            for (int e = 0; e < 16; ++e) chk = fmaf(0.0f, own[x][e], chk);
+        const bool broken = live && !(fabsf(chk) < INFINITY);
+        if (live && whole_block) {
             const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-            uint16_t* dst = a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D + 4 * hf;
+            uint16_t* dst = a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D + 32 * kg + 4 * hf;
 #pragma unroll
-            for (int db = 0; db < 4; ++db)
+            for (int x = 0; x < OWN; ++x)
 #pragma unroll
                 for (int q4 = 0; q4 < 4; ++q4) {
                     u32x2 w;
-                    w[0] = pack_bf16x2(o[db][4 * q4] * inv, o[db][4 * q4 + 1] * inv);
-                    w[1] = pack_bf16x2(o[db][4 * q4 + 2] * inv, o[db][4 * q4 + 3] * inv);
-                    *reinterpret_cast<u32x2*>(dst + 32 * db + 8 * q4) = w;
+                    w[0] = pack_bf16x2(own[x][4 * q4] * inv, own[x][4 * q4 + 1] * inv);
+                    w[1] = pack_bf16x2(own[x][4 * q4 + 2] * inv, own[x][4 * q4 + 3] * inv);
+                    *reinterpret_cast<u32x2*>(dst + 32 * KG * x + 8 * q4) = w;
                 }
+        } else if (live) {
+            const int q = 32 * rb + n;
+#pragma unroll
+            for (int x = 0; x < OWN; ++x)
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const f32x4 y = f32x4{own[x][4 * q4], own[x][4 * q4 + 1], own[x][4 * q4 + 2], own[x][4 * q4 + 3]};
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), rs_o,
+                                                           ((split * BR + q) * D + 32 * (kg + KG * x) + 8 * q4 + 4 * hf) * 4, 0, 16);
+                }
+            if (hf == 0 && kg == 0) put_part(q, m_used, l);
+        }
+        bits = __builtin_amdgcn_ballot_w64(broken);
+    }
+    // rows with an infinity or NaN in some group's dims again, whole, over the seen keys only
+    int* again = reinterpret_cast<int*>(ring);
+    __syncthreads();   // (the merge's reads)
+    if (__syncthreads_or(bits != 0)) {
+        if (tid < RB) again[tid] = 0;
+        LR_WAIT_VMCNT(0);   // (the rows that are overwritten below)
+        __syncthreads();
+        if (lane == 0) atomicOr(again + rb, (int)(uint32_t)(bits | bits >> 32));
+        __syncthreads();
+        uint32_t left = (uint32_t)again[rb];
+        for (int nth = 0; left; left &= left - 1, ++nth) {
+            if (nth % KG != kg) continue;
+            const int q = __builtin_amdgcn_readfirstlane(__builtin_ctz(left));
+            const int ri = __builtin_amdgcn_readlane(i, q), rhead = __builtin_amdgcn_readlane(head, q);
+            redo_row<BT, PAGED>(a, sq, tl, hk, ri, rhead, [&](float o0, float o1, float m, float rl) {
+                if (whole_block) {
+                    put_row(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D, o0, o1, rl);
+                } else {
+                    __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(o0), __float_as_uint(o1)}, rs_o,
+                                                          ((split * BR + 32 * rb + q) * D + 2 * lane) * 4, 0, 16);
+                    if (lane == 0) put_part(32 * rb + q, m, rl);
+                }
+            });
         }
     }
+    if (whole_block) return;
 
-    // rows with an infinity or NaN again, over the seen keys only
-    uint64_t again = __builtin_amdgcn_ballot_w64(broken);
-    again = (again | again >> 32) & 0xffffffffu;
-    while (again) {
-        const int src = __builtin_ctzll(again);
-        again &= again - 1;
-        const int ri = __shfl(i, src, 64), rhead = __shfl(head, src, 64);
-        redo_row<BT, PAGED>(a, sq, tl, hk, ri, rhead,
-                            a.nsplit > 1 ? ((int64_t)(sq.t0 + ri) * a.H + rhead) * a.nsplit + split : -1);
+    // ---- the last of the block's parts to end merges them, in their order. A part whose rows are in memory sets its flag, then
+    // reads all of them: the last to set its own sees every one (two that do write the same rows). Flags need no clearing before
+    // the call: only PART_DONE counts (as a float or a pair of them a NaN that no arithmetic makes), and who merges clears them.
+    LR_WAIT_VMCNT(0);
+    __syncthreads();   // every wave's rows are in memory
+    if (wave == 0) {   // (alone: a flag set after the merge would outlive the call)
+        uint64_t* flags = a.flags + block * a.nsplit;
+        if (lane == 0) __hip_atomic_store(flags + split, PART_DONE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        LR_WAIT_VMCNT(0);
+        bool done = true;
+        for (int s0 = 0; s0 < parts; s0 += 64)
+            done = done && __hip_atomic_load(flags + min(s0 + lane, parts - 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == PART_DONE;
+        const bool last = __builtin_amdgcn_ballot_w64(done) == ~0ull;
+        if (lane == 0) again[0] = last;
+        if (last)
+            for (int s0 = lane; s0 < parts; s0 += 64)
+                __hip_atomic_store(flags + s0, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-}
-
-// One wave per (token, head) merges its parts.
-template <bool PAGED>
-__global__ __launch_bounds__(256) void range_merge_kernel(RangeAttnArgs a) {
-    const int at = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const Seq sq = seq_of<PAGED>(a, blockIdx.y);
-    if (at >= (int64_t)max(sq.n, 0) * a.H) return;
-    const int i = at / a.H, head = at - i * a.H;
-    const int64_t tok = sq.t0 + i;
-    merge_parts(a, (tok * a.H + head) * a.nsplit, a.nsplit, a.out + tok * a.o_rs + head * D);
+    __syncthreads();
+    if (!__builtin_amdgcn_readfirstlane(again[0])) return;
+    for (int q = wave; q < min(BR, rows - row0); q += NW) {
+        const int ri = div_small(row0 + q, a.G, a.rcp_g), rhead = hk * a.G + row0 + q - ri * a.G;
+        merge_parts(
+            parts, a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D,
+            [&](int s) {
+                const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rs_ml, (s * BR + q) * 8, 0, 16);
+                return float2{__uint_as_float(x[0]), __uint_as_float(x[1])};
+            },
+            [&](int s) {
+                const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rs_o, ((s * BR + q) * D + 2 * lane) * 4, 0, 16);
+                return float2{__uint_as_float(x[0]), __uint_as_float(x[1])};
+            });
+    }
 }
 
 template <int RB, int KG, int NS>
@@ -314,13 +393,7 @@ hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int wide, hipSt
     if (rows <= 32) e = launch_blocks<1, 4, 2>(a, paged, stream);
     else if (rows <= 64) e = launch_blocks<2, 2, 4>(a, paged, stream);
     else e = launch_blocks<4, 2, 4>(a, paged, stream);
-    if (e != hipSuccess || a.nsplit <= 1) return e;
-    const int64_t blocks = ((int64_t)(paged ? a.max_rows : a.W) * a.H + 3) / 4;
-    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)blocks, (unsigned)(paged ? a.B : 1));
-    if (paged) hipLaunchKernelGGL(range_merge_kernel<true>, grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL(range_merge_kernel<false>, grid, dim3(256), 0, stream, a);
-    return hipGetLastError();
+    return e;
 }
 
 }  // namespace lr

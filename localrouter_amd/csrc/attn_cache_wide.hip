@@ -459,8 +459,16 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     while (again) {
         const int q = __builtin_ctzll(again);
         again &= again - 1;
-        redo_row<BT, PAGED>(a, sq, tl, hk, __builtin_amdgcn_readlane(i, q), __builtin_amdgcn_readlane(head, q),
-                            cut >= 0 ? slot_of(32 * wv + q) : -1);
+        const int ri = __builtin_amdgcn_readlane(i, q), rhead = __builtin_amdgcn_readlane(head, q);
+        redo_row<BT, PAGED>(a, sq, tl, hk, ri, rhead, [&](float o0, float o1, float m, float rl) {
+            if (cut >= 0) {
+                const int64_t at = slot_of(32 * wv + q);
+                *reinterpret_cast<float2*>(a.part_o + at * D + 2 * lane) = float2{o0, o1};
+                if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = float2{m, rl};
+            } else {
+                put_row(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D, o0, o1, rl);
+            }
+        });
     }
 }
 
@@ -478,7 +486,11 @@ __global__ __launch_bounds__(256) void range_wide_merge_kernel(RangeAttnArgs a) 
     const int r = blk * KBM + q;
     if (r >= max(sq.n, 0) * a.G) return;
     const int i = div_small(r, a.G, a.rcp_g), head = hk * a.G + r - i * a.G;
-    merge_parts(a, ((int64_t)cut * KBM + q) * a.nsplit, a.nsplit, a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D);
+    const int64_t at = ((int64_t)cut * KBM + q) * a.nsplit;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at;
+    const float2* po = reinterpret_cast<const float2*>(a.part_o) + at * (D / 2) + (threadIdx.x & 63);
+    merge_parts(a.nsplit, a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D, [&](int s) { return ml[s]; },
+                [&](int s) { return po[(int64_t)s * (D / 2)]; });
 }
 
 template <int QW, bool PAGED>

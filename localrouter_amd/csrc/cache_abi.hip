@@ -48,10 +48,10 @@ lr::PageArgs page_args(int64_t page, int64_t row, int64_t head, int n_pages, int
 
 // ------------------------------------------------------------------------------------------------ range attention
 // How a call is cut: the kernel (wide: 0, or the waves of the kernel of attn_cache_wide.hip) and its blocks over the keys
-// (RangeAttnArgs: nsplit, per, whole, local, nblk), and the rows of the parts.
+// (RangeAttnArgs: nsplit, per, whole, local, nblk), the rows of the parts and their flags.
 struct Cut {
     int wide, nsplit, per, whole, local, nblk;
-    int64_t part_rows;
+    int64_t part_rows, flags;
 };
 
 // The most key tiles of bt keys that a block of rows needs: of `span` keys beside the first `sinks`, of `keys` in all.
@@ -59,17 +59,18 @@ int64_t tiles_of(int64_t keys, int64_t span, int64_t sinks, int bt) {
     return std::min((keys + bt - 1) / bt, (std::min(sinks, keys) + bt - 1) / bt + span / bt + 2);
 }
 
-// attn_cache.hip: every block in parts of `per` tiles. rows of a kv head a sequence; pairs: sequences x kv heads; tokens x heads
-// of the call.
-Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int64_t token_rows, int page_size) {
+// attn_cache.hip: every block in parts of `per` tiles. rows of a kv head a sequence; pairs: sequences x kv heads.
+Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
     const int64_t br = rows <= 32 ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
     const int64_t staged = page_size ? lr::RANGE_STAGED / std::max(1, lr::RANGE_TILE / page_size) : INT_MAX;
-    int64_t ns = std::min(std::max<int64_t>(1, 512 / base), std::max<int64_t>(1, tiles / 8));
+    int64_t ns = std::min(std::max<int64_t>(1, 512 / base), std::max<int64_t>(1, (tiles + 3) / 4));
     const int64_t per = std::max<int64_t>(1, std::min((tiles + ns - 1) / ns, staged));
     ns = std::max<int64_t>(1, (tiles + per - 1) / per);
     Cut c{};
     c.nsplit = (int)ns; c.per = (int)per;
-    c.part_rows = ns > 1 ? token_rows * ns : 0;
+    c.nblk = (int)((rows + br - 1) / br);
+    c.part_rows = ns > 1 ? base * ns * br : 0;
+    c.flags = ns > 1 ? base * ns : 0;
     return c;
 }
 
@@ -118,17 +119,17 @@ Cut window_cut(int W, int H, int HK, int nkeys, int window, int sinks, int frame
     const int64_t rows = (int64_t)W * (H / HK), tokens = std::min<int64_t>(W, 256 / (H / HK) + 2);
     const int64_t span = (window + 2) * (int64_t)frame + tokens;
     if (narrow && rows > 64) return cut_wide(rows, HK, tiles_of(nkeys, span, sinks, lr::RANGE_WIDE_TILE), 0, HK % 8 == 0);
-    return cut_small(rows, HK, tiles_of(nkeys, span, sinks, lr::RANGE_TILE), (int64_t)W * H, 0);
+    return cut_small(rows, HK, tiles_of(nkeys, span, sinks, lr::RANGE_TILE), 0);
 }
-Cut cache_cut(int B, int T, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks, bool narrow) {
+Cut cache_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks, bool narrow) {
     const int64_t rows = (int64_t)max_rows * (H / HK), pairs = (int64_t)B * HK;
     const int64_t span = window ? (int64_t)window + max_rows + 1 : max_keys;
     if (narrow && rows > 64 && page_size >= lr::RANGE_WIDE_MIN_PAGE)
         return cut_wide(rows, pairs, tiles_of(max_keys, span, sinks, lr::RANGE_WIDE_TILE), page_size, true);
-    return cut_small(rows, pairs, tiles_of(max_keys, span, sinks, lr::RANGE_TILE), (int64_t)T * H, page_size);
+    return cut_small(rows, pairs, tiles_of(max_keys, span, sinks, lr::RANGE_TILE), page_size);
 }
 size_t part_bytes(const Cut& c) {
-    return (((size_t)c.part_rows * lr::D * 4 + 255) & ~(size_t)255) + (((size_t)c.part_rows * 8 + 255) & ~(size_t)255);
+    return (((size_t)c.part_rows * lr::D * 4 + 255) & ~(size_t)255) + (((size_t)(c.part_rows + c.flags) * 8 + 255) & ~(size_t)255);
 }
 void set_cut(lr::RangeAttnArgs& a, void* ws, const Cut& c) {
     a.nsplit = c.nsplit; a.per = c.per; a.whole = c.whole; a.local = c.local; a.nblk = c.nblk;
@@ -138,6 +139,7 @@ void set_cut(lr::RangeAttnArgs& a, void* ws, const Cut& c) {
     a.rcp_hk = lr::rcp_small(a.HK);
     a.part_o = static_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + (((size_t)c.part_rows * lr::D * 4 + 255) & ~(size_t)255));
+    a.flags = reinterpret_cast<uint64_t*>(a.part_ml + 2 * c.part_rows);
 }
 
 bool window_sizes_ok(int W, int H, int HK, int nkeys, int window, int sinks, int frame) {
@@ -199,8 +201,8 @@ int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* 
 size_t lr_cache_attention_ws_bytes(int B, int T, int max_rows, int max_keys, int H, int HK, int page_size, int window,
                                    int sinks) {
     if (!cache_sizes_ok(B, T, max_rows, max_keys, H, HK, page_size, window, sinks)) return 0;
-    return std::max(part_bytes(cache_cut(B, T, max_rows, max_keys, H, HK, page_size, window, sinks, true)),
-                    part_bytes(cache_cut(B, T, max_rows, max_keys, H, HK, page_size, window, sinks, false)));
+    return std::max(part_bytes(cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks, true)),
+                    part_bytes(cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks, false)));
 }
 
 int lr_cache_attention_bf16(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride, const void* k_pages,
@@ -221,7 +223,7 @@ int lr_cache_attention_bf16(const void* q, int64_t q_row_stride, void* out, int6
     if (overlap(so, sq) || overlap(so, sk) || overlap(so, sv)) return ERR_ARGS;
     lr::RangeAttnArgs a{};
     const bool narrow = row_stride < lr::RANGE_WIDE_MAX_RS && (page_size > lr::RANGE_WIDE_MIN_PAGE || sk.hi - sk.lo < (1ull << 32));
-    const Cut cut = cache_cut(B, T, max_rows, max_keys, H, HK, page_size, window, sinks, narrow);
+    const Cut cut = cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks, narrow);
     const size_t need = part_bytes(cut);
     if (need) {
         if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return ERR_ARGS;

@@ -40,13 +40,15 @@ struct RangeAttnArgs {
     int B, T, max_rows, max_keys, words;
     int window, sinks;      // window 0 (pages only): every earlier key
     // Split over the keys: with nsplit > 1 a block of rows is nsplit workgroups, each a part of its key tiles, whose unnormalised
-    // rows, references and sums go to the parts (fp32 [slot][128] and [slot][2]), merged by a second launch. attn_cache.hip: every
-    // block, `per` tiles a part, slots [token][head][part]. attn_cache_wide.hip: the blocks from number `whole` on, in the order
-    // in which an XCD's workgroups start (`local` blocks an XCD, or in all: see its kernel), `per` tiles a part or, per 0, equal
-    // parts; slots [block][row][part].
+    // rows, references and sums go to the parts (fp32 [slot][128] and [slot][2]).
+    // attn_cache.hip: every block, `per` tiles a part, slots [block][part][row]; the last part of a block to end, by the
+    // flags [block][part], merges them. attn_cache_wide.hip: the blocks from number `whole` on, in the order in which an XCD's
+    // workgroups start (`local` blocks an XCD, or in all: see its kernel), `per` tiles a part or, per 0, equal parts; slots
+    // [block][row][part], merged by a second launch.
     int nsplit, per, whole, local;
     float* part_o;
     float* part_ml;
+    uint64_t* flags;
     // rcp_small of the divisors; nblk: blocks of rows a sequence and kv head
     uint32_t rcp_g, rcp_hk, rcp_frame, rcp_split, rcp_nblk;
     int nblk;

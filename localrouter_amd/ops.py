@@ -131,6 +131,8 @@ def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: tor
     """lr_attention_window_bf16: q [w, heads, 128] at positions p0 + i over k / v [nkeys, kv_heads, 128]; a query in frame
     f = position // frame sees the keys of frames f - window + 1 .. f and the first `sinks` keys (up to frame f). frame 1: a
     sliding window of single tokens. A workspace of attention_window_ws_bytes is allocated when none is given."""
+    if not q.is_cuda:
+        raise ValueError(f"attention_window: expected tensors on the GPU, got one on {q.device}")
     dev = torch._C._cuda_getDevice()
     w, heads = q.shape[0], q.shape[1]
     nkeys, kv_heads = k.shape[0], k.shape[1]
