@@ -336,7 +336,7 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
             });
         }
     }
-    if (whole_block) return;
+    if (whole_block || !a.merge_here) return;
 
     // ---- the last of the block's parts to end merges them, in their order. A part whose rows are in memory sets its flag, then
     // reads all of them: the last to set its own sees every one (two that do write the same rows). Flags need no clearing before
@@ -358,29 +358,84 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     }
     __syncthreads();
     if (!__builtin_amdgcn_readfirstlane(again[0])) return;
-    for (int q = wave; q < min(BR, rows - row0); q += NW) {
+    // 16 lanes a row (dims 8 c .. 8 c + 7), four rows a wave, eight parts in flight
+    const int mc = lane & 15;
+    for (int q0 = 4 * wave; q0 < min(BR, rows - row0); q0 += 4 * NW) {
+        const int q = min(q0 + (lane >> 4), rows - row0 - 1);   // (past the last row: that one again, the same)
+        float M = -INFINITY, L = 0.0f, sum[8] = {};
+        for (int s0 = 0; s0 < parts; s0 += 8) {
+            u32x2 ml[8];
+            u32x4 x[8][2];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int at = min(s0 + u, parts - 1) * BR + q;
+                ml[u] = __builtin_amdgcn_raw_buffer_load_b64(rs_ml, at * 8, 0, 16);
+                x[u][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_o, at * D * 4 + 32 * mc, 0, 16);
+                x[u][1] = __builtin_amdgcn_raw_buffer_load_b128(rs_o, at * D * 4 + 32 * mc + 16, 0, 16);
+            }
+            float Mn = M;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) Mn = fmaxf(Mn, __uint_as_float(ml[u][0]));
+            const float ref = Mn > -INFINITY ? Mn : 0.0f, alpha = __builtin_amdgcn_exp2f(M - ref);
+            M = Mn;
+            L *= alpha;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] *= alpha;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                // a part that saw no key has no weight, whatever is in its row
+                const float m = __uint_as_float(ml[u][0]);
+                const bool in = m > -INFINITY && s0 + u < parts;
+                const float w = __builtin_amdgcn_exp2f(m - ref);
+                L = in ? fmaf(w, __uint_as_float(ml[u][1]), L) : L;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[e] = in ? fmaf(w, __uint_as_float(x[u][e >> 2][e & 3]), sum[e]) : sum[e];
+            }
+        }
         const int ri = div_small(row0 + q, a.G, a.rcp_g), rhead = hk * a.G + row0 + q - ri * a.G;
-        merge_parts(
-            parts, a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D,
-            [&](int s) {
-                const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rs_ml, (s * BR + q) * 8, 0, 16);
-                return float2{__uint_as_float(x[0]), __uint_as_float(x[1])};
-            },
-            [&](int s) {
-                const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rs_o, ((s * BR + q) * D + 2 * lane) * 4, 0, 16);
-                return float2{__uint_as_float(x[0]), __uint_as_float(x[1])};
-            });
+        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(sum[2 * e] * inv, sum[2 * e + 1] * inv);
+        *reinterpret_cast<u32x4*>(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D + 8 * mc) = w;
     }
+}
+
+// The parts of the blocks that more than one workgroup had, a wave a row: where they are many, one workgroup a block would take
+// long (64 parts of 32 rows: ~60 us).
+template <int BR, bool PAGED>
+__global__ __launch_bounds__(256) void range_merge_kernel(RangeAttnArgs a) {
+    const int at = blockIdx.x / (BR / 4), q = blockIdx.x % (BR / 4) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int blk = div_small(at, a.HK, a.rcp_hk), hk = at - blk * a.HK, b = blockIdx.y;
+    const Seq sq = seq_of<PAGED>(a, b);
+    const int rows = max(sq.n, 0) * a.G, row0 = blk * BR;
+    if (row0 + q >= rows) return;
+    TileList<RANGE_TILE, PAGED> tl;
+    tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + BR) - 1, a.G, a.rcp_g));
+    const int parts = (tl.total + a.per - 1) / a.per;
+    if (parts <= 1) return;   // (the attention wrote its rows)
+    const int i = div_small(row0 + q, a.G, a.rcp_g), head = hk * a.G + row0 + q - i * a.G;
+    const int64_t first = (((int64_t)b * a.nblk + blk) * a.HK + hk) * a.nsplit * BR + q;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + first;
+    const float2* po = reinterpret_cast<const float2*>(a.part_o) + first * (D / 2) + lane;
+    merge_parts(parts, a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D, [&](int s) { return ml[s * BR]; },
+                [&](int s) { return po[(int64_t)s * BR * (D / 2)]; });
 }
 
 template <int RB, int KG, int NS>
 hipError_t launch_blocks(const RangeAttnArgs& a, bool paged, hipStream_t stream) {
     const int64_t rows = (int64_t)(paged ? a.max_rows : a.W) * a.G;
     const int64_t blocks = (rows + 32 * RB - 1) / (32 * RB) * a.HK * a.nsplit;
-    if (blocks > 0x7fffffff || rows > 0x7fffffff) return hipErrorInvalidValue;
+    // (a grid's work-items are counted in 32 bits)
+    if (blocks > 1 << 22 || blocks / a.nsplit * 8 * RB > 1 << 23) return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks, (unsigned)(paged ? a.B : 1));
     if (paged) hipLaunchKernelGGL((range_attn_kernel<RB, KG, NS, true>), grid, dim3(RB * KG * 64), 0, stream, a);
     else hipLaunchKernelGGL((range_attn_kernel<RB, KG, NS, false>), grid, dim3(RB * KG * 64), 0, stream, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.nsplit == 1 || a.merge_here) return e;
+    const dim3 merge((unsigned)(blocks / a.nsplit * (8 * RB)), grid.y);
+    if (paged) hipLaunchKernelGGL((range_merge_kernel<32 * RB, true>), merge, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((range_merge_kernel<32 * RB, false>), merge, dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 

@@ -50,7 +50,7 @@ lr::PageArgs page_args(int64_t page, int64_t row, int64_t head, int n_pages, int
 // How a call is cut: the kernel (wide: 0, or the waves of the kernel of attn_cache_wide.hip) and its blocks over the keys
 // (RangeAttnArgs: nsplit, per, whole, local, nblk), the rows of the parts and their flags.
 struct Cut {
-    int wide, nsplit, per, whole, local, nblk;
+    int wide, nsplit, per, whole, local, nblk, merge_here;
     int64_t part_rows, flags;
 };
 
@@ -59,16 +59,22 @@ int64_t tiles_of(int64_t keys, int64_t span, int64_t sinks, int bt) {
     return std::min((keys + bt - 1) / bt, (std::min(sinks, keys) + bt - 1) / bt + span / bt + 2);
 }
 
-// attn_cache.hip: every block in parts of `per` tiles. rows of a kv head a sequence; pairs: sequences x kv heads.
+// attn_cache.hip: every block in parts of `per` tiles, one workgroup a CU. rows of a kv head a sequence; pairs: sequences x kv
+// heads. As many parts as fill one round of the CUs, of 8 tiles at least (us over the number of parts; 8 kv heads, 4 rows each: one
+// sequence of 1,900 keys 1 part 29.5, 4 15.1, 8 12.0, 16 11.9, 32 13.8; of 16,000 8 34.0, 16 23.6, 32 22.1, 48 34.3; 16 sequences of
+// 16,000 1 225, 2 188, 4 195; 16 of 1,000 1 20.9, 2 20.0, 4 27.8). The last part to end merges them where they are few; many are
+// merged faster by a second launch (in the same launch / by a second: 16 parts of 4 rows 11.9 / 14.3, of 16 rows 14.4 / 14.9, of 32
+// rows 19.3 / 17.0, of 64 rows 27.0 / 19.6).
 Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
     const int64_t br = rows <= 32 ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
     const int64_t staged = page_size ? lr::RANGE_STAGED / std::max(1, lr::RANGE_TILE / page_size) : INT_MAX;
-    int64_t ns = std::min(std::max<int64_t>(1, 512 / base), std::max<int64_t>(1, (tiles + 3) / 4));
+    int64_t ns = std::max<int64_t>(1, std::min(256 / base, (tiles + 4) / 8));
     const int64_t per = std::max<int64_t>(1, std::min((tiles + ns - 1) / ns, staged));
     ns = std::max<int64_t>(1, (tiles + per - 1) / per);
     Cut c{};
     c.nsplit = (int)ns; c.per = (int)per;
     c.nblk = (int)((rows + br - 1) / br);
+    c.merge_here = ns * std::min(rows, br) <= 256;
     c.part_rows = ns > 1 ? base * ns * br : 0;
     c.flags = ns > 1 ? base * ns : 0;
     return c;
@@ -77,7 +83,7 @@ Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
 // attn_cache_wide.hip. Two workgroups of 4 waves are resident on a CU, 64 on an XCD. Where the last round of them is not full,
 // its blocks may be cut: a block alone on its CU takes ~1.1 us a tile, beside another 1.8, and parts cost a launch (~6 us) and
 // their rows written and read (2,319 tokens x 32 heads over 8, 512 + 72 blocks, windows of 1,024, 2,048 and 8,192: 66.6, 114 and 400
-// us uncut, .
+// us uncut, 63.4, 99 and 309 cut).
 Cut cut_wide(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool by_xcd) {
     const int64_t big = (rows + 255) / 256 * pairs;
     Cut c{};
@@ -132,7 +138,7 @@ size_t part_bytes(const Cut& c) {
     return (((size_t)c.part_rows * lr::D * 4 + 255) & ~(size_t)255) + (((size_t)(c.part_rows + c.flags) * 8 + 255) & ~(size_t)255);
 }
 void set_cut(lr::RangeAttnArgs& a, void* ws, const Cut& c) {
-    a.nsplit = c.nsplit; a.per = c.per; a.whole = c.whole; a.local = c.local; a.nblk = c.nblk;
+    a.nsplit = c.nsplit; a.per = c.per; a.whole = c.whole; a.local = c.local; a.nblk = c.nblk; a.merge_here = c.merge_here;
     a.rcp_split = lr::rcp_small(c.nsplit);
     a.rcp_nblk = lr::rcp_small(c.nblk);
     a.rcp_g = lr::rcp_small(a.G);

@@ -9,6 +9,7 @@ namespace lr {
 namespace {
 
 #include "rope_rows.inc"
+#include "div_small.inc"
 
 // The sequence of token t: the largest b < B with starts[b] <= t, by the 16 lanes of the token's group, 16 probes a round.
 // -1: none. (Every lane of the wave takes the same rounds.)
@@ -146,27 +147,34 @@ hipError_t append_kind(const CacheAppendArgs& a, unsigned blocks, hipStream_t st
     return hipGetLastError();
 }
 
-// A workgroup copies 128 rows (32 KB) of one page of one layer's keys or values: 8 loads in flight a lane.
+// A workgroup copies 128 rows (32 KB) of one page of one layer's keys or values. FLAT: the page's rows lie next to each other, in
+// whichever order: 8 loads of 16 bytes in flight a lane, through buffers of the page's size that end a short last chunk.
 constexpr int COPY_ROWS = 128;
-__global__ __launch_bounds__(256) void cache_copy_kernel(CacheCopyArgs a, int chunks) {
-    const int pair = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+template <bool FLAT>
+__global__ __launch_bounds__(256) void cache_copy_kernel(CacheCopyArgs a, int chunks, uint32_t rcp_chunks, uint32_t rcp_hk) {
+    const int pair = div_small(blockIdx.x, chunks, rcp_chunks), chunk = blockIdx.x - pair * chunks;
     const int src = a.src[pair], dst = a.dst[pair];
     if (src < 0 || src >= a.pg.n_pages || dst < 0 || dst >= a.pg.n_pages || src == dst) return;
-    uint16_t* base = (blockIdx.z ? a.vp : a.kp) + (int64_t)blockIdx.y * a.layer_stride + 8 * (threadIdx.x & 15);
-    const int rows = a.HK << a.pg.shift, page = 1 << a.pg.shift;
-    const bool slot_major = a.pg.hs <= a.pg.rs;
-    u32x4 x[COPY_ROWS / 16];
-    int64_t off[COPY_ROWS / 16];
+    uint16_t* base = (blockIdx.z ? a.vp : a.kp) + (int64_t)blockIdx.y * a.layer_stride;
+    uint16_t *from = base + (int64_t)src * a.pg.ps, *to = base + (int64_t)dst * a.pg.ps;
+    const int rows = a.HK << a.pg.shift;
+    if constexpr (FLAT) {
+        const __amdgpu_buffer_rsrc_t in = __builtin_amdgcn_make_buffer_rsrc(from, 0, rows * D * 2, 0x00020000);
+        const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(to, 0, rows * D * 2, 0x00020000);
+        const int off = chunk * COPY_ROWS * D * 2 + 16 * (int)threadIdx.x;
+        u32x4 x[COPY_ROWS / 16];
 #pragma unroll
-    for (int u = 0; u < COPY_ROWS / 16; ++u) {
-        const int r = chunk * COPY_ROWS + 16 * u + (threadIdx.x >> 4), rr = min(r, rows - 1);
-        const int slot = slot_major ? rr / a.HK : rr & (page - 1), h = slot_major ? rr - slot * a.HK : rr >> a.pg.shift;
-        off[u] = r < rows ? (int64_t)slot * a.pg.rs + (int64_t)h * a.pg.hs : -1;
-        if (off[u] >= 0) x[u] = *reinterpret_cast<const u32x4*>(base + (int64_t)src * a.pg.ps + off[u]);
+        for (int u = 0; u < COPY_ROWS / 16; ++u) x[u] = __builtin_amdgcn_raw_buffer_load_b128(in, off + 4096 * u, 0, 2);
+#pragma unroll
+        for (int u = 0; u < COPY_ROWS / 16; ++u) __builtin_amdgcn_raw_buffer_store_b128(x[u], out, off + 4096 * u, 0, 2);
+    } else {
+        const int end = min(rows, (chunk + 1) * COPY_ROWS);
+        for (int r = chunk * COPY_ROWS + (threadIdx.x >> 4); r < end; r += 16) {
+            const int slot = div_small(r, a.HK, rcp_hk);
+            const int64_t off = (int64_t)slot * a.pg.rs + (int64_t)(r - slot * a.HK) * a.pg.hs + 8 * (threadIdx.x & 15);
+            *reinterpret_cast<u32x4*>(to + off) = *reinterpret_cast<const u32x4*>(from + off);
+        }
     }
-#pragma unroll
-    for (int u = 0; u < COPY_ROWS / 16; ++u)
-        if (off[u] >= 0) *reinterpret_cast<u32x4*>(base + (int64_t)dst * a.pg.ps + off[u]) = x[u];
 }
 
 // A workgroup moves a sequence's rows in `hw` heads of one layer's keys or values: all of them are read before any is
@@ -215,10 +223,15 @@ hipError_t launch_cache_append(const CacheAppendArgs& a, hipStream_t stream) {
 }
 
 hipError_t launch_cache_copy(const CacheCopyArgs& a, hipStream_t stream) {
-    const int chunks = ((a.HK << a.pg.shift) + COPY_ROWS - 1) / COPY_ROWS;
+    const int rows = a.HK << a.pg.shift, chunks = (rows + COPY_ROWS - 1) / COPY_ROWS;
     const int64_t blocks = (int64_t)a.n * chunks;
-    if (blocks > 0x7fffffff || a.layers > 65535) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(cache_copy_kernel, dim3((unsigned)blocks, (unsigned)a.layers, 2), dim3(256), 0, stream, a, chunks);
+    if (blocks > 1 << 23 || a.layers > 65535) return hipErrorInvalidValue;   // (a grid's work-items are counted in 32 bits)
+    const int64_t page = (int64_t)1 << a.pg.shift;
+    // (a buffer's size is 32 bits)
+    const bool flat = rows <= 1 << 22 && ((a.pg.hs == D && a.pg.rs == (int64_t)a.HK * D) || (a.pg.rs == D && a.pg.hs == page * D));
+    const dim3 grid((unsigned)blocks, (unsigned)a.layers, 2);
+    if (flat) hipLaunchKernelGGL(cache_copy_kernel<true>, grid, dim3(256), 0, stream, a, chunks, rcp_small(chunks), rcp_small(a.HK));
+    else hipLaunchKernelGGL(cache_copy_kernel<false>, grid, dim3(256), 0, stream, a, chunks, rcp_small(chunks), rcp_small(a.HK));
     return hipGetLastError();
 }
 

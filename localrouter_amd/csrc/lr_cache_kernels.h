@@ -41,11 +41,11 @@ struct RangeAttnArgs {
     int window, sinks;      // window 0 (pages only): every earlier key
     // Split over the keys: with nsplit > 1 a block of rows is nsplit workgroups, each a part of its key tiles, whose unnormalised
     // rows, references and sums go to the parts (fp32 [slot][128] and [slot][2]).
-    // attn_cache.hip: every block, `per` tiles a part, slots [block][part][row]; the last part of a block to end, by the
-    // flags [block][part], merges them. attn_cache_wide.hip: the blocks from number `whole` on, in the order in which an XCD's
+    // attn_cache.hip: every block, `per` tiles a part, slots [block][part][row]; merged by the last part of a
+    // block to end, by the flags [block][part] (merge_here), or by a second launch. attn_cache_wide.hip: the blocks from number `whole` on, in the order in which an XCD's
     // workgroups start (`local` blocks an XCD, or in all: see its kernel), `per` tiles a part or, per 0, equal parts; slots
     // [block][row][part], merged by a second launch.
-    int nsplit, per, whole, local;
+    int nsplit, per, whole, local, merge_here;
     float* part_o;
     float* part_ml;
     uint64_t* flags;
