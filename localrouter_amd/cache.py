@@ -63,58 +63,62 @@ def _device(t: torch.Tensor) -> int:
     return _current()
 
 
-def _call(name: str, *args) -> None:
-    rc = getattr(_bound or lib(), name)(*args)
+def _check(name: str, rc: int) -> None:
     if rc != 0:
         raise _lib.LrError(name, rc)
 
 
+def _refuse(name: str, want: str, *tensors: torch.Tensor):
+    got = ", ".join(f"{t.dtype} {tuple(t.shape)} / {tuple(t.stride())} on {t.device}" for t in tensors)
+    raise ValueError(f"{name}: expected {want} on the current device, got {got}")
+
+
 def _rows(t: torch.Tensor, name: str, dev: int, n: int, heads: int) -> int:
     """The row stride of bf16 rows [>= n, heads, 128] on device dev."""
-    s, st = t.shape, t.stride()
-    if (t.get_device() != dev or t.dtype is not _BF16 or len(s) != 3 or s[0] < n or s[1] != heads or s[2] != D or st[2] != 1
-            or (st[1] != D and heads > 1)):
-        raise ValueError(f"{name}: expected bf16 [{n}, {heads}, 128] with contiguous heads on the current device, got {t.dtype} "
-                         f"{tuple(s)} / {st} on {t.device}")
-    return st[0] if s[0] > 1 else heads * D
+    if t.dim() == 3:
+        tn, th, td = t.shape
+        rs, hs, ds = t.stride()
+        if (tn >= n and th == heads and td == 128 and ds == 1 and (hs == 128 or heads == 1) and t.dtype is _BF16
+                and t.get_device() == dev):
+            return rs if tn > 1 else heads * 128
+    _refuse(name, f"bf16 [{n}, {heads}, 128] with contiguous heads", t)
 
 
 def _ints(t: torch.Tensor, name: str, dev: int, n: int) -> int:
-    if t.get_device() != dev or t.dtype is not _I32 or t.dim() != 1 or t.numel() < n or not t.is_contiguous():
-        raise ValueError(f"{name}: expected contiguous int32 [{n}] on the current device, got {t.dtype} {tuple(t.shape)} on "
-                         f"{t.device}")
-    return t.data_ptr()
+    if t.get_device() == dev and t.dtype is _I32 and t.dim() == 1 and t.numel() >= n and t.is_contiguous():
+        return t.data_ptr()
+    _refuse(name, f"contiguous int32 [{n}]", t)
 
 
 def _pool(k: torch.Tensor, v: torch.Tensor, dev: int, layers: bool = False) -> tuple:
-    """(k pointer, v pointer, [layers, layer stride,] page, row and head strides, pages, page size, heads)."""
+    """([layers, layer stride,] page, row and head strides, pages, page size, heads)."""
     s, st = k.shape, k.stride()
     n = len(s)
-    if (k.get_device() != dev or v.get_device() != dev or k.dtype is not _BF16 or v.dtype is not _BF16 or v.shape != s
-            or v.stride() != st or not (n == 4 or (layers and n == 5)) or s[-1] != D or st[-1] != 1 or 0 in s):
-        raise ValueError(f"k_pages, v_pages: expected bf16 [n_pages, page_size, heads, 128]{' or [layers, ...]' if layers else ''} "
-                         f"of the same shape and strides on the current device, got {k.dtype} {tuple(s)} / {st} on {k.device} and "
-                         f"{v.dtype} {tuple(v.shape)} / {v.stride()} on {v.device}")
-    P, R, H = s[-4:-1]
-    ps, rs, hs = st[-4:-1]
+    if (v.shape != s or v.stride() != st or not (n == 4 or (layers and n == 5)) or s[-1] != 128 or st[-1] != 1 or 0 in s
+            or k.dtype is not _BF16 or v.dtype is not _BF16 or k.get_device() != dev or v.get_device() != dev):
+        _refuse("k_pages, v_pages", f"bf16 [n_pages, page_size, heads, 128]{' or [layers, ...]' if layers else ''} of the same "
+                "shape and strides", k, v)
+    P, R, H, _ = s[-4:]
+    ps, rs, hs, _ = st[-4:]
     # (a dimension of one element has whatever stride its view left: taken as packed)
     if H == 1:
-        hs = D
+        hs = 128
     if R == 1:
-        rs = max(D, (H - 1) * hs + D)
+        rs = (H - 1) * hs + 128
     if P == 1:
-        ps = (R - 1) * rs + (H - 1) * hs + D
+        ps = (R - 1) * rs + (H - 1) * hs + 128
     if layers:
-        return (k.data_ptr(), v.data_ptr(), s[0] if n == 5 else 1, st[0] if n == 5 and s[0] > 1 else 0, ps, rs, hs, P, R, H)
-    return k.data_ptr(), v.data_ptr(), ps, rs, hs, P, R, H
+        return s[0] if n == 5 else 1, st[0] if n == 5 and s[0] > 1 else 0, ps, rs, hs, P, R, H
+    return ps, rs, hs, P, R, H
 
 
 def _table(t: torch.Tensor, dev: int, B: int) -> tuple:
-    s, st = t.shape, t.stride()
-    if t.get_device() != dev or t.dtype is not _I32 or len(s) != 2 or s[0] < B or (st[1] != 1 and s[1] > 1):
-        raise ValueError(f"page_table: expected int32 [{B}, pages] with contiguous rows on the current device, got {t.dtype} "
-                         f"{tuple(s)} on {t.device}")
-    return t.data_ptr(), st[0] if s[0] > 1 else s[1], s[1]
+    if t.dim() == 2:
+        n, pages = t.shape
+        rs, es = t.stride()
+        if n >= B and (es == 1 or pages == 1) and t.dtype is _I32 and t.get_device() == dev:
+            return t.data_ptr(), rs if n > 1 else pages, pages
+    _refuse("page_table", f"int32 [{B}, pages] with contiguous rows", t)
 
 
 def append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -127,8 +131,7 @@ def append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: to
     as they are. table = (table_a, table_b), one row a position; positions int32 [T]: each token's table row (default its
     position in its sequence). q None: keys and values only. Returns q_out."""
     dev = _device(k_pages)
-    pool = _pool(k_pages, v_pages, dev)
-    HK = pool[7]
+    ps, rs, hs, n_pages, page_size, HK = _pool(k_pages, v_pages, dev)
     T, B = k.shape[0], lens.shape[0]
     k_rs, v_rs = _rows(k, "k", dev, T, HK), _rows(v, "v", dev, T, HK)
     H = q_rs = o_rs = 0
@@ -145,8 +148,8 @@ def append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: to
     qw = kw = ta = tb = pos = None
     stride = rows = 0
     for t in (q_norm, k_norm):
-        if t is not None and (t.get_device() != dev or t.dtype is not _F32 or t.numel() != D or not t.is_contiguous()):
-            raise ValueError("q_norm, k_norm: expected fp32 [128] on the current device")
+        if t is not None and (t.dtype is not _F32 or t.numel() != 128 or not t.is_contiguous() or t.get_device() != dev):
+            _refuse("q_norm, k_norm", "fp32 [128]", t)
     if q_norm is not None:
         qw = q_norm.data_ptr()
     if k_norm is not None:
@@ -156,20 +159,21 @@ def append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: to
             raise ValueError("append: table required")
         a, b = table
         want = _BF16 if table_kind == 2 else _F32
-        st, rows = a.stride(), a.shape[0]
-        stride = st[0]
-        if a.get_device() != dev or a.dtype is not want or a.dim() != 2 or st[1] != 1:
-            raise ValueError(f"table: expected {want} rows on the current device")
-        ta = a.data_ptr()
+        st = a.stride()
+        if a.dim() != 2 or st[1] != 1 or a.dtype is not want or a.get_device() != dev:
+            _refuse("table", f"{want} rows", a)
+        stride, rows, ta = st[0], a.shape[0], a.data_ptr()
         if b is not None:
-            if b.get_device() != dev or b.dtype is not want or b.shape != a.shape or b.stride() != st:
-                raise ValueError("table: expected two tensors of the same type, shape and strides")
+            if b.shape != a.shape or b.stride() != st or b.dtype is not want or b.get_device() != dev:
+                _refuse("table", "two tensors of the same type, shape and strides", a, b)
             tb = b.data_ptr()
     if positions is not None:
         pos = _ints(positions, "positions", dev, T)
-    _call("lr_cache_append_bf16", q_ptr, k.data_ptr(), v.data_ptr(), q_rs, k_rs, v_rs, o_ptr, o_rs, *pool[:7],
-          *_table(page_table, dev, B), _ints(starts, "starts", dev, B + 1), _ints(lens, "lens", dev, B), pos, B, T, H, HK, qw, kw,
-          table_kind, ta, tb, stride, rows, pairing, rot, eps, _raw_stream(dev))
+    tab, tab_rs, tab_pages = _table(page_table, dev, B)
+    _check("lr_cache_append_bf16", lib().lr_cache_append_bf16(
+        q_ptr, k.data_ptr(), v.data_ptr(), q_rs, k_rs, v_rs, o_ptr, o_rs, k_pages.data_ptr(), v_pages.data_ptr(), ps, rs, hs,
+        n_pages, page_size, tab, tab_rs, tab_pages, _ints(starts, "starts", dev, B + 1), _ints(lens, "lens", dev, B), pos, B, T,
+        H, HK, qw, kw, table_kind, ta, tb, stride, rows, pairing, rot, eps, _raw_stream(dev)))
     return q_out
 
 
@@ -198,23 +202,21 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     T, H = q.shape[0], q.shape[1]
     B = lens.shape[0]
     q_rs = _rows(q, "q", dev, T, H)
-    pool = _pool(k_pages, v_pages, dev)
-    ps, HK = pool[6], pool[7]
+    ps, rs, hs, n_pages, page_size, HK = _pool(k_pages, v_pages, dev)
     if out is None:
         out = torch.empty((T, H, D), dtype=_BF16, device=q.device)
     o_rs = _rows(out, "out", dev, T, H)
-    tab = _table(page_table, dev, B)
-    most = tab[2] * ps
+    tab, tab_rs, tab_pages = _table(page_table, dev, B)
+    most = tab_pages * page_size
     max_rows = T if max_rows is None or max_rows > T else max_rows
     max_keys = most if max_keys is None or max_keys > most else max_keys
     words, tree_ptr = 0, None
     if tree is not None:
-        if (tree.get_device() != dev or tree.dtype is not _I64T or tree.dim() != 2 or tree.shape[0] < T
-                or not tree.is_contiguous()):
-            raise ValueError(f"tree: expected contiguous int64 [{T}, words] on the current device, got {tree.dtype} "
-                             f"{tuple(tree.shape)} on {tree.device}")
+        if (tree.dtype is not _I64T or tree.dim() != 2 or tree.shape[0] < T or not tree.is_contiguous()
+                or tree.get_device() != dev):
+            _refuse("tree", f"contiguous int64 [{T}, words]", tree)
         words, tree_ptr = tree.shape[1], tree.data_ptr()
-    need = _ws_bytes(B, T, max_rows, max_keys, H, HK, ps, window, sinks)
+    need = _ws_bytes(B, T, max_rows, max_keys, H, HK, page_size, window, sinks)
     ws, nbytes = None, 0
     if workspace is not None:
         nbytes = workspace.numel() * workspace.element_size()
@@ -224,9 +226,10 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     elif need:
         workspace, nbytes = torch.empty(need, dtype=torch.uint8, device=q.device), need
         ws = workspace.data_ptr()
-    _call("lr_cache_attention_bf16", q.data_ptr(), q_rs, out.data_ptr(), o_rs, *pool[:7], *tab,
-          _ints(starts, "starts", dev, B + 1), _ints(lens, "lens", dev, B), B, T, max_rows, max_keys, H, HK, tree_ptr, words,
-          window, sinks, scale, ws, nbytes, _raw_stream(dev))
+    _check("lr_cache_attention_bf16", lib().lr_cache_attention_bf16(
+        q.data_ptr(), q_rs, out.data_ptr(), o_rs, k_pages.data_ptr(), v_pages.data_ptr(), ps, rs, hs, n_pages, page_size, tab,
+        tab_rs, tab_pages, _ints(starts, "starts", dev, B + 1), _ints(lens, "lens", dev, B), B, T, max_rows, max_keys, H, HK,
+        tree_ptr, words, window, sinks, scale, ws, nbytes, _raw_stream(dev)))
     return out
 
 
@@ -239,7 +242,9 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, 
     if dst.shape[0] != n:
         raise ValueError("copy_pages: src and dst of different lengths")
     if n:
-        _call("lr_cache_copy_pages", *pool, _ints(src, "src", dev, n), _ints(dst, "dst", dev, n), n, _raw_stream(dev))
+        _check("lr_cache_copy_pages", lib().lr_cache_copy_pages(
+            k_pages.data_ptr(), v_pages.data_ptr(), *pool, _ints(src, "src", dev, n), _ints(dst, "dst", dev, n), n,
+            _raw_stream(dev)))
 
 
 def move_rows(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor,
@@ -253,9 +258,10 @@ def move_rows(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Te
     if dst.shape[0] != n:
         raise ValueError("move_rows: src and dst of different lengths")
     if n:
-        _call("lr_cache_move_rows", *pool, *_table(page_table, dev, B), _ints(starts, "starts", dev, B + 1),
-              _ints(src, "src", dev, n), _ints(dst, "dst", dev, n), B, n, n if max_rows is None or max_rows > n else max_rows,
-              _raw_stream(dev))
+        _check("lr_cache_move_rows", lib().lr_cache_move_rows(
+            k_pages.data_ptr(), v_pages.data_ptr(), *pool, *_table(page_table, dev, B), _ints(starts, "starts", dev, B + 1),
+            _ints(src, "src", dev, n), _ints(dst, "dst", dev, n), B, n, n if max_rows is None or max_rows > n else max_rows,
+            _raw_stream(dev)))
 
 
 class PagePool:

@@ -54,18 +54,17 @@ __device__ __forceinline__ int seq_by_length(const RangeAttnArgs& a, int rank) {
 }
 
 // The block of rows of workgroup `id`, its part (0 <= split < nsplit) and its number among the blocks that are cut (-1: whole).
-// Hardware workgroup id runs on XCD id % 8; `idx` is its number there. Rows: an XCD works on whole heads where they divide
-// evenly (the blocks of a head share its keys in the XCD's L2), the last blocks of a head first: without a full window they are
-// the longest; otherwise the heads alternate. Pages: longest sequences first, the blocks of one sequence and head next to each
-// other on one XCD. The first `whole` blocks (of an XCD, or of the launch where the heads do not divide) are not cut.
+// Hardware workgroup id runs on XCD id % 8; with by_xcd `idx` is its number there, else it is id. Rows, by_xcd: an XCD works on
+// whole heads, one after the other (the blocks of a head share its keys in the XCD's L2), the last blocks of a head first:
+// without a full window they are the longest; otherwise the heads alternate. Pages: longest sequences first, the blocks of one
+// sequence and head next to each other, by_xcd on one XCD. The first `whole` blocks (of an XCD, or of the launch) are not cut.
 template <bool PAGED>
 __device__ __forceinline__ bool block_of(const RangeAttnArgs& a, int id, int& b, int& hk, int& blk, int& split, int& cut) {
-    const bool by_xcd = PAGED || a.HK % 8 == 0;
-    const int xcd = by_xcd ? id & 7 : 0;
-    int idx = by_xcd ? id >> 3 : id;
+    const int xcd = a.by_xcd ? id & 7 : 0;
+    int idx = a.by_xcd ? id >> 3 : id;
     // Workgroups 32 apart of an XCD share a CU: where all of them are resident at once, the second 32 go in the opposite
     // order, the shortest beside the longest.
-    if (by_xcd && a.nsplit == 1 && a.local <= 64 && idx >= 32) idx = a.local + 31 - idx;
+    if (a.by_xcd && a.nsplit == 1 && a.local <= 64 && idx >= 32) idx = a.local + 31 - idx;
     split = 0;
     cut = -1;
     if (a.nsplit > 1 && idx >= a.whole) {
@@ -75,11 +74,11 @@ __device__ __forceinline__ bool block_of(const RangeAttnArgs& a, int id, int& b,
         cut = xcd * (a.local - a.whole) + q;
     }
     b = 0;
-    if (by_xcd) {
+    if (PAGED || a.by_xcd) {
         int pair = div_small(idx, a.nblk, a.rcp_nblk);
         blk = a.nblk - 1 - (idx - pair * a.nblk);
         if (PAGED) {
-            pair = pair * 8 + xcd;
+            if (a.by_xcd) pair = pair * 8 + xcd;
             if (pair >= a.B * a.HK) return false;
             b = div_small(pair, a.HK, a.rcp_hk);
             hk = pair - b * a.HK;
@@ -477,10 +476,9 @@ template <int KBM, bool PAGED>
 __global__ __launch_bounds__(256) void range_wide_merge_kernel(RangeAttnArgs a) {
     const int c = blockIdx.x / (KBM / 4), q = blockIdx.x % (KBM / 4) * 4 + (threadIdx.x >> 6);
     const int of = a.local - a.whole;   // cut blocks an XCD
-    const bool by_xcd = PAGED || a.HK % 8 == 0;
-    const int xcd = by_xcd ? c / of : 0, first = a.whole + (c - xcd * of) * a.nsplit;   // the block's first workgroup
+    const int xcd = a.by_xcd ? c / of : 0, first = a.whole + (c - xcd * of) * a.nsplit;   // the block's first workgroup
     int b, hk, blk, split, cut;
-    if (!block_of<PAGED>(a, by_xcd ? 8 * first + xcd : first, b, hk, blk, split, cut)) return;
+    if (!block_of<PAGED>(a, a.by_xcd ? 8 * first + xcd : first, b, hk, blk, split, cut)) return;
     b = __builtin_amdgcn_readfirstlane(b);
     const Seq sq = seq_of<PAGED>(a, b);
     const int r = blk * KBM + q;
@@ -495,7 +493,7 @@ __global__ __launch_bounds__(256) void range_wide_merge_kernel(RangeAttnArgs a) 
 
 template <int QW, bool PAGED>
 hipError_t launch_waves(const RangeAttnArgs& a, hipStream_t stream) {
-    const int xcds = PAGED || a.HK % 8 == 0 ? 8 : 1;
+    const int xcds = a.by_xcd ? 8 : 1;
     const int64_t of = a.nsplit > 1 ? a.local - a.whole : 0;   // cut blocks
     const int64_t blocks = xcds * (a.local + of * (a.nsplit - 1)), merge = xcds * of * (8 * QW);
     if (blocks > 1 << 22 || merge > 1 << 23) return hipErrorInvalidValue;   // (a grid's work-items are counted in 32 bits)

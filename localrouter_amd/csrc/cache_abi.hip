@@ -50,7 +50,7 @@ lr::PageArgs page_args(int64_t page, int64_t row, int64_t head, int n_pages, int
 // How a call is cut: the kernel (wide: 0, or the waves of the kernel of attn_cache_wide.hip) and its blocks over the keys
 // (RangeAttnArgs: nsplit, per, whole, local, nblk), the rows of the parts and their flags.
 struct Cut {
-    int wide, nsplit, per, whole, local, nblk, merge_here;
+    int wide, nsplit, per, whole, local, nblk, merge_here, by_xcd;
     int64_t part_rows, flags;
 };
 
@@ -91,6 +91,7 @@ Cut cut_wide(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool by_
     // waves: 4,096 tokens x 32 heads, windows of 8,192 and 1,024 tokens 493 / 511 and 100 / 92; 3,000 x 32, 1.5 rounds, 91 / 82).
     c.wide = tiles >= 64 && big >= 256 && (big % 256 == 0 || big >= 1024) ? 8 : 4;
     const int br = 32 * c.wide, xcds = by_xcd ? 8 : 1, round = (c.wide == 8 ? 256 : 512) / xcds;
+    c.by_xcd = by_xcd;
     c.nblk = (int)((rows + br - 1) / br);
     c.local = (int)((pairs + xcds - 1) / xcds * c.nblk);
     c.whole = c.local;
@@ -131,14 +132,14 @@ Cut cache_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, i
     const int64_t rows = (int64_t)max_rows * (H / HK), pairs = (int64_t)B * HK;
     const int64_t span = window ? (int64_t)window + max_rows + 1 : max_keys;
     if (narrow && rows > 64 && page_size >= lr::RANGE_WIDE_MIN_PAGE)
-        return cut_wide(rows, pairs, tiles_of(max_keys, span, sinks, lr::RANGE_WIDE_TILE), page_size, true);
+        return cut_wide(rows, pairs, tiles_of(max_keys, span, sinks, lr::RANGE_WIDE_TILE), page_size, pairs % 8 == 0 || pairs >= 64);
     return cut_small(rows, pairs, tiles_of(max_keys, span, sinks, lr::RANGE_TILE), page_size);
 }
 size_t part_bytes(const Cut& c) {
     return (((size_t)c.part_rows * lr::D * 4 + 255) & ~(size_t)255) + (((size_t)(c.part_rows + c.flags) * 8 + 255) & ~(size_t)255);
 }
 void set_cut(lr::RangeAttnArgs& a, void* ws, const Cut& c) {
-    a.nsplit = c.nsplit; a.per = c.per; a.whole = c.whole; a.local = c.local; a.nblk = c.nblk; a.merge_here = c.merge_here;
+    a.nsplit = c.nsplit; a.per = c.per; a.whole = c.whole; a.local = c.local; a.nblk = c.nblk; a.merge_here = c.merge_here; a.by_xcd = c.by_xcd;
     a.rcp_split = lr::rcp_small(c.nsplit);
     a.rcp_nblk = lr::rcp_small(c.nblk);
     a.rcp_g = lr::rcp_small(a.G);

@@ -177,18 +177,19 @@ __global__ __launch_bounds__(256) void cache_copy_kernel(CacheCopyArgs a, int ch
     }
 }
 
-// A workgroup moves a sequence's rows in `hw` heads of one layer's keys or values: all of them are read before any is
-// written, so a row may be the source of one move and the target of another.
+// A workgroup moves a sequence's rows in `hw` heads of one layer's keys or values, at most 16 U rows of a head: all of them are
+// read before any is written, so a row may be the source of one move and the target of another.
 constexpr int MOVE_ROWS = 256;
-__global__ __launch_bounds__(256) void cache_move_kernel(CacheMoveArgs a, int hw) {
+template <int U>
+__global__ __launch_bounds__(256, U == 4 ? 8 : 4) void cache_move_kernel(CacheMoveArgs a, int hw) {
     const int b = blockIdx.x, h0 = blockIdx.z * hw, nh = min(hw, a.HK - h0);
     const int s0 = a.starts[b], n = min(min(a.starts[b + 1], a.n) - s0, a.max_rows);
     if (s0 < 0 || n <= 0) return;
     uint16_t* base = ((blockIdx.y & 1) ? a.vp : a.kp) + (int64_t)(blockIdx.y >> 1) * a.layer_stride + 8 * (threadIdx.x & 15);
-    u32x4 x[MOVE_ROWS / 16];
-    int64_t to[MOVE_ROWS / 16];
+    u32x4 x[U];
+    int64_t to[U];
 #pragma unroll
-    for (int u = 0; u < MOVE_ROWS / 16; ++u) {
+    for (int u = 0; u < U; ++u) {
         const int r = 16 * u + (threadIdx.x >> 4);
         to[u] = -1;
         if (r < n * nh) {
@@ -203,7 +204,7 @@ __global__ __launch_bounds__(256) void cache_move_kernel(CacheMoveArgs a, int hw
     }
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < MOVE_ROWS / 16; ++u)
+    for (int u = 0; u < U; ++u)
         if (to[u] >= 0) *reinterpret_cast<u32x4*>(base + to[u]) = x[u];
 }
 
@@ -236,10 +237,15 @@ hipError_t launch_cache_copy(const CacheCopyArgs& a, hipStream_t stream) {
 }
 
 hipError_t launch_cache_move(const CacheMoveArgs& a, hipStream_t stream) {
-    const int hw = min(a.HK, max(1, MOVE_ROWS / a.max_rows));
+    // few moves: fewer registers a lane, so that twice the workgroups hide each other's chain of loads
+    const int most = min(MOVE_ROWS, max(64, 16 * ((a.max_rows * a.HK + 15) / 16)));
+    const int hw = min(a.HK, max(1, most / a.max_rows));
     if (a.max_rows > MOVE_ROWS || 2 * (int64_t)a.layers > 65535 || (a.HK + hw - 1) / hw > 65535) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(cache_move_kernel, dim3((unsigned)a.B, 2 * (unsigned)a.layers, (unsigned)((a.HK + hw - 1) / hw)),
-                       dim3(256), 0, stream, a, hw);
+    const dim3 grid((unsigned)a.B, 2 * (unsigned)a.layers, (unsigned)((a.HK + hw - 1) / hw));
+    const int rows = hw * a.max_rows;
+    if (rows <= 64) hipLaunchKernelGGL(cache_move_kernel<4>, grid, dim3(256), 0, stream, a, hw);
+    else if (rows <= 128) hipLaunchKernelGGL(cache_move_kernel<8>, grid, dim3(256), 0, stream, a, hw);
+    else hipLaunchKernelGGL(cache_move_kernel<16>, grid, dim3(256), 0, stream, a, hw);
     return hipGetLastError();
 }
 

@@ -45,7 +45,7 @@ struct RangeAttnArgs {
     // block to end, by the flags [block][part] (merge_here), or by a second launch. attn_cache_wide.hip: the blocks from number `whole` on, in the order in which an XCD's
     // workgroups start (`local` blocks an XCD, or in all: see its kernel), `per` tiles a part or, per 0, equal parts; slots
     // [block][row][part], merged by a second launch.
-    int nsplit, per, whole, local, merge_here;
+    int nsplit, per, whole, local, merge_here, by_xcd;
     float* part_o;
     float* part_ml;
     uint64_t* flags;
