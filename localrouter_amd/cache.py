@@ -145,6 +145,8 @@ def append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: to
         q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
     if v.shape[0] != T or (q is not None and q.shape[0] != T):
         raise ValueError("append: q, k and v of different lengths")
+    if T == 0:
+        return q_out
     qw = kw = ta = tb = pos = None
     stride = rows = 0
     for t in (q_norm, k_norm):
@@ -206,6 +208,8 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     if out is None:
         out = torch.empty((T, H, D), dtype=_BF16, device=q.device)
     o_rs = _rows(out, "out", dev, T, H)
+    if T == 0:
+        return out
     tab, tab_rs, tab_pages = _table(page_table, dev, B)
     most = tab_pages * page_size
     max_rows = T if max_rows is None or max_rows > T else max_rows

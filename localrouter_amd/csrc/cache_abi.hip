@@ -124,7 +124,7 @@ Cut cut_wide(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool by_
 
 Cut window_cut(int W, int H, int HK, int nkeys, int window, int sinks, int frame, bool narrow) {
     const int64_t rows = (int64_t)W * (H / HK), tokens = std::min<int64_t>(W, 256 / (H / HK) + 2);
-    const int64_t span = (window + 2) * (int64_t)frame + tokens;
+    const int64_t span = std::min((int64_t)window + 2, (int64_t)MAX_POS) * frame + tokens;
     if (narrow && rows > 64) return cut_wide(rows, HK, tiles_of(nkeys, span, sinks, lr::RANGE_WIDE_TILE), 0, HK % 8 == 0);
     return cut_small(rows, HK, tiles_of(nkeys, span, sinks, lr::RANGE_TILE), 0);
 }

@@ -272,25 +272,68 @@ def test_rows_behind_the_last_sequence_stay():
     check_rows(cut[:2], *ref_rows(q[:2], k, v, ok.cpu()[None].expand(2, 64)))
 
 
-def test_offsets_past_32_bits():
+@pytest.mark.parametrize("ps", [16, 64])
+def test_offsets_past_32_bits(ps):
     """A pool of more than 2^31 elements whose last pages are the ones in use."""
-    ps, HK = 64, 8
-    pages = (1 << 31) // (ps * HK * 128) + 40
+    HK = 8
+    pages = (1 << 31) // (ps * HK * 128) + 200
     kp, vp = (torch.zeros(pages, ps, HK, 128, dtype=BF16, device="cuda") for _ in range(2))
-    B = Batch(18, [1, 2], [500, 130], ps, HK)
-    shift = pages - B.n_pages
-    kp[shift:], vp[shift:] = B.kp, B.vp
-    t = torch.where(B.t >= 0, B.t + shift, B.t)
-    q = rnd(B.g, 3, 16, 128)
-    assert torch.equal(cache.attention(q, kp, vp, t, B.starts, B.lens), cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens))
-    k, v = rnd(B.g, 3, HK, 128), rnd(B.g, 3, HK, 128)
-    cache.append(None, k, v, kp, vp, t, B.starts, B.lens, table_kind=ops.TABLE_NONE)
-    cache.append(None, k, v, B.kp, B.vp, B.t, B.starts, B.lens, table_kind=ops.TABLE_NONE)
-    assert torch.equal(kp[shift:], B.kp) and torch.equal(vp[shift:], B.vp) and not kp[:4].any()
+    for news, lens in (([1, 2], [500, 130]), ([30, 21], [300, 200])):      # few and many rows of a kv head
+        B = Batch(18, news, lens, ps, HK)
+        shift = pages - B.n_pages
+        kp[shift:], vp[shift:] = B.kp, B.vp
+        t = torch.where(B.t >= 0, B.t + shift, B.t)
+        T = sum(news)
+        q = rnd(B.g, T, 32, 128)
+        out = cache.attention(q, kp, vp, t, B.starts, B.lens)
+        B.check(q, out, lambda b: chain_seen(news[b], lens[b]))
+        k, v = rnd(B.g, T, HK, 128), rnd(B.g, T, HK, 128)
+        cache.append(None, k, v, kp, vp, t, B.starts, B.lens, table_kind=ops.TABLE_NONE)
+        cache.append(None, k, v, B.kp, B.vp, B.t, B.starts, B.lens, table_kind=ops.TABLE_NONE)
+        assert torch.equal(kp[shift:], B.kp) and torch.equal(vp[shift:], B.vp) and not kp[:4].any()
     cache.copy_pages(kp, vp, ints([B.table[0][0] + shift]), ints([1]))
     assert torch.equal(kp[1], B.kp[B.table[0][0]]) and torch.equal(vp[1], B.vp[B.table[0][0]])
+    cache.move_rows(kp, vp, t, ints([0, 1, 1]), ints([5]), ints([250]))
+    (p, r), (p2, r2) = divmod(5, ps), divmod(250, ps)
+    assert torch.equal(kp[B.table[0][p2] + shift, r2], B.kp[B.table[0][p], r])
     del kp, vp
     torch.cuda.empty_cache()
+
+
+def test_nothing_to_do():
+    B = Batch(25, [0, 0], [5, 40], 16, 2)
+    q, k = rnd(B.g, 0, 4, 128), rnd(B.g, 0, 2, 128)
+    assert cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens).shape == (0, 4, 128)
+    assert cache.append(q, k, k, B.kp, B.vp, B.t, B.starts, B.lens, table_kind=ops.TABLE_NONE).shape == (0, 4, 128)
+    # rows but no tokens: nothing is written
+    q = rnd(B.g, 3, 4, 128)
+    out = torch.full((3, 4, 128), 2.0, dtype=BF16, device="cuda")
+    before = B.kp.clone()
+    cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, out)
+    cache.append(q, q[:, :2], q[:, 2:], B.kp, B.vp, B.t, B.starts, B.lens, out, table_kind=ops.TABLE_NONE)
+    assert (out == 2.0).all() and torch.equal(B.kp, before)
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_starts_and_lengths_that_make_no_sense(many):
+    """Whatever the device's integers say, nothing outside the tensors is read or written: sequences whose numbers are out of
+    order or too large do less, the others are as always."""
+    news, lens = [2, 30 if many else 3, 2], [200, 150, 90]
+    B = Batch(26, news, lens, 16, 2)
+    T = sum(news)
+    q = rnd(B.g, T, 8, 128)
+    good = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens)
+    for st, ln in (([0, 2, T + 1000, 1 << 30], lens), ([-5, 2, T - 2, T], lens), (B.st, [-3, 150, (1 << 30) + 7]),
+                   ([T, T, 0, 0], lens), (B.st, [1, 2, 1 << 29])):
+        out = torch.full((T + 4, 8, 128), 6.0, dtype=BF16, device="cuda")
+        cache.attention(q, B.kp, B.vp, B.t, ints(st), ints(ln), out[2:2 + T])
+        assert (out[:2] == 6.0).all() and (out[2 + T:] == 6.0).all()
+        k = rnd(B.g, T, 2, 128)
+        kp, vp = B.kp.clone(), B.vp.clone()
+        cache.append(q, k, k, kp, vp, B.t, ints(st), ints(ln), out[2:2 + T], table_kind=ops.TABLE_NONE)
+        cache.move_rows(kp, vp, B.t, ints(st), ints([7] * T), ints([11] * T), max_rows=5)
+        assert (out[:2] == 6.0).all() and (out[2 + T:] == 6.0).all()
+    assert torch.equal(good, cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens))
 
 
 def test_workspace_streams_and_graphs():

@@ -170,6 +170,34 @@ def test_window_on_other_streams_and_in_a_graph():
         assert torch.equal(out, ops.attention_window(q, k, v, **kw))
 
 
+def test_window_rows_far_apart():
+    """Row strides past what the kernel of many rows takes (2^23 elements), and offsets past 32 bits."""
+    g = gen(22)
+    flat = torch.zeros((1 << 23) * 300 + 4096, dtype=torch.bfloat16, device="cuda")
+    k, v = flat.as_strided((300, 2, 128), (1 << 23, 128, 1)), flat.as_strided((300, 2, 128), (1 << 23, 128, 1), 1024)
+    k.copy_(rnd(g, 300, 2, 128))
+    v.copy_(rnd(g, 300, 2, 128))
+    q = rnd(g, 50, 8, 128)
+    out = ops.attention_window(q, k, v, window=100, sinks=3, p0=250)
+    check_rows(out, *ref_rows(q, k, v, window_seen(50, 300, 250, 100, 3, 1)))
+    near = ops.attention_window(q, k.contiguous(), v.contiguous(), window=100, sinks=3, p0=250)
+    check_rows(near, *ref_rows(q, k, v, window_seen(50, 300, 250, 100, 3, 1)))
+    one = ops.attention_window(q[:1], k, v, window=200, sinks=3, p0=299)
+    check_rows(one, *ref_rows(q[:1], k, v, window_seen(1, 300, 299, 200, 3, 1)))
+    del flat
+    torch.cuda.empty_cache()
+
+
+def test_window_largest_arguments():
+    g = gen(23)
+    q, k, v = rnd(g, 70, 2, 128), rnd(g, 150, 1, 128), rnd(g, 150, 1, 128)
+    top = (1 << 31) - 1
+    out = ops.attention_window(q, k, v, window=top, sinks=top, frame=top, p0=(1 << 30) - 70)
+    check_rows(out, *ref_rows(q, k, v, torch.ones(70, 150, dtype=torch.bool)))
+    out = ops.attention_window(q, k, v, window=top, p0=80)
+    check_rows(out, *ref_rows(q, k, v, window_seen(70, 150, 80, 1 << 20, 0, 1)))
+
+
 def test_window_refuses_before_launch():
     g = gen(11)
     q, k, v = rnd(g, 4, 4, 128), rnd(g, 9, 2, 128), rnd(g, 9, 2, 128)
