@@ -16,6 +16,7 @@ without the built library every call raises.
 """
 from __future__ import annotations
 
+import collections
 import ctypes
 import functools
 from pathlib import Path
@@ -38,6 +39,8 @@ SIGNATURES = {
     "lr_cache_copy_pages": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _I, _I, _I, _P, _P, _I, _P]),
     "lr_cache_move_rows": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _I, _I, _I, _P, _I64, _I, _P, _P, _P, _I, _I, _I, _P]),
 }
+
+INT_MAX = 2 ** 31 - 1
 
 _bound = None
 _BF16, _I32, _I64T, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
@@ -220,6 +223,8 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
                 or tree.get_device() != dev):
             _refuse("tree", f"contiguous int64 [{T}, words]", tree)
         words, tree_ptr = tree.shape[1], tree.data_ptr()
+    if window > INT_MAX or sinks > INT_MAX:
+        raise ValueError("attention: window and sinks are 32-bit numbers")
     need = _ws_bytes(B, T, max_rows, max_keys, H, HK, page_size, window, sinks)
     ws, nbytes = None, 0
     if workspace is not None:
@@ -311,7 +316,7 @@ class PagePool:
     def free(self, pages: list[int]) -> None:
         """One holder fewer for each page; a page without one is free again."""
         self._held(pages)
-        if any(self.holders[p] < pages.count(p) for p in set(pages)):
+        if any(self.holders[p] < n for p, n in collections.Counter(pages).items()):
             raise ValueError("PagePool: a page freed more often than it is held")
         for p in pages:
             self.holders[p] -= 1

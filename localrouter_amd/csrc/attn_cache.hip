@@ -51,7 +51,7 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     TileList<BT, PAGED> tl;
     tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + 32 * RB) - 1, a.G, a.rcp_g));
     tl.part(split, a.per);
-    const int parts = max(1, (tl.total + a.per - 1) / a.per);   // of this block: the sequence may be shorter than the longest
+    const int parts = min(a.nsplit, max(1, (tl.total + a.per - 1) / a.per));   // the sequence may be shorter than the longest
     if (split >= parts) return;
     const int x0 = tl.x0, x1 = tl.x1;
 
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(256) void range_merge_kernel(RangeAttnArgs a) {
     if (row0 + q >= rows) return;
     TileList<RANGE_TILE, PAGED> tl;
     tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + BR) - 1, a.G, a.rcp_g));
-    const int parts = (tl.total + a.per - 1) / a.per;
+    const int parts = min(a.nsplit, (tl.total + a.per - 1) / a.per);
     if (parts <= 1) return;   // (the attention wrote its rows)
     const int i = div_small(row0 + q, a.G, a.rcp_g), head = hk * a.G + row0 + q - i * a.G;
     const int64_t first = (((int64_t)b * a.nblk + blk) * a.HK + hk) * a.nsplit * BR + q;
@@ -426,8 +426,9 @@ template <int RB, int KG, int NS>
 hipError_t launch_blocks(const RangeAttnArgs& a, bool paged, hipStream_t stream) {
     const int64_t rows = (int64_t)(paged ? a.max_rows : a.W) * a.G;
     const int64_t blocks = (rows + 32 * RB - 1) / (32 * RB) * a.HK * a.nsplit;
-    // (a grid's work-items are counted in 32 bits)
-    if (blocks > 1 << 22 || blocks / a.nsplit * 8 * RB > 1 << 23) return hipErrorInvalidValue;
+    // (a grid's work-items and a block's bytes of parts are counted in 32 bits)
+    if (blocks > 1 << 22 || blocks / a.nsplit * 8 * RB > 1 << 23 || (int64_t)a.nsplit * 32 * RB * D * 4 > INT32_MAX)
+        return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks, (unsigned)(paged ? a.B : 1));
     if (paged) hipLaunchKernelGGL((range_attn_kernel<RB, KG, NS, true>), grid, dim3(RB * KG * 64), 0, stream, a);
     else hipLaunchKernelGGL((range_attn_kernel<RB, KG, NS, false>), grid, dim3(RB * KG * 64), 0, stream, a);

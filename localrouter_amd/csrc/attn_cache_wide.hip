@@ -117,7 +117,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     if (row0 >= rows) return;
     TileList<BT, PAGED> tl;
     tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + KBM) - 1, a.G, a.rcp_g));
-    if (cut >= 0) tl.part(split, a.per ? a.per : div_small(tl.total + a.nsplit - 1, a.nsplit, a.rcp_split));
+    if (PAGED || cut >= 0) tl.part(split, a.per ? a.per : div_small(tl.total + a.nsplit - 1, a.nsplit, a.rcp_split));
     const bool bad = tl.template stage<64 * QW>(a, b, staged);
     const int x0 = tl.x0, x1 = tl.x1;
 

@@ -22,6 +22,9 @@ inline bool page_size_ok(int ps) { return ps >= 1 && ps <= 65536 && (ps & (ps - 
 bool pool_ok(const void* k, const void* v, int64_t page, int64_t row, int64_t head, int n_pages, int page_size, int HK) {
     if (!k || !v || !aligned(k, 16) || !aligned(v, 16) || n_pages < 1 || HK < 1 || !page_size_ok(page_size)) return false;
     if (page % 8 || row % 8 || head % 8 || page < lr::D || row < lr::D || head < lr::D) return false;
+    // keys and values may interleave in one buffer, but not share a head's row
+    const uintptr_t ka = reinterpret_cast<uintptr_t>(k), va = reinterpret_cast<uintptr_t>(v);
+    if ((ka < va ? va - ka : ka - va) < 2 * lr::D) return false;
     // rows of a page token by token or head by head, pages apart from each other
     const bool by_token = row >= (HK - 1) * head + lr::D && page >= (page_size - 1) * row + (HK - 1) * head + lr::D;
     const bool by_head = head >= (page_size - 1) * row + lr::D && page >= (HK - 1) * head + (page_size - 1) * row + lr::D;
@@ -304,7 +307,7 @@ int lr_cache_copy_pages(void* k_pages, void* v_pages, int layers, int64_t layer_
                         int64_t row_stride, int64_t head_stride, int n_pages, int page_size, int HK, const int* src,
                         const int* dst, int n, lr_stream_t stream) {
     if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK)) return ERR_ARGS;
-    if (layers < 1 || layers > 65535 || layer_stride % 8 || layer_stride < 0 || n < 1 || !src || !dst || !aligned(src, 4) ||
+    if (layers < 1 || layers > 65535 || layer_stride % 8 || (layers > 1 && layer_stride < lr::D) || n < 1 || !src || !dst || !aligned(src, 4) ||
         !aligned(dst, 4))
         return ERR_ARGS;
     lr::CacheCopyArgs a{};
@@ -322,7 +325,7 @@ int lr_cache_move_rows(void* k_pages, void* v_pages, int layers, int64_t layer_s
                        int max_rows, lr_stream_t stream) {
     if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK)) return ERR_ARGS;
     if (!table_args_ok(page_table, table_stride, table_pages, page_size, starts, B)) return ERR_ARGS;
-    if (layers < 1 || layers > 32767 || layer_stride % 8 || layer_stride < 0 || n < 1 || !src || !dst || !aligned(src, 4) ||
+    if (layers < 1 || layers > 32767 || layer_stride % 8 || (layers > 1 && layer_stride < lr::D) || n < 1 || !src || !dst || !aligned(src, 4) ||
         !aligned(dst, 4) || max_rows < 1 || max_rows > 256)
         return ERR_ARGS;
     lr::CacheMoveArgs a{};

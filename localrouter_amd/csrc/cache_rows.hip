@@ -183,8 +183,10 @@ constexpr int MOVE_ROWS = 256;
 template <int U>
 __global__ __launch_bounds__(256, U == 4 ? 8 : 4) void cache_move_kernel(CacheMoveArgs a, int hw) {
     const int b = blockIdx.x, h0 = blockIdx.z * hw, nh = min(hw, a.HK - h0);
-    const int s0 = a.starts[b], n = min(min(a.starts[b + 1], a.n) - s0, a.max_rows);
-    if (s0 < 0 || n <= 0) return;
+    const int s0 = a.starts[b], s1 = a.starts[b + 1];
+    if (s0 < 0 || s1 <= s0) return;
+    const int n = min(min(s1, a.n) - s0, a.max_rows);
+    if (n <= 0) return;
     uint16_t* base = ((blockIdx.y & 1) ? a.vp : a.kp) + (int64_t)(blockIdx.y >> 1) * a.layer_stride + 8 * (threadIdx.x & 15);
     u32x4 x[U];
     int64_t to[U];
@@ -213,7 +215,7 @@ __global__ __launch_bounds__(256, U == 4 ? 8 : 4) void cache_move_kernel(CacheMo
 hipError_t launch_cache_append(const CacheAppendArgs& a, hipStream_t stream) {
     const int64_t hg = (a.H + HPG - 1) / HPG + 2 * ((a.HK + HPG - 1) / HPG);
     const int64_t blocks = (a.T * hg + 15) / 16;
-    if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidValue;
+    if (blocks <= 0 || blocks > 1 << 23) return hipErrorInvalidValue;   // (a grid's work-items are counted in 32 bits)
     switch (a.table_kind) {
         case TABLE_NONE: return append_kind<TABLE_NONE>(a, (unsigned)blocks, stream);
         case TABLE_COSSIN_F32: return append_kind<TABLE_COSSIN_F32>(a, (unsigned)blocks, stream);

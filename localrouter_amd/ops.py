@@ -146,6 +146,8 @@ def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: tor
             raise ValueError(f"attention_window: expected bf16 [{n}, {h}, 128] with contiguous heads on the current device, got "
                              f"{t.dtype} {tuple(s)} / {st} on {t.device}")
         strides.append(st[0] if s[0] > 1 else h * D)
+    if max(window, sinks, frame, p0) >= 1 << 31:
+        raise ValueError("attention_window: window, sinks, frame and p0 are 32-bit numbers")
     need = _window_ws_bytes(w, heads, kv_heads, nkeys, window, sinks, frame)
     ws, nbytes = None, 0
     if workspace is not None:

@@ -140,6 +140,21 @@ def test_move_refuses(kw):
     assert _move(**kw) == BAD
 
 
+def test_pools_that_share_rows_are_refused():
+    """Keys and values may interleave in one buffer (rows of their own), but not share rows; layers neither."""
+    assert _attend(vp=KP) == _append(vp=KP) == _copy(vp=KP) == _move(vp=KP) == BAD
+    assert _attend(vp=KP + 128) == _append(vp=KP - 240) == BAD
+    for ls in (0, 64):
+        assert _copy(ls=ls) == _move(ls=ls) == BAD
+
+
+def test_parts_past_32_bits_are_refused():
+    """A block's parts are addressed in 32 bits: 2^30 keys in pages of one row would have more (a launch error, not a kernel)."""
+    assert cache.attention_ws_bytes(1, 1, 1, 1 << 30, 1, 1, 1) > 1 << 31
+    assert _attend(B=1, T=1, rows=1, keys=1 << 30, H=1, HK=1, page=1, tp=1 << 30, trs=1 << 30, qrs=128, ors=128, ps=128, rs=128,
+                   wsb=1 << 40, ws=1 << 44) == BAD
+
+
 def test_python_checks_refuse_host_tensors():
     t = torch.zeros(4, 2, 128, dtype=torch.bfloat16)
     p = torch.zeros(3, 16, 2, 128, dtype=torch.bfloat16)

@@ -323,8 +323,10 @@ def test_starts_and_lengths_that_make_no_sense(many):
     T = sum(news)
     q = rnd(B.g, T, 8, 128)
     good = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens)
+    low, top = -(1 << 31), (1 << 31) - 1
     for st, ln in (([0, 2, T + 1000, 1 << 30], lens), ([-5, 2, T - 2, T], lens), (B.st, [-3, 150, (1 << 30) + 7]),
-                   ([T, T, 0, 0], lens), (B.st, [1, 2, 1 << 29])):
+                   ([T, T, 0, 0], lens), (B.st, [1, 2, 1 << 29]), ([0, 2, low, T], lens), ([low, 2, top, low], lens),
+                   ([0, 2, top, T], [low, top, top]), ([1, low, 1, top], [0, 0, 0])):
         out = torch.full((T + 4, 8, 128), 6.0, dtype=BF16, device="cuda")
         cache.attention(q, B.kp, B.vp, B.t, ints(st), ints(ln), out[2:2 + T])
         assert (out[:2] == 6.0).all() and (out[2 + T:] == 6.0).all()
@@ -334,6 +336,86 @@ def test_starts_and_lengths_that_make_no_sense(many):
         cache.move_rows(kp, vp, B.t, ints(st), ints([7] * T), ints([11] * T), max_rows=5)
         assert (out[:2] == 6.0).all() and (out[2 + T:] == 6.0).all()
     assert torch.equal(good, cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens))
+
+
+@pytest.mark.parametrize("rows", [4, 20])
+def test_drafted_tokens_beyond_max_rows_are_left_out(rows):
+    """As rows and as keys, on either side of the choice between the kernels."""
+    n, L = 70, 300
+    B = Batch(27, [n], [L], 16, 2)
+    q = rnd(B.g, n, 16, 128)
+    full = [set(range(n)) if i % 2 else set(range(0, n, 3)) for i in range(n)]
+    tree = tree_words([full], 2)
+    for window, sinks in ((0, 0), (50, 5)):
+        out = torch.full((n, 16, 128), 6.0, dtype=BF16, device="cuda")
+        cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, out, max_rows=rows, tree=tree, window=window, sinks=sinks)
+        assert (out[rows:] == 6.0).all()
+        seen = tree_seen(full, L, window, sinks)[:rows]
+        seen[:, L - n + rows:] = False
+        k, v = B.rows(0)
+        check_rows(out[:rows], *ref_rows(q[:rows], k, v, seen))
+
+
+@pytest.mark.parametrize("shape,perm", [((30, 2, 16, 2, 128), 1), ((30, 16, 2, 2, 128), 2), ((30, 16, 2, 2, 128), 3)])
+def test_keys_and_values_in_one_buffer(shape, perm):
+    """Pages whose keys and values interleave page by page, token by token or head by head."""
+    B = Batch(28, [2, 33], [120, 150], 16, 2, pages=30)
+    both = rnd(B.g, *shape)
+    kp, vp = both.unbind(perm)
+    assert kp.shape == B.kp.shape
+    kp.copy_(B.kp)
+    vp.copy_(B.vp)
+    q, k, v = rnd(B.g, 35, 8, 128), rnd(B.g, 35, 2, 128), rnd(B.g, 35, 2, 128)
+    for kk, vv in ((kp, vp), (B.kp, B.vp)):
+        cache.append(None, k, v, kk, vv, B.t, B.starts, B.lens, table_kind=ops.TABLE_NONE)
+        cache.copy_pages(kk, vv, ints([0]), ints([1]))
+        cache.move_rows(kk, vv, B.t, ints([0, 1, 3]), ints([5, 9, 70]), ints([6, 70, 9]))
+    assert torch.equal(kp, B.kp) and torch.equal(vp, B.vp)
+    for few in (slice(0, 2), slice(0, 35)):
+        n = few.stop
+        args = (B.t, ints([0, 2, n][:2 if n == 2 else 3]), B.lens[:1 if n == 2 else 2])
+        assert torch.equal(cache.attention(q[few], kp, vp, *args), cache.attention(q[few], B.kp, B.vp, *args))
+
+
+def test_a_captured_step_of_all_calls():
+    """Append, attention (split over the keys, and of many rows), a move and a page copy in two graphs with workspaces of their own, replayed in
+    turn with eager work between; every replay against the eager calls on copies."""
+    B = Batch(29, [1, 40], [3000, 90], 16, 8)
+    T, H = 41, 32
+    q, k, v = rnd(B.g, T, H, 128), rnd(B.g, T, 8, 128), rnd(B.g, T, 8, 128)
+    one = (ints([0, 1]), B.lens[:1])
+    pairs = ints([B.table[1][5]]), ints([[p for p in range(B.n_pages) if p not in sum(B.table, [])][0]])
+    moves = ints([0, 2, 3]), ints([7, 2999, 3]), ints([2999, 7, 88])
+
+    def step(kp, vp, out, ws):
+        cache.append(None, k, v, kp, vp, B.t, B.starts, B.lens, table_kind=ops.TABLE_NONE)
+        cache.attention(q[:1], kp, vp, B.t, *one, out[:1], max_rows=1, max_keys=3000, workspace=ws)
+        cache.attention(q, kp, vp, B.t, B.starts, B.lens, out[1:], max_rows=40, workspace=ws)
+        cache.move_rows(kp, vp, B.t, *moves, max_rows=2)
+        cache.copy_pages(kp, vp, *pairs)
+
+    need = max(cache.attention_ws_bytes(1, 1, 1, 3000, H, 8, 16),
+               cache.attention_ws_bytes(2, T, 40, B.width * 16, H, 8, 16))
+    assert need > 0
+    graphs = []
+    for _ in range(2):
+        kp, vp, out = B.kp.clone(), B.vp.clone(), torch.zeros(T + 1, H, 128, dtype=BF16, device="cuda")
+        ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step(kp, vp, out, ws)
+        graphs.append((g, kp, vp, out, ws))
+    ek, ev, eo = B.kp.clone(), B.vp.clone(), torch.zeros(T + 1, H, 128, dtype=BF16, device="cuda")
+    ews = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    for i in range(4):
+        for x in (q, k, v):
+            x.copy_(rnd(B.g, *x.shape))
+        step(ek, ev, eo, ews)
+        for g, kp, vp, out, ws in graphs:
+            g.replay()
+            torch.cuda.synchronize()
+            rnd(B.g, 1000, 1000).sum().item()
+            assert torch.equal(out, eo) and torch.equal(kp, ek) and torch.equal(vp, ev), f"replay {i}"
 
 
 def test_workspace_streams_and_graphs():
@@ -574,6 +656,18 @@ def test_refusals_before_launch():
         cache.attention(q, odd, odd.clone(), *ok[3:])                  # pages of 12 rows
     with pytest.raises(_lib.LrError):
         cache.move_rows(B.kp, B.vp, B.t, ints([0, 300]), ints([0] * 300), ints([0] * 300))
+
+
+def test_numbers_past_32_bits_are_refused():
+    B = Batch(33, [1], [20], 16, 2)
+    q = rnd(B.g, 1, 4, 128)
+    for kw in (dict(window=1 << 32), dict(window=4, sinks=(1 << 32) + 4)):
+        with pytest.raises(ValueError):
+            cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, **kw)
+    for kw in (dict(window=1 << 32), dict(window=4, sinks=1 << 31), dict(window=4, frame=(1 << 32) + 1),
+               dict(window=4, p0=1 << 32)):
+        with pytest.raises(ValueError):
+            ops.attention_window(q, B.kp[0], B.vp[0], **kw)
 
 
 # ------------------------------------------------------------------------------------------------ together

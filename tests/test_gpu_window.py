@@ -188,6 +188,26 @@ def test_window_rows_far_apart():
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("w,H,HK,window,sinks,frame", [
+    (2319, 32, 8, 2048, 4, 1),       # 64 whole blocks of an XCD before those that are cut over the keys
+    (1300, 24, 12, 900, 64, 1),      # heads not by XCD, all blocks cut
+    (2048, 64, 8, 5000, 0, 1),       # eight waves, two full rounds
+    (2100, 64, 64, 3, 130, 700),     # frames, a last round cut
+])
+def test_window_of_more_rows_than_one_round(w, H, HK, window, sinks, frame):
+    g = gen(24)
+    n, p0 = (w + 2100, 2100) if frame == 1 else (w, 0)
+    q, k, v = rnd(g, w, H, 128), rnd(g, n, HK, 128), rnd(g, n, HK, 128)
+    need = ops.attention_window_ws_bytes(w, H, HK, n, window=window, sinks=sinks, frame=frame)
+    ws = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")
+    out = ops.attention_window(q, k, v, window=window, sinks=sinks, frame=frame, p0=p0, workspace=ws)
+    assert (ws[need:] == 255).all()
+    at = torch.cat([torch.arange(0, w, 97), torch.tensor([w - 1, w - 33, w - 64])])
+    seen = window_seen(w, n, p0, window, sinks, frame)[at]
+    check_rows(out[at.cuda()], *ref_rows(q[at.cuda()], k, v, seen))
+    assert torch.equal(out, ops.attention_window(q, k, v, window=window, sinks=sinks, frame=frame, p0=p0))
+
+
 def test_window_largest_arguments():
     g = gen(23)
     q, k, v = rnd(g, 70, 2, 128), rnd(g, 150, 1, 128), rnd(g, 150, 1, 128)
