@@ -24,7 +24,158 @@ namespace {
 
 #include "range_attn.inc"
 
+constexpr int STEP_WAVES = 4;   // range_step_kernel's waves a workgroup
 constexpr uint64_t PART_DONE = 0x7ff4a3c57fb5d96e;
+
+// The parts of one block of BR rows. (sc1, 16: coherent at device scope, not kept in this XCD's L2; the last workgroup of the block
+// may run on another.)
+template <int BR>
+struct PartRows {
+    __amdgpu_buffer_rsrc_t rs_o, rs_ml;
+    uint64_t* flags;
+
+    __device__ __forceinline__ PartRows(const RangeAttnArgs& a, int64_t block) {
+        rs_o = __builtin_amdgcn_make_buffer_rsrc(a.part_o + block * a.nsplit * BR * D, 0, a.nsplit * BR * D * 4, 0x00020000);
+        rs_ml = __builtin_amdgcn_make_buffer_rsrc(a.part_ml + block * a.nsplit * BR * 2, 0, a.nsplit * BR * 8, 0x00020000);
+        flags = a.flags + block * a.nsplit;
+    }
+    __device__ __forceinline__ void put_ml(int split, int q, float m, float l) const {
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, rs_ml, (split * BR + q) * 8, 0, 16);
+    }
+    __device__ __forceinline__ void put4(int split, int q, int dim, f32x4 y) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), rs_o, ((split * BR + q) * D + dim) * 4, 0, 16);
+    }
+    __device__ __forceinline__ void put_row2(int split, int q, float o0, float o1, float m, float l) const {
+        const int lane = threadIdx.x & 63;
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(o0), __float_as_uint(o1)}, rs_o,
+                                              ((split * BR + q) * D + 2 * lane) * 4, 0, 16);
+        if (lane == 0) put_ml(split, q, m, l);
+    }
+
+    // The last of the block's parts to end merges them, in their order (every wave's rows are in memory). A part whose rows are
+    // in memory sets its flag, then reads all of them: the last to set its own sees every one (two that do write the same
+    // rows). Flags need no clearing before the call: only PART_DONE counts (as a float or a pair of them a NaN that no arithmetic
+    // makes), and who merges clears them.
+    template <int NW>
+    __device__ __forceinline__ void merge_last(const RangeAttnArgs& a, const Seq& sq, int hk, int row0, int rows, int split,
+                                               int parts, int* shared) const {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (wave == 0) {   // (alone: a flag set after the merge would outlive the call)
+            if (lane == 0) __hip_atomic_store(flags + split, PART_DONE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            LR_WAIT_VMCNT(0);
+            bool done = true;
+            for (int s0 = 0; s0 < parts; s0 += 64)
+                done = done && __hip_atomic_load(flags + min(s0 + lane, parts - 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == PART_DONE;
+            const bool last = __builtin_amdgcn_ballot_w64(done) == ~0ull;
+            if (lane == 0) shared[0] = last;
+            if (last)
+                for (int s0 = lane; s0 < parts; s0 += 64)
+                    __hip_atomic_store(flags + s0, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!__builtin_amdgcn_readfirstlane(shared[0])) return;
+        // 16 lanes a row (dims 8 c .. 8 c + 7), four rows a wave, eight parts in flight
+        const int mc = lane & 15;
+        for (int q0 = 4 * wave; q0 < min(BR, rows - row0); q0 += 4 * NW) {
+            const int q = min(q0 + (lane >> 4), rows - row0 - 1);   // (past the last row: that one again, the same)
+            float M = -INFINITY, L = 0.0f, sum[8] = {};
+            for (int s0 = 0; s0 < parts; s0 += 8) {
+                u32x2 ml[8];
+                u32x4 x[8][2];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int at = min(s0 + u, parts - 1) * BR + q;
+                    ml[u] = __builtin_amdgcn_raw_buffer_load_b64(rs_ml, at * 8, 0, 16);
+                    x[u][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_o, at * D * 4 + 32 * mc, 0, 16);
+                    x[u][1] = __builtin_amdgcn_raw_buffer_load_b128(rs_o, at * D * 4 + 32 * mc + 16, 0, 16);
+                }
+                float Mn = M;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) Mn = fmaxf(Mn, __uint_as_float(ml[u][0]));
+                const float ref = Mn > -INFINITY ? Mn : 0.0f, alpha = __builtin_amdgcn_exp2f(M - ref);
+                M = Mn;
+                L *= alpha;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[e] *= alpha;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    // a part that saw no key has no weight, whatever is in its row
+                    const float m = __uint_as_float(ml[u][0]);
+                    const bool in = m > -INFINITY && s0 + u < parts;
+                    const float w = __builtin_amdgcn_exp2f(m - ref);
+                    L = in ? fmaf(w, __uint_as_float(ml[u][1]), L) : L;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum[e] = in ? fmaf(w, __uint_as_float(x[u][e >> 2][e & 3]), sum[e]) : sum[e];
+                }
+            }
+            const int ri = div_small(row0 + q, a.G, a.rcp_g), rhead = hk * a.G + row0 + q - ri * a.G;
+            const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+            u32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(sum[2 * e] * inv, sum[2 * e + 1] * inv);
+            *reinterpret_cast<u32x4*>(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D + 8 * mc) = w;
+        }
+    }
+};
+
+// The direct loads of a tile by wave rb of RB: instruction u fills rows 4 u .. 4 u + 3, 16-byte chunks swizzled as attn_fwd.hip's.
+template <int RB, bool PAGED>
+__device__ __forceinline__ void load_tile_rows(const RangeAttnArgs& a, const Seq& sq, const TileList<RANGE_TILE, PAGED>& tl, int64_t hoff,
+                                               int x, uint32_t k_lds, uint32_t v_lds, int rb) {
+    constexpr int BT = RANGE_TILE, LOADS = 8 / RB;
+    const int lane = threadIdx.x & 63, lrow = lane >> 4, lchunk = lane & 15, key0 = tl.key0(x);
+    const int64_t k_rs = PAGED ? a.pg.rs : a.k_rs, v_rs = PAGED ? a.pg.rs : a.v_rs;
+    const uint16_t *kp = a.k + hoff, *vp = a.v + hoff;
+    if ((!PAGED || tl.shift >= 5) && key0 + BT <= sq.end) {   // the tile's rows are one run
+        const int64_t row = (PAGED ? key0 & ((1 << tl.shift) - 1) : key0) + 4 * rb + lrow;
+        const int64_t pg = PAGED ? (int64_t)max(tl.entry(x, 0), 0) * a.pg.ps : 0;
+        kp += pg + row * k_rs;
+        vp += pg + row * v_rs + 8 * (lchunk ^ (lrow << 2));
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int inst = rb + RB * u;
+            dma16(kp + 8 * (lchunk ^ ((4 * inst + lrow) & 15)), k_lds + 1024 * inst);
+            dma16(vp, v_lds + 1024 * inst);
+            kp += 4 * RB * k_rs;
+            vp += 4 * RB * v_rs;
+        }
+        return;
+    }
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+        const int inst = rb + RB * u, row = 4 * inst + lrow;
+        const int64_t o = tl.offset(a, x, row, k_rs), ov = PAGED ? o : tl.offset(a, x, row, v_rs);
+        dma16(kp + o + 8 * (lchunk ^ (row & 15)), k_lds + 1024 * inst);
+        dma16(vp + ov + 8 * (lchunk ^ (lrow << 2)), v_lds + 1024 * inst);
+    }
+}
+
+// A lane's value over the four lanes of its row (16 apart).
+__device__ __forceinline__ float quad_max(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return wave_pair_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return wave_pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// The rows of which a group of waves (RB of them) has bits set, again, by its KG waves in turn; f(q): row q of the group. Every
+// wave's rows are in memory afterwards.
+template <int RB, int KG, class F>
+__device__ __forceinline__ void again_rows(int* shared, int rb, int kg, uint32_t bits, F&& f) {
+    LR_WAIT_VMCNT(0);   // (the rows that are overwritten below)
+    if (!__syncthreads_or(bits != 0)) return;
+    if (threadIdx.x < RB) shared[threadIdx.x] = 0;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) atomicOr(shared + rb, (int)bits);
+    __syncthreads();
+    uint32_t left = (uint32_t)shared[rb];
+    for (int nth = 0; left; left &= left - 1, ++nth)
+        if (nth % KG == kg) f(__builtin_amdgcn_readfirstlane(__builtin_ctz(left)));
+    LR_WAIT_VMCNT(0);
+    __syncthreads();
+}
 
 template <int RB, int KG, int NS, bool PAGED>
 __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(RangeAttnArgs a) {
@@ -60,11 +211,9 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     const bool live = r < rows;
     const int rr = min(r, rows - 1), i = div_small(rr, a.G, a.rcp_g), head = hk * a.G + rr - i * a.G;
     const Sees me = sees_of<PAGED>(a, sq, i);
-    // tiles that every row of the wave sees whole need no mask
-    const int hi_all = PAGED && a.tree ? max(0, min(sq.p0, sq.end)) : wave_min_i(me.hi);
-    const int lo_all = wave_max_i(me.lo);
+    int hi_all, lo_all;
+    seen_by_all<PAGED>(a, sq, div_small(min(wr0, rows - 1), a.G, a.rcp_g), div_small(min(wr0 + 31, rows - 1), a.G, a.rcp_g), me, hi_all, lo_all);
 
-    const int64_t k_rs = PAGED ? a.pg.rs : a.k_rs, v_rs = PAGED ? a.pg.rs : a.v_rs;
     const int64_t hoff = (int64_t)hk * (PAGED ? a.pg.hs : D);
     // (the queries first: under pages they arrive while the table's entries are waited for)
     bf16x8 qf[8];
@@ -79,36 +228,8 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     }
     const bool bad = tl.template stage<NW * 64>(a, b, staged);
 
-    // ---- direct loads of a tile: instruction u fills rows 4u .. 4u + 3, swizzled as attn_fwd.hip's
-    const int lrow = lane >> 4, lchunk = lane & 15;
     const uint32_t kr_lds = lds_addr(ring) + kg * NS * TILE * 4, vr_lds = kr_lds + NS * TILE * 2;
-    const bool runs = !PAGED || tl.shift >= 5;   // a whole tile's rows are one run
-    auto load_tile = [&](int x, int slot) {
-        const int key0 = tl.key0(x);
-        const uint16_t *kp = a.k + hoff, *vp = a.v + hoff;
-        if (runs && key0 + BT <= sq.end) {
-            const int64_t row = (PAGED ? key0 & ((1 << tl.shift) - 1) : key0) + 4 * rb + lrow;
-            const int64_t pg = PAGED ? (int64_t)max(tl.entry(x, 0), 0) * a.pg.ps : 0;
-            kp += pg + row * k_rs;
-            vp += pg + row * v_rs + 8 * (lchunk ^ (lrow << 2));
-#pragma unroll
-            for (int u = 0; u < LOADS; ++u) {
-                const int inst = rb + RB * u;
-                dma16(kp + 8 * (lchunk ^ ((4 * inst + lrow) & 15)), kr_lds + 2 * (slot * TILE + 512 * inst));
-                dma16(vp, vr_lds + 2 * (slot * TILE + 512 * inst));
-                kp += 4 * RB * k_rs;
-                vp += 4 * RB * v_rs;
-            }
-            return;
-        }
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-            const int inst = rb + RB * u, row = 4 * inst + lrow;
-            const int64_t o = tl.offset(a, x, row, k_rs), ov = PAGED ? o : tl.offset(a, x, row, v_rs);
-            dma16(kp + o + 8 * (lchunk ^ (row & 15)), kr_lds + 2 * (slot * TILE + 512 * inst));
-            dma16(vp + ov + 8 * (lchunk ^ (lrow << 2)), vr_lds + 2 * (slot * TILE + 512 * inst));
-        }
-    };
+    auto load_tile = [&](int x, int slot) { load_tile_rows<RB, PAGED>(a, sq, tl, hoff, x, kr_lds + 2 * slot * TILE, vr_lds + 2 * slot * TILE, rb); };
 
     const int mine = x1 > x0 + kg ? (x1 - x0 - kg + KG - 1) / KG : 0;   // tiles of this group
     const int steps = x1 > x0 ? (x1 - x0 + KG - 1) / KG : 0;             // of group 0: every group's barriers
@@ -270,12 +391,7 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     constexpr int BR = 32 * RB;
     const bool whole_block = parts == 1;
     const int64_t block = ((int64_t)b * a.nblk + blk) * a.HK + hk;
-    // (sc1: coherent at device scope, not kept in this XCD's L2; the last workgroup of the block may run on another)
-    const __amdgpu_buffer_rsrc_t rs_o = __builtin_amdgcn_make_buffer_rsrc(a.part_o + block * a.nsplit * BR * D, 0, a.nsplit * BR * D * 4, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rs_ml = __builtin_amdgcn_make_buffer_rsrc(a.part_ml + block * a.nsplit * BR * 2, 0, a.nsplit * BR * 8, 0x00020000);
-    auto put_part = [&](int q, float m, float ps) {
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(ps)}, rs_ml, (split * BR + q) * 8, 0, 16);
-    };
+    const PartRows<BR> to(a, block);
     uint64_t bits = 0;
     // (dims of block x of this group's, quarter q4: 32 (kg + KG x) + 8 q4 + 4 hf .. + 3)
     if (any) {
@@ -304,101 +420,239 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
 #pragma unroll
                 for (int q4 = 0; q4 < 4; ++q4) {
                     const f32x4 y = f32x4{own[x][4 * q4], own[x][4 * q4 + 1], own[x][4 * q4 + 2], own[x][4 * q4 + 3]};
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), rs_o,
-                                                           ((split * BR + q) * D + 32 * (kg + KG * x) + 8 * q4 + 4 * hf) * 4, 0, 16);
+                    to.put4(split, q, 32 * (kg + KG * x) + 8 * q4 + 4 * hf, y);
                 }
-            if (hf == 0 && kg == 0) put_part(q, m_used, l);
+            if (hf == 0 && kg == 0) to.put_ml(split, q, m_used, l);
         }
         bits = __builtin_amdgcn_ballot_w64(broken);
     }
-    // rows with an infinity or NaN in some group's dims again, whole, over the seen keys only
+    // ---- rows with an infinity or NaN in some group's dims again, whole, over the seen keys only
     int* again = reinterpret_cast<int*>(ring);
-    __syncthreads();   // (the merge's reads)
-    if (__syncthreads_or(bits != 0)) {
-        if (tid < RB) again[tid] = 0;
-        LR_WAIT_VMCNT(0);   // (the rows that are overwritten below)
-        __syncthreads();
-        if (lane == 0) atomicOr(again + rb, (int)(uint32_t)(bits | bits >> 32));
-        __syncthreads();
-        uint32_t left = (uint32_t)again[rb];
-        for (int nth = 0; left; left &= left - 1, ++nth) {
-            if (nth % KG != kg) continue;
-            const int q = __builtin_amdgcn_readfirstlane(__builtin_ctz(left));
-            const int ri = __builtin_amdgcn_readlane(i, q), rhead = __builtin_amdgcn_readlane(head, q);
-            redo_row<BT, PAGED>(a, sq, tl, hk, ri, rhead, [&](float o0, float o1, float m, float rl) {
-                if (whole_block) {
-                    put_row(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D, o0, o1, rl);
-                } else {
-                    __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(o0), __float_as_uint(o1)}, rs_o,
-                                                          ((split * BR + 32 * rb + q) * D + 2 * lane) * 4, 0, 16);
-                    if (lane == 0) put_part(32 * rb + q, m, rl);
-                }
-            });
-        }
-    }
-    if (whole_block || !a.merge_here) return;
+    again_rows<RB, KG>(again, rb, kg, (uint32_t)(bits | bits >> 32), [&](int q) __attribute__((always_inline)) {
+        const int ri = __builtin_amdgcn_readlane(i, q), rhead = __builtin_amdgcn_readlane(head, q);
+        redo_row<BT, PAGED>(a, sq, tl, hk, ri, rhead, [&](float o0, float o1, float m, float rl) {
+            if (whole_block) put_row(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D, o0, o1, rl);
+            else to.put_row2(split, 32 * rb + q, o0, o1, m, rl);
+        });
+    });
+    if (!whole_block && a.merge_here) to.template merge_last<NW>(a, sq, hk, row0, rows, split, parts, again);
+}
 
-    // ---- the last of the block's parts to end merges them, in their order. A part whose rows are in memory sets its flag, then
-    // reads all of them: the last to set its own sees every one (two that do write the same rows). Flags need no clearing before
-    // the call: only PART_DONE counts (as a float or a pair of them a NaN that no arithmetic makes), and who merges clears them.
-    LR_WAIT_VMCNT(0);
-    __syncthreads();   // every wave's rows are in memory
-    if (wave == 0) {   // (alone: a flag set after the merge would outlive the call)
-        uint64_t* flags = a.flags + block * a.nsplit;
-        if (lane == 0) __hip_atomic_store(flags + split, PART_DONE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        LR_WAIT_VMCNT(0);
-        bool done = true;
-        for (int s0 = 0; s0 < parts; s0 += 64)
-            done = done && __hip_atomic_load(flags + min(s0 + lane, parts - 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == PART_DONE;
-        const bool last = __builtin_amdgcn_ballot_w64(done) == ~0ull;
-        if (lane == 0) again[0] = last;
-        if (last)
-            for (int s0 = lane; s0 < parts; s0 += 64)
-                __hip_atomic_store(flags + s0, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Calls of at most 16 rows of a kv head a sequence (single tokens): the same with tiles of 16 rows, on
+// v_mfma_f32_16x16x32_bf16. What a step costs there is the time from one instruction's result to the next (a wave a SIMD, two
+// tiles each): half the scores and sums a lane, a chain of 4 products for a block of 16 keys in place of 8.
+// Lane 16 g + n: row n; of a tile's scores the keys 4 g + r and 16 + 4 g + r (r < 4), in which order its products take the keys;
+// of the sums the dims 16 db + 4 g + r.
+template <int KG, int NS, bool PAGED>
+__global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnArgs a) {
+    constexpr int BT = RANGE_TILE, TILE = BT * D, BR = 16;
+    typedef __attribute__((address_space(3))) i16x4_t lds_i16x4;
+    constexpr int RING = KG * NS * TILE * 2 * 2, MERGE = KG * (8 * 256 + 32) * 4;
+    __shared__ __attribute__((aligned(1024))) char ring[RING > MERGE ? RING : MERGE];
+    __shared__ int staged[PAGED ? RANGE_STAGED : 1];
+
+    const int tid = threadIdx.x, lane = tid & 63, kg = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+
+    // ---- which rows, which keys
+    const int at = div_small(blockIdx.x, a.nsplit, a.rcp_split), split = blockIdx.x - at * a.nsplit;
+    const int hk = at, b = blockIdx.y;   // (one block of rows a sequence and kv head)
+    // without a window a part's entries do not depend on the sequence: they are read beside its numbers
+    int early = -1;
+    const int per_tile = PAGED ? max(1, BT >> a.pg.shift) : 1;
+    const bool ahead = PAGED && !a.window && a.per * per_tile <= KG * 64;
+    if (ahead && tid < a.per * per_tile) {
+        const int j = BT * (split * a.per + tid / per_tile) + (tid % per_tile << a.pg.shift);
+        if (j >> a.pg.shift < a.pg.table_pages) early = a.pg.table[(int64_t)b * a.pg.table_rs + (j >> a.pg.shift)];
     }
-    __syncthreads();
-    if (!__builtin_amdgcn_readfirstlane(again[0])) return;
-    // 16 lanes a row (dims 8 c .. 8 c + 7), four rows a wave, eight parts in flight
-    const int mc = lane & 15;
-    for (int q0 = 4 * wave; q0 < min(BR, rows - row0); q0 += 4 * NW) {
-        const int q = min(q0 + (lane >> 4), rows - row0 - 1);   // (past the last row: that one again, the same)
-        float M = -INFINITY, L = 0.0f, sum[8] = {};
-        for (int s0 = 0; s0 < parts; s0 += 8) {
-            u32x2 ml[8];
-            u32x4 x[8][2];
+    const Seq sq = seq_of<PAGED>(a, b);
+    const int rows = max(sq.n, 0) * a.G;
+    if (rows <= 0) return;
+    TileList<BT, PAGED> tl;
+    tl.init(a, sq, 0, sq.n - 1);
+    tl.part(split, a.per);
+    const int parts = min(a.nsplit, max(1, (tl.total + a.per - 1) / a.per));   // the sequence may be shorter than the longest
+    if (split >= parts) return;
+    const int x0 = tl.x0, x1 = tl.x1;
+
+    // ---- this lane's row
+    const bool live = n < rows;
+    const int rr = min(n, rows - 1), i = div_small(rr, a.G, a.rcp_g), head = hk * a.G + rr - i * a.G;
+    const Sees me = sees_of<PAGED>(a, sq, i);
+    int hi_all, lo_all;
+    seen_by_all<PAGED>(a, sq, 0, sq.n - 1, me, hi_all, lo_all);
+
+    const int64_t hoff = (int64_t)hk * (PAGED ? a.pg.hs : D);
+    bf16x8 qf[4];
+    {
+        const uint16_t* src = a.q + (int64_t)(sq.t0 + i) * a.q_rs + head * D + 8 * g;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int at = min(s0 + u, parts - 1) * BR + q;
-                ml[u] = __builtin_amdgcn_raw_buffer_load_b64(rs_ml, at * 8, 0, 16);
-                x[u][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_o, at * D * 4 + 32 * mc, 0, 16);
-                x[u][1] = __builtin_amdgcn_raw_buffer_load_b128(rs_o, at * D * 4 + 32 * mc + 16, 0, 16);
+        for (int ks = 0; ks < 4; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(src + 32 * ks);
+    }
+    const bool bad = tl.template stage<KG * 64>(a, b, staged, ahead, early);
+
+    const uint32_t kr_lds = lds_addr(ring) + kg * NS * TILE * 4, vr_lds = kr_lds + NS * TILE * 2;
+    auto load_tile = [&](int x, int slot) { load_tile_rows<1, PAGED>(a, sq, tl, hoff, x, kr_lds + 2 * slot * TILE, vr_lds + 2 * slot * TILE, 0); };
+    const int mine = x1 > x0 + kg ? (x1 - x0 - kg + KG - 1) / KG : 0;   // tiles of this wave
+    auto tile_of = [&](int t) { return x0 + kg + t * KG; };
+    for (int t = 0; t < NS && t < mine; ++t) load_tile(tile_of(t), t);
+
+    int vtr[8];   // (dims 16 db .. of rows 4 g + (n >> 2), and 16 rows on)
+#pragma unroll
+    for (int db = 0; db < 8; ++db)
+        vtr[db] = (4 * g + (n >> 2)) * D + 8 * ((2 * db + ((n & 3) >> 1)) ^ (n >> 2 << 2)) + 4 * (n & 1);
+
+    f32x4 o[8];
+#pragma unroll
+    for (int db = 0; db < 8; ++db) o[db] = f32x4{};
+    float m_used = -INFINITY, l_sum = 0.0f;
+    const float c = a.c;
+    const bf16x2 ones2 = {(bf16)1.0f, (bf16)1.0f};
+
+    for (int t = 0; t < mine; ++t) {
+        if (NS > 1 && t + NS - 1 < mine) LR_WAIT_VMCNT((NS - 1) * 16);   // tile t has landed
+        else LR_WAIT_VMCNT(0);
+        const int x = tile_of(t), key0 = tl.key0(x);
+        const uint16_t* kt = reinterpret_cast<const uint16_t*>(ring) + kg * NS * TILE * 2 + (t % NS) * TILE;
+        const uint16_t* vt = kt + NS * TILE;
+        f32x4 s[2] = {};
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + (16 * kb + n) * D + 8 * ((4 * ks + g) ^ n));
+                s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[ks], s[kb], 0, 0, 0);
             }
-            float Mn = M;
+        bf16x8 vf[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) Mn = fmaxf(Mn, __uint_as_float(ml[u][0]));
-            const float ref = Mn > -INFINITY ? Mn : 0.0f, alpha = __builtin_amdgcn_exp2f(M - ref);
-            M = Mn;
-            L *= alpha;
+        for (int db = 0; db < 8; ++db) {
+            const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vt + vtr[db]));
+            const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vt + vtr[db] + 16 * D));
+            vf[db] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        const bool whole = key0 + BT <= hi_all && (key0 >= lo_all || key0 + BT <= a.sinks) && !bad;
+        if (!whole) {
+            const uint32_t m = seen_bits<BT, PAGED>(a, sq, tl, bad, i, me, x, 0) >> (4 * g);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e] *= alpha;
+            for (int e = 0; e < 8; ++e)
+                if (!(m >> (16 * (e >> 2) + (e & 3)) & 1)) s[e >> 2][e & 3] = -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        mx = quad_max(mx) * c;
+        if (__builtin_amdgcn_ballot_w64(mx > m_used + RESCALE_TAU)) {
+            const float mn = fmaxf(m_used, mx);
+            const float alpha = mn > -INFINITY ? __builtin_amdgcn_exp2f(m_used - mn) : 1.0f;
+            m_used = mn;
+            l_sum *= alpha;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                // a part that saw no key has no weight, whatever is in its row
-                const float m = __uint_as_float(ml[u][0]);
-                const bool in = m > -INFINITY && s0 + u < parts;
-                const float w = __builtin_amdgcn_exp2f(m - ref);
-                L = in ? fmaf(w, __uint_as_float(ml[u][1]), L) : L;
+            for (int db = 0; db < 8; ++db) o[db] *= alpha;
+        }
+        // (no key seen so far: the reference is -inf and every score -inf; any finite reference gives P = 0)
+        const float nm = m_used > -INFINITY ? -m_used : 0.0f;
+        u32x4 pw;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sum[e] = in ? fmaf(w, __uint_as_float(x[u][e >> 2][e & 3]), sum[e]) : sum[e];
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t p2 = pack_bf16x2(__builtin_amdgcn_exp2f(fmaf(s[e >> 1][2 * (e & 1)], c, nm)),
+                                            __builtin_amdgcn_exp2f(fmaf(s[e >> 1][2 * (e & 1) + 1], c, nm)));
+            pw[e] = p2;
+            l_sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p2), ones2, l_sum, false);
+        }
+        if (t + NS < mine) {   // the slot is free again once this wave's reads have returned
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            load_tile(tile_of(t + NS), t % NS);
+        }
+#pragma unroll
+        for (int db = 0; db < 8; ++db) o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[db], __builtin_bit_cast(bf16x8, pw), o[db], 0, 0, 0);
+    }
+
+    // ---- merge the waves: wave u takes the 16-dim blocks u, u + KG, ... from all of them
+    static_assert(KG > 1 && 8 % KG == 0, "waves");
+    constexpr int OWN = 8 / KG;
+    float l = quad_sum(l_sum);
+    f32x4 own[OWN] = {};
+    {
+        __syncthreads();
+        float* mo = reinterpret_cast<float*>(ring);
+        float* mml = mo + KG * 8 * 256;
+        if (live) {
+#pragma unroll
+            for (int db = 0; db < 8; ++db)
+                if (db % KG != kg) *reinterpret_cast<f32x4*>(mo + (kg * 8 + db) * 256 + 4 * lane) = o[db];
+            if (g == 0) *reinterpret_cast<float2*>(mml + kg * 32 + 2 * n) = float2{m_used, l};
+        }
+        __syncthreads();
+        if (live) {
+            float mm = -INFINITY, w[KG];
+            float2 ml[KG];
+#pragma unroll
+            for (int u = 0; u < KG; ++u) {
+                ml[u] = *reinterpret_cast<const float2*>(mml + u * 32 + 2 * n);
+                mm = fmaxf(mm, ml[u].x);
+            }
+            const float ref = mm > -INFINITY ? mm : 0.0f;
+            l = 0.0f;
+#pragma unroll
+            for (int u = 0; u < KG; ++u) {
+                w[u] = __builtin_amdgcn_exp2f(ml[u].x - ref);
+                l = fmaf(w[u], ml[u].y, l);
+            }
+            m_used = mm;
+            // (in the waves' order, whichever wave it is)
+#pragma unroll
+            for (int x = 0; x < OWN; ++x)
+#pragma unroll
+                for (int u = 0; u < KG; ++u) {
+                    f32x4 y{};
+                    if (u == kg) {
+#pragma unroll
+                        for (int g2 = 0; g2 < KG; ++g2)
+                            if (g2 == kg) y = o[g2 + KG * x];
+                    } else {
+                        y = *reinterpret_cast<const f32x4*>(mo + (u * 8 + kg + KG * x) * 256 + 4 * lane);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) own[x][e] = fmaf(w[u], y[e], own[x][e]);
+                }
+        }
+    }
+
+    // ---- rows out: O / l, or this part of them
+    const bool whole_block = parts == 1;
+    const PartRows<BR> to(a, (int64_t)b * a.HK + hk);
+    float chk = l;
+#pragma unroll
+    for (int x = 0; x < OWN; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) chk = fmaf(0.0f, own[x][e], chk);
+    const uint64_t bits = __builtin_amdgcn_ballot_w64(live && !(fabsf(chk) < INFINITY));
+    if (live) {
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        uint16_t* dst = a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D + 4 * g;
+#pragma unroll
+        for (int x = 0; x < OWN; ++x) {
+            const int dim = 16 * (kg + KG * x);
+            if (whole_block) {
+                u32x2 w;
+                w[0] = pack_bf16x2(own[x][0] * inv, own[x][1] * inv);
+                w[1] = pack_bf16x2(own[x][2] * inv, own[x][3] * inv);
+                *reinterpret_cast<u32x2*>(dst + dim) = w;
+            } else {
+                to.put4(split, n, dim + 4 * g, own[x]);
             }
         }
-        const int ri = div_small(row0 + q, a.G, a.rcp_g), rhead = hk * a.G + row0 + q - ri * a.G;
-        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-        u32x4 w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(sum[2 * e] * inv, sum[2 * e + 1] * inv);
-        *reinterpret_cast<u32x4*>(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D + 8 * mc) = w;
+        if (!whole_block && g == 0 && kg == 0) to.put_ml(split, n, m_used, l);
     }
+    // ---- rows with an infinity or NaN in some wave's dims again, whole, over the seen keys only
+    int* again = reinterpret_cast<int*>(ring);
+    const uint32_t half = (uint32_t)(bits | bits >> 32);
+    again_rows<1, KG>(again, 0, kg, (half | half >> 16) & 0xffff, [&](int q) __attribute__((always_inline)) {
+        const int ri = __builtin_amdgcn_readlane(i, q), rhead = __builtin_amdgcn_readlane(head, q);
+        redo_row<BT, PAGED>(a, sq, tl, hk, ri, rhead, [&](float o0, float o1, float m, float rl) {
+            if (whole_block) put_row(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D, o0, o1, rl);
+            else to.put_row2(split, q, o0, o1, m, rl);
+        });
+    });
+    if (!whole_block && a.merge_here) to.template merge_last<KG>(a, sq, hk, 0, rows, split, parts, again);
 }
 
 // The parts of the blocks that more than one workgroup had, a wave a row: where they are many, one workgroup a block would take
@@ -422,21 +676,19 @@ __global__ __launch_bounds__(256) void range_merge_kernel(RangeAttnArgs a) {
                 [&](int s) { return po[(int64_t)s * BR * (D / 2)]; });
 }
 
-template <int RB, int KG, int NS>
-hipError_t launch_blocks(const RangeAttnArgs& a, bool paged, hipStream_t stream) {
+template <int BR>
+hipError_t launch_blocks(const RangeAttnArgs& a, bool paged, int threads, void (*rows_kernel)(RangeAttnArgs),
+                         void (*paged_kernel)(RangeAttnArgs), hipStream_t stream) {
     const int64_t rows = (int64_t)(paged ? a.max_rows : a.W) * a.G;
-    const int64_t blocks = (rows + 32 * RB - 1) / (32 * RB) * a.HK * a.nsplit;
+    const int64_t blocks = (rows + BR - 1) / BR * a.HK * a.nsplit, merge = blocks / a.nsplit * (BR / 4);
     // (a grid's work-items and a block's bytes of parts are counted in 32 bits)
-    if (blocks > 1 << 22 || blocks / a.nsplit * 8 * RB > 1 << 23 || (int64_t)a.nsplit * 32 * RB * D * 4 > INT32_MAX)
-        return hipErrorInvalidValue;
-    const dim3 grid((unsigned)blocks, (unsigned)(paged ? a.B : 1));
-    if (paged) hipLaunchKernelGGL((range_attn_kernel<RB, KG, NS, true>), grid, dim3(RB * KG * 64), 0, stream, a);
-    else hipLaunchKernelGGL((range_attn_kernel<RB, KG, NS, false>), grid, dim3(RB * KG * 64), 0, stream, a);
+    if (blocks > 1 << 22 || merge > 1 << 23 || (int64_t)a.nsplit * BR * D * 4 > INT32_MAX) return hipErrorInvalidValue;
+    const unsigned seqs = paged ? (unsigned)a.B : 1;
+    hipLaunchKernelGGL(paged ? paged_kernel : rows_kernel, dim3((unsigned)blocks, seqs), dim3(threads), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1 || a.merge_here) return e;
-    const dim3 merge((unsigned)(blocks / a.nsplit * (8 * RB)), grid.y);
-    if (paged) hipLaunchKernelGGL((range_merge_kernel<32 * RB, true>), merge, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((range_merge_kernel<32 * RB, false>), merge, dim3(256), 0, stream, a);
+    if (paged) hipLaunchKernelGGL((range_merge_kernel<BR, true>), dim3((unsigned)merge, seqs), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((range_merge_kernel<BR, false>), dim3((unsigned)merge), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
@@ -445,11 +697,10 @@ hipError_t launch_blocks(const RangeAttnArgs& a, bool paged, hipStream_t stream)
 hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int wide, hipStream_t stream) {
     if (wide) return launch_range_wide(a, paged, wide, stream);
     const int64_t rows = (int64_t)(paged ? a.max_rows : a.W) * a.G;
-    hipError_t e;
-    if (rows <= 32) e = launch_blocks<1, 4, 2>(a, paged, stream);
-    else if (rows <= 64) e = launch_blocks<2, 2, 4>(a, paged, stream);
-    else e = launch_blocks<4, 2, 4>(a, paged, stream);
-    return e;
+    if (rows <= RANGE_STEP_ROWS) return launch_blocks<16>(a, paged, STEP_WAVES * 64, range_step_kernel<STEP_WAVES, 8 / STEP_WAVES, false>, range_step_kernel<STEP_WAVES, 8 / STEP_WAVES, true>, stream);
+    if (rows <= 32) return launch_blocks<32>(a, paged, 256, range_attn_kernel<1, 4, 2, false>, range_attn_kernel<1, 4, 2, true>, stream);
+    if (rows <= 64) return launch_blocks<64>(a, paged, 256, range_attn_kernel<2, 2, 4, false>, range_attn_kernel<2, 2, 4, true>, stream);
+    return launch_blocks<128>(a, paged, 512, range_attn_kernel<4, 2, 4, false>, range_attn_kernel<4, 2, 4, true>, stream);
 }
 
 }  // namespace lr

@@ -69,7 +69,7 @@ int64_t tiles_of(int64_t keys, int64_t span, int64_t sinks, int bt) {
 // merged faster by a second launch (in the same launch / by a second: 16 parts of 4 rows 11.9 / 14.3, of 16 rows 14.4 / 14.9, of 32
 // rows 19.3 / 17.0, of 64 rows 27.0 / 19.6).
 Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
-    const int64_t br = rows <= 32 ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
+    const int64_t br = rows <= lr::RANGE_STEP_ROWS ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
     const int64_t staged = page_size ? lr::RANGE_STAGED / std::max(1, lr::RANGE_TILE / page_size) : INT_MAX;
     int64_t ns = std::max<int64_t>(1, std::min(256 / base, (tiles + 4) / 8));
     const int64_t per = std::max<int64_t>(1, std::min((tiles + ns - 1) / ns, staged));

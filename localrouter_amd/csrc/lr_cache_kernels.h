@@ -57,6 +57,7 @@ struct RangeAttnArgs {
 // floor(2^32 / d), 2^32 - 1 for d = 1: what the kernels divide by d with.
 inline uint32_t rcp_small(int64_t d) { return d > 1 ? (uint32_t)(((uint64_t)1 << 32) / (uint64_t)d) : 0xffffffffu; }
 
+constexpr int RANGE_STEP_ROWS = 16;         // attn_cache.hip: most rows of the kernel of single tokens,
 constexpr int RANGE_TILE = 32;              // attn_cache.hip: keys a tile,
 constexpr int RANGE_STAGED = 2048;          // page-table entries a workgroup holds
 constexpr int RANGE_WIDE_TILE = 64;         // attn_cache_wide.hip: the same, and
