@@ -24,7 +24,7 @@ namespace {
 
 #include "range_attn.inc"
 
-constexpr int STEP_WAVES = 4;   // range_step_kernel's waves a workgroup
+constexpr int STEP_WAVES = 8;   // range_step_kernel's waves a workgroup
 constexpr uint64_t PART_DONE = 0x7ff4a3c57fb5d96e;
 
 // The parts of one block of BR rows. (sc1, 16: coherent at device scope, not kept in this XCD's L2; the last workgroup of the block
@@ -74,20 +74,20 @@ struct PartRows {
         }
         __syncthreads();
         if (!__builtin_amdgcn_readfirstlane(shared[0])) return;
-        // 16 lanes a row (dims 8 c .. 8 c + 7), four rows a wave, eight parts in flight
-        const int mc = lane & 15;
-        for (int q0 = 4 * wave; q0 < min(BR, rows - row0); q0 += 4 * NW) {
-            const int q = min(q0 + (lane >> 4), rows - row0 - 1);   // (past the last row: that one again, the same)
-            float M = -INFINITY, L = 0.0f, sum[8] = {};
+        // 32 lanes a row (dims 4 c .. 4 c + 3), two rows a wave, eight parts in flight
+        const int mc = lane & 31;
+        for (int q0 = 2 * wave; q0 < min(BR, rows - row0); q0 += 2 * NW) {
+            const int q = min(q0 + (lane >> 5), rows - row0 - 1);   // (past the last row: that one again, the same)
+            float M = -INFINITY, L = 0.0f;
+            f32x4 sum{};
             for (int s0 = 0; s0 < parts; s0 += 8) {
                 u32x2 ml[8];
-                u32x4 x[8][2];
+                u32x4 x[8];
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
                     const int at = min(s0 + u, parts - 1) * BR + q;
                     ml[u] = __builtin_amdgcn_raw_buffer_load_b64(rs_ml, at * 8, 0, 16);
-                    x[u][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_o, at * D * 4 + 32 * mc, 0, 16);
-                    x[u][1] = __builtin_amdgcn_raw_buffer_load_b128(rs_o, at * D * 4 + 32 * mc + 16, 0, 16);
+                    x[u] = __builtin_amdgcn_raw_buffer_load_b128(rs_o, at * D * 4 + 16 * mc, 0, 16);
                 }
                 float Mn = M;
 #pragma unroll
@@ -95,8 +95,7 @@ struct PartRows {
                 const float ref = Mn > -INFINITY ? Mn : 0.0f, alpha = __builtin_amdgcn_exp2f(M - ref);
                 M = Mn;
                 L *= alpha;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum[e] *= alpha;
+                sum *= alpha;
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
                     // a part that saw no key has no weight, whatever is in its row
@@ -105,15 +104,15 @@ struct PartRows {
                     const float w = __builtin_amdgcn_exp2f(m - ref);
                     L = in ? fmaf(w, __uint_as_float(ml[u][1]), L) : L;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sum[e] = in ? fmaf(w, __uint_as_float(x[u][e >> 2][e & 3]), sum[e]) : sum[e];
+                    for (int e = 0; e < 4; ++e) sum[e] = in ? fmaf(w, __uint_as_float(x[u][e]), sum[e]) : sum[e];
                 }
             }
             const int ri = div_small(row0 + q, a.G, a.rcp_g), rhead = hk * a.G + row0 + q - ri * a.G;
             const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-            u32x4 w;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(sum[2 * e] * inv, sum[2 * e + 1] * inv);
-            *reinterpret_cast<u32x4*>(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D + 8 * mc) = w;
+            u32x2 w;
+            w[0] = pack_bf16x2(sum[0] * inv, sum[1] * inv);
+            w[1] = pack_bf16x2(sum[2] * inv, sum[3] * inv);
+            *reinterpret_cast<u32x2*>(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D + 4 * mc) = w;
         }
     }
 };
@@ -565,7 +564,7 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
         for (int db = 0; db < 8; ++db) o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[db], __builtin_bit_cast(bf16x8, pw), o[db], 0, 0, 0);
     }
 
-    // ---- merge the waves: wave u takes the 16-dim blocks u, u + KG, ... from all of them
+    // ---- merge the waves: wave u takes the 16-dim blocks u, u + KG, ... from all of them (its own too: without a branch a block)
     static_assert(KG > 1 && 8 % KG == 0, "waves");
     constexpr int OWN = 8 / KG;
     float l = quad_sum(l_sum);
@@ -576,8 +575,7 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
         float* mml = mo + KG * 8 * 256;
         if (live) {
 #pragma unroll
-            for (int db = 0; db < 8; ++db)
-                if (db % KG != kg) *reinterpret_cast<f32x4*>(mo + (kg * 8 + db) * 256 + 4 * lane) = o[db];
+            for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4*>(mo + (kg * 8 + db) * 256 + 4 * lane) = o[db];
             if (g == 0) *reinterpret_cast<float2*>(mml + kg * 32 + 2 * n) = float2{m_used, l};
         }
         __syncthreads();
@@ -597,19 +595,11 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
                 l = fmaf(w[u], ml[u].y, l);
             }
             m_used = mm;
-            // (in the waves' order, whichever wave it is)
 #pragma unroll
             for (int x = 0; x < OWN; ++x)
 #pragma unroll
                 for (int u = 0; u < KG; ++u) {
-                    f32x4 y{};
-                    if (u == kg) {
-#pragma unroll
-                        for (int g2 = 0; g2 < KG; ++g2)
-                            if (g2 == kg) y = o[g2 + KG * x];
-                    } else {
-                        y = *reinterpret_cast<const f32x4*>(mo + (u * 8 + kg + KG * x) * 256 + 4 * lane);
-                    }
+                    const f32x4 y = *reinterpret_cast<const f32x4*>(mo + (u * 8 + kg + KG * x) * 256 + 4 * lane);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) own[x][e] = fmaf(w[u], y[e], own[x][e]);
                 }
