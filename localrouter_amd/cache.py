@@ -78,17 +78,16 @@ def _refuse(name: str, want: str, *tensors: torch.Tensor):
 
 def _rows(t: torch.Tensor, name: str, dev: int, n: int, heads: int) -> int:
     """The row stride of bf16 rows [>= n, heads, 128] on device dev."""
-    if t.dim() == 3:
-        tn, th, td = t.shape
-        rs, hs, ds = t.stride()
-        if (tn >= n and th == heads and td == 128 and ds == 1 and (hs == 128 or heads == 1) and t.dtype is _BF16
-                and t.get_device() == dev):
-            return rs if tn > 1 else heads * 128
+    s, st = t.shape, t.stride()
+    if (len(s) == 3 and s[0] >= n and s[1] == heads and s[2] == 128 and st[2] == 1 and (st[1] == 128 or heads == 1)
+            and t.dtype is _BF16 and t.get_device() == dev):
+        return st[0] if s[0] > 1 else heads * 128
     _refuse(name, f"bf16 [{n}, {heads}, 128] with contiguous heads", t)
 
 
 def _ints(t: torch.Tensor, name: str, dev: int, n: int) -> int:
-    if t.get_device() == dev and t.dtype is _I32 and t.dim() == 1 and t.numel() >= n and t.is_contiguous():
+    s = t.shape
+    if len(s) == 1 and s[0] >= n and t.dtype is _I32 and t.get_device() == dev and t.is_contiguous():
         return t.data_ptr()
     _refuse(name, f"contiguous int32 [{n}]", t)
 
@@ -97,12 +96,16 @@ def _pool(k: torch.Tensor, v: torch.Tensor, dev: int, layers: bool = False) -> t
     """([layers, layer stride,] page, row and head strides, pages, page size, heads)."""
     s, st = k.shape, k.stride()
     n = len(s)
-    if (v.shape != s or v.stride() != st or not (n == 4 or (layers and n == 5)) or s[-1] != 128 or st[-1] != 1 or 0 in s
+    if (v.shape != s or v.stride() != st or (n != 4 and (n != 5 or not layers)) or s[-1] != 128 or st[-1] != 1
             or k.dtype is not _BF16 or v.dtype is not _BF16 or k.get_device() != dev or v.get_device() != dev):
         _refuse("k_pages, v_pages", f"bf16 [n_pages, page_size, heads, 128]{' or [layers, ...]' if layers else ''} of the same "
                 "shape and strides", k, v)
-    P, R, H, _ = s[-4:]
-    ps, rs, hs, _ = st[-4:]
+    if n == 4:
+        P, R, H, _ = s
+        ps, rs, hs, _ = st
+    else:
+        L, P, R, H, _ = s
+        ls, ps, rs, hs, _ = st
     # (a dimension of one element has whatever stride its view left: taken as packed)
     if H == 1:
         hs = 128
@@ -111,16 +114,14 @@ def _pool(k: torch.Tensor, v: torch.Tensor, dev: int, layers: bool = False) -> t
     if P == 1:
         ps = (R - 1) * rs + (H - 1) * hs + 128
     if layers:
-        return s[0] if n == 5 else 1, st[0] if n == 5 and s[0] > 1 else 0, ps, rs, hs, P, R, H
+        return (L, ls if L > 1 else 0, ps, rs, hs, P, R, H) if n == 5 else (1, 0, ps, rs, hs, P, R, H)
     return ps, rs, hs, P, R, H
 
 
 def _table(t: torch.Tensor, dev: int, B: int) -> tuple:
-    if t.dim() == 2:
-        n, pages = t.shape
-        rs, es = t.stride()
-        if n >= B and (es == 1 or pages == 1) and t.dtype is _I32 and t.get_device() == dev:
-            return t.data_ptr(), rs if n > 1 else pages, pages
+    s, st = t.shape, t.stride()
+    if len(s) == 2 and s[0] >= B and (st[1] == 1 or s[1] == 1) and t.dtype is _I32 and t.get_device() == dev:
+        return t.data_ptr(), st[0] if s[0] > 1 else s[1], s[1]
     _refuse("page_table", f"int32 [{B}, pages] with contiguous rows", t)
 
 

@@ -63,21 +63,33 @@ int64_t tiles_of(int64_t keys, int64_t span, int64_t sinks, int bt) {
 }
 
 // attn_cache.hip: every block in parts of `per` tiles, one workgroup a CU. rows of a kv head a sequence; pairs: sequences x kv
-// heads. As many parts as fill one round of the CUs, of 8 tiles at least (us over the number of parts; 8 kv heads, 4 rows each: one
-// sequence of 1,900 keys 1 part 29.5, 4 15.1, 8 12.0, 16 11.9, 32 13.8; of 16,000 8 34.0, 16 23.6, 32 22.1, 48 34.3; 16 sequences of
-// 16,000 1 225, 2 188, 4 195; 16 of 1,000 1 20.9, 2 20.0, 4 27.8). The last part to end merges them where they are few; many are
-// merged faster by a second launch (in the same launch / by a second: 16 parts of 4 rows 11.9 / 14.3, of 16 rows 14.4 / 14.9, of 32
-// rows 19.3 / 17.0, of 64 rows 27.0 / 19.6).
+// heads. As many parts as fill one round of the CUs, of 8 tiles at least (us over the number of parts; 8 kv heads, 32 rows each: one
+// sequence of 1,900 keys 1 part 29.5, 4 15.1, 8 12.0, 16 11.9, 32 13.8; 16 sequences of 16,000 1 225, 2 188, 4 195; 16 of 1,000
+// 1 20.9, 2 20.0, 4 27.8). At most 16 rows: a round of eight tiles takes ~1.6 us, parts ~1.2 and eight more of them to merge
+// another 1.2 (500 keys 1 part 7.6, 2 8.6, 4 8.1; 1,900 2 parts 12.4, 4 9.9, 8 8.7, 15 9.5; 6,000 6 14.1, 12 12.4, 24 13.1; 16,000
+// over 2 heads 16 14.5, 32 13.5, 63 17.5).
+// The last part to end merges them where they are few; many are merged faster by a second launch (in the same launch / by a second:
+// 16 parts of 16 rows 14.4 / 14.9, of 32 rows 19.3 / 17.0, of 64 rows 27.0 / 19.6; the kernel of at most 16 rows, with more lanes a
+// row: 24 of 4 13.1 / 14.5, 32 of 16 20.9 / 22.1, 63 of 8 15.4 / 17.5).
 Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
     const int64_t br = rows <= lr::RANGE_STEP_ROWS ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
     const int64_t staged = page_size ? lr::RANGE_STAGED / std::max(1, lr::RANGE_TILE / page_size) : INT_MAX;
     int64_t ns = std::max<int64_t>(1, std::min(256 / base, (tiles + 4) / 8));
+    if (br == 16) {   // the kernel of single tokens: eight waves, a tile each a round
+        auto cost = [&](int64_t n) {
+            return 1.6 * (double)(((tiles + n - 1) / n + 7) / 8) + (n > 1 ? 1.2 + 1.2 * (double)((n + 7) / 8) : 0.0);
+        };
+        const int64_t most = ns;
+        ns = 1;
+        for (int64_t n = 2; n <= most; ++n)
+            if (cost(n) < cost(ns)) ns = n;
+    }
     const int64_t per = std::max<int64_t>(1, std::min((tiles + ns - 1) / ns, staged));
     ns = std::max<int64_t>(1, (tiles + per - 1) / per);
     Cut c{};
     c.nsplit = (int)ns; c.per = (int)per;
     c.nblk = (int)((rows + br - 1) / br);
-    c.merge_here = ns * std::min(rows, br) <= 256;
+    c.merge_here = ns * std::min(rows, br) <= (br == 16 ? 1024 : 256);
     c.part_rows = ns > 1 ? base * ns * br : 0;
     c.flags = ns > 1 ? base * ns : 0;
     return c;
