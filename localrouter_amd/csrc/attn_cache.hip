@@ -24,7 +24,6 @@ namespace {
 
 #include "range_attn.inc"
 
-constexpr int STEP_WAVES = 8;   // range_step_kernel's waves a workgroup
 constexpr uint64_t PART_DONE = 0x7ff4a3c57fb5d96e;
 
 // The parts of one block of BR rows. (sc1, 16: coherent at device scope, not kept in this XCD's L2; the last workgroup of the block
@@ -447,16 +446,16 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     if (!whole_block && a.merge_here) to.template merge_last<NW>(a, sq, hk, row0, rows, split, parts, again);
 }
 
-// Calls of at most 16 rows of a kv head a sequence (single tokens): the same with tiles of 16 rows, on
-// v_mfma_f32_16x16x32_bf16. What a step costs there is the time from one instruction's result to the next (a wave a SIMD, two
-// tiles each): half the scores and sums a lane, a chain of 4 products for a block of 16 keys in place of 8.
-// Lane 16 g + n: row n; of a tile's scores the keys 4 g + r and 16 + 4 g + r (r < 4), in which order its products take the keys;
-// of the sums the dims 16 db + 4 g + r.
-template <int KG, int NS, bool PAGED>
+// Calls of few rows of a kv head a sequence (single tokens, small trees): NB blocks of 16 rows, on v_mfma_f32_16x16x32_bf16. What
+// they cost is the time from one instruction's result to the next: half the scores and sums a lane of a block of 32, a chain of
+// 4 products for a block of 16 keys in place of 8, eight waves of one tile each in place of four of two.
+// Lane 16 g + n: row n of each block; of a tile's scores the keys 4 g + r and 16 + 4 g + r (r < 4), in which order its products
+// take the keys; of the sums the dims 16 db + 4 g + r.
+template <int NB, int KG, int NS, bool PAGED>
 __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnArgs a) {
-    constexpr int BT = RANGE_TILE, TILE = BT * D, BR = 16;
+    constexpr int BT = RANGE_TILE, TILE = BT * D, BR = 16 * NB;
     typedef __attribute__((address_space(3))) i16x4_t lds_i16x4;
-    constexpr int RING = KG * NS * TILE * 2 * 2, MERGE = KG * (8 * 256 + 32) * 4;
+    constexpr int RING = KG * NS * TILE * 2 * 2, MERGE = KG * NB * (8 * 256 + 32) * 4;
     __shared__ __attribute__((aligned(1024))) char ring[RING > MERGE ? RING : MERGE];
     __shared__ int staged[PAGED ? RANGE_STAGED : 1];
 
@@ -465,7 +464,7 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
 
     // ---- which rows, which keys
     const int at = div_small(blockIdx.x, a.nsplit, a.rcp_split), split = blockIdx.x - at * a.nsplit;
-    const int hk = at, b = blockIdx.y;   // (one block of rows a sequence and kv head)
+    const int blk = div_small(at, a.HK, a.rcp_hk), hk = at - blk * a.HK, b = blockIdx.y;
     // without a window a part's entries do not depend on the sequence: they are read beside its numbers
     int early = -1;
     const int per_tile = PAGED ? max(1, BT >> a.pg.shift) : 1;
@@ -475,28 +474,38 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
         if (j >> a.pg.shift < a.pg.table_pages) early = a.pg.table[(int64_t)b * a.pg.table_rs + (j >> a.pg.shift)];
     }
     const Seq sq = seq_of<PAGED>(a, b);
-    const int rows = max(sq.n, 0) * a.G;
-    if (rows <= 0) return;
+    const int row0 = blk * BR, rows = max(sq.n, 0) * a.G;   // (at most 2^30: the host checks)
+    if (row0 >= rows) return;
+    const int i_first = div_small(row0, a.G, a.rcp_g), i_last = div_small(min(rows, row0 + BR) - 1, a.G, a.rcp_g);
     TileList<BT, PAGED> tl;
-    tl.init(a, sq, 0, sq.n - 1);
+    tl.init(a, sq, i_first, i_last);
     tl.part(split, a.per);
     const int parts = min(a.nsplit, max(1, (tl.total + a.per - 1) / a.per));   // the sequence may be shorter than the longest
     if (split >= parts) return;
     const int x0 = tl.x0, x1 = tl.x1;
 
-    // ---- this lane's row
-    const bool live = n < rows;
-    const int rr = min(n, rows - 1), i = div_small(rr, a.G, a.rcp_g), head = hk * a.G + rr - i * a.G;
-    const Sees me = sees_of<PAGED>(a, sq, i);
-    int hi_all, lo_all;
-    seen_by_all<PAGED>(a, sq, 0, sq.n - 1, me, hi_all, lo_all);
-
+    // ---- this lane's rows
     const int64_t hoff = (int64_t)hk * (PAGED ? a.pg.hs : D);
-    bf16x8 qf[4];
-    {
-        const uint16_t* src = a.q + (int64_t)(sq.t0 + i) * a.q_rs + head * D + 8 * g;
+    bool live[NB];
+    int ri[NB], head[NB];
+    Sees me[NB];
+    bf16x8 qf[NB][4];
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(src + 32 * ks);
+    for (int nb = 0; nb < NB; ++nb) {
+        const int r = row0 + 16 * nb + n, rr = min(r, rows - 1);
+        live[nb] = r < rows;
+        ri[nb] = div_small(rr, a.G, a.rcp_g);
+        head[nb] = hk * a.G + rr - ri[nb] * a.G;
+        me[nb] = sees_of<PAGED>(a, sq, ri[nb]);
+        const uint16_t* src = a.q + (int64_t)(sq.t0 + ri[nb]) * a.q_rs + head[nb] * D + 8 * g;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) qf[nb][ks] = *reinterpret_cast<const bf16x8*>(src + 32 * ks);
+    }
+    int hi_all, lo_all, lo_last;
+    seen_by_all<PAGED>(a, sq, i_first, i_last, me[0], hi_all, lo_all);
+    if (NB > 1) {
+        seen_by_all<PAGED>(a, sq, i_first, i_last, me[NB - 1], hi_all, lo_last);
+        lo_all = max(lo_all, lo_last);
     }
     const bool bad = tl.template stage<KG * 64>(a, b, staged, ahead, early);
 
@@ -511,10 +520,15 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
     for (int db = 0; db < 8; ++db)
         vtr[db] = (4 * g + (n >> 2)) * D + 8 * ((2 * db + ((n & 3) >> 1)) ^ (n >> 2 << 2)) + 4 * (n & 1);
 
-    f32x4 o[8];
+    f32x4 o[NB][8];
+    float m_used[NB], l[NB];
 #pragma unroll
-    for (int db = 0; db < 8; ++db) o[db] = f32x4{};
-    float m_used = -INFINITY, l_sum = 0.0f;
+    for (int nb = 0; nb < NB; ++nb) {
+        m_used[nb] = -INFINITY;
+        l[nb] = 0.0f;
+#pragma unroll
+        for (int db = 0; db < 8; ++db) o[nb][db] = f32x4{};
+    }
     const float c = a.c;
     const bf16x2 ones2 = {(bf16)1.0f, (bf16)1.0f};
 
@@ -524,13 +538,14 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
         const int x = tile_of(t), key0 = tl.key0(x);
         const uint16_t* kt = reinterpret_cast<const uint16_t*>(ring) + kg * NS * TILE * 2 + (t % NS) * TILE;
         const uint16_t* vt = kt + NS * TILE;
-        f32x4 s[2] = {};
+        f32x4 s[NB][2] = {};
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + (16 * kb + n) * D + 8 * ((4 * ks + g) ^ n));
-                s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[ks], s[kb], 0, 0, 0);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) s[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nb][ks], s[nb][kb], 0, 0, 0);
             }
         bf16x8 vf[8];
 #pragma unroll
@@ -540,119 +555,131 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
             vf[db] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
         }
         const bool whole = key0 + BT <= hi_all && (key0 >= lo_all || key0 + BT <= a.sinks) && !bad;
-        if (!whole) {
-            const uint32_t m = seen_bits<BT, PAGED>(a, sq, tl, bad, i, me, x, 0) >> (4 * g);
+        u32x4 pw[NB];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (!(m >> (16 * (e >> 2) + (e & 3)) & 1)) s[e >> 2][e & 3] = -INFINITY;
-        }
-        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        mx = quad_max(mx) * c;
-        if (__builtin_amdgcn_ballot_w64(mx > m_used + RESCALE_TAU)) {
-            const float mn = fmaxf(m_used, mx);
-            const float alpha = mn > -INFINITY ? __builtin_amdgcn_exp2f(m_used - mn) : 1.0f;
-            m_used = mn;
-            l_sum *= alpha;
+        for (int nb = 0; nb < NB; ++nb) {
+            f32x4 &s0 = s[nb][0], &s1 = s[nb][1];
+            if (!whole) {
+                const uint32_t m = seen_bits<BT, PAGED>(a, sq, tl, bad, ri[nb], me[nb], x, 0) >> (4 * g);
 #pragma unroll
-            for (int db = 0; db < 8; ++db) o[db] *= alpha;
-        }
-        // (no key seen so far: the reference is -inf and every score -inf; any finite reference gives P = 0)
-        const float nm = m_used > -INFINITY ? -m_used : 0.0f;
-        u32x4 pw;
+                for (int e = 0; e < 4; ++e) {
+                    if (!(m >> e & 1)) s0[e] = -INFINITY;
+                    if (!(m >> (16 + e) & 1)) s1[e] = -INFINITY;
+                }
+            }
+            const float mx = c * quad_max(fmaxf(fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3])),
+                                                fmaxf(fmaxf(s1[0], s1[1]), fmaxf(s1[2], s1[3]))));
+            if (__builtin_amdgcn_ballot_w64(mx > m_used[nb] + RESCALE_TAU)) {
+                const float mn = fmaxf(m_used[nb], mx);
+                const float alpha = mn > -INFINITY ? __builtin_amdgcn_exp2f(m_used[nb] - mn) : 1.0f;
+                m_used[nb] = mn;
+                l[nb] *= alpha;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t p2 = pack_bf16x2(__builtin_amdgcn_exp2f(fmaf(s[e >> 1][2 * (e & 1)], c, nm)),
-                                            __builtin_amdgcn_exp2f(fmaf(s[e >> 1][2 * (e & 1) + 1], c, nm)));
-            pw[e] = p2;
-            l_sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p2), ones2, l_sum, false);
+                for (int db = 0; db < 8; ++db) o[nb][db] *= alpha;
+            }
+            // (no key seen so far: the reference is -inf and every score -inf; any finite reference gives P = 0)
+            const float nm = m_used[nb] > -INFINITY ? -m_used[nb] : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t p2 = pack_bf16x2(__builtin_amdgcn_exp2f(fmaf(s[nb][e >> 1][2 * (e & 1)], c, nm)),
+                                                __builtin_amdgcn_exp2f(fmaf(s[nb][e >> 1][2 * (e & 1) + 1], c, nm)));
+                pw[nb][e] = p2;
+                l[nb] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p2), ones2, l[nb], false);
+            }
         }
         if (t + NS < mine) {   // the slot is free again once this wave's reads have returned
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             load_tile(tile_of(t + NS), t % NS);
         }
 #pragma unroll
-        for (int db = 0; db < 8; ++db) o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[db], __builtin_bit_cast(bf16x8, pw), o[db], 0, 0, 0);
+        for (int db = 0; db < 8; ++db)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+                o[nb][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[db], __builtin_bit_cast(bf16x8, pw[nb]), o[nb][db], 0, 0, 0);
     }
 
-    // ---- merge the waves: wave u takes the 16-dim blocks u, u + KG, ... from all of them (its own too: without a branch a block)
-    static_assert(KG > 1 && 8 % KG == 0, "waves");
+    // ---- merge the waves: wave u takes the 16-dim blocks u, u + KG, ... from all of them (its own too: without a branch a
+    // block); rows out: O / l, or this part of them
+    static_assert(NB <= 2 && KG > 1 && 8 % KG == 0, "waves");
     constexpr int OWN = 8 / KG;
-    float l = quad_sum(l_sum);
-    f32x4 own[OWN] = {};
-    {
-        __syncthreads();
-        float* mo = reinterpret_cast<float*>(ring);
-        float* mml = mo + KG * 8 * 256;
-        if (live) {
+    const bool whole_block = parts == 1;
+    const PartRows<BR> to(a, ((int64_t)b * a.nblk + blk) * a.HK + hk);
+    float* mo = reinterpret_cast<float*>(ring);
+    float* mml = mo + KG * NB * 8 * 256;
+    __syncthreads();
 #pragma unroll
-            for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4*>(mo + (kg * 8 + db) * 256 + 4 * lane) = o[db];
-            if (g == 0) *reinterpret_cast<float2*>(mml + kg * 32 + 2 * n) = float2{m_used, l};
+    for (int nb = 0; nb < NB; ++nb) {
+        l[nb] = quad_sum(l[nb]);
+        if (live[nb]) {
+#pragma unroll
+            for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4*>(mo + ((kg * NB + nb) * 8 + db) * 256 + 4 * lane) = o[nb][db];
+            if (g == 0) *reinterpret_cast<float2*>(mml + (kg * NB + nb) * 32 + 2 * n) = float2{m_used[nb], l[nb]};
         }
-        __syncthreads();
-        if (live) {
-            float mm = -INFINITY, w[KG];
+    }
+    __syncthreads();
+    uint32_t broken = 0;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        bool mine_broken = false;
+        if (live[nb]) {
+            float mm = -INFINITY, w[KG], sum = 0.0f;
             float2 ml[KG];
 #pragma unroll
             for (int u = 0; u < KG; ++u) {
-                ml[u] = *reinterpret_cast<const float2*>(mml + u * 32 + 2 * n);
+                ml[u] = *reinterpret_cast<const float2*>(mml + (u * NB + nb) * 32 + 2 * n);
                 mm = fmaxf(mm, ml[u].x);
             }
             const float ref = mm > -INFINITY ? mm : 0.0f;
-            l = 0.0f;
 #pragma unroll
             for (int u = 0; u < KG; ++u) {
                 w[u] = __builtin_amdgcn_exp2f(ml[u].x - ref);
-                l = fmaf(w[u], ml[u].y, l);
+                sum = fmaf(w[u], ml[u].y, sum);
             }
-            m_used = mm;
+            const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+            float chk = sum;
+            uint16_t* dst = a.out + (int64_t)(sq.t0 + ri[nb]) * a.o_rs + head[nb] * D + 4 * g;
 #pragma unroll
-            for (int x = 0; x < OWN; ++x)
+            for (int x = 0; x < OWN; ++x) {
+                f32x4 own{};
 #pragma unroll
                 for (int u = 0; u < KG; ++u) {
-                    const f32x4 y = *reinterpret_cast<const f32x4*>(mo + (u * 8 + kg + KG * x) * 256 + 4 * lane);
+                    const f32x4 y = *reinterpret_cast<const f32x4*>(mo + ((u * NB + nb) * 8 + kg + KG * x) * 256 + 4 * lane);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) own[x][e] = fmaf(w[u], y[e], own[x][e]);
+                    for (int e = 0; e < 4; ++e) own[e] = fmaf(w[u], y[e], own[e]);
                 }
-        }
-    }
-
-    // ---- rows out: O / l, or this part of them
-    const bool whole_block = parts == 1;
-    const PartRows<BR> to(a, (int64_t)b * a.HK + hk);
-    float chk = l;
 #pragma unroll
-    for (int x = 0; x < OWN; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) chk = fmaf(0.0f, own[x][e], chk);
-    const uint64_t bits = __builtin_amdgcn_ballot_w64(live && !(fabsf(chk) < INFINITY));
-    if (live) {
-        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-        uint16_t* dst = a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D + 4 * g;
-#pragma unroll
-        for (int x = 0; x < OWN; ++x) {
-            const int dim = 16 * (kg + KG * x);
-            if (whole_block) {
-                u32x2 w;
-                w[0] = pack_bf16x2(own[x][0] * inv, own[x][1] * inv);
-                w[1] = pack_bf16x2(own[x][2] * inv, own[x][3] * inv);
-                *reinterpret_cast<u32x2*>(dst + dim) = w;
-            } else {
-                to.put4(split, n, dim + 4 * g, own[x]);
+                for (int e = 0; e < 4; ++e) chk = fmaf(0.0f, own[e], chk);
+                const int dim = 16 * (kg + KG * x);
+                if (whole_block) {
+                    u32x2 v;
+                    v[0] = pack_bf16x2(own[0] * inv, own[1] * inv);
+                    v[1] = pack_bf16x2(own[2] * inv, own[3] * inv);
+                    *reinterpret_cast<u32x2*>(dst + dim) = v;
+                } else {
+                    to.put4(split, 16 * nb + n, dim + 4 * g, own);
+                }
             }
+            if (!whole_block && g == 0 && kg == 0) to.put_ml(split, 16 * nb + n, mm, sum);
+            mine_broken = !(fabsf(chk) < INFINITY);
         }
-        if (!whole_block && g == 0 && kg == 0) to.put_ml(split, n, m_used, l);
+        const uint64_t bits = __builtin_amdgcn_ballot_w64(mine_broken);
+        const uint32_t half = (uint32_t)(bits | bits >> 32);
+        broken |= ((half | half >> 16) & 0xffff) << (16 * nb);
     }
     // ---- rows with an infinity or NaN in some wave's dims again, whole, over the seen keys only
     int* again = reinterpret_cast<int*>(ring);
-    const uint32_t half = (uint32_t)(bits | bits >> 32);
-    again_rows<1, KG>(again, 0, kg, (half | half >> 16) & 0xffff, [&](int q) __attribute__((always_inline)) {
-        const int ri = __builtin_amdgcn_readlane(i, q), rhead = __builtin_amdgcn_readlane(head, q);
-        redo_row<BT, PAGED>(a, sq, tl, hk, ri, rhead, [&](float o0, float o1, float m, float rl) {
-            if (whole_block) put_row(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D, o0, o1, rl);
+    again_rows<1, KG>(again, 0, kg, broken, [&](int q) __attribute__((always_inline)) {
+        int i = __builtin_amdgcn_readlane(ri[0], q & 15), h = __builtin_amdgcn_readlane(head[0], q & 15);
+        if (NB > 1 && q >= 16) {
+            i = __builtin_amdgcn_readlane(ri[NB - 1], q & 15);
+            h = __builtin_amdgcn_readlane(head[NB - 1], q & 15);
+        }
+        redo_row<BT, PAGED>(a, sq, tl, hk, i, h, [&](float o0, float o1, float m, float rl) {
+            if (whole_block) put_row(a.out + (int64_t)(sq.t0 + i) * a.o_rs + h * D, o0, o1, rl);
             else to.put_row2(split, q, o0, o1, m, rl);
         });
     });
-    if (!whole_block && a.merge_here) to.template merge_last<KG>(a, sq, hk, 0, rows, split, parts, again);
+    if (!whole_block && a.merge_here) to.template merge_last<KG>(a, sq, hk, row0, rows, split, parts, again);
 }
 
 // The parts of the blocks that more than one workgroup had, a wave a row: where they are many, one workgroup a block would take
@@ -694,12 +721,10 @@ hipError_t launch_blocks(const RangeAttnArgs& a, bool paged, int threads, void (
 
 }  // namespace
 
-hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int wide, hipStream_t stream) {
-    if (wide) return launch_range_wide(a, paged, wide, stream);
-    const int64_t rows = (int64_t)(paged ? a.max_rows : a.W) * a.G;
-    if (rows <= RANGE_STEP_ROWS) return launch_blocks<16>(a, paged, STEP_WAVES * 64, range_step_kernel<STEP_WAVES, 8 / STEP_WAVES, false>, range_step_kernel<STEP_WAVES, 8 / STEP_WAVES, true>, stream);
-    if (rows <= 32) return launch_blocks<32>(a, paged, 256, range_attn_kernel<1, 4, 2, false>, range_attn_kernel<1, 4, 2, true>, stream);
-    if (rows <= 64) return launch_blocks<64>(a, paged, 256, range_attn_kernel<2, 2, 4, false>, range_attn_kernel<2, 2, 4, true>, stream);
+hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int br, hipStream_t stream) {
+    if (br == 16) return launch_blocks<16>(a, paged, 512, range_step_kernel<1, 8, 1, false>, range_step_kernel<1, 8, 1, true>, stream);
+    if (br == 32) return launch_blocks<32>(a, paged, 512, range_step_kernel<2, 8, 1, false>, range_step_kernel<2, 8, 1, true>, stream);
+    if (br == 64) return launch_blocks<64>(a, paged, 256, range_attn_kernel<2, 2, 4, false>, range_attn_kernel<2, 2, 4, true>, stream);
     return launch_blocks<128>(a, paged, 512, range_attn_kernel<4, 2, 4, false>, range_attn_kernel<4, 2, 4, true>, stream);
 }
 

@@ -50,10 +50,10 @@ lr::PageArgs page_args(int64_t page, int64_t row, int64_t head, int n_pages, int
 }
 
 // ------------------------------------------------------------------------------------------------ range attention
-// How a call is cut: the kernel (wide: 0, or the waves of the kernel of attn_cache_wide.hip) and its blocks over the keys
+// How a call is cut: the kernel (wide: 0, or the waves of the kernel of attn_cache_wide.hip; br: attn_cache.hip's rows a block) and its blocks over the keys
 // (RangeAttnArgs: nsplit, per, whole, local, nblk), the rows of the parts and their flags.
 struct Cut {
-    int wide, nsplit, per, whole, local, nblk, merge_here, by_xcd;
+    int wide, br, nsplit, per, whole, local, nblk, merge_here, by_xcd;
     int64_t part_rows, flags;
 };
 
@@ -72,10 +72,10 @@ int64_t tiles_of(int64_t keys, int64_t span, int64_t sinks, int bt) {
 // 16 parts of 16 rows 14.4 / 14.9, of 32 rows 19.3 / 17.0, of 64 rows 27.0 / 19.6; the kernel of at most 16 rows, with more lanes a
 // row: 24 of 4 13.1 / 14.5, 32 of 16 20.9 / 22.1, 63 of 8 15.4 / 17.5).
 Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
-    const int64_t br = rows <= lr::RANGE_STEP_ROWS ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
+    const int64_t br = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
     const int64_t staged = page_size ? lr::RANGE_STAGED / std::max(1, lr::RANGE_TILE / page_size) : INT_MAX;
     int64_t ns = std::max<int64_t>(1, std::min(256 / base, (tiles + 4) / 8));
-    if (br == 16) {   // the kernel of single tokens: eight waves, a tile each a round
+    if (br <= 32) {   // the kernel of few rows: eight waves, a tile each a round
         auto cost = [&](int64_t n) {
             return 1.6 * (double)(((tiles + n - 1) / n + 7) / 8) + (n > 1 ? 1.2 + 1.2 * (double)((n + 7) / 8) : 0.0);
         };
@@ -87,9 +87,9 @@ Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
     const int64_t per = std::max<int64_t>(1, std::min((tiles + ns - 1) / ns, staged));
     ns = std::max<int64_t>(1, (tiles + per - 1) / per);
     Cut c{};
-    c.nsplit = (int)ns; c.per = (int)per;
+    c.br = (int)br; c.nsplit = (int)ns; c.per = (int)per;
     c.nblk = (int)((rows + br - 1) / br);
-    c.merge_here = ns * std::min(rows, br) <= (br == 16 ? 1024 : 256);
+    c.merge_here = ns * std::min(rows, br) <= (br <= 32 ? 1024 : 256);
     c.part_rows = ns > 1 ? base * ns * br : 0;
     c.flags = ns > 1 ? base * ns : 0;
     return c;
@@ -164,6 +164,11 @@ void set_cut(lr::RangeAttnArgs& a, void* ws, const Cut& c) {
     a.flags = reinterpret_cast<uint64_t*>(a.part_ml + 2 * c.part_rows);
 }
 
+int launch(const lr::RangeAttnArgs& a, bool paged, const Cut& c, lr_stream_t stream) {
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    return (int)(c.wide ? lr::launch_range_wide(a, paged, c.wide, s) : lr::launch_range_attn(a, paged, c.br, s));
+}
+
 bool window_sizes_ok(int W, int H, int HK, int nkeys, int window, int sinks, int frame) {
     return W >= 1 && H >= 1 && HK >= 1 && H % HK == 0 && nkeys >= 1 && nkeys <= MAX_POS && window >= 1 && sinks >= 0 &&
            frame >= 1 && (int64_t)W * (H / HK) <= MAX_POS;
@@ -217,7 +222,7 @@ int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* 
     a.W = W; a.p0 = p0; a.nkeys = nkeys; a.frame = std::min(frame, MAX_POS);   // (positions are below it either way)
     a.rcp_frame = lr::rcp_small(a.frame);
     a.window = std::min(window, MAX_POS); a.sinks = std::min(sinks, MAX_POS);
-    return (int)lr::launch_range_attn(a, false, cut.wide, reinterpret_cast<hipStream_t>(stream));
+    return launch(a, false, cut, stream);
 }
 
 size_t lr_cache_attention_ws_bytes(int B, int T, int max_rows, int max_keys, int H, int HK, int page_size, int window,
@@ -265,7 +270,7 @@ int lr_cache_attention_bf16(const void* q, int64_t q_row_stride, void* out, int6
     a.starts = starts; a.lens = lens; a.tree = tree; a.words = tree ? words : 0;
     a.B = B; a.T = T; a.max_rows = max_rows; a.max_keys = max_keys;
     a.window = std::min(window, MAX_POS); a.sinks = window ? std::min(sinks, MAX_POS) : 0;
-    return (int)lr::launch_range_attn(a, true, cut.wide, reinterpret_cast<hipStream_t>(stream));
+    return launch(a, true, cut, stream);
 }
 
 int lr_cache_append_bf16(const void* q, const void* k, const void* v, int64_t q_row_stride, int64_t k_row_stride,

@@ -57,7 +57,6 @@ struct RangeAttnArgs {
 // floor(2^32 / d), 2^32 - 1 for d = 1: what the kernels divide by d with.
 inline uint32_t rcp_small(int64_t d) { return d > 1 ? (uint32_t)(((uint64_t)1 << 32) / (uint64_t)d) : 0xffffffffu; }
 
-constexpr int RANGE_STEP_ROWS = 16;         // attn_cache.hip: most rows of the kernel of single tokens,
 constexpr int RANGE_TILE = 32;              // attn_cache.hip: keys a tile,
 constexpr int RANGE_STAGED = 2048;          // page-table entries a workgroup holds
 constexpr int RANGE_WIDE_TILE = 64;         // attn_cache_wide.hip: the same, and
@@ -65,9 +64,9 @@ constexpr int RANGE_WIDE_STAGED = 3840;     // (both of its forms: 4 and 8 waves
 constexpr int RANGE_WIDE_MIN_PAGE = 16;     // rows a page at least (of 16 rows: in pools of less than 4 GB),
 constexpr int64_t RANGE_WIDE_MAX_RS = 1 << 23;   // and row strides (elements) below this
 
-// The attention and, with a.nsplit > 1, the merge of its parts. wide: 0, or the waves of the kernel of attn_cache_wide.hip (the
-// cut's tiles are then its own).
-hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int wide, hipStream_t stream);
+// The attention and, with a.nsplit > 1, the merge of its parts: attn_cache.hip in blocks of br rows (16, 32, 64 or 128), or
+// attn_cache_wide.hip in workgroups of `waves` waves of 32 rows (the cut's tiles are each kernel's own).
+hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int br, hipStream_t stream);
 hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, int waves, hipStream_t stream);
 
 // cache_rows.hip
