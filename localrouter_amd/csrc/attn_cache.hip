@@ -9,10 +9,13 @@
 //          on are seen where the token's mask has their bit, and p is the context's length plus the bits set less one
 // A token that sees nothing gets zeros, and a key that it does not see has no part in it whatever it holds.
 //
-// The rows of one kv head (tokens x the G query heads that share it) form blocks of 32 RB rows; a workgroup of RB x KG waves
-// takes one block and one range of key tiles, its KG groups of RB waves alternate over the tiles. Products, score layout and
-// fragments are those of the pipelined kernel (attn_fwd.hip): S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16_bf16,
-// P in registers, K and V tiles row-major in LDS by direct loads.
+// The rows of one kv head (tokens x the G query heads that share it) form blocks of rows; a workgroup takes one block and one part
+// of its key tiles, its waves (or groups of waves) alternate over the tiles. S^T = K Q^T and O^T += V^T P^T with P in registers, K
+// and V tiles row-major in LDS by direct loads. Two kernels here, for the calls that the one of attn_cache_wide.hip does not take:
+//   range_step_kernel   blocks of 16 or 32 rows: single tokens, small trees; bound by the chain from one load and one instruction
+//                       to the next. 8 kv heads, one token: 500 keys 7.6 us, 1,900 8.7, 16,000 19; 64 sequences of 16,000
+//                       bound by HBM (5.7 TB/s).
+//   range_attn_kernel   blocks of 64 or 128 rows: larger batches of trees, pages of fewer than 16 rows, rows far apart.
 #include "lr_common.h"
 #include "lr_cache_kernels.h"
 
@@ -243,7 +246,7 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     const int steps = x1 > x0 ? (x1 - x0 + KG - 1) / KG : 0;             // of group 0: every group's barriers
     auto tile_of = [&](int t) { return x0 + kg + t * KG; };
 
-    constexpr int AHEAD = RB == 1 ? NS : NS - 1;   // tiles in flight before the first step
+    constexpr int AHEAD = NS - 1;   // tiles in flight before the first step
     for (int t = 0; t < AHEAD && t < mine; ++t) load_tile(tile_of(t), t);
 
     const int pr = key_perm(n);
@@ -267,13 +270,11 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     for (int t = 0; t < steps; ++t) {
         const bool have = t < mine;
         // tile t must have landed; of the later ones at most `later` may be in flight
-        if (t + AHEAD - 1 < mine && AHEAD > 1) LR_WAIT_VMCNT((AHEAD - 1) * 2 * LOADS);
+        if (t + AHEAD - 1 < mine) LR_WAIT_VMCNT((AHEAD - 1) * 2 * LOADS);
         else LR_WAIT_VMCNT(0);
-        if constexpr (RB > 1) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this wave's reads of tile t - 1, whose slot is refilled
-            block_barrier();
-            if (t + NS - 1 < mine) load_tile(tile_of(t + NS - 1), (t + NS - 1) % NS);
-        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this wave's reads of tile t - 1, whose slot is refilled
+        block_barrier();
+        if (t + NS - 1 < mine) load_tile(tile_of(t + NS - 1), (t + NS - 1) % NS);
         if (have && any) {
             const int x = tile_of(t), key0 = tl.key0(x);
             const uint16_t* kt = reinterpret_cast<const uint16_t*>(ring) + kg * NS * TILE * 2 + (t % NS) * TILE;
@@ -324,13 +325,6 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
                                                               0, 1, 2, 3, 4, 5, 6, 7);
                     o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, o[db], 0, 0, 0);
                 }
-            }
-        }
-        if constexpr (RB == 1) {
-            // this wave's own slot is free again once its reads have returned
-            if (t + NS < mine) {
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                load_tile(tile_of(t + NS), t % NS);
             }
         }
     }
@@ -443,7 +437,6 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
             else to.put_row2(split, 32 * rb + q, o0, o1, m, rl);
         });
     });
-    if (!whole_block && a.merge_here) to.template merge_last<NW>(a, sq, hk, row0, rows, split, parts, again);
 }
 
 // Calls of few rows of a kv head a sequence (single tokens, small trees): NB blocks of 16 rows, on v_mfma_f32_16x16x32_bf16. What

@@ -62,22 +62,27 @@ int64_t tiles_of(int64_t keys, int64_t span, int64_t sinks, int bt) {
     return std::min((keys + bt - 1) / bt, (std::min(sinks, keys) + bt - 1) / bt + span / bt + 2);
 }
 
-// attn_cache.hip: every block in parts of `per` tiles, one workgroup a CU. rows of a kv head a sequence; pairs: sequences x kv
-// heads. As many parts as fill one round of the CUs, of 8 tiles at least (us over the number of parts; 8 kv heads, 32 rows each: one
-// sequence of 1,900 keys 1 part 29.5, 4 15.1, 8 12.0, 16 11.9, 32 13.8; 16 sequences of 16,000 1 225, 2 188, 4 195; 16 of 1,000
-// 1 20.9, 2 20.0, 4 27.8). At most 16 rows: a round of eight tiles takes ~1.6 us, parts ~1.2 and eight more of them to merge
-// another 1.2 (500 keys 1 part 7.6, 2 8.6, 4 8.1; 1,900 2 parts 12.4, 4 9.9, 8 8.7, 15 9.5; 6,000 6 14.1, 12 12.4, 24 13.1; 16,000
-// over 2 heads 16 14.5, 32 13.5, 63 17.5).
-// The last part to end merges them where they are few; many are merged faster by a second launch (in the same launch / by a second:
-// 16 parts of 16 rows 14.4 / 14.9, of 32 rows 19.3 / 17.0, of 64 rows 27.0 / 19.6; the kernel of at most 16 rows, with more lanes a
-// row: 24 of 4 13.1 / 14.5, 32 of 16 20.9 / 22.1, 63 of 8 15.4 / 17.5).
+// attn_cache.hip: every block in parts of `per` tiles, one workgroup a CU; rows of a kv head a sequence, pairs: sequences x kv heads.
+// Blocks of 16 and 32 rows (the kernel of few rows) up to 32 rows, and up to 64 in two blocks while the keys that both read are
+// few (us of 64 rows over 8 kv heads as two blocks / as one of the other kernel: one sequence of 500 keys 10.4 / 16.6, of 16,000 22 /
+// 30; 8 and 16 of 4,000 33 / 42 and 62 / 66; 8 and 32 of 16,000 120 / 112 and 435 / 383; 32 of 500 24 / 22).
+// Parts of the kernel of few rows: as few as cost least, when a round of eight tiles takes ~1.5 us. Of at most 16 rows the last part
+// to end merges them all in ~1.2 us, eight more of them in another 1.2 (500 keys 1 part 7.6, 2 8.6, 4 8.1; 1,900 2 parts 12.4, 4 9.9,
+// 8 8.7, 15 9.5; 6,000 6 14.1, 12 12.4, 24 13.1; 16,000 over 2 heads 16 14.5, 32 13.5, 63 17.5). Of more rows a second launch does,
+// in ~2.5 us and with each part's stores (20 rows: 500 keys 1 part 10.1, 2 11.5; 1,900 4 13.1, 8 11.8, 16 12.7; 6,000 8 16.7,
+// 16 15.9, 32 18.2), but few parts of few rows (in the same launch / by a second: 8 parts of 20 rows 12.5 / 11.8, of 32 13.4 /
+// 11.9, without the second launch's ~2.5 us on the host; of 16 rows 32 20.9 / 22.1; of 8 63 15.4 / 17.5; of 4 24 13.1 / 14.5).
+// The other kernel: parts of 8 tiles at least, merged by a second launch (64 rows over 500 keys 19.1 / 16.0).
 Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
-    const int64_t br = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
+    const bool two = rows > 32 && rows <= 64 && pairs <= 128 && pairs * tiles <= 16000;
+    const int64_t br = rows <= 16 ? 16 : rows <= 32 || two ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
     const int64_t staged = page_size ? lr::RANGE_STAGED / std::max(1, lr::RANGE_TILE / page_size) : INT_MAX;
     int64_t ns = std::max<int64_t>(1, std::min(256 / base, (tiles + 4) / 8));
-    if (br <= 32) {   // the kernel of few rows: eight waves, a tile each a round
+    if (br <= 32) {
         auto cost = [&](int64_t n) {
-            return 1.6 * (double)(((tiles + n - 1) / n + 7) / 8) + (n > 1 ? 1.2 + 1.2 * (double)((n + 7) / 8) : 0.0);
+            const double rounds = (double)(((tiles + n - 1) / n + 7) / 8);
+            if (br == 16) return 1.6 * rounds + (n > 1 ? 1.2 + 1.2 * (double)((n + 7) / 8) : 0.0);
+            return 1.4 * rounds + (n > 1 ? 2.4 + 0.18 * (double)n : 0.0);
         };
         const int64_t most = ns;
         ns = 1;
@@ -89,9 +94,9 @@ Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
     Cut c{};
     c.br = (int)br; c.nsplit = (int)ns; c.per = (int)per;
     c.nblk = (int)((rows + br - 1) / br);
-    c.merge_here = ns * std::min(rows, br) <= (br <= 32 ? 1024 : 256);
+    c.merge_here = br <= 32 && ns * std::min(rows, br) <= (br == 16 ? 1024 : 128);
     c.part_rows = ns > 1 ? base * ns * br : 0;
-    c.flags = ns > 1 ? base * ns : 0;
+    c.flags = c.merge_here && ns > 1 ? base * ns : 0;
     return c;
 }
 
