@@ -62,10 +62,19 @@ int64_t tiles_of(int64_t keys, int64_t span, int64_t sinks, int bt) {
     return std::min((keys + bt - 1) / bt, (std::min(sinks, keys) + bt - 1) / bt + span / bt + 2);
 }
 
+// Whether blocks of 32 rows are taken, each reading its keys by itself, in place of 64 or of attn_cache_wide.hip's 128 and 256: one
+// round of the CUs, and few keys in all. Us with blocks of 32 / without: 64 rows over 8 kv heads, 1 sequence of 500 keys 10.4 /
+// 16.6, of 16,000 22 / 30, 8 and 16 of 4,000 33 / 42 and 62 / 66, 8 of 16,000 (64,000 tiles) 120 / 112; 128 rows over 8, 1 of 300
+// 9.5 / 15.2, of 16,000 (16,000 tiles) 26 / 31, 4 of 1,900 20 / 26, of 16,000 94 / 82; 96 over 2, 4 of 6,000 (4,500) 17 / 24, of
+// 16,000 (12,000) 39 / 30; 600 over 4, 1 of 1,900 17 / 24, of 16,000 49 / 47; 16 of 300 (1,216 blocks) 42 / 21.
+bool few_rows(int64_t rows, int64_t pairs, int64_t tiles) {
+    const int64_t blocks = (rows + 31) / 32 * pairs;
+    return rows <= 32 || (blocks <= 256 && blocks * tiles <= (rows <= 64 ? 32000 : 12000));
+}
+
 // attn_cache.hip: every block in parts of `per` tiles, one workgroup a CU; rows of a kv head a sequence, pairs: sequences x kv heads.
-// Blocks of 16 and 32 rows (the kernel of few rows) up to 32 rows, and up to 64 in two blocks while the keys that both read are
-// few (us of 64 rows over 8 kv heads as two blocks / as one of the other kernel: one sequence of 500 keys 10.4 / 16.6, of 16,000 22 /
-// 30; 8 and 16 of 4,000 33 / 42 and 62 / 66; 8 and 32 of 16,000 120 / 112 and 435 / 383; 32 of 500 24 / 22).
+// Blocks of 16 and 32 rows (the kernel of few rows) up to 32 rows a kv head, and of 32 above while there are few blocks with few
+// keys, which every block reads (few_rows). Elsewhere blocks of 64 and 128 rows.
 // Parts of the kernel of few rows: as few as cost least, when a round of eight tiles takes ~1.5 us. Of at most 16 rows the last part
 // to end merges them all in ~1.2 us, eight more of them in another 1.2 (500 keys 1 part 7.6, 2 8.6, 4 8.1; 1,900 2 parts 12.4, 4 9.9,
 // 8 8.7, 15 9.5; 6,000 6 14.1, 12 12.4, 24 13.1; 16,000 over 2 heads 16 14.5, 32 13.5, 63 17.5). Of more rows a second launch does,
@@ -74,8 +83,7 @@ int64_t tiles_of(int64_t keys, int64_t span, int64_t sinks, int bt) {
 // 11.9, without the second launch's ~2.5 us on the host; of 16 rows 32 20.9 / 22.1; of 8 63 15.4 / 17.5; of 4 24 13.1 / 14.5).
 // The other kernel: parts of 8 tiles at least, merged by a second launch (64 rows over 500 keys 19.1 / 16.0).
 Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
-    const bool two = rows > 32 && rows <= 64 && pairs <= 128 && pairs * tiles <= 16000;
-    const int64_t br = rows <= 16 ? 16 : rows <= 32 || two ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
+    const int64_t br = rows <= 16 ? 16 : few_rows(rows, pairs, tiles) ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
     const int64_t staged = page_size ? lr::RANGE_STAGED / std::max(1, lr::RANGE_TILE / page_size) : INT_MAX;
     int64_t ns = std::max<int64_t>(1, std::min(256 / base, (tiles + 4) / 8));
     if (br <= 32) {
@@ -145,15 +153,18 @@ Cut cut_wide(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool by_
 Cut window_cut(int W, int H, int HK, int nkeys, int window, int sinks, int frame, bool narrow) {
     const int64_t rows = (int64_t)W * (H / HK), tokens = std::min<int64_t>(W, 256 / (H / HK) + 2);
     const int64_t span = std::min((int64_t)window + 2, (int64_t)MAX_POS) * frame + tokens;
-    if (narrow && rows > 64) return cut_wide(rows, HK, tiles_of(nkeys, span, sinks, lr::RANGE_WIDE_TILE), 0, HK % 8 == 0);
-    return cut_small(rows, HK, tiles_of(nkeys, span, sinks, lr::RANGE_TILE), 0);
+    const int64_t tiles = tiles_of(nkeys, span, sinks, lr::RANGE_TILE);
+    if (narrow && rows > 64 && !few_rows(rows, HK, tiles))
+        return cut_wide(rows, HK, tiles_of(nkeys, span, sinks, lr::RANGE_WIDE_TILE), 0, HK % 8 == 0);
+    return cut_small(rows, HK, tiles, 0);
 }
 Cut cache_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks, bool narrow) {
     const int64_t rows = (int64_t)max_rows * (H / HK), pairs = (int64_t)B * HK;
     const int64_t span = window ? (int64_t)window + max_rows + 1 : max_keys;
-    if (narrow && rows > 64 && page_size >= lr::RANGE_WIDE_MIN_PAGE)
+    const int64_t tiles = tiles_of(max_keys, span, sinks, lr::RANGE_TILE);
+    if (narrow && rows > 64 && page_size >= lr::RANGE_WIDE_MIN_PAGE && !few_rows(rows, pairs, tiles))
         return cut_wide(rows, pairs, tiles_of(max_keys, span, sinks, lr::RANGE_WIDE_TILE), page_size, pairs % 8 == 0 || pairs >= 64);
-    return cut_small(rows, pairs, tiles_of(max_keys, span, sinks, lr::RANGE_TILE), page_size);
+    return cut_small(rows, pairs, tiles, page_size);
 }
 size_t part_bytes(const Cut& c) {
     return (((size_t)c.part_rows * lr::D * 4 + 255) & ~(size_t)255) + (((size_t)(c.part_rows + c.flags) * 8 + 255) & ~(size_t)255);
