@@ -28,10 +28,17 @@ def make_pool(g, pages, ps, HK, by_head=False, layers=None):
     return one(), one()
 
 
-class Batch:
-    """Sequences over a pool: n tokens of the call each, L positions in all."""
+# empty sequences behind a batch: the launch is sized for as many blocks of rows, more than a round of the CUs, whose choice of
+# kernel is another one (64 sequences of two kv heads, or more of one)
+PADS = [0, 61, 300]
+pads = pytest.mark.parametrize("pad", PADS)
 
-    def __init__(self, seed, news, lens, ps, HK, by_head=False, spare=3, pages=None):
+
+class Batch:
+    """Sequences over a pool: n tokens of the call each, L positions in all; pad: empty ones behind them."""
+
+    def __init__(self, seed, news, lens, ps, HK, by_head=False, spare=3, pages=None, pad=0):
+        news, lens = news + [0] * pad, lens + [0] * pad
         rng = random.Random(seed)
         self.g, self.ps, self.HK, self.news, self.L = gen(seed), ps, HK, news, lens
         need = [-(-x // ps) for x in lens]
@@ -118,10 +125,11 @@ CHAINS = [
 ]
 
 
+@pads
 @pytest.mark.parametrize("c", CHAINS, ids=lambda c: f"{len(c[0])}seq{max(c[0])}of{max(c[1])}h{c[2]}g{c[3]}p{c[4]}w{c[5]}")
-def test_attention_of_chains(c):
+def test_attention_of_chains(c, pad):
     news, lens, H, HK, ps, window, sinks, by_head = c
-    B = Batch(11, news, lens, ps, HK, by_head)
+    B = Batch(11, news, lens, ps, HK, by_head, pad=pad)
     q = rnd(B.g, sum(news), H, 128)
     out = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, max_rows=max(news), max_keys=max(lens), window=window,
                           sinks=sinks)
@@ -142,12 +150,13 @@ TREES = [
 ]
 
 
+@pads
 @pytest.mark.parametrize("c", TREES, ids=lambda c: f"{len(c[0])}seq{max(c[0])}of{max(c[1])}h{c[2]}g{c[3]}p{c[4]}w{c[5]}")
-def test_attention_of_trees(c):
+def test_attention_of_trees(c, pad):
     news, lens, H, HK, ps, window, sinks = c
     rng = random.Random(5)
     trees = [random_tree(rng, n) for n in news]
-    B = Batch(12, news, lens, ps, HK)
+    B = Batch(12, news, lens, ps, HK, pad=pad)
     q = rnd(B.g, sum(news), H, 128)
     out = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, max_rows=max(news), tree=tree_words(trees, (max(news) + 63) // 64),
                           window=window, sinks=sinks)
@@ -188,21 +197,25 @@ def test_a_tree_of_one_branch_is_a_chain():
     B.check(q, a, lambda b: chain_seen(news[b], lens[b]))
 
 
-def test_masks_that_leave_a_row_empty():
+@pads
+@pytest.mark.parametrize("heads", [2, 40])
+def test_masks_that_leave_a_row_empty(heads, pad):
     """A token whose mask has no bit, first with nothing before it (zeros), then behind a context."""
-    B = Batch(14, [3, 3], [3, 40], 16, 1)
-    q = rnd(B.g, 6, 2, 128)
+    B = Batch(14, [3, 3], [3, 40], 16, 1, pad=pad)
+    q = rnd(B.g, 6, heads, 128)
     trees = [[{0}, set(), {0, 2}], [set(), {1}, {1, 2}]]
     out = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, tree=tree_words(trees, 1))
     assert (out[1] == 0).all()
     B.check(q, out, lambda b: tree_seen(trees[b], B.L[b]))
 
 
-@pytest.mark.parametrize("news,lens,tree", [([1, 1], [70, 3000], False), ([6, 20], [70, 333], True), ([90], [200], False)])
+@pads
+@pytest.mark.parametrize("news,lens,tree", [([1, 1], [70, 3000], False), ([6, 20], [70, 333], True), ([90], [200], False),
+                                            ([6, 60], [70, 333], True)])
 @pytest.mark.parametrize("what", [float("nan"), float("inf")])
-def test_positions_that_are_not_seen_have_no_part(news, lens, tree, what):
+def test_positions_that_are_not_seen_have_no_part(news, lens, tree, what, pad):
     """Pages' rows behind the sequences' ends, free pages, and drafted tokens of other branches hold NaN or infinities."""
-    B = Batch(15, news, lens, 16, 2)
+    B = Batch(15, news, lens, 16, 2, pad=pad)
     used = torch.zeros(B.n_pages, 16, dtype=torch.bool, device="cuda")
     for b, L in enumerate(lens):
         at = torch.arange(L, device="cuda")
@@ -221,18 +234,20 @@ def test_positions_that_are_not_seen_have_no_part(news, lens, tree, what):
     B.check(q, out, lambda b: tree_seen(trees[b], lens[b]) if tree else chain_seen(news[b], lens[b]))
 
 
-def test_pages_outside_the_pool_hold_nothing():
+@pads
+@pytest.mark.parametrize("heads", [4, 80])
+def test_pages_outside_the_pool_hold_nothing(heads, pad):
     """Entries below and past the pool's pages: their positions are not seen; a sequence of nothing else gets zeros."""
     news, lens = [1, 2, 1], [100, 60, 40]
     for ps in (16, 64, 8):
-        B = Batch(16, news, lens, ps, 2)
+        B = Batch(16, news, lens, ps, 2, pad=pad)
         table = [list(r) for r in B.table]
         gone = [set(), set(), set()]
         for b, e, value in ((0, 1, -1), (0, 0, B.n_pages), (1, 0, 1 << 30), (2, None, -7)):
             for x in range(len(table[b])) if e is None else [min(e, -(-lens[b] // ps) - 1)]:
                 table[b][x] = value
                 gone[b] |= set(range(x * ps, (x + 1) * ps))
-        q = rnd(B.g, 4, 4, 128)
+        q = rnd(B.g, 4, heads, 128)
         out = cache.attention(q, B.kp, B.vp, ints(table), B.starts, B.lens)
 
         def seen(b):
@@ -243,13 +258,15 @@ def test_pages_outside_the_pool_hold_nothing():
         assert (out[3] == 0).all()
 
 
-def test_rows_behind_the_last_sequence_stay():
+@pads
+@pytest.mark.parametrize("H", [4, 40])
+def test_rows_behind_the_last_sequence_stay(H, pad):
     """A padded batch: more rows than tokens, a table wider than the sequences, sequences longer than the launch was sized
     for."""
     news, lens = [2, 1], [50, 3000]
-    B = Batch(17, news, lens, 16, 1)
-    q = rnd(B.g, 7, 4, 128)
-    out = torch.full((9, 4, 128), 3.0, dtype=BF16, device="cuda")
+    B = Batch(17, news, lens, 16, 1, pad=pad)
+    q = rnd(B.g, 7, H, 128)
+    out = torch.full((9, H, 128), 3.0, dtype=BF16, device="cuda")
     cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, out, max_rows=2)
     B.check(q, out, lambda b: chain_seen(news[b], lens[b]))
     assert (out[3:] == 3.0).all()
@@ -272,14 +289,15 @@ def test_rows_behind_the_last_sequence_stay():
     check_rows(cut[:2], *ref_rows(q[:2], k, v, ok.cpu()[None].expand(2, 64)))
 
 
+@pads
 @pytest.mark.parametrize("ps", [16, 64])
-def test_offsets_past_32_bits(ps):
+def test_offsets_past_32_bits(ps, pad):
     """A pool of more than 2^31 elements whose last pages are the ones in use."""
     HK = 8
     pages = (1 << 31) // (ps * HK * 128) + 200
     kp, vp = (torch.zeros(pages, ps, HK, 128, dtype=BF16, device="cuda") for _ in range(2))
     for news, lens in (([1, 2], [500, 130]), ([30, 21], [300, 200])):      # few and many rows of a kv head
-        B = Batch(18, news, lens, ps, HK)
+        B = Batch(18, news, lens, ps, HK, pad=pad)
         shift = pages - B.n_pages
         kp[shift:], vp[shift:] = B.kp, B.vp
         t = torch.where(B.t >= 0, B.t + shift, B.t)
@@ -314,19 +332,21 @@ def test_nothing_to_do():
     assert (out == 2.0).all() and torch.equal(B.kp, before)
 
 
+@pads
 @pytest.mark.parametrize("many", [False, True])
-def test_starts_and_lengths_that_make_no_sense(many):
+def test_starts_and_lengths_that_make_no_sense(many, pad):
     """Whatever the device's integers say, nothing outside the tensors is read or written: sequences whose numbers are out of
     order or too large do less, the others are as always."""
     news, lens = [2, 30 if many else 3, 2], [200, 150, 90]
-    B = Batch(26, news, lens, 16, 2)
+    B = Batch(26, news, lens, 16, 2, pad=pad)
     T = sum(news)
     q = rnd(B.g, T, 8, 128)
     good = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens)
     low, top = -(1 << 31), (1 << 31) - 1
-    for st, ln in (([0, 2, T + 1000, 1 << 30], lens), ([-5, 2, T - 2, T], lens), (B.st, [-3, 150, (1 << 30) + 7]),
-                   ([T, T, 0, 0], lens), (B.st, [1, 2, 1 << 29]), ([0, 2, low, T], lens), ([low, 2, top, low], lens),
+    for st, ln in (([0, 2, T + 1000, 1 << 30], lens), ([-5, 2, T - 2, T], lens), (B.st[:4], [-3, 150, (1 << 30) + 7]),
+                   ([T, T, 0, 0], lens), (B.st[:4], [1, 2, 1 << 29]), ([0, 2, low, T], lens), ([low, 2, top, low], lens),
                    ([0, 2, top, T], [low, top, top]), ([1, low, 1, top], [0, 0, 0])):
+        st, ln = st + [st[-1]] * pad, ln + [top] * pad
         out = torch.full((T + 4, 8, 128), 6.0, dtype=BF16, device="cuda")
         cache.attention(q, B.kp, B.vp, B.t, ints(st), ints(ln), out[2:2 + T])
         assert (out[:2] == 6.0).all() and (out[2 + T:] == 6.0).all()
@@ -338,11 +358,12 @@ def test_starts_and_lengths_that_make_no_sense(many):
     assert torch.equal(good, cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens))
 
 
-@pytest.mark.parametrize("rows", [4, 20])
-def test_drafted_tokens_beyond_max_rows_are_left_out(rows):
-    """As rows and as keys, on either side of the choice between the kernels."""
+@pads
+@pytest.mark.parametrize("rows", [2, 4, 7, 20])
+def test_drafted_tokens_beyond_max_rows_are_left_out(rows, pad):
+    """As rows and as keys, on either side of the choices between the kernels."""
     n, L = 70, 300
-    B = Batch(27, [n], [L], 16, 2)
+    B = Batch(27, [n], [L], 16, 2, pad=pad)
     q = rnd(B.g, n, 16, 128)
     full = [set(range(n)) if i % 2 else set(range(0, n, 3)) for i in range(n)]
     tree = tree_words([full], 2)
@@ -357,9 +378,10 @@ def test_drafted_tokens_beyond_max_rows_are_left_out(rows):
 
 
 @pytest.mark.parametrize("shape,perm", [((30, 2, 16, 2, 128), 1), ((30, 16, 2, 2, 128), 2), ((30, 16, 2, 2, 128), 3)])
-def test_keys_and_values_in_one_buffer(shape, perm):
+@pads
+def test_keys_and_values_in_one_buffer(shape, perm, pad):
     """Pages whose keys and values interleave page by page, token by token or head by head."""
-    B = Batch(28, [2, 33], [120, 150], 16, 2, pages=30)
+    B = Batch(28, [2, 33], [120, 150], 16, 2, pages=30, pad=pad)
     both = rnd(B.g, *shape)
     kp, vp = both.unbind(perm)
     assert kp.shape == B.kp.shape
@@ -373,7 +395,7 @@ def test_keys_and_values_in_one_buffer(shape, perm):
     assert torch.equal(kp, B.kp) and torch.equal(vp, B.vp)
     for few in (slice(0, 2), slice(0, 35)):
         n = few.stop
-        args = (B.t, ints([0, 2, n][:2 if n == 2 else 3]), B.lens[:1 if n == 2 else 2])
+        args = (B.t, ints([0, 2] + [n] * (pad + 1)), B.lens)
         assert torch.equal(cache.attention(q[few], kp, vp, *args), cache.attention(q[few], B.kp, B.vp, *args))
 
 

@@ -68,6 +68,37 @@ def test_window_scale_and_large_scores(scale):
     check_rows(out, *ref_rows(q, k, v, window_seen(100, 900, 800, 500, 3, 1), scale))
 
 
+@pytest.mark.parametrize("c", [c for c in CASES if c[0] * c[3] // c[4] > 64], ids=_ids)
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_window_of_many_heads(c, what):
+    """So many heads that the blocks fill more than a round of the CUs, whatever the queries; the first and the last kv heads
+    checked. Views of packed rows, and infinities and NaN in every key that no query sees."""
+    w, n, p0, H, HK, window, sinks, frame = c
+    G, many = H // HK, 96 + w % 2
+    g = gen(30 + w + n)
+    q, kv = rnd(g, w, G * many, 128), rnd(g, n, 2 * many + 1, 128)
+    k, v = kv[:, :many], kv[:, many:2 * many]
+    seen = window_seen(w, n, p0, window, sinks, frame)
+    kv[~seen.any(0).cuda()] = what
+    out = ops.attention_window(q, k, v, window=window, sinks=sinks, frame=frame, p0=p0)
+    assert torch.isfinite(out).all()
+    for hk in (0, many - 1):
+        s = slice(G * hk, G * hk + G)
+        check_rows(out[:, s], *ref_rows(q[:, s], k[:, hk:hk + 1], v[:, hk:hk + 1], seen), what=f"kv head {hk}")
+
+
+@pytest.mark.parametrize("scale", [0.02, 1.0])
+def test_window_of_many_heads_and_large_scores(scale):
+    """Scores rising along the keys, past what the first reference allows for; a NaN in a seen key of one head."""
+    g = gen(31)
+    q, k, v = rnd(g, 100, 97, 128), rnd(g, 900, 97, 128), rnd(g, 900, 97, 128)
+    k = (k.float() * torch.linspace(0.1, 2.0, 900, device="cuda")[:, None, None]).to(torch.bfloat16)
+    k[850, 5, 77] = float("nan")
+    out = ops.attention_window(q, k, v, window=500, sinks=3, p0=800, scale=scale)
+    at = [0, 5, 50, 96]
+    check_rows(out[:, at], *ref_rows(q[:, at], k[:, at], v[:, at], window_seen(100, 900, 800, 500, 3, 1), scale))
+
+
 def test_wide_window_is_causal_attention():
     g = gen(4)
     q, k, v = rnd(g, 250, 8, 128), rnd(g, 700, 2, 128), rnd(g, 700, 2, 128)
