@@ -97,7 +97,11 @@ __device__ __forceinline__ bool block_of(const RangeAttnArgs& a, int id, int& b,
 template <int QW, bool PAGED>
 __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu(2, 2))) void range_wide_kernel(RangeAttnArgs a) {
     constexpr int KBM = 32 * QW;                        // rows per block
-    constexpr int RING_LDS = 4 * IMG_TILE_BYTES;        // two key tiles, two value tiles
+    // steps of refills in flight beside the current one's. (8 waves have the LDS for 2: pages come from HBM, ~2 us away under load: 16
+    // trees of up to 64 tokens over up to 30,000 keys 860 -> 841 us; keys from L2 the same either way.)
+    constexpr int E = QW == 8 ? 2 : 0;
+    constexpr int SLOTS = 2 + E;                        // key tiles and value tiles
+    constexpr int RING_LDS = 2 * SLOTS * IMG_TILE_BYTES;
     constexpr int LP = 16 / QW;                         // direct loads of a tile per wave
     static_assert(8 / QW * (RING_LDS + 4 * RANGE_WIDE_STAGED + 256) <= 160 * 1024, "8 waves a CU");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[RING_LDS];
@@ -161,7 +165,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     const int64_t hoff = (int64_t)hk * (PAGED ? a.pg.hs : D);
     const uint64_t khead = (uint64_t)(uintptr_t)(a.k + hoff), vhead = (uint64_t)(uintptr_t)(a.v + hoff);
     const uint32_t krowb = (uint32_t)k_rs * 2u, rowb = (uint32_t)v_rs * 2u;   // (below 2^24: the host checks)
-    const uint32_t ring = lds_addr(lds), vring = ring + 2 * IMG_TILE_BYTES;
+    const uint32_t ring = lds_addr(lds), vring = ring + SLOTS * IMG_TILE_BYTES;
     const uint32_t lane16 = (uint32_t)lane * 16u;
     const uint32_t krow = (uint32_t)img_key_perm(n), kcol = (uint32_t)(32 * LP * (wv % (QW / 2)) + 16 * hf);
     const uint32_t vrow = (uint32_t)(vt_lane_row(lane) + 4 * LP * wv % 16), vchunk = (uint32_t)(16 * vt_lane_chunk(lane));
@@ -300,16 +304,16 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto slot = [](int x) __attribute__((always_inline)) { return (uint32_t)(x % 2 * IMG_TILE_BYTES); };
-    // a step's refills, one load every other slot of its first half: V(t) from slot 1 on, then K(t + 1) (past the last tile
-    // repeats of it, never read); their addresses in the slots before, under the products
+    auto slot = [](int x) __attribute__((always_inline)) { return (uint32_t)(x % SLOTS * IMG_TILE_BYTES); };
+    // a step's refills, one load every other slot of its first half: V(t + E) from slot 1 on, then K(t + E + 1) (past the last
+    // tile repeats of it, never read); their addresses in the slots before, under the products
     uint64_t src = 0;
     auto refill = [&](int f, int t) __attribute__((always_inline)) {
-        if (f == 0) src = v_src(tile_of(t));
-        if (f == 2 * LP) src = k_src(tile_of(t + 1));
+        if (f == 0) src = v_src(tile_of(t + E));
+        if (f == 2 * LP) src = k_src(tile_of(t + E + 1));
         if (f % 2 == 1) {
-            if (f / 2 < LP) load_v1(src, vring + slot(t), f / 2);
-            else if (f / 2 < 2 * LP) load_k1(src, ring + slot(t + 1), f / 2 - LP);
+            if (f / 2 < LP) load_v1(src, vring + slot(t + E), f / 2);
+            else if (f / 2 < 2 * LP) load_k1(src, ring + slot(t + E + 1), f / 2 - LP);
         }
     };
 
@@ -319,11 +323,17 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     negm = f32x16{};
     LR_WAIT_VMCNT(0);
     block_barrier();
-    {
-        v_page(tile_of(0));
-        const uint64_t vs = v_src(tile_of(0));
 #pragma unroll
-        for (int u = 0; u < LP; ++u) load_v1(vs, vring, u);
+    for (int t = 0; t <= E; ++t) {
+        v_page(tile_of(t));
+        const uint64_t vs = v_src(tile_of(t));
+#pragma unroll
+        for (int u = 0; u < LP; ++u) load_v1(vs, vring + slot(t), u);
+        k_page(tile_of(t + 1));
+        if (t == E && E == 0) break;   // (in step 0, under its products)
+        const uint64_t ks = k_src(tile_of(t + 1));
+#pragma unroll
+        for (int u = 0; u < LP; ++u) load_k1(ks, ring + slot(t + 1), u);
     }
     {
         uint32_t kb0 = ring + lane16;
@@ -340,10 +350,9 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     }
     // ---- step 0: S of half-tile 1 (K(0), fragments 8-15), P of half-tile 0
     {
-        k_page(tile_of(1));
-        const uint64_t ks = k_src(tile_of(1));   // (one tile in all: a repeat of it, never read)
-        v_page(tile_of(1));   // (of step 1's refills)
-        k_page(tile_of(2));
+        const uint64_t ks = E == 0 ? k_src(tile_of(1)) : 0;   // (one tile in all: a repeat of it, never read)
+        v_page(tile_of(1 + E));   // (of step 1's refills)
+        k_page(tile_of(2 + E));
         uint32_t kb = ring + lane16;
         asm volatile("" : "+v"(kb));
         auto rd0 = [&](int f) __attribute__((always_inline)) {
@@ -352,14 +361,14 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
         for (int f = 0; f < RA; ++f) rd0(f);
         half_step(s[1], p[1], s[0], p[0], BoolTag<false>{}, [&](int f) __attribute__((always_inline)) {
-            if ((f - RA) % 2 == 0 && f - RA < 2 * LP) load_k1(ks, ring + slot(1), (f - RA) / 2);
+            if (E == 0 && (f - RA) % 2 == 0 && f - RA < 2 * LP) load_k1(ks, ring + slot(1), (f - RA) / 2);
             rd0(f);
         });
-        LR_WAIT_VMCNT(0);
+        LR_WAIT_VMCNT(2 * E * LP);
         block_barrier();
     }
     // ---- step u: key tile u (both halves), value tile u - 1. Its refills go to the slots of V(u - 2) and K(u - 1), both
-    // read before the last barrier, and have landed at its end.
+    // read before the last barrier, and have landed at the end of step u + E.
     for (int u = 1; u < nsteps; ++u) {
         const int x = x0 + u, xp = x - 1;
         uint32_t kb = ring + slot(u) + lane16, vb = vring + slot(u - 1) + vlane;
@@ -371,8 +380,8 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         };
         auto rd_a = [&](int f) __attribute__((always_inline)) {
             if (PAGED && f == 8) {
-                v_page(tile_of(u + 1));
-                k_page(tile_of(u + 2));
+                v_page(tile_of(u + 1 + E));
+                k_page(tile_of(u + 2 + E));
             }
             if (f < 8) fr[f % FR] = frag_at(kb + (8 + f) * IMG_FRAG_BYTES);
             else if (f < 16) fr[f % FR] = vfrag_at(vb + vfrag_off(f));
@@ -386,12 +395,13 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         });
         if (special(x, 0)) mask_half(s[0], x, 0);
         half_step(s[1], p[1], s[0], p[0], BoolTag<true>{}, rd_a);
-        LR_WAIT_VMCNT(0);
+        LR_WAIT_VMCNT(2 * E * LP);
         block_barrier();
     }
     // ---- the last half-tile's P and the last value tile's products
     {
         const int u = nsteps - 1, x = x0 + u;
+        if constexpr (E > 0) LR_WAIT_VMCNT(0);   // (no load into LDS outlives the workgroup)
         if (special(x, 1)) mask_half(s[1], x, 1);
         uint32_t vb0 = vring + slot(u) + vlane;
         asm volatile("" : "+v"(vb0));
