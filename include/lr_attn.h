@@ -142,8 +142,9 @@ int lr_attention_bf16_ws(const void* q, const void* k, const void* v, void* out,
  * not see has no part in its result, whatever it holds (infinities and NaN included). Layouts, arithmetic and other
  * requirements as lr_attention_bf16, with separate k and v row strides; window >= 1, sinks >= 0, frame >= 1, nkeys and
  * p0 + W at most 2^30. out must not overlap q, k or v (rejected).
- * Calls of few rows are split over the keys: workspace of lr_attention_window_ws_bytes bytes (0: none, it may be NULL),
- * 256-byte aligned, not overlapping the tensors (rejected); calls that overlap in time on one workspace race.
+ * Calls that do not fill the GPU, and the last blocks of others, are split over the keys: workspace of
+ * lr_attention_window_ws_bytes bytes (0: none, it may be NULL), 256-byte aligned, not overlapping the tensors (rejected). What it
+ * holds before the call does not matter; calls that overlap in time on one workspace race.
  */
 size_t lr_attention_window_ws_bytes(int W, int H, int HK, int nkeys, int window, int sinks, int frame);
 int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* out, int p0, int W, int H, int HK, int nkeys,

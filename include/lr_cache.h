@@ -7,7 +7,8 @@
  * The pool. k_pages and v_pages hold n_pages pages of page_size rows (a power of two) of HK heads each: row r of page p of
  * head g at base + p * page_stride + r * row_stride + g * head_stride, in both the same strides (multiples of 8 elements, the
  * head's 128 elements contiguous). Rows of one page may lie token by token (head_stride 128) or head by head.
- * Calls over layers take base + l * layer_stride for layer l; pages have the same number in every layer.
+ * Calls over layers take base + l * layer_stride for layer l; pages have the same number in every layer. Keys and values, and
+ * layers, may interleave in one buffer; pools or layers that are the same rows are rejected.
  *
  * A batch. Sequence b < B has the tokens starts[b] .. starts[b + 1] - 1 of the call's T (n_b of them; int32 [B + 1] on the
  * device, ascending) and lens[b] positions in all (int32 [B]), the call's tokens being its last ones: the first of them at
@@ -52,10 +53,12 @@ int lr_cache_append_bf16(const void* q, const void* k, const void* v, int64_t q_
  * window >= 1: of the positions below its own (under a tree: below c_b) a token at p sees those with p - j < window or
  * j < sinks. window 0: all.
  * A token that sees nothing gets zeros; a position that it does not see has no part in its result, whatever it holds.
- * max_rows: no sequence has more tokens in the call (those beyond are left out); max_keys: no sequence has more positions
+ * max_rows: no sequence has more tokens in the call (those beyond are left out, under a tree as keys too); max_keys: no
+ * sequence has more positions
  * (those beyond are not seen). Both size the launch. At most 2^30 positions; B at most 65,535.
  * workspace: lr_cache_attention_ws_bytes bytes (0: none, it may be NULL), 256-byte aligned; it must not overlap q, out or the
- * pool, nor out q or the pool (rejected). Calls that overlap in time on one workspace race.
+ * pool, nor out q or the pool (rejected). What it holds before the call does not matter. Calls that overlap in time on one
+ * workspace race.
  */
 size_t lr_cache_attention_ws_bytes(int B, int T, int max_rows, int max_keys, int H, int HK, int page_size, int window,
                                    int sinks);

@@ -2,7 +2,9 @@
 // products bound it. The same contract; the loop is that of the key-split kernel (attn_keysplit.hip): a half-step of 16 MFMA
 // slots runs the next half-tile's scores, the previous one's products and this one's exponentials. A workgroup is 128 rows
 // (tokens x the query heads of one kv head), four waves of 32 rows over a ring of two key tiles and two value tiles; two
-// workgroups share a CU, one's start, end and waits under the other's products. What differs from there:
+// workgroups share a CU, one's start, end and waits under the other's products. Long calls that fill the CUs take 256 rows, eight
+// waves and four of each tile. What bounds them is the clock under the power limit: 16,384 tokens x 32 heads over windows of four
+// frames of 1,024 run at 1,110 TFLOP/s and ~1.7 GHz, MFMA busy ~60 %. What differs from the key-split kernel:
 //
 //  * The tiles are a list (the first tokens' tiles, then the rows' own range), and a half-tile that some row of the wave does
 //    not see whole takes a masked step: its 32 keys' visibility as one word a row, built from the row's limits (and its tree

@@ -1,5 +1,5 @@
 // Internal launch interface between the C ABI of the paged cache and the windowed attention (cache_abi.hip) and their
-// kernels (attn_cache.hip, cache_rows.hip).
+// kernels (attn_cache.hip, attn_cache_wide.hip, cache_rows.hip).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -41,10 +41,11 @@ struct RangeAttnArgs {
     int window, sinks;      // window 0 (pages only): every earlier key
     // Split over the keys: with nsplit > 1 a block of rows is nsplit workgroups, each a part of its key tiles, whose unnormalised
     // rows, references and sums go to the parts (fp32 [slot][128] and [slot][2]).
-    // attn_cache.hip: every block, `per` tiles a part, slots [block][part][row]; merged by the last part of a
-    // block to end, by the flags [block][part] (merge_here), or by a second launch. attn_cache_wide.hip: the blocks from number `whole` on, in the order in which an XCD's
-    // workgroups start (`local` blocks an XCD, or in all: see its kernel), `per` tiles a part or, per 0, equal parts; slots
-    // [block][row][part], merged by a second launch.
+    // attn_cache.hip: every block, `per` tiles a part, slots [block][part][row]; merged by the last part of a block to end, by the
+    // flags [block][part] (merge_here), or by a second launch.
+    // attn_cache_wide.hip: the blocks from number `whole` on, in the order in which an XCD's workgroups start (`local` blocks an
+    // XCD, or with by_xcd 0 in all: see its kernel), `per` tiles a part or, per 0, equal parts; slots [block][row][part], merged
+    // by a second launch.
     int nsplit, per, whole, local, merge_here, by_xcd;
     float* part_o;
     float* part_ml;
