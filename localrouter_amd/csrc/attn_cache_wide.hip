@@ -337,6 +337,25 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
         for (int u = 0; u < LP; ++u) load_k1(ks, ring + slot(t + 1), u);
     }
+    // a wave without rows only loads its share of the tiles (and leaves the clock to the others)
+    if (row0 + 32 * wv >= rows) {
+        if constexpr (E == 0) {
+            const uint64_t ks = k_src(tile_of(1));
+#pragma unroll
+            for (int u = 0; u < LP; ++u) load_k1(ks, ring + slot(1), u);
+        }
+        for (int u = 0;; ++u) {
+            v_page(tile_of(u + 1 + E));
+            k_page(tile_of(u + 2 + E));
+            LR_WAIT_VMCNT(2 * E * LP);
+            block_barrier();
+            if (u + 1 >= nsteps) break;
+#pragma unroll
+            for (int f = 0; f < 4 * LP; ++f) refill(f, u + 1);
+        }
+        LR_WAIT_VMCNT(0);
+        return;
+    }
     {
         uint32_t kb0 = ring + lane16;
         asm volatile("" : "+v"(kb0));
