@@ -96,6 +96,58 @@ __device__ __forceinline__ bool block_of(const RangeAttnArgs& a, int id, int& b,
     return true;
 }
 
+// The keys of a batch in pieces of equal length (a.teams). Sequences of one launch end when the longest does; here the pairs (sequence,
+// kv head) of an XCD lie end to end and are cut every Q tiles, so that each place has Q tiles of work whatever the lengths, and the
+// row blocks of a pair, next to each other, read the same keys at the same time (apart, each would read them from HBM). Lane j < P:
+// the piece that starts with pair j; lane P + t - 1: the one that starts at the cut t Q inside a pair. Pieces go out longest first:
+// a place whose piece was short takes the longest of the rest.
+struct Pieces {
+    int P, tiles, end, Q;   // pairs an XCD; lane j's pair: its tiles, and where it ends
+    int j, x0, x1;          // lane's piece: its pair, its tiles (none: x0 == x1)
+
+    template <int KBM>
+    __device__ __forceinline__ void init(const RangeAttnArgs& a, int xcd) {
+        const int lane = threadIdx.x & 63;
+        P = a.B * a.HK >> 3;
+        const int pair = min(lane, P - 1) * 8 + xcd;
+        const Seq sq = seq_of<true>(a, div_small(pair, a.HK, a.rcp_hk));
+        const int rows = max(sq.n, 0) * a.G;
+        tiles = lane < P && rows > 0 ? max(1, (sq.end + IMG_TILE_KEYS - 1) / IMG_TILE_KEYS) : 0;
+        end = tiles;
+        int work = tiles * ((rows + KBM - 1) / KBM);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int x = __shfl_up(end, d, 64), y = __shfl_xor(work, d, 64);
+            end += lane >= d ? x : 0;
+            work += y;
+        }
+        const int all = __builtin_amdgcn_readlane(end, 63);
+        work = __builtin_amdgcn_readfirstlane(work);
+        const int teams = work > 0 ? min(a.teams, max(1, (a.places * all + work / 2) / work)) : 1;
+        Q = max(16, (all + teams - 1) / teams);   // (shorter pieces cost more than they spread)
+        const int pos = (lane - P + 1) * Q;
+        int at = 0;   // pairs that end at or before this lane's cut
+        for (int k = 0; k < P; ++k) at += __builtin_amdgcn_readlane(end, k) <= pos;
+        j = lane < P ? lane : min(at, P - 1);
+        const int e = __shfl(end, j, 64), s = e - __shfl(tiles, j, 64);
+        const int first = lane < P ? s : pos, last = min(e, lane < P ? (s / Q + 1) * Q : pos + Q);
+        const bool is = lane < P ? tiles > 0 : pos < all && s < pos;
+        x0 = is ? first - s : 0;
+        x1 = is ? last - s : 0;
+    }
+    // the piece of rank r: its lane, or -1
+    __device__ __forceinline__ int rank(int r) const {
+        const int lane = threadIdx.x & 63, len = x1 - x0;
+        int before = 0;
+        for (int k = 0; k < 64; ++k) {
+            const int other = __builtin_amdgcn_readlane(len, k);
+            before += other > len || (other == len && k < lane);
+        }
+        const uint64_t m = __builtin_amdgcn_ballot_w64(before == r && len > 0);
+        return m ? __builtin_ctzll(m) : -1;
+    }
+};
+
 template <int QW, bool PAGED>
 __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu(2, 2))) void range_wide_kernel(RangeAttnArgs a) {
     constexpr int KBM = 32 * QW;                        // rows per block
@@ -114,32 +166,51 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, hf = lane >> 5;
 
-    int b, hk, blk, split, cut;
-    if (!block_of<PAGED>(a, blockIdx.x, b, hk, blk, split, cut)) return;
+    int b, hk, blk, split, cut, px0 = 0, px1 = 0;
+    if (PAGED && a.teams) {
+        const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3, r = div_small(idx, a.nblk, a.rcp_nblk);
+        Pieces pc;
+        pc.template init<KBM>(a, xcd);
+        const int at = pc.rank(r);
+        if (at < 0) return;
+        const int j = __builtin_amdgcn_readlane(pc.j, at), pair = 8 * j + xcd;
+        px0 = __builtin_amdgcn_readlane(pc.x0, at);
+        px1 = __builtin_amdgcn_readlane(pc.x1, at);
+        b = div_small(pair, a.HK, a.rcp_hk);
+        hk = pair - b * a.HK;
+        blk = a.nblk - 1 - (idx - r * a.nblk);
+        split = 0;
+        const bool all = px1 - px0 == __builtin_amdgcn_readlane(pc.tiles, j);
+        cut = all ? -1 : (xcd * (pc.P + a.teams) + at) * a.nblk + blk;
+    } else if (!block_of<PAGED>(a, blockIdx.x, b, hk, blk, split, cut)) {
+        return;
+    }
     b = __builtin_amdgcn_readfirstlane(b);
+    hk = __builtin_amdgcn_readfirstlane(hk);
+    blk = __builtin_amdgcn_readfirstlane(blk);
     const Seq sq = seq_of<PAGED>(a, b);
     const int row0 = blk * KBM;
     const int rows = max(sq.n, 0) * a.G;   // (at most 2^30: the host checks)
     if (row0 >= rows) return;
     TileList<BT, PAGED> tl;
     tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + KBM) - 1, a.G, a.rcp_g));
-    if (PAGED || cut >= 0) tl.part(split, a.per ? a.per : div_small(tl.total + a.nsplit - 1, a.nsplit, a.rcp_split));
+    if (PAGED && a.teams) {
+        tl.x0 = px0;
+        tl.x1 = min(tl.total, px1);
+    } else if (PAGED || cut >= 0) tl.part(split, a.per ? a.per : div_small(tl.total + a.nsplit - 1, a.nsplit, a.rcp_split));
     const bool bad = tl.template stage<64 * QW>(a, b, staged);
-    const int x0 = tl.x0, x1 = tl.x1;
+    const int x0 = __builtin_amdgcn_readfirstlane(tl.x0), x1 = __builtin_amdgcn_readfirstlane(tl.x1);
 
     // ---- this lane's row
     const int r = row0 + 32 * wv + n, rr = min(r, rows - 1);
     const bool live = r < rows;
     const int i = div_small(rr, a.G, a.rcp_g), head = hk * a.G + rr - i * a.G;
     const Sees me = sees_of<PAGED>(a, sq, i);
-    // its slot among the parts
-    auto slot_of = [&](int q) __attribute__((always_inline)) { return ((int64_t)cut * KBM + q) * a.nsplit + split; };
+    const int64_t part = (int64_t)cut * a.nsplit + split;   // its slot among the parts (merge_rows)
     if (x0 >= x1) {   // nothing to see in this part
         if (live) {
             if (cut >= 0) {
-                const int64_t at = slot_of(32 * wv + n);
-                if (hf == 0) a.part_ml[2 * at] = -INFINITY;
-                else a.part_ml[2 * at + 1] = 0.0f;
+                a.part_ml[2 * (part * KBM + 32 * wv + n) + hf] = hf ? 0.0f : -INFINITY;
             } else {
                 uint16_t* dst = a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D + 64 * hf;
 #pragma unroll
@@ -453,18 +524,13 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     again = (again | again >> 32) & 0xffffffffu;
     if (cut >= 0) {
         if (live) {
-            const int64_t at = slot_of(32 * wv + n);
-            float* po = a.part_o + at * D + 4 * hf;
+            f32x4* po = reinterpret_cast<f32x4*>(a.part_o) + (part * QW + wv) * 1024 + lane;
 #pragma unroll
             for (int db = 0; db < 4; ++db)
 #pragma unroll
                 for (int gg = 0; gg < 4; ++gg)
-                    *reinterpret_cast<f32x4*>(po + 32 * db + 8 * gg) =
-                        f32x4{o[db][4 * gg], o[db][4 * gg + 1], o[db][4 * gg + 2], o[db][4 * gg + 3]};
-            if (hf == 0) {
-                a.part_ml[2 * at] = l > 0.0f ? mref : -INFINITY;
-                a.part_ml[2 * at + 1] = l;
-            }
+                    po[64 * (4 * db + gg)] = f32x4{o[db][4 * gg], o[db][4 * gg + 1], o[db][4 * gg + 2], o[db][4 * gg + 3]};
+            a.part_ml[2 * (part * KBM + 32 * wv + n) + hf] = hf ? l : l > 0.0f ? mref : -INFINITY;
         }
     } else {
         // 8 dims a store: the lower lanes take both halves' words of the even 8-dim groups, the upper lanes of the odd ones
@@ -492,9 +558,9 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         const int ri = __builtin_amdgcn_readlane(i, q), rhead = __builtin_amdgcn_readlane(head, q);
         redo_row<BT, PAGED>(a, sq, tl, hk, ri, rhead, [&](float o0, float o1, float m, float rl) {
             if (cut >= 0) {
-                const int64_t at = slot_of(32 * wv + q);
-                *reinterpret_cast<float2*>(a.part_o + at * D + 2 * lane) = float2{o0, o1};
-                if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = float2{m, rl};
+                float* po = a.part_o + (part * QW + wv) * 4096 + 256 * (lane >> 2) + 4 * (q + 32 * (lane >> 1 & 1)) + 2 * (lane & 1);
+                *reinterpret_cast<float2*>(po) = float2{o0, o1};
+                if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * (part * KBM + 32 * wv + q)) = float2{m, rl};
             } else {
                 put_row(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D, o0, o1, rl);
             }
@@ -502,36 +568,106 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     }
 }
 
-// The parts of the blocks that were cut, a wave a row: workgroup (cut block, four rows).
-template <int KBM, bool PAGED>
+// The parts of 32 rows of a block (wave w of the workgroups that had it), by four waves, wave d the dims 32 d .. 32 d + 31. Part x
+// lies as its wave held it (slot(x)): row n's references and sums in order, its dims 8 c + 4 hf .. + 3 of 32 d at [4 d + c][n + 32 hf].
+// Four parts are in flight. A part that saw no key (reference -inf) has no weight, and its row may never have been written.
+template <int QW, class Slot>
+__device__ __forceinline__ void merge_rows(const RangeAttnArgs& a, const Seq& sq, int hk, int blk, int w, int parts, Slot&& slot) {
+    const int lane = threadIdx.x & 63, n = lane & 31, hf = lane >> 5, d = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rows = max(sq.n, 0) * a.G, r = (blk * QW + w) * 32 + n;
+    if ((blk * QW + w) * 32 >= rows) return;
+    float M = -INFINITY, L = 0.0f;
+    f32x4 sum[4] = {};
+    for (int s0 = 0; s0 < parts; s0 += 4) {
+        float2 ml[4];
+        f32x4 x[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t at = slot(min(s0 + u, parts - 1)) * QW + w;
+            ml[u] = reinterpret_cast<const float2*>(a.part_ml)[at * 32 + n];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[u][c] = reinterpret_cast<const f32x4*>(a.part_o)[at * 1024 + 64 * (4 * d + c) + lane];
+        }
+        float Mn = M;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) Mn = fmaxf(Mn, ml[u].x);
+        const float ref = Mn > -INFINITY ? Mn : 0.0f, alpha = __builtin_amdgcn_exp2f(M - ref);
+        M = Mn;
+        L *= alpha;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[c] *= alpha;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const bool in = ml[u].x > -INFINITY && s0 + u < parts;
+            const float wt = __builtin_amdgcn_exp2f(ml[u].x - ref);
+            L = in ? fmaf(wt, ml[u].y, L) : L;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[c][e] = in ? fmaf(wt, x[u][c][e], sum[c][e]) : sum[c][e];
+        }
+    }
+    if (r >= rows) return;
+    const int i = div_small(r, a.G, a.rcp_g), head = hk * a.G + r - i * a.G;
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+    uint16_t* dst = a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D + 32 * d + 4 * hf;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        u32x2 v;
+        v[0] = pack_bf16x2(sum[c][0] * inv, sum[c][1] * inv);
+        v[1] = pack_bf16x2(sum[c][2] * inv, sum[c][3] * inv);
+        *reinterpret_cast<u32x2*>(dst + 8 * c) = v;
+    }
+}
+
+// The parts of the blocks that were cut: workgroup (cut block, 32 rows).
+template <int QW, bool PAGED>
 __global__ __launch_bounds__(256) void range_wide_merge_kernel(RangeAttnArgs a) {
-    const int c = blockIdx.x / (KBM / 4), q = blockIdx.x % (KBM / 4) * 4 + (threadIdx.x >> 6);
+    const int c = blockIdx.x / QW, w = blockIdx.x % QW;
     const int of = a.local - a.whole;   // cut blocks an XCD
     const int xcd = a.by_xcd ? c / of : 0, first = a.whole + (c - xcd * of) * a.nsplit;   // the block's first workgroup
     int b, hk, blk, split, cut;
     if (!block_of<PAGED>(a, a.by_xcd ? 8 * first + xcd : first, b, hk, blk, split, cut)) return;
     b = __builtin_amdgcn_readfirstlane(b);
     const Seq sq = seq_of<PAGED>(a, b);
-    const int r = blk * KBM + q;
-    if (r >= max(sq.n, 0) * a.G) return;
-    const int i = div_small(r, a.G, a.rcp_g), head = hk * a.G + r - i * a.G;
-    const int64_t at = ((int64_t)cut * KBM + q) * a.nsplit;
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at;
-    const float2* po = reinterpret_cast<const float2*>(a.part_o) + at * (D / 2) + (threadIdx.x & 63);
-    merge_parts(a.nsplit, a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D, [&](int s) { return ml[s]; },
-                [&](int s) { return po[(int64_t)s * (D / 2)]; });
+    merge_rows<QW>(a, sq, hk, blk, w, a.nsplit, [&](int x) { return (int64_t)cut * a.nsplit + x; });
+}
+
+// The same of pieces: workgroup (pair, row block, 32 rows).
+template <int QW>
+__global__ __launch_bounds__(256) void range_pieces_merge_kernel(RangeAttnArgs a) {
+    const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3, c = at / QW, j = div_small(c, a.nblk, a.rcp_nblk), blk = c - j * a.nblk;
+    Pieces pc;
+    pc.template init<32 * QW>(a, xcd);
+    const int e = __builtin_amdgcn_readlane(pc.end, j), s = e - __builtin_amdgcn_readlane(pc.tiles, j), t0 = s / pc.Q;
+    const int parts = 1 + (max(e - 1, 0) / pc.Q - t0);
+    if (s == e || parts <= 1) return;   // (the attention wrote its rows)
+    const int pair = 8 * j + xcd, b = div_small(pair, a.HK, a.rcp_hk), hk = pair - b * a.HK;
+    const Seq sq = seq_of<true>(a, b);
+    merge_rows<QW>(a, sq, hk, blk, at % QW, parts, [&](int x) {
+        return (int64_t)(xcd * (pc.P + a.teams) + (x == 0 ? j : pc.P + t0 + x - 1)) * a.nblk + blk;
+    });
 }
 
 template <int QW, bool PAGED>
 hipError_t launch_waves(const RangeAttnArgs& a, hipStream_t stream) {
+    if constexpr (PAGED)
+        if (a.teams) {
+            const int64_t pairs = (int64_t)a.B * a.HK, blocks = (pairs + 8 * a.teams) * a.nblk, merge = pairs * a.nblk * QW;
+            hipLaunchKernelGGL((range_wide_kernel<QW, PAGED>), dim3((unsigned)blocks), dim3(64 * QW), 0, stream, a);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+            hipLaunchKernelGGL(range_pieces_merge_kernel<QW>, dim3((unsigned)merge), dim3(256), 0, stream, a);
+            return hipGetLastError();
+        }
     const int xcds = a.by_xcd ? 8 : 1;
     const int64_t of = a.nsplit > 1 ? a.local - a.whole : 0;   // cut blocks
-    const int64_t blocks = xcds * (a.local + of * (a.nsplit - 1)), merge = xcds * of * (8 * QW);
+    const int64_t blocks = xcds * (a.local + of * (a.nsplit - 1)), merge = xcds * of * QW;
     if (blocks > 1 << 22 || merge > 1 << 23) return hipErrorInvalidValue;   // (a grid's work-items are counted in 32 bits)
     hipLaunchKernelGGL((range_wide_kernel<QW, PAGED>), dim3((unsigned)blocks), dim3(64 * QW), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || of == 0) return e;
-    hipLaunchKernelGGL((range_wide_merge_kernel<32 * QW, PAGED>), dim3((unsigned)merge), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((range_wide_merge_kernel<QW, PAGED>), dim3((unsigned)merge), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 

@@ -53,7 +53,7 @@ lr::PageArgs page_args(int64_t page, int64_t row, int64_t head, int n_pages, int
 // How a call is cut: the kernel (wide: 0, or the waves of the kernel of attn_cache_wide.hip; br: attn_cache.hip's rows a block) and its blocks over the keys
 // (RangeAttnArgs: nsplit, per, whole, local, nblk), the rows of the parts and their flags.
 struct Cut {
-    int wide, br, nsplit, per, whole, local, nblk, merge_here, by_xcd;
+    int wide, br, nsplit, per, whole, local, nblk, merge_here, by_xcd, teams, places;
     int64_t part_rows, flags;
 };
 
@@ -150,6 +150,27 @@ Cut cut_wide(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool by_
     return c;
 }
 
+// attn_cache_wide.hip's pieces of equal length, for batches of long sequences in at most three rounds of blocks of more than 128 rows
+// (us with whole blocks / pieces; 8 kv heads, lengths from N / 2, from N / 20, all N): 16 x 256 rows, N 8,000 162 / 138, 132 / 103,
+// 174 / 168; N 30,000 535 / 445, 507 / 355, 605 / 521; 40 x 256, N 30,000 1160 / 957, 897 / 689, 1965 / 1257; 16 x 512, N 8,000
+// 222 / 219, 217 / 160, 270 / 263; N 30,000 820 / 785, 782 / 629, 926 / 932. Not short ones (40 x 256, N 2,000 61 / 91 from N / 20),
+// nor of 128 rows (16 x 128, N 30,000 368 / 385, 339 / 303, 409 / 474). Workgroups of 256 rows where they hold as few empty rows as
+// those of 128 (16 x 320 rows over 2 heads, N 30,000, of 256 / of 128: 258 / 179, 209 / 168, 303 / 224; whole blocks 193, 189, 206).
+void cut_pieces(Cut& c, int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
+    if (rows <= 128 || pairs % 8 || tiles < 64) return;
+    const int waves = (rows + 255) / 256 * 2 == (rows + 127) / 128 ? 8 : 4;
+    const int64_t P = pairs / 8, places = waves == 8 ? 32 : 64, nblk = (rows + 32 * waves - 1) / (32 * waves);
+    // (nblk: of more blocks a pair is balanced without, and the parts would take gigabytes)
+    if (P > 48 || nblk > places / 8 || P * nblk > 3 * places || P * nblk * tiles < 60 * places) return;
+    const int64_t teams = std::min<int64_t>(places, 64 - P), least = std::max<int64_t>(1, std::min(teams, places / nblk));
+    const int64_t longest = std::max<int64_t>(16, (P * tiles + least - 1) / least);   // what a workgroup holds page entries for
+    if (longest * std::max(1, lr::RANGE_WIDE_TILE / page_size) > lr::RANGE_WIDE_STAGED) return;
+    c.wide = waves; c.nblk = (int)nblk; c.by_xcd = 1;
+    c.nsplit = 1; c.per = 0;
+    c.teams = (int)teams; c.places = (int)places;
+    c.part_rows = 8 * (P + teams) * nblk * 32 * waves;
+}
+
 Cut window_cut(int W, int H, int HK, int nkeys, int window, int sinks, int frame, bool narrow) {
     const int64_t rows = (int64_t)W * (H / HK), tokens = std::min<int64_t>(W, 256 / (H / HK) + 2);
     const int64_t span = std::min((int64_t)window + 2, (int64_t)MAX_POS) * frame + tokens;
@@ -162,8 +183,12 @@ Cut cache_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, i
     const int64_t rows = (int64_t)max_rows * (H / HK), pairs = (int64_t)B * HK;
     const int64_t span = window ? (int64_t)window + max_rows + 1 : max_keys;
     const int64_t tiles = tiles_of(max_keys, span, sinks, lr::RANGE_TILE);
-    if (narrow && rows > 64 && page_size >= lr::RANGE_WIDE_MIN_PAGE && !few_rows(rows, pairs, tiles))
-        return cut_wide(rows, pairs, tiles_of(max_keys, span, sinks, lr::RANGE_WIDE_TILE), page_size, pairs % 8 == 0 || pairs >= 64);
+    if (narrow && rows > 64 && page_size >= lr::RANGE_WIDE_MIN_PAGE && !few_rows(rows, pairs, tiles)) {
+        const int64_t wide_tiles = tiles_of(max_keys, span, sinks, lr::RANGE_WIDE_TILE);
+        Cut c = cut_wide(rows, pairs, wide_tiles, page_size, pairs % 8 == 0 || pairs >= 64);
+        if (B > 1 && !window) cut_pieces(c, rows, pairs, wide_tiles, page_size);
+        return c;
+    }
     return cut_small(rows, pairs, tiles, page_size);
 }
 size_t part_bytes(const Cut& c) {
@@ -171,6 +196,7 @@ size_t part_bytes(const Cut& c) {
 }
 void set_cut(lr::RangeAttnArgs& a, void* ws, const Cut& c) {
     a.nsplit = c.nsplit; a.per = c.per; a.whole = c.whole; a.local = c.local; a.nblk = c.nblk; a.merge_here = c.merge_here; a.by_xcd = c.by_xcd;
+    a.teams = c.teams; a.places = c.places;
     a.rcp_split = lr::rcp_small(c.nsplit);
     a.rcp_nblk = lr::rcp_small(c.nblk);
     a.rcp_g = lr::rcp_small(a.G);

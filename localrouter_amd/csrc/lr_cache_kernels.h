@@ -46,7 +46,9 @@ struct RangeAttnArgs {
     // attn_cache_wide.hip: the blocks from number `whole` on, in the order in which an XCD's workgroups start (`local` blocks an
     // XCD, or with by_xcd 0 in all: see its kernel), `per` tiles a part or, per 0, equal parts; slots [block][row][part], merged
     // by a second launch.
-    int nsplit, per, whole, local, merge_here, by_xcd;
+    // teams > 0 (attn_cache_wide.hip): cut by the sequences' own lengths into pieces of equal length, up to `teams` of them an XCD
+    // whose `places` workgroups are resident at once.
+    int nsplit, per, whole, local, merge_here, by_xcd, teams, places;
     float* part_o;
     float* part_ml;
     uint64_t* flags;

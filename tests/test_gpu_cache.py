@@ -188,6 +188,71 @@ def test_attention_of_whole_rounds(ps, tree):
         check_rows(out[rows], *ref_rows(q[rows], k, v, seen), what=f"sequence {b}")
 
 
+@pytest.mark.parametrize("H,rows,ps", [(80, 20, 16), (80, 20, 64), (64, 40, 32), (128, 32, 16)])   # 200, 320 and 512 rows
+@pytest.mark.parametrize("tree", [False, True])
+def test_attention_of_ragged_batches(H, rows, ps, tree):
+    """Batches cut into pieces of equal length: sequences of very different lengths, some without tokens or hardly any keys, a page
+    that the pool does not have, NaN behind the sequences; then the same launch over other lengths, captured and replayed."""
+    rng = random.Random(H + ps)
+    news = [rows, 3, 0, rows - 1] + [rng.randrange(1, rows + 1) for _ in range(12)]
+    lens = [4000, 3, 700, rows - 1, 64, 65, 128 + rows, 1500] + [rng.randrange(rows, 900) for _ in range(8)]
+    news[4], news[5] = min(news[4], 64), min(news[5], 65)
+    B = Batch(34, news, lens, ps, 8)
+    used = torch.zeros(B.n_pages, ps, dtype=torch.bool, device="cuda")
+    for b, L in enumerate(lens):
+        at = torch.arange(L, device="cuda")
+        used[B.t[b][at // ps].long(), at % ps] = True
+    B.kp[~used], B.vp[~used] = float("nan"), float("inf")
+    table = [list(r) for r in B.table]
+    table[7][2] = B.n_pages + 5
+    gone = list(range(2 * ps, 3 * ps))
+    t = ints(table)
+    T = sum(news)
+    q = rnd(B.g, T, H, 128)
+    trees = [random_tree(rng, n) for n in news]
+    words = tree_words(trees, 1) if tree else None
+    kw = dict(max_rows=rows, max_keys=16000, tree=words)
+    need = cache.attention_ws_bytes(16, T, rows, B.width * ps, H, 8, ps)
+    need = max(need, cache.attention_ws_bytes(16, T, rows, 16000, H, 8, ps))
+    ws = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")
+    wide = torch.cat([t, torch.full((16, 16000 // ps - B.width), -1, dtype=torch.int32, device="cuda")], 1)
+    out = torch.full((T + 2, H, 128), 9.0, dtype=BF16, device="cuda")
+    lens_t = B.lens.clone()
+    call = lambda: cache.attention(q, B.kp, B.vp, wide, B.starts, lens_t, out[:T], workspace=ws, **kw)
+
+    def check(L):
+        for b, n in enumerate(news):
+            if not n:
+                continue
+            at = sorted({0, n // 2, n - 1}) if L[b] > 300 else list(range(n))
+            seen = (tree_seen(trees[b], L[b]) if tree else chain_seen(n, L[b]))[at]
+            if b == 7:
+                seen[:, [j for j in gone if j < L[b]]] = False
+            p = torch.arange(L[b], device="cuda")
+            page = B.t[b][p // ps].long()
+            r = [B.st[b] + i for i in at]
+            check_rows(out[r], *ref_rows(q[r], B.kp[page, p % ps], B.vp[page, p % ps], seen), what=f"sequence {b}")
+        assert (out[T:] == 9.0).all() and (ws[need:] == 255).all()
+
+    call()
+    check(lens)
+    first = out.clone()
+    call()
+    assert torch.equal(out, first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    other = [max(n, L // 3) for n, L in zip(news, lens)]
+    other[0] = 4000 if tree else rows      # (the longest stays, or is the first tokens alone)
+    for L in (other, lens):
+        lens_t.copy_(ints(L))
+        out[:T].fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(L)
+    assert torch.equal(out, first)
+
+
 def test_a_tree_of_one_branch_is_a_chain():
     news, lens = [9, 70], [100, 70]
     B = Batch(13, news, lens, 16, 2)
