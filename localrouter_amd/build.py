@@ -62,6 +62,23 @@ RESOURCES = PKG / "_build" / "resources.json"
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-ffp-contract=off"]
 
 
+# the host side of cache.py's calls: a Python extension over torch's own headers, linked to nothing but torch
+HOST_CALLS = PKG / "native" / "host_calls.cpp"
+HOST_CALLS_LIB = PKG / "_host_calls.so"
+
+
+def host_calls_cmd(out: Path) -> list[str]:
+    import importlib.util
+    import sysconfig
+    spec = importlib.util.find_spec("torch")   # (found, not imported)
+    if spec is None:
+        raise RuntimeError("torch not found (its headers are required to build localrouter_amd)")
+    torch_dir = Path(spec.origin).parent
+    return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", str(HOST_CALLS),
+            "-o", str(out), f"-I{torch_dir / 'include'}", f"-I{torch_dir / 'include/torch/csrc/api/include'}",
+            f"-I{sysconfig.get_paths()['include']}", f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+
+
 def hipcc() -> str:
     for cand in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
         if cand and Path(cand).exists():
@@ -175,6 +192,9 @@ def build(verbose: bool = False) -> Path:
     tmp = LIB.with_suffix(".so.tmp")
     _run([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, *LIBS, "-o", str(tmp)])
     os.replace(tmp, LIB)
+    tmp = HOST_CALLS_LIB.with_suffix(".so.tmp")
+    _run(host_calls_cmd(tmp))
+    os.replace(tmp, HOST_CALLS_LIB)
     return LIB
 
 

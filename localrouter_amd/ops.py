@@ -19,7 +19,6 @@ torch supplies device memory and the stream handle only; all compute is the libr
 """
 from __future__ import annotations
 
-import functools
 import math
 
 import torch
@@ -114,15 +113,10 @@ def attention_ws(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.T
     return out
 
 
-@functools.lru_cache(maxsize=1024)
-def _window_ws_bytes(*sizes: int) -> int:
-    return int(_lib.load().lr_attention_window_ws_bytes(*sizes))
-
-
 def attention_window_ws_bytes(w: int, heads: int, kv_heads: int, nkeys: int, *, window: int, sinks: int = 0,
                               frame: int = 1) -> int:
     """lr_attention_window_ws_bytes: the workspace lr_attention_window_bf16 needs (0: none)."""
-    return _window_ws_bytes(w, heads, kv_heads, nkeys, window, sinks, frame)
+    return int(_lib.load().lr_attention_window_ws_bytes(w, heads, kv_heads, nkeys, window, sinks, frame))
 
 
 def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor | None = None, *, window: int,
@@ -131,36 +125,9 @@ def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: tor
     """lr_attention_window_bf16: q [w, heads, 128] at positions p0 + i over k / v [nkeys, kv_heads, 128]; a query in frame
     f = position // frame sees the keys of frames f - window + 1 .. f and the first `sinks` keys (up to frame f). frame 1: a
     sliding window of single tokens. A workspace of attention_window_ws_bytes is allocated when none is given."""
-    if not q.is_cuda:
-        raise ValueError(f"attention_window: expected tensors on the GPU, got one on {q.device}")
-    dev = torch._C._cuda_getDevice()
-    w, heads = q.shape[0], q.shape[1]
-    nkeys, kv_heads = k.shape[0], k.shape[1]
-    if out is None:
-        out = torch.empty((w, heads, D), dtype=torch.bfloat16, device=q.device)
-    strides = []
-    for t, n, h in ((q, w, heads), (k, nkeys, kv_heads), (v, nkeys, kv_heads), (out, w, heads)):
-        s, st = t.shape, t.stride()
-        if (t.get_device() != dev or t.dtype is not torch.bfloat16 or len(s) != 3 or s[0] < n or s[1] != h or s[2] != D
-                or st[2] != 1 or (st[1] != D and h > 1)):
-            raise ValueError(f"attention_window: expected bf16 [{n}, {h}, 128] with contiguous heads on the current device, got "
-                             f"{t.dtype} {tuple(s)} / {st} on {t.device}")
-        strides.append(st[0] if s[0] > 1 else h * D)
-    if max(window, sinks, frame, p0) >= 1 << 31:
-        raise ValueError("attention_window: window, sinks, frame and p0 are 32-bit numbers")
-    need = _window_ws_bytes(w, heads, kv_heads, nkeys, window, sinks, frame)
-    ws, nbytes = None, 0
-    if workspace is not None:
-        nbytes = workspace.numel() * workspace.element_size()
-        if nbytes < need or workspace.get_device() != dev or not workspace.is_contiguous():
-            raise ValueError(f"workspace: {need} contiguous bytes on the current device needed")
-        ws = workspace.data_ptr()
-    elif need:
-        workspace, nbytes = torch.empty(need, dtype=torch.uint8, device=q.device), need
-        ws = workspace.data_ptr()
-    _lib.call("lr_attention_window_bf16", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), p0, w, heads, kv_heads,
-              nkeys, window, sinks, frame, scale, *strides, ws, nbytes, torch._C._cuda_getCurrentRawStream(dev))
-    return out
+    from . import cache   # (its host calls; it imports this module)
+    dev = cache._device(q)
+    return cache._host().attention_window(dev, cache._raw_stream(dev), q, k, v, out, window, sinks, frame, p0, scale, workspace)
 
 
 def attention_kmask(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kmask: torch.Tensor | None,

@@ -223,3 +223,25 @@ def test_pool_compact_packs_to_the_front():
     assert tables == [[moved.get(p, p) for p in t] for t in before] and sorted({p for t in tables for p in t}) == [0, 1, 2, 3]
     assert c == d and pool.free_pages == 4 and sorted(pool.alloc(4)) == [4, 5, 6, 7]
     assert pool.compact([]) == ([], []) if pool.free_pages == 8 else True
+
+
+def test_host_calls_refuse_host_tensors_by_name():
+    """The calls' own checks, past the Python side's: every tensor is refused by its name, with what it is."""
+    h = cache._host()
+    t = torch.zeros(4, 2, 128, dtype=torch.bfloat16)
+    p = torch.zeros(3, 16, 2, 128, dtype=torch.bfloat16)
+    i = torch.zeros(5, dtype=torch.int32)
+    with pytest.raises(ValueError, match=r"q: expected bf16 \[4, 2, 128\].*BFloat16 \[4, 2, 128\] / \[256, 128, 1\] on cpu"):
+        h.attention(-1, 0, t, p, p, i[None], i, i[:1], None, None, None, None, 0, 0, 0.1, None)
+    with pytest.raises(ValueError, match="k_pages, v_pages"):
+        h.append(-1, 0, t, t, t, p, p, i[None], i, i[:1], None, None, None, 0, None, None, None, 0, 128, 1e-6)
+    with pytest.raises(ValueError, match="k_pages, v_pages: expected .* or .layers"):
+        h.copy_pages(-1, 0, p, p, i, i)
+    with pytest.raises(ValueError, match="k_pages: expected a tensor on the current device, got NoneType"):
+        h.move_rows(-1, 0, None, p, i[None], i, i, i, None)
+    with pytest.raises(ValueError, match="q: expected bf16"):
+        h.attention_window(-1, 0, t, t, t, None, 4, 0, 1, 0, 0.1, None)
+    with pytest.raises(TypeError):
+        h.attention(1, 2, 3)
+    with pytest.raises(TypeError):
+        h.attention("cuda", 0, t, p, p, i[None], i, i[:1], None, None, None, None, 0, 0, 0.1, None)
