@@ -76,23 +76,21 @@ struct PartRows {
         }
         __syncthreads();
         if (!__builtin_amdgcn_readfirstlane(shared[0])) return;
-        // LPR lanes a row (V float4s each), 64 / LPR rows a wave, eight parts in flight. (More lanes a row are a shorter chain; of
-        // more than 16 rows a workgroup then has twice the passes.)
-        constexpr int LPR = BR <= 16 ? 32 : 16, V = 32 / LPR, RW = 64 / LPR;
-        const int mc = lane % LPR;
-        for (int q0 = RW * wave; q0 < min(BR, rows - row0); q0 += RW * NW) {
-            const int q = min(q0 + lane / LPR, rows - row0 - 1);   // (past the last row: that one again, the same)
+        // 32 lanes a row (dims 4 c .. 4 c + 3), two rows a wave, eight parts in flight
+        static_assert(BR == 2 * NW, "one pass");
+        const int mc = lane & 31;
+        if (2 * wave < rows - row0) {
+            const int q = min(2 * wave + (lane >> 5), rows - row0 - 1);   // (past the last row: that one again, the same)
             float M = -INFINITY, L = 0.0f;
-            f32x4 sum[V] = {};
+            f32x4 sum{};
             for (int s0 = 0; s0 < parts; s0 += 8) {
                 u32x2 ml[8];
-                u32x4 x[8][V];
+                u32x4 x[8];
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
                     const int at = min(s0 + u, parts - 1) * BR + q;
                     ml[u] = __builtin_amdgcn_raw_buffer_load_b64(rs_ml, at * 8, 0, 16);
-#pragma unroll
-                    for (int d = 0; d < V; ++d) x[u][d] = __builtin_amdgcn_raw_buffer_load_b128(rs_o, at * D * 4 + 16 * (V * mc + d), 0, 16);
+                    x[u] = __builtin_amdgcn_raw_buffer_load_b128(rs_o, at * D * 4 + 16 * mc, 0, 16);
                 }
                 float Mn = M;
 #pragma unroll
@@ -100,8 +98,7 @@ struct PartRows {
                 const float ref = Mn > -INFINITY ? Mn : 0.0f, alpha = __builtin_amdgcn_exp2f(M - ref);
                 M = Mn;
                 L *= alpha;
-#pragma unroll
-                for (int d = 0; d < V; ++d) sum[d] *= alpha;
+                sum *= alpha;
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
                     // a part that saw no key has no weight, whatever is in its row
@@ -110,21 +107,15 @@ struct PartRows {
                     const float w = __builtin_amdgcn_exp2f(m - ref);
                     L = in ? fmaf(w, __uint_as_float(ml[u][1]), L) : L;
 #pragma unroll
-                    for (int d = 0; d < V; ++d)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sum[d][e] = in ? fmaf(w, __uint_as_float(x[u][d][e]), sum[d][e]) : sum[d][e];
+                    for (int e = 0; e < 4; ++e) sum[e] = in ? fmaf(w, __uint_as_float(x[u][e]), sum[e]) : sum[e];
                 }
             }
             const int ri = div_small(row0 + q, a.G, a.rcp_g), rhead = hk * a.G + row0 + q - ri * a.G;
             const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-            uint16_t* dst = a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D + 4 * V * mc;
-#pragma unroll
-            for (int d = 0; d < V; ++d) {
-                u32x2 w;
-                w[0] = pack_bf16x2(sum[d][0] * inv, sum[d][1] * inv);
-                w[1] = pack_bf16x2(sum[d][2] * inv, sum[d][3] * inv);
-                *reinterpret_cast<u32x2*>(dst + 4 * d) = w;
-            }
+            u32x2 w;
+            w[0] = pack_bf16x2(sum[0] * inv, sum[1] * inv);
+            w[1] = pack_bf16x2(sum[2] * inv, sum[3] * inv);
+            *reinterpret_cast<u32x2*>(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D + 4 * mc) = w;
         }
     }
 };
@@ -672,7 +663,8 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
             else to.put_row2(split, q, o0, o1, m, rl);
         });
     });
-    if (!whole_block && a.merge_here) to.template merge_last<KG>(a, sq, hk, row0, rows, split, parts, again);
+    if constexpr (NB == 1)
+        if (!whole_block && a.merge_here) to.template merge_last<KG>(a, sq, hk, row0, rows, split, parts, again);
 }
 
 // The parts of the blocks that more than one workgroup had, a wave a row: where they are many, one workgroup a block would take

@@ -79,9 +79,9 @@ bool few_rows(int64_t rows, int64_t pairs, int64_t tiles) {
 // to end merges them all in ~1.2 us, eight more of them in another 1.2 (500 keys 1 part 7.6, 2 8.6, 4 8.1; 1,900 2 parts 12.4, 4 9.9,
 // 8 8.7, 15 9.5; 6,000 6 14.1, 12 12.4, 24 13.1; 16,000 over 2 heads 16 14.5, 32 13.5, 63 17.5). Of more rows a second launch does,
 // in ~2.5 us and with each part's stores (20 rows: 500 keys 1 part 10.1, 2 11.5; 1,900 4 13.1, 8 11.8, 16 12.7; 6,000 8 16.7,
-// 16 15.9, 32 18.2), but few parts of few rows (in the same launch / by a second: 8 parts of 20 rows 12.5 / 11.8, of 32 13.4 /
-// 11.9, without the second launch's ~2.5 us on the host; of 16 rows 32 20.9 / 22.1; of 8 63 15.4 / 17.5; of 4 24 13.1 / 14.5).
-// The other kernel: parts of 8 tiles at least, merged by a second launch (64 rows over 500 keys 19.1 / 16.0).
+// 16 15.9, 32 18.2). In the same launch / by a second: 24 parts of 4 rows 13.1 / 14.5, 63 of 8 15.4 / 17.5, 32 of 16 20.9 / 22.1, 8 of
+// 20 12.5 / 11.8, 8 of 32 13.4 / 11.9, 2 of 64 19.1 / 16.0.
+// The other kernel: parts of 8 tiles at least, merged by a second launch.
 Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
     const int64_t br = rows <= 16 ? 16 : few_rows(rows, pairs, tiles) ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
     const int64_t staged = page_size ? lr::RANGE_STAGED / std::max(1, lr::RANGE_TILE / page_size) : INT_MAX;
@@ -102,7 +102,7 @@ Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
     Cut c{};
     c.br = (int)br; c.nsplit = (int)ns; c.per = (int)per;
     c.nblk = (int)((rows + br - 1) / br);
-    c.merge_here = br <= 32 && ns * std::min(rows, br) <= (br == 16 ? 1024 : 128);
+    c.merge_here = br == 16 && ns * std::min(rows, br) <= 1024;
     c.part_rows = ns > 1 ? base * ns * br : 0;
     c.flags = c.merge_here && ns > 1 ? base * ns : 0;
     return c;
