@@ -153,7 +153,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     constexpr int KBM = 32 * QW;                        // rows per block
     // steps of refills in flight beside the current one's. (8 waves have the LDS for 2: pages come from HBM, ~2 us away under load: 16
     // trees of up to 64 tokens over up to 30,000 keys 860 -> 841 us. Rows come from the L2s: 16,384 tokens of video 1,171 us with 2,
-    // 1,164 with 0 on one box.)
+    // 1,164 with 0.)
     constexpr int E = QW == 8 && PAGED ? 2 : 0;
     constexpr int SLOTS = 2 + E;                        // key tiles and value tiles
     constexpr int RING_LDS = 2 * SLOTS * IMG_TILE_BYTES;
