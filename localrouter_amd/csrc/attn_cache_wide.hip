@@ -155,9 +155,12 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     // trees of up to 64 tokens over up to 30,000 keys 860 -> 841 us. Rows come from the L2s: 16,384 tokens of video 1,171 us with 2,
     // 1,164 with 0.)
     constexpr int E = QW == 8 && PAGED ? 2 : 0;
+    constexpr int LP = 16 / QW;                         // direct loads of a tile per wave
+    // loads in flight at a step's end, when the next step's keys and this one's values have landed; with E > 0 a step early, so that
+    // the next step's first key fragments are read before the barrier (the trees 811 -> 798 us)
+    constexpr int AHEAD = E > 0 ? (E - 1) * 2 * LP : 0;
     constexpr int SLOTS = 2 + E;                        // key tiles and value tiles
     constexpr int RING_LDS = 2 * SLOTS * IMG_TILE_BYTES;
-    constexpr int LP = 16 / QW;                         // direct loads of a tile per wave
     static_assert(8 / QW * (RING_LDS + 4 * RANGE_WIDE_STAGED + 256) <= 160 * 1024, "8 waves a CU");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[RING_LDS];
     __shared__ int staged[PAGED ? RANGE_WIDE_STAGED : 1];
@@ -419,7 +422,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         for (int u = 0;; ++u) {
             v_page(tile_of(u + 1 + E));
             k_page(tile_of(u + 2 + E));
-            LR_WAIT_VMCNT(2 * E * LP);
+            LR_WAIT_VMCNT(AHEAD);
             block_barrier();
             if (u + 1 >= nsteps) break;
 #pragma unroll
@@ -457,15 +460,21 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
             if (E == 0 && (f - RA) % 2 == 0 && f - RA < 2 * LP) load_k1(ks, ring + slot(1), (f - RA) / 2);
             rd0(f);
         });
-        LR_WAIT_VMCNT(2 * E * LP);
+        LR_WAIT_VMCNT(AHEAD);
         block_barrier();
+        if constexpr (E > 0) {
+            uint32_t kn = ring + slot(1) + lane16;
+            asm volatile("" : "+v"(kn));
+#pragma unroll
+            for (int f = 0; f < RA; ++f) fr[f % FR] = frag_at(kn + f * IMG_FRAG_BYTES);
+        }
     }
     // ---- step u: key tile u (both halves), value tile u - 1. Its refills go to the slots of V(u - 2) and K(u - 1), both
-    // read before the last barrier, and have landed at the end of step u + E.
+    // read before the last barrier, and have landed at the end of step u (of step u + E - 1 with E > 0).
     for (int u = 1; u < nsteps; ++u) {
         const int x = x0 + u, xp = x - 1;
-        uint32_t kb = ring + slot(u) + lane16, vb = vring + slot(u - 1) + vlane;
-        asm volatile("" : "+v"(kb), "+v"(vb));
+        uint32_t kb = ring + slot(u) + lane16, vb = vring + slot(u - 1) + vlane, kn = ring + slot(u + 1) + lane16;
+        asm volatile("" : "+v"(kb), "+v"(vb), "+v"(kn));
         auto rd_b = [&](int f) __attribute__((always_inline)) {
             if (f < 8) fr[f % FR] = frag_at(kb + f * IMG_FRAG_BYTES);
             else if (f < 16) fr[f % FR] = vfrag_at(vb + vfrag_off(f - 8));
@@ -478,9 +487,11 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
             }
             if (f < 8) fr[f % FR] = frag_at(kb + (8 + f) * IMG_FRAG_BYTES);
             else if (f < 16) fr[f % FR] = vfrag_at(vb + vfrag_off(f));
+            else if (E > 0) fr[f % FR] = frag_at(kn + (f - 16) * IMG_FRAG_BYTES);   // (the next step's first)
         };
+        if constexpr (E == 0)
 #pragma unroll
-        for (int f = 0; f < RA; ++f) rd_b(f);
+            for (int f = 0; f < RA; ++f) rd_b(f);
         if (special(xp, 1)) mask_half(s[1], xp, 1);
         half_step(s[0], p[0], s[1], p[1], BoolTag<true>{}, [&](int f) __attribute__((always_inline)) {
             refill(f - RA, u);
@@ -488,7 +499,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         });
         if (special(x, 0)) mask_half(s[0], x, 0);
         half_step(s[1], p[1], s[0], p[0], BoolTag<true>{}, rd_a);
-        LR_WAIT_VMCNT(2 * E * LP);
+        LR_WAIT_VMCNT(AHEAD);
         block_barrier();
     }
     // ---- the last half-tile's P and the last value tile's products
