@@ -67,7 +67,8 @@ struct PartRows {
             LR_WAIT_VMCNT(0);
             bool done = true;
             for (int s0 = 0; s0 < parts; s0 += 64)
-                done = done && __hip_atomic_load(flags + min(s0 + lane, parts - 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == PART_DONE;
+                done = done && __hip_atomic_load(flags + min(s0 + lane, parts - 1), __ATOMIC_RELAXED,
+                                                 __HIP_MEMORY_SCOPE_AGENT) == PART_DONE;
             const bool last = __builtin_amdgcn_ballot_w64(done) == ~0ull;
             if (lane == 0) shared[0] = last;
             if (last)
@@ -122,8 +123,8 @@ struct PartRows {
 
 // The direct loads of a tile by wave rb of RB: instruction u fills rows 4 u .. 4 u + 3, 16-byte chunks swizzled as attn_fwd.hip's.
 template <int RB, bool PAGED>
-__device__ __forceinline__ void load_tile_rows(const RangeAttnArgs& a, const Seq& sq, const TileList<RANGE_TILE, PAGED>& tl, int64_t hoff,
-                                               int x, uint32_t k_lds, uint32_t v_lds, int rb) {
+__device__ __forceinline__ void load_tile_rows(const RangeAttnArgs& a, const Seq& sq, const TileList<RANGE_TILE, PAGED>& tl,
+                                               int64_t hoff, int x, uint32_t k_lds, uint32_t v_lds, int rb) {
     constexpr int BT = RANGE_TILE, LOADS = 8 / RB;
     const int lane = threadIdx.x & 63, lrow = lane >> 4, lchunk = lane & 15, key0 = tl.key0(x);
     const int64_t k_rs = PAGED ? a.pg.rs : a.k_rs, v_rs = PAGED ? a.pg.rs : a.v_rs;
@@ -214,7 +215,8 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     const int rr = min(r, rows - 1), i = div_small(rr, a.G, a.rcp_g), head = hk * a.G + rr - i * a.G;
     const Sees me = sees_of<PAGED>(a, sq, i);
     int hi_all, lo_all;
-    seen_by_all<PAGED>(a, sq, div_small(min(wr0, rows - 1), a.G, a.rcp_g), div_small(min(wr0 + 31, rows - 1), a.G, a.rcp_g), me, hi_all, lo_all);
+    seen_by_all<PAGED>(a, sq, div_small(min(wr0, rows - 1), a.G, a.rcp_g), div_small(min(wr0 + 31, rows - 1), a.G, a.rcp_g), me,
+                       hi_all, lo_all);
 
     const int64_t hoff = (int64_t)hk * (PAGED ? a.pg.hs : D);
     // (the queries first: under pages they arrive while the table's entries are waited for)
@@ -231,7 +233,9 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     const bool bad = tl.template stage<NW * 64>(a, b, staged);
 
     const uint32_t kr_lds = lds_addr(ring) + kg * NS * TILE * 4, vr_lds = kr_lds + NS * TILE * 2;
-    auto load_tile = [&](int x, int slot) { load_tile_rows<RB, PAGED>(a, sq, tl, hoff, x, kr_lds + 2 * slot * TILE, vr_lds + 2 * slot * TILE, rb); };
+    auto load_tile = [&](int x, int slot) {
+        load_tile_rows<RB, PAGED>(a, sq, tl, hoff, x, kr_lds + 2 * slot * TILE, vr_lds + 2 * slot * TILE, rb);
+    };
 
     const int mine = x1 > x0 + kg ? (x1 - x0 - kg + KG - 1) / KG : 0;   // tiles of this group
     const int steps = x1 > x0 ? (x1 - x0 + KG - 1) / KG : 0;             // of group 0: every group's barriers
@@ -494,7 +498,9 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
     const bool bad = tl.template stage<KG * 64>(a, b, staged, ahead, early);
 
     const uint32_t kr_lds = lds_addr(ring) + kg * NS * TILE * 4, vr_lds = kr_lds + NS * TILE * 2;
-    auto load_tile = [&](int x, int slot) { load_tile_rows<1, PAGED>(a, sq, tl, hoff, x, kr_lds + 2 * slot * TILE, vr_lds + 2 * slot * TILE, 0); };
+    auto load_tile = [&](int x, int slot) {
+        load_tile_rows<1, PAGED>(a, sq, tl, hoff, x, kr_lds + 2 * slot * TILE, vr_lds + 2 * slot * TILE, 0);
+    };
     const int mine = x1 > x0 + kg ? (x1 - x0 - kg + KG - 1) / KG : 0;   // tiles of this wave
     auto tile_of = [&](int t) { return x0 + kg + t * KG; };
     for (int t = 0; t < NS && t < mine; ++t) load_tile(tile_of(t), t);

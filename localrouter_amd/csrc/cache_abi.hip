@@ -50,8 +50,8 @@ lr::PageArgs page_args(int64_t page, int64_t row, int64_t head, int n_pages, int
 }
 
 // ------------------------------------------------------------------------------------------------ range attention
-// How a call is cut: the kernel (wide: 0, or the waves of the kernel of attn_cache_wide.hip; br: attn_cache.hip's rows a block) and its blocks over the keys
-// (RangeAttnArgs: nsplit, per, whole, local, nblk), the rows of the parts and their flags.
+// How a call is cut: the kernel (wide: 0, or the waves of the kernel of attn_cache_wide.hip; br: attn_cache.hip's rows a block) and its
+// blocks over the keys (RangeAttnArgs: nsplit, per, whole, local, nblk, teams, places), the rows of the parts and their flags.
 struct Cut {
     int wide, br, nsplit, per, whole, local, nblk, merge_here, by_xcd, teams, places;
     int64_t part_rows, flags;
@@ -195,7 +195,8 @@ size_t part_bytes(const Cut& c) {
     return (((size_t)c.part_rows * lr::D * 4 + 255) & ~(size_t)255) + (((size_t)(c.part_rows + c.flags) * 8 + 255) & ~(size_t)255);
 }
 void set_cut(lr::RangeAttnArgs& a, void* ws, const Cut& c) {
-    a.nsplit = c.nsplit; a.per = c.per; a.whole = c.whole; a.local = c.local; a.nblk = c.nblk; a.merge_here = c.merge_here; a.by_xcd = c.by_xcd;
+    a.nsplit = c.nsplit; a.per = c.per; a.whole = c.whole; a.local = c.local; a.nblk = c.nblk;
+    a.merge_here = c.merge_here; a.by_xcd = c.by_xcd;
     a.teams = c.teams; a.places = c.places;
     a.rcp_split = lr::rcp_small(c.nsplit);
     a.rcp_nblk = lr::rcp_small(c.nblk);
@@ -366,8 +367,8 @@ int lr_cache_copy_pages(void* k_pages, void* v_pages, int layers, int64_t layer_
                         int64_t row_stride, int64_t head_stride, int n_pages, int page_size, int HK, const int* src,
                         const int* dst, int n, lr_stream_t stream) {
     if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK)) return ERR_ARGS;
-    if (layers < 1 || layers > 65535 || layer_stride % 8 || (layers > 1 && layer_stride < lr::D) || n < 1 || !src || !dst || !aligned(src, 4) ||
-        !aligned(dst, 4))
+    if (layers < 1 || layers > 65535 || layer_stride % 8 || (layers > 1 && layer_stride < lr::D) || n < 1 || !src || !dst ||
+        !aligned(src, 4) || !aligned(dst, 4))
         return ERR_ARGS;
     lr::CacheCopyArgs a{};
     a.kp = static_cast<uint16_t*>(k_pages);
@@ -384,8 +385,8 @@ int lr_cache_move_rows(void* k_pages, void* v_pages, int layers, int64_t layer_s
                        int max_rows, lr_stream_t stream) {
     if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK)) return ERR_ARGS;
     if (!table_args_ok(page_table, table_stride, table_pages, page_size, starts, B)) return ERR_ARGS;
-    if (layers < 1 || layers > 32767 || layer_stride % 8 || (layers > 1 && layer_stride < lr::D) || n < 1 || !src || !dst || !aligned(src, 4) ||
-        !aligned(dst, 4) || max_rows < 1 || max_rows > 256)
+    if (layers < 1 || layers > 32767 || layer_stride % 8 || (layers > 1 && layer_stride < lr::D) || n < 1 || !src || !dst ||
+        !aligned(src, 4) || !aligned(dst, 4) || max_rows < 1 || max_rows > 256)
         return ERR_ARGS;
     lr::CacheMoveArgs a{};
     a.kp = static_cast<uint16_t*>(k_pages);
