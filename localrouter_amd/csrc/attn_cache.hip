@@ -163,12 +163,12 @@ __device__ __forceinline__ float quad_sum(float x) {
     return wave_pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-// The rows of which a group of waves (RB of them) has bits set, again, by its KG waves in turn; f(q): row q of the group. Every
-// wave's rows are in memory afterwards.
+// The rows of which a group of waves (RB of them) has bits set, again, by its KG waves in turn; f(q): row q of the group. Where every
+// wave's rows were in memory before, they are afterwards.
 template <int RB, int KG, class F>
 __device__ __forceinline__ void again_rows(int* shared, int rb, int kg, uint32_t bits, F&& f) {
-    LR_WAIT_VMCNT(0);   // (the rows that are overwritten below)
     if (!__syncthreads_or(bits != 0)) return;
+    LR_WAIT_VMCNT(0);   // (the rows that are overwritten below)
     if (threadIdx.x < RB) shared[threadIdx.x] = 0;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) atomicOr(shared + rb, (int)bits);
@@ -443,8 +443,10 @@ template <int NB, int KG, int NS, bool PAGED>
 __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnArgs a) {
     constexpr int BT = RANGE_TILE, TILE = BT * D, BR = 16 * NB;
     typedef __attribute__((address_space(3))) i16x4_t lds_i16x4;
-    constexpr int RING = KG * NS * TILE * 2 * 2, MERGE = KG * NB * (8 * 256 + 32) * 4;
-    __shared__ __attribute__((aligned(1024))) char ring[RING > MERGE ? RING : MERGE];
+    constexpr int OWN_LDS = NS * TILE * 2 * 2;   // bytes of LDS a wave: its tiles, then its sums
+    static_assert(OWN_LDS >= NB * 8 * 1024, "a wave's sums in the place of its tiles");
+    __shared__ __attribute__((aligned(1024))) char ring[KG * OWN_LDS];
+    __shared__ float2 mls[KG * NB * 16];
     __shared__ int staged[PAGED ? RANGE_STAGED : 1];
 
     const int tid = threadIdx.x, lane = tid & 63, kg = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -595,15 +597,15 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
     const bool whole_block = parts == 1;
     const PartRows<BR> to(a, ((int64_t)b * a.nblk + blk) * a.HK + hk);
     float* mo = reinterpret_cast<float*>(ring);
-    float* mml = mo + KG * NB * 8 * 256;
-    __syncthreads();
+    constexpr int OWN_F = OWN_LDS / 4;
+    asm volatile("" ::: "memory");   // (the wave's own tiles are read)
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         l[nb] = quad_sum(l[nb]);
         if (live[nb]) {
 #pragma unroll
-            for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4*>(mo + ((kg * NB + nb) * 8 + db) * 256 + 4 * lane) = o[nb][db];
-            if (g == 0) *reinterpret_cast<float2*>(mml + (kg * NB + nb) * 32 + 2 * n) = float2{m_used[nb], l[nb]};
+            for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4*>(mo + kg * OWN_F + (nb * 8 + db) * 256 + 4 * lane) = o[nb][db];
+            if (g == 0) mls[(kg * NB + nb) * 16 + n] = float2{m_used[nb], l[nb]};
         }
     }
     __syncthreads();
@@ -616,7 +618,7 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
             float2 ml[KG];
 #pragma unroll
             for (int u = 0; u < KG; ++u) {
-                ml[u] = *reinterpret_cast<const float2*>(mml + (u * NB + nb) * 32 + 2 * n);
+                ml[u] = mls[(u * NB + nb) * 16 + n];
                 mm = fmaxf(mm, ml[u].x);
             }
             const float ref = mm > -INFINITY ? mm : 0.0f;
@@ -633,7 +635,7 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
                 f32x4 own{};
 #pragma unroll
                 for (int u = 0; u < KG; ++u) {
-                    const f32x4 y = *reinterpret_cast<const f32x4*>(mo + ((u * NB + nb) * 8 + kg + KG * x) * 256 + 4 * lane);
+                    const f32x4 y = *reinterpret_cast<const f32x4*>(mo + u * OWN_F + (nb * 8 + kg + KG * x) * 256 + 4 * lane);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) own[e] = fmaf(w[u], y[e], own[e]);
                 }
@@ -657,6 +659,7 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
         broken |= ((half | half >> 16) & 0xffff) << (16 * nb);
     }
     // ---- rows with an infinity or NaN in some wave's dims again, whole, over the seen keys only
+    if (!whole_block) LR_WAIT_VMCNT(0);   // (this wave's part is in memory)
     int* again = reinterpret_cast<int*>(ring);
     again_rows<1, KG>(again, 0, kg, broken, [&](int q) __attribute__((always_inline)) {
         int i = __builtin_amdgcn_readlane(ri[0], q & 15), h = __builtin_amdgcn_readlane(head[0], q & 15);
