@@ -439,11 +439,11 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
 // 4 products for a block of 16 keys in place of 8, eight waves of one tile each in place of four of two.
 // Lane 16 g + n: row n of each block; of a tile's scores the keys 4 g + r and 16 + 4 g + r (r < 4), in which order its products
 // take the keys; of the sums the dims 16 db + 4 g + r.
-template <int NB, int KG, int NS, bool PAGED>
+template <int NB, int KG, bool PAGED>
 __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnArgs a) {
     constexpr int BT = RANGE_TILE, TILE = BT * D, BR = 16 * NB;
     typedef __attribute__((address_space(3))) i16x4_t lds_i16x4;
-    constexpr int OWN_LDS = NS * TILE * 2 * 2;   // bytes of LDS a wave: its tiles, then its sums
+    constexpr int OWN_LDS = TILE * 2 * 2;   // bytes of LDS a wave: its tiles, then its sums
     static_assert(OWN_LDS >= NB * 8 * 1024, "a wave's sums in the place of its tiles");
     __shared__ __attribute__((aligned(1024))) char ring[KG * OWN_LDS];
     __shared__ float2 mls[KG * NB * 16];
@@ -499,14 +499,9 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
     }
     const bool bad = tl.template stage<KG * 64>(a, b, staged, ahead, early);
 
-    const uint32_t kr_lds = lds_addr(ring) + kg * NS * TILE * 4, vr_lds = kr_lds + NS * TILE * 2;
-    auto load_tile = [&](int x, int slot) {
-        load_tile_rows<1, PAGED>(a, sq, tl, hoff, x, kr_lds + 2 * slot * TILE, vr_lds + 2 * slot * TILE, 0);
-    };
+    const uint32_t kr_lds = lds_addr(ring) + kg * OWN_LDS, vr_lds = kr_lds + TILE * 2;
     const int mine = x1 > x0 + kg ? (x1 - x0 - kg + KG - 1) / KG : 0;   // tiles of this wave
     auto tile_of = [&](int t) { return x0 + kg + t * KG; };
-    for (int t = 0; t < NS && t < mine; ++t) load_tile(tile_of(t), t);
-
     int vtr[8];   // (dims 16 db .. of rows 4 g + (n >> 2), and 16 rows on)
 #pragma unroll
     for (int db = 0; db < 8; ++db)
@@ -524,65 +519,67 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
     const float c = a.c;
     const bf16x2 ones2 = {(bf16)1.0f, (bf16)1.0f};
 
-    for (int t = 0; t < mine; ++t) {
-        if (NS > 1 && t + NS - 1 < mine) LR_WAIT_VMCNT((NS - 1) * 16);   // tile t has landed
-        else LR_WAIT_VMCNT(0);
-        const int x = tile_of(t), key0 = tl.key0(x);
-        const uint16_t* kt = reinterpret_cast<const uint16_t*>(ring) + kg * NS * TILE * 2 + (t % NS) * TILE;
-        const uint16_t* vt = kt + NS * TILE;
-        f32x4 s[NB][2] = {};
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + (16 * kb + n) * D + 8 * ((4 * ks + g) ^ n));
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) s[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nb][ks], s[nb][kb], 0, 0, 0);
-            }
-        bf16x8 vf[8];
-#pragma unroll
-        for (int db = 0; db < 8; ++db) {
-            const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vt + vtr[db]));
-            const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vt + vtr[db] + 16 * D));
-            vf[db] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-        const bool whole = key0 + BT <= hi_all && (key0 >= lo_all || key0 + BT <= a.sinks) && !bad;
+    const uint16_t *kt = reinterpret_cast<const uint16_t*>(ring) + kg * TILE * 2, *vt = kt + TILE;
+    // (one place that loads, its first pass before any tile: instructions not met yet cost as much as memory)
+    for (int t = -1; t < mine; ++t) {
         u32x4 pw[NB];
+        bf16x8 vf[8];
+        if (t >= 0) {
+            LR_WAIT_VMCNT(0);   // tile t has landed
+            const int x = tile_of(t), key0 = tl.key0(x);
+            f32x4 s[NB][2] = {};
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            f32x4 &s0 = s[nb][0], &s1 = s[nb][1];
-            if (!whole) {
-                const uint32_t m = seen_bits<BT, PAGED>(a, sq, tl, bad, ri[nb], me[nb], x, 0) >> (4 * g);
+            for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + (16 * kb + n) * D + 8 * ((4 * ks + g) ^ n));
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) s[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nb][ks], s[nb][kb], 0, 0, 0);
+                }
+#pragma unroll
+            for (int db = 0; db < 8; ++db) {
+                const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vt + vtr[db]));
+                const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vt + vtr[db] + 16 * D));
+                vf[db] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+            const bool whole = key0 + BT <= hi_all && (key0 >= lo_all || key0 + BT <= a.sinks) && !bad;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                f32x4 &s0 = s[nb][0], &s1 = s[nb][1];
+                if (!whole) {
+                    const uint32_t m = seen_bits<BT, PAGED>(a, sq, tl, bad, ri[nb], me[nb], x, 0) >> (4 * g);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (!(m >> e & 1)) s0[e] = -INFINITY;
+                        if (!(m >> (16 + e) & 1)) s1[e] = -INFINITY;
+                    }
+                }
+                const float mx = c * quad_max(fmaxf(fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3])),
+                                                    fmaxf(fmaxf(s1[0], s1[1]), fmaxf(s1[2], s1[3]))));
+                if (__builtin_amdgcn_ballot_w64(mx > m_used[nb] + RESCALE_TAU)) {
+                    const float mn = fmaxf(m_used[nb], mx);
+                    const float alpha = mn > -INFINITY ? __builtin_amdgcn_exp2f(m_used[nb] - mn) : 1.0f;
+                    m_used[nb] = mn;
+                    l[nb] *= alpha;
+#pragma unroll
+                    for (int db = 0; db < 8; ++db) o[nb][db] *= alpha;
+                }
+                // (no key seen so far: the reference is -inf and every score -inf; any finite reference gives P = 0)
+                const float nm = m_used[nb] > -INFINITY ? -m_used[nb] : 0.0f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (!(m >> e & 1)) s0[e] = -INFINITY;
-                    if (!(m >> (16 + e) & 1)) s1[e] = -INFINITY;
+                    const uint32_t p2 = pack_bf16x2(__builtin_amdgcn_exp2f(fmaf(s[nb][e >> 1][2 * (e & 1)], c, nm)),
+                                                    __builtin_amdgcn_exp2f(fmaf(s[nb][e >> 1][2 * (e & 1) + 1], c, nm)));
+                    pw[nb][e] = p2;
+                    l[nb] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p2), ones2, l[nb], false);
                 }
             }
-            const float mx = c * quad_max(fmaxf(fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3])),
-                                                fmaxf(fmaxf(s1[0], s1[1]), fmaxf(s1[2], s1[3]))));
-            if (__builtin_amdgcn_ballot_w64(mx > m_used[nb] + RESCALE_TAU)) {
-                const float mn = fmaxf(m_used[nb], mx);
-                const float alpha = mn > -INFINITY ? __builtin_amdgcn_exp2f(m_used[nb] - mn) : 1.0f;
-                m_used[nb] = mn;
-                l[nb] *= alpha;
-#pragma unroll
-                for (int db = 0; db < 8; ++db) o[nb][db] *= alpha;
-            }
-            // (no key seen so far: the reference is -inf and every score -inf; any finite reference gives P = 0)
-            const float nm = m_used[nb] > -INFINITY ? -m_used[nb] : 0.0f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t p2 = pack_bf16x2(__builtin_amdgcn_exp2f(fmaf(s[nb][e >> 1][2 * (e & 1)], c, nm)),
-                                                __builtin_amdgcn_exp2f(fmaf(s[nb][e >> 1][2 * (e & 1) + 1], c, nm)));
-                pw[nb][e] = p2;
-                l[nb] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p2), ones2, l[nb], false);
-            }
         }
-        if (t + NS < mine) {   // the slot is free again once this wave's reads have returned
+        if (t + 1 < mine) {   // the tile's place is free again once this wave's reads have returned
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            load_tile(tile_of(t + NS), t % NS);
+            load_tile_rows<1, PAGED>(a, sq, tl, hoff, tile_of(t + 1), kr_lds, vr_lds, 0);
         }
+        if (t < 0) continue;
 #pragma unroll
         for (int db = 0; db < 8; ++db)
 #pragma unroll
@@ -716,8 +713,8 @@ hipError_t launch_blocks(const RangeAttnArgs& a, bool paged, int threads, void (
 }  // namespace
 
 hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int br, hipStream_t stream) {
-    if (br == 16) return launch_blocks<16>(a, paged, 512, range_step_kernel<1, 8, 1, false>, range_step_kernel<1, 8, 1, true>, stream);
-    if (br == 32) return launch_blocks<32>(a, paged, 512, range_step_kernel<2, 8, 1, false>, range_step_kernel<2, 8, 1, true>, stream);
+    if (br == 16) return launch_blocks<16>(a, paged, 512, range_step_kernel<1, 8, false>, range_step_kernel<1, 8, true>, stream);
+    if (br == 32) return launch_blocks<32>(a, paged, 512, range_step_kernel<2, 8, false>, range_step_kernel<2, 8, true>, stream);
     if (br == 64) return launch_blocks<64>(a, paged, 256, range_attn_kernel<2, 2, 4, false>, range_attn_kernel<2, 2, 4, true>, stream);
     return launch_blocks<128>(a, paged, 512, range_attn_kernel<4, 2, 4, false>, range_attn_kernel<4, 2, 4, true>, stream);
 }
