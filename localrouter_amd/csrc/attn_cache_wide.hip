@@ -310,12 +310,12 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
 
     {
         const uint16_t* src = a.q + (int64_t)(sq.t0 + i) * a.q_rs + head * D + 8 * hf;
+        k_page(tile_of(0));
+        const uint64_t kb = k_src(tile_of(0));
+#pragma unroll
+        for (int u = 0; u < LP; ++u) load_k1(kb, ring, u);
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) qa[ks] = *reinterpret_cast<const bf16x8*>(src + 16 * ks);
-        k_page(tile_of(0));
-        const uint64_t ks = k_src(tile_of(0));
-#pragma unroll
-        for (int u = 0; u < LP; ++u) load_k1(ks, ring, u);
     }
 
     // ---- masked half-tiles: what the row does not see out, and a reference for the rows that have none yet
