@@ -308,6 +308,21 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     const uint32_t vlane = (uint32_t)vt_lane(lane);
     auto vfrag_off = [](int x) __attribute__((always_inline)) { return 4096 * (x >> 2) + 256 * (x & 3); };
 
+    auto slot = [](int x) __attribute__((always_inline)) { return (uint32_t)(x % SLOTS * IMG_TILE_BYTES); };
+    // V(0) .. V(E) and K(1) .. K(E + 1)
+    auto first_pairs = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t <= E; ++t) {
+            v_page(tile_of(t));
+            const uint64_t vs = v_src(tile_of(t));
+#pragma unroll
+            for (int u = 0; u < LP; ++u) load_v1(vs, vring + slot(t), u);
+            k_page(tile_of(t + 1));
+            const uint64_t ks = k_src(tile_of(t + 1));
+#pragma unroll
+            for (int u = 0; u < LP; ++u) load_k1(ks, ring + slot(t + 1), u);
+        }
+    };
     {
         const uint16_t* src = a.q + (int64_t)(sq.t0 + i) * a.q_rs + head * D + 8 * hf;
         k_page(tile_of(0));
@@ -316,6 +331,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         for (int u = 0; u < LP; ++u) load_k1(kb, ring, u);
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) qa[ks] = *reinterpret_cast<const bf16x8*>(src + 16 * ks);
+        if constexpr (E == 0) first_pairs();   // (more of them at once would keep the first product waiting)
     }
 
     // ---- masked half-tiles: what the row does not see out, and a reference for the rows that have none yet
@@ -381,7 +397,6 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto slot = [](int x) __attribute__((always_inline)) { return (uint32_t)(x % SLOTS * IMG_TILE_BYTES); };
     // a step's refills, one load every other slot of its first half: V(t + E) from slot 1 on, then K(t + E + 1) (past the last
     // tile repeats of it, never read); their addresses in the slots before, under the products
     uint64_t src = 0;
@@ -400,25 +415,9 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     negm = f32x16{};
     LR_WAIT_VMCNT(0);
     block_barrier();
-#pragma unroll
-    for (int t = 0; t <= E; ++t) {
-        v_page(tile_of(t));
-        const uint64_t vs = v_src(tile_of(t));
-#pragma unroll
-        for (int u = 0; u < LP; ++u) load_v1(vs, vring + slot(t), u);
-        k_page(tile_of(t + 1));
-        if (t == E && E == 0) break;   // (in step 0, under its products)
-        const uint64_t ks = k_src(tile_of(t + 1));
-#pragma unroll
-        for (int u = 0; u < LP; ++u) load_k1(ks, ring + slot(t + 1), u);
-    }
+    if constexpr (E > 0) first_pairs();
     // a wave without rows only loads its share of the tiles (and leaves the clock to the others)
     if (row0 + 32 * wv >= rows) {
-        if constexpr (E == 0) {
-            const uint64_t ks = k_src(tile_of(1));
-#pragma unroll
-            for (int u = 0; u < LP; ++u) load_k1(ks, ring + slot(1), u);
-        }
         for (int u = 0;; ++u) {
             v_page(tile_of(u + 1 + E));
             k_page(tile_of(u + 2 + E));
@@ -446,7 +445,6 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     }
     // ---- step 0: S of half-tile 1 (K(0), fragments 8-15), P of half-tile 0
     {
-        const uint64_t ks = E == 0 ? k_src(tile_of(1)) : 0;   // (one tile in all: a repeat of it, never read)
         v_page(tile_of(1 + E));   // (of step 1's refills)
         k_page(tile_of(2 + E));
         uint32_t kb = ring + lane16;
@@ -457,7 +455,6 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
         for (int f = 0; f < RA; ++f) rd0(f);
         half_step(s[1], p[1], s[0], p[0], BoolTag<false>{}, [&](int f) __attribute__((always_inline)) {
-            if (E == 0 && (f - RA) % 2 == 0 && f - RA < 2 * LP) load_k1(ks, ring + slot(1), (f - RA) / 2);
             rd0(f);
         });
         LR_WAIT_VMCNT(AHEAD);
