@@ -75,9 +75,10 @@ bool few_rows(int64_t rows, int64_t pairs, int64_t tiles) {
 // attn_cache.hip: every block in parts of `per` tiles, one workgroup a CU; rows of a kv head a sequence, pairs: sequences x kv heads.
 // Blocks of 16 and 32 rows (the kernel of few rows) up to 32 rows a kv head, and of 32 above while there are few blocks with few
 // keys, which every block reads (few_rows). Elsewhere blocks of 64 and 128 rows.
-// Parts of the kernel of few rows: as few as cost least, when a round of eight tiles takes ~1.5 us. Of at most 16 rows the last part
-// to end merges them all in ~1.2 us, eight more of them in another 1.2 (500 keys 1 part 7.6, 2 8.6, 4 8.1; 1,900 2 parts 12.4, 4 9.9,
-// 8 8.7, 15 9.5; 6,000 6 14.1, 12 12.4, 24 13.1; 16,000 over 2 heads 16 14.5, 32 13.5, 63 17.5). Of more rows a second launch does,
+// Parts of the kernel of few rows: as few as cost least, when a round of eight tiles takes 1.2 to 1.6 us. Of at most 16 rows the last
+// part to end merges them all in ~2.5 us, eight more of them in another 1.2 (rows of 600 keys 1 part 6.3, 3 7.3; 1,100 3 7.8, 5 7.4;
+// pages of 500 1 7.6, 2 8.6, 4 8.1; 1,900 2 parts 12.4, 4 9.9, 8 8.7, 15 9.5; 6,000 6 14.1, 12 12.4, 24 13.1; 16,000 over 2 heads
+// 16 14.5, 32 13.0, 63 15.4, over 8 16 18.5, 32 19.1). Of more rows a second launch does,
 // in ~2.5 us and with each part's stores (20 rows: 500 keys 1 part 10.1, 2 11.5; 1,900 4 13.1, 8 11.8, 16 12.7; 6,000 8 16.7,
 // 16 15.9, 32 18.2). In the same launch / by a second: 24 parts of 4 rows 13.1 / 14.5, 63 of 8 15.4 / 17.5, 32 of 16 20.9 / 22.1, 8 of
 // 20 12.5 / 11.8, 8 of 32 13.4 / 11.9, 2 of 64 19.1 / 16.0.
@@ -89,10 +90,10 @@ Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
     if (br <= 32) {
         auto cost = [&](int64_t n) {
             const double rounds = (double)(((tiles + n - 1) / n + 7) / 8);
-            if (br == 16) return 1.6 * rounds + (n > 1 ? 1.2 + 1.2 * (double)((n + 7) / 8) : 0.0);
+            if (br == 16) return 1.25 * rounds + (n > 1 ? 1.4 + 1.2 * (double)((n + 7) / 8) : 0.0);
             return 1.4 * rounds + (n > 1 ? 2.4 + 0.18 * (double)n : 0.0);
         };
-        const int64_t most = ns;
+        const int64_t most = std::max<int64_t>(1, std::min(256 / base, (tiles + 7) / 8));
         ns = 1;
         for (int64_t n = 2; n <= most; ++n)
             if (cost(n) < cost(ns)) ns = n;
