@@ -13,8 +13,8 @@
 // of its key tiles, its waves (or groups of waves) alternate over the tiles. S^T = K Q^T and O^T += V^T P^T with P in registers, K
 // and V tiles row-major in LDS by direct loads. Two kernels here, for the calls that the one of attn_cache_wide.hip does not take:
 //   range_step_kernel   blocks of 16 or 32 rows: single tokens, small trees; bound by the chain from one load and one instruction
-//                       to the next. 8 kv heads, one token: 500 keys 7.6 us, 1,900 8.7, 16,000 19; 64 sequences of 16,000
-//                       bound by HBM (5.7 TB/s).
+//                       to the next. 8 kv heads, one token of 4 query heads each: 500 keys 7.4 us, 1,900 8.7, 16,000 19; from a
+//                       few dozen MB on by HBM (64 sequences of 7,000 keys, 2.7 GB, 477 us = 5.7 TB/s).
 //   range_attn_kernel   blocks of 64 or 128 rows: larger batches of trees, pages of fewer than 16 rows, rows far apart.
 #include "lr_common.h"
 #include "lr_cache_kernels.h"
@@ -180,6 +180,9 @@ __device__ __forceinline__ void again_rows(int* shared, int rb, int kg, uint32_t
     __syncthreads();
 }
 
+// Blocks of 64 and 128 rows: KG groups of RB waves (32 rows each) alternate over the tiles, a ring of NS of them a group, on
+// v_mfma_f32_32x32x16_bf16 (the pipelined kernel's fragments, attn_fwd.hip). Bound by HBM where it is taken (32 sequences of 16,000
+// keys over 8 kv heads, 64 rows each, 2.1 GB, 384 us = 5.5 TB/s): one read of the keys for all rows is what counts.
 template <int RB, int KG, int NS, bool PAGED>
 __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(RangeAttnArgs a) {
     constexpr int BT = RANGE_TILE, TILE = BT * D, NW = RB * KG;
