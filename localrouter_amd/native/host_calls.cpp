@@ -61,6 +61,10 @@ int int32(PyObject* o, const char* name) {
     if (x < INT_MIN || x > INT_MAX) refuse(std::string(name) + ": a 32-bit number expected");
     return (int)x;
 }
+// a count that None or more than `most` makes `most` (below 1: as it is, for the entry point to refuse)
+int at_most(PyObject* o, const char* name, int64_t most) {
+    return (int)(none(o) ? most : std::max<int64_t>(-1, std::min(integer(o, name), most)));
+}
 float number(PyObject* o) {
     const double x = PyFloat_AsDouble(o);
     if (x == -1.0 && PyErr_Occurred()) throw Raised{};
@@ -279,8 +283,7 @@ PyObject* attention(PyObject* const* a) {
     if (T == 0) return held.release();
     const Table table(a[5], w, B);
     const int64_t most = std::min<int64_t>((int64_t)table.pages * pool.page_size, INT_MAX);
-    const int max_rows = (int)(none(a[9]) ? T : std::min(integer(a[9], "max_rows"), T));
-    const int max_keys = (int)(none(a[10]) ? most : std::min(integer(a[10], "max_keys"), most));
+    const int max_rows = at_most(a[9], "max_rows", T), max_keys = at_most(a[10], "max_keys", most);
     const uint64_t* tree = nullptr;
     int words = 0;
     if (!none(a[11])) {
@@ -330,7 +333,7 @@ PyObject* move_rows(PyObject* const* a) {
     if (n > 0) {
         const Table table(a[4], w, B);
         const int *starts = ints(a[5], "starts", w, B + 1), *src = ints(a[6], "src", w, n), *dst = ints(a[7], "dst", w, n);
-        const int max_rows = (int)(none(a[8]) ? n : std::min(integer(a[8], "max_rows"), n));
+        const int max_rows = at_most(a[8], "max_rows", n);
         call("lr_cache_move_rows", [&] {
             return f_move(pool.k, pool.v, pool.layers, pool.ls, pool.ps, pool.rs, pool.hs, pool.n_pages, pool.page_size, pool.heads,
                           table.p, table.rs, table.pages, starts, src, dst, (int)B, (int)n, max_rows,

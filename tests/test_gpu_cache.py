@@ -751,6 +751,11 @@ def test_numbers_past_32_bits_are_refused():
     for kw in (dict(window=1 << 32), dict(window=4, sinks=(1 << 32) + 4)):
         with pytest.raises(ValueError):
             cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, **kw)
+    for kw in (dict(max_rows=5 - (1 << 33)), dict(max_keys=-(1 << 40) + 20), dict(max_rows=0), dict(max_keys=-1)):
+        with pytest.raises(_lib.LrError):
+            cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, **kw)
+    assert torch.equal(cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, max_rows=1 << 40, max_keys=1 << 40),
+                       cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens))
     for kw in (dict(window=1 << 32), dict(window=4, sinks=1 << 31), dict(window=4, frame=(1 << 32) + 1),
                dict(window=4, p0=1 << 32)):
         with pytest.raises(ValueError):
