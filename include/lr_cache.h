@@ -54,8 +54,9 @@ int lr_cache_append_bf16(const void* q, const void* k, const void* v, int64_t q_
  * j < sinks. window 0: all.
  * A token that sees nothing gets zeros; a position that it does not see has no part in its result, whatever it holds.
  * max_rows: no sequence has more tokens in the call (those beyond are left out, under a tree as keys too); max_keys: no
- * sequence has more positions
- * (those beyond are not seen). Both size the launch. At most 2^30 positions; B at most 65,535.
+ * sequence has more positions (those beyond are not seen). Both size the launch: a max_rows far above the tokens of any sequence
+ * launches workgroups without rows for every sequence, and one that makes more of them than a grid holds (2^22) is rejected. At
+ * most 2^30 positions; B at most 65,535.
  * workspace: lr_cache_attention_ws_bytes bytes (0: none, it may be NULL), 256-byte aligned; it must not overlap q, out or the
  * pool, nor out q or the pool (rejected). What it holds before the call does not matter. Calls that overlap in time on one
  * workspace race.

@@ -702,8 +702,8 @@ hipError_t launch_blocks(const RangeAttnArgs& a, bool paged, int threads, void (
                          void (*paged_kernel)(RangeAttnArgs), hipStream_t stream) {
     const int64_t rows = (int64_t)(paged ? a.max_rows : a.W) * a.G;
     const int64_t blocks = (rows + BR - 1) / BR * a.HK * a.nsplit, merge = blocks / a.nsplit * (BR / 4);
-    // (a grid's work-items and a block's bytes of parts are counted in 32 bits)
-    if (blocks > 1 << 22 || merge > 1 << 23 || (int64_t)a.nsplit * BR * D * 4 > INT32_MAX) return hipErrorInvalidValue;
+    // (a block's bytes of parts are counted in 32 bits)
+    if (blocks > RANGE_MAX_BLOCKS || merge > 2 * RANGE_MAX_BLOCKS || (int64_t)a.nsplit * BR * D * 4 > INT32_MAX) return hipErrorInvalidValue;
     const unsigned seqs = paged ? (unsigned)a.B : 1;
     hipLaunchKernelGGL(paged ? paged_kernel : rows_kernel, dim3((unsigned)blocks, seqs), dim3(threads), 0, stream, a);
     const hipError_t e = hipGetLastError();

@@ -672,7 +672,7 @@ hipError_t launch_waves(const RangeAttnArgs& a, hipStream_t stream) {
     const int xcds = a.by_xcd ? 8 : 1;
     const int64_t of = a.nsplit > 1 ? a.local - a.whole : 0;   // cut blocks
     const int64_t blocks = xcds * (a.local + of * (a.nsplit - 1)), merge = xcds * of * QW;
-    if (blocks > 1 << 22 || merge > 1 << 23) return hipErrorInvalidValue;   // (a grid's work-items are counted in 32 bits)
+    if (blocks > RANGE_MAX_BLOCKS || merge > 2 * RANGE_MAX_BLOCKS) return hipErrorInvalidValue;
     hipLaunchKernelGGL((range_wide_kernel<QW, PAGED>), dim3((unsigned)blocks), dim3(64 * QW), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || of == 0) return e;

@@ -53,8 +53,8 @@ lr::PageArgs page_args(int64_t page, int64_t row, int64_t head, int n_pages, int
 // How a call is cut: the kernel (wide: 0, or the waves of the kernel of attn_cache_wide.hip; br: attn_cache.hip's rows a block) and its
 // blocks over the keys (RangeAttnArgs: nsplit, per, whole, local, nblk, teams, places), the rows of the parts and their flags.
 struct Cut {
-    int wide, br, nsplit, per, whole, local, nblk, merge_here, by_xcd, teams, places;
-    int64_t part_rows, flags;
+    int wide, br, nsplit, per, nblk, merge_here, by_xcd, teams, places;
+    int64_t whole, local, part_rows, flags;   // (blocks of every sequence and kv head: past 32 bits before the launch is refused)
 };
 
 // The most key tiles of bt keys that a block of rows needs: of `span` keys beside the first `sinks`, of `keys` in all.
@@ -122,7 +122,7 @@ Cut cut_wide(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool by_
     const int br = 32 * c.wide, xcds = by_xcd ? 8 : 1, round = (c.wide == 8 ? 256 : 512) / xcds;
     c.by_xcd = by_xcd;
     c.nblk = (int)((rows + br - 1) / br);
-    c.local = (int)((pairs + xcds - 1) / xcds * c.nblk);
+    c.local = (pairs + xcds - 1) / xcds * c.nblk;
     c.whole = c.local;
     c.nsplit = 1;
     const int64_t staged = page_size ? lr::RANGE_WIDE_STAGED / std::max(1, lr::RANGE_WIDE_TILE / page_size) : INT_MAX;
@@ -145,7 +145,7 @@ Cut cut_wide(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool by_
     }
     if (ns > 1) {
         c.nsplit = (int)ns;
-        c.whole = (int)(c.local - tail);
+        c.whole = c.local - tail;
         c.part_rows = tail * xcds * br * ns;
     }
     return c;
@@ -192,11 +192,16 @@ Cut cache_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, i
     }
     return cut_small(rows, pairs, tiles, page_size);
 }
+// Whether the grid of attn_cache_wide.hip's launch holds its workgroups (attn_cache.hip's counts its own, launch_blocks).
+bool launch_fits(const Cut& c) {
+    return !c.wide || (c.by_xcd ? 8 : 1) * (c.whole + (c.local - c.whole) * c.nsplit) <= lr::RANGE_MAX_BLOCKS;
+}
 size_t part_bytes(const Cut& c) {
     return (((size_t)c.part_rows * lr::D * 4 + 255) & ~(size_t)255) + (((size_t)(c.part_rows + c.flags) * 8 + 255) & ~(size_t)255);
 }
 void set_cut(lr::RangeAttnArgs& a, void* ws, const Cut& c) {
-    a.nsplit = c.nsplit; a.per = c.per; a.whole = c.whole; a.local = c.local; a.nblk = c.nblk;
+    a.nsplit = c.nsplit; a.per = c.per; a.nblk = c.nblk;
+    a.whole = (int)c.whole; a.local = (int)c.local;   // (launch_fits; attn_cache.hip has no use for them)
     a.merge_here = c.merge_here; a.by_xcd = c.by_xcd;
     a.teams = c.teams; a.places = c.places;
     a.rcp_split = lr::rcp_small(c.nsplit);
@@ -248,6 +253,7 @@ int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* 
     lr::RangeAttnArgs a{};
     const bool narrow = k_row_stride < lr::RANGE_WIDE_MAX_RS && v_row_stride < lr::RANGE_WIDE_MAX_RS;
     const Cut cut = window_cut(W, H, HK, nkeys, window, sinks, frame, narrow);
+    if (!launch_fits(cut)) return ERR_ARGS;
     const size_t need = part_bytes(cut);
     if (need) {
         if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return ERR_ARGS;
@@ -295,6 +301,7 @@ int lr_cache_attention_bf16(const void* q, int64_t q_row_stride, void* out, int6
     lr::RangeAttnArgs a{};
     const bool narrow = row_stride < lr::RANGE_WIDE_MAX_RS && (page_size > lr::RANGE_WIDE_MIN_PAGE || sk.hi - sk.lo < (1ull << 32));
     const Cut cut = cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks, narrow);
+    if (!launch_fits(cut)) return ERR_ARGS;
     const size_t need = part_bytes(cut);
     if (need) {
         if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return ERR_ARGS;

@@ -66,6 +66,7 @@ constexpr int RANGE_WIDE_TILE = 64;         // attn_cache_wide.hip: the same, an
 constexpr int RANGE_WIDE_STAGED = 3840;     // (both of its forms: 4 and 8 waves of 32 rows);
 constexpr int RANGE_WIDE_MIN_PAGE = 16;     // rows a page at least (of 16 rows: in pools of less than 4 GB),
 constexpr int64_t RANGE_WIDE_MAX_RS = 1 << 23;   // and row strides (elements) below this
+constexpr int64_t RANGE_MAX_BLOCKS = 1 << 22;    // workgroups a launch: a grid's work-items are counted in 32 bits
 
 // The attention and, with a.nsplit > 1, the merge of its parts: attn_cache.hip in blocks of br rows (16, 32, 64 or 128), or
 // attn_cache_wide.hip in workgroups of `waves` waves of 32 rows (the cut's tiles are each kernel's own).

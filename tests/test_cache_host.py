@@ -155,6 +155,14 @@ def test_parts_past_32_bits_are_refused():
                    wsb=1 << 40, ws=1 << 44) == BAD
 
 
+@pytest.mark.parametrize("T", [524304, 524312, 524360, 1 << 24])
+def test_launches_past_a_grid_are_refused(T):
+    """65,535 sequences and max_rows left at all the tokens: 65,535 x 8 x 16 T / 128 blocks of rows, whose number an XCD is 65,534 or
+    a little more when it is cut to 32 bits. Refused before that, not launched with too few."""
+    far = dict(q=1 << 44, out=2 << 44, kp=3 << 44, vp=4 << 44, table=5 << 44, starts=6 << 44, lens=7 << 44, ws=8 << 44, wsb=1 << 43)
+    assert _attend(B=65535, T=T, rows=T, keys=160, H=128, HK=8, qrs=128 * 128, ors=128 * 128, ps=16 * 1024, rs=1024, **far) == BAD
+
+
 def test_python_checks_refuse_host_tensors():
     t = torch.zeros(4, 2, 128, dtype=torch.bfloat16)
     p = torch.zeros(3, 16, 2, 128, dtype=torch.bfloat16)
