@@ -81,8 +81,8 @@ def append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: to
            eps: float = 1e-6) -> torch.Tensor | None:
     """lr_cache_append_bf16: new tokens q [T, H, 128], k / v [T, HK, 128] (views of a packed projection allowed): queries
     normalised and rotated into q_out (allocated when None; q itself is allowed), keys the same way into their pages, values
-    as they are. table = (table_a, table_b), one row a position; positions int32 [T]: each token's table row (default its
-    position in its sequence). q None: keys and values only. Returns q_out."""
+    as they are. table = (table_a, table_b), one row a position, of rot / 2 columns at least (cos and sin) or 2 rot (2x2 kinds);
+    positions int32 [T]: each token's table row (default its position in its sequence). q None: keys and values only. Returns q_out."""
     dev = _device(k_pages)
     if table is None:
         if table_kind != TABLE_NONE:

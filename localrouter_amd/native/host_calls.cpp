@@ -162,6 +162,38 @@ struct Table {
     }
 };
 
+// The rotation tables of append: rows of at least the columns that rot dims take (its own view's: a row's stride may be another
+// tensor's).
+struct Rotation {
+    int kind = LR_TABLE_NONE, rot = 0, rows = 0;
+    const at::Tensor *a = nullptr, *b = nullptr;
+    Rotation() = default;
+    Rotation(PyObject* k, PyObject* ao, PyObject* bo, PyObject* r) : kind(int32(k, "table_kind")), rot(int32(r, "rot")) {
+        if (kind == LR_TABLE_NONE) return;
+        const int64_t dims = rot == 0 ? 128 : rot;
+        const int64_t columns = kind == LR_TABLE_COSSIN_F32 ? dims / 2
+                                : kind == LR_TABLE_MAT2_BF16 || kind == LR_TABLE_MAT2_F32 ? 2 * dims : 0;   // (others: no kind)
+        a = &checked(ao, columns);
+        rows = (int)a->size(0);
+        if (!none(bo)) b = &checked(bo, columns);
+    }
+    const at::Tensor& checked(PyObject* o, int64_t columns) const {
+        const at::Tensor& t = tensor(o, "table");
+        if (t.dim() != 2 || t.stride(1) != 1 || t.size(0) > INT_MAX) refuse("table", "contiguous rows", o);
+        if (t.size(1) < columns)
+            refuse("table: rows of " + std::to_string(t.size(1)) + " columns, rot " + std::to_string(rot) + " needs " +
+                   std::to_string(columns));
+        return t;
+    }
+    // on the device, of the kind's type
+    void at(const Where& w, PyObject* ao, PyObject* bo) const {
+        const at::ScalarType type = kind == LR_TABLE_MAT2_BF16 ? at::kBFloat16 : at::kFloat;
+        if (a && !w.holds(*a, type)) refuse("table", kind == LR_TABLE_MAT2_BF16 ? "bf16 rows" : "fp32 rows", ao);
+        if (b && (b->sizes() != a->sizes() || b->strides() != a->strides() || !w.holds(*b, type)))
+            refuse("table", "two tensors of the same type, shape and strides", ao, bo);
+    }
+};
+
 // The given workspace, or one allocated on torch's current stream when `need` is not 0.
 struct Workspace {
     void* p = nullptr;
@@ -216,8 +248,9 @@ void call(const char* name, F&& f) {
 // pairing, rot, eps)
 PyObject* append(PyObject* const* a) {
     const Where w(a[0], a[1]);
-    const Pool pool(a[5], a[6], w, false);
     const int64_t T = size0(a[3], "k"), B = size0(a[9], "lens");
+    const Rotation tab = T > 0 ? Rotation(a[13], a[14], a[15], a[18]) : Rotation();
+    const Pool pool(a[5], a[6], w, false);
     const Rows k(a[3], "k", w, T, pool.heads), v(a[4], "v", w, T, pool.heads);
     Rows q, out;
     Held held{nullptr};
@@ -233,37 +266,21 @@ PyObject* append(PyObject* const* a) {
     if (size0(a[4], "v") != T) refuse("append: q, k and v of different lengths");
     if (B > INT_MAX || T > INT_MAX) refuse("append: too many tokens");
     if (T > 0) {
-        const int kind = int32(a[13], "table_kind");
         const float *qw = nullptr, *kw = nullptr;
         if (!none(a[11])) qw = static_cast<const float*>(vector(a[11], "q_norm", w, 128, at::kFloat, "fp32"));
         if (!none(a[12])) kw = static_cast<const float*>(vector(a[12], "k_norm", w, 128, at::kFloat, "fp32"));
-        const void *ta = nullptr, *tb = nullptr;
-        int64_t stride = 0;
-        int rows = 0;
-        if (kind != LR_TABLE_NONE) {
-            const at::ScalarType type = kind == LR_TABLE_MAT2_BF16 ? at::kBFloat16 : at::kFloat;
-            const at::Tensor& t = tensor(a[14], "table");
-            if (t.dim() != 2 || t.stride(1) != 1 || t.size(0) > INT_MAX || !w.holds(t, type))
-                refuse("table", kind == LR_TABLE_MAT2_BF16 ? "bf16 rows" : "fp32 rows", a[14]);
-            stride = t.stride(0);
-            rows = (int)t.size(0);
-            ta = t.data_ptr();
-            if (!none(a[15])) {
-                const at::Tensor& t2 = tensor(a[15], "table");
-                if (t2.sizes() != t.sizes() || t2.strides() != t.strides() || !w.holds(t2, type))
-                    refuse("table", "two tensors of the same type, shape and strides", a[14], a[15]);
-                tb = t2.data_ptr();
-            }
-        }
+        tab.at(w, a[14], a[15]);
         const Table table(a[7], w, B);
         const int *starts = ints(a[8], "starts", w, B + 1), *lens = ints(a[9], "lens", w, B);
         const int* pos = none(a[16]) ? nullptr : ints(a[16], "positions", w, T);
-        const int pairing = int32(a[17], "pairing"), rot = int32(a[18], "rot");
+        const int pairing = int32(a[17], "pairing");
         const float eps = number(a[19]);
+        const void *ta = tab.a ? tab.a->data_ptr() : nullptr, *tb = tab.b ? tab.b->data_ptr() : nullptr;
+        const int64_t stride = tab.a ? tab.a->stride(0) : 0;
         call("lr_cache_append_bf16", [&] {
             return f_append(q.p, k.p, v.p, q.rs, k.rs, v.rs, out.p, out.rs, pool.k, pool.v, pool.ps, pool.rs, pool.hs, pool.n_pages,
                             pool.page_size, table.p, table.rs, table.pages, starts, lens, pos, (int)B, (int)T, (int)H, pool.heads, qw,
-                            kw, kind, ta, tb, stride, rows, pairing, rot, eps, static_cast<lr_stream_t>(w.stream));
+                            kw, tab.kind, ta, tb, stride, tab.rows, pairing, tab.rot, eps, static_cast<lr_stream_t>(w.stream));
         });
     }
     if (held.o) return held.release();

@@ -253,3 +253,26 @@ def test_host_calls_refuse_host_tensors_by_name():
         h.attention(1, 2, 3)
     with pytest.raises(TypeError):
         h.attention("cuda", 0, t, p, p, i[None], i, i[:1], None, None, None, None, 0, 0, 0.1, None)
+
+
+@pytest.mark.parametrize("kind,rot,columns", [(ops.TABLE_COSSIN_F32, 128, 64), (ops.TABLE_COSSIN_F32, 0, 64), (ops.TABLE_COSSIN_F32, 96, 48),
+                                              (ops.TABLE_MAT2_BF16, 128, 256), (ops.TABLE_MAT2_F32, 64, 128)])
+def test_append_refuses_tables_that_are_narrower_than_the_rotation(kind, rot, columns):
+    """A view of a table's columns has its parent's row stride: with fewer columns than the rotation takes, a row would go on in the
+    next one and the last row past the storage."""
+    h = cache._host()
+    x, p, i = torch.zeros(4, 2, 128, dtype=torch.bfloat16), torch.zeros(3, 16, 2, 128, dtype=torch.bfloat16), torch.zeros(5, dtype=torch.int32)
+    whole = torch.zeros(50, 2 * columns, dtype=torch.bfloat16 if kind == ops.TABLE_MAT2_BF16 else torch.float32)
+    call = lambda a, b: h.append(-1, 0, None, x, x, p, p, i[None], i, i[:1], None, None, None, kind, a, b, None, 0, rot, 1e-6)
+    two = kind == ops.TABLE_COSSIN_F32
+    for a, b in ((whole[:, columns + 1:], whole[:, columns + 1:]), (whole[:, :columns - 1], whole[:, :columns - 1]),
+                 (whole[:, :columns], whole[:, :columns - 1])):
+        if two or a.shape[1] < columns:
+            with pytest.raises(ValueError, match=rf"table: rows of {columns - 1} columns, rot {rot} needs {columns}"):
+                call(a, b if two else None)
+    # wide enough (the next refusal is the host tensors'), and no table at all
+    for a in (whole, whole[:, :columns], whole[:, columns:]):
+        with pytest.raises(ValueError, match="k_pages, v_pages"):
+            call(a, a if two else None)
+    with pytest.raises(ValueError, match="table: expected a tensor"):
+        call(None, None)

@@ -666,6 +666,26 @@ def test_append_leaves_out_what_has_no_place():
     assert torch.equal(out[3:5], same)
 
 
+def test_append_of_column_views_of_a_table():
+    """cos and sin as columns of a wider table: the view's columns count, not its rows' stride. Too narrow ones are refused, and
+    nothing is written."""
+    B = Batch(35, [3], [20], 16, 1)
+    q, k = rnd(B.g, 3, 2, 128), rnd(B.g, 3, 1, 128)
+    (cos, sin), _ = tables(ops.TABLE_COSSIN_F32, 20, 128, B.g)
+    wide = torch.cat([cos, sin, cos], 1)
+    before_k, before_v = B.kp.clone(), B.vp.clone()
+    for a, b in ((cos[:, 32:], sin[:, 32:]), (wide[:, 129:], wide[:, 129:]), (wide[:, :32], wide[:, 64:96])):
+        with pytest.raises(ValueError, match="table: rows of"):
+            cache.append(q, k, k, B.kp, B.vp, B.t, B.starts, B.lens, table=(a, b))
+    assert torch.equal(B.kp, before_k) and torch.equal(B.vp, before_v)
+    got = cache.append(q, k, k, B.kp, B.vp, B.t, B.starts, B.lens, table=(wide[:, :64], wide[:, 64:128]))
+    keys = B.kp.clone()
+    assert torch.equal(got, cache.append(q, k, k, B.kp, B.vp, B.t, B.starts, B.lens, table=(cos, sin))) and torch.equal(keys, B.kp)
+    half = cache.append(q, k, k, B.kp, B.vp, B.t, B.starts, B.lens, table=(cos[:, 32:], sin[:, 32:]), rot=64)
+    assert torch.equal(half, cache.append(q, k, k, B.kp, B.vp, B.t, B.starts, B.lens, rot=64,
+                                          table=(cos[:, 32:].contiguous(), sin[:, 32:].contiguous())))
+
+
 # ------------------------------------------------------------------------------------------------ copies and moves
 @pytest.mark.parametrize("ps,HK,by_head,layers", [(16, 8, False, 3), (1, 1, False, None), (64, 3, True, 2), (128, 5, False, 1),
                                                   (8, 7, True, None)])
