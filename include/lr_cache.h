@@ -8,7 +8,7 @@
  * head g at base + p * page_stride + r * row_stride + g * head_stride, in both the same strides (multiples of 8 elements, the
  * head's 128 elements contiguous). Rows of one page may lie token by token (head_stride 128) or head by head.
  * Calls over layers take base + l * layer_stride for layer l; pages have the same number in every layer. Keys and values, and
- * layers, may interleave in one buffer; pools or layers that are the same rows are rejected.
+ * layers, may interleave in one buffer; those that share a row, or part of one, are rejected.
  *
  * A batch. Sequence b < B has the tokens starts[b] .. starts[b + 1] - 1 of the call's T (n_b of them; int32 [B + 1] on the
  * device, ascending) and lens[b] positions in all (int32 [B]), the call's tokens being its last ones: the first of them at

@@ -18,17 +18,50 @@ constexpr int MAX_POS = 1 << 30;
 inline int shift_of(int page_size) { return __builtin_ctz((unsigned)page_size); }
 inline bool page_size_ok(int ps) { return ps >= 1 && ps <= 65536 && (ps & (ps - 1)) == 0; }
 
-// A pool of pages: aligned bases, strides that hold what they step over.
-bool pool_ok(const void* k, const void* v, int64_t page, int64_t row, int64_t head, int n_pages, int page_size, int HK) {
+// One level of a set of rows: `stride` elements times any of lo .. hi.
+struct Level {
+    int64_t stride, lo, hi;
+};
+
+// Whether d, less some sum of the levels' steps, is within 128 elements of 0: whether two heads' rows that far apart meet. Levels by
+// falling stride; where a level's stride holds the extent of those below it (nested layouts) two of its steps are tried, else as
+// many as reach, `left` in all: past that the answer is that they do.
+bool rows_meet(int64_t d, const Level* levels, int n, int& left) {
+    if (n == 0) return --left < 0 || (d > -lr::D && d < lr::D);
+    const Level& l = levels[0];
+    if (l.lo == l.hi) return rows_meet(d - l.lo * l.stride, levels + 1, n - 1, left);
+    int64_t below = lr::D - 1;
+    for (int i = 1; i < n; ++i) below += levels[i].hi * levels[i].stride;
+    const int64_t least = d - below;   // <= x * stride <= d + below
+    for (int64_t x = std::max(least / l.stride + (least > 0 && least % l.stride), l.lo); x <= l.hi && x * l.stride <= d + below; ++x)
+        if (rows_meet(d - x * l.stride, levels + 1, n - 1, left)) return true;
+    return false;
+}
+
+// A pool of pages: aligned bases, strides that hold what they step over, no row of keys and values, or of two layers, the same.
+bool pool_ok(const void* k, const void* v, int64_t page, int64_t row, int64_t head, int n_pages, int page_size, int HK,
+             int layers = 1, int64_t layer = 0) {
     if (!k || !v || !aligned(k, 16) || !aligned(v, 16) || n_pages < 1 || HK < 1 || !page_size_ok(page_size)) return false;
     if (page % 8 || row % 8 || head % 8 || page < lr::D || row < lr::D || head < lr::D) return false;
-    // keys and values may interleave in one buffer, but not share a head's row
-    const uintptr_t ka = reinterpret_cast<uintptr_t>(k), va = reinterpret_cast<uintptr_t>(v);
-    if ((ka < va ? va - ka : ka - va) < 2 * lr::D) return false;
+    if (layers < 1 || layers > 65535 || layer % 8 || (layers > 1 && layer < lr::D)) return false;
+    auto far = [](int64_t stride, int64_t count) { return stride > ((int64_t)1 << 48) / count; };   // (no address space holds it)
+    if (far(page, n_pages) || far(row, page_size) || far(head, HK) || far(layer, layers)) return false;
     // rows of a page token by token or head by head, pages apart from each other
     const bool by_token = row >= (HK - 1) * head + lr::D && page >= (page_size - 1) * row + (HK - 1) * head + lr::D;
     const bool by_head = head >= (page_size - 1) * row + lr::D && page >= (HK - 1) * head + (page_size - 1) * row + lr::D;
-    return by_token || by_head;
+    if (!by_token && !by_head) return false;
+    Level levels[4] = {{page, 1 - n_pages, n_pages - 1}, {row, 1 - page_size, page_size - 1}, {head, 1 - HK, HK - 1},
+                       {layer, 1 - layers, layers - 1}};
+    std::sort(levels, levels + 4, [](const Level& x, const Level& y) { return x.stride > y.stride; });
+    int left = 4096;   // (nested layouts: at most 16)
+    if (rows_meet((reinterpret_cast<intptr_t>(v) - reinterpret_cast<intptr_t>(k)) / 2, levels, 4, left)) return false;
+    if (layers == 1) return true;
+    for (Level& l : levels)
+        if (l.stride == layer && l.hi == layers - 1 && l.lo == 1 - layers) {   // (another level of the same numbers is as good)
+            l.lo = 1;
+            break;
+        }
+    return !rows_meet(0, levels, 4, left);
 }
 Span pool_span(const void* p, int layers, int64_t layer, int64_t page, int64_t row, int64_t head, int n_pages, int page_size,
                int HK) {
@@ -374,10 +407,9 @@ int lr_cache_append_bf16(const void* q, const void* k, const void* v, int64_t q_
 int lr_cache_copy_pages(void* k_pages, void* v_pages, int layers, int64_t layer_stride, int64_t page_stride,
                         int64_t row_stride, int64_t head_stride, int n_pages, int page_size, int HK, const int* src,
                         const int* dst, int n, lr_stream_t stream) {
-    if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK)) return ERR_ARGS;
-    if (layers < 1 || layers > 65535 || layer_stride % 8 || (layers > 1 && layer_stride < lr::D) || n < 1 || !src || !dst ||
-        !aligned(src, 4) || !aligned(dst, 4))
+    if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK, layers, layer_stride))
         return ERR_ARGS;
+    if (n < 1 || !src || !dst || !aligned(src, 4) || !aligned(dst, 4)) return ERR_ARGS;
     lr::CacheCopyArgs a{};
     a.kp = static_cast<uint16_t*>(k_pages);
     a.vp = static_cast<uint16_t*>(v_pages);
@@ -391,10 +423,10 @@ int lr_cache_move_rows(void* k_pages, void* v_pages, int layers, int64_t layer_s
                        int64_t row_stride, int64_t head_stride, int n_pages, int page_size, int HK, const int* page_table,
                        int64_t table_stride, int table_pages, const int* starts, const int* src, const int* dst, int B, int n,
                        int max_rows, lr_stream_t stream) {
-    if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK)) return ERR_ARGS;
+    if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK, layers, layer_stride))
+        return ERR_ARGS;
     if (!table_args_ok(page_table, table_stride, table_pages, page_size, starts, B)) return ERR_ARGS;
-    if (layers < 1 || layers > 32767 || layer_stride % 8 || (layers > 1 && layer_stride < lr::D) || n < 1 || !src || !dst ||
-        !aligned(src, 4) || !aligned(dst, 4) || max_rows < 1 || max_rows > 256)
+    if (layers > 32767 || n < 1 || !src || !dst || !aligned(src, 4) || !aligned(dst, 4) || max_rows < 1 || max_rows > 256)
         return ERR_ARGS;
     lr::CacheMoveArgs a{};
     a.kp = static_cast<uint16_t*>(k_pages);

@@ -2,6 +2,7 @@
 refused before any GPU call, and the page bookkeeping. No compute calls."""
 from __future__ import annotations
 
+import random
 import re
 from pathlib import Path
 
@@ -146,6 +147,77 @@ def test_pools_that_share_rows_are_refused():
     assert _attend(vp=KP + 128) == _append(vp=KP - 240) == BAD
     for ls in (0, 64):
         assert _copy(ls=ls) == _move(ls=ls) == BAD
+
+
+def _rows_of(base, layers, ls, ps, rs, hs, n_pages, page, HK):
+    """(set of the pool's heads' rows in units of 8 elements, their number) of one of keys and values."""
+    units = [base + l * ls + p * ps + r * rs + h * hs + x for l in range(layers) for p in range(n_pages) for r in range(page)
+             for h in range(HK) for x in range(0, 128, 8)]
+    return set(units), len(units)
+
+
+def _shares(d, **kw):
+    k, nk = _rows_of(0, **kw)
+    v, _ = _rows_of(d, **kw)
+    return len(k) < nk or bool(k & v)
+
+
+PARTLY = [   # keys' rows and values' rows d elements apart; layers, their stride, strides of pages, rows and heads
+    dict(d=128, layers=1, ls=0, ps=4096, rs=256, hs=128),            # value head 0 is key head 1
+    dict(d=-128, layers=1, ls=0, ps=4096, rs=256, hs=128),
+    dict(d=8, layers=1, ls=0, ps=4096, rs=256, hs=128),
+    dict(d=4096, layers=1, ls=0, ps=4096, rs=256, hs=128),           # value page 0 is key page 1
+    dict(d=4096 - 256, layers=1, ls=0, ps=4096, rs=256, hs=128),     # value row 0 is the last key row of page 0
+    dict(d=39 * 4096 + 15 * 256 + 128, layers=1, ls=0, ps=4096, rs=256, hs=128),   # the last row alone
+    dict(d=256 - 64, layers=1, ls=0, ps=8192, rs=512, hs=128),       # half a head
+    dict(d=1 << 40, layers=2, ls=128, ps=4096, rs=256, hs=128),      # layer 1's head 0 is layer 0's head 1
+    dict(d=1 << 40, layers=2, ls=4096, ps=4096, rs=256, hs=128),     # layer 1's page 0 is layer 0's page 1
+    dict(d=1 << 40, layers=3, ls=39 * 4096 + 8, ps=4096, rs=256, hs=128),
+    dict(d=256, layers=5, ls=64 * 4096, ps=8192, rs=512, hs=128, n_pages=33),      # the layers meet, keys and values do not
+    dict(d=4 << 20, layers=3, ls=2 << 20, ps=4096, rs=256, hs=128),  # layer 0's values are layer 2's keys
+]
+
+
+@pytest.mark.parametrize("c", PARTLY, ids=lambda c: "-".join(map(str, c.values())))
+def test_pools_that_share_some_rows_are_refused(c):
+    a = dict(dict(n_pages=40, page=16, HK=2), **c)
+    assert _shares(**a)
+    kw = {x: a[x] for x in ("layers", "ls", "ps", "rs", "hs", "n_pages")}
+    kp = 1 << 44
+    assert _copy(kp=kp, vp=kp + 2 * a["d"], **kw) == _move(kp=kp, vp=kp + 2 * a["d"], **kw) == BAD
+    if a["layers"] == 1:
+        one = {x: a[x] for x in ("ps", "rs", "hs", "n_pages")}
+        assert _attend(kp=kp, vp=kp + 2 * a["d"], **one) == _append(kp=kp, vp=kp + 2 * a["d"], **one) == BAD
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses of calls that are not refused are no memory")
+def test_pools_are_refused_where_they_share_rows_and_nowhere_else():
+    """Random small layouts, nested in every order and not nested, against the rows themselves. (Without a GPU a call that is not
+    refused ends in an error of its own.)"""
+    rng = random.Random(3)
+    some = [0, 0]
+    for _ in range(1500):
+        layers, n_pages, page, HK = rng.choice([1, 2, 3, 5]), rng.choice([1, 2, 4]), rng.choice([1, 2, 4]), rng.choice([1, 2, 3])
+        dims = [["ls", layers], ["ps", n_pages], ["rs", page], ["hs", HK], ["kv", 2]]
+        rng.shuffle(dims)
+        at, st = 128, {}
+        for name, n in dims:
+            st[name] = at
+            at = at * n + rng.choice([0, 0, 0, 8, 128])
+        if rng.random() < 0.5:
+            st["kv"] = rng.choice([1, -1]) * 8 * rng.randrange(0, at // 8 + 2)
+        if rng.random() < 0.3:
+            st["ls"] = 8 * rng.randrange(16, at // 8 + 2)
+        kw = dict(layers=layers, ls=st["ls"], ps=st["ps"], rs=st["rs"], hs=st["hs"], n_pages=n_pages, page=page, HK=HK)
+        token = st["rs"] >= (HK - 1) * st["hs"] + 128 and st["ps"] >= (page - 1) * st["rs"] + (HK - 1) * st["hs"] + 128
+        head = st["hs"] >= (page - 1) * st["rs"] + 128 and st["ps"] >= (HK - 1) * st["hs"] + (page - 1) * st["rs"] + 128
+        if not token and not head:
+            continue
+        shared = _shares(st["kv"], **kw)
+        some[shared] += 1
+        kp = 1 << 44
+        assert (_copy(kp=kp, vp=kp + 2 * st["kv"], **kw) == BAD) == shared, (kw, st["kv"])
+    assert min(some) > 100
 
 
 def test_parts_past_32_bits_are_refused():
