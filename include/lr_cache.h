@@ -33,8 +33,9 @@ extern "C" {
  * 0), rounded once to bf16; queries go to q_out rows, keys to the tokens' positions in the pages, values there as they are.
  * A token is rotated by table row positions[t] (int32 [T]), or without positions (NULL) by the row of its position in its
  * sequence; a token whose row is not one of the table's table_rows, or whose position the sequence's table or the pool does
- * not have, is left out whole. q NULL: keys and values only (q_out is not used). q_out may be q itself (same stride);
- * otherwise it must not overlap q, and the pool must not overlap q, k, v or q_out (rejected).
+ * not have, is left out whole. q NULL: keys and values only (q_out is not used). q_out may be q itself (same stride; k and v in
+ * other columns of the same rows, if they are views of one projection); otherwise it must not overlap q, k or v. The pool must not
+ * overlap q, k, v or q_out (all rejected).
  */
 int lr_cache_append_bf16(const void* q, const void* k, const void* v, int64_t q_row_stride, int64_t k_row_stride,
                          int64_t v_row_stride, void* q_out, int64_t q_out_row_stride, void* k_pages, void* v_pages,

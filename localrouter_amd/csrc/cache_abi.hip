@@ -31,7 +31,7 @@ bool rows_meet(int64_t d, const Level* levels, int n, int& left) {
     const Level& l = levels[0];
     if (l.lo == l.hi) return rows_meet(d - l.lo * l.stride, levels + 1, n - 1, left);
     int64_t below = lr::D - 1;
-    for (int i = 1; i < n; ++i) below += levels[i].hi * levels[i].stride;
+    for (int i = 1; i < n; ++i) below += std::max(-levels[i].lo, levels[i].hi) * levels[i].stride;
     const int64_t least = d - below;   // <= x * stride <= d + below
     for (int64_t x = std::max(least / l.stride + (least > 0 && least % l.stride), l.lo); x <= l.hi && x * l.stride <= d + below; ++x)
         if (rows_meet(d - x * l.stride, levels + 1, n - 1, left)) return true;
@@ -62,6 +62,20 @@ bool pool_ok(const void* k, const void* v, int64_t page, int64_t row, int64_t he
             break;
         }
     return !rows_meet(0, levels, 4, left);
+}
+// Whether a row of x (T of them, hx heads, x_rs apart) meets one of q (hq heads, q_rs apart): tensors that interleave, as the views of
+// one packed projection do, share a span but no row.
+bool packed_rows_meet(const void* q, int64_t q_rs, int hq, const void* x, int64_t x_rs, int hx, int T) {
+    if (!overlap(rows_span(q, T, q_rs, hq), rows_span(x, T, x_rs, hx))) return false;
+    const int64_t d = (reinterpret_cast<intptr_t>(x) - reinterpret_cast<intptr_t>(q)) / 2, last = T - 1;
+    int left = 4096;
+    if (last == 0 || q_rs == x_rs) {
+        const Level levels[2] = {{q_rs, -last, last}, {lr::D, 1 - hx, hq - 1}};
+        return rows_meet(d, levels, 2, left);
+    }
+    Level levels[3] = {{q_rs, 0, last}, {x_rs, -last, 0}, {lr::D, 1 - hx, hq - 1}};
+    if (x_rs > q_rs) std::swap(levels[0], levels[1]);
+    return rows_meet(d, levels, 3, left);
 }
 Span pool_span(const void* p, int layers, int64_t layer, int64_t page, int64_t row, int64_t head, int n_pages, int page_size,
                int HK) {
@@ -383,8 +397,11 @@ int lr_cache_append_bf16(const void* q, const void* k, const void* v, int64_t q_
         const Span sq = rows_span(q, T, q_row_stride, H), so = rows_span(q_out, T, q_out_row_stride, H);
         if (overlap(pk, sq) || overlap(pv, sq) || overlap(pk, so) || overlap(pv, so)) return ERR_ARGS;
         if (!(q_out == q && q_out_row_stride == q_row_stride) && overlap(sq, so)) return ERR_ARGS;
-        // (packed rows interleave: in place on the queries of a packed projection, its keys and values keep their columns)
-        if (!(q_out == q && q_out_row_stride == q_row_stride) && (overlap(so, sk) || overlap(so, sv))) return ERR_ARGS;
+        // (in place on the queries of a packed projection, whose keys and values have columns of their own)
+        if (q_out == q && q_out_row_stride == q_row_stride
+                ? packed_rows_meet(q, q_row_stride, H, k, k_row_stride, HK, T) || packed_rows_meet(q, q_row_stride, H, v, v_row_stride, HK, T)
+                : overlap(so, sk) || overlap(so, sv))
+            return ERR_ARGS;
     }
     lr::CacheAppendArgs a{};
     a.q = static_cast<const uint16_t*>(q);

@@ -114,6 +114,28 @@ def test_append_refuses(kw):
     assert _append(**kw) == BAD
 
 
+# in place on rows of 8 query heads: k or v over columns that are overwritten
+@pytest.mark.parametrize("kw", [
+    dict(k=Q), dict(v=Q), dict(k=Q + 2 * 896), dict(v=Q + 2 * (1536 - 128)), dict(k=Q + 2 * (5 * 1536 + 512)),
+    dict(v=Q + 2 * (1016)), dict(k=Q - 2 * 128), dict(k=Q + 2 * 1024, krs=768), dict(v=Q + 2 * 1024, vrs=1584),
+    dict(k=Q, krs=256, T=1), dict(v=Q + 2 * 1000, vrs=256, T=1),
+], ids=str)
+def test_append_in_place_refuses_keys_and_values_in_the_queries_columns(kw):
+    assert _append(**dict(dict(qo=Q, qrs=1536, qors=1536, krs=1536, vrs=1536), **kw)) == BAD
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses of calls that are not refused are no memory")
+@pytest.mark.parametrize("kw", [
+    dict(), dict(k=Q + 2 * 1024, v=Q + 2 * 1280), dict(k=Q + 2 * (4 * 1536 + 1024)), dict(v=Q + 2 * (1280 - 1536)),
+    dict(v=Q + 2 * 1024, vrs=1552),   # (row u, from column 1024 + 16 u on, ends at column 1456 at most)
+    dict(k=Q + 2 * 1024, krs=3072), dict(k=Q + 2 * 1024, krs=256, T=1), dict(k=Q + 2 * (1024 + 11 * 1536), krs=256),
+], ids=str)
+def test_append_in_place_on_a_packed_projection(kw):
+    """Keys and values in columns of their own, of these rows or others, are none of the queries' (without a GPU such a call ends in
+    an error of its own)."""
+    assert _append(**dict(dict(qo=Q, qrs=1536, qors=1536, krs=1536, vrs=1536), **kw)) != BAD
+
+
 def _copy(**kw):
     a = dict(kp=KP, vp=VP, layers=2, ls=1 << 20, ps=4096, rs=256, hs=128, n_pages=40, page=16, HK=2, src=I1, dst=I2, n=5,
              stream=None)

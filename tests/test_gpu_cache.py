@@ -666,6 +666,21 @@ def test_append_leaves_out_what_has_no_place():
     assert torch.equal(out[3:5], same)
 
 
+def test_append_in_place_needs_columns_of_its_own():
+    B = Batch(36, [5, 4], [20, 11], 16, 2)
+    qkv = rnd(B.g, 9, 8, 128)
+    args = (B.kp, B.vp, B.t, B.starts, B.lens)
+    for k, v in ((qkv[:, :2], qkv[:, 6:]), (qkv[:, 4:6], qkv[:, 3:5])):
+        with pytest.raises(_lib.LrError):
+            cache.append(qkv[:, :4], k, v, *args, qkv[:, :4], table_kind=ops.TABLE_NONE)
+    want_k, want_v = B.kp.clone(), B.vp.clone()
+    want = cache.append(qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], want_k, want_v, *args[2:], table_kind=ops.TABLE_NONE)
+    keep = qkv[:, 4:].clone()
+    cache.append(qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], *args, qkv[:, :4], table_kind=ops.TABLE_NONE)
+    assert torch.equal(qkv[:, :4], want) and torch.equal(qkv[:, 4:], keep)
+    assert torch.equal(B.kp, want_k) and torch.equal(B.vp, want_v)
+
+
 def test_append_of_column_views_of_a_table():
     """cos and sin as columns of a wider table: the view's columns count, not its rows' stride. Too narrow ones are refused, and
     nothing is written."""
