@@ -58,7 +58,8 @@ int lr_cache_append_bf16(const void* q, const void* k, const void* v, int64_t q_
  * sequence has more positions (those beyond are not seen). Both size the launch: a max_rows far above the tokens of any sequence
  * launches workgroups without rows for every sequence, and one that makes more of them than a grid holds (2^22) is rejected. At
  * most 2^30 positions; B at most 65,535.
- * workspace: lr_cache_attention_ws_bytes bytes (0: none, it may be NULL), 256-byte aligned; it must not overlap q, out or the
+ * workspace: lr_cache_attention_ws_bytes bytes for the same numbers (0: none, it may be NULL; fewer rows or positions may take
+ * more), 256-byte aligned; it must not overlap q, out or the
  * pool, nor out q or the pool (rejected). What it holds before the call does not matter. Calls that overlap in time on one
  * workspace race.
  */

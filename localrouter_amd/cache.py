@@ -94,7 +94,7 @@ def append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: to
 
 def attention_ws_bytes(B: int, T: int, max_rows: int, max_keys: int, heads: int, kv_heads: int, page_size: int, *,
                        window: int = 0, sinks: int = 0) -> int:
-    """lr_cache_attention_ws_bytes: the workspace a call needs (0: none)."""
+    """lr_cache_attention_ws_bytes: the workspace that a call with these numbers needs (0: none); smaller ones may need more."""
     return int(lib().lr_cache_attention_ws_bytes(B, T, max_rows, max_keys, heads, kv_heads, page_size, window, sinks))
 
 
@@ -106,8 +106,8 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     position p sees positions j <= p; with tree (int64 [T, words], bit x of a token's words: it sees the sequence's x-th token
     of the call) drafted tokens see everything before the call's tokens and what their bits say. window n >= 1: earlier
     positions (under a tree: those before the call's tokens) only where p - j < n or j < sinks. max_rows: the most tokens of a
-    sequence (default T); max_keys: the longest sequence (default what the table holds). A workspace of attention_ws_bytes is
-    allocated when none is given."""
+    sequence (default T); max_keys: the longest sequence (default what the table holds). A workspace of attention_ws_bytes
+    for the same numbers is allocated when none is given."""
     dev = _device(q)
     return (_calls or _host()).attention(dev, _raw_stream(dev), q, k_pages, v_pages, page_table, starts, lens, out, max_rows, max_keys,
                                          tree, window, sinks, scale, workspace)

@@ -300,7 +300,7 @@ PyObject* attention(PyObject* const* a) {
     if (T == 0) return held.release();
     const Table table(a[5], w, B);
     const int64_t most = std::min<int64_t>((int64_t)table.pages * pool.page_size, INT_MAX);
-    const int max_rows = at_most(a[9], "max_rows", T), max_keys = at_most(a[10], "max_keys", most);
+    int max_rows = at_most(a[9], "max_rows", T), max_keys = at_most(a[10], "max_keys", most);
     const uint64_t* tree = nullptr;
     int words = 0;
     if (!none(a[11])) {
@@ -313,8 +313,24 @@ PyObject* attention(PyObject* const* a) {
     const int window = int32(a[12], "window"), sinks = int32(a[13], "sinks");
     const float scale = number(a[14]);
     const int *starts = ints(a[6], "starts", w, B + 1), *lens = ints(a[7], "lens", w, B);
-    const Workspace ws(a[15], w, f_attention_ws((int)B, (int)T, max_rows, max_keys, (int)H, pool.heads, pool.page_size, window, sinks),
-                       qt);
+    auto ws_need = [&](int rows, int keys) {
+        return f_attention_ws((int)B, (int)T, rows, keys, (int)H, pool.heads, pool.page_size, window, sinks);
+    };
+    size_t need = ws_need(max_rows, max_keys);
+    // A workspace for a max_rows or max_keys beyond this call's tokens or its table may be smaller (more rows fill the GPU without
+    // parts): the launch is then sized as the workspace was.
+    if (!none(a[15]) && tensor(a[15], "workspace").nbytes() < need) {
+        constexpr int64_t MOST = 1 << 30;   // (the most rows and positions of a call)
+        const int rows = none(a[9]) ? max_rows : at_most(a[9], "max_rows", MOST / std::max<int64_t>(1, H / std::max(1, pool.heads)));
+        const int keys = none(a[10]) ? max_keys : at_most(a[10], "max_keys", MOST);
+        const size_t given = ws_need(rows, keys);
+        if (given <= tensor(a[15], "workspace").nbytes()) {
+            need = given;
+            max_rows = rows;
+            max_keys = keys;
+        }
+    }
+    const Workspace ws(a[15], w, need, qt);
     call("lr_cache_attention_bf16", [&] {
         return f_attention(q.p, q.rs, out.p, out.rs, pool.k, pool.v, pool.ps, pool.rs, pool.hs, pool.n_pages, pool.page_size, table.p,
                            table.rs, table.pages, starts, lens, (int)B, (int)T, max_rows, max_keys, (int)H, pool.heads, tree, words,

@@ -541,6 +541,28 @@ def test_workspace_streams_and_graphs():
         B.check(q, out, lambda b: chain_seen(1, new_lens[b]))
 
 
+@pytest.mark.parametrize("news,lens,H,HK,rows,keys", [
+    ([1, 1], [3900, 700], 32, 8, None, 6000),       # a table of fewer positions than max_keys says
+    ([8] * 8, [900] * 7 + [3900], 32, 8, 128, None),   # fewer tokens than max_rows says: none needed for as many as that
+])
+def test_workspaces_of_larger_numbers(news, lens, H, HK, rows, keys):
+    """A workspace of attention_ws_bytes for a max_rows or max_keys that is more than the tokens or the table is taken, also where the
+    call itself would be cut into more parts."""
+    B = Batch(37, news, lens, 16, HK)
+    T = sum(news)
+    q = rnd(B.g, T, H, 128)
+    most = B.width * 16
+    need = cache.attention_ws_bytes(len(news), T, rows or T, keys or most, H, HK, 16)
+    assert need < cache.attention_ws_bytes(len(news), T, min(rows or T, T), min(keys or most, most), H, HK, 16)
+    ws = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")
+    out = cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, max_rows=rows, max_keys=keys, workspace=ws[:need])
+    B.check(q, out, lambda b: chain_seen(news[b], lens[b]))
+    assert (ws[need:] == 255).all()
+    if need:
+        with pytest.raises(ValueError, match="contiguous bytes on the current device needed"):
+            cache.attention(q, B.kp, B.vp, B.t, B.starts, B.lens, max_rows=rows, max_keys=keys, workspace=ws[:need - 256])
+
+
 def test_the_same_call_gives_the_same_bits():
     B = Batch(20, [3, 1, 40], [2000, 700, 900], 16, 2)
     q = rnd(B.g, 44, 8, 128)
