@@ -88,6 +88,14 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+def int32(**numbers: int) -> list[int]:
+    """The numbers, none of them past 32 bits (ctypes would cut them)."""
+    for name, x in numbers.items():
+        if not -(1 << 31) <= x < 1 << 31:
+            raise ValueError(f"{name}: a 32-bit number expected")
+    return list(numbers.values())
+
+
 def call(name: str, *args) -> None:
     """Call an lr_* entry point that returns a hipError_t; raise LrError when it is not 0."""
     rc = getattr(load(), name)(*args)

@@ -95,7 +95,8 @@ def append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: to
 def attention_ws_bytes(B: int, T: int, max_rows: int, max_keys: int, heads: int, kv_heads: int, page_size: int, *,
                        window: int = 0, sinks: int = 0) -> int:
     """lr_cache_attention_ws_bytes: the workspace that a call with these numbers needs (0: none); smaller ones may need more."""
-    return int(lib().lr_cache_attention_ws_bytes(B, T, max_rows, max_keys, heads, kv_heads, page_size, window, sinks))
+    return int(lib().lr_cache_attention_ws_bytes(*_lib.int32(B=B, T=T, max_rows=max_rows, max_keys=max_keys, heads=heads,
+                                                             kv_heads=kv_heads, page_size=page_size, window=window, sinks=sinks)))
 
 
 def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor,

@@ -116,7 +116,8 @@ def attention_ws(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.T
 def attention_window_ws_bytes(w: int, heads: int, kv_heads: int, nkeys: int, *, window: int, sinks: int = 0,
                               frame: int = 1) -> int:
     """lr_attention_window_ws_bytes: the workspace lr_attention_window_bf16 needs (0: none)."""
-    return int(_lib.load().lr_attention_window_ws_bytes(w, heads, kv_heads, nkeys, window, sinks, frame))
+    return int(_lib.load().lr_attention_window_ws_bytes(*_lib.int32(w=w, heads=heads, kv_heads=kv_heads, nkeys=nkeys, window=window,
+                                                                    sinks=sinks, frame=frame)))
 
 
 def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor | None = None, *, window: int,

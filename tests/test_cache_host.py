@@ -73,6 +73,25 @@ def test_window_workspace_sizes():
     assert ops.attention_window_ws_bytes(1, 8, 2, 1 << 29, window=64) <= ops.attention_window_ws_bytes(1, 8, 2, 512, window=512)
 
 
+@pytest.mark.parametrize("name", ["w", "heads", "kv_heads", "nkeys", "window", "sinks", "frame"])
+@pytest.mark.parametrize("far", [1 << 32, -(1 << 33), 1 << 31])
+def test_window_workspace_of_numbers_past_32_bits(name, far):
+    """Refused by name, not cut to some other call's workspace."""
+    kw = dict(w=1, heads=8, kv_heads=2, nkeys=100000, window=100000, sinks=0, frame=1)
+    assert ops.attention_window_ws_bytes(**kw) > 0
+    with pytest.raises(ValueError, match=f"^{name}: a 32-bit number"):
+        ops.attention_window_ws_bytes(**dict(kw, **{name: kw[name] + far}))
+
+
+@pytest.mark.parametrize("name", ["B", "T", "max_rows", "max_keys", "heads", "kv_heads", "page_size", "window", "sinks"])
+@pytest.mark.parametrize("far", [1 << 32, -(1 << 33), 1 << 31])
+def test_cache_workspace_of_numbers_past_32_bits(name, far):
+    kw = dict(B=1, T=1, max_rows=1, max_keys=30000, heads=8, kv_heads=2, page_size=16, window=0, sinks=0)
+    assert cache.attention_ws_bytes(**kw) > 0
+    with pytest.raises(ValueError, match=f"^{name}: a 32-bit number"):
+        cache.attention_ws_bytes(**dict(kw, **{name: kw[name] + far}))
+
+
 def _attend(**kw):
     a = dict(q=Q, qrs=1024, out=O, ors=1024, kp=KP, vp=VP, ps=4096, rs=256, hs=128, n_pages=40, page=16, table=I1, trs=10,
              tp=10, starts=I2, lens=I3, B=3, T=12, rows=6, keys=160, H=8, HK=2, tree=0, words=0, window=0, sinks=0,
