@@ -386,6 +386,7 @@ PyObject* attention_window(PyObject* const* a) {
     Held held{rows_like(a[5], W, H, qt)};
     const Rows out(held.o, "out", w, W, H);
     if (W > INT_MAX || N > INT_MAX || H > INT_MAX || HK > INT_MAX) refuse("attention_window: too many rows");
+    if (W == 0) return held.release();
     const int window = int32(a[6], "window"), sinks = int32(a[7], "sinks"), frame = int32(a[8], "frame"), p0 = int32(a[9], "p0");
     const float scale = number(a[10]);
     const Workspace ws(a[11], w, f_window_ws((int)W, (int)H, (int)HK, (int)N, window, sinks, frame), qt);

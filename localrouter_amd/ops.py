@@ -125,7 +125,8 @@ def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: tor
                      workspace: torch.Tensor | None = None) -> torch.Tensor:
     """lr_attention_window_bf16: q [w, heads, 128] at positions p0 + i over k / v [nkeys, kv_heads, 128]; a query in frame
     f = position // frame sees the keys of frames f - window + 1 .. f and the first `sinks` keys (up to frame f). frame 1: a
-    sliding window of single tokens. A workspace of attention_window_ws_bytes is allocated when none is given."""
+    sliding window of single tokens. No queries: nothing to do. A workspace of attention_window_ws_bytes is allocated when none is
+    given."""
     from . import cache   # (its host calls; it imports this module)
     dev = cache._device(q)
     return cache._host().attention_window(dev, cache._raw_stream(dev), q, k, v, out, window, sinks, frame, p0, scale, workspace)

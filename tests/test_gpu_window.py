@@ -249,6 +249,17 @@ def test_window_largest_arguments():
     check_rows(out, *ref_rows(q, k, v, window_seen(70, 150, 80, 1 << 20, 0, 1)))
 
 
+def test_window_of_no_queries():
+    """As the cache's calls: an empty result, and the given tensor where there is one."""
+    g = gen(12)
+    q, k, v = rnd(g, 0, 4, 128), rnd(g, 9, 2, 128), rnd(g, 9, 2, 128)
+    assert ops.attention_window(q, k, v, window=4).shape == (0, 4, 128)
+    out = torch.full((3, 4, 128), 2.0, dtype=torch.bfloat16, device="cuda")
+    assert ops.attention_window(q, k, v, out, window=4) is out and (out == 2.0).all()
+    with pytest.raises(ValueError):
+        ops.attention_window(q, k, v[:5], window=4)
+
+
 def test_window_refuses_before_launch():
     g = gen(11)
     q, k, v = rnd(g, 4, 4, 128), rnd(g, 9, 2, 128), rnd(g, 9, 2, 128)
