@@ -67,16 +67,32 @@ HOST_CALLS = PKG / "native" / "host_calls.cpp"
 HOST_CALLS_LIB = PKG / "_host_calls.so"
 
 
-def host_calls_cmd(out: Path) -> list[str]:
+def host_calls_cmd(out: Path) -> list[str] | None:
+    """The compiler's command, or None where torch or Python's headers are not installed."""
     import importlib.util
     import sysconfig
     spec = importlib.util.find_spec("torch")   # (found, not imported)
-    if spec is None:
-        raise RuntimeError("torch not found (its headers are required to build localrouter_amd)")
+    include = Path(sysconfig.get_paths()["include"])
+    if spec is None or not (include / "Python.h").exists():
+        return None
     torch_dir = Path(spec.origin).parent
     return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", str(HOST_CALLS),
             "-o", str(out), f"-I{torch_dir / 'include'}", f"-I{torch_dir / 'include/torch/csrc/api/include'}",
-            f"-I{sysconfig.get_paths()['include']}", f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+            f"-I{include}", f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+
+
+def build_host_calls() -> Path | None:
+    """Compile the Python extension; None, said on stderr, where it cannot be: the library is whole without it, and the calls that go
+    through it raise."""
+    tmp = HOST_CALLS_LIB.with_suffix(".so.tmp")
+    cmd = host_calls_cmd(tmp)
+    if cmd is None:
+        HOST_CALLS_LIB.unlink(missing_ok=True)   # (an older one would be of another interface)
+        print("localrouter_amd: torch or Python.h not found: built without localrouter_amd.cache's host calls", file=sys.stderr)
+        return None
+    _run(cmd)
+    os.replace(tmp, HOST_CALLS_LIB)
+    return HOST_CALLS_LIB
 
 
 def hipcc() -> str:
@@ -154,7 +170,7 @@ def _run(cmd: list[str]) -> str:
 
 
 def build(verbose: bool = False) -> Path:
-    """Compile every HIP source to an object, then link liblr_attn.so. Always recompiles."""
+    """Compile every HIP source to an object, then link liblr_attn.so; then the Python extension. Always recompiles."""
     cc = hipcc()
     objdir = PKG / "_build"
     objdir.mkdir(exist_ok=True)
@@ -192,9 +208,7 @@ def build(verbose: bool = False) -> Path:
     tmp = LIB.with_suffix(".so.tmp")
     _run([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, *LIBS, "-o", str(tmp)])
     os.replace(tmp, LIB)
-    tmp = HOST_CALLS_LIB.with_suffix(".so.tmp")
-    _run(host_calls_cmd(tmp))
-    os.replace(tmp, HOST_CALLS_LIB)
+    build_host_calls()
     return LIB
 
 

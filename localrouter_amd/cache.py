@@ -59,7 +59,11 @@ def _host():
     """The host side of the calls (native/host_calls.cpp), given the library's addresses at the first call."""
     global _calls
     if _calls is None:
-        from . import _host_calls
+        try:
+            from . import _host_calls
+        except ImportError as e:
+            raise RuntimeError("localrouter_amd._host_calls is missing: build it with `python -m localrouter_amd.build` where torch and "
+                               "Python's headers are installed (there is no fallback path)") from e
         L = lib()
         names = [*SIGNATURES, "lr_attention_window_bf16", "lr_attention_window_ws_bytes"]
         _host_calls.bind(_lib.LrError, {n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names})

@@ -389,3 +389,34 @@ def test_append_refuses_tables_that_are_narrower_than_the_rotation(kind, rot, co
             call(a, a if two else None)
     with pytest.raises(ValueError, match="table: expected a tensor"):
         call(None, None)
+
+
+@pytest.mark.parametrize("missing", ["torch", "Python.h"])
+def test_the_library_is_built_without_torch_or_python_headers(missing, monkeypatch, tmp_path, capsys):
+    """The extension is left out and said to be, an older one goes away, and nothing else fails."""
+    import importlib.util
+    import sysconfig
+
+    from localrouter_amd import build
+    find, paths = importlib.util.find_spec, sysconfig.get_paths()
+    if missing == "torch":
+        monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: None if name == "torch" else find(name, *a))
+    else:
+        monkeypatch.setattr(sysconfig, "get_paths", lambda *a, **kw: dict(paths, include=str(tmp_path)))
+    old = tmp_path / "_host_calls.so"
+    old.write_bytes(b"old")
+    monkeypatch.setattr(build, "HOST_CALLS_LIB", old)
+    monkeypatch.setattr(build, "_run", lambda cmd: pytest.fail(f"ran {cmd}"))
+    assert build.build_host_calls() is None and not old.exists()
+    assert "without localrouter_amd.cache's host calls" in capsys.readouterr().err
+
+
+def test_calls_without_the_extension_raise(monkeypatch):
+    import sys
+
+    import localrouter_amd
+    monkeypatch.setitem(sys.modules, "localrouter_amd._host_calls", None)
+    monkeypatch.delattr(localrouter_amd, "_host_calls", raising=False)
+    monkeypatch.setattr(cache, "_calls", None)
+    with pytest.raises(RuntimeError, match="_host_calls is missing"):
+        cache._host()
