@@ -346,6 +346,18 @@ def test_pool_compact_packs_to_the_front():
     assert pool.compact([]) == ([], []) if pool.free_pages == 8 else True
 
 
+def test_pool_compact_of_nothing():
+    for pool in (cache.PagePool(8), cache.PagePool(1)):
+        n = pool.free_pages
+        assert pool.compact([]) == ([], []) and pool.free_pages == n and sorted(pool.alloc(n)) == list(range(n))
+    pool = cache.PagePool(8)
+    pool.free(pool.alloc(5))
+    assert pool.compact([[], []]) == ([], []) and pool.free_pages == 8
+    pool.alloc(1)
+    with pytest.raises(ValueError):
+        pool.compact([])
+
+
 def test_host_calls_refuse_host_tensors_by_name():
     """The calls' own checks, past the Python side's: every tensor is refused by its name, with what it is."""
     h = cache._host()
