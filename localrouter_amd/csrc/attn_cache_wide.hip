@@ -15,6 +15,7 @@
 //    two: scalar bases from the staged page-table entries.
 //  * A row that overflowed its reference, or met an infinity or NaN, is computed again over the keys that it sees.
 #include "lr_common.h"
+#include "block_order.h"
 #include "lr_cache_kernels.h"
 #include "tile_image.h"
 
@@ -60,13 +61,11 @@ __device__ __forceinline__ int seq_by_length(const RangeAttnArgs& a, int rank) {
 // whole heads, one after the other (the blocks of a head share its keys in the XCD's L2), the last blocks of a head first:
 // without a full window they are the longest; otherwise the heads alternate. Pages: longest sequences first, the blocks of one
 // sequence and head next to each other, by_xcd on one XCD. The first `whole` blocks (of an XCD, or of the launch) are not cut.
-template <bool PAGED>
+template <int QW, bool PAGED>
 __device__ __forceinline__ bool block_of(const RangeAttnArgs& a, int id, int& b, int& hk, int& blk, int& split, int& cut) {
     const int xcd = a.by_xcd ? id & 7 : 0;
     int idx = a.by_xcd ? id >> 3 : id;
-    // Workgroups 32 apart of an XCD share a CU: where all of them are resident at once, the second 32 go in the opposite
-    // order, the shortest beside the longest.
-    if (a.by_xcd && a.nsplit == 1 && a.local <= 64 && idx >= 32) idx = a.local + 31 - idx;
+    if (a.by_xcd && a.nsplit == 1) idx = start_order(idx, a.local, 8 / QW);
     split = 0;
     cut = -1;
     if (a.nsplit > 1 && idx >= a.whole) {
@@ -186,7 +185,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         split = 0;
         const bool all = px1 - px0 == __builtin_amdgcn_readlane(pc.tiles, j);
         cut = all ? -1 : (xcd * (pc.P + a.teams) + at) * a.nblk + blk;
-    } else if (!block_of<PAGED>(a, blockIdx.x, b, hk, blk, split, cut)) {
+    } else if (!block_of<QW, PAGED>(a, blockIdx.x, b, hk, blk, split, cut)) {
         return;
     }
     b = __builtin_amdgcn_readfirstlane(b);
@@ -636,7 +635,7 @@ __global__ __launch_bounds__(256) void range_wide_merge_kernel(RangeAttnArgs a) 
     const int of = a.local - a.whole;   // cut blocks an XCD
     const int xcd = a.by_xcd ? c / of : 0, first = a.whole + (c - xcd * of) * a.nsplit;   // the block's first workgroup
     int b, hk, blk, split, cut;
-    if (!block_of<PAGED>(a, a.by_xcd ? 8 * first + xcd : first, b, hk, blk, split, cut)) return;
+    if (!block_of<QW, PAGED>(a, a.by_xcd ? 8 * first + xcd : first, b, hk, blk, split, cut)) return;
     b = __builtin_amdgcn_readfirstlane(b);
     const Seq sq = seq_of<PAGED>(a, b);
     merge_rows<QW>(a, sq, hk, blk, w, a.nsplit, [&](int x) { return (int64_t)cut * a.nsplit + x; });
