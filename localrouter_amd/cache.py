@@ -111,7 +111,9 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     position p sees positions j <= p; with tree (int64 [T, words], bit x of a token's words: it sees the sequence's x-th token
     of the call) drafted tokens see everything before the call's tokens and what their bits say. window n >= 1: earlier
     positions (under a tree: those before the call's tokens) only where p - j < n or j < sinks. max_rows: the most tokens of a
-    sequence (default T); max_keys: the longest sequence (default what the table holds). A workspace of attention_ws_bytes
+    sequence; max_keys: the longest sequence. Both choose the kernel and size the launch, which has workgroups for max_rows tokens of
+    every sequence: give them. Their defaults, all T tokens and what the table holds, are for single sequences; of a batch most
+    workgroups are without rows then, and where a grid does not hold them the call is refused. A workspace of attention_ws_bytes
     for the same numbers is allocated when none is given."""
     dev = _device(q)
     return (_calls or _host()).attention(dev, _raw_stream(dev), q, k_pages, v_pages, page_table, starts, lens, out, max_rows, max_keys,

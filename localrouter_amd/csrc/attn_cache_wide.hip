@@ -4,7 +4,8 @@
 // (tokens x the query heads of one kv head), four waves of 32 rows over a ring of two key tiles and two value tiles; two
 // workgroups share a CU, one's start, end and waits under the other's products. Long calls that fill the CUs take 256 rows, eight
 // waves and four of each tile. What bounds them is the clock under the power limit: 16,384 tokens x 32 heads over windows of four
-// frames of 1,024 run at 1,110 TFLOP/s and ~1.7 GHz, MFMA busy ~60 %. What differs from the key-split kernel:
+// frames of 1,024 run at 1,034 to 1,135 TFLOP/s; under the profiler at 1.79 GHz, MFMA busy 52 % of the call. What differs from the
+// key-split kernel:
 //
 //  * The tiles are a list (the first tokens' tiles, then the rows' own range), and a half-tile that some row of the wave does
 //    not see whole takes a masked step: its 32 keys' visibility as one word a row, built from the row's limits (and its tree
@@ -60,7 +61,8 @@ __device__ __forceinline__ int seq_by_length(const RangeAttnArgs& a, int rank) {
 // Hardware workgroup id runs on XCD id % 8; with by_xcd `idx` is its number there, else it is id. Rows, by_xcd: an XCD works on
 // whole heads, one after the other (the blocks of a head share its keys in the XCD's L2), the last blocks of a head first:
 // without a full window they are the longest; otherwise the heads alternate. Pages: longest sequences first, the blocks of one
-// sequence and head next to each other, by_xcd on one XCD. The first `whole` blocks (of an XCD, or of the launch) are not cut.
+// sequence and head next to each other, by_xcd on one XCD (in the order of
+// block_order.h). The first `whole` blocks (of an XCD, or of the launch) are not cut.
 template <int QW, bool PAGED>
 __device__ __forceinline__ bool block_of(const RangeAttnArgs& a, int id, int& b, int& hk, int& blk, int& split, int& cut) {
     const int xcd = a.by_xcd ? id & 7 : 0;

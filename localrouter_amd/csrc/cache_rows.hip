@@ -1,8 +1,9 @@
 // The passes that write a cache in pages (gfx950): the append (head norms and rotation of new tokens, their keys and values
 // into pages), page copies and row moves. All three are bound by memory: every byte is read once and written once, 16 bytes
 // a lane, a row of one head (256 bytes) by 16 lanes. 16,000 tokens of 32 + 2 x 8 heads appended 60 us (4.9 TB/s), 1,000 pages of 16
-// rows x 8 heads copied in 16 layers 387 us (5.4 TB/s), 40 x 5 rows moved in 32 layers 12.7 us (4.1 TB/s; the chain starts, positions,
-// page entries, rows); the smallest calls 3 to 4.5 us, launch and chain.
+// rows x 8 heads copied in 16 layers 387 us (5.4 TB/s), 40 x 5 rows moved in 32 layers 12.7 to 14.2 us (3.7 to 4.1 TB/s; the chain
+// starts, positions, page entries, rows); the smallest calls 3 (a page's copy) to 4.5 us (32 tokens appended: the chain of a token's
+// sequence, its length, page entry and table row).
 #include "lr_common.h"
 #include "lr_cache_kernels.h"
 
