@@ -84,9 +84,9 @@ int lr_cache_copy_pages(void* k_pages, void* v_pages, int layers, int64_t layer_
 /*
  * Rows moved inside their sequences, in every layer: for the moves starts[b] .. starts[b + 1] - 1 of sequence b (n in all, at
  * most max_rows <= 256 a sequence: those beyond are left out), position src[i] to position dst[i]. All of a sequence's rows
- * are read before any is written, so the moves of a sequence may chain or swap; of several moves to one position one wins.
- * Moves with a position that the table or the pool does not have are left out. Sequences that share pages must not move
- * rows of those.
+ * are read before any is written, so the moves of a sequence may chain or swap. No position may be the target of two moves of a
+ * sequence: each of its heads' keys and values would be either one's, not all of them the same one's. Moves with a position that
+ * the table or the pool does not have are left out. Sequences that share pages must not move rows of those.
  */
 int lr_cache_move_rows(void* k_pages, void* v_pages, int layers, int64_t layer_stride, int64_t page_stride,
                        int64_t row_stride, int64_t head_stride, int n_pages, int page_size, int HK, const int* page_table,

@@ -130,8 +130,8 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, 
 def move_rows(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor,
               src: torch.Tensor, dst: torch.Tensor, *, max_rows: int | None = None) -> None:
     """lr_cache_move_rows: for the moves starts[b] .. starts[b + 1] of sequence b, its position src[i] to its position dst[i],
-    in every layer; a sequence's rows are all read before any is written. max_rows: the most moves of a sequence (at most 256;
-    default all of them)."""
+    in every layer; a sequence's rows are all read before any is written. No position may be a target
+    twice. max_rows: the most moves of a sequence (at most 256; default all of them)."""
     dev = _device(k_pages)
     (_calls or _host()).move_rows(dev, _raw_stream(dev), k_pages, v_pages, page_table, starts, src, dst, max_rows)
 
