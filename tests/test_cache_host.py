@@ -147,7 +147,7 @@ def test_append_in_place_refuses_keys_and_values_in_the_queries_columns(kw):
 @pytest.mark.parametrize("kw", [
     dict(), dict(k=Q + 2 * 1024, v=Q + 2 * 1280), dict(k=Q + 2 * (4 * 1536 + 1024)), dict(v=Q + 2 * (1280 - 1536)),
     dict(v=Q + 2 * 1024, vrs=1552),   # (row u, from column 1024 + 16 u on, ends at column 1456 at most)
-    dict(k=Q + 2 * 1024, krs=3072), dict(k=Q + 2 * 1024, krs=256, T=1), dict(k=Q + 2 * (1024 + 11 * 1536), krs=256),
+    dict(k=Q + 2 * 1024, krs=4608), dict(k=Q + 2 * 1024, krs=256, T=1), dict(k=Q + 2 * (1024 + 11 * 1536), krs=256),
 ], ids=str)
 def test_append_in_place_on_a_packed_projection(kw):
     """Keys and values in columns of their own, of these rows or others, are none of the queries' (without a GPU such a call ends in
