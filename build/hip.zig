@@ -28,6 +28,8 @@ const sources = [_]Source{
     .{ .file = "attn_cache_wide.hip", .extra = &.{ "-mllvm", "-pragma-unroll-threshold=1000000" } },
     .{ .file = "cache_rows.hip" },
     .{ .file = "cache_abi.hip" },
+    .{ .file = "attn_cache8.hip" },
+    .{ .file = "cache8_rows.hip" },
 };
 
 /// hipcc flags of every device source: gfx950 only, no packed-fp32 instruction selection (v_pk_*_f32 are left to

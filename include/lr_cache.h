@@ -16,6 +16,7 @@
  * (int32, table_pages entries a sequence). An entry outside [0, n_pages) holds no rows: nothing is written there, and its
  * positions are not seen. Tokens at and behind starts[B], if T is larger, are left out: their output rows stay as they were.
  * starts, lens and the tables are read by the kernels: a captured call follows what they hold at its replay.
+ * Pages of 8 bits: lr_cache8.h.
  */
 #ifndef LR_CACHE_H
 #define LR_CACHE_H

@@ -22,7 +22,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "liblr_attn.so"
 SOURCES = ["attn_fwd.hip", "attn_stream.hip", "attn_keysplit.hip", "kv_image.hip", "rms_rope.hip", "int8_attn.hip",
            "keys.hip", "lr_abi.hip", "mmdit.hip", "attn_cache.hip", "attn_cache_wide.hip",
-           "cache_rows.hip", "cache_abi.hip", "rope_host.cpp"]
+           "cache_rows.hip", "cache_abi.hip", "attn_cache8.hip", "cache8_rows.hip", "rope_host.cpp"]
 # libraries the shared object links: hipBLASLt for the MMDiT block's projections and MLP
 LIBS = ["-L/opt/rocm/lib", "-lhipblaslt"]
 ARCH = "gfx950"

@@ -1,15 +1,20 @@
-"""ctypes mirror of include/lr_cache.h for torch tensors: a key / value cache in pages.
+"""ctypes mirror of include/lr_cache.h and lr_cache8.h for torch tensors: a key / value cache in pages.
 
     append(q, k, v, k_pages, v_pages, page_table, starts, lens, ...)   norms, rotation and the write of new tokens, one pass
     attention(q, k_pages, v_pages, page_table, starts, lens, ...)      decode steps, chunks, drafted trees, windows
     copy_pages(k_pages, v_pages, src, dst)                             pages copied inside the pool, in every layer
     move_rows(k_pages, v_pages, page_table, starts, src, dst, ...)     rows moved inside their sequences, in every layer
+    append_f8, attention_f8, copy_pages_f8                             the same over pages in 8 bits
     PagePool(n_pages)                                                  which pages are free, and who shares one (host only)
 
 k_pages / v_pages: bf16 [n_pages, page_size, heads, 128] (copy_pages and move_rows also [layers, ...]), the same strides in
 both; a pool laid out head by head is the permuted view of [n_pages, heads, page_size, 128]. page_table: int32 [B, pages a
 sequence]; starts: int32 [B + 1], the call's tokens of sequence b being rows starts[b] .. starts[b + 1]; lens: int32 [B], the
 sequences' lengths with those tokens. All on the current device.
+
+Pages in 8 bits: float8_e4m3fn of the same shape (page_size 16 or more), and k_scales / v_scales: float8_e8m0fnu
+[n_pages, page_size / 16, heads], its last two dimensions contiguous: the power of two of 16 rows of a page and head. What a pool holds
+is pages.float() * scales.float().repeat_interleave(16, 1)[..., None].
 
 Every call checks its tensors on the host (native/host_calls.cpp), then goes through the C ABI on torch's current HIP stream. There
 is no fallback: without the built library every call raises.
@@ -26,6 +31,7 @@ from . import _lib
 from .ops import PAIR_INTERLEAVED, SCALE_128, TABLE_COSSIN_F32, TABLE_NONE
 
 HEADER = Path(__file__).resolve().parent.parent / "include" / "lr_cache.h"
+HEADER_F8 = HEADER.with_name("lr_cache8.h")
 
 _P, _I, _I64, _F, _SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
 
@@ -39,6 +45,15 @@ SIGNATURES = {
     "lr_cache_move_rows": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _I, _I, _I, _P, _I64, _I, _P, _P, _P, _I, _I, _I, _P]),
 }
 
+SIGNATURES_F8 = {
+    "lr_cache_append_f8": (_I, [_P, _P, _P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I, _I, _P, _P, _I64, _P, _I64, _I,
+                                _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _P, _P, _I64, _I, _I, _I, _F, _P]),
+    "lr_cache_attention_f8_ws_bytes": (_SZ, [_I] * 9),
+    "lr_cache_attention_f8": (_I, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I, _I, _P, _P, _I64, _P, _I64, _I, _P, _P, _I, _I,
+                                   _I, _I, _I, _I, _P, _I, _I, _I, _F, _P, _SZ, _P]),
+    "lr_cache_copy_pages_f8": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _I, _I, _I, _P, _P, _I64, _I64, _P, _P, _I, _P]),
+}
+
 _bound = None
 _calls = None
 _current, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
@@ -48,7 +63,7 @@ def lib() -> ctypes.CDLL:
     global _bound
     if _bound is None:
         L = _lib.load()
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in (SIGNATURES | SIGNATURES_F8).items():
             fn = getattr(L, name)
             fn.restype, fn.argtypes = res, args
         _bound = L
@@ -65,7 +80,7 @@ def _host():
             raise RuntimeError("localrouter_amd._host_calls is missing: build it with `python -m localrouter_amd.build` where torch and "
                                "Python's headers are installed (there is no fallback path)") from e
         L = lib()
-        names = [*SIGNATURES, "lr_attention_window_bf16", "lr_attention_window_ws_bytes"]
+        names = [*SIGNATURES, *SIGNATURES_F8, "lr_attention_window_bf16", "lr_attention_window_ws_bytes"]
         _host_calls.bind(_lib.LrError, {n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names})
         _calls = _host_calls
     return _calls
@@ -134,6 +149,47 @@ def move_rows(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Te
     twice. max_rows: the most moves of a sequence (at most 256; default all of them)."""
     dev = _device(k_pages)
     (_calls or _host()).move_rows(dev, _raw_stream(dev), k_pages, v_pages, page_table, starts, src, dst, max_rows)
+
+
+def append_f8(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+              k_scales: torch.Tensor, v_scales: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor,
+              q_out: torch.Tensor | None = None, *, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+              table_kind: int = TABLE_COSSIN_F32, table: tuple | None = None, positions: torch.Tensor | None = None,
+              pairing: int = PAIR_INTERLEAVED, rot: int = 128, eps: float = 1e-6) -> torch.Tensor | None:
+    """lr_cache_append_f8: append() into pages in 8 bits. Keys and values are rounded once, from fp32, to the scale of their 16 rows, the
+    least power of two that holds the call's rows among them; where earlier positions of the sequence lie among them it is no less
+    than before, and if it rises their rows are rounded again. An infinity or NaN is held as NaN and has no part in the scale."""
+    dev = _device(k_pages)
+    if table is None:
+        if table_kind != TABLE_NONE:
+            raise ValueError("append_f8: table required")
+        table = (None, None)
+    return (_calls or _host()).append_f8(dev, _raw_stream(dev), q, k, v, k_pages, v_pages, page_table, starts, lens, q_out, q_norm,
+                                         k_norm, table_kind, table[0], table[1], positions, pairing, rot, eps, k_scales, v_scales)
+
+
+def attention_f8_ws_bytes(B: int, T: int, max_rows: int, max_keys: int, heads: int, kv_heads: int, page_size: int, *,
+                          window: int = 0, sinks: int = 0) -> int:
+    """lr_cache_attention_f8_ws_bytes: the workspace that attention_f8 with these numbers needs (0: none); smaller ones may need more."""
+    return int(lib().lr_cache_attention_f8_ws_bytes(*_lib.int32(B=B, T=T, max_rows=max_rows, max_keys=max_keys, heads=heads,
+                                                                kv_heads=kv_heads, page_size=page_size, window=window, sinks=sinks)))
+
+
+def attention_f8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                 page_table: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, out: torch.Tensor | None = None, *,
+                 max_rows: int | None = None, max_keys: int | None = None, tree: torch.Tensor | None = None, window: int = 0,
+                 sinks: int = 0, scale: float = SCALE_128, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """lr_cache_attention_f8: attention() over pages in 8 bits; queries, probabilities and the output are bf16."""
+    dev = _device(q)
+    return (_calls or _host()).attention_f8(dev, _raw_stream(dev), q, k_pages, v_pages, page_table, starts, lens, out, max_rows,
+                                            max_keys, tree, window, sinks, scale, workspace, k_scales, v_scales)
+
+
+def copy_pages_f8(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor, src: torch.Tensor,
+                  dst: torch.Tensor) -> None:
+    """lr_cache_copy_pages_f8: copy_pages() of pages in 8 bits and their scales ([layers, ...] in both or in neither)."""
+    dev = _device(k_pages)
+    (_calls or _host()).copy_pages_f8(dev, _raw_stream(dev), k_pages, v_pages, k_scales, v_scales, src, dst)
 
 
 class PagePool:

@@ -26,106 +26,14 @@ namespace {
 #include "attn_common.inc"
 
 #include "range_attn.inc"
-
-constexpr uint64_t PART_DONE = 0x7ff4a3c57fb5d96e;
-
-// The parts of one block of BR rows. (sc1, 16: coherent at device scope, not kept in this XCD's L2; the last workgroup of the block
-// may run on another.)
-template <int BR>
-struct PartRows {
-    __amdgpu_buffer_rsrc_t rs_o, rs_ml;
-    uint64_t* flags;
-
-    __device__ __forceinline__ PartRows(const RangeAttnArgs& a, int64_t block) {
-        rs_o = __builtin_amdgcn_make_buffer_rsrc(a.part_o + block * a.nsplit * BR * D, 0, a.nsplit * BR * D * 4, 0x00020000);
-        rs_ml = __builtin_amdgcn_make_buffer_rsrc(a.part_ml + block * a.nsplit * BR * 2, 0, a.nsplit * BR * 8, 0x00020000);
-        flags = a.flags + block * a.nsplit;
-    }
-    __device__ __forceinline__ void put_ml(int split, int q, float m, float l) const {
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, rs_ml, (split * BR + q) * 8, 0, 16);
-    }
-    __device__ __forceinline__ void put4(int split, int q, int dim, f32x4 y) const {
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), rs_o, ((split * BR + q) * D + dim) * 4, 0, 16);
-    }
-    __device__ __forceinline__ void put_row2(int split, int q, float o0, float o1, float m, float l) const {
-        const int lane = threadIdx.x & 63;
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(o0), __float_as_uint(o1)}, rs_o,
-                                              ((split * BR + q) * D + 2 * lane) * 4, 0, 16);
-        if (lane == 0) put_ml(split, q, m, l);
-    }
-
-    // The last of the block's parts to end merges them, in their order (every wave's rows are in memory). A part whose rows are
-    // in memory sets its flag, then reads all of them: the last to set its own sees every one (two that do write the same
-    // rows). Flags need no clearing before the call: only PART_DONE counts (as a float or a pair of them a NaN that no arithmetic
-    // makes), and who merges clears them.
-    template <int NW>
-    __device__ __forceinline__ void merge_last(const RangeAttnArgs& a, const Seq& sq, int hk, int row0, int rows, int split,
-                                               int parts, int* shared) const {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        if (wave == 0) {   // (alone: a flag set after the merge would outlive the call)
-            if (lane == 0) __hip_atomic_store(flags + split, PART_DONE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            LR_WAIT_VMCNT(0);
-            bool done = true;
-            for (int s0 = 0; s0 < parts; s0 += 64)
-                done = done && __hip_atomic_load(flags + min(s0 + lane, parts - 1), __ATOMIC_RELAXED,
-                                                 __HIP_MEMORY_SCOPE_AGENT) == PART_DONE;
-            const bool last = __builtin_amdgcn_ballot_w64(done) == ~0ull;
-            if (lane == 0) shared[0] = last;
-            if (last)
-                for (int s0 = lane; s0 < parts; s0 += 64)
-                    __hip_atomic_store(flags + s0, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        __syncthreads();
-        if (!__builtin_amdgcn_readfirstlane(shared[0])) return;
-        // 32 lanes a row (dims 4 c .. 4 c + 3), two rows a wave, eight parts in flight
-        static_assert(BR == 2 * NW, "one pass");
-        const int mc = lane & 31;
-        if (2 * wave < rows - row0) {
-            const int q = min(2 * wave + (lane >> 5), rows - row0 - 1);   // (past the last row: that one again, the same)
-            float M = -INFINITY, L = 0.0f;
-            f32x4 sum{};
-            for (int s0 = 0; s0 < parts; s0 += 8) {
-                u32x2 ml[8];
-                u32x4 x[8];
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int at = min(s0 + u, parts - 1) * BR + q;
-                    ml[u] = __builtin_amdgcn_raw_buffer_load_b64(rs_ml, at * 8, 0, 16);
-                    x[u] = __builtin_amdgcn_raw_buffer_load_b128(rs_o, at * D * 4 + 16 * mc, 0, 16);
-                }
-                float Mn = M;
-#pragma unroll
-                for (int u = 0; u < 8; ++u) Mn = fmaxf(Mn, __uint_as_float(ml[u][0]));
-                const float ref = Mn > -INFINITY ? Mn : 0.0f, alpha = __builtin_amdgcn_exp2f(M - ref);
-                M = Mn;
-                L *= alpha;
-                sum *= alpha;
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    // a part that saw no key has no weight, whatever is in its row
-                    const float m = __uint_as_float(ml[u][0]);
-                    const bool in = m > -INFINITY && s0 + u < parts;
-                    const float w = __builtin_amdgcn_exp2f(m - ref);
-                    L = in ? fmaf(w, __uint_as_float(ml[u][1]), L) : L;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sum[e] = in ? fmaf(w, __uint_as_float(x[u][e]), sum[e]) : sum[e];
-                }
-            }
-            const int ri = div_small(row0 + q, a.G, a.rcp_g), rhead = hk * a.G + row0 + q - ri * a.G;
-            const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-            u32x2 w;
-            w[0] = pack_bf16x2(sum[0] * inv, sum[1] * inv);
-            w[1] = pack_bf16x2(sum[2] * inv, sum[3] * inv);
-            *reinterpret_cast<u32x2*>(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D + 4 * mc) = w;
-        }
-    }
-};
+#include "range_parts.inc"
 
 // The direct loads of a tile by wave rb of RB: instruction u fills rows 4 u .. 4 u + 3, 16-byte chunks swizzled as attn_fwd.hip's.
-template <int RB, bool PAGED>
-__device__ __forceinline__ void load_tile_rows(const RangeAttnArgs& a, const Seq& sq, const TileList<RANGE_TILE, PAGED>& tl,
+template <int RB, int SRC>
+__device__ __forceinline__ void load_tile_rows(const RangeAttnArgs& a, const Seq& sq, const TileList<RANGE_TILE, SRC>& tl,
                                                int64_t hoff, int x, uint32_t k_lds, uint32_t v_lds, int rb) {
     constexpr int BT = RANGE_TILE, LOADS = 8 / RB;
+    constexpr bool PAGED = paged(SRC);
     const int lane = threadIdx.x & 63, lrow = lane >> 4, lchunk = lane & 15, key0 = tl.key0(x);
     const int64_t k_rs = PAGED ? a.pg.rs : a.k_rs, v_rs = PAGED ? a.pg.rs : a.v_rs;
     const uint16_t *kp = a.k + hoff, *vp = a.v + hoff;
@@ -153,39 +61,13 @@ __device__ __forceinline__ void load_tile_rows(const RangeAttnArgs& a, const Seq
     }
 }
 
-// A lane's value over the four lanes of its row (16 apart).
-__device__ __forceinline__ float quad_max(float x) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return wave_pair_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-}
-__device__ __forceinline__ float quad_sum(float x) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return wave_pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-}
-
-// The rows of which a group of waves (RB of them) has bits set, again, by its KG waves in turn; f(q): row q of the group. Where every
-// wave's rows were in memory before, they are afterwards.
-template <int RB, int KG, class F>
-__device__ __forceinline__ void again_rows(int* shared, int rb, int kg, uint32_t bits, F&& f) {
-    if (!__syncthreads_or(bits != 0)) return;
-    LR_WAIT_VMCNT(0);   // (the rows that are overwritten below)
-    if (threadIdx.x < RB) shared[threadIdx.x] = 0;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) atomicOr(shared + rb, (int)bits);
-    __syncthreads();
-    uint32_t left = (uint32_t)shared[rb];
-    for (int nth = 0; left; left &= left - 1, ++nth)
-        if (nth % KG == kg) f(__builtin_amdgcn_readfirstlane(__builtin_ctz(left)));
-    LR_WAIT_VMCNT(0);
-    __syncthreads();
-}
-
 // Blocks of 64 and 128 rows: KG groups of RB waves (32 rows each) alternate over the tiles, a ring of NS of them a group, on
 // v_mfma_f32_32x32x16_bf16 (the pipelined kernel's fragments, attn_fwd.hip). Bound by HBM where it is taken (32 sequences of 16,000
 // keys over 8 kv heads, 64 rows each, 2.1 GB, 384 us = 5.5 TB/s): one read of the keys for all rows is what counts.
-template <int RB, int KG, int NS, bool PAGED>
+template <int RB, int KG, int NS, int SRC>
 __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(RangeAttnArgs a) {
     constexpr int BT = RANGE_TILE, TILE = BT * D, NW = RB * KG;
+    constexpr bool PAGED = paged(SRC);
     constexpr int LOADS = 8 / RB;   // direct loads (4 rows each) per wave per K or V tile
     typedef __attribute__((address_space(3))) i16x4_t lds_i16x4;
     constexpr int RING = KG * NS * TILE * 2 * 2, MERGE = KG * RB * (64 * 64 + 2 * 64) * 4;
@@ -201,11 +83,11 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     const int at = div_small(idx, a.nsplit, a.rcp_split), split = idx - at * a.nsplit;
     const int blk = div_small(at, a.HK, a.rcp_hk), hk = at - blk * a.HK;
     const int b = blockIdx.y;
-    const Seq sq = seq_of<PAGED>(a, b);
+    const Seq sq = seq_of<SRC>(a, b);
     const int row0 = blk * 32 * RB;
     const int rows = max(sq.n, 0) * a.G;   // (at most 2^30: the host checks)
     if (row0 >= rows) return;
-    TileList<BT, PAGED> tl;
+    TileList<BT, SRC> tl;
     tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + 32 * RB) - 1, a.G, a.rcp_g));
     tl.part(split, a.per);
     const int parts = min(a.nsplit, max(1, (tl.total + a.per - 1) / a.per));   // the sequence may be shorter than the longest
@@ -216,9 +98,9 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     const int wr0 = row0 + 32 * rb, r = wr0 + n;
     const bool live = r < rows;
     const int rr = min(r, rows - 1), i = div_small(rr, a.G, a.rcp_g), head = hk * a.G + rr - i * a.G;
-    const Sees me = sees_of<PAGED>(a, sq, i);
+    const Sees me = sees_of<SRC>(a, sq, i);
     int hi_all, lo_all;
-    seen_by_all<PAGED>(a, sq, div_small(min(wr0, rows - 1), a.G, a.rcp_g), div_small(min(wr0 + 31, rows - 1), a.G, a.rcp_g), me,
+    seen_by_all<SRC>(a, sq, div_small(min(wr0, rows - 1), a.G, a.rcp_g), div_small(min(wr0 + 31, rows - 1), a.G, a.rcp_g), me,
                        hi_all, lo_all);
 
     const int64_t hoff = (int64_t)hk * (PAGED ? a.pg.hs : D);
@@ -237,7 +119,7 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
 
     const uint32_t kr_lds = lds_addr(ring) + kg * NS * TILE * 4, vr_lds = kr_lds + NS * TILE * 2;
     auto load_tile = [&](int x, int slot) {
-        load_tile_rows<RB, PAGED>(a, sq, tl, hoff, x, kr_lds + 2 * slot * TILE, vr_lds + 2 * slot * TILE, rb);
+        load_tile_rows<RB, SRC>(a, sq, tl, hoff, x, kr_lds + 2 * slot * TILE, vr_lds + 2 * slot * TILE, rb);
     };
 
     const int mine = x1 > x0 + kg ? (x1 - x0 - kg + KG - 1) / KG : 0;   // tiles of this group
@@ -285,7 +167,7 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
             }
             const bool whole = key0 + BT <= hi_all && (key0 >= lo_all || key0 + BT <= a.sinks) && !bad;
             if (!whole) {
-                const uint32_t m = seen_bits<BT, PAGED>(a, sq, tl, bad, i, me, x, 0) >> (8 * hf);
+                const uint32_t m = seen_bits<BT, SRC>(a, sq, tl, bad, i, me, x, 0) >> (8 * hf);
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                     if (!(m >> (16 * (e >> 3) + (e & 7)) & 1)) s[e] = -INFINITY;
@@ -430,7 +312,7 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
     int* again = reinterpret_cast<int*>(ring);
     again_rows<RB, KG>(again, rb, kg, (uint32_t)(bits | bits >> 32), [&](int q) __attribute__((always_inline)) {
         const int ri = __builtin_amdgcn_readlane(i, q), rhead = __builtin_amdgcn_readlane(head, q);
-        redo_row<BT, PAGED>(a, sq, tl, hk, ri, rhead, [&](float o0, float o1, float m, float rl) {
+        redo_row<BT, SRC>(a, sq, tl, hk, ri, rhead, [&](float o0, float o1, float m, float rl) {
             if (whole_block) put_row(a.out + (int64_t)(sq.t0 + ri) * a.o_rs + rhead * D, o0, o1, rl);
             else to.put_row2(split, 32 * rb + q, o0, o1, m, rl);
         });
@@ -442,9 +324,10 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
 // 4 products for a block of 16 keys in place of 8, eight waves of one tile each in place of four of two.
 // Lane 16 g + n: row n of each block; of a tile's scores the keys 4 g + r and 16 + 4 g + r (r < 4), in which order its products
 // take the keys; of the sums the dims 16 db + 4 g + r.
-template <int NB, int KG, bool PAGED>
+template <int NB, int KG, int SRC>
 __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnArgs a) {
     constexpr int BT = RANGE_TILE, TILE = BT * D, BR = 16 * NB;
+    constexpr bool PAGED = paged(SRC);
     typedef __attribute__((address_space(3))) i16x4_t lds_i16x4;
     constexpr int OWN_LDS = TILE * 2 * 2;   // bytes of LDS a wave: its tiles, then its sums
     static_assert(OWN_LDS >= NB * 8 * 1024, "a wave's sums in the place of its tiles");
@@ -466,11 +349,11 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
         const int j = BT * (split * a.per + tid / per_tile) + (tid % per_tile << a.pg.shift);
         if (j >> a.pg.shift < a.pg.table_pages) early = a.pg.table[(int64_t)b * a.pg.table_rs + (j >> a.pg.shift)];
     }
-    const Seq sq = seq_of<PAGED>(a, b);
+    const Seq sq = seq_of<SRC>(a, b);
     const int row0 = blk * BR, rows = max(sq.n, 0) * a.G;   // (at most 2^30: the host checks)
     if (row0 >= rows) return;
     const int i_first = div_small(row0, a.G, a.rcp_g), i_last = div_small(min(rows, row0 + BR) - 1, a.G, a.rcp_g);
-    TileList<BT, PAGED> tl;
+    TileList<BT, SRC> tl;
     tl.init(a, sq, i_first, i_last);
     tl.part(split, a.per);
     const int parts = min(a.nsplit, max(1, (tl.total + a.per - 1) / a.per));   // the sequence may be shorter than the longest
@@ -489,15 +372,15 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
         live[nb] = r < rows;
         ri[nb] = div_small(rr, a.G, a.rcp_g);
         head[nb] = hk * a.G + rr - ri[nb] * a.G;
-        me[nb] = sees_of<PAGED>(a, sq, ri[nb]);
+        me[nb] = sees_of<SRC>(a, sq, ri[nb]);
         const uint16_t* src = a.q + (int64_t)(sq.t0 + ri[nb]) * a.q_rs + head[nb] * D + 8 * g;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) qf[nb][ks] = *reinterpret_cast<const bf16x8*>(src + 32 * ks);
     }
     int hi_all, lo_all, lo_last;
-    seen_by_all<PAGED>(a, sq, i_first, i_last, me[0], hi_all, lo_all);
+    seen_by_all<SRC>(a, sq, i_first, i_last, me[0], hi_all, lo_all);
     if (NB > 1) {
-        seen_by_all<PAGED>(a, sq, i_first, i_last, me[NB - 1], hi_all, lo_last);
+        seen_by_all<SRC>(a, sq, i_first, i_last, me[NB - 1], hi_all, lo_last);
         lo_all = max(lo_all, lo_last);
     }
     const bool bad = tl.template stage<KG * 64>(a, b, staged, ahead, early);
@@ -550,7 +433,7 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
             for (int nb = 0; nb < NB; ++nb) {
                 f32x4 &s0 = s[nb][0], &s1 = s[nb][1];
                 if (!whole) {
-                    const uint32_t m = seen_bits<BT, PAGED>(a, sq, tl, bad, ri[nb], me[nb], x, 0) >> (4 * g);
+                    const uint32_t m = seen_bits<BT, SRC>(a, sq, tl, bad, ri[nb], me[nb], x, 0) >> (4 * g);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         if (!(m >> e & 1)) s0[e] = -INFINITY;
@@ -580,7 +463,7 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
         }
         if (t + 1 < mine) {   // the tile's place is free again once this wave's reads have returned
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            load_tile_rows<1, PAGED>(a, sq, tl, hoff, tile_of(t + 1), kr_lds, vr_lds, 0);
+            load_tile_rows<1, SRC>(a, sq, tl, hoff, tile_of(t + 1), kr_lds, vr_lds, 0);
         }
         if (t < 0) continue;
 #pragma unroll
@@ -667,34 +550,13 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
             i = __builtin_amdgcn_readlane(ri[NB - 1], q & 15);
             h = __builtin_amdgcn_readlane(head[NB - 1], q & 15);
         }
-        redo_row<BT, PAGED>(a, sq, tl, hk, i, h, [&](float o0, float o1, float m, float rl) {
+        redo_row<BT, SRC>(a, sq, tl, hk, i, h, [&](float o0, float o1, float m, float rl) {
             if (whole_block) put_row(a.out + (int64_t)(sq.t0 + i) * a.o_rs + h * D, o0, o1, rl);
             else to.put_row2(split, q, o0, o1, m, rl);
         });
     });
     if constexpr (NB == 1)
         if (!whole_block && a.merge_here) to.template merge_last<KG>(a, sq, hk, row0, rows, split, parts, again);
-}
-
-// The parts of the blocks that more than one workgroup had, a wave a row: where they are many, one workgroup a block would take
-// long (64 parts of 32 rows: ~60 us).
-template <int BR, bool PAGED>
-__global__ __launch_bounds__(256) void range_merge_kernel(RangeAttnArgs a) {
-    const int at = blockIdx.x / (BR / 4), q = blockIdx.x % (BR / 4) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int blk = div_small(at, a.HK, a.rcp_hk), hk = at - blk * a.HK, b = blockIdx.y;
-    const Seq sq = seq_of<PAGED>(a, b);
-    const int rows = max(sq.n, 0) * a.G, row0 = blk * BR;
-    if (row0 + q >= rows) return;
-    TileList<RANGE_TILE, PAGED> tl;
-    tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + BR) - 1, a.G, a.rcp_g));
-    const int parts = min(a.nsplit, (tl.total + a.per - 1) / a.per);
-    if (parts <= 1) return;   // (the attention wrote its rows)
-    const int i = div_small(row0 + q, a.G, a.rcp_g), head = hk * a.G + row0 + q - i * a.G;
-    const int64_t first = (((int64_t)b * a.nblk + blk) * a.HK + hk) * a.nsplit * BR + q;
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + first;
-    const float2* po = reinterpret_cast<const float2*>(a.part_o) + first * (D / 2) + lane;
-    merge_parts(parts, a.out + (int64_t)(sq.t0 + i) * a.o_rs + head * D, [&](int s) { return ml[s * BR]; },
-                [&](int s) { return po[(int64_t)s * BR * (D / 2)]; });
 }
 
 template <int BR>
@@ -708,18 +570,18 @@ hipError_t launch_blocks(const RangeAttnArgs& a, bool paged, int threads, void (
     hipLaunchKernelGGL(paged ? paged_kernel : rows_kernel, dim3((unsigned)blocks, seqs), dim3(threads), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1 || a.merge_here) return e;
-    if (paged) hipLaunchKernelGGL((range_merge_kernel<BR, true>), dim3((unsigned)merge, seqs), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((range_merge_kernel<BR, false>), dim3((unsigned)merge), dim3(256), 0, stream, a);
+    if (paged) hipLaunchKernelGGL((range_merge_kernel<BR, PAGES>), dim3((unsigned)merge, seqs), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((range_merge_kernel<BR, ROWS>), dim3((unsigned)merge), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int br, hipStream_t stream) {
-    if (br == 16) return launch_blocks<16>(a, paged, 512, range_step_kernel<1, 8, false>, range_step_kernel<1, 8, true>, stream);
-    if (br == 32) return launch_blocks<32>(a, paged, 512, range_step_kernel<2, 8, false>, range_step_kernel<2, 8, true>, stream);
-    if (br == 64) return launch_blocks<64>(a, paged, 256, range_attn_kernel<2, 2, 4, false>, range_attn_kernel<2, 2, 4, true>, stream);
-    return launch_blocks<128>(a, paged, 512, range_attn_kernel<4, 2, 4, false>, range_attn_kernel<4, 2, 4, true>, stream);
+    if (br == 16) return launch_blocks<16>(a, paged, 512, range_step_kernel<1, 8, ROWS>, range_step_kernel<1, 8, PAGES>, stream);
+    if (br == 32) return launch_blocks<32>(a, paged, 512, range_step_kernel<2, 8, ROWS>, range_step_kernel<2, 8, PAGES>, stream);
+    if (br == 64) return launch_blocks<64>(a, paged, 256, range_attn_kernel<2, 2, 4, ROWS>, range_attn_kernel<2, 2, 4, PAGES>, stream);
+    return launch_blocks<128>(a, paged, 512, range_attn_kernel<4, 2, 4, ROWS>, range_attn_kernel<4, 2, 4, PAGES>, stream);
 }
 
 }  // namespace lr

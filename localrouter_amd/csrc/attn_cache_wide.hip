@@ -63,8 +63,9 @@ __device__ __forceinline__ int seq_by_length(const RangeAttnArgs& a, int rank) {
 // without a full window they are the longest; otherwise the heads alternate. Pages: longest sequences first, the blocks of one
 // sequence and head next to each other, by_xcd on one XCD (in the order of
 // block_order.h). The first `whole` blocks (of an XCD, or of the launch) are not cut.
-template <int QW, bool PAGED>
+template <int QW, int SRC>
 __device__ __forceinline__ bool block_of(const RangeAttnArgs& a, int id, int& b, int& hk, int& blk, int& split, int& cut) {
+    constexpr bool PAGED = paged(SRC);
     const int xcd = a.by_xcd ? id & 7 : 0;
     int idx = a.by_xcd ? id >> 3 : id;
     if (a.by_xcd && a.nsplit == 1) idx = start_order(idx, a.local, 8 / QW);
@@ -111,7 +112,7 @@ struct Pieces {
         const int lane = threadIdx.x & 63;
         P = a.B * a.HK >> 3;
         const int pair = min(lane, P - 1) * 8 + xcd;
-        const Seq sq = seq_of<true>(a, div_small(pair, a.HK, a.rcp_hk));
+        const Seq sq = seq_of<PAGES>(a, div_small(pair, a.HK, a.rcp_hk));
         const int rows = max(sq.n, 0) * a.G;
         tiles = lane < P && rows > 0 ? max(1, (sq.end + IMG_TILE_KEYS - 1) / IMG_TILE_KEYS) : 0;
         end = tiles;
@@ -149,9 +150,10 @@ struct Pieces {
     }
 };
 
-template <int QW, bool PAGED>
+template <int QW, int SRC>
 __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu(2, 2))) void range_wide_kernel(RangeAttnArgs a) {
     constexpr int KBM = 32 * QW;                        // rows per block
+    constexpr bool PAGED = paged(SRC);
     // steps of refills in flight beside the current one's. (8 waves have the LDS for 2: pages come from HBM, ~2 us away under load: 16
     // trees of up to 64 tokens over up to 30,000 keys 860 -> 841 us. Rows come from the L2s: 16,384 tokens of video 1,171 us with 2,
     // 1,164 with 0.)
@@ -187,17 +189,17 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         split = 0;
         const bool all = px1 - px0 == __builtin_amdgcn_readlane(pc.tiles, j);
         cut = all ? -1 : (xcd * (pc.P + a.teams) + at) * a.nblk + blk;
-    } else if (!block_of<QW, PAGED>(a, blockIdx.x, b, hk, blk, split, cut)) {
+    } else if (!block_of<QW, SRC>(a, blockIdx.x, b, hk, blk, split, cut)) {
         return;
     }
     b = __builtin_amdgcn_readfirstlane(b);
     hk = __builtin_amdgcn_readfirstlane(hk);
     blk = __builtin_amdgcn_readfirstlane(blk);
-    const Seq sq = seq_of<PAGED>(a, b);
+    const Seq sq = seq_of<SRC>(a, b);
     const int row0 = blk * KBM;
     const int rows = max(sq.n, 0) * a.G;   // (at most 2^30: the host checks)
     if (row0 >= rows) return;
-    TileList<BT, PAGED> tl;
+    TileList<BT, SRC> tl;
     tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + KBM) - 1, a.G, a.rcp_g));
     if (PAGED && a.teams) {
         tl.x0 = px0;
@@ -210,7 +212,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     const int r = row0 + 32 * wv + n, rr = min(r, rows - 1);
     const bool live = r < rows;
     const int i = div_small(rr, a.G, a.rcp_g), head = hk * a.G + rr - i * a.G;
-    const Sees me = sees_of<PAGED>(a, sq, i);
+    const Sees me = sees_of<SRC>(a, sq, i);
     const int64_t part = (int64_t)cut * a.nsplit + split;   // its slot among the parts (merge_rows)
     if (x0 >= x1) {   // nothing to see in this part
         if (live) {
@@ -345,7 +347,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         return unset_any || !(h < free_s || (h >= free_lo && h < free_hi));
     };
     auto mask_half = [&](f32x16& sb, int x, int half) __attribute__((always_inline)) {
-        const uint32_t m = seen_bits<BT, PAGED>(a, sq, tl, bad, i, me, x, 32 * half) >> (8 * hf);
+        const uint32_t m = seen_bits<BT, SRC>(a, sq, tl, bad, i, me, x, 32 * half) >> (8 * hf);
 #pragma unroll
         for (int q = 0; q < 16; ++q)
             if (!(m >> (16 * (q >> 3) + (q & 7)) & 1)) sb[q] = -INFINITY;
@@ -566,7 +568,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         const int q = __builtin_ctzll(again);
         again &= again - 1;
         const int ri = __builtin_amdgcn_readlane(i, q), rhead = __builtin_amdgcn_readlane(head, q);
-        redo_row<BT, PAGED>(a, sq, tl, hk, ri, rhead, [&](float o0, float o1, float m, float rl) {
+        redo_row<BT, SRC>(a, sq, tl, hk, ri, rhead, [&](float o0, float o1, float m, float rl) {
             if (cut >= 0) {
                 float* po = a.part_o + (part * QW + wv) * 4096 + 256 * (lane >> 2) + 4 * (q + 32 * (lane >> 1 & 1)) + 2 * (lane & 1);
                 *reinterpret_cast<float2*>(po) = float2{o0, o1};
@@ -631,15 +633,15 @@ __device__ __forceinline__ void merge_rows(const RangeAttnArgs& a, const Seq& sq
 }
 
 // The parts of the blocks that were cut: workgroup (cut block, 32 rows).
-template <int QW, bool PAGED>
+template <int QW, int SRC>
 __global__ __launch_bounds__(256) void range_wide_merge_kernel(RangeAttnArgs a) {
     const int c = blockIdx.x / QW, w = blockIdx.x % QW;
     const int of = a.local - a.whole;   // cut blocks an XCD
     const int xcd = a.by_xcd ? c / of : 0, first = a.whole + (c - xcd * of) * a.nsplit;   // the block's first workgroup
     int b, hk, blk, split, cut;
-    if (!block_of<QW, PAGED>(a, a.by_xcd ? 8 * first + xcd : first, b, hk, blk, split, cut)) return;
+    if (!block_of<QW, SRC>(a, a.by_xcd ? 8 * first + xcd : first, b, hk, blk, split, cut)) return;
     b = __builtin_amdgcn_readfirstlane(b);
-    const Seq sq = seq_of<PAGED>(a, b);
+    const Seq sq = seq_of<SRC>(a, b);
     merge_rows<QW>(a, sq, hk, blk, w, a.nsplit, [&](int x) { return (int64_t)cut * a.nsplit + x; });
 }
 
@@ -653,18 +655,18 @@ __global__ __launch_bounds__(256) void range_pieces_merge_kernel(RangeAttnArgs a
     const int parts = 1 + (max(e - 1, 0) / pc.Q - t0);
     if (s == e || parts <= 1) return;   // (the attention wrote its rows)
     const int pair = 8 * j + xcd, b = div_small(pair, a.HK, a.rcp_hk), hk = pair - b * a.HK;
-    const Seq sq = seq_of<true>(a, b);
+    const Seq sq = seq_of<PAGES>(a, b);
     merge_rows<QW>(a, sq, hk, blk, at % QW, parts, [&](int x) {
         return (int64_t)(xcd * (pc.P + a.teams) + (x == 0 ? j : pc.P + t0 + x - 1)) * a.nblk + blk;
     });
 }
 
-template <int QW, bool PAGED>
+template <int QW, int SRC>
 hipError_t launch_waves(const RangeAttnArgs& a, hipStream_t stream) {
-    if constexpr (PAGED)
+    if constexpr (paged(SRC))
         if (a.teams) {
             const int64_t pairs = (int64_t)a.B * a.HK, blocks = (pairs + 8 * a.teams) * a.nblk, merge = pairs * a.nblk * QW;
-            hipLaunchKernelGGL((range_wide_kernel<QW, PAGED>), dim3((unsigned)blocks), dim3(64 * QW), 0, stream, a);
+            hipLaunchKernelGGL((range_wide_kernel<QW, SRC>), dim3((unsigned)blocks), dim3(64 * QW), 0, stream, a);
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
             hipLaunchKernelGGL(range_pieces_merge_kernel<QW>, dim3((unsigned)merge), dim3(256), 0, stream, a);
@@ -674,18 +676,18 @@ hipError_t launch_waves(const RangeAttnArgs& a, hipStream_t stream) {
     const int64_t of = a.nsplit > 1 ? a.local - a.whole : 0;   // cut blocks
     const int64_t blocks = xcds * (a.local + of * (a.nsplit - 1)), merge = xcds * of * QW;
     if (blocks > RANGE_MAX_BLOCKS || merge > 2 * RANGE_MAX_BLOCKS) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((range_wide_kernel<QW, PAGED>), dim3((unsigned)blocks), dim3(64 * QW), 0, stream, a);
+    hipLaunchKernelGGL((range_wide_kernel<QW, SRC>), dim3((unsigned)blocks), dim3(64 * QW), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || of == 0) return e;
-    hipLaunchKernelGGL((range_wide_merge_kernel<QW, PAGED>), dim3((unsigned)merge), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((range_wide_merge_kernel<QW, SRC>), dim3((unsigned)merge), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, int waves, hipStream_t stream) {
-    if (waves == 8) return paged ? launch_waves<8, true>(a, stream) : launch_waves<8, false>(a, stream);
-    return paged ? launch_waves<4, true>(a, stream) : launch_waves<4, false>(a, stream);
+    if (waves == 8) return paged ? launch_waves<8, PAGES>(a, stream) : launch_waves<8, ROWS>(a, stream);
+    return paged ? launch_waves<4, PAGES>(a, stream) : launch_waves<4, ROWS>(a, stream);
 }
 
 }  // namespace lr

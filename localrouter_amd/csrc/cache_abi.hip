@@ -2,10 +2,12 @@
 // include/lr_attn.h): argument validation, then launches on the caller's stream. Nothing here synchronises, allocates or keeps
 // state.
 #include <limits.h>
+#include <stdlib.h>
 
 #include <algorithm>
 
 #include "../../include/lr_cache.h"
+#include "../../include/lr_cache8.h"
 #include "abi_checks.h"
 #include "lr_cache_kernels.h"
 
@@ -38,12 +40,14 @@ bool rows_meet(int64_t d, const Level* levels, int n, int& left) {
     return false;
 }
 
-// A pool of pages: aligned bases, strides that hold what they step over, no row of keys and values, or of two layers, the same.
+// A pool of pages of elements of `es` bytes: aligned bases, strides that hold what they step over, no row of keys and values, or of
+// two layers, the same.
 bool pool_ok(const void* k, const void* v, int64_t page, int64_t row, int64_t head, int n_pages, int page_size, int HK,
-             int layers = 1, int64_t layer = 0) {
+             int layers = 1, int64_t layer = 0, int es = 2) {
+    const int unit = 16 / es;
     if (!k || !v || !aligned(k, 16) || !aligned(v, 16) || n_pages < 1 || HK < 1 || !page_size_ok(page_size)) return false;
-    if (page % 8 || row % 8 || head % 8 || page < lr::D || row < lr::D || head < lr::D) return false;
-    if (layers < 1 || layers > 65535 || layer % 8 || (layers > 1 && layer < lr::D)) return false;
+    if (page % unit || row % unit || head % unit || page < lr::D || row < lr::D || head < lr::D) return false;
+    if (layers < 1 || layers > 65535 || layer % unit || (layers > 1 && layer < lr::D)) return false;
     auto far = [](int64_t stride, int64_t count) { return stride > ((int64_t)1 << 48) / count; };   // (no address space holds it)
     if (far(page, n_pages) || far(row, page_size) || far(head, HK) || far(layer, layers)) return false;
     // rows of a page token by token or head by head, pages apart from each other
@@ -54,7 +58,7 @@ bool pool_ok(const void* k, const void* v, int64_t page, int64_t row, int64_t he
                        {layer, 1 - layers, layers - 1}};
     std::sort(levels, levels + 4, [](const Level& x, const Level& y) { return x.stride > y.stride; });
     int left = 4096;   // (nested layouts: at most 16)
-    if (rows_meet((reinterpret_cast<intptr_t>(v) - reinterpret_cast<intptr_t>(k)) / 2, levels, 4, left)) return false;
+    if (rows_meet((reinterpret_cast<intptr_t>(v) - reinterpret_cast<intptr_t>(k)) / es, levels, 4, left)) return false;
     if (layers == 1) return true;
     for (Level& l : levels)
         if (l.stride == layer && l.hi == layers - 1 && l.lo == 1 - layers) {   // (another level of the same numbers is as good)
@@ -78,10 +82,28 @@ bool packed_rows_meet(const void* q, int64_t q_rs, int hq, const void* x, int64_
     return rows_meet(d, levels, 3, left);
 }
 Span pool_span(const void* p, int layers, int64_t layer, int64_t page, int64_t row, int64_t head, int n_pages, int page_size,
-               int HK) {
+               int HK, int es = 2) {
     const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
-    return Span{lo, lo + 2 * (uintptr_t)((layers - 1) * layer + (n_pages - 1) * page + (page_size - 1) * row +
+    return Span{lo, lo + es * (uintptr_t)((layers - 1) * layer + (n_pages - 1) * page + (page_size - 1) * row +
                                          (HK - 1) * head + lr::D)};
+}
+// The scales of a pool in 8 bits: pages of page_size / GROUP8 * HK bytes, `page` apart, layers `layer` apart; those of keys and of
+// values in memory of their own, or each page's next to each other.
+bool page8_ok(int page_size, int64_t row) { return page_size >= lr::GROUP8 && row < lr::RANGE_WIDE_MAX_RS; }
+int64_t scales_bytes(int page_size, int HK) { return (int64_t)(page_size / lr::GROUP8) * HK; }
+Span scales_span(const void* p, int layers, int64_t layer, int64_t page, int n_pages, int page_size, int HK) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+    return Span{lo, lo + (uintptr_t)((layers - 1) * layer + (n_pages - 1) * page + scales_bytes(page_size, HK))};
+}
+bool scales_ok(const void* k, const void* v, int64_t page, int n_pages, int page_size, int HK, int layers = 1, int64_t layer = 0) {
+    const int64_t bytes = scales_bytes(page_size, HK);
+    if (!k || !v || page < bytes || page > ((int64_t)1 << 48) / n_pages || (layers > 1 && layer > ((int64_t)1 << 48) / layers)) return false;
+    // layers one after the other, or side by side inside what a page steps over
+    if (layers > 1 && layer < (n_pages - 1) * page + bytes && (layer < bytes || (layers - 1) * layer + bytes > page)) return false;
+    const Span a = scales_span(k, layers, layer, page, n_pages, page_size, HK), b = scales_span(v, layers, layer, page, n_pages, page_size, HK);
+    if (!overlap(a, b)) return true;
+    const int64_t d = std::llabs(reinterpret_cast<intptr_t>(v) - reinterpret_cast<intptr_t>(k)), step = layers > 1 ? std::min(page, layer) : page;
+    return d >= bytes && d + bytes <= step;
 }
 bool table_args_ok(const int* table, int64_t stride, int pages, int page_size, const int* starts, int B) {
     return table && aligned(table, 4) && starts && aligned(starts, 4) && B >= 1 && pages >= 1 && stride >= pages &&
@@ -130,8 +152,8 @@ bool few_rows(int64_t rows, int64_t pairs, int64_t tiles) {
 // 16 15.9, 32 18.2). In the same launch / by a second: 24 parts of 4 rows 13.1 / 14.5, 63 of 8 15.4 / 17.5, 32 of 16 20.9 / 22.1, 8 of
 // 20 12.5 / 11.8, 8 of 32 13.4 / 11.9, 2 of 64 19.1 / 16.0.
 // The other kernel: parts of 8 tiles at least, merged by a second launch.
-Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
-    const int64_t br = rows <= 16 ? 16 : few_rows(rows, pairs, tiles) ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
+Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool few = false) {
+    const int64_t br = rows <= 16 ? 16 : few || few_rows(rows, pairs, tiles) ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
     const int64_t staged = page_size ? lr::RANGE_STAGED / std::max(1, lr::RANGE_TILE / page_size) : INT_MAX;
     int64_t ns = std::max<int64_t>(1, std::min(256 / base, (tiles + 4) / 8));
     if (br <= 32) {
@@ -239,6 +261,12 @@ Cut cache_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, i
     }
     return cut_small(rows, pairs, tiles, page_size);
 }
+// Pages in 8 bits (attn_cache8.hip): blocks of 16 or 32 rows.
+Cut cache8_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks) {
+    const int64_t rows = (int64_t)max_rows * (H / HK), pairs = (int64_t)B * HK;
+    const int64_t span = window ? (int64_t)window + max_rows + 1 : max_keys;
+    return cut_small(rows, pairs, tiles_of(max_keys, span, sinks, lr::RANGE_TILE), page_size, true);
+}
 // Whether the grid of attn_cache_wide.hip's launch holds its workgroups (attn_cache.hip's counts its own, launch_blocks).
 bool launch_fits(const Cut& c) {
     return !c.wide || (c.by_xcd ? 8 : 1) * (c.whole + (c.local - c.whole) * c.nsplit) <= lr::RANGE_MAX_BLOCKS;
@@ -273,6 +301,96 @@ bool cache_sizes_ok(int B, int T, int max_rows, int max_keys, int H, int HK, int
     return B >= 1 && B <= 65535 && T >= 1 && T <= MAX_POS && max_rows >= 1 && max_rows <= MAX_POS && max_keys >= 1 &&
            max_keys <= MAX_POS && H >= 1 && HK >= 1 && H % HK == 0 && page_size_ok(page_size) && window >= 0 && sinks >= 0 &&
            (int64_t)max_rows * (H / HK) <= MAX_POS;
+}
+
+// What both attentions over pages check, and their arguments but for the cut; es: bytes of a page's element. spans: the rows of out and
+// q, and the pools.
+bool attention_args(lr::RangeAttnArgs& a, Span (&spans)[4], int es, const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride,
+                    const void* k_pages, const void* v_pages, int64_t page_stride, int64_t row_stride, int64_t head_stride, int n_pages,
+                    int page_size, const int* page_table, int64_t table_stride, int table_pages, const int* starts, const int* lens, int B,
+                    int T, int max_rows, int max_keys, int H, int HK, const uint64_t* tree, int words, int window, int sinks, float scale) {
+    if (!cache_sizes_ok(B, T, max_rows, max_keys, H, HK, page_size, window, sinks) || !scale_ok(scale)) return false;
+    if (!rows_ok(q, q_row_stride, H) || !rows_ok(out, out_row_stride, H)) return false;
+    if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK, 1, 0, es)) return false;
+    if (!table_args_ok(page_table, table_stride, table_pages, page_size, starts, B) || !lens || !aligned(lens, 4))
+        return false;
+    if (tree && (words < 1 || words > 64 || !aligned(tree, 8))) return false;
+    const Span so = rows_span(out, T, out_row_stride, H), sq = rows_span(q, T, q_row_stride, H),
+               sk = pool_span(k_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK, es),
+               sv = pool_span(v_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK, es);
+    if (overlap(so, sq) || overlap(so, sk) || overlap(so, sv)) return false;
+    spans[0] = so; spans[1] = sq; spans[2] = sk; spans[3] = sv;
+    a.q = static_cast<const uint16_t*>(q);
+    a.k = static_cast<const uint16_t*>(k_pages);
+    a.v = static_cast<const uint16_t*>(v_pages);
+    a.out = static_cast<uint16_t*>(out);
+    a.q_rs = q_row_stride; a.o_rs = out_row_stride;
+    a.H = H; a.HK = HK; a.G = H / HK;
+    a.c = scale * 1.4426950408889634f;
+    a.pg = page_args(page_stride, row_stride, head_stride, n_pages, page_size, page_table, table_stride, table_pages);
+    a.starts = starts; a.lens = lens; a.tree = tree; a.words = tree ? words : 0;
+    a.B = B; a.T = T; a.max_rows = max_rows; a.max_keys = max_keys;
+    a.window = std::min(window, MAX_POS); a.sinks = window ? std::min(sinks, MAX_POS) : 0;
+    return true;
+}
+// The workspace of a call that is cut as c, apart from everything it reads and writes.
+bool workspace_ok(const Cut& c, void* workspace, size_t workspace_bytes, const Span* spans, int n) {
+    const size_t need = part_bytes(c);
+    if (!need) return true;
+    if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return false;
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(workspace);
+    for (int i = 0; i < n; ++i)
+        if (overlap(Span{lo, lo + need}, spans[i])) return false;
+    return true;
+}
+
+// What both appends check, and their arguments; es: bytes of a page's element.
+bool append_args(lr::CacheAppendArgs& a, int es, const void* q, const void* k, const void* v, int64_t q_row_stride, int64_t k_row_stride,
+                 int64_t v_row_stride, void* q_out, int64_t q_out_row_stride, void* k_pages, void* v_pages, int64_t page_stride,
+                 int64_t row_stride, int64_t head_stride, int n_pages, int page_size, const int* page_table, int64_t table_stride,
+                 int table_pages, const int* starts, const int* lens, const int* positions, int B, int T, int H, int HK,
+                 const float* q_norm_w, const float* k_norm_w, int table_kind, const void* table_a, const void* table_b,
+                 int64_t table_row_stride, int table_rows, int pairing, int rot_dim, float eps) {
+    const int rot = rot_dim == 0 ? lr::D : rot_dim;
+    if (T < 1 || T > MAX_POS || HK < 1 || (q && H < 1) || !(eps >= 0.0f) || !isfinite(eps)) return false;
+    if (!rows_ok(k, k_row_stride, HK) || !rows_ok(v, v_row_stride, HK)) return false;
+    if (q && (!rows_ok(q, q_row_stride, H) || !rows_ok(q_out, q_out_row_stride, H))) return false;
+    if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK, 1, 0, es)) return false;
+    if (!table_args_ok(page_table, table_stride, table_pages, page_size, starts, B) || !lens || !aligned(lens, 4) ||
+        (positions && !aligned(positions, 4)))
+        return false;
+    if ((q_norm_w && !aligned(q_norm_w, 16)) || (k_norm_w && !aligned(k_norm_w, 16))) return false;
+    if (!table_ok(table_kind, table_a, table_b, table_row_stride, rot, pairing, 16)) return false;
+    if (table_kind != LR_TABLE_NONE && table_rows < 1) return false;
+    const Span pk = pool_span(k_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK, es),
+               pv = pool_span(v_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK, es),
+               sk = rows_span(k, T, k_row_stride, HK), sv = rows_span(v, T, v_row_stride, HK);
+    if (overlap(pk, sk) || overlap(pk, sv) || overlap(pv, sk) || overlap(pv, sv)) return false;
+    if (q) {
+        const Span sq = rows_span(q, T, q_row_stride, H), so = rows_span(q_out, T, q_out_row_stride, H);
+        if (overlap(pk, sq) || overlap(pv, sq) || overlap(pk, so) || overlap(pv, so)) return false;
+        if (!(q_out == q && q_out_row_stride == q_row_stride) && overlap(sq, so)) return false;
+        // (in place on the queries of a packed projection, whose keys and values have columns of their own)
+        if (q_out == q && q_out_row_stride == q_row_stride
+                ? packed_rows_meet(q, q_row_stride, H, k, k_row_stride, HK, T) || packed_rows_meet(q, q_row_stride, H, v, v_row_stride, HK, T)
+                : overlap(so, sk) || overlap(so, sv))
+            return false;
+    }
+    a.q = static_cast<const uint16_t*>(q);
+    a.k = static_cast<const uint16_t*>(k);
+    a.v = static_cast<const uint16_t*>(v);
+    a.q_out = static_cast<uint16_t*>(q_out);
+    a.kp = static_cast<uint16_t*>(k_pages);
+    a.vp = static_cast<uint16_t*>(v_pages);
+    a.q_rs = q_row_stride; a.k_rs = k_row_stride; a.v_rs = v_row_stride; a.qo_rs = q_out_row_stride;
+    a.pg = page_args(page_stride, row_stride, head_stride, n_pages, page_size, page_table, table_stride, table_pages);
+    a.starts = starts; a.lens = lens; a.pos = positions;
+    a.B = B; a.T = T; a.H = q ? H : 0; a.HK = HK;
+    a.qw = q_norm_w; a.kw = k_norm_w;
+    a.table_kind = table_kind; a.pairing = pairing; a.rot = rot; a.tab_rows = table_rows;
+    a.tab_vec = tab_vec(table_kind, table_a, table_b, table_row_stride);
+    a.ta = table_a; a.tb = table_b; a.tab_stride = table_row_stride; a.eps = eps;
+    return true;
 }
 
 }  // namespace
@@ -335,40 +453,50 @@ int lr_cache_attention_bf16(const void* q, int64_t q_row_stride, void* out, int6
                             const int* lens, int B, int T, int max_rows, int max_keys, int H, int HK, const uint64_t* tree,
                             int words, int window, int sinks, float scale, void* workspace, size_t workspace_bytes,
                             lr_stream_t stream) {
-    if (!cache_sizes_ok(B, T, max_rows, max_keys, H, HK, page_size, window, sinks) || !scale_ok(scale)) return ERR_ARGS;
-    if (!rows_ok(q, q_row_stride, H) || !rows_ok(out, out_row_stride, H)) return ERR_ARGS;
-    if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK)) return ERR_ARGS;
-    if (!table_args_ok(page_table, table_stride, table_pages, page_size, starts, B) || !lens || !aligned(lens, 4))
-        return ERR_ARGS;
-    if (tree && (words < 1 || words > 64 || !aligned(tree, 8))) return ERR_ARGS;
-    const Span so = rows_span(out, T, out_row_stride, H), sq = rows_span(q, T, q_row_stride, H),
-               sk = pool_span(k_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK),
-               sv = pool_span(v_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK);
-    if (overlap(so, sq) || overlap(so, sk) || overlap(so, sv)) return ERR_ARGS;
     lr::RangeAttnArgs a{};
-    const bool narrow = row_stride < lr::RANGE_WIDE_MAX_RS && (page_size > lr::RANGE_WIDE_MIN_PAGE || sk.hi - sk.lo < (1ull << 32));
+    Span spans[4];
+    if (!attention_args(a, spans, 2, q, q_row_stride, out, out_row_stride, k_pages, v_pages, page_stride, row_stride, head_stride, n_pages,
+                        page_size, page_table, table_stride, table_pages, starts, lens, B, T, max_rows, max_keys, H, HK, tree, words,
+                        window, sinks, scale))
+        return ERR_ARGS;
+    const bool narrow =
+        row_stride < lr::RANGE_WIDE_MAX_RS && (page_size > lr::RANGE_WIDE_MIN_PAGE || spans[2].hi - spans[2].lo < (1ull << 32));
     const Cut cut = cache_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks, narrow);
-    if (!launch_fits(cut)) return ERR_ARGS;
-    const size_t need = part_bytes(cut);
-    if (need) {
-        if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return ERR_ARGS;
-        const uintptr_t lo = reinterpret_cast<uintptr_t>(workspace);
-        const Span w{lo, lo + need};
-        if (overlap(w, so) || overlap(w, sq) || overlap(w, sk) || overlap(w, sv)) return ERR_ARGS;
-    }
-    a.q = static_cast<const uint16_t*>(q);
-    a.k = static_cast<const uint16_t*>(k_pages);
-    a.v = static_cast<const uint16_t*>(v_pages);
-    a.out = static_cast<uint16_t*>(out);
-    a.q_rs = q_row_stride; a.o_rs = out_row_stride;
-    a.H = H; a.HK = HK; a.G = H / HK;
-    a.c = scale * 1.4426950408889634f;
-    a.pg = page_args(page_stride, row_stride, head_stride, n_pages, page_size, page_table, table_stride, table_pages);
+    if (!launch_fits(cut) || !workspace_ok(cut, workspace, workspace_bytes, spans, 4)) return ERR_ARGS;
     set_cut(a, workspace, cut);
-    a.starts = starts; a.lens = lens; a.tree = tree; a.words = tree ? words : 0;
-    a.B = B; a.T = T; a.max_rows = max_rows; a.max_keys = max_keys;
-    a.window = std::min(window, MAX_POS); a.sinks = window ? std::min(sinks, MAX_POS) : 0;
     return launch(a, true, cut, stream);
+}
+
+size_t lr_cache_attention_f8_ws_bytes(int B, int T, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks) {
+    if (!cache_sizes_ok(B, T, max_rows, max_keys, H, HK, page_size, window, sinks) || page_size < lr::GROUP8) return 0;
+    return part_bytes(cache8_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks));
+}
+
+int lr_cache_attention_f8(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride, const void* k_pages, const void* v_pages,
+                          int64_t page_stride, int64_t row_stride, int64_t head_stride, int n_pages, int page_size, const void* k_scales,
+                          const void* v_scales, int64_t scale_page_stride, const int* page_table, int64_t table_stride, int table_pages,
+                          const int* starts, const int* lens, int B, int T, int max_rows, int max_keys, int H, int HK,
+                          const uint64_t* tree, int words, int window, int sinks, float scale, void* workspace, size_t workspace_bytes,
+                          lr_stream_t stream) {
+    lr::RangeAttnArgs a{};
+    Span spans[6];
+    Span(&four)[4] = reinterpret_cast<Span(&)[4]>(spans);
+    if (!attention_args(a, four, 1, q, q_row_stride, out, out_row_stride, k_pages, v_pages, page_stride, row_stride, head_stride, n_pages,
+                        page_size, page_table, table_stride, table_pages, starts, lens, B, T, max_rows, max_keys, H, HK, tree, words,
+                        window, sinks, scale) ||
+        !page8_ok(page_size, row_stride) || !scales_ok(k_scales, v_scales, scale_page_stride, n_pages, page_size, HK))
+        return ERR_ARGS;
+    spans[4] = scales_span(k_scales, 1, 0, scale_page_stride, n_pages, page_size, HK);
+    spans[5] = scales_span(v_scales, 1, 0, scale_page_stride, n_pages, page_size, HK);
+    for (int i : {0, 2, 3})
+        if (overlap(spans[i], spans[4]) || overlap(spans[i], spans[5])) return ERR_ARGS;
+    const Cut cut = cache8_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks);
+    if (!launch_fits(cut) || !workspace_ok(cut, workspace, workspace_bytes, spans, 6)) return ERR_ARGS;
+    set_cut(a, workspace, cut);
+    a.k_sc = static_cast<const uint8_t*>(k_scales);
+    a.v_sc = static_cast<const uint8_t*>(v_scales);
+    a.sc_ps = scale_page_stride;
+    return (int)lr::launch_range8(a, cut.br, reinterpret_cast<hipStream_t>(stream));
 }
 
 int lr_cache_append_bf16(const void* q, const void* k, const void* v, int64_t q_row_stride, int64_t k_row_stride,
@@ -378,47 +506,40 @@ int lr_cache_append_bf16(const void* q, const void* k, const void* v, int64_t q_
                          const int* positions, int B, int T, int H, int HK, const float* q_norm_w, const float* k_norm_w,
                          int table_kind, const void* table_a, const void* table_b, int64_t table_row_stride, int table_rows,
                          int pairing, int rot_dim, float eps, lr_stream_t stream) {
-    const int rot = rot_dim == 0 ? lr::D : rot_dim;
-    if (T < 1 || T > MAX_POS || HK < 1 || (q && H < 1) || !(eps >= 0.0f) || !isfinite(eps)) return ERR_ARGS;
-    if (!rows_ok(k, k_row_stride, HK) || !rows_ok(v, v_row_stride, HK)) return ERR_ARGS;
-    if (q && (!rows_ok(q, q_row_stride, H) || !rows_ok(q_out, q_out_row_stride, H))) return ERR_ARGS;
-    if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK)) return ERR_ARGS;
-    if (!table_args_ok(page_table, table_stride, table_pages, page_size, starts, B) || !lens || !aligned(lens, 4) ||
-        (positions && !aligned(positions, 4)))
+    lr::CacheAppendArgs a{};
+    if (!append_args(a, 2, q, k, v, q_row_stride, k_row_stride, v_row_stride, q_out, q_out_row_stride, k_pages, v_pages, page_stride,
+                     row_stride, head_stride, n_pages, page_size, page_table, table_stride, table_pages, starts, lens, positions, B, T, H,
+                     HK, q_norm_w, k_norm_w, table_kind, table_a, table_b, table_row_stride, table_rows, pairing, rot_dim, eps))
         return ERR_ARGS;
-    if ((q_norm_w && !aligned(q_norm_w, 16)) || (k_norm_w && !aligned(k_norm_w, 16))) return ERR_ARGS;
-    if (!table_ok(table_kind, table_a, table_b, table_row_stride, rot, pairing, 16)) return ERR_ARGS;
-    if (table_kind != LR_TABLE_NONE && table_rows < 1) return ERR_ARGS;
-    const Span pk = pool_span(k_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK),
-               pv = pool_span(v_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK),
-               sk = rows_span(k, T, k_row_stride, HK), sv = rows_span(v, T, v_row_stride, HK);
-    if (overlap(pk, sk) || overlap(pk, sv) || overlap(pv, sk) || overlap(pv, sv)) return ERR_ARGS;
-    if (q) {
-        const Span sq = rows_span(q, T, q_row_stride, H), so = rows_span(q_out, T, q_out_row_stride, H);
-        if (overlap(pk, sq) || overlap(pv, sq) || overlap(pk, so) || overlap(pv, so)) return ERR_ARGS;
-        if (!(q_out == q && q_out_row_stride == q_row_stride) && overlap(sq, so)) return ERR_ARGS;
-        // (in place on the queries of a packed projection, whose keys and values have columns of their own)
-        if (q_out == q && q_out_row_stride == q_row_stride
-                ? packed_rows_meet(q, q_row_stride, H, k, k_row_stride, HK, T) || packed_rows_meet(q, q_row_stride, H, v, v_row_stride, HK, T)
-                : overlap(so, sk) || overlap(so, sv))
+    return (int)lr::launch_cache_append(a, reinterpret_cast<hipStream_t>(stream));
+}
+
+int lr_cache_append_f8(const void* q, const void* k, const void* v, int64_t q_row_stride, int64_t k_row_stride, int64_t v_row_stride,
+                       void* q_out, int64_t q_out_row_stride, void* k_pages, void* v_pages, int64_t page_stride, int64_t row_stride,
+                       int64_t head_stride, int n_pages, int page_size, void* k_scales, void* v_scales, int64_t scale_page_stride,
+                       const int* page_table, int64_t table_stride, int table_pages, const int* starts, const int* lens,
+                       const int* positions, int B, int T, int H, int HK, const float* q_norm_w, const float* k_norm_w, int table_kind,
+                       const void* table_a, const void* table_b, int64_t table_row_stride, int table_rows, int pairing, int rot_dim,
+                       float eps, lr_stream_t stream) {
+    lr::CacheAppend8Args a{};
+    if (!append_args(a.at, 1, q, k, v, q_row_stride, k_row_stride, v_row_stride, q_out, q_out_row_stride, k_pages, v_pages, page_stride,
+                     row_stride, head_stride, n_pages, page_size, page_table, table_stride, table_pages, starts, lens, positions, B, T, H,
+                     HK, q_norm_w, k_norm_w, table_kind, table_a, table_b, table_row_stride, table_rows, pairing, rot_dim, eps) ||
+        B > 65535 || !page8_ok(page_size, row_stride) || !scales_ok(k_scales, v_scales, scale_page_stride, n_pages, page_size, HK))
+        return ERR_ARGS;
+    const Span pools[2] = {pool_span(k_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK, 1),
+                           pool_span(v_pages, 1, 0, page_stride, row_stride, head_stride, n_pages, page_size, HK, 1)};
+    for (void* p : {k_scales, v_scales}) {
+        const Span sc = scales_span(p, 1, 0, scale_page_stride, n_pages, page_size, HK);
+        if (overlap(sc, pools[0]) || overlap(sc, pools[1]) || overlap(sc, rows_span(k, T, k_row_stride, HK)) ||
+            overlap(sc, rows_span(v, T, v_row_stride, HK)) ||
+            (q && (overlap(sc, rows_span(q, T, q_row_stride, H)) || overlap(sc, rows_span(q_out, T, q_out_row_stride, H)))))
             return ERR_ARGS;
     }
-    lr::CacheAppendArgs a{};
-    a.q = static_cast<const uint16_t*>(q);
-    a.k = static_cast<const uint16_t*>(k);
-    a.v = static_cast<const uint16_t*>(v);
-    a.q_out = static_cast<uint16_t*>(q_out);
-    a.kp = static_cast<uint16_t*>(k_pages);
-    a.vp = static_cast<uint16_t*>(v_pages);
-    a.q_rs = q_row_stride; a.k_rs = k_row_stride; a.v_rs = v_row_stride; a.qo_rs = q_out_row_stride;
-    a.pg = page_args(page_stride, row_stride, head_stride, n_pages, page_size, page_table, table_stride, table_pages);
-    a.starts = starts; a.lens = lens; a.pos = positions;
-    a.B = B; a.T = T; a.H = q ? H : 0; a.HK = HK;
-    a.qw = q_norm_w; a.kw = k_norm_w;
-    a.table_kind = table_kind; a.pairing = pairing; a.rot = rot; a.tab_rows = table_rows;
-    a.tab_vec = tab_vec(table_kind, table_a, table_b, table_row_stride);
-    a.ta = table_a; a.tb = table_b; a.tab_stride = table_row_stride; a.eps = eps;
-    return (int)lr::launch_cache_append(a, reinterpret_cast<hipStream_t>(stream));
+    a.k_sc = static_cast<uint8_t*>(k_scales);
+    a.v_sc = static_cast<uint8_t*>(v_scales);
+    a.sc_ps = scale_page_stride;
+    return (int)lr::launch_cache_append8(a, reinterpret_cast<hipStream_t>(stream));
 }
 
 int lr_cache_copy_pages(void* k_pages, void* v_pages, int layers, int64_t layer_stride, int64_t page_stride,
@@ -432,8 +553,41 @@ int lr_cache_copy_pages(void* k_pages, void* v_pages, int layers, int64_t layer_
     a.vp = static_cast<uint16_t*>(v_pages);
     a.pg = page_args(page_stride, row_stride, head_stride, n_pages, page_size, nullptr, 0, 0);
     a.layer_stride = layer_stride;
-    a.src = src; a.dst = dst; a.n = n; a.layers = layers; a.HK = HK;
+    a.src = src; a.dst = dst; a.n = n; a.layers = layers; a.HK = HK; a.es = 2;
     return (int)lr::launch_cache_copy(a, reinterpret_cast<hipStream_t>(stream));
+}
+
+int lr_cache_copy_pages_f8(void* k_pages, void* v_pages, int layers, int64_t layer_stride, int64_t page_stride, int64_t row_stride,
+                           int64_t head_stride, int n_pages, int page_size, int HK, void* k_scales, void* v_scales,
+                           int64_t scale_layer_stride, int64_t scale_page_stride, const int* src, const int* dst, int n,
+                           lr_stream_t stream) {
+    if (!pool_ok(k_pages, v_pages, page_stride, row_stride, head_stride, n_pages, page_size, HK, layers, layer_stride, 1) ||
+        !page8_ok(page_size, row_stride) ||
+        !scales_ok(k_scales, v_scales, scale_page_stride, n_pages, page_size, HK, layers, scale_layer_stride))
+        return ERR_ARGS;
+    if (n < 1 || !src || !dst || !aligned(src, 4) || !aligned(dst, 4)) return ERR_ARGS;
+    for (void* p : {k_scales, v_scales}) {
+        const Span sc = scales_span(p, layers, scale_layer_stride, scale_page_stride, n_pages, page_size, HK);
+        for (void* x : {k_pages, v_pages})
+            if (overlap(sc, pool_span(x, layers, layer_stride, page_stride, row_stride, head_stride, n_pages, page_size, HK, 1)))
+                return ERR_ARGS;
+    }
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    lr::CacheCopyArgs a{};
+    a.kp = static_cast<uint16_t*>(k_pages);
+    a.vp = static_cast<uint16_t*>(v_pages);
+    a.pg = page_args(page_stride, row_stride, head_stride, n_pages, page_size, nullptr, 0, 0);
+    a.layer_stride = layer_stride;
+    a.src = src; a.dst = dst; a.n = n; a.layers = layers; a.HK = HK; a.es = 1;
+    const hipError_t e = lr::launch_cache_copy(a, s);
+    if (e != hipSuccess) return (int)e;
+    lr::CacheCopyScalesArgs c{};
+    c.k_sc = static_cast<uint8_t*>(k_scales);
+    c.v_sc = static_cast<uint8_t*>(v_scales);
+    c.sc_ps = scale_page_stride; c.layer_stride = scale_layer_stride;
+    c.src = src; c.dst = dst; c.n = n; c.layers = layers; c.n_pages = n_pages;
+    c.bytes = (int)scales_bytes(page_size, HK);
+    return (int)lr::launch_cache_copy_scales(c, s);
 }
 
 int lr_cache_move_rows(void* k_pages, void* v_pages, int layers, int64_t layer_stride, int64_t page_stride,

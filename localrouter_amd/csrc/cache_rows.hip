@@ -11,32 +11,8 @@ namespace lr {
 
 namespace {
 
-#include "rope_rows.inc"
+#include "append_rows.inc"
 #include "div_small.inc"
-
-// The sequence of token t: the largest b < B with starts[b] <= t, by the 16 lanes of the token's group, 16 probes a round.
-// -1: none. (Every lane of the wave takes the same rounds.)
-__device__ __forceinline__ int seq_of_token(const int* starts, int B, int t) {
-    const int lane = threadIdx.x & 63, c = lane & 15;
-    int lo = 0, width = B;
-    while (width > 1) {
-        const int step = (width + 15) >> 4;
-        const int i = lo + c * step;
-        const bool le = c * step < width && i < B && starts[min(i, B - 1)] <= t;
-        const int cnt = __popcll((__builtin_amdgcn_ballot_w64(le) >> (lane & 48)) & 0xffff);
-        lo += max(cnt - 1, 0) * step;
-        width = step;
-    }
-    return starts[lo] <= t && t < starts[lo + 1] ? lo : -1;
-}
-
-// Offset (elements) of position j of sequence b in the pool, or -1 where the sequence's table or the pool does not have it.
-__device__ __forceinline__ int64_t page_offset(const PageArgs& g, int b, int j) {
-    if (j < 0 || (j >> g.shift) >= g.table_pages) return -1;
-    const int page = g.table[(int64_t)b * g.table_rs + (j >> g.shift)];
-    if (page < 0 || page >= g.n_pages) return -1;
-    return (int64_t)page * g.ps + (int64_t)(j & ((1 << g.shift) - 1)) * g.rs;
-}
 
 // One 16-lane group owns one token and HPG heads of one of q, k and v; lane c dims 8c .. 8c + 7 (rope_rows.inc's layout).
 template <int KIND, int PAIRING>
@@ -79,17 +55,7 @@ __global__ __launch_bounds__(256) void cache_append_kernel(CacheAppendArgs a) {
         // (no return: the other groups of the wave exchange lanes below)
     }
     Rot2 rt[8];
-    const int P = a.rot >> 1;
-    if constexpr (KIND != TABLE_NONE) {
-        const int64_t toff = (int64_t)(live ? pos : 0) * a.tab_stride;
-        if constexpr (PAIRING == PAIR_INTERLEAVED) {
-            rot4<KIND>(a.ta, a.tb, toff, 4 * c, P, a.tab_vec, rt);
-        } else {
-            const int hc = a.rot >> 4, pc = c < hc ? c : c - hc;
-            rot4<KIND>(a.ta, a.tb, toff, 8 * pc, P, a.tab_vec, rt);
-            rot4<KIND>(a.ta, a.tb, toff, 8 * pc + 4, P, a.tab_vec, rt + 4);
-        }
-    }
+    table_rot<KIND, PAIRING>(a.ta, a.tb, (int64_t)(live ? pos : 0) * a.tab_stride, c, a.rot, a.tab_vec, rt);
 #pragma unroll
     for (int i = 0; i < HPG; ++i) {
         const int h = h0 + i;
@@ -99,38 +65,7 @@ __global__ __launch_bounds__(256) void cache_append_kernel(CacheAppendArgs a) {
             x[2 * j] = lo_bf16(xin[i][j]);
             x[2 * j + 1] = hi_bf16(xin[i][j]);
         }
-        float ss = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
-        ss = row16_sum(ss);
-        const float rr = rsqrtf(ss * (1.0f / D) + a.eps);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = x[j] * rr * wv[j];
-        if constexpr (KIND != TABLE_NONE) {
-            if constexpr (PAIRING == PAIR_INTERLEAVED) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const bool on = 8 * c + 2 * j < a.rot;
-                    const float x0 = x[2 * j], x1 = x[2 * j + 1];
-                    const float y0 = fmaf(rt[j].f00, x0, rt[j].f01 * x1);
-                    const float y1 = fmaf(rt[j].f10, x0, rt[j].f11 * x1);
-                    x[2 * j] = on ? y0 : x0;
-                    x[2 * j + 1] = on ? y1 : x1;
-                }
-            } else {
-                const int hc = a.rot >> 4, base = tid & 48;
-                const bool first = c < hc, second = c >= hc && c < 2 * hc;
-                const int partner = base + (first ? c + hc : (second ? c - hc : c));
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float y = __shfl(x[j], partner, 64);
-                    const float a0 = first ? x[j] : y, b0 = first ? y : x[j];
-                    const float ya = fmaf(rt[j].f00, a0, rt[j].f01 * b0);
-                    const float yb = fmaf(rt[j].f10, a0, rt[j].f11 * b0);
-                    x[j] = first ? ya : (second ? yb : x[j]);
-                }
-            }
-        }
+        norm_turn<KIND, PAIRING>(x, wv, rt, a.eps, a.rot);
         if (live && (is_q || is_k) && h < heads) {
             u32x4 o;
 #pragma unroll
@@ -150,31 +85,33 @@ hipError_t append_kind(const CacheAppendArgs& a, unsigned blocks, hipStream_t st
     return hipGetLastError();
 }
 
-// A workgroup copies 128 rows (32 KB) of one page of one layer's keys or values. FLAT: the page's rows lie next to each other, in
+// A workgroup copies 128 rows of bf16 (32 KB), 256 of 8 bits, of one page of one layer's keys or values. FLAT: the page's rows lie next to each other, in
 // whichever order: 8 loads of 16 bytes in flight a lane, through buffers of the page's size that end a short last chunk.
-constexpr int COPY_ROWS = 128;
-template <bool FLAT>
+constexpr int COPY_BYTES = 32768;
+// ES: bytes of an element.
+template <bool FLAT, int ES>
 __global__ __launch_bounds__(256) void cache_copy_kernel(CacheCopyArgs a, int chunks, uint32_t rcp_chunks, uint32_t rcp_hk) {
     const int pair = div_small(blockIdx.x, chunks, rcp_chunks), chunk = blockIdx.x - pair * chunks;
     const int src = a.src[pair], dst = a.dst[pair];
     if (src < 0 || src >= a.pg.n_pages || dst < 0 || dst >= a.pg.n_pages || src == dst) return;
-    uint16_t* base = (blockIdx.z ? a.vp : a.kp) + (int64_t)blockIdx.y * a.layer_stride;
-    uint16_t *from = base + (int64_t)src * a.pg.ps, *to = base + (int64_t)dst * a.pg.ps;
+    char* base = reinterpret_cast<char*>(blockIdx.z ? a.vp : a.kp) + (int64_t)blockIdx.y * a.layer_stride * ES;
+    char *from = base + (int64_t)src * a.pg.ps * ES, *to = base + (int64_t)dst * a.pg.ps * ES;
     const int rows = a.HK << a.pg.shift;
     if constexpr (FLAT) {
-        const __amdgpu_buffer_rsrc_t in = __builtin_amdgcn_make_buffer_rsrc(from, 0, rows * D * 2, 0x00020000);
-        const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(to, 0, rows * D * 2, 0x00020000);
-        const int off = chunk * COPY_ROWS * D * 2 + 16 * (int)threadIdx.x;
-        u32x4 x[COPY_ROWS / 16];
+        const __amdgpu_buffer_rsrc_t in = __builtin_amdgcn_make_buffer_rsrc(from, 0, rows * D * ES, 0x00020000);
+        const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(to, 0, rows * D * ES, 0x00020000);
+        const int off = chunk * COPY_BYTES + 16 * (int)threadIdx.x;
+        u32x4 x[COPY_BYTES / 4096];
 #pragma unroll
-        for (int u = 0; u < COPY_ROWS / 16; ++u) x[u] = __builtin_amdgcn_raw_buffer_load_b128(in, off + 4096 * u, 0, 2);
+        for (int u = 0; u < COPY_BYTES / 4096; ++u) x[u] = __builtin_amdgcn_raw_buffer_load_b128(in, off + 4096 * u, 0, 2);
 #pragma unroll
-        for (int u = 0; u < COPY_ROWS / 16; ++u) __builtin_amdgcn_raw_buffer_store_b128(x[u], out, off + 4096 * u, 0, 2);
+        for (int u = 0; u < COPY_BYTES / 4096; ++u) __builtin_amdgcn_raw_buffer_store_b128(x[u], out, off + 4096 * u, 0, 2);
     } else {
-        const int end = min(rows, (chunk + 1) * COPY_ROWS);
-        for (int r = chunk * COPY_ROWS + (threadIdx.x >> 4); r < end; r += 16) {
+        constexpr int ROWS = COPY_BYTES / (D * ES), LANES = D * ES / 16;
+        const int end = min(rows, (chunk + 1) * ROWS);
+        for (int r = chunk * ROWS + threadIdx.x / LANES; r < end; r += 256 / LANES) {
             const int slot = div_small(r, a.HK, rcp_hk);
-            const int64_t off = (int64_t)slot * a.pg.rs + (int64_t)(r - slot * a.HK) * a.pg.hs + 8 * (threadIdx.x & 15);
+            const int64_t off = ((int64_t)slot * a.pg.rs + (int64_t)(r - slot * a.HK) * a.pg.hs) * ES + 16 * (threadIdx.x % LANES);
             *reinterpret_cast<u32x4*>(to + off) = *reinterpret_cast<const u32x4*>(from + off);
         }
     }
@@ -229,15 +166,16 @@ hipError_t launch_cache_append(const CacheAppendArgs& a, hipStream_t stream) {
 }
 
 hipError_t launch_cache_copy(const CacheCopyArgs& a, hipStream_t stream) {
-    const int rows = a.HK << a.pg.shift, chunks = (rows + COPY_ROWS - 1) / COPY_ROWS;
+    const int rows = a.HK << a.pg.shift, each = COPY_BYTES / (D * a.es), chunks = (rows + each - 1) / each;
     const int64_t blocks = (int64_t)a.n * chunks;
     if (blocks > 1 << 23 || a.layers > 65535) return hipErrorInvalidValue;   // (a grid's work-items are counted in 32 bits)
     const int64_t page = (int64_t)1 << a.pg.shift;
     // (a buffer's size is 32 bits)
     const bool flat = rows <= 1 << 22 && ((a.pg.hs == D && a.pg.rs == (int64_t)a.HK * D) || (a.pg.rs == D && a.pg.hs == page * D));
     const dim3 grid((unsigned)blocks, (unsigned)a.layers, 2);
-    if (flat) hipLaunchKernelGGL(cache_copy_kernel<true>, grid, dim3(256), 0, stream, a, chunks, rcp_small(chunks), rcp_small(a.HK));
-    else hipLaunchKernelGGL(cache_copy_kernel<false>, grid, dim3(256), 0, stream, a, chunks, rcp_small(chunks), rcp_small(a.HK));
+    const auto kernel = a.es == 1 ? (flat ? cache_copy_kernel<true, 1> : cache_copy_kernel<false, 1>)
+                                  : (flat ? cache_copy_kernel<true, 2> : cache_copy_kernel<false, 2>);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a, chunks, rcp_small(chunks), rcp_small(a.HK));
     return hipGetLastError();
 }
 

@@ -18,8 +18,8 @@ struct PageArgs {
     int n_pages, shift, table_pages;
 };
 
-// Attention of query tokens over a sequence's keys, each token over its own range of them. Two sources of keys:
-// rows (paged = 0: one sequence, key j of kv head g at k + j * k_rs + g * 128) and pages.
+// Attention of query tokens over a sequence's keys, each token over its own range of them. Sources of keys (range_attn.inc's Source):
+// rows of one sequence (key j of kv head g at k + j * k_rs + g * 128), rows of sequences packed end to end, pages, pages in 8 bits.
 struct RangeAttnArgs {
     const uint16_t* q;   // bf16 [T][H][128], row stride q_rs
     uint16_t* out;       // bf16 [T][H][128], row stride o_rs
@@ -39,6 +39,11 @@ struct RangeAttnArgs {
     const uint64_t* tree;   // [T][words]: bit x of a token's words: it sees the sequence's drafted token x; null: chains
     int B, T, max_rows, max_keys, words;
     int window, sinks;      // window 0 (pages only): every earlier key
+    // pages in 8 bits: k and v are bytes (the strides of pg too), 16 rows of a page and head with a scale 2^(byte - 127): of page p,
+    // row r and head g at k_sc / v_sc + p * sc_ps + (r / 16) * HK + g
+    const uint8_t* k_sc;
+    const uint8_t* v_sc;
+    int64_t sc_ps;
     // Split over the keys: with nsplit > 1 a block of rows is nsplit workgroups, each a part of its key tiles, whose unnormalised
     // rows, references and sums go to the parts (fp32 [slot][128] and [slot][2]).
     // attn_cache.hip: every block, `per` tiles a part, slots [block][part][row]; merged by the last part of a block to end, by the
@@ -72,6 +77,8 @@ constexpr int64_t RANGE_MAX_BLOCKS = 1 << 22;    // workgroups a launch: a grid'
 // attn_cache_wide.hip in workgroups of `waves` waves of 32 rows (the cut's tiles are each kernel's own).
 hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int br, hipStream_t stream);
 hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, int waves, hipStream_t stream);
+// Pages in 8 bits, in blocks of br rows (16 or 32): attn_cache8.hip.
+hipError_t launch_range8(const RangeAttnArgs& a, int br, hipStream_t stream);
 
 // cache_rows.hip
 struct CacheAppendArgs {
@@ -97,16 +104,37 @@ struct CacheAppendArgs {
 };
 hipError_t launch_cache_append(const CacheAppendArgs& a, hipStream_t stream);
 
+// cache8_rows.hip: the same into pages in 8 bits (k and v pages as bytes, the strides of pg too) and their scales (RangeAttnArgs').
+constexpr int GROUP8 = 16;   // rows of a page and head that share a scale
+struct CacheAppend8Args {
+    CacheAppendArgs at;      // (kp and vp: bytes)
+    uint8_t* k_sc;
+    uint8_t* v_sc;
+    int64_t sc_ps;
+};
+hipError_t launch_cache_append8(const CacheAppend8Args& a, hipStream_t stream);
+
 struct CacheCopyArgs {
-    uint16_t* kp;
+    uint16_t* kp;        // (pages of `es` bytes an element: strides are elements)
     uint16_t* vp;
     PageArgs pg;         // no table
     int64_t layer_stride;
     const int* src;
     const int* dst;
-    int n, layers, HK;
+    int n, layers, HK, es;
 };
 hipError_t launch_cache_copy(const CacheCopyArgs& a, hipStream_t stream);
+
+// cache8_rows.hip: `bytes` scales of each page, of both tensors, in every layer.
+struct CacheCopyScalesArgs {
+    uint8_t* k_sc;
+    uint8_t* v_sc;
+    int64_t sc_ps, layer_stride;
+    const int* src;
+    const int* dst;
+    int n, layers, n_pages, bytes;
+};
+hipError_t launch_cache_copy_scales(const CacheCopyScalesArgs& a, hipStream_t stream);
 
 struct CacheMoveArgs {
     uint16_t* kp;

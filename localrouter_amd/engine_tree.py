@@ -7,9 +7,9 @@ source and `kernels/hip/rope_host.cpp`, and its sources include `../../include/l
 `src/engines/hip/lr_attn.zig`. This script writes exactly that layout:
 
     DEST/kernels/hip/         every file of localrouter_amd/csrc (the .hip sources, their .inc / .h parts, rope_host.cpp)
-    DEST/include/             lr_attn.h, lr_cache.h, lr_mmdit.h, lr_rope.h
+    DEST/include/             lr_attn.h, lr_cache.h, lr_cache8.h, lr_mmdit.h, lr_rope.h
     DEST/build/hip.zig        the build module (the root build.zig calls hip.lrAttn(b, target, optimize))
-    DEST/src/engines/hip/     lr_attn.zig, lr_cache.zig (the extern declarations)
+    DEST/src/engines/hip/     lr_attn.zig, lr_cache.zig, lr_cache8.zig (the extern declarations)
 
 Files are copied (or symlinked with --symlink, so that the engine tree follows this repository). Existing files of
 the same names are replaced; nothing else in DEST is touched. Returns / prints the list of files written.

@@ -15,6 +15,7 @@
 #include <string>
 
 #include "../../include/lr_cache.h"
+#include "../../include/lr_cache8.h"
 
 namespace {
 
@@ -24,6 +25,10 @@ decltype(&lr_cache_attention_bf16) f_attention = nullptr;
 decltype(&lr_cache_attention_ws_bytes) f_attention_ws = nullptr;
 decltype(&lr_cache_copy_pages) f_copy = nullptr;
 decltype(&lr_cache_move_rows) f_move = nullptr;
+decltype(&lr_cache_append_f8) f_append8 = nullptr;
+decltype(&lr_cache_attention_f8) f_attention8 = nullptr;
+decltype(&lr_cache_attention_f8_ws_bytes) f_attention8_ws = nullptr;
+decltype(&lr_cache_copy_pages_f8) f_copy8 = nullptr;
 decltype(&lr_attention_window_bf16) f_window = nullptr;
 decltype(&lr_attention_window_ws_bytes) f_window_ws = nullptr;
 
@@ -117,18 +122,18 @@ const int* ints(PyObject* o, const char* name, const Where& w, int64_t n) {
     return static_cast<const int*>(vector(o, name, w, n, at::kInt, "int32"));
 }
 
-// bf16 [[layers,] n_pages, page_size, heads, 128] of keys and values
+// bf16 (or e4m3) [[layers,] n_pages, page_size, heads, 128] of keys and values
 struct Pool {
     void *k, *v;
     int64_t ls = 0, ps, rs, hs;
     int layers = 1, n_pages, page_size, heads;
-    Pool(PyObject* ko, PyObject* vo, const Where& w, bool with_layers) {
+    Pool(PyObject* ko, PyObject* vo, const Where& w, bool with_layers, at::ScalarType type = at::kBFloat16) {
         const at::Tensor &kt = tensor(ko, "k_pages"), &vt = tensor(vo, "v_pages");
         const int64_t n = kt.dim();
         if (vt.sizes() != kt.sizes() || vt.strides() != kt.strides() || (n != 4 && !(with_layers && n == 5)) ||
-            kt.size(n - 1) != 128 || kt.stride(n - 1) != 1 || !w.holds(kt, at::kBFloat16) || !w.holds(vt, at::kBFloat16))
-            refuse("k_pages, v_pages", std::string("bf16 [n_pages, page_size, heads, 128]") + (with_layers ? " or [layers, ...]" : "") +
-                   " of the same shape and strides", ko, vo);
+            kt.size(n - 1) != 128 || kt.stride(n - 1) != 1 || !w.holds(kt, type) || !w.holds(vt, type))
+            refuse("k_pages, v_pages", std::string(type == at::kBFloat16 ? "bf16" : "float8_e4m3fn") + " [n_pages, page_size, heads, 128]" +
+                   (with_layers ? " or [layers, ...]" : "") + " of the same shape and strides", ko, vo);
         const auto s = kt.sizes().slice(n - 4), st = kt.strides().slice(n - 4);
         for (int i = 0; i < 3; ++i)
             if (s[i] > INT_MAX) refuse("k_pages: too large");
@@ -143,6 +148,29 @@ struct Pool {
             layers = (int)kt.size(0);
             ls = layers > 1 ? kt.stride(0) : 0;
         }
+        k = kt.data_ptr();
+        v = vt.data_ptr();
+    }
+};
+
+// The scales of a pool in 8 bits: e8m0 [[layers,] n_pages, page_size / 16, heads], the last two dimensions contiguous, of keys and values
+struct Scales {
+    void *k, *v;
+    int64_t ls = 0, ps;
+    Scales(PyObject* ko, PyObject* vo, const Where& w, const Pool& pool, int64_t dims) {
+        const at::Tensor &kt = tensor(ko, "k_scales"), &vt = tensor(vo, "v_scales");
+        const int64_t n = kt.dim(), groups = pool.page_size / 16;
+        bool ok = n == dims - 1 && vt.sizes() == kt.sizes() && vt.strides() == kt.strides() && w.holds(kt, at::kFloat8_e8m0fnu) &&
+                  w.holds(vt, at::kFloat8_e8m0fnu);
+        ok = ok && kt.size(n - 3) == pool.n_pages && kt.size(n - 2) == groups && kt.size(n - 1) == pool.heads &&
+             (pool.heads == 1 || kt.stride(n - 1) == 1) && (groups == 1 || kt.stride(n - 2) == pool.heads) &&
+             (n < 4 || kt.size(0) == pool.layers);
+        if (!ok)
+            refuse("k_scales, v_scales", "float8_e8m0fnu [" + std::string(dims == 5 ? "layers, " : "") + std::to_string(pool.n_pages) + ", " +
+                   std::to_string(groups) + ", " + std::to_string(pool.heads) + "] of the same strides, its last two dimensions contiguous,",
+                   ko, vo);
+        ps = pool.n_pages > 1 ? kt.stride(n - 3) : groups * pool.heads;
+        ls = n == 4 && pool.layers > 1 ? kt.stride(0) : 0;
         k = kt.data_ptr();
         v = vt.data_ptr();
     }
@@ -245,12 +273,13 @@ void call(const char* name, F&& f) {
 }
 
 // (device, stream, q, k, v, k_pages, v_pages, page_table, starts, lens, q_out, q_norm, k_norm, kind, table_a, table_b, positions,
-// pairing, rot, eps)
+// pairing, rot, eps[, k_scales, v_scales])
+template <bool F8>
 PyObject* append(PyObject* const* a) {
     const Where w(a[0], a[1]);
     const int64_t T = size0(a[3], "k"), B = size0(a[9], "lens");
     const Rotation tab = T > 0 ? Rotation(a[13], a[14], a[15], a[18]) : Rotation();
-    const Pool pool(a[5], a[6], w, false);
+    const Pool pool(a[5], a[6], w, false, F8 ? at::kFloat8_e4m3fn : at::kBFloat16);
     const Rows k(a[3], "k", w, T, pool.heads), v(a[4], "v", w, T, pool.heads);
     Rows q, out;
     Held held{nullptr};
@@ -277,23 +306,35 @@ PyObject* append(PyObject* const* a) {
         const float eps = number(a[19]);
         const void *ta = tab.a ? tab.a->data_ptr() : nullptr, *tb = tab.b ? tab.b->data_ptr() : nullptr;
         const int64_t stride = tab.a ? tab.a->stride(0) : 0;
-        call("lr_cache_append_bf16", [&] {
-            return f_append(q.p, k.p, v.p, q.rs, k.rs, v.rs, out.p, out.rs, pool.k, pool.v, pool.ps, pool.rs, pool.hs, pool.n_pages,
-                            pool.page_size, table.p, table.rs, table.pages, starts, lens, pos, (int)B, (int)T, (int)H, pool.heads, qw,
-                            kw, tab.kind, ta, tb, stride, tab.rows, pairing, tab.rot, eps, static_cast<lr_stream_t>(w.stream));
-        });
+        const lr_stream_t stream = static_cast<lr_stream_t>(w.stream);
+        if constexpr (F8) {
+            const Scales scales(a[20], a[21], w, pool, 4);
+            call("lr_cache_append_f8", [&] {
+                return f_append8(q.p, k.p, v.p, q.rs, k.rs, v.rs, out.p, out.rs, pool.k, pool.v, pool.ps, pool.rs, pool.hs, pool.n_pages,
+                                 pool.page_size, scales.k, scales.v, scales.ps, table.p, table.rs, table.pages, starts, lens, pos, (int)B,
+                                 (int)T, (int)H, pool.heads, qw, kw, tab.kind, ta, tb, stride, tab.rows, pairing, tab.rot, eps, stream);
+            });
+        } else {
+            call("lr_cache_append_bf16", [&] {
+                return f_append(q.p, k.p, v.p, q.rs, k.rs, v.rs, out.p, out.rs, pool.k, pool.v, pool.ps, pool.rs, pool.hs, pool.n_pages,
+                                pool.page_size, table.p, table.rs, table.pages, starts, lens, pos, (int)B, (int)T, (int)H, pool.heads, qw,
+                                kw, tab.kind, ta, tb, stride, tab.rows, pairing, tab.rot, eps, stream);
+            });
+        }
     }
     if (held.o) return held.release();
     Py_RETURN_NONE;
 }
 
-// (device, stream, q, k_pages, v_pages, page_table, starts, lens, out, max_rows, max_keys, tree, window, sinks, scale, workspace)
+// (device, stream, q, k_pages, v_pages, page_table, starts, lens, out, max_rows, max_keys, tree, window, sinks, scale, workspace[,
+// k_scales, v_scales])
+template <bool F8>
 PyObject* attention(PyObject* const* a) {
     const Where w(a[0], a[1]);
     const at::Tensor& qt = tensor(a[2], "q");
     const int64_t T = size0(a[2], "q"), H = qt.dim() == 3 ? qt.size(1) : 0, B = size0(a[7], "lens");
     const Rows q(a[2], "q", w, T, H);
-    const Pool pool(a[3], a[4], w, false);
+    const Pool pool(a[3], a[4], w, false, F8 ? at::kFloat8_e4m3fn : at::kBFloat16);
     Held held{rows_like(a[8], T, H, qt)};
     const Rows out(held.o, "out", w, T, H);
     if (B > INT_MAX || T > INT_MAX || H > INT_MAX) refuse("attention: too many tokens");
@@ -314,7 +355,7 @@ PyObject* attention(PyObject* const* a) {
     const float scale = number(a[14]);
     const int *starts = ints(a[6], "starts", w, B + 1), *lens = ints(a[7], "lens", w, B);
     auto ws_need = [&](int rows, int keys) {
-        return f_attention_ws((int)B, (int)T, rows, keys, (int)H, pool.heads, pool.page_size, window, sinks);
+        return (F8 ? f_attention8_ws : f_attention_ws)((int)B, (int)T, rows, keys, (int)H, pool.heads, pool.page_size, window, sinks);
     };
     size_t need = ws_need(max_rows, max_keys);
     // A workspace for a max_rows or max_keys beyond this call's tokens or its table may be smaller (more rows fill the GPU without
@@ -331,11 +372,21 @@ PyObject* attention(PyObject* const* a) {
         }
     }
     const Workspace ws(a[15], w, need, qt);
-    call("lr_cache_attention_bf16", [&] {
-        return f_attention(q.p, q.rs, out.p, out.rs, pool.k, pool.v, pool.ps, pool.rs, pool.hs, pool.n_pages, pool.page_size, table.p,
-                           table.rs, table.pages, starts, lens, (int)B, (int)T, max_rows, max_keys, (int)H, pool.heads, tree, words,
-                           window, sinks, scale, ws.p, ws.bytes, static_cast<lr_stream_t>(w.stream));
-    });
+    const lr_stream_t stream = static_cast<lr_stream_t>(w.stream);
+    if constexpr (F8) {
+        const Scales scales(a[16], a[17], w, pool, 4);
+        call("lr_cache_attention_f8", [&] {
+            return f_attention8(q.p, q.rs, out.p, out.rs, pool.k, pool.v, pool.ps, pool.rs, pool.hs, pool.n_pages, pool.page_size, scales.k,
+                                scales.v, scales.ps, table.p, table.rs, table.pages, starts, lens, (int)B, (int)T, max_rows, max_keys,
+                                (int)H, pool.heads, tree, words, window, sinks, scale, ws.p, ws.bytes, stream);
+        });
+    } else {
+        call("lr_cache_attention_bf16", [&] {
+            return f_attention(q.p, q.rs, out.p, out.rs, pool.k, pool.v, pool.ps, pool.rs, pool.hs, pool.n_pages, pool.page_size, table.p,
+                               table.rs, table.pages, starts, lens, (int)B, (int)T, max_rows, max_keys, (int)H, pool.heads, tree, words,
+                               window, sinks, scale, ws.p, ws.bytes, stream);
+        });
+    }
     return held.release();
 }
 
@@ -351,6 +402,24 @@ PyObject* copy_pages(PyObject* const* a) {
         call("lr_cache_copy_pages", [&] {
             return f_copy(pool.k, pool.v, pool.layers, pool.ls, pool.ps, pool.rs, pool.hs, pool.n_pages, pool.page_size, pool.heads, src,
                           dst, (int)n, static_cast<lr_stream_t>(w.stream));
+        });
+    }
+    Py_RETURN_NONE;
+}
+
+// (device, stream, k_pages, v_pages, k_scales, v_scales, src, dst)
+PyObject* copy_pages_f8(PyObject* const* a) {
+    const Where w(a[0], a[1]);
+    const Pool pool(a[2], a[3], w, true, at::kFloat8_e4m3fn);
+    const Scales scales(a[4], a[5], w, pool, tensor(a[2], "k_pages").dim());
+    const int64_t n = size0(a[6], "src");
+    if (size0(a[7], "dst") != n) refuse("copy_pages_f8: src and dst of different lengths");
+    if (n > INT_MAX) refuse("copy_pages_f8: too many pages");
+    if (n > 0) {
+        const int *src = ints(a[6], "src", w, n), *dst = ints(a[7], "dst", w, n);
+        call("lr_cache_copy_pages_f8", [&] {
+            return f_copy8(pool.k, pool.v, pool.layers, pool.ls, pool.ps, pool.rs, pool.hs, pool.n_pages, pool.page_size, pool.heads,
+                           scales.k, scales.v, scales.ls, scales.ps, src, dst, (int)n, static_cast<lr_stream_t>(w.stream));
         });
     }
     Py_RETURN_NONE;
@@ -429,7 +498,9 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!take(f_append, "lr_cache_append_bf16") || !take(f_attention, "lr_cache_attention_bf16") ||
         !take(f_attention_ws, "lr_cache_attention_ws_bytes") || !take(f_copy, "lr_cache_copy_pages") ||
         !take(f_move, "lr_cache_move_rows") || !take(f_window, "lr_attention_window_bf16") ||
-        !take(f_window_ws, "lr_attention_window_ws_bytes")) {
+        !take(f_window_ws, "lr_attention_window_ws_bytes") || !take(f_append8, "lr_cache_append_f8") ||
+        !take(f_attention8, "lr_cache_attention_f8") || !take(f_attention8_ws, "lr_cache_attention_f8_ws_bytes") ||
+        !take(f_copy8, "lr_cache_copy_pages_f8")) {
         if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: an address is missing");
         return nullptr;
     }
@@ -441,9 +512,12 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)), METH_FASTCALL, nullptr
 PyMethodDef methods[] = {{"bind", FAST(bind)},
-                         {"append", FAST((&guarded<append, 20>))},
-                         {"attention", FAST((&guarded<attention, 16>))},
+                         {"append", FAST((&guarded<append<false>, 20>))},
+                         {"append_f8", FAST((&guarded<append<true>, 22>))},
+                         {"attention", FAST((&guarded<attention<false>, 16>))},
+                         {"attention_f8", FAST((&guarded<attention<true>, 18>))},
                          {"copy_pages", FAST((&guarded<copy_pages, 6>))},
+                         {"copy_pages_f8", FAST((&guarded<copy_pages_f8, 8>))},
                          {"move_rows", FAST((&guarded<move_rows, 9>))},
                          {"attention_window", FAST((&guarded<attention_window, 12>))},
                          {nullptr, nullptr, 0, nullptr}};

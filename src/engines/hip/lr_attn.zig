@@ -18,6 +18,8 @@ const std = @import("std");
 
 /// include/lr_cache.h: the cache in pages.
 pub const cache = @import("lr_cache.zig");
+/// include/lr_cache8.h: the cache in pages of 8 bits.
+pub const cache8 = @import("lr_cache8.zig");
 
 pub const Stream = ?*anyopaque;
 
