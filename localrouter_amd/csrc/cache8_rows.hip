@@ -110,7 +110,8 @@ __device__ __forceinline__ int seq_of_group(const int* starts, int B, int u) {
     while (width > 1) {
         const int step = (width + 63) >> 6, at = lane * step, i = lo + at;
         const bool le = at < width && i < B && (starts[min(i, B - 1)] >> 4) + 2 * i <= u;
-        lo += max(__popcll(__builtin_amdgcn_ballot_w64(le)) - 1, 0) * step;
+        const int cnt = __popcll(__builtin_amdgcn_ballot_w64(le));   // (unsigned as it comes; 0 of starts that begin later)
+        lo += max(cnt - 1, 0) * step;
         width = step;
     }
     return lo;

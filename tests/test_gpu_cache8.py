@@ -428,6 +428,18 @@ def test_append_token_by_token_holds_what_one_call_does():
     assert (d <= 2.0 ** -4 * v.double().abs() + 12 * 2.0 ** -10 * top).all()
 
 
+@pytest.mark.parametrize("B", [1, 3, 90])
+def test_append_of_sequences_that_begin_late(B):
+    """Rows before the first sequence are left out: the search for a group's sequence begins behind its first numbers."""
+    b = Batch8(36, [17] * B, [40] * B, 16, 2)
+    v, lead = rnd(b.g, 200 + 17 * B, 2, 128), 150
+    want = [x.clone() for x in (b.kp, b.vp, b.ks, b.vs)]
+    cache.append_f8(None, v[lead:], v[lead:], *want, b.t, b.starts, b.lens, table_kind=ops.TABLE_NONE)
+    cache.append_f8(None, v, v, b.kp, b.vp, b.ks, b.vs, b.t, b.starts + lead, b.lens, table_kind=ops.TABLE_NONE)
+    for x, y in zip((b.kp, b.vp, b.ks, b.vs), want):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
 def test_append_leaves_the_rest():
     """Rows behind the sequences, pages of others and their scales, queries' columns of others; a page that the pool does not have."""
     B = Batch8(35, [3, 20], [21, 20], 16, 2)
