@@ -153,6 +153,19 @@ int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* 
                              lr_stream_t stream);
 
 /*
+ * Causal attention over whole prompts packed end to end: sequence b < B is the rows starts[b] .. starts[b + 1] - 1 of q, k, v and out
+ * (int32 [B + 1] on the device, ascending; T rows in all), and its i-th token sees its tokens j <= i; with window >= 1 those with
+ * i - j < window or j < sinks (window 0: all). Rows at and behind starts[B], and before starts[0], are left out: their output rows
+ * stay as they were. Grouped heads: query head h reads kv head h / (H / HK). A key that a token does not see has no part in its
+ * result, whatever it holds. starts is read by the kernels: a captured call follows what it holds at its replay. Layouts, arithmetic
+ * and other requirements as lr_attention_bf16, with separate k and v row strides below 2^23; T times H / HK at most 2^30, B at most
+ * 65,535. out must not overlap q, k or v (rejected).
+ */
+int lr_attention_packed_bf16(const void* q, const void* k, const void* v, void* out, const int* starts, int B, int T, int H, int HK,
+                             int window, int sinks, float scale, int64_t q_row_stride, int64_t k_row_stride, int64_t v_row_stride,
+                             int64_t out_row_stride, lr_stream_t stream);
+
+/*
  * Attention under a key-padding mask: keys j with kmask[j] == 0 are left out (torch's bool key-padding mask, SDPA's
  * additive 0 / -inf), the drop-in for Kandinsky-6's attention.Call with mask = .keys
  * (src/engines/kandinsky6/dit/attention.zig:21-27, dispatched by launch.zig:239-255). Non-causal; q, out rows

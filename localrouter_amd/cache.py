@@ -80,7 +80,7 @@ def _host():
             raise RuntimeError("localrouter_amd._host_calls is missing: build it with `python -m localrouter_amd.build` where torch and "
                                "Python's headers are installed (there is no fallback path)") from e
         L = lib()
-        names = [*SIGNATURES, *SIGNATURES_F8, "lr_attention_window_bf16", "lr_attention_window_ws_bytes"]
+        names = [*SIGNATURES, *SIGNATURES_F8, "lr_attention_window_bf16", "lr_attention_window_ws_bytes", "lr_attention_packed_bf16"]
         _host_calls.bind(_lib.LrError, {n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names})
         _calls = _host_calls
     return _calls

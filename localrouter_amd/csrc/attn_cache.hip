@@ -38,7 +38,7 @@ __device__ __forceinline__ void load_tile_rows(const RangeAttnArgs& a, const Seq
     const int64_t k_rs = PAGED ? a.pg.rs : a.k_rs, v_rs = PAGED ? a.pg.rs : a.v_rs;
     const uint16_t *kp = a.k + hoff, *vp = a.v + hoff;
     if ((!PAGED || tl.shift >= 5) && key0 + BT <= sq.end) {   // the tile's rows are one run
-        const int64_t row = (PAGED ? key0 & ((1 << tl.shift) - 1) : key0) + 4 * rb + lrow;
+        const int64_t row = (PAGED ? key0 & ((1 << tl.shift) - 1) : tl.row0 + key0) + 4 * rb + lrow;
         const int64_t pg = PAGED ? (int64_t)max(tl.entry(x, 0), 0) * a.pg.ps : 0;
         kp += pg + row * k_rs;
         vp += pg + row * v_rs + 8 * (lchunk ^ (lrow << 2));
@@ -340,7 +340,9 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
 
     // ---- which rows, which keys
     const int at = div_small(blockIdx.x, a.nsplit, a.rcp_split), split = blockIdx.x - at * a.nsplit;
-    const int blk = div_small(at, a.HK, a.rcp_hk), hk = at - blk * a.HK, b = blockIdx.y;
+    int blk = div_small(at, a.HK, a.rcp_hk), b = blockIdx.y;
+    const int hk = at - blk * a.HK;
+    if (SRC == PACKED && !packed_block<BR>(a, blk, b, blk)) return;
     // without a window a part's entries do not depend on the sequence: they are read beside its numbers
     int early = -1;
     const int per_tile = PAGED ? max(1, BT >> a.pg.shift) : 1;
@@ -576,6 +578,14 @@ hipError_t launch_blocks(const RangeAttnArgs& a, bool paged, int threads, void (
 }
 
 }  // namespace
+
+hipError_t launch_packed_attn(const RangeAttnArgs& a, int br, hipStream_t stream) {
+    const int64_t blocks = ((int64_t)a.T * a.G / br + a.B) * a.HK;
+    if (blocks > RANGE_MAX_BLOCKS) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((br == 16 ? range_step_kernel<1, 8, PACKED> : range_step_kernel<2, 8, PACKED>), dim3((unsigned)blocks), dim3(512), 0,
+                       stream, a);
+    return hipGetLastError();
+}
 
 hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int br, hipStream_t stream) {
     if (br == 16) return launch_blocks<16>(a, paged, 512, range_step_kernel<1, 8, ROWS>, range_step_kernel<1, 8, PAGES>, stream);

@@ -78,6 +78,11 @@ __device__ __forceinline__ bool block_of(const RangeAttnArgs& a, int id, int& b,
         cut = xcd * (a.local - a.whole) + q;
     }
     b = 0;
+    if constexpr (SRC == PACKED) {   // every XCD works on its own heads, or with fewer than 8 shares one with others
+        const int u = div_small(idx, a.HK, a.rcp_hk);
+        hk = idx - u * a.HK;
+        return packed_block<32 * QW>(a, u, b, blk);
+    }
     if (PAGED || a.by_xcd) {
         int pair = div_small(idx, a.nblk, a.rcp_nblk);
         blk = a.nblk - 1 - (idx - pair * a.nblk);
@@ -262,7 +267,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         if constexpr (PAGED)
             return (uint64_t)(((int64_t)__builtin_amdgcn_readfirstlane(max(entry, 0)) * a.pg.ps +
                                (int64_t)(j & ((1 << tl.shift) - 1)) * rs) * 2);
-        return (uint64_t)((int64_t)j * rs * 2);
+        return (uint64_t)((int64_t)(tl.row0 + j) * rs * 2);
     };
     // the page-table entries of the next refills, read a half-step ahead (read where they are used, each kept the wave's
     // products waiting for LDS)
@@ -684,6 +689,14 @@ hipError_t launch_waves(const RangeAttnArgs& a, hipStream_t stream) {
 }
 
 }  // namespace
+
+hipError_t launch_packed_wide(const RangeAttnArgs& a, int waves, hipStream_t stream) {
+    const int64_t blocks = ((int64_t)a.T * a.G / (32 * waves) + a.B) * a.HK;
+    if (blocks > RANGE_MAX_BLOCKS) return hipErrorInvalidValue;
+    if (waves == 8) hipLaunchKernelGGL((range_wide_kernel<8, PACKED>), dim3((unsigned)blocks), dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((range_wide_kernel<4, PACKED>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
 
 hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, int waves, hipStream_t stream) {
     if (waves == 8) return paged ? launch_waves<8, PAGES>(a, stream) : launch_waves<8, ROWS>(a, stream);

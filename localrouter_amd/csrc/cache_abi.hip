@@ -261,6 +261,17 @@ Cut cache_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, i
     }
     return cut_small(rows, pairs, tiles, page_size);
 }
+// Sequences packed end to end: blocks of 16 and 32 rows of few rows in all, else workgroups of four or eight waves.
+Cut packed_cut(int B, int T, int H, int HK) {
+    const int64_t rows = (int64_t)T * (H / HK);
+    Cut c{};
+    c.nsplit = 1; c.per = MAX_POS;
+    if (rows * HK <= 16384) c.br = rows <= 16 * (int64_t)B ? 16 : 32;
+    else c.wide = rows * HK >= 256 * 2048 ? 8 : 4;
+    const int64_t br = c.wide ? 32 * c.wide : c.br;
+    c.nblk = (int)((rows + br - 1) / br);
+    return c;
+}
 // Pages in 8 bits (attn_cache8.hip): blocks of 16 or 32 rows.
 Cut cache8_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks) {
     const int64_t rows = (int64_t)max_rows * (H / HK), pairs = (int64_t)B * HK;
@@ -438,6 +449,35 @@ int lr_attention_window_bf16(const void* q, const void* k, const void* v, void* 
     a.rcp_frame = lr::rcp_small(a.frame);
     a.window = std::min(window, MAX_POS); a.sinks = std::min(sinks, MAX_POS);
     return launch(a, false, cut, stream);
+}
+
+int lr_attention_packed_bf16(const void* q, const void* k, const void* v, void* out, const int* starts, int B, int T, int H, int HK,
+                             int window, int sinks, float scale, int64_t q_row_stride, int64_t k_row_stride, int64_t v_row_stride,
+                             int64_t out_row_stride, lr_stream_t stream) {
+    if (B < 1 || B > 65535 || T < 1 || T > MAX_POS || H < 1 || HK < 1 || H % HK || (int64_t)T * (H / HK) > MAX_POS || window < 0 ||
+        sinks < 0 || !scale_ok(scale) || !starts || !aligned(starts, 4))
+        return ERR_ARGS;
+    if (!rows_ok(q, q_row_stride, H) || !rows_ok(out, out_row_stride, H) || !rows_ok(k, k_row_stride, HK) ||
+        !rows_ok(v, v_row_stride, HK) || k_row_stride >= lr::RANGE_WIDE_MAX_RS || v_row_stride >= lr::RANGE_WIDE_MAX_RS)
+        return ERR_ARGS;
+    const Span so = rows_span(out, T, out_row_stride, H);
+    if (overlap(so, rows_span(q, T, q_row_stride, H)) || overlap(so, rows_span(k, T, k_row_stride, HK)) ||
+        overlap(so, rows_span(v, T, v_row_stride, HK)))
+        return ERR_ARGS;
+    lr::RangeAttnArgs a{};
+    a.q = static_cast<const uint16_t*>(q);
+    a.k = static_cast<const uint16_t*>(k);
+    a.v = static_cast<const uint16_t*>(v);
+    a.out = static_cast<uint16_t*>(out);
+    a.q_rs = q_row_stride; a.k_rs = k_row_stride; a.v_rs = v_row_stride; a.o_rs = out_row_stride;
+    a.H = H; a.HK = HK; a.G = H / HK;
+    a.c = scale * 1.4426950408889634f;
+    a.starts = starts; a.B = B; a.T = T;
+    a.window = std::min(window, MAX_POS); a.sinks = window ? std::min(sinks, MAX_POS) : 0;
+    Cut cut = packed_cut(B, T, H, HK);
+    set_cut(a, nullptr, cut);
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    return (int)(cut.wide ? lr::launch_packed_wide(a, cut.wide, s) : lr::launch_packed_attn(a, cut.br, s));
 }
 
 size_t lr_cache_attention_ws_bytes(int B, int T, int max_rows, int max_keys, int H, int HK, int page_size, int window,

@@ -38,7 +38,8 @@ struct RangeAttnArgs {
     const int* lens;
     const uint64_t* tree;   // [T][words]: bit x of a token's words: it sees the sequence's drafted token x; null: chains
     int B, T, max_rows, max_keys, words;
-    int window, sinks;      // window 0 (pages only): every earlier key
+    int window, sinks;      // window 0 (not of rows): every earlier key
+    // packed: tokens starts[b] .. starts[b + 1] are sequence b, its keys in the same rows of k and v; T rows in all
     // pages in 8 bits: k and v are bytes (the strides of pg too), 16 rows of a page and head with a scale 2^(byte - 127): of page p,
     // row r and head g at k_sc / v_sc + p * sc_ps + (r / 16) * HK + g
     const uint8_t* k_sc;
@@ -77,6 +78,10 @@ constexpr int64_t RANGE_MAX_BLOCKS = 1 << 22;    // workgroups a launch: a grid'
 // attn_cache_wide.hip in workgroups of `waves` waves of 32 rows (the cut's tiles are each kernel's own).
 hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int br, hipStream_t stream);
 hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, int waves, hipStream_t stream);
+// Sequences packed end to end, whole: the same kernels, in blocks of br rows (16 or 32) or of `waves` waves. (nblk: the most blocks a
+// sequence may have.)
+hipError_t launch_packed_attn(const RangeAttnArgs& a, int br, hipStream_t stream);
+hipError_t launch_packed_wide(const RangeAttnArgs& a, int waves, hipStream_t stream);
 // Pages in 8 bits, in blocks of br rows (16 or 32): attn_cache8.hip.
 hipError_t launch_range8(const RangeAttnArgs& a, int br, hipStream_t stream);
 

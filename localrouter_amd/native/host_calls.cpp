@@ -29,6 +29,7 @@ decltype(&lr_cache_append_f8) f_append8 = nullptr;
 decltype(&lr_cache_attention_f8) f_attention8 = nullptr;
 decltype(&lr_cache_attention_f8_ws_bytes) f_attention8_ws = nullptr;
 decltype(&lr_cache_copy_pages_f8) f_copy8 = nullptr;
+decltype(&lr_attention_packed_bf16) f_packed = nullptr;
 decltype(&lr_attention_window_bf16) f_window = nullptr;
 decltype(&lr_attention_window_ws_bytes) f_window_ws = nullptr;
 
@@ -466,6 +467,29 @@ PyObject* attention_window(PyObject* const* a) {
     return held.release();
 }
 
+// (device, stream, q, k, v, starts, out, window, sinks, scale)
+PyObject* attention_packed(PyObject* const* a) {
+    const Where w(a[0], a[1]);
+    const at::Tensor &qt = tensor(a[2], "q"), &kt = tensor(a[3], "k");
+    const int64_t T = size0(a[2], "q"), H = qt.dim() == 3 ? qt.size(1) : 0, HK = kt.dim() == 3 ? kt.size(1) : 0;
+    const Rows q(a[2], "q", w, T, H), k(a[3], "k", w, T, HK), v(a[4], "v", w, T, HK);
+    if (kt.size(0) != T || size0(a[4], "v") != T) refuse("attention_packed: q, k and v of different lengths");
+    const int64_t B = size0(a[5], "starts") - 1;
+    if (B < 1) refuse("starts", "int32 [sequences + 1]", a[5]);
+    Held held{rows_like(a[6], T, H, qt)};
+    const Rows out(held.o, "out", w, T, H);
+    if (T > INT_MAX || B > INT_MAX || H > INT_MAX || HK > INT_MAX) refuse("attention_packed: too many rows");
+    if (T == 0) return held.release();
+    const int* starts = ints(a[5], "starts", w, B + 1);
+    const int window = int32(a[7], "window"), sinks = int32(a[8], "sinks");
+    const float scale = number(a[9]);
+    call("lr_attention_packed_bf16", [&] {
+        return f_packed(q.p, k.p, v.p, out.p, starts, (int)B, (int)T, (int)H, (int)HK, window, sinks, scale, q.rs, k.rs, v.rs, out.rs,
+                        static_cast<lr_stream_t>(w.stream));
+    });
+    return held.release();
+}
+
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* guarded(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != N || !lr_error) {
@@ -500,7 +524,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !take(f_move, "lr_cache_move_rows") || !take(f_window, "lr_attention_window_bf16") ||
         !take(f_window_ws, "lr_attention_window_ws_bytes") || !take(f_append8, "lr_cache_append_f8") ||
         !take(f_attention8, "lr_cache_attention_f8") || !take(f_attention8_ws, "lr_cache_attention_f8_ws_bytes") ||
-        !take(f_copy8, "lr_cache_copy_pages_f8")) {
+        !take(f_copy8, "lr_cache_copy_pages_f8") || !take(f_packed, "lr_attention_packed_bf16")) {
         if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: an address is missing");
         return nullptr;
     }
@@ -520,6 +544,7 @@ PyMethodDef methods[] = {{"bind", FAST(bind)},
                          {"copy_pages_f8", FAST((&guarded<copy_pages_f8, 8>))},
                          {"move_rows", FAST((&guarded<move_rows, 9>))},
                          {"attention_window", FAST((&guarded<attention_window, 12>))},
+                         {"attention_packed", FAST((&guarded<attention_packed, 10>))},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -3,6 +3,7 @@
   attention(...)        <- Ops.attention, src/engines/qwen_image/ops_launch.zig:163-172
   rms_rope(...)         <- Triton.ropeRun + Rope, src/engines/qwen_image/triton_k.zig:44-53
   rms_rope_qk(...)      <- Kitchen.rmsRope, src/engines/minimax_h3/launch.zig:421-441
+  attention_packed(...) prompts packed end to end, causal (no counterpart in the reference)
   attention_window(...) a window of frames and first tokens (no counterpart in the reference)
   joint_attention(...)  <- Dit.block's rope_q / rope_k / V copy / attention chain, src/engines/qwen_image/dit.zig:252-293
   joint_kv_prepare(...), joint_attention_prepared(...)  <- its two stages (keys / values reused across calls)
@@ -130,6 +131,17 @@ def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: tor
     from . import cache   # (its host calls; it imports this module)
     dev = cache._device(q)
     return cache._host().attention_window(dev, cache._raw_stream(dev), q, k, v, out, window, sinks, frame, p0, scale, workspace)
+
+
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, out: torch.Tensor | None = None, *,
+                     window: int = 0, sinks: int = 0, scale: float = SCALE_128) -> torch.Tensor:
+    """lr_attention_packed_bf16: causal attention over prompts packed end to end: sequence b is the rows starts[b] .. starts[b + 1] of
+    q [T, heads, 128] and k / v [T, kv_heads, 128] (views of a packed projection allowed); starts int32 [B + 1] on the GPU. window
+    n >= 1: a token sees the last n tokens up to its own and its sequence's first `sinks`. Rows of no sequence: their output rows
+    stay as they were."""
+    from . import cache   # (its host calls; it imports this module)
+    dev = cache._device(q)
+    return cache._host().attention_packed(dev, cache._raw_stream(dev), q, k, v, starts, out, window, sinks, scale)
 
 
 def attention_kmask(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kmask: torch.Tensor | None,

@@ -47,6 +47,9 @@ pub const JOINT_NOALLOC_SCRATCH_BYTES: usize = (64 << 20) + JOINT_SPLIT_BYTES;
 /// hipBLASLt workspace of one lr_mmdit_linear_bf16 call (LR_MMDIT_GEMM_WORKSPACE).
 pub const MMDIT_GEMM_WORKSPACE: usize = 64 << 20;
 
+/// Causal attention over prompts packed end to end.
+pub extern "lr_attn" fn lr_attention_packed_bf16(q: u64, k: u64, v: u64, out: u64, starts: u64, b: c_int, t: c_int, h: c_int,
+    hk: c_int, window: c_int, sinks: c_int, scale: f32, q_rs: i64, k_rs: i64, v_rs: i64, out_rs: i64, s: Stream) c_int;
 // ---------------------------------------------------------------------------------------------- include/lr_attn.h
 pub extern "lr_attn" fn lr_attn_abi_version() c_int;
 pub extern "lr_attn" fn lr_attn_init() c_int;
