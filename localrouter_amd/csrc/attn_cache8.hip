@@ -22,14 +22,6 @@ namespace {
 #include "range_attn.inc"
 #include "range_parts.inc"
 
-// Eight e4m3 bytes times 2^k, as bf16.
-__device__ __forceinline__ bf16x8 widen(uint32_t w0, uint32_t w1, float s) {
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, true);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, true);
-    const bf16x4 x = __builtin_shufflevector(a, b, 0, 1, 2, 3), y = __builtin_shufflevector(c, d, 0, 1, 2, 3);
-    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
 // Bytes of four words a, b, c, d: word i of the result holds byte i of each.
 __device__ __forceinline__ u32x4 transpose4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     const uint32_t ab0 = __builtin_amdgcn_perm(b, a, 0x05010400), ab1 = __builtin_amdgcn_perm(b, a, 0x07030602);

@@ -162,7 +162,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     // steps of refills in flight beside the current one's. (8 waves have the LDS for 2: pages come from HBM, ~2 us away under load: 16
     // trees of up to 64 tokens over up to 30,000 keys 860 -> 841 us. Rows come from the L2s: 16,384 tokens of video 1,171 us with 2,
     // 1,164 with 0.)
-    constexpr int E = QW == 8 && PAGED ? 2 : 0;
+    constexpr int E = QW == 8 && SRC == PAGES ? 2 : 0;
     constexpr int LP = 16 / QW;                         // direct loads of a tile per wave
     // loads in flight at a step's end, when the next step's keys and this one's values have landed; with E > 0 a step early, so that
     // the next step's first key fragments are read before the barrier (the trees 811 -> 798 us)
@@ -307,6 +307,52 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         dma1_at<0>(src, __umul24(min(vrow + 4 * u, (uint32_t)vlast), rowb) + vchunk, dst + (uint32_t)(1024 * (LP * wv + u)));
     };
 
+    // ---- pages in 8 bits: a step's tiles go through registers, loaded a step before they are converted and written to their
+    // slots (the same as above: what reads them does not differ). Of a key tile a wave takes 32 rows (two groups of 16 with a scale and
+    // a page each, lane's group n >> 4) and 32 LP dims less, of a value tile 64 / QW rows: LP / 2 loads of 16 dims each a lane, which become
+    // two fragments' halves, or two chunks.
+    constexpr int L8 = LP / 2;
+    u32x4 kr8[L8], vr8[L8];
+    uint32_t ksc = 0, vsc = 0;
+    const uint32_t rs8 = (uint32_t)a.pg.rs;   // (below 2^23: the host checks)
+    const uint8_t *const k8 = reinterpret_cast<const uint8_t*>(a.k) + hoff, *const v8 = reinterpret_cast<const uint8_t*>(a.v) + hoff;
+    const int kq = wv % (QW / 2), kg8 = kg + (n & 16);   // (wave's dims 32 LP / 2 kq ..; lane's group of rows)
+    const uint32_t k8_at = (uint32_t)((8 * (2 * wv / QW) + L8 * 2 * kq + hf) * IMG_FRAG_BYTES + 16 * n);
+    const int vrow8 = 64 / QW * wv % 16 + 4 * hf + ((lane >> 1) & 3), vcol8 = (lane & 1) + 2 * ((lane >> 3) & 3);
+    const uint32_t v8_at = (uint32_t)vt_offset(64 / QW * wv + 4 * hf + ((lane >> 1) & 3), 2 * vcol8);
+    auto pages8 = [&](int vx, int kx) __attribute__((always_inline)) {   // the entries of the next loads
+        ev = tl.entry(vx, first(vx, vg, 16) - tl.key0(vx));
+        ek = tl.entry(kx, first(kx, kg8, 16) - tl.key0(kx));
+    };
+    auto load8_k = [&](int x) __attribute__((always_inline)) {
+        const int j = first(x, kg8, 16), r = j & ((1 << tl.shift) - 1);
+        const int64_t page = max(ek, 0);
+        const uint8_t* src = k8 + page * a.pg.ps + (int64_t)((uint64_t)(uint32_t)r * rs8) +
+                             (min(krow & 15, (uint32_t)(tl.end - 1 - j)) * rs8 + (uint32_t)(32 * L8 * kq + 16 * hf));
+#pragma unroll
+        for (int u = 0; u < L8; ++u) kr8[u] = *reinterpret_cast<const u32x4*>(src + 32 * u);
+        ksc = a.k_sc[page * a.sc_ps + (int64_t)((r >> 4) * a.HK + hk)];
+    };
+    auto load8_v = [&](int x) __attribute__((always_inline)) {
+        const int j = first(x, vg, 16), r = j & ((1 << tl.shift) - 1), last = tl.end - 1 - j;
+        const int64_t page = __builtin_amdgcn_readfirstlane(max(ev, 0));
+        const uint8_t* src = v8 + page * a.pg.ps + (int64_t)((uint64_t)(uint32_t)r * rs8);
+#pragma unroll
+        for (int u = 0; u < L8; ++u)
+            vr8[u] = *reinterpret_cast<const u32x4*>(src + ((uint32_t)min(vrow8 + 8 * u, last) * rs8 + (uint32_t)(16 * vcol8)));
+        vsc = a.v_sc[page * a.sc_ps + (int64_t)((r >> 4) * a.HK + hk)];
+    };
+    typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+    // half h of a load's 16 dims
+    auto put8_k = [&](uint32_t to, int u, int h) __attribute__((always_inline)) {
+        *(lds_u32x4*)(uintptr_t)(to + k8_at + (uint32_t)(2 * IMG_FRAG_BYTES * u + 512 * h)) =
+            __builtin_bit_cast(u32x4, widen(kr8[u][2 * h], kr8[u][2 * h + 1], scale8(ksc)));
+    };
+    auto put8_v = [&](uint32_t to, int u, int h) __attribute__((always_inline)) {
+        *(lds_u32x4*)(uintptr_t)(to + v8_at + (uint32_t)(2048 * u + 16 * h)) =
+            __builtin_bit_cast(u32x4, widen(vr8[u][2 * h], vr8[u][2 * h + 1], scale8(vsc)));
+    };
+
     // ---- registers (as the key-split kernel's)
     bf16x8 qa[8];
     f32x16 o[4], s[2], negm;
@@ -319,6 +365,28 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     auto slot = [](int x) __attribute__((always_inline)) { return (uint32_t)(x % SLOTS * IMG_TILE_BYTES); };
     // V(0) .. V(E) and K(1) .. K(E + 1)
     auto first_pairs = [&]() __attribute__((always_inline)) {
+        if constexpr (SRC == PAGES8) {   // K(0) as well; the loads of step 1's
+            pages8(tile_of(0), tile_of(0));
+            load8_v(tile_of(0));
+            load8_k(tile_of(0));
+            pages8(tile_of(1), tile_of(1));
+#pragma unroll
+            for (int u = 0; u < L8; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    put8_k(ring, u, h);
+                    put8_v(vring, u, h);
+                }
+            load8_k(tile_of(1));
+            load8_v(tile_of(1));
+            pages8(tile_of(2), tile_of(2));
+#pragma unroll
+            for (int u = 0; u < L8; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) put8_k(ring + slot(1), u, h);
+            load8_k(tile_of(2));
+            return;
+        }
 #pragma unroll
         for (int t = 0; t <= E; ++t) {
             v_page(tile_of(t));
@@ -333,10 +401,12 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     };
     {
         const uint16_t* src = a.q + (int64_t)(sq.t0 + i) * a.q_rs + head * D + 8 * hf;
-        k_page(tile_of(0));
-        const uint64_t kb = k_src(tile_of(0));
+        if constexpr (SRC != PAGES8) {
+            k_page(tile_of(0));
+            const uint64_t kb = k_src(tile_of(0));
 #pragma unroll
-        for (int u = 0; u < LP; ++u) load_k1(kb, ring, u);
+            for (int u = 0; u < LP; ++u) load_k1(kb, ring, u);
+        }
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) qa[ks] = *reinterpret_cast<const bf16x8*>(src + 16 * ks);
         if constexpr (E == 0) first_pairs();   // (more of them at once would keep the first product waiting)
@@ -408,7 +478,16 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     // a step's refills, one load every other slot of its first half: V(t + E) from slot 1 on, then K(t + E + 1) (past the last
     // tile repeats of it, never read); their addresses in the slots before, under the products
     uint64_t src = 0;
+    // (in 8 bits: a piece of V(t), loaded in the step before, every other slot, then its registers' next loads; then K(t + 1).)
     auto refill = [&](int f, int t) __attribute__((always_inline)) {
+        if constexpr (SRC == PAGES8) {
+            constexpr int PIECES = 2 * L8;
+            if (f % 2 == 0 && f / 2 < PIECES) put8_v(vring + slot(t), f / 2 / 2, f / 2 % 2);
+            if (f == 2 * PIECES - 1) load8_v(tile_of(t + 1));
+            if (f % 2 == 0 && f / 2 >= PIECES && f / 2 < 2 * PIECES) put8_k(ring + slot(t + 1), (f / 2 - PIECES) / 2, f / 2 % 2);
+            if (f == 4 * PIECES - 1) load8_k(tile_of(t + 2));
+            return;
+        }
         if (f == 0) src = v_src(tile_of(t + E));
         if (f == 2 * LP) src = k_src(tile_of(t + E + 1));
         if (f % 2 == 1) {
@@ -421,21 +500,34 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
     for (int db = 0; db < 4; ++db) o[db] = f32x16{};
     negm = f32x16{};
-    LR_WAIT_VMCNT(0);
+    if constexpr (SRC == PAGES8) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    else LR_WAIT_VMCNT(0);
     block_barrier();
     if constexpr (E > 0) first_pairs();
+    // the entries of step u + 1's refills (of their loads); what a step's end waits for
+    auto next_pages = [&](int u) __attribute__((always_inline)) {
+        if constexpr (SRC == PAGES8) {
+            pages8(tile_of(u + 2), tile_of(u + 3));
+        } else {
+            v_page(tile_of(u + 1 + E));
+            k_page(tile_of(u + 2 + E));
+        }
+    };
+    auto landed = [&]() __attribute__((always_inline)) {
+        if constexpr (SRC == PAGES8) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        else LR_WAIT_VMCNT(AHEAD);
+    };
     // a wave without rows only loads its share of the tiles (and leaves the clock to the others)
     if (row0 + 32 * wv >= rows) {
         for (int u = 0;; ++u) {
-            v_page(tile_of(u + 1 + E));
-            k_page(tile_of(u + 2 + E));
-            LR_WAIT_VMCNT(AHEAD);
+            next_pages(u);
+            landed();
             block_barrier();
             if (u + 1 >= nsteps) break;
 #pragma unroll
             for (int f = 0; f < 4 * LP; ++f) refill(f, u + 1);
         }
-        LR_WAIT_VMCNT(0);
+        if constexpr (SRC != PAGES8) LR_WAIT_VMCNT(0);
         return;
     }
     {
@@ -453,8 +545,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     }
     // ---- step 0: S of half-tile 1 (K(0), fragments 8-15), P of half-tile 0
     {
-        v_page(tile_of(1 + E));   // (of step 1's refills)
-        k_page(tile_of(2 + E));
+        next_pages(0);
         uint32_t kb = ring + lane16;
         asm volatile("" : "+v"(kb));
         auto rd0 = [&](int f) __attribute__((always_inline)) {
@@ -465,7 +556,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         half_step(s[1], p[1], s[0], p[0], BoolTag<false>{}, [&](int f) __attribute__((always_inline)) {
             rd0(f);
         });
-        LR_WAIT_VMCNT(AHEAD);
+        landed();
         block_barrier();
         if constexpr (E > 0) {
             uint32_t kn = ring + slot(1) + lane16;
@@ -486,10 +577,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
             else fr[f % FR] = frag_at(kb + (f - 8) * IMG_FRAG_BYTES);
         };
         auto rd_a = [&](int f) __attribute__((always_inline)) {
-            if (PAGED && f == 8) {
-                v_page(tile_of(u + 1 + E));
-                k_page(tile_of(u + 2 + E));
-            }
+            if (PAGED && f == 8) next_pages(u);
             if (f < 8) fr[f % FR] = frag_at(kb + (8 + f) * IMG_FRAG_BYTES);
             else if (f < 16) fr[f % FR] = vfrag_at(vb + vfrag_off(f));
             else if (E > 0) fr[f % FR] = frag_at(kn + (f - 16) * IMG_FRAG_BYTES);   // (the next step's first)
@@ -504,7 +592,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         });
         if (special(x, 0)) mask_half(s[0], x, 0);
         half_step(s[1], p[1], s[0], p[0], BoolTag<true>{}, rd_a);
-        LR_WAIT_VMCNT(AHEAD);
+        landed();
         block_barrier();
     }
     // ---- the last half-tile's P and the last value tile's products
@@ -696,6 +784,10 @@ hipError_t launch_packed_wide(const RangeAttnArgs& a, int waves, hipStream_t str
     if (waves == 8) hipLaunchKernelGGL((range_wide_kernel<8, PACKED>), dim3((unsigned)blocks), dim3(512), 0, stream, a);
     else hipLaunchKernelGGL((range_wide_kernel<4, PACKED>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
     return hipGetLastError();
+}
+
+hipError_t launch_range_wide8(const RangeAttnArgs& a, int waves, hipStream_t stream) {
+    return waves == 8 ? launch_waves<8, PAGES8>(a, stream) : launch_waves<4, PAGES8>(a, stream);
 }
 
 hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, int waves, hipStream_t stream) {

@@ -276,7 +276,12 @@ Cut packed_cut(int B, int T, int H, int HK) {
 Cut cache8_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks) {
     const int64_t rows = (int64_t)max_rows * (H / HK), pairs = (int64_t)B * HK;
     const int64_t span = window ? (int64_t)window + max_rows + 1 : max_keys;
-    return cut_small(rows, pairs, tiles_of(max_keys, span, sinks, lr::RANGE_TILE), page_size, true);
+    const int64_t tiles = tiles_of(max_keys, span, sinks, lr::RANGE_TILE);
+    if (rows <= 64 || few_rows(rows, pairs, tiles)) return cut_small(rows, pairs, tiles, page_size, true);
+    const int64_t wide_tiles = tiles_of(max_keys, span, sinks, lr::RANGE_WIDE_TILE);
+    Cut c = cut_wide(rows, pairs, wide_tiles, page_size, pairs % 8 == 0 || pairs >= 64);
+    if (B > 1 && !window) cut_pieces(c, rows, pairs, wide_tiles, page_size);
+    return c;
 }
 // Whether the grid of attn_cache_wide.hip's launch holds its workgroups (attn_cache.hip's counts its own, launch_blocks).
 bool launch_fits(const Cut& c) {
@@ -536,7 +541,8 @@ int lr_cache_attention_f8(const void* q, int64_t q_row_stride, void* out, int64_
     a.k_sc = static_cast<const uint8_t*>(k_scales);
     a.v_sc = static_cast<const uint8_t*>(v_scales);
     a.sc_ps = scale_page_stride;
-    return (int)lr::launch_range8(a, cut.br, reinterpret_cast<hipStream_t>(stream));
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    return (int)(cut.wide ? lr::launch_range_wide8(a, cut.wide, s) : lr::launch_range8(a, cut.br, s));
 }
 
 int lr_cache_append_bf16(const void* q, const void* k, const void* v, int64_t q_row_stride, int64_t k_row_stride,

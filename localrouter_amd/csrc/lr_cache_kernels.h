@@ -82,8 +82,9 @@ hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, int waves, hipS
 // sequence may have.)
 hipError_t launch_packed_attn(const RangeAttnArgs& a, int br, hipStream_t stream);
 hipError_t launch_packed_wide(const RangeAttnArgs& a, int waves, hipStream_t stream);
-// Pages in 8 bits, in blocks of br rows (16 or 32): attn_cache8.hip.
+// Pages in 8 bits: attn_cache8.hip in blocks of br rows (16 or 32), or attn_cache_wide.hip.
 hipError_t launch_range8(const RangeAttnArgs& a, int br, hipStream_t stream);
+hipError_t launch_range_wide8(const RangeAttnArgs& a, int waves, hipStream_t stream);
 
 // cache_rows.hip
 struct CacheAppendArgs {
