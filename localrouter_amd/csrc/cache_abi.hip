@@ -122,7 +122,7 @@ lr::PageArgs page_args(int64_t page, int64_t row, int64_t head, int n_pages, int
 // How a call is cut: the kernel (wide: 0, or the waves of the kernel of attn_cache_wide.hip; br: attn_cache.hip's rows a block) and its
 // blocks over the keys (RangeAttnArgs: nsplit, per, whole, local, nblk, teams, places), the rows of the parts and their flags.
 struct Cut {
-    int wide, br, nsplit, per, nblk, merge_here, by_xcd, teams, places;
+    int wide, br, nsplit, per, nblk, merge_here, by_xcd, teams, places, kh, hw;
     int64_t whole, local, part_rows, flags;   // (blocks of every sequence and kv head: past 32 bits before the launch is refused)
 };
 
@@ -152,8 +152,8 @@ bool few_rows(int64_t rows, int64_t pairs, int64_t tiles) {
 // 16 15.9, 32 18.2). In the same launch / by a second: 24 parts of 4 rows 13.1 / 14.5, 63 of 8 15.4 / 17.5, 32 of 16 20.9 / 22.1, 8 of
 // 20 12.5 / 11.8, 8 of 32 13.4 / 11.9, 2 of 64 19.1 / 16.0.
 // The other kernel: parts of 8 tiles at least, merged by a second launch.
-Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool few = false) {
-    const int64_t br = rows <= 16 ? 16 : few || few_rows(rows, pairs, tiles) ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
+Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
+    const int64_t br = rows <= 16 ? 16 : few_rows(rows, pairs, tiles) ? 32 : rows <= 64 ? 64 : 128, base = (rows + br - 1) / br * pairs;
     const int64_t staged = page_size ? lr::RANGE_STAGED / std::max(1, lr::RANGE_TILE / page_size) : INT_MAX;
     int64_t ns = std::max<int64_t>(1, std::min(256 / base, (tiles + 4) / 8));
     if (br <= 32) {
@@ -272,12 +272,61 @@ Cut packed_cut(int B, int T, int H, int HK) {
     c.nblk = (int)((rows + br - 1) / br);
     return c;
 }
-// Pages in 8 bits (attn_cache8.hip): blocks of 16 or 32 rows.
+// Pages in 8 bits, few rows (attn_cache8.hip): blocks of 16 or 32 rows of hw kv heads, kh waves a head.
+// Batches of one block a sequence and kv head with much to read: equal shares of all tiles, whatever the lengths, for one workgroup a CU
+// of 8 waves and two heads, or of an odd number of heads two of 4 waves and one. Us with whole pairs or parts as below / shares, 32 heads
+// over 8, lengths from half to N: 4 sequences, N 24,000 39.8 / 41.6; 16, 6,000 33.1 / 37.7; 64, 1,500 32.7 / 38.6; 32, 6,000 66.8 / 58.9;
+// 16, 24,000 146 / 121; 64, 6,000 144 / 124, 24,000 558 / 440 (5.5 TB/s); 27 rows, 16 of 6,000 38.9 / 47.7, 40 112 / 104, 20 of 12,000
+// 123 / 98.8.
+// Otherwise parts, as few as cost least (cut_small's costs: what a round takes is the chain of loads and instructions, not the bytes),
+// by 8 waves of one head; of more blocks than CUs by 4, of more than three a CU by 2 of each of two heads, whose rows are next to
+// each other (us with 8 / 4 / 2 x 2: 64 x 300 keys 14.2 / 10.8 / 11.0, 64 x 1,500 35.9 / 32.7 / 35.2, 128 x 1,500 80 / 68 / 61.5, 256 x 1,500
+// 158 / 137 / 129; 32 x 1,500 20.1 / 20.9 / 33.4).
+Cut cut_small8(int64_t rows, int64_t B, int64_t HK, int64_t tiles, int page_size) {
+    Cut c{};
+    c.br = rows <= 16 ? 16 : 32;
+    const int64_t nblk = (rows + c.br - 1) / c.br, base = nblk * B * HK;
+    c.nblk = (int)nblk;
+    c.nsplit = 1;
+    const int64_t staged = lr::RANGE8_STAGED / std::max(1, lr::RANGE_TILE / page_size), paired = HK % 2 ? 1 : 2;
+    if (nblk == 1 && B <= 64 && base * tiles >= 32768 && base * tiles <= MAX_POS) {
+        const int64_t places = paired == 2 ? 256 : 512, share = (base / paired * tiles + places - 1) / places;
+        if (share <= staged) {   // (what a workgroup holds page entries for)
+            c.kh = 4; c.hw = (int)paired;
+            c.places = (int)places;
+            c.per = 4;   // at least so many tiles a share
+            c.merge_here = c.br == 16;
+            c.part_rows = 2 * places * c.br * paired;
+            c.flags = c.merge_here ? 2 * places : 0;
+            return c;
+        }
+    }
+    int64_t ns = 1;
+    c.kh = base <= 256 ? 8 : 4; c.hw = 1;
+    if (base > 768 && paired == 2 && c.br == 16) c.kh = c.hw = 2;
+    if (base <= 256) {
+        auto cost = [&](int64_t n) {
+            const double rounds = (double)(((tiles + n - 1) / n + 7) / 8);
+            if (c.br == 16) return 1.25 * rounds + (n > 1 ? 1.4 + 1.2 * (double)((n + 7) / 8) : 0.0);
+            return 1.4 * rounds + (n > 1 ? 2.4 + 0.18 * (double)n : 0.0);
+        };
+        const int64_t most = std::max<int64_t>(1, std::min(256 / base, (tiles + 7) / 8));
+        for (int64_t n = 2; n <= most; ++n)
+            if (cost(n) < cost(ns)) ns = n;
+    }
+    const int64_t per = std::max<int64_t>(1, std::min((tiles + ns - 1) / ns, staged));
+    ns = std::max<int64_t>(1, (tiles + per - 1) / per);
+    c.nsplit = (int)std::min<int64_t>(ns, INT_MAX); c.per = (int)per;
+    c.merge_here = c.br == 16 && ns * std::min<int64_t>(rows, c.br) <= 1024;
+    c.part_rows = ns > 1 ? base * ns * c.br : 0;
+    c.flags = c.merge_here && ns > 1 ? base / c.hw * ns : 0;
+    return c;
+}
 Cut cache8_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, int window, int sinks) {
     const int64_t rows = (int64_t)max_rows * (H / HK), pairs = (int64_t)B * HK;
     const int64_t span = window ? (int64_t)window + max_rows + 1 : max_keys;
     const int64_t tiles = tiles_of(max_keys, span, sinks, lr::RANGE_TILE);
-    if (rows <= 64 || few_rows(rows, pairs, tiles)) return cut_small(rows, pairs, tiles, page_size, true);
+    if (rows <= 64 || few_rows(rows, pairs, tiles)) return cut_small8(rows, B, HK, tiles, page_size);
     const int64_t wide_tiles = tiles_of(max_keys, span, sinks, lr::RANGE_WIDE_TILE);
     Cut c = cut_wide(rows, pairs, wide_tiles, page_size, pairs % 8 == 0 || pairs >= 64);
     if (B > 1 && !window) cut_pieces(c, rows, pairs, wide_tiles, page_size);
@@ -538,11 +587,15 @@ int lr_cache_attention_f8(const void* q, int64_t q_row_stride, void* out, int64_
     const Cut cut = cache8_cut(B, max_rows, max_keys, H, HK, page_size, window, sinks);
     if (!launch_fits(cut) || !workspace_ok(cut, workspace, workspace_bytes, spans, 6)) return ERR_ARGS;
     set_cut(a, workspace, cut);
+    if (!cut.wide) {
+        a.hgroups = HK / cut.hw;
+        a.rcp_hk = lr::rcp_small(a.hgroups);
+    }
     a.k_sc = static_cast<const uint8_t*>(k_scales);
     a.v_sc = static_cast<const uint8_t*>(v_scales);
     a.sc_ps = scale_page_stride;
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    return (int)(cut.wide ? lr::launch_range_wide8(a, cut.wide, s) : lr::launch_range8(a, cut.br, s));
+    return (int)(cut.wide ? lr::launch_range_wide8(a, cut.wide, s) : lr::launch_range8(a, cut.br, cut.kh, cut.hw, s));
 }
 
 int lr_cache_append_bf16(const void* q, const void* k, const void* v, int64_t q_row_stride, int64_t k_row_stride,

@@ -60,7 +60,7 @@ struct RangeAttnArgs {
     uint64_t* flags;
     // rcp_small of the divisors; nblk: blocks of rows a sequence and kv head
     uint32_t rcp_g, rcp_hk, rcp_frame, rcp_split, rcp_nblk;
-    int nblk;
+    int nblk, hgroups;   // attn_cache8.hip: workgroups of several kv heads each, HK / heads of them (rcp_hk its)
 };
 
 // floor(2^32 / d), 2^32 - 1 for d = 1: what the kernels divide by d with.
@@ -82,8 +82,9 @@ hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, int waves, hipS
 // sequence may have.)
 hipError_t launch_packed_attn(const RangeAttnArgs& a, int br, hipStream_t stream);
 hipError_t launch_packed_wide(const RangeAttnArgs& a, int waves, hipStream_t stream);
-// Pages in 8 bits: attn_cache8.hip in blocks of br rows (16 or 32), or attn_cache_wide.hip.
-hipError_t launch_range8(const RangeAttnArgs& a, int br, hipStream_t stream);
+// Pages in 8 bits: attn_cache8.hip in blocks of br rows (16 or 32) of hw kv heads, kh waves each, or attn_cache_wide.hip.
+constexpr int RANGE8_STAGED = 1024;
+hipError_t launch_range8(const RangeAttnArgs& a, int br, int kh, int hw, hipStream_t stream);
 hipError_t launch_range_wide8(const RangeAttnArgs& a, int waves, hipStream_t stream);
 
 // cache_rows.hip

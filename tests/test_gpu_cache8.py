@@ -122,6 +122,85 @@ def test_attention_of_many_rows(ps, tree):
         check_rows(out[rows], *ref_rows(q[rows], k, v, seen), what=f"sequence {b}")
 
 
+SHARES = [
+    # heads, kv heads, tokens, page, window, sinks, tree, long sequences
+    (32, 8, 1, 16, 0, 0, False, 2),
+    (32, 8, 1, 64, 700, 5, False, 3),
+    (8, 8, 2, 32, 0, 0, False, 1),
+    (16, 4, 4, 16, 0, 0, True, 2),
+    (24, 8, 9, 32, 0, 0, True, 2),          # 27 rows of a kv head
+    (24, 8, 9, 16, 300, 4, True, 2),
+    (64, 8, 4, 16, 0, 0, False, 2),         # 32
+    (4, 1, 3, 16, 0, 0, False, 4),          # an odd number of kv heads
+    (21, 7, 5, 32, 0, 0, False, 1),
+    (35, 7, 5, 32, 0, 0, True, 3),          # 25 rows
+]
+
+
+@pytest.mark.parametrize("c", SHARES, ids=lambda c: f"h{c[0]}g{c[1]}n{c[2]}p{c[3]}w{c[4]}t{int(c[6])}l{c[7]}")
+@pytest.mark.parametrize("B", [16, 64])
+def test_attention_of_batches_in_equal_shares(c, B):
+    """Batches sized for long sequences: shares that hold many short pairs, pairs of many shares, sequences without tokens, a page that
+    the pool does not have, NaN behind the sequences; then the same launch over other lengths, captured and replayed; bit for bit again
+    in the same workspace."""
+    H, HK, rows, ps, window, sinks, tree, longs = c
+    rng = random.Random(H + B)
+    news = [rows] + [rng.randrange(0, rows + 1) for _ in range(B - 1)]
+    lens = [3000 + 97 * i for i in range(longs)] + [rng.randrange(rows, 70) for _ in range(B - longs)]
+    news[longs - 1], lens[-1], news[-1] = rows, rows, rows
+    X = Batch8(25, news, lens, ps, HK)
+    used = torch.zeros(X.n_pages, ps, dtype=torch.bool, device="cuda")
+    for b, L in enumerate(lens):
+        at = torch.arange(L, device="cuda")
+        used[X.t[b][at // ps].long(), at % ps] = True
+    X.kp.view(torch.uint8)[~used], X.vp.view(torch.uint8)[~used] = 0x7f, 0xff
+    most = 32 * -(-32768 // (B * HK))
+    table = torch.full((B, max(X.width, -(-most // ps))), -1, dtype=torch.int32, device="cuda")
+    table[:, :X.width] = X.t
+    gone = list(range(2 * ps, 3 * ps)) if longs > 1 else []
+    if gone:
+        table[0, 2] = X.n_pages + 5
+    T = sum(news)
+    q = rnd(X.g, T, H, 128)
+    trees = [random_tree(rng, n) for n in news]
+    kw = dict(max_rows=rows, max_keys=max(most, max(lens)), tree=tree_words(trees, 1) if tree else None, window=window, sinks=sinks)
+    need = cache.attention_f8_ws_bytes(B, T, rows, kw["max_keys"], H, HK, ps, window=window, sinks=sinks)
+    ws = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")
+    out = torch.full((T + 2, H, 128), 9.0, dtype=BF16, device="cuda")
+    lens_t = X.lens.clone()
+    call = lambda: cache.attention_f8(q, X.kp, X.vp, X.ks, X.vs, table, X.starts, lens_t, out[:T], workspace=ws, **kw)
+
+    def check(L):
+        k8, v8 = values(X.kp, X.ks), values(X.vp, X.vs)
+        for b, n in enumerate(news):
+            if not n:
+                continue
+            seen = tree_seen(trees[b], L[b], window, sinks) if tree else chain_seen(n, L[b], window, sinks)
+            if b == 0:
+                seen[:, [j for j in gone if j < L[b]]] = False
+            p = torch.arange(L[b], device="cuda")
+            page = X.t[b][p // ps].long()
+            r = slice(X.st[b], X.st[b] + n)
+            check_rows(out[r], *ref_rows(q[r], k8[page, p % ps], v8[page, p % ps], seen), what=f"sequence {b}")
+        assert (out[T:] == 9.0).all() and (ws[need:] == 255).all()
+
+    call()
+    check(lens)
+    first = out.clone()
+    call()
+    assert torch.equal(out, first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for L in ([max(n, x // 3) for n, x in zip(news, lens)], lens):
+        lens_t.copy_(ints(L))
+        out[:T].fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(L)
+    assert torch.equal(out, first)
+
+
 @pads
 @pytest.mark.parametrize("heads", [2, 40])
 def test_masks_that_leave_a_row_empty(heads, pad):
