@@ -30,6 +30,7 @@ const sources = [_]Source{
     .{ .file = "cache_abi.hip" },
     .{ .file = "attn_cache8.hip" },
     .{ .file = "cache8_rows.hip" },
+    .{ .file = "attn_packed.hip", .extra = &.{ "-mllvm", "-pragma-unroll-threshold=1000000" } },
 };
 
 /// hipcc flags of every device source: gfx950 only, no packed-fp32 instruction selection (v_pk_*_f32 are left to

@@ -22,7 +22,8 @@ CSRC = PKG / "csrc"
 LIB = PKG / "liblr_attn.so"
 SOURCES = ["attn_fwd.hip", "attn_stream.hip", "attn_keysplit.hip", "kv_image.hip", "rms_rope.hip", "int8_attn.hip",
            "keys.hip", "lr_abi.hip", "mmdit.hip", "attn_cache.hip", "attn_cache_wide.hip",
-           "cache_rows.hip", "cache_abi.hip", "attn_cache8.hip", "cache8_rows.hip", "rope_host.cpp"]
+           "cache_rows.hip", "cache_abi.hip", "attn_cache8.hip", "cache8_rows.hip",
+           "attn_packed.hip", "rope_host.cpp"]
 # libraries the shared object links: hipBLASLt for the MMDiT block's projections and MLP
 LIBS = ["-L/opt/rocm/lib", "-lhipblaslt"]
 ARCH = "gfx950"
@@ -43,7 +44,8 @@ HIPCC_FLAGS = [
 # `#pragma unroll`, and a partly unrolled step would index its register arrays at run time
 EXTRA_FLAGS = {"attn_stream.hip": ["-mllvm", "-pragma-unroll-threshold=1000000"],
                "attn_keysplit.hip": ["-mllvm", "-pragma-unroll-threshold=1000000"],
-               "attn_cache_wide.hip": ["-mllvm", "-pragma-unroll-threshold=1000000"]}
+               "attn_cache_wide.hip": ["-mllvm", "-pragma-unroll-threshold=1000000"],
+               "attn_packed.hip": ["-mllvm", "-pragma-unroll-threshold=1000000"]}
 
 # Scratch (spill) budget per kernel, bytes per lane. The streaming attention kernel and the INT8 attention kernel count
 # their direct global->LDS refills with explicit `s_waitcnt vmcnt(N)`; a scratch access among those loads would be

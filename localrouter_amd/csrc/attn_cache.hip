@@ -342,7 +342,12 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
     const int at = div_small(blockIdx.x, a.nsplit, a.rcp_split), split = blockIdx.x - at * a.nsplit;
     int blk = div_small(at, a.HK, a.rcp_hk), b = blockIdx.y;
     const int hk = at - blk * a.HK;
-    if (SRC == PACKED && !packed_block<BR>(a, blk, b, blk)) return;
+    Seq sq;
+    if constexpr (SRC == PACKED) {
+        PackedBlocks<BR> pb;
+        pb.init(a);
+        if (!pb.at(a, blk, a.nblk, sq, blk)) return;
+    }
     // without a window a part's entries do not depend on the sequence: they are read beside its numbers
     int early = -1;
     const int per_tile = PAGED ? max(1, BT >> a.pg.shift) : 1;
@@ -351,7 +356,7 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
         const int j = BT * (split * a.per + tid / per_tile) + (tid % per_tile << a.pg.shift);
         if (j >> a.pg.shift < a.pg.table_pages) early = a.pg.table[(int64_t)b * a.pg.table_rs + (j >> a.pg.shift)];
     }
-    const Seq sq = seq_of<SRC>(a, b);
+    if constexpr (SRC != PACKED) sq = seq_of<SRC>(a, b);
     const int row0 = blk * BR, rows = max(sq.n, 0) * a.G;   // (at most 2^30: the host checks)
     if (row0 >= rows) return;
     const int i_first = div_small(row0, a.G, a.rcp_g), i_last = div_small(min(rows, row0 + BR) - 1, a.G, a.rcp_g);

@@ -1,5 +1,5 @@
 // The ranged attention (attn_cache.hip) of calls with many rows of a kv head: chunks, frames and large trees, where the matrix
-// products bound it. The same contract; the loop is that of the key-split kernel (attn_keysplit.hip): a half-step of 16 MFMA
+// products bound it, over rows, pages and pages of 8 bits. The same contract; the loop is that of the key-split kernel (attn_keysplit.hip): a half-step of 16 MFMA
 // slots runs the next half-tile's scores, the previous one's products and this one's exponentials. A workgroup is 128 rows
 // (tokens x the query heads of one kv head), four waves of 32 rows over a ring of two key tiles and two value tiles; two
 // workgroups share a CU, one's start, end and waits under the other's products. Long calls that fill the CUs take 256 rows, eight
@@ -15,6 +15,9 @@
 //  * Pages hold at least 16 rows, so the 16 rows of a value load are in one page, and the 32 rows of a key load in at most
 //    two: scalar bases from the staged page-table entries.
 //  * A row that overflowed its reference, or met an infinity or NaN, is computed again over the keys that it sees.
+//  * Pages of 8 bits: the tiles go through registers, loaded a step ahead, and are converted on their way into LDS, once for all the
+//    workgroup's rows (in the products' place each wave would convert every fragment): 32 conversions and 8 LDS writes a wave and
+//    step beside 32 MFMA. 2,048 tokens x 32 heads over 8 behind 6,000 positions 252 us, over bf16 pages 232.
 #include "lr_common.h"
 #include "block_order.h"
 #include "lr_cache_kernels.h"
@@ -31,18 +34,8 @@ constexpr int FR = 4;             // fragment ring entries
 static_assert(IMG_TILE_KEYS == RANGE_WIDE_TILE, "the host's cut");
 
 #include "attn_tiles.inc"
+#include "dma1.inc"
 #include "range_attn.inc"
-
-// One 1 KB direct load, global -> LDS: lane l's 16 bytes come from gaddr + voff + OFF and land at lds + 16 l (the instruction
-// offset applies to both addresses).
-template <int OFF>
-__device__ __forceinline__ void dma1_at(uint64_t gaddr, uint32_t voff, uint32_t lds) {
-    LR_ASM_M0_BEGIN
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3" ::"v"(voff), "s"(gaddr), "s"(lds - OFF),
-                 "n"(OFF)
-                 : "memory", "m0");
-    LR_ASM_M0_END
-}
 
 // The sequence of rank `rank` when the batch is ordered longest first (B <= 64), so that the last workgroups to start are
 // short ones.
@@ -78,11 +71,6 @@ __device__ __forceinline__ bool block_of(const RangeAttnArgs& a, int id, int& b,
         cut = xcd * (a.local - a.whole) + q;
     }
     b = 0;
-    if constexpr (SRC == PACKED) {   // every XCD works on its own heads, or with fewer than 8 shares one with others
-        const int u = div_small(idx, a.HK, a.rcp_hk);
-        hk = idx - u * a.HK;
-        return packed_block<32 * QW>(a, u, b, blk);
-    }
     if (PAGED || a.by_xcd) {
         int pair = div_small(idx, a.nblk, a.rcp_nblk);
         blk = a.nblk - 1 - (idx - pair * a.nblk);
@@ -267,7 +255,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         if constexpr (PAGED)
             return (uint64_t)(((int64_t)__builtin_amdgcn_readfirstlane(max(entry, 0)) * a.pg.ps +
                                (int64_t)(j & ((1 << tl.shift) - 1)) * rs) * 2);
-        return (uint64_t)((int64_t)(tl.row0 + j) * rs * 2);
+        return (uint64_t)((int64_t)j * rs * 2);
     };
     // the page-table entries of the next refills, read a half-step ahead (read where they are used, each kept the wave's
     // products waiting for LDS)
@@ -777,14 +765,6 @@ hipError_t launch_waves(const RangeAttnArgs& a, hipStream_t stream) {
 }
 
 }  // namespace
-
-hipError_t launch_packed_wide(const RangeAttnArgs& a, int waves, hipStream_t stream) {
-    const int64_t blocks = ((int64_t)a.T * a.G / (32 * waves) + a.B) * a.HK;
-    if (blocks > RANGE_MAX_BLOCKS) return hipErrorInvalidValue;
-    if (waves == 8) hipLaunchKernelGGL((range_wide_kernel<8, PACKED>), dim3((unsigned)blocks), dim3(512), 0, stream, a);
-    else hipLaunchKernelGGL((range_wide_kernel<4, PACKED>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
-    return hipGetLastError();
-}
 
 hipError_t launch_range_wide8(const RangeAttnArgs& a, int waves, hipStream_t stream) {
     return waves == 8 ? launch_waves<8, PAGES8>(a, stream) : launch_waves<4, PAGES8>(a, stream);

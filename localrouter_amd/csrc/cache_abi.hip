@@ -261,13 +261,26 @@ Cut cache_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, i
     }
     return cut_small(rows, pairs, tiles, page_size);
 }
-// Sequences packed end to end: blocks of 16 and 32 rows of few rows in all, else workgroups of four or eight waves.
+// Sequences packed end to end; the host knows how many and how many rows in all. Blocks of 16 rows (attn_cache.hip, whose eight waves
+// share a block's keys) while all of them are resident at once; else blocks of 32 rows or the stream of blocks of 128 (attn_packed.hip),
+// by what they cost when the sequences are of one length: a round of blocks of 32 starts and ends in ~5 us and takes 0.75 per 256
+// keys of its longest; the blocks of 128 take ~6 and 1.2 per 64 keys of the longest, or what the GPU does in all. Us with 16 / 32 / 128
+// rows: one of 1,000 tokens, one head, 9.2 / 11.7 / 25.7; one of 300, 32 heads over 8, 14.0 / 11.2 / 13.2; 891 tokens of 2, 32 over 8, 37
+// / 28 / 19; 4,017 of 2, 4 over 1, 41 / 28 / 60; one of 7,000, 4 over 1, 149 / 91 / 141, 8 over 8 273 / 173 / 156; 611 of 18, 16 over 8,
+// 12.5 / 11.0 / 7.8.
+// Blocks of 256 where there are many and each XCD has kv heads of its own, whose keys its workgroups move half as often (us with 128 /
+// 256 rows: 10,900 tokens of 19, 32 over 8, 120 / 116; 58,000 of 60, 16 over 8, 441 / 414; one of 4,096, 32 over 8, 147 / 139; of 53,000 of 38,
+// 8 over 8, 283 / 289; 43,000 of 27, 8 over 2, 217 / 223).
 Cut packed_cut(int B, int T, int H, int HK) {
-    const int64_t rows = (int64_t)T * (H / HK);
+    const int64_t G = H / HK, rows = (int64_t)T * G;
+    auto blocks = [&](int64_t br) { return (rows / br + B) * HK; };
     Cut c{};
     c.nsplit = 1; c.per = MAX_POS;
-    if (rows * HK <= 16384) c.br = rows <= 16 * (int64_t)B ? 16 : 32;
-    else c.wide = rows * HK >= 256 * 2048 ? 8 : 4;
+    const double len = (double)T / B, t32 = 1.1 * (double)blocks(32) / 256 * (5.0 + 0.0029 * len),
+                 t128 = std::max(6.0 + 1.2 / 64 * len, (double)blocks(128) / 512 * (6.0 + 1.75 / 128 * len));
+    if (blocks(16) <= 256) c.br = 16;
+    else if (t32 <= t128) c.br = 32;
+    else c.wide = blocks(128) >= 1024 && HK % 8 == 0 && G > 1 ? 8 : 4;
     const int64_t br = c.wide ? 32 * c.wide : c.br;
     c.nblk = (int)((rows + br - 1) / br);
     return c;

@@ -1,5 +1,5 @@
-// Internal launch interface between the C ABI of the paged cache and the windowed attention (cache_abi.hip) and their
-// kernels (attn_cache.hip, attn_cache_wide.hip, cache_rows.hip).
+// Internal launch interface between the C ABI of the paged caches, the windowed and the packed attention (cache_abi.hip) and their
+// kernels (attn_cache.hip, attn_cache_wide.hip, attn_cache8.hip, attn_packed.hip, cache_rows.hip, cache8_rows.hip).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -52,6 +52,7 @@ struct RangeAttnArgs {
     // attn_cache_wide.hip: the blocks from number `whole` on, in the order in which an XCD's workgroups start (`local` blocks an
     // XCD, or with by_xcd 0 in all: see its kernel), `per` tiles a part or, per 0, equal parts; slots [block][row][part], merged
     // by a second launch.
+    // attn_cache8.hip, places > 0: `places` workgroups with equal shares of all tiles, at least `per`; two slots each.
     // teams > 0 (attn_cache_wide.hip): cut by the sequences' own lengths into pieces of equal length, up to `teams` of them an XCD
     // whose `places` workgroups are resident at once.
     int nsplit, per, whole, local, merge_here, by_xcd, teams, places;
@@ -78,8 +79,8 @@ constexpr int64_t RANGE_MAX_BLOCKS = 1 << 22;    // workgroups a launch: a grid'
 // attn_cache_wide.hip in workgroups of `waves` waves of 32 rows (the cut's tiles are each kernel's own).
 hipError_t launch_range_attn(const RangeAttnArgs& a, bool paged, int br, hipStream_t stream);
 hipError_t launch_range_wide(const RangeAttnArgs& a, bool paged, int waves, hipStream_t stream);
-// Sequences packed end to end, whole: the same kernels, in blocks of br rows (16 or 32) or of `waves` waves. (nblk: the most blocks a
-// sequence may have.)
+// Sequences packed end to end: attn_cache.hip's kernel of few rows in blocks of br (16 or 32), or attn_packed.hip's workgroups of `waves`
+// waves of 32 rows. (nblk: the most blocks a sequence may have.)
 hipError_t launch_packed_attn(const RangeAttnArgs& a, int br, hipStream_t stream);
 hipError_t launch_packed_wide(const RangeAttnArgs& a, int waves, hipStream_t stream);
 // Pages in 8 bits: attn_cache8.hip in blocks of br rows (16 or 32) of hw kv heads, kh waves each, or attn_cache_wide.hip.
