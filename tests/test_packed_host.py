@@ -21,7 +21,7 @@ def _packed(**kw):
     dict(q=0), dict(k=0), dict(v=0), dict(out=0), dict(starts=0), dict(starts=S + 2), dict(B=0), dict(B=65536), dict(T=0), dict(T=(1 << 28) + 1),
     dict(H=9), dict(HK=0), dict(H=0), dict(window=-1), dict(sinks=-1), dict(scale=0.0), dict(scale=float("inf")), dict(q=Q + 8),
     dict(qrs=1000), dict(krs=128), dict(vrs=252), dict(ors=1020), dict(krs=1 << 23), dict(vrs=1 << 23), dict(out=Q), dict(out=K + 4096),
-    dict(out=V + 256), dict(T=1 << 28, HK=8, H=32, qrs=4096, ors=4096, krs=1024, vrs=1024, q=1 << 50, k=2 << 50, v=3 << 50, out=4 << 50),
+    dict(out=V + 256),
 ], ids=str)
 def test_packed_refuses(kw):
     assert _packed(**kw) == BAD
