@@ -143,6 +143,83 @@ struct Pieces {
     }
 };
 
+// Blocks in equal shares (a.places without a.teams): the blocks of an XCD's pairs, each counted as its sequence's tiles, lie end to
+// end and are cut every Q tiles, so that each place has Q tiles of work however many blocks there are. Number x < PLACES: the piece
+// that starts at the cut x Q; PLACES + m: the one that starts with block m, unless a cut is there (m < 128: the host checks it).
+// Longest first, as Pieces.
+struct BlockPieces {
+    static constexpr int PLACES = RANGE_WIDE_PLACES, E = 3;   // pieces a lane
+    int P, tiles, blocks, end, last, Q;        // pairs an XCD; lane j's pair: a block's tiles, its blocks, where tiles and blocks end
+    int pos[E], len[E];
+
+    template <int KBM>
+    __device__ __forceinline__ void init(const RangeAttnArgs& a, int xcd) {
+        const int lane = threadIdx.x & 63;
+        P = a.B * a.HK >> 3;
+        const Seq sq = seq_of<PAGES8>(a, div_small(min(lane, P - 1) * 8 + xcd, a.HK, a.rcp_hk));
+        const int rows = lane < P ? max(sq.n, 0) * a.G : 0;
+        tiles = max(1, (sq.end + IMG_TILE_KEYS - 1) / IMG_TILE_KEYS);
+        blocks = (rows + KBM - 1) / KBM;
+        end = tiles * blocks;   // (the host checks that all of them fit)
+        last = blocks;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int x = __shfl_up(end, d, 64), y = __shfl_up(last, d, 64);
+            end += lane >= d ? x : 0;
+            last += lane >= d ? y : 0;
+        }
+        Q = max(16, (__builtin_amdgcn_readlane(end, 63) + PLACES - 1) / PLACES);   // (shorter pieces cost more than they spread)
+    }
+    // pair j's block number nth, from the one with the most keys on: where it begins
+    __device__ __forceinline__ int begin(int j, int nth) const {
+        return __builtin_amdgcn_readlane(end, j) - (__builtin_amdgcn_readlane(blocks, j) - nth) * __builtin_amdgcn_readlane(tiles, j);
+    }
+    __device__ __forceinline__ void cut() {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int at = i == 0 ? lane * Q : (i - 1) * 64 + lane;
+            int j = 0;
+            for (int k = 0; k < P; ++k) j += __builtin_amdgcn_readlane(i == 0 ? end : last, k) <= at;
+            const bool is = j < P;
+            j = min(j, P - 1);
+            const int n = __shfl(tiles, j, 64), all = __shfl(blocks, j, 64), e = __shfl(end, j, 64);
+            const int nth = i == 0 ? all - (e - at + n - 1) / n : all - (__shfl(last, j, 64) - at), from = e - (all - nth) * n;
+            pos[i] = i == 0 ? at : from;
+            len[i] = is && (i == 0 || from % Q != 0) ? min(from + n, (pos[i] / Q + 1) * Q) - pos[i] : 0;
+        }
+    }
+    // the piece of rank r: its number and where it starts and ends
+    __device__ __forceinline__ bool rank(int r, int& x, int& p0, int& p1) const {
+        const int lane = threadIdx.x & 63;
+        int key[E], found = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) key[i] = len[i] > 0 ? len[i] << 8 | (255 - i * 64 - lane) : 0;
+        for (int bit = 1 << 24; bit; bit >>= 1) {   // the greatest value that more than r of them reach
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < E; ++i) n += __popcll(__builtin_amdgcn_ballot_w64(key[i] >= (found | bit)));
+            found |= n > r ? bit : 0;
+        }
+        if (found == 0) return false;
+        x = 255 - (found & 255);
+        p0 = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int at = __builtin_amdgcn_readlane(pos[i], x & 63);
+            p0 = x >> 6 == i ? at : p0;
+        }
+        p1 = p0 + (found >> 8);
+        return true;
+    }
+    // the pair and the block in which tile p0 lies
+    __device__ __forceinline__ void block(int p0, int& j, int& nth) const {
+        j = __popcll(__builtin_amdgcn_ballot_w64(end <= p0));
+        const int n = __builtin_amdgcn_readlane(tiles, j);
+        nth = __builtin_amdgcn_readlane(blocks, j) - (__builtin_amdgcn_readlane(end, j) - p0 + n - 1) / n;
+    }
+};
+
 template <int QW, int SRC>
 __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu(2, 2))) void range_wide_kernel(RangeAttnArgs a) {
     constexpr int KBM = 32 * QW;                        // rows per block
@@ -166,8 +243,24 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, hf = lane >> 5;
 
-    int b, hk, blk, split, cut, px0 = 0, px1 = 0;
-    if (PAGED && a.teams) {
+    int b, hk, blk, split, cut, px0 = 0, px1 = 0;   // (px1: of a piece)
+    if (SRC == PAGES8 && QW == 4 && a.places && !a.teams) {
+        const int xcd = blockIdx.x & 7;
+        BlockPieces pc;
+        pc.template init<KBM>(a, xcd);
+        pc.cut();
+        int x, p0, p1, j, nth;
+        if (!pc.rank(blockIdx.x >> 3, x, p0, p1)) return;
+        pc.block(p0, j, nth);
+        const int pair = 8 * j + xcd, from = pc.begin(j, nth);
+        px0 = p0 - from;
+        px1 = p1 - from;
+        b = div_small(pair, a.HK, a.rcp_hk);
+        hk = pair - b * a.HK;
+        blk = __builtin_amdgcn_readlane(pc.blocks, j) - 1 - nth;
+        split = 0;
+        cut = px1 - px0 == __builtin_amdgcn_readlane(pc.tiles, j) ? -1 : xcd * (BlockPieces::PLACES + pc.P * a.nblk) + x;
+    } else if (PAGED && a.teams) {
         const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3, r = div_small(idx, a.nblk, a.rcp_nblk);
         Pieces pc;
         pc.template init<KBM>(a, xcd);
@@ -194,7 +287,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     if (row0 >= rows) return;
     TileList<BT, SRC> tl;
     tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + KBM) - 1, a.G, a.rcp_g));
-    if (PAGED && a.teams) {
+    if (PAGED && (SRC == PAGES8 ? px1 : a.teams) > 0) {
         tl.x0 = px0;
         tl.x1 = min(tl.total, px1);
     } else if (PAGED || cut >= 0) tl.part(split, a.per ? a.per : div_small(tl.total + a.nsplit - 1, a.nsplit, a.rcp_split));
@@ -742,6 +835,23 @@ __global__ __launch_bounds__(256) void range_pieces_merge_kernel(RangeAttnArgs a
     });
 }
 
+// The same of shares: workgroup (pair, block, 32 rows).
+template <int QW>
+__global__ __launch_bounds__(256) void range_shares_merge_kernel(RangeAttnArgs a) {
+    const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3, c = at / QW, j = div_small(c, a.nblk, a.rcp_nblk), nth = c - j * a.nblk;
+    BlockPieces pc;
+    pc.template init<32 * QW>(a, xcd);
+    const int blocks = __builtin_amdgcn_readlane(pc.blocks, j);
+    if (nth >= blocks) return;
+    const int p0 = pc.begin(j, nth), first = p0 / pc.Q, parts = (p0 + __builtin_amdgcn_readlane(pc.tiles, j) - 1) / pc.Q - first + 1;
+    if (parts <= 1) return;   // (the attention wrote its rows)
+    const int pair = 8 * j + xcd, b = div_small(pair, a.HK, a.rcp_hk), hk = pair - b * a.HK;
+    const int x0 = p0 % pc.Q ? BlockPieces::PLACES + __builtin_amdgcn_readlane(pc.last, j) - blocks + nth : first;
+    merge_rows<QW>(a, seq_of<PAGES8>(a, b), hk, blocks - 1 - nth, at % QW, parts, [&](int x) {
+        return (int64_t)xcd * (BlockPieces::PLACES + pc.P * a.nblk) + (x == 0 ? x0 : first + x);
+    });
+}
+
 template <int QW, int SRC>
 hipError_t launch_waves(const RangeAttnArgs& a, hipStream_t stream) {
     if constexpr (paged(SRC))
@@ -751,6 +861,15 @@ hipError_t launch_waves(const RangeAttnArgs& a, hipStream_t stream) {
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
             hipLaunchKernelGGL(range_pieces_merge_kernel<QW>, dim3((unsigned)merge), dim3(256), 0, stream, a);
+            return hipGetLastError();
+        }
+    if constexpr (SRC == PAGES8 && QW == 4)
+        if (a.places) {
+            const int64_t pairs = (int64_t)a.B * a.HK, blocks = 8 * BlockPieces::PLACES + pairs * a.nblk;
+            hipLaunchKernelGGL((range_wide_kernel<QW, SRC>), dim3((unsigned)blocks), dim3(64 * QW), 0, stream, a);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+            hipLaunchKernelGGL(range_shares_merge_kernel<QW>, dim3((unsigned)(pairs * a.nblk * QW)), dim3(256), 0, stream, a);
             return hipGetLastError();
         }
     const int xcds = a.by_xcd ? 8 : 1;

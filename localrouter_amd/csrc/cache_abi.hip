@@ -343,6 +343,20 @@ Cut cache8_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, 
     const int64_t wide_tiles = tiles_of(max_keys, span, sinks, lr::RANGE_WIDE_TILE);
     Cut c = cut_wide(rows, pairs, wide_tiles, page_size, pairs % 8 == 0 || pairs >= 64);
     if (B > 1 && !window) cut_pieces(c, rows, pairs, wide_tiles, page_size);
+    // Blocks in equal shares (attn_cache_wide.hip, BlockPieces). An XCD has room for 64 workgroups of 4 waves: 44 blocks leave 20 of
+    // the places empty, 66 leave 62 of them in the second round. Cut evenly, 44 blocks of 89 tiles take 171 us instead of 186 (35 of
+    // 125: 185 and 239; 66 of 141: 346 and 454; 94 of 97: 325 and 350). Rounds that are nearly full gain nothing by it (57 of 313: 651
+    // and 630; 122 of 250: 1,015 and 949), nor do few tiles (44 of 47: 109 and 108). Blocks count as equally long: chunks behind three
+    // times as many positions as their own, or more.
+    const int64_t P = pairs / 8, nblk = (rows + 127) / 128, blocks = P * nblk, all = blocks * wide_tiles;
+    const int64_t places = lr::RANGE_WIDE_PLACES, share = std::max<int64_t>(16, (all + places - 1) / places), full = (blocks + places - 1) / places * places;
+    if (pairs % 8 == 0 && P <= 64 && !window && !c.teams && blocks > 32 && blocks <= 128 && 10 * full >= 13 * blocks && wide_tiles >= 64 &&
+        4 * (int64_t)max_rows <= max_keys && std::min(share, wide_tiles) * std::max(1, lr::RANGE_WIDE_TILE / page_size) <= lr::RANGE_WIDE_STAGED) {
+        c = Cut{};
+        c.wide = 4; c.nblk = (int)nblk; c.by_xcd = 1;
+        c.nsplit = 1; c.places = (int)places;
+        c.part_rows = 8 * (places + blocks) * 128;
+    }
     return c;
 }
 // Whether the grid of attn_cache_wide.hip's launch holds its workgroups (attn_cache.hip's counts its own, launch_blocks).

@@ -122,6 +122,81 @@ def test_attention_of_many_rows(ps, tree):
         check_rows(out[rows], *ref_rows(q[rows], k, v, seen), what=f"sequence {b}")
 
 
+BLOCK_SHARES = [
+    # heads, kv heads, tokens, lengths, page, tree, of sizes for
+    (128, 8, [290], [4500], 16, False, (290, 4500)),
+    (128, 8, [600], [5555], 32, False, (600, 5555)),          # more blocks than an XCD has places
+    (64, 8, [320, 300], [5700, 5200], 16, False, (320, 5700)),
+    (56, 8, [320, 0], [4999, 70], 64, False, (350, 9000)),    # a sequence without tokens, fewer positions than the call is sized for
+    (56, 8, [3, 345], [3, 700], 64, False, (350, 9000)),      # short shares: several of them, and the end of the row of blocks, empty
+    (72, 4, [277, 241], [277, 4100], 128, False, (280, 4100)),   # a prompt without context
+    (64, 8, [300, 320], [4700, 400], 16, True, (320, 4800)),
+    (64, 8, [205, 1, 190], [5100, 4000, 190], 32, True, (205, 5100)),
+]
+
+
+@pytest.mark.parametrize("c", BLOCK_SHARES, ids=lambda c: f"{len(c[2])}seq{max(c[2])}of{max(c[3])}h{c[0]}g{c[1]}p{c[4]}t{int(c[5])}")
+def test_attention_of_chunks_in_equal_shares(c):
+    """Blocks of rows that do not fill the chip's places evenly, cut into equal shares of their tiles: some tokens of each sequence
+    checked, a page that the pool does not have, NaN behind the sequences; bit for bit again, and as rows of a captured call over other
+    lengths."""
+    H, HK, news, lens, ps, tree, (rows, most) = c
+    rng = random.Random(H)
+    X = Batch8(26, news, lens, ps, HK)
+    used = torch.zeros(X.n_pages, ps, dtype=torch.bool, device="cuda")
+    for b, L in enumerate(lens):
+        at = torch.arange(L, device="cuda")
+        used[X.t[b][at // ps].long(), at % ps] = True
+    X.kp.view(torch.uint8)[~used], X.vp.view(torch.uint8)[~used] = 0x7f, 0xff
+    table = torch.full((len(news), max(X.width, -(-most // ps))), -1, dtype=torch.int32, device="cuda")
+    table[:, :X.width] = X.t
+    gone = list(range(ps, 2 * ps)) if lens[0] > 2 * ps else []
+    if gone:
+        table[0, 1] = X.n_pages + 5
+    T = sum(news)
+    q = rnd(X.g, T, H, 128)
+    trees = [random_tree(rng, n) for n in news]
+    kw = dict(max_rows=rows, max_keys=most, tree=tree_words(trees, (rows + 63) // 64) if tree else None)
+    need = cache.attention_f8_ws_bytes(len(news), T, rows, most, H, HK, ps)
+    assert need
+    ws = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")
+    out = torch.full((T + 2, H, 128), 9.0, dtype=BF16, device="cuda")
+    lens_t = X.lens.clone()
+    call = lambda: cache.attention_f8(q, X.kp, X.vp, X.ks, X.vs, table, X.starts, lens_t, out[:T], workspace=ws, **kw)
+
+    def check(L):
+        k8, v8 = values(X.kp, X.ks), values(X.vp, X.vs)
+        for b, n in enumerate(news):
+            if not n:
+                continue
+            at = sorted({0, n // 3, n // 2, n - 1})
+            seen = (tree_seen(trees[b], L[b]) if tree else chain_seen(n, L[b]))[at]
+            if b == 0:
+                seen[:, [j for j in gone if j < L[b]]] = False
+            p = torch.arange(L[b], device="cuda")
+            page = X.t[b][p // ps].long()
+            r = [X.st[b] + i for i in at]
+            check_rows(out[r], *ref_rows(q[r], k8[page, p % ps], v8[page, p % ps], seen), what=f"sequence {b}")
+        assert (out[T:] == 9.0).all() and (ws[need:] == 255).all() and out.isfinite().all()
+
+    call()
+    check(lens)
+    first = out.clone()
+    out[:T].fill_(7.0)
+    call()
+    assert torch.equal(out, first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for L in ([max(n, x // 3) for n, x in zip(news, lens)], lens):
+        lens_t.copy_(ints(L))
+        out[:T].fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(L)
+    assert torch.equal(out, first)
+
+
 SHARES = [
     # heads, kv heads, tokens, page, window, sinks, tree, long sequences
     (32, 8, 1, 16, 0, 0, False, 2),
