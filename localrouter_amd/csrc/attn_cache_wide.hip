@@ -143,16 +143,15 @@ struct Pieces {
     }
 };
 
-// Blocks in equal shares (a.places without a.teams): the blocks of an XCD's pairs, each counted as its sequence's tiles, lie end to
-// end and are cut every Q tiles, so that each place has Q tiles of work however many blocks there are. Number x < PLACES: the piece
-// that starts at the cut x Q; PLACES + m: the one that starts with block m, unless a cut is there (m < 128: the host checks it).
+// Blocks of 8-bit pages in equal shares (a.places without a.teams): the blocks of an XCD's pairs, each counted as its sequence's tiles,
+// lie end to end and are cut every Q tiles, so that each place has Q tiles of work however many blocks there are. Number x < PLACES: the
+// piece that starts at the cut x Q; PLACES + m: the one that starts with block m, unless a cut is there (m < 128: the host checks it).
 // Longest first, as Pieces.
 struct BlockPieces {
-    static constexpr int PLACES = RANGE_WIDE_PLACES, E = 3;   // pieces a lane
+    static constexpr int KBM = 256, PLACES = RANGE_WIDE_PLACES, E = 3;   // pieces a lane
     int P, tiles, blocks, end, last, Q;        // pairs an XCD; lane j's pair: a block's tiles, its blocks, where tiles and blocks end
     int pos[E], len[E];
 
-    template <int KBM>
     __device__ __forceinline__ void init(const RangeAttnArgs& a, int xcd) {
         const int lane = threadIdx.x & 63;
         P = a.B * a.HK >> 3;
@@ -209,6 +208,7 @@ struct BlockPieces {
             const int at = __builtin_amdgcn_readlane(pos[i], x & 63);
             p0 = x >> 6 == i ? at : p0;
         }
+        x = x < 64 ? x : PLACES + x - 64;   // (a lane's first entry holds a cut, the others blocks)
         p1 = p0 + (found >> 8);
         return true;
     }
@@ -244,10 +244,10 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     const int n = lane & 31, hf = lane >> 5;
 
     int b, hk, blk, split, cut, px0 = 0, px1 = 0;   // (px1: of a piece)
-    if (SRC == PAGES8 && QW == 4 && a.places && !a.teams) {
+    if (SRC == PAGES8 && QW == 8 && a.places && !a.teams) {
         const int xcd = blockIdx.x & 7;
         BlockPieces pc;
-        pc.template init<KBM>(a, xcd);
+        pc.init(a, xcd);
         pc.cut();
         int x, p0, p1, j, nth;
         if (!pc.rank(blockIdx.x >> 3, x, p0, p1)) return;
@@ -840,7 +840,7 @@ template <int QW>
 __global__ __launch_bounds__(256) void range_shares_merge_kernel(RangeAttnArgs a) {
     const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3, c = at / QW, j = div_small(c, a.nblk, a.rcp_nblk), nth = c - j * a.nblk;
     BlockPieces pc;
-    pc.template init<32 * QW>(a, xcd);
+    pc.init(a, xcd);
     const int blocks = __builtin_amdgcn_readlane(pc.blocks, j);
     if (nth >= blocks) return;
     const int p0 = pc.begin(j, nth), first = p0 / pc.Q, parts = (p0 + __builtin_amdgcn_readlane(pc.tiles, j) - 1) / pc.Q - first + 1;
@@ -863,7 +863,7 @@ hipError_t launch_waves(const RangeAttnArgs& a, hipStream_t stream) {
             hipLaunchKernelGGL(range_pieces_merge_kernel<QW>, dim3((unsigned)merge), dim3(256), 0, stream, a);
             return hipGetLastError();
         }
-    if constexpr (SRC == PAGES8 && QW == 4)
+    if constexpr (SRC == PAGES8 && QW == 8)
         if (a.places) {
             const int64_t pairs = (int64_t)a.B * a.HK, blocks = 8 * BlockPieces::PLACES + pairs * a.nblk;
             hipLaunchKernelGGL((range_wide_kernel<QW, SRC>), dim3((unsigned)blocks), dim3(64 * QW), 0, stream, a);

@@ -181,13 +181,13 @@ Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
 // attn_cache_wide.hip. Two workgroups of 4 waves are resident on a CU, 64 on an XCD. Where the last round of them is not full,
 // its blocks may be cut: a block alone on its CU takes ~1.1 us a tile, beside another 1.8, and parts cost a launch (~6 us) and
 // their rows written and read (2,319 tokens x 32 heads over 8, 512 + 72 blocks, windows of 1,024, 2,048 and 8,192: 66.6, 114 and 400
-// us uncut, 63.4, 99 and 309 cut).
-Cut cut_wide(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool by_xcd) {
+// us uncut, 63.4, 99 and 309 cut). `waves`: given by the caller, or 0; a block of 8 that it gives takes 1.9 us a tile.
+Cut cut_wide(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool by_xcd, int waves = 0) {
     const int64_t big = (rows + 255) / 256 * pairs;
     Cut c{};
     // 8 waves: half the keys and values moved into LDS. Long ranges that fill the rounds of 256 such workgroups (us, 8 / 4
     // waves: 4,096 tokens x 32 heads, windows of 8,192 and 1,024 tokens 493 / 511 and 100 / 92; 3,000 x 32, 1.5 rounds, 91 / 82).
-    c.wide = tiles >= 64 && big >= 256 && (big % 256 == 0 || big >= 1024) ? 8 : 4;
+    c.wide = waves ? waves : tiles >= 64 && big >= 256 && (big % 256 == 0 || big >= 1024) ? 8 : 4;
     const int br = 32 * c.wide, xcds = by_xcd ? 8 : 1, round = (c.wide == 8 ? 256 : 512) / xcds;
     c.by_xcd = by_xcd;
     c.nblk = (int)((rows + br - 1) / br);
@@ -200,7 +200,7 @@ Cut cut_wide(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool by_
     if (page_size && c.local > round) tail = 0;
     if (tail) {
         auto cost = [&](int64_t n) {
-            return (double)((tiles + n - 1) / n) * (2 * tail * n <= round ? 1.1 : 1.8) +
+            return (double)((tiles + n - 1) / n) * (waves == 8 ? 1.9 : 2 * tail * n <= round ? 1.1 : 1.8) +
                    (n > 1 ? 6.0 + 2.0 * (double)(tail * xcds * br * n) * lr::D * 4 / 5e6 : 0.0);
         };
         for (int64_t n = 2; n <= std::min<int64_t>(std::min(round / tail, tiles / 2), 64); ++n)
@@ -341,21 +341,28 @@ Cut cache8_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, 
     const int64_t tiles = tiles_of(max_keys, span, sinks, lr::RANGE_TILE);
     if (rows <= 64 || few_rows(rows, pairs, tiles)) return cut_small8(rows, B, HK, tiles, page_size);
     const int64_t wide_tiles = tiles_of(max_keys, span, sinks, lr::RANGE_WIDE_TILE);
-    Cut c = cut_wide(rows, pairs, wide_tiles, page_size, pairs % 8 == 0 || pairs >= 64);
+    // Workgroups of 8 waves, which convert each key half as often, unless ranges are short or rows would be empty (us with 4 / 8 waves:
+    // one of 2,048 tokens behind 28,000 987 / 925, of 16,384 from an empty cache 2,207 / 2,091, 3 trees of 94 over 17,000 105 / 93; from
+    // an empty cache 2,048 tokens 62.7 / 69.8, 3,000 103 / 107; 64 x 256 156 / 181).
+    const int64_t n128 = (rows + 127) / 128, n256 = (rows + 255) / 256;
+    const int waves = wide_tiles >= 64 && 16 * n256 <= 9 * n128 ? 8 : 4;
+    Cut c = cut_wide(rows, pairs, wide_tiles, page_size, pairs % 8 == 0 || pairs >= 64, waves);
     if (B > 1 && !window) cut_pieces(c, rows, pairs, wide_tiles, page_size);
-    // Blocks in equal shares (attn_cache_wide.hip, BlockPieces). An XCD has room for 64 workgroups of 4 waves: 44 blocks leave 20 of
-    // the places empty, 66 leave 62 of them in the second round. Cut evenly, 44 blocks of 89 tiles take 171 us instead of 186 (35 of
-    // 125: 185 and 239; 66 of 141: 346 and 454; 94 of 97: 325 and 350). Rounds that are nearly full gain nothing by it (57 of 313: 651
-    // and 630; 122 of 250: 1,015 and 949), nor do few tiles (44 of 47: 109 and 108). Blocks count as equally long: chunks behind three
-    // times as many positions as their own, or more.
-    const int64_t P = pairs / 8, nblk = (rows + 127) / 128, blocks = P * nblk, all = blocks * wide_tiles;
-    const int64_t places = lr::RANGE_WIDE_PLACES, share = std::max<int64_t>(16, (all + places - 1) / places), full = (blocks + places - 1) / places * places;
-    if (pairs % 8 == 0 && P <= 64 && !window && !c.teams && blocks > 32 && blocks <= 128 && 10 * full >= 13 * blocks && wide_tiles >= 64 &&
-        4 * (int64_t)max_rows <= max_keys && std::min(share, wide_tiles) * std::max(1, lr::RANGE_WIDE_TILE / page_size) <= lr::RANGE_WIDE_STAGED) {
-        c = Cut{};
-        c.wide = 4; c.nblk = (int)nblk; c.by_xcd = 1;
-        c.nsplit = 1; c.places = (int)places;
-        c.part_rows = 8 * (places + blocks) * 128;
+    // Blocks in equal shares (attn_cache_wide.hip, BlockPieces) where whole blocks, or their parts, would leave a quarter of an XCD's 32
+    // places empty (us whole or in parts / in shares: 22 blocks of 90 tiles 185 / 160, 18 of 125 237 / 171, 33 of 141 432 / 319, 46 of 188
+    // 606 / 547, 11 of 79 95 / 87; 24 of 66 133 / 136, and fuller: 27 of 141 272 / 270, 30 of 141 271 / 299, 61 of 250 851 / 925). They count as
+    // equally long: chunks behind three times as many positions as their own, or more (71 of 141, half of them its own: 586 / 551, but
+    // 54 of 141 431 / 488).
+    const int64_t P = pairs / 8, blocks = P * n256, all = blocks * wide_tiles;
+    if (waves == 8 && pairs % 8 == 0 && P <= 64 && blocks <= 128 && !window && !c.teams && 4 * (int64_t)max_rows <= max_keys) {
+        const int64_t places = lr::RANGE_WIDE_PLACES, share = std::max<int64_t>(16, (all + places - 1) / places);
+        const int64_t used = blocks * std::max<int64_t>(1, places / blocks), rounds = (blocks + places - 1) / places * places;
+        if (4 * used <= 3 * rounds && std::min(share, wide_tiles) * std::max(1, lr::RANGE_WIDE_TILE / page_size) <= lr::RANGE_WIDE_STAGED) {
+            c = Cut{};
+            c.wide = 8; c.nblk = (int)n256; c.by_xcd = 1;
+            c.nsplit = 1; c.places = (int)places;
+            c.part_rows = 8 * (places + blocks) * 256;
+        }
     }
     return c;
 }

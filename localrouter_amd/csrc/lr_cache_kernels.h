@@ -71,7 +71,7 @@ constexpr int RANGE_TILE = 32;              // attn_cache.hip: keys a tile,
 constexpr int RANGE_STAGED = 2048;          // page-table entries a workgroup holds
 constexpr int RANGE_WIDE_TILE = 64;         // attn_cache_wide.hip: the same, and
 constexpr int RANGE_WIDE_STAGED = 3840;     // (both of its forms: 4 and 8 waves of 32 rows);
-constexpr int RANGE_WIDE_PLACES = 64;       // workgroups of 4 waves that an XCD holds at once
+constexpr int RANGE_WIDE_PLACES = 32;       // workgroups of 8 waves that an XCD holds at once
 constexpr int RANGE_WIDE_MIN_PAGE = 16;     // rows a page at least (of 16 rows: in pools of less than 4 GB),
 constexpr int64_t RANGE_WIDE_MAX_RS = 1 << 23;   // and row strides (elements) below this
 constexpr int64_t RANGE_MAX_BLOCKS = 1 << 22;    // workgroups a launch: a grid's work-items are counted in 32 bits
