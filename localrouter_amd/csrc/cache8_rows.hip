@@ -13,6 +13,9 @@
 // it finds their maximum: four rows a round, 16 lanes of 8 dims. A sequence of n tokens touches at most (n - 2) / 16 + 2 groups;
 // sequence b's are numbered from starts[b] / 16 + 2 b on, which leaves room for as many whatever the lengths, so a wave finds its
 // group from starts alone, and the launch is sized by T and B.
+//
+// What bounds it: HBM with prompts (11 of up to 1,500 tokens, 32 heads over 8, 265 MB: 58 us, 4.6 TB/s), else the launch and the chain of
+// loads (the token's sequence among starts, its length, page entry and table row): 24 single tokens 4.6 us, 7 chunks of up to 37 4.7.
 #include "lr_common.h"
 #include "lr_cache_kernels.h"
 
