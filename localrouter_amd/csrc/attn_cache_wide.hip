@@ -1,6 +1,6 @@
 // The ranged attention (attn_cache.hip) of calls with many rows of a kv head: chunks, frames and large trees, where the matrix
-// products bound it, over rows, pages and pages of 8 bits. The same contract; the loop is that of the key-split kernel (attn_keysplit.hip): a half-step of 16 MFMA
-// slots runs the next half-tile's scores, the previous one's products and this one's exponentials. A workgroup is 128 rows
+// products bound it, over rows, pages and pages of 8 bits. The same contract; the loop is that of the key-split kernel
+// (attn_keysplit.hip): a half-step of 16 MFMA slots runs the next half-tile's scores, the previous one's products and this one's exponentials. A workgroup is 128 rows
 // (tokens x the query heads of one kv head), four waves of 32 rows over a ring of two key tiles and two value tiles; two
 // workgroups share a CU, one's start, end and waits under the other's products. Long calls that fill the CUs take 256 rows, eight
 // waves and four of each tile. What bounds them is the clock under the power limit: 16,384 tokens x 32 heads over windows of four
@@ -16,8 +16,9 @@
 //    two: scalar bases from the staged page-table entries.
 //  * A row that overflowed its reference, or met an infinity or NaN, is computed again over the keys that it sees.
 //  * Pages of 8 bits: the tiles go through registers, loaded a step ahead, and are converted on their way into LDS, once for all the
-//    workgroup's rows (in the products' place each wave would convert every fragment): 32 conversions and 8 LDS writes a wave and
-//    step beside 32 MFMA. 2,048 tokens x 32 heads over 8 behind 6,000 positions 252 us, over bf16 pages 232.
+//    workgroup's rows (in the products' place each wave would convert every fragment): 16 conversions and 4 LDS writes a wave and
+//    step beside 32 MFMA, twice as many in workgroups of four waves. 2,048 tokens x 32 heads over 8 behind 6,000 positions 268 us, over
+//    bf16 pages 249.
 #include "lr_common.h"
 #include "block_order.h"
 #include "lr_cache_kernels.h"

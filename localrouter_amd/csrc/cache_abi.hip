@@ -2,7 +2,6 @@
 // include/lr_attn.h): argument validation, then launches on the caller's stream. Nothing here synchronises, allocates or keeps
 // state.
 #include <limits.h>
-#include <stdlib.h>
 
 #include <algorithm>
 

@@ -415,6 +415,54 @@ def test_far_pages():
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
 
 
+def test_far_pages_of_chunks():
+    """The same of a chunk, whose tiles go through the kernel of many rows, and single tokens beside it."""
+    pages, ps, HK = 8, 256, 2
+    stride = (1 << 31) + 4096
+    big = torch.zeros(7 * stride + 2 * ps * HK * 128, dtype=torch.uint8, device="cuda")
+    kp, vp = (big.as_strided((pages, ps, HK, 128), (stride, 2 * HK * 128, 128, 1), o).view(F8) for o in (0, HK * 128))
+    B = Batch8(27, [600, 1], [1100, 300], ps, HK, pages=pages)
+    kp.view(torch.uint8).copy_(B.kp.view(torch.uint8))
+    vp.view(torch.uint8).copy_(B.vp.view(torch.uint8))
+    q = rnd(B.g, 601, 6, 128)
+    want = B.attend(q)
+    assert torch.equal(cache.attention_f8(q, kp, vp, B.ks, B.vs, B.t, B.starts, B.lens), want)
+    B.check(q, want, lambda b: chain_seen(B.news[b], B.L[b]))
+
+
+@pytest.mark.parametrize("H", [2, 80])
+def test_tokens_before_the_first_position(H):
+    """More tokens than positions: those before the first see nothing, and have no place in the pages."""
+    B = Batch8(28, [40, 3], [25, 70], 16, 2)
+    q = rnd(B.g, 43, H, 128)
+    out = torch.full((43, H, 128), 9.0, dtype=BF16, device="cuda")
+    B.attend(q, out=out)
+    assert (out[:15] == 0).all()
+    seen = chain_seen(25, 25)
+    k, v = B.rows(0)
+    check_rows(out[15:40], *ref_rows(q[15:40], k, v, seen), what="the rest")
+    k, v = rnd(B.g, 43, 2, 128), rnd(B.g, 43, 2, 128)
+    kp, vp, ks, vs = (x.clone() for x in (B.kp, B.vp, B.ks, B.vs))
+    q_out = torch.full((43, H, 128), 9.0, dtype=BF16, device="cuda")
+    cache.append_f8(q, k, v, B.kp, B.vp, B.ks, B.vs, B.t, B.starts, B.lens, q_out, table_kind=ops.TABLE_NONE)
+    assert (q_out[:15] == 9.0).all() and not (q_out[15:] == 9.0).all((1, 2)).any()
+    cache.append_f8(q[15:], k[15:], v[15:], kp, vp, ks, vs, B.t, ints([0, 25, 28]), B.lens, table_kind=ops.TABLE_NONE)
+    for x, y in ((kp, B.kp), (vp, B.vp), (ks, B.ks), (vs, B.vs)):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+@pytest.mark.parametrize("H,n,rows,L", [(16, 9, 7, 500), (128, 300, 290, 4500)])
+def test_more_tokens_than_the_call_is_sized_for(H, n, rows, L):
+    B = Batch8(29, [n], [L], 32, 8)
+    q = rnd(B.g, n, H, 128)
+    out = torch.full((n, H, 128), 9.0, dtype=BF16, device="cuda")
+    B.attend(q, out=out, max_rows=rows, max_keys=L)
+    at = [0, rows // 2, rows - 1]
+    k, v = B.rows(0)
+    check_rows(out[at], *ref_rows(q[at], k, v, chain_seen(n, L)[at]), what="rows")
+    assert (out[rows:] == 9.0).all()
+
+
 # ------------------------------------------------------------------------------------------------ append
 def angles(n):
     a = torch.arange(n, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(64, dtype=torch.float64) / 64)
