@@ -170,7 +170,7 @@ __global__ __launch_bounds__(RB * KG * 64, RB * KG / 4) void range_attn_kernel(R
                 const uint32_t m = seen_bits<BT, SRC>(a, sq, tl, bad, i, me, x, 0) >> (8 * hf);
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (!(m >> (16 * (e >> 3) + (e & 7)) & 1)) s[e] = -INFINITY;
+                    s[e] = if_seen(s[e], m, 16 * (e >> 3) + (e & 7));
             }
             float mx = s[0];
 #pragma unroll
@@ -443,8 +443,8 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void range_step_kernel(RangeAttnAr
                     const uint32_t m = seen_bits<BT, SRC>(a, sq, tl, bad, ri[nb], me[nb], x, 0) >> (4 * g);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        if (!(m >> e & 1)) s0[e] = -INFINITY;
-                        if (!(m >> (16 + e) & 1)) s1[e] = -INFINITY;
+                        s0[e] = if_seen(s0[e], m, e);
+                        s1[e] = if_seen(s1[e], m, 16 + e);
                     }
                 }
                 const float mx = c * quad_max(fmaxf(fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3])),

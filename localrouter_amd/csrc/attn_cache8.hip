@@ -248,8 +248,8 @@ __global__ __launch_bounds__(KH * HW * 64, NB == 1 && !SHARES ? 3 : 2) void rang
                 const uint32_t m = seen_bits<BT, SRC>(a, sq, tl, bad, ri[nb], me[nb], x, 0) >> (4 * g);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (!(m >> e & 1)) s0[e] = -INFINITY;
-                    if (!(m >> (16 + e) & 1)) s1[e] = -INFINITY;
+                    s0[e] = if_seen(s0[e], m, e);
+                    s1[e] = if_seen(s1[e], m, 16 + e);
                 }
             }
             const float mx = c * quad_max(fmaxf(fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3])),

@@ -507,7 +507,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
         const uint32_t m = seen_bits<BT, SRC>(a, sq, tl, bad, i, me, x, 32 * half) >> (8 * hf);
 #pragma unroll
         for (int q = 0; q < 16; ++q)
-            if (!(m >> (16 * (q >> 3) + (q & 7)) & 1)) sb[q] = -INFINITY;
+            sb[q] = if_seen(sb[q], m, 16 * (q >> 3) + (q & 7));
         if (unset_any) {
             float mx = sb[0];
 #pragma unroll

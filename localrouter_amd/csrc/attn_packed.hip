@@ -246,8 +246,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
             auto mask_half = [&](f32x16& sb, int x, int half) __attribute__((always_inline)) {
                 const uint32_t m = seen_bits<BT, SRC>(a, cur.sq, cur.tl, false, i, me, x, 32 * half) >> (8 * hf);
 #pragma unroll
-                for (int q = 0; q < 16; ++q)
-                    if (!(m >> (16 * (q >> 3) + (q & 7)) & 1)) sb[q] = -INFINITY;
+                for (int q = 0; q < 16; ++q) sb[q] = if_seen(sb[q], m, 16 * (q >> 3) + (q & 7));
                 if (unset_any) {
                     float mx = sb[0];
 #pragma unroll
