@@ -307,7 +307,9 @@ Cut cut_small8(int64_t rows, int64_t B, int64_t HK, int64_t tiles, int page_size
             c.kh = 4; c.hw = (int)paired;
             c.places = (int)places;
             c.per = 4;   // at least so many tiles a share
-            c.merge_here = c.br == 16;
+            // (us of blocks of 32 rows merged by a second launch / by the last part to end: 40 sequences of up to 6,000 104 / 102, 64 151 / 145, but
+            // 20 of 12,000, whose pairs have more parts, 99.5 / 99.7, 16 of 24,000 140.8 / 142.4)
+            c.merge_here = c.br == 16 || 2 * (base / paired) >= places;
             c.part_rows = 2 * places * c.br * paired;
             c.flags = c.merge_here ? 2 * places : 0;
             return c;
