@@ -393,6 +393,22 @@ def test_scales_and_large_scores(scale, n):
     B.check(q, out, lambda b: chain_seen(n, 900), scale)
 
 
+@pytest.mark.parametrize("scale", [0.02, 1.0])
+@pytest.mark.parametrize("H,HK,n,L", [(128, 8, 290, 4500), (14, 2, 300, 1300), (64, 8, 200, 1000)])
+def test_large_scores_of_chunks(H, HK, n, L, scale):
+    """The same of many rows: rows whose sums grow take higher references, in the middle of a block and of its parts."""
+    B = Batch8(30, [n], [L], 32, HK)
+    e = exps(B.ks)
+    pages = -(-L // 32)
+    e[B.t[0][:pages].long()] += (torch.arange(pages, device="cuda") * 6 // pages)[:, None, None].int()
+    B.ks = scales_of(e)
+    q = rnd(B.g, n, H, 128)
+    out = B.attend(q, scale=scale)
+    at = [0, 1, n // 2, n - 1]
+    k, v = B.rows(0)
+    check_rows(out[at], *ref_rows(q[at], k, v, chain_seen(n, L)[at], scale), what="rows")
+
+
 def test_far_pages():
     """Pages whose offsets pass 32 bits, interleaved keys and values, scales side by side in one buffer."""
     pages, ps, HK = 10, 16, 2
