@@ -180,7 +180,9 @@ Cut cut_small(int64_t rows, int64_t pairs, int64_t tiles, int page_size) {
 // attn_cache_wide.hip. Two workgroups of 4 waves are resident on a CU, 64 on an XCD. Where the last round of them is not full,
 // its blocks may be cut: a block alone on its CU takes ~1.1 us a tile, beside another 1.8, and parts cost a launch (~6 us) and
 // their rows written and read (2,319 tokens x 32 heads over 8, 512 + 72 blocks, windows of 1,024, 2,048 and 8,192: 66.6, 114 and 400
-// us uncut, 63.4, 99 and 309 cut). `waves`: given by the caller, or 0; a block of 8 that it gives takes 1.9 us a tile.
+// us uncut, 63.4, 99 and 309 cut). `waves`: given by the caller (8-bit
+// pages), or 0; a block of 8 that it gives takes 1.9 us a tile, of 4 1.8 also alone (4 chunks of 100 tokens over 3,000, 32 heads over 8, whole 56
+// us, in parts 47).
 Cut cut_wide(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool by_xcd, int waves = 0) {
     const int64_t big = (rows + 255) / 256 * pairs;
     Cut c{};
@@ -199,7 +201,7 @@ Cut cut_wide(int64_t rows, int64_t pairs, int64_t tiles, int page_size, bool by_
     if (page_size && c.local > round) tail = 0;
     if (tail) {
         auto cost = [&](int64_t n) {
-            return (double)((tiles + n - 1) / n) * (waves == 8 ? 1.9 : 2 * tail * n <= round ? 1.1 : 1.8) +
+            return (double)((tiles + n - 1) / n) * (waves == 8 ? 1.9 : waves == 4 || 2 * tail * n > round ? 1.8 : 1.1) +
                    (n > 1 ? 6.0 + 2.0 * (double)(tail * xcds * br * n) * lr::D * 4 / 5e6 : 0.0);
         };
         for (int64_t n = 2; n <= std::min<int64_t>(std::min(round / tail, tiles / 2), 64); ++n)
