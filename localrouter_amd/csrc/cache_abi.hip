@@ -293,9 +293,9 @@ Cut packed_cut(int B, int T, int H, int HK) {
 // 16, 24,000 146 / 121; 64, 6,000 144 / 124, 24,000 558 / 440 (5.5 TB/s); 27 rows, 16 of 6,000 38.9 / 47.7, 40 112 / 104, 20 of 12,000
 // 123 / 98.8.
 // Otherwise parts, as few as cost least (cut_small's costs: what a round takes is the chain of loads and instructions, not the bytes),
-// by 8 waves of one head; of more blocks than CUs by 4, of more than three a CU by 2 of each of two heads, whose rows are next to
-// each other (us with 8 / 4 / 2 x 2: 64 x 300 keys 14.2 / 10.8 / 11.0, 64 x 1,500 35.9 / 32.7 / 35.2, 128 x 1,500 80 / 68 / 61.5, 256 x 1,500
-// 158 / 137 / 129; 32 x 1,500 20.1 / 20.9 / 33.4).
+// by 8 waves of one head; of at most 4 tiles, or of more blocks than CUs, by 4 (8 sequences of 4 tokens over 60 keys 5.9 / 5.7); of more
+// than three a CU by 2 of each of two heads, whose rows are next to each other (us with 8 / 4 / 2 x 2: 64 x 300 keys 14.2 / 10.8 / 11.0,
+// 64 x 1,500 35.9 / 32.7 / 35.2, 128 x 1,500 80 / 68 / 61.5, 256 x 1,500 158 / 137 / 129; 32 x 1,500 20.1 / 20.9 / 33.4).
 Cut cut_small8(int64_t rows, int64_t B, int64_t HK, int64_t tiles, int page_size) {
     Cut c{};
     c.br = rows <= 16 ? 16 : 32;
@@ -318,7 +318,7 @@ Cut cut_small8(int64_t rows, int64_t B, int64_t HK, int64_t tiles, int page_size
         }
     }
     int64_t ns = 1;
-    c.kh = base <= 256 ? 8 : 4; c.hw = 1;
+    c.kh = base <= 256 && tiles > 4 ? 8 : 4; c.hw = 1;
     if (base > 768 && paired == 2 && c.br == 16) c.kh = c.hw = 2;
     if (base <= 256) {
         auto cost = [&](int64_t n) {
