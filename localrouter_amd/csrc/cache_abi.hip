@@ -279,7 +279,7 @@ Cut packed_cut(int B, int T, int H, int HK) {
     c.nsplit = 1; c.per = MAX_POS;
     const double len = (double)T / B, t32 = 1.1 * (double)blocks(32) / 256 * (5.0 + 0.0029 * len),
                  t128 = std::max(6.0 + 1.2 / 64 * len, (double)blocks(128) / 512 * (6.0 + 1.75 / 128 * len));
-    if (blocks(16) <= 256) c.br = 16;
+    if ((B == 1 ? (rows + 15) / 16 : rows / 16 + (B + 1) / 2) * HK <= 256) c.br = 16;
     else if (t32 <= t128) c.br = 32;
     else c.wide = blocks(128) >= 1024 && HK % 8 == 0 && G > 1 ? 8 : 4;
     const int64_t br = c.wide ? 32 * c.wide : c.br;
@@ -292,13 +292,18 @@ Cut packed_cut(int B, int T, int H, int HK) {
 // over 8, lengths from half to N: 4 sequences, N 24,000 39.8 / 41.6; 16, 6,000 33.1 / 37.7; 64, 1,500 32.7 / 38.6; 32, 6,000 66.8 / 58.9;
 // 16, 24,000 146 / 121; 64, 6,000 144 / 124, 24,000 558 / 440 (5.5 TB/s); 27 rows, 16 of 6,000 38.9 / 47.7, 40 112 / 104, 20 of 12,000
 // 123 / 98.8.
+// Blocks of 16 rows also where that makes more of them, unless it is the bytes that count: keys are read once a block, but its chain of
+// steps and the merge of its parts are shorter (us in blocks of 32 / 16, 32 heads over 8: 8 tokens over 60 keys 7.6 / 5.7, 400 11.1 / 8.7, 3,000
+// 15.1 / 12.3, 30,000 25.6 / 24.6; 16 sequences of 8 over 1,000 17.7 / 12.2; 8 of 8 over 3,000 20.2 / 19.9, but 4 over 9,000 23.7 / 24.5; 480
+// blocks of 64 keys 8.0 / 6.9, 512 of 400 11.4 / 11.3).
 // Otherwise parts, as few as cost least (cut_small's costs: what a round takes is the chain of loads and instructions, not the bytes),
 // by 8 waves of one head; of at most 4 tiles, or of more blocks than CUs, by 4 (8 sequences of 4 tokens over 60 keys 5.9 / 5.7); of more
 // than three a CU by 2 of each of two heads, whose rows are next to each other (us with 8 / 4 / 2 x 2: 64 x 300 keys 14.2 / 10.8 / 11.0,
 // 64 x 1,500 35.9 / 32.7 / 35.2, 128 x 1,500 80 / 68 / 61.5, 256 x 1,500 158 / 137 / 129; 32 x 1,500 20.1 / 20.9 / 33.4).
 Cut cut_small8(int64_t rows, int64_t B, int64_t HK, int64_t tiles, int page_size) {
     Cut c{};
-    c.br = rows <= 16 ? 16 : 32;
+    const int64_t blocks16 = (rows + 15) / 16 * B * HK;
+    c.br = rows <= 16 || (blocks16 <= 512 && blocks16 * tiles <= 14000) ? 16 : 32;
     const int64_t nblk = (rows + c.br - 1) / c.br, base = nblk * B * HK;
     c.nblk = (int)nblk;
     c.nsplit = 1;
@@ -342,7 +347,12 @@ Cut cache8_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, 
     const int64_t rows = (int64_t)max_rows * (H / HK), pairs = (int64_t)B * HK;
     const int64_t span = window ? (int64_t)window + max_rows + 1 : max_keys;
     const int64_t tiles = tiles_of(max_keys, span, sinks, lr::RANGE_TILE);
-    if (rows <= 64 || few_rows(rows, pairs, tiles)) return cut_small8(rows, B, HK, tiles, page_size);
+    // The kernel of few rows while it has few blocks with few keys, which every block reads (us with it / without: 1 sequence of 256 tokens
+    // behind 1,750, 32 heads over 8, 22 / 32, of 128 behind 3,900 29 / 37, 4 of 100 behind 900 22 / 34, 1 of 400 from an empty cache 13 / 18; 4
+    // of 64 behind 3,000, 24,000 tiles in all, 29 / 35, 1 of 128 behind 7,900, 32,000, 42 / 44; 4 of 64 behind 9,000, 72,000, 73 / 55; 784 blocks
+    // of 34 tiles 39 / 37, 1,152 of 30 42 / 37).
+    const int64_t blocks32 = (rows + 31) / 32 * pairs;
+    if (rows <= 64 || (blocks32 <= 600 && blocks32 * tiles <= 30000)) return cut_small8(rows, B, HK, tiles, page_size);
     const int64_t wide_tiles = tiles_of(max_keys, span, sinks, lr::RANGE_WIDE_TILE);
     // Workgroups of 8 waves, which convert each key half as often, unless ranges are short or rows would be empty (us with 4 / 8 waves:
     // one of 2,048 tokens behind 28,000 987 / 925, of 16,384 from an empty cache 2,207 / 2,091, 3 trees of 94 over 17,000 105 / 93; from

@@ -197,6 +197,39 @@ def test_attention_of_chunks_in_equal_shares(c):
     assert torch.equal(out, first)
 
 
+CHUNKS = [
+    # tokens of each sequence, lengths, heads, kv heads, page size, window, sinks, by_head, tree: more than 600 blocks of 32 rows
+    ([700, 333], [700, 1500], 32, 2, 16, 0, 0, False, False),
+    ([300], [1300], 128, 4, 64, 0, 0, True, False),
+    ([400, 170], [3000, 170], 64, 4, 32, 333, 7, False, False),
+    ([256, 200, 1, 0, 256, 30, 256, 99], [8000, 4000, 900, 50, 5000, 30, 256, 6500], 32, 8, 64, 0, 0, False, False),
+    ([250], [2600], 96, 3, 128, 1000, 4, True, False),
+    ([180, 220], [900, 4000], 64, 2, 16, 0, 0, False, True),
+    ([220], [1700], 100, 4, 256, 600, 5, False, True),
+    ([900], [900], 40, 1, 16, 0, 0, False, False),
+]
+
+
+@pads
+@pytest.mark.parametrize("c", CHUNKS, ids=lambda c: f"{len(c[0])}seq{max(c[0])}of{max(c[1])}h{c[2]}g{c[3]}p{c[4]}w{c[5]}t{int(c[8])}")
+def test_attention_of_chunks(c, pad):
+    news, lens, H, HK, ps, window, sinks, by_head, tree = c
+    B = Batch8(31, news, lens, ps, HK, by_head, pad=pad)
+    rng = random.Random(8)
+    trees = [random_tree(rng, n) for n in news]
+    q = rnd(B.g, sum(news), H, 128)
+    out = B.attend(q, max_rows=max(news), max_keys=max(lens), tree=tree_words(trees, (max(news) + 63) // 64) if tree else None, window=window,
+                   sinks=sinks)
+    for b, n in enumerate(news):
+        at = sorted({i for i in (0, 1, n // 3, n // 2, n - 1) if 0 <= i < n})
+        if not at:
+            continue
+        seen = (tree_seen(trees[b], lens[b], window, sinks) if tree else chain_seen(n, lens[b], window, sinks))[at]
+        k, v = B.rows(b)
+        rows = [B.st[b] + i for i in at]
+        check_rows(out[rows], *ref_rows(q[rows], k, v, seen), what=f"sequence {b}")
+
+
 SHARES = [
     # heads, kv heads, tokens, page, window, sinks, tree, long sequences
     (32, 8, 1, 16, 0, 0, False, 2),
@@ -277,7 +310,7 @@ def test_attention_of_batches_in_equal_shares(c, B):
 
 
 @pads
-@pytest.mark.parametrize("heads", [2, 40])
+@pytest.mark.parametrize("heads", [2, 40, 3600])
 def test_masks_that_leave_a_row_empty(heads, pad):
     B = Batch8(14, [3, 3], [3, 40], 16, 1, pad=pad)
     q = rnd(B.g, 6, heads, 128)
@@ -288,9 +321,10 @@ def test_masks_that_leave_a_row_empty(heads, pad):
 
 
 @pads
+@pytest.mark.parametrize("H", [4, 480])
 @pytest.mark.parametrize("news,lens,tree", [([1, 1], [70, 3000], False), ([6, 20], [70, 333], True), ([90], [200], False),
                                             ([6, 60], [70, 333], True)])
-def test_positions_that_are_not_seen_have_no_part(news, lens, tree, pad):
+def test_positions_that_are_not_seen_have_no_part(news, lens, tree, pad, H):
     """Pages' rows behind the sequences' ends, free pages and drafted tokens of other branches hold NaN, free pages scales of NaN too."""
     B = Batch8(15, news, lens, 16, 2, pad=pad)
     used = torch.zeros(B.n_pages, 16, dtype=torch.bool, device="cuda")
@@ -306,12 +340,12 @@ def test_positions_that_are_not_seen_have_no_part(news, lens, tree, pad):
         at = lens[1] - 1
         B.kp.view(torch.uint8)[B.table[1][at // 16], at % 16, 0] = 0xff
         B.vp.view(torch.uint8)[B.table[1][at // 16], at % 16, 1] = 0xff
-    q = rnd(B.g, sum(news), 4, 128)
+    q = rnd(B.g, sum(news), H, 128)
     out = B.attend(q, **(dict(tree=tree_words(trees, 1)) if tree else {}))
     B.check(q, out, lambda b: tree_seen(trees[b], lens[b]) if tree else chain_seen(news[b], lens[b]))
 
 
-@pytest.mark.parametrize("heads", [4, 80])
+@pytest.mark.parametrize("heads", [4, 80, 3600])
 def test_seen_values_that_are_not_finite(heads):
     """A NaN in a seen value reaches its dim of the rows that see it, a NaN in a seen key their every dim; a scale of NaN as its rows
     would."""
@@ -328,7 +362,7 @@ def test_seen_values_that_are_not_finite(heads):
 
 
 @pads
-@pytest.mark.parametrize("heads", [4, 80])
+@pytest.mark.parametrize("heads", [4, 80, 3600])
 def test_pages_outside_the_pool_hold_nothing(heads, pad):
     news, lens = [1, 2, 1], [100, 60, 40]
     for ps in (16, 64):
@@ -351,7 +385,7 @@ def test_pages_outside_the_pool_hold_nothing(heads, pad):
 
 
 @pads
-@pytest.mark.parametrize("H", [4, 40])
+@pytest.mark.parametrize("H", [4, 40, 2600])
 def test_rows_behind_the_last_sequence_stay(H, pad):
     """A padded batch: more rows than tokens, output rows and columns beyond the call's left as they were, queries as views."""
     B = Batch8(18, [2, 5], [100, 37], 16, 2, pad=pad)
@@ -363,14 +397,15 @@ def test_rows_behind_the_last_sequence_stay(H, pad):
     assert (out[7:] == 9.0).all() and (out[:, H:] == 9.0).all()
 
 
+@pytest.mark.parametrize("H", [4, 3200])
 @pytest.mark.parametrize("starts,lens", [([0, 3, 1, 4], [50, 50, 50]), ([-1, 2, 3, 4], [50, 50, 50]), ([0, 1, 2, 4], [-5, 50, 1 << 30]),
                                          ([0, 1, 2, 1 << 30], [50, 2000000000, 0])])
-def test_senseless_numbers_do_nothing_outside(starts, lens):
+def test_senseless_numbers_do_nothing_outside(starts, lens, H):
     """Starts that do not ascend, negative and huge lengths: whatever rows come out, nothing outside the tensors is touched."""
     B = Batch8(19, [1, 1, 2], [50, 50, 50], 16, 2)
     pool = torch.cat([x.view(torch.uint8).flatten() for x in (B.kp, B.vp, B.ks, B.vs)])
-    q, k, v = rnd(B.g, 4, 4, 128), rnd(B.g, 4, 2, 128), rnd(B.g, 4, 2, 128)
-    out = torch.full((6, 4, 128), 9.0, dtype=BF16, device="cuda")
+    q, k, v = rnd(B.g, 4, H, 128), rnd(B.g, 4, 2, 128), rnd(B.g, 4, 2, 128)
+    out = torch.full((6, H, 128), 9.0, dtype=BF16, device="cuda")
     cache.attention_f8(q, B.kp, B.vp, B.ks, B.vs, B.t, ints(starts), ints(lens), out[:4])
     cache.attention_f8(q, B.kp, B.vp, B.ks, B.vs, B.t, ints(starts), ints(lens), out[:4], max_rows=1, max_keys=20)
     assert (out[4:] == 9.0).all()
@@ -394,7 +429,7 @@ def test_scales_and_large_scores(scale, n):
 
 
 @pytest.mark.parametrize("scale", [0.02, 1.0])
-@pytest.mark.parametrize("H,HK,n,L", [(128, 8, 290, 4500), (14, 2, 300, 1300), (64, 8, 200, 1000)])
+@pytest.mark.parametrize("H,HK,n,L", [(128, 8, 290, 4500), (14, 2, 300, 1300), (64, 8, 200, 1000), (40, 2, 600, 1300)])
 def test_large_scores_of_chunks(H, HK, n, L, scale):
     """The same of many rows: rows whose sums grow take higher references, in the middle of a block and of its parts."""
     B = Batch8(30, [n], [L], 32, HK)
@@ -431,8 +466,9 @@ def test_far_pages():
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
 
 
-def test_far_pages_of_chunks():
-    """The same of a chunk, whose tiles go through the kernel of many rows, and single tokens beside it."""
+@pytest.mark.parametrize("H", [6, 30])
+def test_far_pages_of_chunks(H):
+    """The same of a chunk and a single token beside it; of many heads in the kernel of many rows."""
     pages, ps, HK = 8, 256, 2
     stride = (1 << 31) + 4096
     big = torch.zeros(7 * stride + 2 * ps * HK * 128, dtype=torch.uint8, device="cuda")
@@ -440,10 +476,12 @@ def test_far_pages_of_chunks():
     B = Batch8(27, [600, 1], [1100, 300], ps, HK, pages=pages)
     kp.view(torch.uint8).copy_(B.kp.view(torch.uint8))
     vp.view(torch.uint8).copy_(B.vp.view(torch.uint8))
-    q = rnd(B.g, 601, 6, 128)
+    q = rnd(B.g, 601, H, 128)
     want = B.attend(q)
     assert torch.equal(cache.attention_f8(q, kp, vp, B.ks, B.vs, B.t, B.starts, B.lens), want)
-    B.check(q, want, lambda b: chain_seen(B.news[b], B.L[b]))
+    for b, at in ((0, [0, 300, 599]), (1, [0])):
+        k, v = B.rows(b)
+        check_rows(want[[B.st[b] + i for i in at]], *ref_rows(q[[B.st[b] + i for i in at]], k, v, chain_seen(B.news[b], B.L[b])[at]))
 
 
 @pytest.mark.parametrize("H", [2, 80])
