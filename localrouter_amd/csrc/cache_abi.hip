@@ -279,7 +279,7 @@ Cut packed_cut(int B, int T, int H, int HK) {
     c.nsplit = 1; c.per = MAX_POS;
     const double len = (double)T / B, t32 = 1.1 * (double)blocks(32) / 256 * (5.0 + 0.0029 * len),
                  t128 = std::max(6.0 + 1.2 / 64 * len, (double)blocks(128) / 512 * (6.0 + 1.75 / 128 * len));
-    if ((B == 1 ? (rows + 15) / 16 : rows / 16 + (B + 1) / 2) * HK <= 256) c.br = 16;
+    if ((B == 1 ? (rows + 15) / 16 : rows / 16 + (3 * B + 3) / 4) * HK <= 256) c.br = 16;   // (all resident, but for a few of ragged batches)
     else if (t32 <= t128) c.br = 32;
     else c.wide = blocks(128) >= 1024 && HK % 8 == 0 && G > 1 ? 8 : 4;
     const int64_t br = c.wide ? 32 * c.wide : c.br;
