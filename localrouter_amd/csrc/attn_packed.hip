@@ -14,9 +14,9 @@
 // Blocks are ordered by the tiles that they take, most first, and dealt to the workgroups in turn, each second round in the opposite
 // order, so that all have about as much; a head's blocks go to the workgroups of one XCD, whose L2 then holds its keys and values.
 //
-// What bounds it: of long prompts the clock under the power limit (4 of up to 7,000 tokens, 32 heads over 4, 510 to 540 us, 1,020 TFLOP/s; under the
-// profiler 1.82 GHz, MFMA busy 49 %). Of short ones what a block takes beside its tiles, ~1,000 vector instructions a wave (its mask and
-// references, zeros, queries and rows out) at 1.75 us a tile and ~6 a block (19 of up to 1,100, 32 over 8: 120 us, 640 TFLOP/s; with a
+// What bounds it: of long prompts the clock under the power limit (4 of up to 7,000 tokens, 32 heads over 4, 500 to 530 us, 1,020 TFLOP/s; under the
+// profiler 1.78 GHz, MFMA busy 50 %). Of short ones what a block takes beside its tiles, ~800 vector instructions a wave (its masks and
+// references, zeros, queries and rows out): 1.75 us a tile and ~5 a block (19 of up to 1,100, 32 over 8: 119 us, 640 TFLOP/s; with a
 // workgroup for each block 135). Of captions the two rounds of loads from HBM (40 of up to 257, 16 over 16, 93 MB: 33 us).
 #include "lr_common.h"
 #include "lr_cache_kernels.h"
