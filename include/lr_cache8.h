@@ -5,8 +5,8 @@
  * Pages in 8 bits. k_pages and v_pages are e4m3 (OCP, finite) bytes, strides in bytes (multiples of 16; row_stride below 2^23), page_size
  * 16 or more. 16 rows of a page (r / 16 the same) and a head share a scale 2^(x - 127), x the byte at
  * k_scales + p * scale_page_stride + (r / 16) * HK + g, in v_scales likewise; an element stands for its e4m3 value times that. Between layers the
- * scales are scale_layer_stride apart. The scales of keys and values, and of layers, may lie side by side in one buffer; they must not
- * overlap the pages, nor rows that the call reads or writes (rejected).
+ * scales are scale_layer_stride apart. The scales of keys and values, and of layers, may lie side by side in one buffer, in any order;
+ * two that share a byte are rejected, and so is a span of scales that meets the pages' or that of rows which the call reads or writes.
  *
  * lr_cache_append_f8 is lr_cache_append_bf16 into such pages (B at most 65,535). Keys and values are rounded once, from fp32, to the scale of
  * their 16 rows: the least 2^e with max|y| <= 448 * 2^e over the call's rows among them, e in [-100, 119], and where positions before

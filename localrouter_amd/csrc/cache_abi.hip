@@ -24,19 +24,33 @@ struct Level {
     int64_t stride, lo, hi;
 };
 
-// Whether d, less some sum of the levels' steps, is within 128 elements of 0: whether two heads' rows that far apart meet. Levels by
-// falling stride; where a level's stride holds the extent of those below it (nested layouts) two of its steps are tried, else as
-// many as reach, `left` in all: past that the answer is that they do.
-bool rows_meet(int64_t d, const Level* levels, int n, int& left) {
-    if (n == 0) return --left < 0 || (d > -lr::D && d < lr::D);
+// Whether d, less some sum of the levels' steps, is within `width` elements of 0: whether two rows of that width (a head's: 128) that far
+// apart meet. Levels by falling stride; where a level's stride holds the extent of those below it (nested layouts) two of its steps are
+// tried, else as many as reach, `left` in all: past that the answer is that they do.
+bool rows_meet(int64_t d, const Level* levels, int n, int64_t width, int& left) {
+    if (n == 0) return --left < 0 || (d > -width && d < width);
     const Level& l = levels[0];
-    if (l.lo == l.hi) return rows_meet(d - l.lo * l.stride, levels + 1, n - 1, left);
-    int64_t below = lr::D - 1;
+    if (l.lo == l.hi) return rows_meet(d - l.lo * l.stride, levels + 1, n - 1, width, left);
+    int64_t below = width - 1;
     for (int i = 1; i < n; ++i) below += std::max(-levels[i].lo, levels[i].hi) * levels[i].stride;
     const int64_t least = d - below;   // <= x * stride <= d + below
     for (int64_t x = std::max(least / l.stride + (least > 0 && least % l.stride), l.lo); x <= l.hi && x * l.stride <= d + below; ++x)
-        if (rows_meet(d - x * l.stride, levels + 1, n - 1, left)) return true;
+        if (rows_meet(d - x * l.stride, levels + 1, n - 1, width, left)) return true;
     return false;
+}
+// Whether no row of keys is one of values, d elements from them, nor a row of one layer one of another's. levels: the differences of two
+// rows' numbers in every dimension, in any order, those of the layers (`layer` apart) among them.
+bool apart(int64_t d, Level* levels, int n, int layers, int64_t layer, int64_t width) {
+    std::sort(levels, levels + n, [](const Level& x, const Level& y) { return x.stride > y.stride; });
+    int left = 4096;   // (nested layouts: at most 16)
+    if (rows_meet(d, levels, n, width, left)) return false;
+    if (layers == 1) return true;
+    for (int i = 0; i < n; ++i)
+        if (levels[i].stride == layer && levels[i].hi == layers - 1 && levels[i].lo == 1 - layers) {   // (another level of the same numbers is as good)
+            levels[i].lo = 1;
+            break;
+        }
+    return !rows_meet(0, levels, n, width, left);
 }
 
 // A pool of pages of elements of `es` bytes: aligned bases, strides that hold what they step over, no row of keys and values, or of
@@ -55,16 +69,7 @@ bool pool_ok(const void* k, const void* v, int64_t page, int64_t row, int64_t he
     if (!by_token && !by_head) return false;
     Level levels[4] = {{page, 1 - n_pages, n_pages - 1}, {row, 1 - page_size, page_size - 1}, {head, 1 - HK, HK - 1},
                        {layer, 1 - layers, layers - 1}};
-    std::sort(levels, levels + 4, [](const Level& x, const Level& y) { return x.stride > y.stride; });
-    int left = 4096;   // (nested layouts: at most 16)
-    if (rows_meet((reinterpret_cast<intptr_t>(v) - reinterpret_cast<intptr_t>(k)) / es, levels, 4, left)) return false;
-    if (layers == 1) return true;
-    for (Level& l : levels)
-        if (l.stride == layer && l.hi == layers - 1 && l.lo == 1 - layers) {   // (another level of the same numbers is as good)
-            l.lo = 1;
-            break;
-        }
-    return !rows_meet(0, levels, 4, left);
+    return apart((reinterpret_cast<intptr_t>(v) - reinterpret_cast<intptr_t>(k)) / es, levels, 4, layers, layer, lr::D);
 }
 // Whether a row of x (T of them, hx heads, x_rs apart) meets one of q (hq heads, q_rs apart): tensors that interleave, as the views of
 // one packed projection do, share a span but no row.
@@ -74,11 +79,11 @@ bool packed_rows_meet(const void* q, int64_t q_rs, int hq, const void* x, int64_
     int left = 4096;
     if (last == 0 || q_rs == x_rs) {
         const Level levels[2] = {{q_rs, -last, last}, {lr::D, 1 - hx, hq - 1}};
-        return rows_meet(d, levels, 2, left);
+        return rows_meet(d, levels, 2, lr::D, left);
     }
     Level levels[3] = {{q_rs, 0, last}, {x_rs, -last, 0}, {lr::D, 1 - hx, hq - 1}};
     if (x_rs > q_rs) std::swap(levels[0], levels[1]);
-    return rows_meet(d, levels, 3, left);
+    return rows_meet(d, levels, 3, lr::D, left);
 }
 Span pool_span(const void* p, int layers, int64_t layer, int64_t page, int64_t row, int64_t head, int n_pages, int page_size,
                int HK, int es = 2) {
@@ -86,8 +91,8 @@ Span pool_span(const void* p, int layers, int64_t layer, int64_t page, int64_t r
     return Span{lo, lo + es * (uintptr_t)((layers - 1) * layer + (n_pages - 1) * page + (page_size - 1) * row +
                                          (HK - 1) * head + lr::D)};
 }
-// The scales of a pool in 8 bits: pages of page_size / GROUP8 * HK bytes, `page` apart, layers `layer` apart; those of keys and of
-// values in memory of their own, or each page's next to each other.
+// The scales of a pool in 8 bits: pages of page_size / GROUP8 * HK bytes, `page` apart, layers `layer` apart; no byte of keys and values,
+// or of two layers, the same.
 bool page8_ok(int page_size, int64_t row) { return page_size >= lr::GROUP8 && row < lr::RANGE_WIDE_MAX_RS; }
 int64_t scales_bytes(int page_size, int HK) { return (int64_t)(page_size / lr::GROUP8) * HK; }
 Span scales_span(const void* p, int layers, int64_t layer, int64_t page, int n_pages, int page_size, int HK) {
@@ -96,13 +101,10 @@ Span scales_span(const void* p, int layers, int64_t layer, int64_t page, int n_p
 }
 bool scales_ok(const void* k, const void* v, int64_t page, int n_pages, int page_size, int HK, int layers = 1, int64_t layer = 0) {
     const int64_t bytes = scales_bytes(page_size, HK);
-    if (!k || !v || page < bytes || page > ((int64_t)1 << 48) / n_pages || (layers > 1 && layer > ((int64_t)1 << 48) / layers)) return false;
-    // layers one after the other, or side by side inside what a page steps over
-    if (layers > 1 && layer < (n_pages - 1) * page + bytes && (layer < bytes || (layers - 1) * layer + bytes > page)) return false;
-    const Span a = scales_span(k, layers, layer, page, n_pages, page_size, HK), b = scales_span(v, layers, layer, page, n_pages, page_size, HK);
-    if (!overlap(a, b)) return true;
-    const int64_t d = std::llabs(reinterpret_cast<intptr_t>(v) - reinterpret_cast<intptr_t>(k)), step = layers > 1 ? std::min(page, layer) : page;
-    return d >= bytes && d + bytes <= step;
+    if (!k || !v || page < bytes || page > ((int64_t)1 << 48) / n_pages || (layers > 1 && (layer < bytes || layer > ((int64_t)1 << 48) / layers)))
+        return false;
+    Level levels[2] = {{page, 1 - n_pages, n_pages - 1}, {layer, 1 - layers, layers - 1}};
+    return apart(reinterpret_cast<intptr_t>(v) - reinterpret_cast<intptr_t>(k), levels, 2, layers, layer, bytes);
 }
 bool table_args_ok(const int* table, int64_t stride, int pages, int page_size, const int* starts, int B) {
     return table && aligned(table, 4) && starts && aligned(starts, 4) && B >= 1 && pages >= 1 && stride >= pages &&

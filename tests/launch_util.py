@@ -1,0 +1,80 @@
+"""The host side of the paged cache and of the packed attention (localrouter_amd/csrc/cache_abi.hip) built by itself for the CPU, with
+launches that only write down what they were given: which kernel a call's sizes and layouts lead to, and which calls are refused. No
+GPU call is made, whatever the addresses are."""
+from __future__ import annotations
+
+import ctypes
+import subprocess
+import tempfile
+from pathlib import Path
+
+from localrouter_amd import _lib as bindings
+from localrouter_amd import build, cache
+
+CSRC = Path(__file__).resolve().parent.parent / "localrouter_amd" / "csrc"
+FIELDS = ("kernel", "br", "waves", "kh", "hw", "nsplit", "per", "places", "teams", "merge_here", "nblk")
+KERNELS = {1: "step", 2: "wide", 3: "step packed", 4: "wide packed", 5: "step8", 6: "wide8", 7: "append", 8: "append8", 9: "copy",
+           10: "scales"}
+
+SOURCE = """
+#include "cache_abi.hip"
+static int64_t last[11];
+static int launches;
+static hipError_t note(int kernel, const lr::RangeAttnArgs& a, int br, int waves, int kh, int hw) {
+    const int64_t x[11] = {kernel, br, waves, kh, hw, a.nsplit, a.per, a.places, a.teams, a.merge_here, a.nblk};
+    std::copy(x, x + 11, last);
+    ++launches;
+    return hipSuccess;
+}
+static hipError_t note(int kernel) { return note(kernel, lr::RangeAttnArgs{}, 0, 0, 0, 0); }
+namespace lr {
+hipError_t launch_range_attn(const RangeAttnArgs& a, bool, int br, hipStream_t) { return note(1, a, br, 0, 0, 0); }
+hipError_t launch_range_wide(const RangeAttnArgs& a, bool, int waves, hipStream_t) { return note(2, a, 0, waves, 0, 0); }
+hipError_t launch_packed_attn(const RangeAttnArgs& a, int br, hipStream_t) { return note(3, a, br, 0, 0, 0); }
+hipError_t launch_packed_wide(const RangeAttnArgs& a, int waves, hipStream_t) { return note(4, a, 0, waves, 0, 0); }
+hipError_t launch_range8(const RangeAttnArgs& a, int br, int kh, int hw, hipStream_t) { return note(5, a, br, 0, kh, hw); }
+hipError_t launch_range_wide8(const RangeAttnArgs& a, int waves, hipStream_t) { return note(6, a, 0, waves, 0, 0); }
+hipError_t launch_cache_append(const CacheAppendArgs&, hipStream_t) { return note(7); }
+hipError_t launch_cache_append8(const CacheAppend8Args&, hipStream_t) { return note(8); }
+hipError_t launch_cache_copy(const CacheCopyArgs&, hipStream_t) { return note(9); }
+hipError_t launch_cache_copy_scales(const CacheCopyScalesArgs&, hipStream_t) { return note(10); }
+hipError_t launch_cache_move(const CacheMoveArgs&, hipStream_t) { return hipSuccess; }
+}
+extern "C" int launched(int64_t* to) {
+    std::copy(last, last + 11, to);
+    const int n = launches;
+    launches = 0;
+    return n;
+}
+"""
+
+_lib = None
+
+
+def lib() -> ctypes.CDLL:
+    global _lib
+    if _lib is None:
+        d = Path(tempfile.mkdtemp(prefix="launches"))
+        (d / "l.hip").write_text(SOURCE)
+        subprocess.run([build.hipcc(), "--offload-host-only", "-x", "hip", "-O1", "-std=c++17", "-shared", "-fPIC", "-w", f"-I{CSRC}",
+                        str(d / "l.hip"), "-o", str(d / "l.so")], check=True)
+        L = ctypes.CDLL(str(d / "l.so"))
+        for name, (res, args) in (cache.SIGNATURES | cache.SIGNATURES_F8).items():
+            fn = getattr(L, name)
+            fn.restype, fn.argtypes = res, args
+        L.lr_attention_packed_bf16.restype, L.lr_attention_packed_bf16.argtypes = bindings.SIGNATURES["lr_attention_packed_bf16"]
+        _lib = L
+    return _lib
+
+
+def launch_of(name: str, *args) -> dict | None:
+    """The last launch of the call (its sizes and choices by name), None where it is refused before any."""
+    L = lib()
+    x = (ctypes.c_int64 * len(FIELDS))()
+    L.launched(x)
+    rc = getattr(L, name)(*args)
+    n = L.launched(x)
+    assert (rc == 0) == (n > 0), (rc, n)
+    if not n:
+        return None
+    return dict(zip(FIELDS, x), kernel=KERNELS[x[0]])
