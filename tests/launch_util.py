@@ -78,3 +78,28 @@ def launch_of(name: str, *args) -> dict | None:
     if not n:
         return None
     return dict(zip(FIELDS, x), kernel=KERNELS[x[0]])
+
+
+# attention_f8's sizes (sequences, max_rows, max_keys, heads, kv heads, page size) and the launches that they lead to: kernels whose batch
+# is large, and parts that there are only because a workgroup holds so many entries of the page table (step8 1,024, wide8 3,840)
+LAUNCHES8 = [
+    ((100, 1, 400, 32, 8, 16), dict(kernel="step8", br=16, kh=2, hw=2, nsplit=1)),
+    ((64, 1, 300, 64, 16, 32), dict(kernel="step8", br=16, kh=2, hw=2, nsplit=1)),
+    ((100, 4, 400, 32, 8, 16), dict(kernel="step8", br=16, kh=2, hw=2, nsplit=1)),
+    ((100, 1, 20000, 32, 8, 16), dict(kernel="step8", br=16, kh=2, hw=2, nsplit=2, per=512, merge_here=1)),
+    ((100, 4, 16400, 32, 8, 16), dict(kernel="step8", br=16, kh=2, hw=2, nsplit=2, per=512, merge_here=1)),
+    ((120, 1, 20000, 14, 7, 16), dict(kernel="step8", br=16, kh=4, hw=1, nsplit=2, per=512, merge_here=1)),
+    ((20, 16, 20000, 32, 8, 16), dict(kernel="step8", br=32, kh=4, hw=1, nsplit=2, per=512, merge_here=0, nblk=2)),
+    ((70, 6, 20000, 32, 8, 16), dict(kernel="step8", br=32, kh=4, hw=1, nsplit=2, per=512, merge_here=0, nblk=1)),
+    ((1, 1200, 66000, 64, 1, 16), dict(kernel="wide8", waves=8, nsplit=2, per=960, places=0, teams=0)),
+    ((24, 12, 66000, 256, 8, 16), dict(kernel="wide8", waves=4, nsplit=2, per=960, places=0, teams=0)),
+]
+
+
+def attention_f8(B, rows, keys, H, HK, ps, window=0, sinks=0) -> dict | None:
+    """The launch of cache.attention_f8 for a batch of B x rows tokens."""
+    q, out, kp, vp, ks, vs, table, starts, lens, ws = (x << 44 for x in range(1, 11))
+    pages = -(-keys // ps)
+    return launch_of("lr_cache_attention_f8", q, 128 * H, out, 128 * H, kp, vp, 128 * HK * ps, 128 * HK, 128, 1 << 16, ps, ks, vs,
+                     ps // 16 * HK, table, pages, pages, starts, lens, B, B * rows, rows, keys, H, HK, None, 0, window, sinks, 0.088, ws,
+                     1 << 43, None)
