@@ -60,9 +60,9 @@ int lr_cache_append_bf16(const void* q, const void* k, const void* v, int64_t q_
  * launches workgroups without rows for every sequence, and one that makes more of them than a grid holds (2^22) is rejected. At
  * most 2^30 positions; B at most 65,535.
  * workspace: lr_cache_attention_ws_bytes bytes for the same numbers (0: none, it may be NULL; fewer rows or positions may take
- * more), 256-byte aligned; it must not overlap q, out or the
- * pool, nor out q or the pool (rejected). What it holds before the call does not matter. Calls that overlap in time on one
- * workspace race.
+ * more; up to 273 MB, but where max_keys takes more entries of the table than a workgroup holds, 2,048, every row takes 520 bytes for
+ * each part of as many), 256-byte aligned; it must not overlap q, out or the pool, nor out q or the pool (rejected). What it holds
+ * before the call does not matter. Calls that overlap in time on one workspace race.
  */
 size_t lr_cache_attention_ws_bytes(int B, int T, int max_rows, int max_keys, int H, int HK, int page_size, int window,
                                    int sinks);

@@ -17,6 +17,7 @@
  *
  * lr_cache_attention_f8 is lr_cache_attention_bf16 over such pages: queries, probabilities and the output are bf16, sums fp32; the
  * values that the bytes stand for take part as they are. (A scale byte of 255 stands for NaN.)
+ * A workgroup holds 1,024 entries of the table (3,840 with more than 64 rows of a kv head): the workspace grows past them as there.
  *
  * lr_cache_copy_pages_f8 copies pages and their scales, in two launches.
  *
