@@ -35,6 +35,7 @@ constexpr int FR = 4;             // fragment ring entries
 static_assert(IMG_TILE_KEYS == RANGE_WIDE_TILE, "the host's cut");
 
 #include "attn_tiles.inc"
+#include "raise_rows.inc"
 #include "dma1.inc"
 #include "range_attn.inc"
 
@@ -557,29 +558,6 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // A row whose sum passes 2^32 takes a reference as much higher (a power of two of P, sums and the scores to come): it would be
-    // computed again, key by key, if it came to overflow. Of rows whose scores spread over a hundred binary orders, those of keys of
-    // large heads, some do: 2 x 700 tokens behind 5,000 positions, keys of 1, 12 and 24 times the queries' size, 182, 208 and ~300 to
-    // 800 us (without it 185, 1,424 and 4,112).
-    auto raise = [&]() __attribute__((always_inline)) {
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(ls > 0x1p32f) == 0, 1)) return;
-        const float big = wave_pair_max(ls);
-        const int e = big > 0x1p32f && big < INFINITY ? min((int)(__float_as_uint(big) >> 23) - 127, 126) : 0;
-        const float f = __uint_as_float((uint32_t)(127 - e) << 23), dm = (float)e / c;
-        ls *= f;
-#pragma unroll
-        for (int db = 0; db < 4; ++db) o[db] *= f;
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-            const uint32_t w = p[0][x >> 2][x & 3];
-            p[0][x >> 2][x & 3] = pack_bf16x2(lo_bf16(w) * f, hi_bf16(w) * f);
-        }
-        fence_s(s[1]);
-        s[1] -= dm;
-        negm -= dm;
-        mref = fmaf(dm, c, mref);
-        asm volatile(LR_NOP48 : "+v"(negm));
-    };
     // a step's refills, one load every other slot of its first half: V(t + E) from slot 1 on, then K(t + E + 1) (past the last
     // tile repeats of it, never read); their addresses in the slots before, under the products
     uint64_t src = 0;
@@ -673,7 +651,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     // ---- step u: key tile u (both halves), value tile u - 1. Its refills go to the slots of V(u - 2) and K(u - 1), both
     // read before the last barrier, and have landed at the end of step u (of step u + E - 1 with E > 0).
     for (int u = 1; u < nsteps; ++u) {
-        if constexpr (SRC == PAGES8) raise();
+        if constexpr (SRC == PAGES8) mref = fmaf(raise_rows(c, ls, o, p[0], s[1], negm), c, mref);
         const int x = x0 + u, xp = x - 1;
         uint32_t kb = ring + slot(u) + lane16, vb = vring + slot(u - 1) + vlane, kn = ring + slot(u + 1) + lane16;
         asm volatile("" : "+v"(kb), "+v"(vb), "+v"(kn));
@@ -703,7 +681,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
     }
     // ---- the last half-tile's P and the last value tile's products
     {
-        if constexpr (SRC == PAGES8) raise();
+        if constexpr (SRC == PAGES8) mref = fmaf(raise_rows(c, ls, o, p[0], s[1], negm), c, mref);
         const int u = nsteps - 1, x = x0 + u;
         if constexpr (E > 0) LR_WAIT_VMCNT(0);   // (no load into LDS outlives the workgroup)
         if (special(x, 1)) mask_half(s[1], x, 1);

@@ -32,6 +32,7 @@ constexpr int RA = 3;             // fragments read ahead
 constexpr int FR = 4;             // fragment ring entries
 
 #include "attn_tiles.inc"
+#include "raise_rows.inc"
 #include "dma1.inc"
 #include "range_attn.inc"
 
@@ -236,7 +237,6 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
             load_q(nxt);
         } else {
             // ---- masked half-tiles: what the row does not see out, and a reference for the rows that have none yet
-            float mref = 0.0f;
             bool set = !live;
             bool unset_any = true;
             auto special = [&](int x, int half) __attribute__((always_inline)) {
@@ -257,35 +257,11 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
                     set = set || mx > -INFINITY;
                     sb -= dm;
                     negm -= dm;
-                    mref = fmaf(dm, c, mref);
                     asm volatile(LR_NOP48 : "+v"(negm));
                     // rows that see nothing further on need none
                     const int next = cur.tl.key0(x) + 32 * half + 32;
                     unset_any = __builtin_amdgcn_ballot_w64(!set && me.hi > next) != 0;
                 }
-            };
-            // A row whose sum passes 2^32 takes a reference as much higher (a power of two of P, sums and the scores to come): it would be
-            // computed again, key by key, if it came to overflow. Of rows whose scores spread over a hundred binary orders, those of keys of
-            // large heads, some do: 3,840 tokens of 6, 32 heads over 8, keys of 1, 24 and 40 times the queries' size, 45, 53
-            // and 350 us (without it 45, 333 and 2,384).
-            auto raise = [&]() __attribute__((always_inline)) {
-                if (__builtin_expect(__builtin_amdgcn_ballot_w64(ls > 0x1p32f) == 0, 1)) return;
-                const float big = wave_pair_max(ls);
-                const int e = big > 0x1p32f && big < INFINITY ? min((int)(__float_as_uint(big) >> 23) - 127, 126) : 0;
-                const float f = __uint_as_float((uint32_t)(127 - e) << 23), dm = (float)e / c;
-                ls *= f;
-#pragma unroll
-                for (int db = 0; db < 4; ++db) o[db] *= f;
-#pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    const uint32_t w = p[0][x >> 2][x & 3];
-                    p[0][x >> 2][x & 3] = pack_bf16x2(lo_bf16(w) * f, hi_bf16(w) * f);
-                }
-                fence_s(s[1]);
-                s[1] -= dm;
-                negm -= dm;
-                mref = fmaf(dm, c, mref);
-                asm volatile(LR_NOP48 : "+v"(negm));
             };
             ls = 0.0f;
 #pragma unroll
@@ -321,7 +297,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
             // ---- step u: key tile u (both halves), value tile u - 1. Its refills go to the slots of V(u - 2) and K(u - 1), both
             // read before the last barrier, and have landed at the end of step u.
             for (int u = 1; u < nsteps; ++u) {
-                raise();
+                raise_rows(c, ls, o, p[0], s[1], negm);
                 uint32_t kb = ring + slot(at + u) + lane16, vb = vring + slot(at + u - 1) + vlane;
                 asm volatile("" : "+v"(kb), "+v"(vb));
                 auto rd_b = [&](int f) __attribute__((always_inline)) {
@@ -349,7 +325,7 @@ __global__ __launch_bounds__(64 * QW, 8 / QW) __attribute__((amdgpu_waves_per_eu
             lead();
             if (more) load_q(nxt);
             {
-                raise();
+                raise_rows(c, ls, o, p[0], s[1], negm);
                 const int u = nsteps - 1;
                 if (special(u, 1)) mask_half(s[1], u, 1);
                 uint32_t vb0 = vring + slot(at + u) + vlane;
