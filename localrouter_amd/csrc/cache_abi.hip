@@ -270,17 +270,23 @@ Cut cache_cut(int B, int max_rows, int max_keys, int H, int HK, int page_size, i
 // keys of its longest; the blocks of 128 take ~6 and 1.2 per 64 keys of the longest, or what the GPU does in all. Us with 16 / 32 / 128
 // rows: one of 1,000 tokens, one head, 9.2 / 11.7 / 25.7; one of 300, 32 heads over 8, 14.0 / 11.2 / 13.2; 891 tokens of 2, 32 over 8, 37
 // / 28 / 19; 4,017 of 2, 4 over 1, 41 / 28 / 60; one of 7,000, 4 over 1, 149 / 91 / 141, 8 over 8 273 / 173 / 156; 611 of 18, 16 over 8,
-// 12.5 / 11.0 / 7.8.
+// 12.5 / 11.0 / 7.8. Under a window a block reads that and its own tokens (us with 32 / 128 rows, windows of 64, 256 and 1,024: one of 7,000, 4
+// over 1, 25 / 12, 34 / 17, 48 / 32; one of 4,000, 8 over 2, 24 / 12, 32 / 17, 46 / 31; one of 500, 32 over 8, 64 11.2 / 10.6, but one of
+// 8,000, one head, 7.6 / 12.2, 9.5 / 16.8, 14.0 / 30.9).
 // Blocks of 256 where there are many and each XCD has kv heads of its own, whose keys its workgroups move half as often (us with 128 /
 // 256 rows: 10,900 tokens of 19, 32 over 8, 120 / 116; 58,000 of 60, 16 over 8, 441 / 414; one of 4,096, 32 over 8, 147 / 139; of 53,000 of 38,
 // 8 over 8, 283 / 289; 43,000 of 27, 8 over 2, 217 / 223).
-Cut packed_cut(int B, int T, int H, int HK) {
+Cut packed_cut(int B, int T, int H, int HK, int window, int sinks) {
     const int64_t G = H / HK, rows = (int64_t)T * G;
     auto blocks = [&](int64_t br) { return (rows / br + B) * HK; };
     Cut c{};
     c.nsplit = 1; c.per = MAX_POS;
-    const double len = (double)T / B, t32 = 1.1 * (double)blocks(32) / 256 * (5.0 + 0.0029 * len),
-                 t128 = std::max(6.0 + 1.2 / 64 * len, (double)blocks(128) / 512 * (6.0 + 1.75 / 128 * len));
+    const double len = (double)T / B;
+    // the most keys of a block of br rows, and twice their mean: the first tokens see fewer, of a prompt without a window half as many
+    auto most = [&](int64_t br) { return window ? std::min(len, (double)window + (double)sinks + (double)br / (double)G) : len; };
+    auto twice = [&](int64_t br) { return most(br) < len ? 2 * most(br) - most(br) * most(br) / len : len; };
+    const double t32 = 1.1 * (double)blocks(32) / 256 * (5.0 + 0.0029 * twice(32)),
+                 t128 = std::max(6.0 + 1.2 / 64 * most(128), (double)blocks(128) / 512 * (6.0 + 1.75 / 128 * twice(128)));
     if ((B == 1 ? (rows + 15) / 16 : rows / 16 + (3 * B + 3) / 4) * HK <= 256) c.br = 16;   // (all resident, but for a few of ragged batches)
     else if (t32 <= t128) c.br = 32;
     else c.wide = blocks(128) >= 1024 && HK % 8 == 0 && G > 1 ? 8 : 4;
@@ -577,7 +583,7 @@ int lr_attention_packed_bf16(const void* q, const void* k, const void* v, void* 
     a.c = scale * 1.4426950408889634f;
     a.starts = starts; a.B = B; a.T = T;
     a.window = std::min(window, MAX_POS); a.sinks = window ? std::min(sinks, MAX_POS) : 0;
-    Cut cut = packed_cut(B, T, H, HK);
+    const Cut cut = packed_cut(B, T, H, HK, a.window, a.sinks);
     set_cut(a, nullptr, cut);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     return (int)(cut.wide ? lr::launch_packed_wide(a, cut.wide, s) : lr::launch_packed_attn(a, cut.br, s));

@@ -103,3 +103,15 @@ def attention_f8(B, rows, keys, H, HK, ps, window=0, sinks=0) -> dict | None:
     return launch_of("lr_cache_attention_f8", q, 128 * H, out, 128 * H, kp, vp, 128 * HK * ps, 128 * HK, 128, 1 << 16, ps, ks, vs,
                      ps // 16 * HK, table, pages, pages, starts, lens, B, B * rows, rows, keys, H, HK, None, 0, window, sinks, 0.088, ws,
                      1 << 43, None)
+
+
+# attention_packed under windows: prompts, heads, kv heads, the rows of the blocks that every window of WINDOWS leads to
+WINDOWED = [([1000], 1, 1, 16), ([8000], 1, 1, 32), ([7000], 4, 1, 128), ([4100, 3, 0, 3900], 4, 1, 128), ([1500, 1700] * 4, 32, 8, 256)]
+WINDOWS = [(1, 0), (64, 0), (65, 3), (256, 4), (1000, 70)]
+
+
+def attention_packed(B, T, H, HK, window=0, sinks=0) -> dict | None:
+    """The launch of ops.attention_packed for T tokens of B prompts."""
+    q, k, v, out, starts = (x << 44 for x in range(1, 6))
+    return launch_of("lr_attention_packed_bf16", q, k, v, out, starts, B, T, H, HK, window, sinks, 0.088, 128 * H, 128 * HK, 128 * HK, 128 * H,
+                     None)
