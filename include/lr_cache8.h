@@ -16,7 +16,8 @@
  * Scales that the call finds in its 16 rows must be such as it writes (bytes 27 .. 246).
  *
  * lr_cache_attention_f8 is lr_cache_attention_bf16 over such pages: queries, probabilities and the output are bf16, sums fp32; the
- * values that the bytes stand for take part as they are. (A scale byte of 255 stands for NaN.)
+ * values that the bytes stand for take part as they are. A scale byte of 255 stands for NaN. Where other bytes than append's make values
+ * that are no normal numbers of bf16, they are infinite from 2^128 on, and off by at most 2^-126 (0, for one) below 2^-126.
  * A workgroup holds 1,024 entries of the table (3,840 with more than 64 rows of a kv head): the workspace grows past them as there.
  *
  * lr_cache_copy_pages_f8 copies pages and their scales, in two launches.
