@@ -5,11 +5,12 @@
 // for single tokens and small trees: bound by HBM where there is much to read (half of what bf16 pages take), and by the chain
 // from one load and one instruction to the next where there is not.
 //
-// A workgroup is a block of 16 or 32 rows (tokens x the query heads of one kv head) and a part of its tiles of 32 keys, which its
-// eight waves take in turn. Keys and values go from memory to registers, not through LDS: a lane's 32 bytes of a key are four steps
-// of its products' operand (dims 32 g .. 32 g + 31 of row n for lane 16 g + n; the queries' lanes hold the same dims), and of the
-// values it takes 8 dims of the 8 keys whose probabilities it holds, transposed by byte permutations. Conversion to bf16 with the
-// scale is one instruction for two values, and exact: e4m3 has 4 significant bits and bf16's exponents.
+// A workgroup is a block of 16 or 32 rows (tokens x the query heads of one kv head), or the same block of two kv heads, and a part of its
+// tiles of 32 keys, which a head's waves (two, four or eight) take in turn. Keys and values go from memory to registers, not through LDS:
+// a lane's 32 bytes of a key are four steps of its products' operand (dims 16 g .. + 15 and 64 + 16 g .. + 15 of row n for lane 16 g + n;
+// the queries' lanes hold the same dims), and of the values it takes 8 dims of the 8 keys whose probabilities it holds, transposed by byte
+// permutations. Conversion to bf16 with the scale is one instruction for two values, and exact: e4m3 has 4 significant bits and bf16's
+// exponents.
 //
 // Single tokens of 48 sequences of up to 9,000 positions, 32 heads over 8, 648 MB: 135 us, 4.8 TB/s; of one sequence of 2,100 10.0 us. 20
 // trees of 9 tokens over up to 12,000, 24 over 8, 363 MB: 96 us, of which the merge is 6.
@@ -51,7 +52,6 @@ struct Values8 {
 // SHARES: a batch of one block a sequence and kv head in equal shares. Its pairs (sequence, workgroup's heads) lie end to end, and a
 // workgroup takes the Q tiles from w Q on, whatever the lengths: the end of one pair, whole ones, the beginning of another. Parts of a
 // pair: slot 2 w + 1 of the workgroup where it begins, slot 2 w of the others.
-template <int BR>
 struct Shares {
     int B, tiles, end, Q;   // lane b: the sequence's tiles, and where its pairs end
 
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(KH * HW * 64, NB == 1 && !SHARES ? 3 : 2) void rang
 
     // ---- which rows, which keys
     int at = 0, split = 0, blk = 0, hg, b, pos = 0, pos_end = 1, pair_tiles = 0, pair = 0;
-    Shares<BR> sh;
+    Shares sh;
     if constexpr (SHARES) {
         sh.init(a);
         pos = blockIdx.x * sh.Q;
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(256) void range8_merge_kernel(RangeAttnArgs a) {
     tl.init(a, sq, div_small(row0, a.G, a.rcp_g), div_small(min(rows, row0 + BR) - 1, a.G, a.rcp_g));
     int parts = min(a.nsplit, (tl.total + a.per - 1) / a.per), first_share = 0;
     if constexpr (SHARES) {
-        Shares<BR> sh;
+        Shares sh;
         sh.init(a);
         const int n = __builtin_amdgcn_readlane(sh.tiles, b), begin = __builtin_amdgcn_readlane(sh.end, b) - (a.hgroups - hg) * n;
         first_share = (int)((uint32_t)begin / (uint32_t)sh.Q);

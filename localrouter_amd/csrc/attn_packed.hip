@@ -11,8 +11,10 @@
 // across them: the next block's first tiles and queries are on their way while the last tile's products are computed and the rows
 // written.
 //
-// Blocks are ordered by the tiles that they take, most first, and dealt to the workgroups in turn, each second round in the opposite
-// order, so that all have about as much; a head's blocks go to the workgroups of one XCD, whose L2 then holds its keys and values.
+// Blocks of up to 64 sequences are ordered by the number that they have in their sequence, the last first (without a window that is by
+// their tiles, most first), and dealt to the workgroups in turn, each second round in the opposite order, so that all have about as
+// much; those of more sequences go out in the sequences' order. A head's blocks go to the workgroups of one XCD (of a number of kv heads
+// that 8 divides), whose L2 then holds its keys and values.
 //
 // What bounds it: of long prompts the clock under the power limit (4 of up to 7,000 tokens, 32 heads over 4, 500 to 530 us, 1,020 TFLOP/s; under the
 // profiler 1.78 GHz, MFMA busy 50 %). Of short ones what a block takes beside its tiles, ~800 vector instructions a wave (its masks and
