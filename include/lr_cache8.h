@@ -11,8 +11,9 @@
  * lr_cache_append_f8 is lr_cache_append_bf16 into such pages (B at most 65,535). Keys and values are rounded once, from fp32, to the scale of
  * their 16 rows: the least 2^e with max|y| <= 448 * 2^e over the call's rows among them, e in [-100, 119], and where positions before
  * the call's lie among them no less than what is there: then those are rounded again to the new scale (exactly, but for values below
- * its 2^-6). An infinity or NaN is held as NaN and has no part in the scale; finite values beyond 448 * 2^119 are held as that. Tokens that are
- * left out have no part in the scale either. Rows behind the sequence's last position stay as they were, whatever their scale does.
+ * its 2^-6): a scale that drafted tokens raised does not fall again where they are not accepted and written over behind others. An
+ * infinity or NaN is held as NaN and has no part in the scale; finite values beyond 448 * 2^119 are held as that. Tokens that are left
+ * out have no part in the scale either. Rows behind the sequence's last position stay as they were, whatever their scale does.
  * Scales that the call finds in its 16 rows must be such as it writes (bytes 27 .. 246).
  *
  * lr_cache_attention_f8 is lr_cache_attention_bf16 over such pages: queries, probabilities and the output are bf16, sums fp32; the
