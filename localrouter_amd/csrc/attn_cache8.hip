@@ -10,7 +10,8 @@
 // a lane's 32 bytes of a key are four steps of its products' operand (dims 16 g .. + 15 and 64 + 16 g .. + 15 of row n for lane 16 g + n;
 // the queries' lanes hold the same dims), and of the values it takes 8 dims of the 8 keys whose probabilities it holds, transposed by byte
 // permutations. Conversion to bf16 with the scale is one instruction for two values, and exact: e4m3 has 4 significant bits and bf16's
-// exponents.
+// exponents. P is rounded to bf16, which the products take, and the sum is that of the rounded P; everything else is fp32. (Error against
+// 64 bits, relative L2: 0.0017 to 0.0020; the output's own rounding alone 0.0017.)
 //
 // Single tokens of 48 sequences of up to 9,000 positions, 32 heads over 8, 648 MB: 135 us, 4.8 TB/s; of one sequence of 2,100 10.0 us. 20
 // trees of 9 tokens over up to 12,000, 24 over 8, 363 MB: 96 us, of which the merge is 6.

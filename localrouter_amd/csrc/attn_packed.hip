@@ -4,6 +4,9 @@
 //
 //   out_i = sum_{j seen by i} 2^(c <q_i, k_j> - m_i) v_j / sum_{j seen by i} 2^(c <q_i, k_j> - m_i),  c = scale log2(e)
 //
+// P is rounded to bf16, which the products take, and the row's sum is that of the rounded P, so that the weights add up to 1; sums and
+// references are fp32. (Error against 64 bits, relative L2: 0.0017 to 0.0021; the output's own rounding alone 0.0016.)
+//
 // The inner loop is that of attn_cache_wide.hip: a half-step of 16 MFMA slots runs the next half-tile's scores, the previous one's
 // products and this one's exponentials, over a ring of two key tiles and two value tiles that direct loads fill. What differs is what
 // a batch of prompts needs: its blocks of rows are short (a prompt of 600 tokens has blocks of one to ten key tiles), so that starting

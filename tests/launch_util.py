@@ -54,11 +54,12 @@ _lib = None
 def lib() -> ctypes.CDLL:
     global _lib
     if _lib is None:
-        d = Path(tempfile.mkdtemp(prefix="launches"))
-        (d / "l.hip").write_text(SOURCE)
-        subprocess.run([build.hipcc(), "--offload-host-only", "-x", "hip", "-O1", "-std=c++17", "-shared", "-fPIC", "-w", f"-I{CSRC}",
-                        str(d / "l.hip"), "-o", str(d / "l.so")], check=True)
-        L = ctypes.CDLL(str(d / "l.so"))
+        with tempfile.TemporaryDirectory() as d:
+            src, out = Path(d) / "l.hip", Path(d) / "l.so"
+            src.write_text(SOURCE)
+            subprocess.run([build.hipcc(), "--offload-host-only", "-x", "hip", "-O1", "-std=c++17", "-shared", "-fPIC", "-w", f"-I{CSRC}",
+                            str(src), "-o", str(out)], check=True)
+            L = ctypes.CDLL(str(out))
         for name, (res, args) in (cache.SIGNATURES | cache.SIGNATURES_F8).items():
             fn = getattr(L, name)
             fn.restype, fn.argtypes = res, args
